@@ -1,0 +1,318 @@
+// Rows of logits read once for their softmax statistics: shared by the token
+// log probabilities (token_logprobs.hip) and the distillation loss
+// (topk_distill.hip).
+//
+// With the score y = softcap tanh(x / softcap) (or x) and c2 = log2(e) /
+// temperature, a row's statistics are its maximum m of y and
+//   t = (y - m) c2,   s = sum 2^t,   u = sum 2^t t,
+// so that ln p = ln2 (t - log2 s) and the entropy is ln2 (log2 s - u / s).
+// y - m is formed before the product: it is exact at the maximum whatever the
+// logits' size, where fma(y, c2, -m c2) would leave m c2's rounding in every
+// exponent. All statistics are fp32.
+//
+// A row is cut into `segs` segments of `span` 16-byte vectors. One workgroup
+// holds a segment in registers, packed, so that it crosses HBM once. One
+// segment a row where rows fill the GPU and a row fits a workgroup; otherwise
+// each segment leaves its (m, s, u) in a workspace and a second kernel joins
+// them, as a decode step's few rows need every CU (plan below).
+#pragma once
+
+#include <algorithm>
+
+#include "ak_common.h"
+
+namespace ak {
+
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+
+// What the statistics mean: the capped, tempered logits.
+struct ScoreParams {
+  float cap, inv_cap;  // softcap (with CAP)
+  float c2;            // log2(e) / temperature
+  float inv_t;         // 1 / temperature
+  int64_t ignore_index;
+};
+
+inline ScoreParams score_params(float temperature, float softcap, int64_t ignore_index) {
+  ScoreParams p;
+  p.cap = softcap;
+  p.inv_cap = softcap > 0.0f ? 1.0f / softcap : 0.0f;
+  p.c2 = (float)(1.4426950408889634 / (double)temperature);
+  p.inv_t = 1.0f / temperature;
+  p.ignore_index = ignore_index;
+  return p;
+}
+
+template <bool CAP>
+__device__ __forceinline__ float score(const ScoreParams& p, float x) {
+  return CAP ? p.cap * tanh_f32(x * p.inv_cap) : x;
+}
+
+// (m, s, u) of a row or a segment of one.
+struct RowStats {
+  float m, s, u;
+};
+
+// A row of -inf alone has no distribution: m = -inf, s = 0. (A row that holds
+// a NaN or +inf has s = NaN.)
+__device__ __forceinline__ bool empty_row(float m, float s) { return m == -INFINITY && s == 0.0f; }
+
+// log2 s as the log probabilities take it (0 for an empty row, whose scores are -inf already).
+__device__ __forceinline__ float log2_sum(const RowStats& r) {
+  return empty_row(r.m, r.s) ? 0.0f : __builtin_amdgcn_logf(r.s);
+}
+
+// ln p of a score; l2: log2_sum. (In natural units: a mask of the type's
+// lowest value stays in fp32's range, which its product with c2 would leave.)
+__device__ __forceinline__ float log_prob(const ScoreParams& p, float y, float m, float l2) {
+  return m == -INFINITY && y == -INFINITY ? y - l2 : (y - m) * p.inv_t - kLn2 * l2;
+}
+
+__device__ __forceinline__ float row_entropy(const RowStats& r) {
+  if (empty_row(r.m, r.s)) return 0.0f;
+  const float h = kLn2 * (__builtin_amdgcn_logf(r.s) - r.u / r.s);
+  return h < 0.0f ? 0.0f : h;  // one rounding below zero where one entry holds all
+}
+
+// Statistics of two parts of one row.
+__device__ __forceinline__ RowStats join_stats(const ScoreParams& p, RowStats a, RowStats b) {
+  const float m = fmaxf(a.m, b.m);
+  RowStats r{m, 0.0f, 0.0f};
+  auto add = [&](const RowStats& q) {
+    if (q.s == 0.0f) return;
+    const float d = (q.m - m) * p.c2;  // NaN for +inf maxima: the row's sum becomes NaN
+    const float f = __builtin_amdgcn_exp2f(d);
+    r.s += f * q.s;
+    // f = 0 where a part vanishes beside the other: its d may be -inf
+    r.u += f * (q.u + fmaxf(d, -1000.0f) * q.s);
+  };
+  add(a);
+  add(b);
+  return r;
+}
+
+__device__ __forceinline__ RowStats wave_join(const ScoreParams& p, RowStats st) {
+  for (int off = 1; off < 64; off <<= 1) {
+    const RowStats o{__shfl_xor(st.m, off, 64), __shfl_xor(st.s, off, 64), __shfl_xor(st.u, off, 64)};
+    // the lower lane's part first, so that every lane ends with the same bits
+    st = (threadIdx.x & off) ? join_stats(p, o, st) : join_stats(p, st, o);
+  }
+  return st;
+}
+
+// A segment of a row in registers: TPR threads, VPT vectors each, and the
+// elements around the row's vectors (at most 14, with the first segment) one
+// to a thread.
+template <typename T, int VPT, int TPR>
+struct Segment {
+  static constexpr int VE = Vec16<T>::VE;
+  Vec16<T> raw[VPT];
+  T xe;
+  int nv, nx;  // vectors of the segment, single elements
+  int col0;    // column of its first vector
+  RowSplit<T> sp;
+
+  // The thread's index, opaque to the compiler in each pass: the VPT offsets
+  // and bounds derived from it would otherwise be held from pass to pass
+  // beside the segment, and spill.
+  static __device__ __forceinline__ int thread() {
+    int t = threadIdx.x;
+    asm volatile("" : "+v"(t));
+    return t;
+  }
+
+  __device__ __forceinline__ Segment(const T* __restrict__ row, int vocab, int seg, int span) : sp(row, vocab) {
+    const int v0 = seg * span;
+    nv = min(span, sp.nvec - v0);
+    nx = seg == 0 ? sp.nx : 0;
+    col0 = sp.head + v0 * VE;
+    const int t = thread();
+    xe = T(0.0f);
+    if (t < nx) xe = row[sp.extra(t)];
+    const T* rv = row + col0;
+#pragma unroll
+    for (int k = 0; k < VPT; ++k) {
+      raw[k].u = u32x4{0, 0, 0, 0};
+      if (t + k * TPR < nv) raw[k] = load16_any_nt(rv + k * TPR * VE + (unsigned)(t * VE));
+    }
+  }
+
+  // f(logit, column) of each element that this thread holds.
+  template <typename F>
+  __device__ __forceinline__ void each(F f) {
+    const int t = thread();
+#pragma unroll
+    for (int k = 0; k < VPT; ++k) {
+      if (t + k * TPR < nv) {
+#pragma unroll
+        for (int e = 0; e < VE; ++e) f(to_f32(raw[k].e[e]), col0 + (t + k * TPR) * VE + e);
+      }
+      keep_packed(raw[k]);
+    }
+    if (t < nx) f(to_f32(xe), sp.extra(t));
+  }
+
+  // This thread's largest logit (NaN ignored).
+  __device__ __forceinline__ float largest() {
+    const int t = thread();
+    float m = t < nx ? to_f32(xe) : -INFINITY;
+#pragma unroll
+    for (int k = 0; k < VPT; ++k) {
+      if (t + k * TPR < nv) {
+#pragma unroll
+        for (int e = 0; e < VE; ++e) m = fmaxf(m, to_f32(raw[k].e[e]));
+      }
+      keep_packed(raw[k]);
+    }
+    return m;
+  }
+
+  // This thread's part of s and, with ENT, of u.
+  template <bool CAP, bool ENT>
+  __device__ __forceinline__ void sums(const ScoreParams& p, float m, float& s, float& u) {
+    const float off = m == -INFINITY ? 0.0f : m;
+    s = u = 0.0f;
+    each([&](float x, int) {
+      const float t = (score<CAP>(p, x) - off) * p.c2;
+      const float e = __builtin_amdgcn_exp2f(t);
+      s += e;
+      // 2^t is 0 from -150 on, and t may be -inf there
+      if constexpr (ENT) u = fmaf(e, fmaxf(t, -1000.0f), u);
+    });
+  }
+};
+
+// How rows are cut and held (host).
+struct ScorePlan {
+  int segs, span;  // segments a row, vectors a segment
+};
+
+constexpr int kSegVectors = 8192;            // most vectors of a segment: 1024 threads x 8
+constexpr int64_t kScoreVocab = 1 << 20;     // widest row
+constexpr int kMaxTop = 256;                 // most alternatives
+constexpr int kJoinKeys = 8192;              // most keys that the join holds in LDS
+
+// One segment a row where there are rows for every CU. Fewer rows are cut so
+// that about two workgroups a CU share the work, in segments of at least 256
+// vectors (one a thread), and with `top` alternatives in at most kJoinKeys /
+// 2 keys for the join.
+inline ScorePlan score_plan(int64_t rows, int64_t vocab, int ve, int top) {
+  const int64_t nvec = std::max<int64_t>(1, vocab / ve);
+  const int64_t least = (nvec + kSegVectors - 1) / kSegVectors;
+  int64_t segs = least;
+  if (rows < 256) {
+    segs = std::max(segs, std::min((512 + rows - 1) / rows, nvec / 256));
+    if (top > 0) segs = std::max(least, std::min<int64_t>(segs, kJoinKeys / 2 / top));
+  }
+  const int64_t span = (nvec + segs - 1) / segs;
+  return {(int)((nvec + span - 1) / span), (int)span};
+}
+
+// kernel<VPT, TPR> for a segment of `span` vectors: the fewest vectors a
+// thread that the workgroup sizes allow.
+#define AK_SEGMENT_DISPATCH(span, GO) \
+  do {                                \
+    if ((span) <= 256) GO(1, 256);    \
+    else if ((span) <= 512) GO(2, 256);  \
+    else if ((span) <= 1024) GO(4, 256); \
+    else if ((span) <= 2048) GO(4, 512); \
+    else if ((span) <= 4096) GO(8, 512); \
+    else GO(8, 1024);                 \
+  } while (0)
+
+// ---------------------------------------------------------------------------
+// Gradients: rows written whole from their statistics
+// ---------------------------------------------------------------------------
+constexpr int kGradThreads = 256;
+
+// d(score / temperature) / d(logit), and the score.
+template <bool CAP>
+__device__ __forceinline__ float score_and_slope(const ScoreParams& p, float x, float& slope) {
+  if constexpr (CAP) {
+    const float th = tanh_f32(x * p.inv_cap);
+    slope = p.inv_t * (1.0f - th * th);
+    return p.cap * th;
+  }
+  slope = p.inv_t;
+  return x;
+}
+
+// out[v] = f(x[v]) over the row's vectors [v0, v1) and, with `ends`, the
+// elements around the vectors; U vectors of a thread are loaded before the
+// first is used.
+template <typename T, bool NT, int U, typename F>
+__device__ __forceinline__ void map_row(const T* __restrict__ row, T* __restrict__ out, int vocab, int v0, int v1,
+                                        bool ends, F f) {
+  constexpr int VE = Vec16<T>::VE;
+  const RowSplit<T> sp(row, vocab);
+  const int t = threadIdx.x;
+  const T* rv = row + sp.head;
+  T* ov = out + sp.head;
+  if (v1 > sp.nvec) v1 = sp.nvec;
+  auto ld = [](const T* q) { return NT ? load16_any_nt(q) : load16_any(q); };
+  auto one = [&](const Vec16<T>& x, int v) {
+    Vec16<T> o;
+#pragma unroll
+    for (int e = 0; e < VE; ++e) o.e[e] = from_f32<T>(f(to_f32(x.e[e])));
+    if (NT) store16_any_nt(ov + (int64_t)v * VE, o);
+    else store16_any(ov + (int64_t)v * VE, o);
+  };
+  int v = v0 + t;
+  for (; U > 1 && v + (U - 1) * kGradThreads < v1; v += U * kGradThreads) {
+    Vec16<T> x[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) x[i] = ld(rv + (int64_t)(v + i * kGradThreads) * VE);
+#pragma unroll
+    for (int i = 0; i < U; ++i) one(x[i], v + i * kGradThreads);
+  }
+  for (; v < v1; v += kGradThreads) one(ld(rv + (int64_t)v * VE), v);
+  if (ends && t < sp.nx) {
+    const int c = sp.extra(t);
+    out[c] = from_f32<T>(f(to_f32(row[c])));
+  }
+}
+
+// Whether map_row wrote column c for these vectors.
+template <typename T>
+__device__ __forceinline__ bool wrote_column(const T* row, int vocab, int v0, int v1, bool ends, int c) {
+  const RowSplit<T> sp(row, vocab);
+  const int v = c - sp.head;
+  if (v < 0 || v >= sp.nvec * Vec16<T>::VE) return ends;
+  return v / Vec16<T>::VE >= v0 && v / Vec16<T>::VE < v1;
+}
+
+// Between map_row's stores and another thread's store to one of the same
+// elements: the workgroup's stores have left before any wave goes on.
+__device__ __forceinline__ void stores_done() {
+  __builtin_amdgcn_s_waitcnt(0);
+  __syncthreads();
+}
+
+// Spans of the gradient's grid: rounds of four vectors a thread where a row is
+// that wide, so that few rows fill the GPU too.
+inline ScorePlan grad_plan(int64_t vocab, int ve) {
+  const int64_t nvec = vocab / ve;
+  const int64_t n = std::max<int64_t>(1, nvec / (4 * kGradThreads));
+  return {(int)n, (int)((nvec + n - 1) / n)};
+}
+
+// Whether that many bytes pass the 256 MiB last-level cache.
+inline bool score_past_cache(int64_t bytes) { return bytes > (int64_t)300 << 20; }
+
+// Argument checks that the row entry points share.
+inline int check_score_rows(const char* name, int64_t rows, int64_t vocab, int64_t ld, float temperature,
+                            float softcap, int dtype) {
+  if (ak_dtype_size(dtype) == 0) return ak_set_error(AK_ERR_UNSUPPORTED, "%s: unsupported dtype code %d", name, dtype);
+  if (rows < 0 || vocab <= 0) return ak_set_error(AK_ERR_INVALID_ARG, "%s: bad shape rows=%lld vocab=%lld", name, (long long)rows, (long long)vocab);
+  if (vocab > kScoreVocab) return ak_set_error(AK_ERR_UNSUPPORTED, "%s: vocab=%lld is over %lld", name, (long long)vocab, (long long)kScoreVocab);
+  if (ld < vocab) return ak_set_error(AK_ERR_INVALID_ARG, "%s: row pitch smaller than vocab", name);
+  if (!ak_extent_ok(rows, ld, vocab, ak_dtype_size(dtype)))
+    return ak_set_error(AK_ERR_INVALID_ARG, "%s: rows=%lld x pitch exceed 64-bit addressing", name, (long long)rows);
+  if (!(temperature >= 1e-18f && temperature <= 1e18f))  // its square is a float, too
+    return ak_set_error(AK_ERR_INVALID_ARG, "%s: temperature must be between 1e-18 and 1e18", name);
+  if (!(softcap >= 0.0f) || softcap == INFINITY)
+    return ak_set_error(AK_ERR_INVALID_ARG, "%s: softcap must be finite and >= 0", name);
+  return AK_OK;
+}
+
+}  // namespace ak

@@ -1,0 +1,368 @@
+// Distillation from a teacher's top logits, for gfx950.
+//
+//   y = softcap > 0 ? softcap * tanh(x / softcap) : x,  p = softmax(y / T) over the vocabulary
+//   q = softmax(teacher / T) over the row's given entries (at most 256)
+//   loss  = T^2 sum_k q_k (ln q_k - ln p[id_k])
+//   dx_v  = g T^2 (p_v - sum of q_k with id_k == v) (1 - tanh^2) / T
+// An entry whose id is ignore_index is not there; a row without entries has
+// loss 0, a zero gradient and no part in the mean. The same id twice counts
+// twice.
+//
+// HBM-bound: the forward reads the student's logits once (score_rows.h), one
+// wave a row adds the teacher's entries; the backward reads the logits once
+// more and writes the gradient once. Writing the gradient in the forward would
+// save that read where the upstream gradient is exactly 1, but such a loss is
+// weighted against another (or scaled, in fp16): the stored gradient would
+// then be read, scaled, rounded a second time and written again.
+#include "score_rows.h"
+
+namespace ak {
+namespace {
+
+constexpr int kPerLane = kMaxTop / 64;  // a row's entries held by one wave
+
+struct TeacherArgs {
+  const void* logits;  // [rows, top] of dtype `code`
+  const int64_t* ids;  // [rows, top]
+  int64_t ld, ld_ids;
+  int top, code, vocab;
+  float t2;            // temperature^2
+};
+
+__device__ __forceinline__ float teacher_logit(const TeacherArgs& a, int64_t row, int k) {
+  const int64_t at = row * a.ld + k;
+  if (a.code == AK_DTYPE_F32) return static_cast<const float*>(a.logits)[at];
+  if (a.code == AK_DTYPE_F16) return to_f32(static_cast<const f16*>(a.logits)[at]);
+  return to_f32(static_cast<const bf16*>(a.logits)[at]);
+}
+
+// One row's entries in one wave: -inf where there is none.
+struct Entries {
+  float t[kPerLane];
+  int id[kPerLane];
+  bool bad;  // an id outside the vocabulary
+  __device__ __forceinline__ Entries(const TeacherArgs& a, int64_t row, int64_t ignore_index) {
+    bad = false;
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int i = 0; i < kPerLane; ++i) {
+      t[i] = -INFINITY;
+      id[i] = 0;
+      const int k = lane + 64 * i;
+      if (k >= a.top) continue;
+      const int64_t c = a.ids[row * a.ld_ids + k];
+      if (c == ignore_index) continue;
+      if (c < 0 || c >= a.vocab) bad = true;
+      else {
+        id[i] = (int)c;
+        t[i] = teacher_logit(a, row, k);
+      }
+    }
+  }
+};
+
+// Loss of a row, by one wave. out: (m, log2 s, the largest teacher logit, log2
+// of the sum of 2^((t - largest) c2)) for the backward; m is NaN where the
+// loss is.
+template <bool CAP>
+__device__ __forceinline__ void finish_row(const ScoreParams& p, const TeacherArgs& a, int64_t row, const RowStats& st,
+                                           const Entries& en, const float* x, float* __restrict__ losses,
+                                           f32x4_t* __restrict__ out) {
+  float tm = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < kPerLane; ++i) tm = fmaxf(tm, en.t[i]);
+  tm = wave_max(tm);
+  const bool any_bad = __any(en.bad);
+  bool nan = false;
+#pragma unroll
+  for (int i = 0; i < kPerLane; ++i) nan |= en.t[i] != en.t[i];
+  nan = __any(nan) || any_bad;
+  float loss = 0.0f, tl = 0.0f, m = st.m;
+  const float l2 = log2_sum(st);
+  if (nan) {
+    loss = m = NAN;
+    tm = 0.0f;
+  } else if (tm != -INFINITY) {
+    float ts = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kPerLane; ++i) ts += __builtin_amdgcn_exp2f((en.t[i] - tm) * p.c2);
+    tl = __builtin_amdgcn_logf(wave_sum(ts));
+#pragma unroll
+    for (int i = 0; i < kPerLane; ++i) {
+      const float lq = (en.t[i] - tm) * p.c2 - tl;
+      const float q = __builtin_amdgcn_exp2f(lq);
+      if (q != 0.0f) loss += q * (kLn2 * lq - log_prob(p, score<CAP>(p, x[i]), st.m, l2));
+    }
+    loss = wave_sum(loss) * a.t2;
+    if (loss != loss) m = NAN;
+  }
+  if ((threadIdx.x & 63) == 0) {
+    losses[row] = loss;
+    out[row] = f32x4_t{m, l2, tm, tl};
+  }
+}
+
+// One workgroup per segment (units by grid stride; the loop bound is uniform).
+template <typename T, int VPT, int TPR, bool CAP>
+__global__ void __launch_bounds__(TPR, VPT == 8 ? 8 : 1)
+distill_segment_kernel(const T* __restrict__ logits, int64_t rows, int64_t ld, int segs, int span, ScoreParams p,
+                       TeacherArgs a, float* __restrict__ losses, f32x4_t* __restrict__ stats,
+                       f32x4_t* __restrict__ part) {
+  constexpr int W = TPR / 64;
+  __shared__ float part_m[W], part_s[W];
+  for (int64_t unit = blockIdx.x; unit < rows * segs; unit += gridDim.x) {
+    const int64_t row = segs == 1 ? unit : unit / segs;
+    const int seg = segs == 1 ? 0 : (int)(unit - row * segs);
+    const T* x = logits + row * ld;
+    Segment<T, VPT, TPR> sg(x, a.vocab, seg, span);
+    float m = wave_max(sg.largest());
+    if ((threadIdx.x & 63) == 0) part_m[threadIdx.x / 64] = m;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < W; ++i) m = fmaxf(m, part_m[i]);
+    RowStats st;
+    st.m = CAP ? score<CAP>(p, m) : m;
+    sg.template sums<CAP, false>(p, st.m, st.s, st.u);
+    st.s = wave_sum(st.s);
+    if ((threadIdx.x & 63) == 0) part_s[threadIdx.x / 64] = st.s;
+    __syncthreads();  // part_m has been read by all, so the next unit may write it
+    st.s = part_s[0];
+#pragma unroll
+    for (int i = 1; i < W; ++i) st.s += part_s[i];
+    if (segs > 1) {
+      if (threadIdx.x == 0) part[unit] = f32x4_t{st.m, st.s, 0.0f, 0.0f};
+    } else if (threadIdx.x < 64) {
+      const Entries en(a, row, p.ignore_index);
+      float xs[kPerLane];
+#pragma unroll
+      for (int i = 0; i < kPerLane; ++i) xs[i] = to_f32(x[en.id[i]]);
+      finish_row<CAP>(p, a, row, st, en, xs, losses, stats);
+    }
+    __syncthreads();  // part_s is rewritten for the workgroup's next unit
+  }
+}
+
+// Joins a row's segments, one wave a row.
+template <typename T, bool CAP>
+__global__ void __launch_bounds__(64)
+distill_join_kernel(const T* __restrict__ logits, int64_t ld, int segs, ScoreParams p, TeacherArgs a,
+                    float* __restrict__ losses, f32x4_t* __restrict__ stats, const f32x4_t* __restrict__ part) {
+  const int64_t row = blockIdx.x;
+  const Entries en(a, row, p.ignore_index);
+  float xs[kPerLane];
+#pragma unroll
+  for (int i = 0; i < kPerLane; ++i) xs[i] = to_f32(logits[row * ld + en.id[i]]);
+  RowStats st{-INFINITY, 0.0f, 0.0f};
+  for (int i = threadIdx.x; i < segs; i += 64) {
+    const f32x4_t q = part[row * segs + i];
+    st = join_stats(p, st, RowStats{q[0], q[1], 0.0f});
+  }
+  st = wave_join(p, st);
+  finish_row<CAP>(p, a, row, st, en, xs, losses, stats);
+}
+
+// loss[0] = sum of losses / max(1, #rows with entries), scale[0] = 1 / that
+// divisor; one workgroup, in a fixed order.
+constexpr int kMeanThreads = 1024;
+
+__global__ void __launch_bounds__(kMeanThreads)
+distill_mean_kernel(const float* __restrict__ losses, const f32x4_t* __restrict__ stats, int64_t rows,
+                    float* __restrict__ loss, float* __restrict__ scale) {
+  __shared__ float part_s[kMeanThreads / 64], part_n[kMeanThreads / 64];
+  float s = 0.0f;
+  int n = 0;
+  for (int64_t i = threadIdx.x; i < rows; i += kMeanThreads) {
+    s += losses[i];
+    n += stats[i][2] != -INFINITY;
+  }
+  s = wave_sum(s);
+  for (int off = 32; off >= 1; off >>= 1) n += __shfl_xor(n, off, 64);
+  if ((threadIdx.x & 63) == 0) {
+    part_s[threadIdx.x / 64] = s;
+    part_n[threadIdx.x / 64] = (float)n;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    float c = part_n[0];
+    s = part_s[0];
+    for (int i = 1; i < kMeanThreads / 64; ++i) {
+      s += part_s[i];
+      c += part_n[i];
+    }
+    c = fmaxf(c, 1.0f);
+    loss[0] = s / c;
+    scale[0] = 1.0f / c;
+  }
+}
+
+// The gradient from the forward's statistics; blockIdx.y takes `span` vectors
+// of the row. The entries' columns are written again, with their terms, once
+// the row's others have left; the same id twice writes the same value twice.
+template <typename T, bool CAP, bool NT, int U>
+__global__ void __launch_bounds__(kGradThreads)
+distill_grad_kernel(const T* __restrict__ logits, const f32x4_t* __restrict__ stats, const float* __restrict__ g_loss,
+                    int64_t g_stride, const float* __restrict__ scale, T* __restrict__ grad, int64_t rows,
+                    int64_t ld, int64_t ld_g, int span, ScoreParams p, TeacherArgs a) {
+  __shared__ int sid[kMaxTop];
+  __shared__ float sq[kMaxTop];
+  const int v0 = blockIdx.y * span, v1 = v0 + span;
+  const bool ends = blockIdx.y == 0;
+  const int t = threadIdx.x;
+  static_assert(kMaxTop <= kGradThreads, "an entry a thread");
+  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+    const T* x = logits + row * ld;
+    T* gx = grad + row * ld_g;
+    const f32x4_t st = stats[row];
+    if (st[2] == -INFINITY) {  // no entries
+      map_row<T, NT, 1>(x, gx, a.vocab, v0, v1, ends, [](float) { return 0.0f; });
+      continue;
+    }
+    if (t < a.top) {
+      const int64_t c = a.ids[row * a.ld_ids + t];
+      const bool there = c != p.ignore_index && c >= 0 && c < a.vocab;
+      sid[t] = there ? (int)c : -1;
+      sq[t] = there ? __builtin_amdgcn_exp2f((teacher_logit(a, row, t) - st[2]) * p.c2 - st[3]) : 0.0f;
+    }
+    const float m = st[0] == -INFINITY ? 0.0f : st[0], l2 = st[1];
+    const float c = g_loss[row * g_stride] * (scale ? scale[0] : 1.0f) * a.t2;
+    auto term = [&](float v, float q) {
+      float slope;
+      const float y = score_and_slope<CAP>(p, v, slope);
+      return (__builtin_amdgcn_exp2f((y - m) * p.c2 - l2) - q) * (c * slope);
+    };
+    map_row<T, NT, U>(x, gx, a.vocab, v0, v1, ends, [&](float v) { return term(v, 0.0f); });
+    stores_done();
+    if (t < a.top) {
+      const int id = sid[t];
+      if (id >= 0 && wrote_column(x, a.vocab, v0, v1, ends, id)) {
+        float q = 0.0f;
+        for (int k = 0; k < a.top; ++k) q += sid[k] == id ? sq[k] : 0.0f;
+        gx[id] = from_f32<T>(term(to_f32(x[id]), q));
+      }
+    }
+    __syncthreads();  // sid / sq are rewritten for the workgroup's next row
+  }
+}
+
+size_t part_bytes(int64_t rows, const ScorePlan& pl) {
+  return pl.segs > 1 && rows > 0 ? ((size_t)rows * pl.segs * sizeof(f32x4_t) + 255) & ~(size_t)255 : 0;
+}
+
+template <typename T, bool CAP>
+void launch_fwd(const void* logits, int64_t rows, int64_t ld, const ScorePlan& pl, const ScoreParams& p,
+                const TeacherArgs& a, float* losses, float* stats, void* ws, hipStream_t s) {
+  const T* x = static_cast<const T*>(logits);
+  f32x4_t* st = reinterpret_cast<f32x4_t*>(stats);
+  f32x4_t* part = static_cast<f32x4_t*>(ws);
+  const dim3 grid(row_grid(rows * pl.segs));
+#define GO(VPT, TPR) \
+  distill_segment_kernel<T, VPT, TPR, CAP><<<grid, dim3(TPR), 0, s>>>(x, rows, ld, pl.segs, pl.span, p, a, losses, st, part)
+  AK_SEGMENT_DISPATCH(pl.span, GO);
+#undef GO
+  if (pl.segs > 1) distill_join_kernel<T, CAP><<<dim3((unsigned)rows), dim3(64), 0, s>>>(x, ld, pl.segs, p, a, losses, st, part);
+}
+
+template <typename T, bool CAP>
+void launch_bwd(const void* logits, const float* stats, const float* g_loss, int64_t g_stride, const float* scale,
+                void* grad, int64_t rows, int64_t ld, int64_t ld_g, const ScoreParams& p, const TeacherArgs& a,
+                hipStream_t s) {
+  constexpr int VE = Vec16<T>::VE;
+  const ScorePlan pl = grad_plan(a.vocab, VE);
+  const dim3 grid(row_grid(rows), pl.segs), block(kGradThreads);
+  const T* x = static_cast<const T*>(logits);
+  T* g = static_cast<T*>(grad);
+  const f32x4_t* st = reinterpret_cast<const f32x4_t*>(stats);
+  if (a.vocab / VE < 4 * kGradThreads)
+    distill_grad_kernel<T, CAP, false, 1><<<grid, block, 0, s>>>(x, st, g_loss, g_stride, scale, g, rows, ld, ld_g, pl.span, p, a);
+  else if (score_past_cache(2 * rows * a.vocab * (int64_t)sizeof(T)))
+    distill_grad_kernel<T, CAP, true, 4><<<grid, block, 0, s>>>(x, st, g_loss, g_stride, scale, g, rows, ld, ld_g, pl.span, p, a);
+  else
+    distill_grad_kernel<T, CAP, false, 4><<<grid, block, 0, s>>>(x, st, g_loss, g_stride, scale, g, rows, ld, ld_g, pl.span, p, a);
+}
+
+int check(const char* name, const void* logits, const void* teacher, const int64_t* ids, int64_t rows, int64_t vocab,
+          int64_t top, int64_t ld, int64_t ld_t, int64_t ld_ids, float temperature, float softcap, int dtype,
+          int teacher_dtype) {
+  const int rc = check_score_rows(name, rows, vocab, ld, temperature, softcap, dtype);
+  if (rc) return rc;
+  if (ak_dtype_size(teacher_dtype) == 0) return ak_set_error(AK_ERR_UNSUPPORTED, "%s: unsupported teacher dtype code %d", name, teacher_dtype);
+  if (top < 1 || top > kMaxTop)
+    return ak_set_error(AK_ERR_INVALID_ARG, "%s: %lld teacher entries a row, 1 to %d are taken", name, (long long)top, kMaxTop);
+  if (ld_t < top || ld_ids < top) return ak_set_error(AK_ERR_INVALID_ARG, "%s: row pitch smaller than the entries", name);
+  if (!ak_extent_ok(rows, ld_t, top, 4) || !ak_extent_ok(rows, ld_ids, top, 8))
+    return ak_set_error(AK_ERR_INVALID_ARG, "%s: rows=%lld x pitch exceed 64-bit addressing", name, (long long)rows);
+  if (rows > 0 && (!logits || !teacher || !ids)) return ak_set_error(AK_ERR_INVALID_ARG, "%s: null pointer", name);
+  return AK_OK;
+}
+
+}  // namespace
+}  // namespace ak
+
+extern "C" size_t ak_topk_distill_workspace_bytes(int64_t rows, int64_t vocab, int dtype) {
+  const int esz = ak_dtype_size(dtype);
+  if (rows <= 0 || vocab <= 0 || vocab > ak::kScoreVocab || esz == 0) return 0;
+  return ak::part_bytes(rows, ak::score_plan(rows, vocab, 16 / esz, 0));
+}
+
+extern "C" int ak_topk_distill_fwd(const void* logits, const void* teacher_logits, const int64_t* teacher_ids,
+                                   float* losses, float* stats, float* loss, float* scale, void* workspace,
+                                   size_t workspace_bytes, int64_t rows, int64_t vocab, int64_t top, int64_t ld_logits,
+                                   int64_t ld_teacher, int64_t ld_ids, float temperature, float softcap,
+                                   int64_t ignore_index, int dtype, int teacher_dtype, void* stream) {
+  const char* name = "ak_topk_distill_fwd";
+  const int rc = ak::check(name, logits, teacher_logits, teacher_ids, rows, vocab, top, ld_logits, ld_teacher, ld_ids,
+                           temperature, softcap, dtype, teacher_dtype);
+  if (rc) return rc;
+  if (!loss != !scale || (rows > 0 && (!losses || !stats))) return ak_set_error(AK_ERR_INVALID_ARG, "%s: null pointer", name);
+  if (stats && !ak::aligned16(stats)) return ak_set_error(AK_ERR_INVALID_ARG, "%s: stats must be 16-byte aligned", name);
+  hipStream_t s = ak_stream(stream);
+  if (rows > 0) {
+    const ak::ScorePlan pl = ak::score_plan(rows, vocab, 16 / ak_dtype_size(dtype), 0);
+    const size_t need = ak::part_bytes(rows, pl);
+    if (workspace_bytes < need || (need && (!workspace || !ak::aligned16(workspace))))
+      return ak_set_error(AK_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed (16-byte aligned)", name, workspace_bytes, need);
+    const ak::ScoreParams p = ak::score_params(temperature, softcap, ignore_index);
+    const ak::TeacherArgs a{teacher_logits, teacher_ids, ld_teacher, ld_ids, (int)top, teacher_dtype, (int)vocab,
+                            temperature * temperature};
+    auto go = [&](auto t) {
+      using T = decltype(t);
+      if (softcap > 0.0f) ak::launch_fwd<T, true>(logits, rows, ld_logits, pl, p, a, losses, stats, workspace, s);
+      else ak::launch_fwd<T, false>(logits, rows, ld_logits, pl, p, a, losses, stats, workspace, s);
+    };
+    if (dtype == AK_DTYPE_F32) go(float());
+    else if (dtype == AK_DTYPE_F16) go(ak::f16());
+    else go(ak::bf16());
+  }
+  if (loss)
+    ak::distill_mean_kernel<<<dim3(1), dim3(ak::kMeanThreads), 0, s>>>(losses, reinterpret_cast<ak::f32x4_t*>(stats), rows, loss, scale);
+  return ak_check_launch(name);
+}
+
+extern "C" int ak_topk_distill_bwd(const void* logits, const void* teacher_logits, const int64_t* teacher_ids,
+                                   const float* stats, const float* grad_loss, int64_t grad_stride, const float* scale,
+                                   void* grad_logits, int64_t rows, int64_t vocab, int64_t top, int64_t ld_logits,
+                                   int64_t ld_teacher, int64_t ld_ids, int64_t ld_grad, float temperature,
+                                   float softcap, int64_t ignore_index, int dtype, int teacher_dtype, void* stream) {
+  const char* name = "ak_topk_distill_bwd";
+  int rc = ak::check(name, logits, teacher_logits, teacher_ids, rows, vocab, top, ld_logits, ld_teacher, ld_ids,
+                     temperature, softcap, dtype, teacher_dtype);
+  if (!rc) rc = ak::check_score_rows(name, rows, vocab, ld_grad, temperature, softcap, dtype);
+  if (rc) return rc;
+  if (grad_stride != 0 && grad_stride != 1) return ak_set_error(AK_ERR_INVALID_ARG, "%s: grad_stride must be 0 or 1", name);
+  if (rows == 0) return AK_OK;
+  if (!stats || !grad_loss || !grad_logits) return ak_set_error(AK_ERR_INVALID_ARG, "%s: null pointer", name);
+  if (!ak::aligned16(stats)) return ak_set_error(AK_ERR_INVALID_ARG, "%s: stats must be 16-byte aligned", name);
+  const ak::ScoreParams p = ak::score_params(temperature, softcap, ignore_index);
+  const ak::TeacherArgs a{teacher_logits, teacher_ids, ld_teacher, ld_ids, (int)top, teacher_dtype, (int)vocab,
+                          temperature * temperature};
+  hipStream_t s = ak_stream(stream);
+  auto go = [&](auto t) {
+    using T = decltype(t);
+    if (softcap > 0.0f) ak::launch_bwd<T, true>(logits, stats, grad_loss, grad_stride, scale, grad_logits, rows, ld_logits, ld_grad, p, a, s);
+    else ak::launch_bwd<T, false>(logits, stats, grad_loss, grad_stride, scale, grad_logits, rows, ld_logits, ld_grad, p, a, s);
+  };
+  if (dtype == AK_DTYPE_F32) go(float());
+  else if (dtype == AK_DTYPE_F16) go(ak::f16());
+  else go(ak::bf16());
+  return ak_check_launch(name);
+}

@@ -67,6 +67,15 @@ _SIGNATURES = {
     "ak_ce_mean": [_c_void_p, _c_void_p, _c_void_p, _i64, _i64, _f32, _c_void_p, _c_void_p,
                    _c_void_p],
     "ak_scale_inplace": [_c_void_p, _i64, _c_void_p, _int, _c_void_p],
+    "ak_token_logprobs_workspace_bytes": [_i64, _i64, _int, _int],
+    "ak_token_logprobs_fwd": [_c_void_p] * 8 + [ctypes.c_size_t, _i64, _i64, _i64, _int, _f32, _f32, _i64, _int,
+                                                _c_void_p],
+    "ak_token_logprobs_bwd": [_c_void_p] * 6 + [_i64] * 4 + [_f32, _f32, _i64, _int, _c_void_p],
+    "ak_topk_distill_workspace_bytes": [_i64, _i64, _int],
+    "ak_topk_distill_fwd": [_c_void_p] * 8 + [ctypes.c_size_t] + [_i64] * 6 + [_f32, _f32, _i64, _int, _int,
+                                                                             _c_void_p],
+    "ak_topk_distill_bwd": [_c_void_p] * 5 + [_i64, _c_void_p, _c_void_p] + [_i64] * 7
+    + [_f32, _f32, _i64, _int, _int, _c_void_p],
     "ak_lmhead_ce_workspace_bytes": [_i64, _i64],
     "ak_lmhead_ce_fwd": [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
                          _c_void_p, ctypes.c_size_t, _i64, _i64, _i64, _i64, _i64, _i64, _f32, _f32,
@@ -93,6 +102,8 @@ _SIGNATURES = {
 _RESTYPES = {
     "ak_last_error": ctypes.c_char_p,
     "ak_target_arch": ctypes.c_char_p,
+    "ak_token_logprobs_workspace_bytes": ctypes.c_size_t,
+    "ak_topk_distill_workspace_bytes": ctypes.c_size_t,
     "ak_lmhead_ce_workspace_bytes": ctypes.c_size_t,
     "ak_lmhead_grad_workspace_bytes": ctypes.c_size_t,
     "ak_rmsnorm_bwd_workspace_bytes": ctypes.c_size_t,
@@ -464,6 +475,96 @@ def scale_inplace(x: torch.Tensor, scale: torch.Tensor) -> None:
     with _on_device(x):
         rc = load().ak_scale_inplace(_ptr(x), x.numel(), _ptr(scale), dtype_code(x.dtype), _stream(x))
     _check(rc, "ak_scale_inplace")
+
+
+# Most alternatives of a row, and the widest row, of the entry points below.
+MAX_TOP = 256
+MAX_SCORE_VOCAB = 1 << 20
+
+
+def _workspace(nbytes: int, device: torch.device) -> Optional[torch.Tensor]:
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+def token_logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor], logprobs: Optional[torch.Tensor],
+                   entropy: Optional[torch.Tensor], stats: Optional[torch.Tensor],
+                   top_logprobs: Optional[torch.Tensor], top_ids: Optional[torch.Tensor], temperature: float,
+                   softcap: float, ignore_index: int) -> None:
+    """Log probabilities of ``tokens`` (int64), entropies and the top
+    alternatives (``[rows, k]``) of ``logits [rows, vocab]``; ``stats`` fp32
+    ``[rows, 4]`` is for the backward. Outputs that are None are not written."""
+    require_device(logits, tokens, logprobs, entropy, stats, top_logprobs, top_ids)
+    rows, vocab = logits.shape
+    top = top_ids.shape[1] if top_ids is not None else 0
+    code = dtype_code(logits.dtype)
+    lib = load()
+    nbytes = int(lib.ak_token_logprobs_workspace_bytes(rows, vocab, top, code))
+    with _on_device(logits):
+        ws = _workspace(nbytes, logits.device)
+        rc = lib.ak_token_logprobs_fwd(_ptr(logits), _ptr(tokens), _ptr(logprobs), _ptr(entropy), _ptr(stats),
+                                       _ptr(top_logprobs), _ptr(top_ids), _ptr(ws), nbytes, rows, vocab,
+                                       _rows_view(logits, "logits"), top, float(temperature), float(softcap),
+                                       int(ignore_index), code, _stream(logits))
+    _check(rc, "ak_token_logprobs_fwd")
+
+
+def token_logprobs_bwd(logits: torch.Tensor, tokens: Optional[torch.Tensor], stats: torch.Tensor,
+                       grad_logprobs: Optional[torch.Tensor], grad_entropy: Optional[torch.Tensor],
+                       grad: torch.Tensor, temperature: float, softcap: float, ignore_index: int) -> None:
+    """Gradient of :func:`token_logprobs` into ``grad [rows, vocab]`` from the
+    upstream gradients (contiguous fp32 ``[rows]``, or None)."""
+    require_device(logits, tokens, stats, grad_logprobs, grad_entropy, grad)
+    rows, vocab = logits.shape
+    with _on_device(logits):
+        rc = load().ak_token_logprobs_bwd(_ptr(logits), _ptr(tokens), _ptr(stats), _ptr(grad_logprobs),
+                                          _ptr(grad_entropy), _ptr(grad), rows, vocab,
+                                          _rows_view(logits, "logits"), _rows_view(grad, "grad"),
+                                          float(temperature), float(softcap), int(ignore_index),
+                                          dtype_code(logits.dtype), _stream(logits))
+    _check(rc, "ak_token_logprobs_bwd")
+
+
+def topk_distill(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_ids: torch.Tensor,
+                 losses: torch.Tensor, stats: torch.Tensor, loss: Optional[torch.Tensor],
+                 scale: Optional[torch.Tensor], temperature: float, softcap: float, ignore_index: int) -> None:
+    """Per-row distillation losses of ``logits [rows, vocab]`` against
+    ``teacher_logits [rows, k]`` at the columns ``teacher_ids`` (int64), and
+    with ``loss`` and ``scale`` their mean over the rows that have entries and
+    the reciprocal of its divisor. ``stats``: fp32 ``[rows, 4]``."""
+    require_device(logits, teacher_logits, teacher_ids, losses, stats, loss, scale)
+    rows, vocab = logits.shape
+    code = dtype_code(logits.dtype)
+    lib = load()
+    nbytes = int(lib.ak_topk_distill_workspace_bytes(rows, vocab, code))
+    with _on_device(logits):
+        ws = _workspace(nbytes, logits.device)
+        rc = lib.ak_topk_distill_fwd(_ptr(logits), _ptr(teacher_logits), _ptr(teacher_ids), _ptr(losses),
+                                     _ptr(stats), _ptr(loss), _ptr(scale), _ptr(ws), nbytes, rows, vocab,
+                                     teacher_ids.shape[1], _rows_view(logits, "logits"),
+                                     _rows_view(teacher_logits, "teacher_logits"),
+                                     _rows_view(teacher_ids, "teacher_ids"), float(temperature), float(softcap),
+                                     int(ignore_index), code, dtype_code(teacher_logits.dtype), _stream(logits))
+    _check(rc, "ak_topk_distill_fwd")
+
+
+def topk_distill_bwd(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_ids: torch.Tensor,
+                     stats: torch.Tensor, grad_loss: torch.Tensor, scale: Optional[torch.Tensor],
+                     grad: torch.Tensor, temperature: float, softcap: float, ignore_index: int) -> None:
+    """Gradient of :func:`topk_distill` into ``grad [rows, vocab]``;
+    ``grad_loss`` (fp32) is one upstream gradient (with ``scale``, the
+    mean's), or one a row."""
+    require_device(logits, teacher_logits, teacher_ids, stats, grad_loss, scale, grad)
+    rows, vocab = logits.shape
+    with _on_device(logits):
+        rc = load().ak_topk_distill_bwd(_ptr(logits), _ptr(teacher_logits), _ptr(teacher_ids), _ptr(stats),
+                                        _ptr(grad_loss), 0 if scale is not None else 1, _ptr(scale), _ptr(grad),
+                                        rows, vocab, teacher_ids.shape[1], _rows_view(logits, "logits"),
+                                        _rows_view(teacher_logits, "teacher_logits"),
+                                        _rows_view(teacher_ids, "teacher_ids"), _rows_view(grad, "grad"),
+                                        float(temperature), float(softcap), int(ignore_index),
+                                        dtype_code(logits.dtype), dtype_code(teacher_logits.dtype),
+                                        _stream(logits))
+    _check(rc, "ak_topk_distill_bwd")
 
 
 def lmhead_ce_workspace_bytes(n_rows: int, vocab: int) -> int:

@@ -236,6 +236,78 @@ int ak_ce_mean(const float* losses, const float* lse, const int64_t* targets,
 int ak_scale_inplace(void* x, int64_t n, const float* scale, int dtype, void* stream);
 
 /*
+ * Log probabilities of given tokens, with the entropy and the top alternatives
+ * of each row of logits [rows, vocab]:
+ *   y = softcap > 0 ? softcap * tanh(x / softcap) : x,  p = softmax(y / temperature)
+ *   logprobs[r] = ln p[tokens[r]]     entropy[r] = -sum_v p_v ln p_v
+ *   top_logprobs / top_ids [rows, top_k]: the largest ln p, descending, and
+ *   their columns; equal logits go by column, NaN come first.
+ * tokens (and then logprobs), entropy and stats may be NULL. A row whose token
+ * is ignore_index has logprob and entropy 0; a token outside [0, vocab) that is
+ * not ignore_index has logprob NaN. A row of -inf alone has logprob -inf and
+ * entropy 0; a row that holds a NaN or +inf has NaN results. stats [rows, 4]
+ * fp32, 16-byte aligned, is what ak_token_logprobs_bwd takes. top_k is at most
+ * 256 and vocab, vocab at most 2^20. workspace: as many bytes as the query says
+ * (0 for most calls; few or very wide rows are cut into segments), 16-byte
+ * aligned. No counterpart in the reference, whose cross-entropy
+ * (kernels/ce_fused.py:122-382) gives the loss of given tokens only.
+ */
+size_t ak_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int top_k, int dtype);
+int ak_token_logprobs_fwd(const void* logits, const int64_t* tokens, float* logprobs, float* entropy,
+                          float* stats, float* top_logprobs, int64_t* top_ids, void* workspace,
+                          size_t workspace_bytes, int64_t rows, int64_t vocab, int64_t ld_logits,
+                          int top_k, float temperature, float softcap, int64_t ignore_index,
+                          int dtype, void* stream);
+
+/*
+ * Backward of ak_token_logprobs_fwd, with g = grad_logprobs[r] and e =
+ * grad_entropy[r] (fp32 [rows]; NULL: no such gradient):
+ *   grad[r, v] = (g ([v == tokens[r]] - p_v) - e p_v (ln p_v + entropy))
+ *                * (softcap > 0 ? 1 - tanh^2 : 1) / temperature
+ * rounded once to the element type. Rows of an ignored token, and rows of -inf
+ * alone, get zeros; a token outside [0, vocab) a NaN row.
+ */
+int ak_token_logprobs_bwd(const void* logits, const int64_t* tokens, const float* stats,
+                          const float* grad_logprobs, const float* grad_entropy, void* grad_logits,
+                          int64_t rows, int64_t vocab, int64_t ld_logits, int64_t ld_grad,
+                          float temperature, float softcap, int64_t ignore_index, int dtype,
+                          void* stream);
+
+/*
+ * Distillation from a teacher's top logits: teacher_logits [rows, top] of
+ * teacher_dtype at the columns teacher_ids [rows, top] of the student's
+ * logits [rows, vocab]. With p as above and q = softmax(teacher_logits /
+ * temperature) over the row's entries (those whose id is not ignore_index),
+ *   losses[r] = temperature^2 sum_k q_k (ln q_k - ln p[id_k]),
+ * 0 for a row without entries (or whose teacher logits are all -inf). loss[0]
+ * = their sum / max(1, #rows with entries), in a fixed order, and scale[0] = 1 /
+ * that divisor (both NULL: no mean). An id outside [0, vocab) that is not
+ * ignore_index gives a NaN loss and gradient row. stats [rows, 4] fp32,
+ * 16-byte aligned, is written for the backward and the mean. top is 1 to 256,
+ * vocab at most 2^20. workspace as above. No counterpart in the reference.
+ */
+size_t ak_topk_distill_workspace_bytes(int64_t rows, int64_t vocab, int dtype);
+int ak_topk_distill_fwd(const void* logits, const void* teacher_logits, const int64_t* teacher_ids,
+                        float* losses, float* stats, float* loss, float* scale, void* workspace,
+                        size_t workspace_bytes, int64_t rows, int64_t vocab, int64_t top,
+                        int64_t ld_logits, int64_t ld_teacher, int64_t ld_ids, float temperature,
+                        float softcap, int64_t ignore_index, int dtype, int teacher_dtype,
+                        void* stream);
+
+/*
+ * Its backward: grad[r, v] = grad_loss[r * grad_stride] * scale[0] (NULL: 1) *
+ *   temperature (p_v - sum of q_k with id_k == v) (softcap > 0 ? 1 - tanh^2 : 1),
+ * rounded once; grad_stride 0 takes one upstream gradient for all rows, 1 one
+ * a row. Rows without entries get zeros.
+ */
+int ak_topk_distill_bwd(const void* logits, const void* teacher_logits, const int64_t* teacher_ids,
+                        const float* stats, const float* grad_loss, int64_t grad_stride,
+                        const float* scale, void* grad_logits, int64_t rows, int64_t vocab,
+                        int64_t top, int64_t ld_logits, int64_t ld_teacher, int64_t ld_ids,
+                        int64_t ld_grad, float temperature, float softcap, int64_t ignore_index,
+                        int dtype, int teacher_dtype, void* stream);
+
+/*
  * Fused lm-head + cross-entropy forward: logits = hidden @ weight^T are
  * produced tile by tile on the matrix cores and folded into an online
  * logsumexp; they are never written to memory.
