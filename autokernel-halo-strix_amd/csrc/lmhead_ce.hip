@@ -16,7 +16,8 @@
 // ignored tokens contribute 0 and are excluded from the mean's
 // denominator, which is clamped to >= 1). The logsumexp runs over all
 // `vocab` columns (padded vocab entries are not masked, as in the reference).
-// Options: a logit softcap z' = cap tanh(z / cap), and label smoothing a
+// The same tiles give log probabilities and entropies (kEnt; the section of
+// that name below). Options: a logit softcap z' = cap tanh(z / cap), and label smoothing a
 // (loss = lse - (1 - a) z'_t - a mean(z'); the tile kernel then also writes
 // per-partial sums of z', merged by the row kernel in a fixed order).
 //
@@ -55,6 +56,8 @@ constexpr int kGroupV = 4;                               // vocab tiles per XCD 
 struct MSPair {
   float m, s;
 };
+
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
 // Tile coordinates of this workgroup's i-th tile. Work item w = block + i *
 // grid runs on XCD w % 8 (workgroups are dealt to the 8 XCDs round-robin);
@@ -128,6 +131,10 @@ struct GradArgs {
   // vocabulary of vocab_total entries
   int64_t v0;
   int64_t vocab_total;
+  // log probabilities (kEnt): log2(e) / temperature, and the backward's row
+  // coefficients (lse2, c0, c1, g / temperature)
+  float c2;
+  const f32x4_t* coefs;
 };
 
 // Logit softcap z' = cap * tanh(z / cap), evaluated without cancellation
@@ -151,7 +158,12 @@ struct Cap {
 // kLs (forward): label smoothing; the tile also writes the sum of its (capped)
 // logits per token to ga.zsum, laid out as the partials. A template flag, so
 // that the kernels without it carry no extra register pressure.
-template <typename T, bool kShift, bool kFineMask, bool kGrad, bool kCap = false, bool kLs = false>
+// kEnt: log probabilities and entropies of softmax(z' / temperature). Forward:
+// t = (z' - m) c2 with the partial's own maximum m, s = sum 2^t, and ga.zsum
+// takes u = sum 2^t t, from which the entropy is ln2 (log2 s - u / s) once the
+// partials are joined. Backward: dz = 2^t (c0 + c1 t) with t = z' c2 - lse2, the
+// row's coefficients in ga.coefs.
+template <typename T, bool kShift, bool kFineMask, bool kGrad, bool kCap = false, bool kLs = false, bool kEnt = false>
 __global__ void __launch_bounds__(kLThreads) __attribute__((amdgpu_waves_per_eu(1, 1)))
 lmhead_ce_tile_kernel(const T* __restrict__ H, const T* __restrict__ W, MSPair* __restrict__ part,
                       int n_rows, int vocab, int d, int64_t ldh, int64_t ldw, int n_vt, int n_tt,
@@ -330,7 +342,7 @@ lmhead_ce_tile_kernel(const T* __restrict__ H, const T* __restrict__ W, MSPair* 
   using yes = std::true_type;
   using no = std::false_type;
   // backward: upstream gradient / number of counted tokens, read once
-  const float gs = kGrad ? ga.grad_loss[0] / ga.denom[0] : 0.0f;
+  const float gs = kGrad && !kEnt ? ga.grad_loss[0] / ga.denom[0] : 0.0f;
   for (int it = 0; it < n_my; ++it) {
     int vt, tt;
     tile_coords(it, n_vt, n_tt, vt, tt);
@@ -347,8 +359,12 @@ lmhead_ce_tile_kernel(const T* __restrict__ H, const T* __restrict__ W, MSPair* 
     // is behind it.
     float pre_lse[4];
     int64_t pre_tg[4];
+    f32x4_t pre_co[4];
     auto prefetch_rows = [&]() {
-      if constexpr (kGrad) {
+      if constexpr (kGrad && kEnt) {
+#pragma unroll
+        for (int tb = 0; tb < 4; ++tb) pre_co[tb] = ga.coefs[min(t_first + wt * 128 + tb * 32 + fr, n_rows - 1)];
+      } else if constexpr (kGrad) {
 #pragma unroll
         for (int tb = 0; tb < 4; ++tb) {
           const int tok_c = min(t_first + wt * 128 + tb * 32 + fr, n_rows - 1);
@@ -397,11 +413,12 @@ lmhead_ce_tile_kernel(const T* __restrict__ H, const T* __restrict__ W, MSPair* 
         const int tok = t_first + wt * 128 + tb * 32 + fr;
         const int tok_c = min(tok, n_rows - 1);
         const bool tok_ok = tok >= t_own && tok < n_rows;
-        const float lse2 = pre_lse[tb] * kLog2e;
-        const float cl2 = kCap ? ga.cap * kLog2e - lse2 : 0.0f;  // log2 of exp(cap - lse)
-        const int64_t tg = pre_tg[tb];
+        const float lse2 = kEnt ? pre_co[tb][0] : pre_lse[tb] * kLog2e;
+        const float cl2 = kCap ? ga.cap * (kEnt ? ga.c2 : kLog2e) - lse2 : 0.0f;  // log2 of exp(cap - lse)
+        const float c0 = kEnt ? pre_co[tb][1] : 0.0f, c1 = kEnt ? pre_co[tb][2] : 0.0f;
+        const int64_t tg = kEnt ? 0 : pre_tg[tb];
         const float st = tg == ga.ignore_index ? 0.0f : ((tg < 0 || tg >= ga.vocab_total) ? NAN : gs);
-        const float nls = -(ga.ls / (float)ga.vocab_total) * st;  // label smoothing's uniform term
+        const float nls = kEnt ? 0.0f : -(ga.ls / (float)ga.vocab_total) * st;  // label smoothing's uniform term
         T* drow = dzp + (int64_t)tok_c * ga.ld_dz + v_first + wv * 128;
 #pragma unroll
         for (int vb = 0; vb < 4; ++vb) {
@@ -412,7 +429,19 @@ lmhead_ce_tile_kernel(const T* __restrict__ H, const T* __restrict__ W, MSPair* 
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               const float z = acc_read(acc[vb][tb][4 * g4 + j]);
-              if constexpr (kCap) {
+              if constexpr (kEnt) {
+                float t, slope = 1.0f;
+                if constexpr (kCap) {
+                  const Cap cp(ga.cap);
+                  const float q = cp.q(z);
+                  const float r = __builtin_amdgcn_rcpf(q + 1.0f);
+                  t = fmaf(-2.0f * ga.cap * ga.c2, r, cl2);
+                  slope = q < INFINITY ? 4.0f * q * r * r : 0.0f;
+                } else {
+                  t = fmaf(z, ga.c2, -lse2);
+                }
+                e[j] = __builtin_amdgcn_exp2f(t) * fmaf(c1, t, c0) * slope;
+              } else if constexpr (kCap) {
                 // softmax(z')_v * s_t * dz'/dz
                 const Cap cp(ga.cap);
                 const float q = cp.q(z);
@@ -480,7 +509,18 @@ lmhead_ce_tile_kernel(const T* __restrict__ H, const T* __restrict__ W, MSPair* 
               x[vb][r] = (o >= lo && o < hi) ? x[vb][r] : -INFINITY;
             }
           }
-        if constexpr (kCap) {
+        if constexpr (kEnt && kCap) {
+          // with a temperature the scores may lie far below cap / T: their own maximum
+          const Cap cp(ga.cap);
+#pragma unroll
+          for (int vb = 0; vb < 4; ++vb)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const float z = fmaf(-2.0f * ga.cap, __builtin_amdgcn_rcpf(cp.q(x[vb][r]) + 1.0f), ga.cap);
+              x[vb][r] = kTail && x[vb][r] == -INFINITY ? -INFINITY : z;
+            }
+        }
+        if constexpr (kCap && !kEnt) {
           // (cap, sum exp(z' - cap)) with exp(z' - cap) = exp2(nc r); masked
           // rows (x = -inf) would give exp(-2 cap) and are dropped. With label
           // smoothing the capped logits z' = cap - 2 cap r are summed too.
@@ -521,15 +561,24 @@ lmhead_ce_tile_kernel(const T* __restrict__ H, const T* __restrict__ W, MSPair* 
           for (int r = 0; r < 16; ++r) m4[r & 3] = fmaxf(m4[r & 3], x[vb][r]);
         float m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
         m = fmaxf(m, __shfl_xor(m, 32, 64));
-        const float ms = m * kLog2e;
-        float s4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        const float c2 = kEnt ? ga.c2 : kLog2e;
+        const float ms = m * c2;
+        float s4[4] = {0.0f, 0.0f, 0.0f, 0.0f}, u4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int vb = 0; vb < 4; ++vb)
 #pragma unroll
-          for (int r = 0; r < 16; ++r)
-            s4[r & 3] += __builtin_amdgcn_exp2f(fmaf(x[vb][r], kLog2e, -ms));
+          for (int r = 0; r < 16; ++r) {
+            const float t = fmaf(x[vb][r], c2, -ms);
+            const float e = __builtin_amdgcn_exp2f(t);
+            s4[r & 3] += e;
+            if constexpr (kEnt) u4[r & 3] = fmaf(e, kTail ? fmaxf(t, -1000.0f) : t, u4[r & 3]);
+          }
         float s = (s4[0] + s4[1]) + (s4[2] + s4[3]);
         s += __shfl_xor(s, 32, 64);
+        if constexpr (kEnt) {
+          const float u = (u4[0] + u4[1]) + (u4[2] + u4[3]);
+          zres[tb] = u + __shfl_xor(u, 32, 64);
+        }
         res[tb] = MSPair{m, s};
         __builtin_amdgcn_sched_barrier(0);  // one token block's values live at a time
       }
@@ -550,7 +599,7 @@ lmhead_ce_tile_kernel(const T* __restrict__ H, const T* __restrict__ W, MSPair* 
       const int tok = t_first + wt * 128 + tb * 32 + fr;
       if (lane < 32 && tok >= t_own && tok < n_rows) {
         prow[tok] = res[tb];
-        if constexpr (kLs) ga.zsum[(int64_t)(2 * vt + wv) * n_rows + tok] = zres[tb];
+        if constexpr (kLs || kEnt) ga.zsum[(int64_t)(2 * vt + wv) * n_rows + tok] = zres[tb];
       }
     }
   }
@@ -791,6 +840,153 @@ lmhead_ce_grad_target_kernel(const T* __restrict__ H, const T* __restrict__ W, G
   }
 }
 
+// ---------------------------------------------------------------------------
+// Log probabilities and entropies of softmax(z' / temperature)
+// ---------------------------------------------------------------------------
+
+// hidden[t] . weight[v], by one wave; every lane returns it.
+template <typename T>
+__device__ __forceinline__ float wave_dot(const T* __restrict__ hp, const T* __restrict__ wp, int d) {
+  float acc = 0.0f;
+#pragma unroll 4
+  for (int c = threadIdx.x & 63; c < d / 8; c += 64) {
+    const Vec16<T> a = load16<T>(hp + 8 * c);
+    const Vec16<T> b = load16<T>(wp + 8 * c);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc = fmaf(to_f32(a.e[e]), to_f32(b.e[e]), acc);
+  }
+  return wave_sum(acc);
+}
+
+// cap tanh(z / cap)
+__device__ __forceinline__ float capped(float z, float cap) {
+  return cap > 0.0f ? fmaf(-2.0f * cap, __builtin_amdgcn_rcpf(Cap(cap).q(z) + 1.0f), cap) : z;
+}
+
+struct MSU {
+  float m, s, u;
+};
+
+// Partial q folded into st; c2 as in the tile kernel.
+__device__ __forceinline__ MSU msu_merge(MSU a, MSU b, float c2) {
+  const float m = fmaxf(a.m, b.m);
+  MSU r{m, 0.0f, 0.0f};
+  auto add = [&](const MSU& q) {
+    if (q.s == 0.0f) return;
+    const float d = (q.m - m) * c2;
+    const float f = __builtin_amdgcn_exp2f(d);
+    r.s += f * q.s;
+    r.u += f * (q.u + fmaxf(d, -1000.0f) * q.s);  // f = 0 there
+  };
+  add(a);
+  add(b);
+  return r;
+}
+
+// Rows from the tile partials: a 512-thread workgroup owns 32 tokens, 16
+// threads a token fold every 16th partial and are joined in a fixed order; the
+// workgroup's waves form the given tokens' scores as their own dot products
+// meanwhile. stats: (lse2, entropy) of each row for the backward, lse2 = m c2 +
+// log2 s.
+template <typename T>
+__global__ void __launch_bounds__(kRowsPerBlock * kRowGroups)
+lmhead_logprob_rows_kernel(const T* __restrict__ H, const T* __restrict__ W, const MSPair* __restrict__ part,
+                           const float* __restrict__ usum, const int64_t* __restrict__ tokens,
+                           float* __restrict__ logprobs, float* __restrict__ entropy, f32x2_t* __restrict__ stats,
+                           int n_rows, int vocab, int d, int64_t ldh, int64_t ldw, int n_part, int64_t ignore_index,
+                           float cap, float c2, float inv_t) {
+  __shared__ MSU red[kRowGroups][kRowsPerBlock];
+  __shared__ float tl[kRowsPerBlock];
+  const int r = threadIdx.x % kRowsPerBlock, grp = threadIdx.x / kRowsPerBlock;
+  const int row0 = blockIdx.x * kRowsPerBlock, row = row0 + r;
+  constexpr int kWaves = kRowsPerBlock * kRowGroups / 64;
+  constexpr int kInFlight = 8;
+  MSU st{-INFINITY, 0.0f, 0.0f};
+  if (row < n_rows) {
+    for (int v0 = grp; v0 < n_part; v0 += kInFlight * kRowGroups) {
+      MSPair a[kInFlight];
+      float u[kInFlight];
+#pragma unroll
+      for (int i = 0; i < kInFlight; ++i) {
+        const int64_t at = (int64_t)min(v0 + i * kRowGroups, n_part - 1) * n_rows + row;
+        a[i] = part[at];
+        u[i] = usum[at];
+      }
+#pragma unroll
+      for (int i = 0; i < kInFlight; ++i)
+        if (v0 + i * kRowGroups < n_part) st = msu_merge(st, MSU{a[i].m, a[i].s, u[i]}, c2);
+    }
+  }
+  red[grp][r] = st;
+  if (tokens) {
+    for (int i = threadIdx.x / 64; i < kRowsPerBlock; i += kWaves) {
+      const int q = row0 + i;
+      const int64_t t = q < n_rows ? tokens[q] : -1;
+      float z = 0.0f;
+      if (t != ignore_index && t >= 0 && t < vocab) z = wave_dot(H + (int64_t)q * ldh, W + t * ldw, d);  // wave-uniform
+      if ((threadIdx.x & 63) == 0) tl[i] = z;
+    }
+  }
+  __syncthreads();
+  if (grp != 0 || row >= n_rows) return;
+  for (int g = 1; g < kRowGroups; ++g) st = msu_merge(st, red[g][r], c2);
+  const float l2 = __builtin_amdgcn_logf(st.s);
+  float h = kLn2 * (l2 - st.u / st.s);
+  if (h < 0.0f) h = 0.0f;  // one rounding below zero where one token holds all
+  if (stats) stats[row] = f32x2_t{fmaf(st.m, c2, l2), h};
+  if (tokens) {
+    const int64_t t = tokens[row];
+    float lp = (capped(tl[r], cap) - st.m) * inv_t - kLn2 * l2;
+    if (t == ignore_index) lp = h = 0.0f;
+    else if (t < 0 || t >= vocab) lp = NAN;
+    logprobs[row] = lp;
+  }
+  if (entropy) entropy[row] = h;
+}
+
+// Row coefficients of the backward from the upstream gradients g and e:
+// -(g + e (ln p + H)) / T = c0 + c1 log2 p.
+__global__ void __launch_bounds__(256)
+lmhead_logprob_coef_kernel(const int64_t* __restrict__ tokens, const f32x2_t* __restrict__ stats,
+                           const float* __restrict__ g_logprobs, const float* __restrict__ g_entropy,
+                           f32x4_t* __restrict__ coefs, int n_rows, int vocab, int64_t ignore_index, float inv_t) {
+  const int row = blockIdx.x * 256 + threadIdx.x;
+  if (row >= n_rows) return;
+  const f32x2_t st = stats[row];
+  float g = tokens && g_logprobs ? g_logprobs[row] : 0.0f, e = g_entropy ? g_entropy[row] : 0.0f;
+  if (tokens) {
+    const int64_t t = tokens[row];
+    if (t == ignore_index) g = e = 0.0f;
+    else if (t < 0 || t >= vocab) g = NAN;
+  }
+  g *= inv_t;
+  e *= inv_t;
+  coefs[row] = f32x4_t{st[0], g == 0.0f && e == 0.0f ? 0.0f : -fmaf(e, st[1], g), -e * kLn2, g};
+}
+
+// The given tokens' entries, from their own dot products: what the tile kernel
+// wrote plus g / T, through the softcap's slope.
+template <typename T>
+__global__ void __launch_bounds__(256)
+lmhead_logprob_grad_token_kernel(const T* __restrict__ H, const T* __restrict__ W, const int64_t* __restrict__ tokens,
+                                 GradArgs ga, int n_rows, int vocab, int d, int64_t ldh, int64_t ldw) {
+  const int tok = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (tok >= n_rows) return;  // the whole wave
+  const int64_t tl = tokens[tok] - ga.v0;  // the token's column in this range (W starts at row v0)
+  if (tokens[tok] == ga.ignore_index || tl < 0 || tl >= vocab) return;
+  const float z = wave_dot(H + (int64_t)tok * ldh, W + tl * ldw, d);
+  if ((threadIdx.x & 63) != 0) return;
+  const f32x4_t co = ga.coefs[tok];
+  const float t = fmaf(capped(z, ga.cap), ga.c2, -co[0]);
+  float slope = 1.0f;
+  if (ga.cap > 0.0f) {
+    const float q = Cap(ga.cap).q(z), r = __builtin_amdgcn_rcpf(q + 1.0f);
+    slope = q < INFINITY ? 4.0f * q * r * r : 0.0f;
+  }
+  static_cast<T*>(ga.dz)[(int64_t)tok * ga.ld_dz + tl] =
+      from_f32<T>(fmaf(__builtin_amdgcn_exp2f(t), fmaf(co[2], t, co[1]), co[3]) * slope);
+}
+
 size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
 
 struct WsLayout {
@@ -807,16 +1003,16 @@ WsLayout ws_layout(int64_t n_rows, int64_t vocab) {
   return w;
 }
 
-template <typename T, bool kCap, bool kLs>
+template <typename T, bool kCap, bool kLs, bool kEnt = false>
 void launch_tiles_fwd(const T* hp, const T* wp, MSPair* part, int n_rows, int vocab, int d,
                       int64_t ldh, int64_t ldw, int n_vt, int n_tt, const GradArgs& ga, dim3 gd,
                       dim3 bd, hipStream_t s) {
   if (vocab >= kTV && n_rows >= kTT && vocab % 128 == 0)
-    lmhead_ce_tile_kernel<T, true, false, false, kCap, kLs><<<gd, bd, 0, s>>>(hp, wp, part, n_rows, vocab, d, ldh, ldw, n_vt, n_tt, ga);
+    lmhead_ce_tile_kernel<T, true, false, false, kCap, kLs, kEnt><<<gd, bd, 0, s>>>(hp, wp, part, n_rows, vocab, d, ldh, ldw, n_vt, n_tt, ga);
   else if (vocab >= kTV && n_rows >= kTT)
-    lmhead_ce_tile_kernel<T, true, true, false, kCap, kLs><<<gd, bd, 0, s>>>(hp, wp, part, n_rows, vocab, d, ldh, ldw, n_vt, n_tt, ga);
+    lmhead_ce_tile_kernel<T, true, true, false, kCap, kLs, kEnt><<<gd, bd, 0, s>>>(hp, wp, part, n_rows, vocab, d, ldh, ldw, n_vt, n_tt, ga);
   else
-    lmhead_ce_tile_kernel<T, false, true, false, kCap, kLs><<<gd, bd, 0, s>>>(hp, wp, part, n_rows, vocab, d, ldh, ldw, n_vt, n_tt, ga);
+    lmhead_ce_tile_kernel<T, false, true, false, kCap, kLs, kEnt><<<gd, bd, 0, s>>>(hp, wp, part, n_rows, vocab, d, ldh, ldw, n_vt, n_tt, ga);
 }
 
 template <typename T>
@@ -854,15 +1050,15 @@ void launch_lmhead(const void* h, const void* w, const int64_t* targets, float* 
                                                       ignore_index);
 }
 
-template <typename T, bool kCap>
+template <typename T, bool kCap, bool kEnt = false>
 void launch_tiles_bwd(const T* hp, const T* wp, int n_rows, int vocab, int d, int64_t ldh,
                       int64_t ldw, int n_vt, int n_tt, const GradArgs& ga, dim3 gd, dim3 bd, hipStream_t s) {
   if (vocab >= kTV && n_rows >= kTT && vocab % 128 == 0)
-    lmhead_ce_tile_kernel<T, true, false, true, kCap><<<gd, bd, 0, s>>>(hp, wp, nullptr, n_rows, vocab, d, ldh, ldw, n_vt, n_tt, ga);
+    lmhead_ce_tile_kernel<T, true, false, true, kCap, false, kEnt><<<gd, bd, 0, s>>>(hp, wp, nullptr, n_rows, vocab, d, ldh, ldw, n_vt, n_tt, ga);
   else if (vocab >= kTV && n_rows >= kTT)
-    lmhead_ce_tile_kernel<T, true, true, true, kCap><<<gd, bd, 0, s>>>(hp, wp, nullptr, n_rows, vocab, d, ldh, ldw, n_vt, n_tt, ga);
+    lmhead_ce_tile_kernel<T, true, true, true, kCap, false, kEnt><<<gd, bd, 0, s>>>(hp, wp, nullptr, n_rows, vocab, d, ldh, ldw, n_vt, n_tt, ga);
   else
-    lmhead_ce_tile_kernel<T, false, true, true, kCap><<<gd, bd, 0, s>>>(hp, wp, nullptr, n_rows, vocab, d, ldh, ldw, n_vt, n_tt, ga);
+    lmhead_ce_tile_kernel<T, false, true, true, kCap, false, kEnt><<<gd, bd, 0, s>>>(hp, wp, nullptr, n_rows, vocab, d, ldh, ldw, n_vt, n_tt, ga);
 }
 
 template <typename T>
@@ -881,8 +1077,160 @@ void launch_lmhead_bwd(const void* h, const void* w, const GradArgs& ga, int n_r
   lmhead_ce_grad_target_kernel<T><<<dim3((n_rows + 3) / 4), dim3(256), 0, s>>>(hp, wp, ga, n_rows, vocab, d, ldh, ldw);
 }
 
+struct LogprobWs {
+  size_t part, usum, total;
+};
+
+LogprobWs logprob_ws(int64_t n_rows, int64_t vocab) {
+  const size_t n = (size_t)2 * ((vocab + kTV - 1) / kTV) * n_rows;
+  LogprobWs w;
+  w.part = 0;
+  w.usum = align256(n * sizeof(MSPair));
+  w.total = w.usum + align256(n * sizeof(float));
+  return w;
+}
+
+template <typename T>
+void launch_logprobs(const void* h, const void* w, const int64_t* tokens, float* logprobs, float* entropy, float* stats,
+                     void* ws, int n_rows, int vocab, int d, int64_t ldh, int64_t ldw, int64_t ignore_index,
+                     float temperature, float cap, hipStream_t s) {
+  const int n_vt = (vocab + kTV - 1) / kTV, n_tt = (n_rows + kTT - 1) / kTT;
+  const LogprobWs L = logprob_ws(n_rows, vocab);
+  char* base = static_cast<char*>(ws);
+  MSPair* part = reinterpret_cast<MSPair*>(base + L.part);
+  const T* hp = static_cast<const T*>(h);
+  const T* wp = static_cast<const T*>(w);
+  GradArgs ga{};
+  ga.cap = cap;
+  ga.c2 = (float)(1.4426950408889634 / (double)temperature);
+  ga.zsum = reinterpret_cast<float*>(base + L.usum);
+  const dim3 gd(min(n_vt * n_tt, cu_count())), bd(kLThreads);
+  if (cap > 0.0f)
+    launch_tiles_fwd<T, true, false, true>(hp, wp, part, n_rows, vocab, d, ldh, ldw, n_vt, n_tt, ga, gd, bd, s);
+  else
+    launch_tiles_fwd<T, false, false, true>(hp, wp, part, n_rows, vocab, d, ldh, ldw, n_vt, n_tt, ga, gd, bd, s);
+  lmhead_logprob_rows_kernel<T><<<dim3((n_rows + kRowsPerBlock - 1) / kRowsPerBlock), dim3(kRowsPerBlock * kRowGroups), 0, s>>>(
+      hp, wp, part, ga.zsum, tokens, logprobs, entropy, reinterpret_cast<f32x2_t*>(stats), n_rows, vocab, d, ldh, ldw,
+      2 * n_vt, ignore_index, cap, ga.c2, 1.0f / temperature);
+}
+
+template <typename T>
+void launch_logprobs_bwd(const void* h, const void* w, const int64_t* tokens, const GradArgs& ga, int n_rows, int vocab,
+                         int d, int64_t ldh, int64_t ldw, hipStream_t s) {
+  const int n_vt = (vocab + kTV - 1) / kTV, n_tt = (n_rows + kTT - 1) / kTT;
+  const T* hp = static_cast<const T*>(h);
+  const T* wp = static_cast<const T*>(w);
+  const dim3 gd(min(n_vt * n_tt, cu_count())), bd(kLThreads);
+  if (ga.cap > 0.0f)
+    launch_tiles_bwd<T, true, true>(hp, wp, n_rows, vocab, d, ldh, ldw, n_vt, n_tt, ga, gd, bd, s);
+  else
+    launch_tiles_bwd<T, false, true>(hp, wp, n_rows, vocab, d, ldh, ldw, n_vt, n_tt, ga, gd, bd, s);
+  if (tokens)
+    lmhead_logprob_grad_token_kernel<T><<<dim3((n_rows + 3) / 4), dim3(256), 0, s>>>(hp, wp, tokens, ga, n_rows, vocab, d, ldh, ldw);
+}
+
+// What the log-probability entry points ask of their operands.
+int check_logprobs(const char* name, const void* hidden, const void* weight, int64_t n_rows, int64_t vocab, int64_t v_count,
+                   int64_t d, int64_t ld_h, int64_t ld_w, float temperature, float softcap, int dtype) {
+  if (!(temperature >= 1e-18f && temperature <= 1e18f))
+    return ak_set_error(AK_ERR_INVALID_ARG, "%s: temperature must be between 1e-18 and 1e18", name);
+  if (!(softcap >= 0.0f) || softcap == INFINITY)
+    return ak_set_error(AK_ERR_INVALID_ARG, "%s: softcap must be finite and >= 0", name);
+  if (dtype != AK_DTYPE_BF16 && dtype != AK_DTYPE_F16)
+    return ak_set_error(AK_ERR_UNSUPPORTED, "%s: dtype must be bf16 or fp16", name);
+  if (n_rows <= 0 || vocab <= 0 || d <= 0 || n_rows > (1 << 30) || vocab > (1 << 30) || d > (1 << 20))
+    return ak_set_error(AK_ERR_INVALID_ARG, "%s: bad shape n_rows=%lld vocab=%lld d=%lld", name, (long long)n_rows,
+                        (long long)vocab, (long long)d);
+  if (d % kKB) return ak_set_error(AK_ERR_UNSUPPORTED, "%s: d=%lld must be a multiple of %d", name, (long long)d, kKB);
+  if (ld_h < d || ld_w < d || ld_h % 8 || ld_w % 8 || ld_h >= (1 << 23) || ld_w >= (1 << 23))
+    return ak_set_error(AK_ERR_INVALID_ARG, "%s: row pitches must be >= d, multiples of 8 and < 2^23 elements", name);
+  if (!hidden || !weight) return ak_set_error(AK_ERR_INVALID_ARG, "%s: null pointer", name);
+  if (!aligned16(hidden) || !aligned16(weight))
+    return ak_set_error(AK_ERR_INVALID_ARG, "%s: hidden and weight must be 16-byte aligned", name);
+  if (((v_count + kTV - 1) / kTV) * ((n_rows + kTT - 1) / kTT) > 0x7FFFFFFF)
+    return ak_set_error(AK_ERR_INVALID_ARG, "%s: too many tiles", name);
+  return AK_OK;
+}
+
 }  // namespace
 }  // namespace ak
+
+extern "C" size_t ak_lmhead_logprobs_workspace_bytes(int64_t n_rows, int64_t vocab) {
+  if (n_rows <= 0 || vocab <= 0) return 0;
+  return ak::logprob_ws(n_rows, vocab).total;
+}
+
+extern "C" int ak_lmhead_logprobs_fwd(const void* hidden, const void* weight, const int64_t* tokens, float* logprobs,
+                                      float* entropy, float* stats, void* workspace, size_t workspace_bytes,
+                                      int64_t n_rows, int64_t vocab, int64_t d, int64_t ld_h, int64_t ld_w,
+                                      float temperature, float softcap, int64_t ignore_index, int dtype, void* stream) {
+  const char* name = "ak_lmhead_logprobs_fwd";
+  const int rc = ak::check_logprobs(name, hidden, weight, n_rows, vocab, vocab, d, ld_h, ld_w, temperature, softcap, dtype);
+  if (rc) return rc;
+  if (tokens && !logprobs) return ak_set_error(AK_ERR_INVALID_ARG, "%s: null pointer", name);
+  if (reinterpret_cast<uintptr_t>(stats) & 7u) return ak_set_error(AK_ERR_INVALID_ARG, "%s: stats must be 8-byte aligned", name);
+  const size_t need = ak::logprob_ws(n_rows, vocab).total;
+  if (workspace_bytes < need || !workspace || !ak::aligned16(workspace))
+    return ak_set_error(AK_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed (16-byte aligned)", name, workspace_bytes, need);
+  hipStream_t s = ak_stream(stream);
+  if (dtype == AK_DTYPE_BF16)
+    ak::launch_logprobs<ak::bf16>(hidden, weight, tokens, logprobs, entropy, stats, workspace, (int)n_rows, (int)vocab, (int)d, ld_h, ld_w, ignore_index, temperature, softcap, s);
+  else
+    ak::launch_logprobs<ak::f16>(hidden, weight, tokens, logprobs, entropy, stats, workspace, (int)n_rows, (int)vocab, (int)d, ld_h, ld_w, ignore_index, temperature, softcap, s);
+  return ak_check_launch(name);
+}
+
+extern "C" int ak_lmhead_logprobs_coefs(const int64_t* tokens, const float* stats, const float* grad_logprobs,
+                                        const float* grad_entropy, float* coefs, int64_t n_rows, int64_t vocab,
+                                        float temperature, int64_t ignore_index, void* stream) {
+  const char* name = "ak_lmhead_logprobs_coefs";
+  if (n_rows < 0 || n_rows > (1 << 30) || vocab <= 0 || vocab > (1 << 30))
+    return ak_set_error(AK_ERR_INVALID_ARG, "%s: bad shape n_rows=%lld vocab=%lld", name, (long long)n_rows, (long long)vocab);
+  if (!(temperature >= 1e-18f && temperature <= 1e18f))
+    return ak_set_error(AK_ERR_INVALID_ARG, "%s: temperature must be between 1e-18 and 1e18", name);
+  if (n_rows == 0) return AK_OK;
+  if (!stats || !coefs) return ak_set_error(AK_ERR_INVALID_ARG, "%s: null pointer", name);
+  if ((reinterpret_cast<uintptr_t>(stats) & 7u) || !ak::aligned16(coefs))
+    return ak_set_error(AK_ERR_INVALID_ARG, "%s: stats must be 8-byte and coefs 16-byte aligned", name);
+  ak::lmhead_logprob_coef_kernel<<<dim3((unsigned)((n_rows + 255) / 256)), dim3(256), 0, ak_stream(stream)>>>(
+      tokens, reinterpret_cast<const ak::f32x2_t*>(stats), grad_logprobs, grad_entropy, reinterpret_cast<ak::f32x4_t*>(coefs),
+      (int)n_rows, (int)vocab, ignore_index, 1.0f / temperature);
+  return ak_check_launch(name);
+}
+
+extern "C" int ak_lmhead_logprobs_bwd_range(const void* hidden, const void* weight, const int64_t* tokens,
+                                            const float* coefs, void* grad_logits, int64_t ld_gl, int64_t n_rows,
+                                            int64_t vocab, int64_t v_begin, int64_t v_count, int64_t d, int64_t ld_h,
+                                            int64_t ld_w, float temperature, float softcap, int64_t ignore_index,
+                                            int dtype, void* stream) {
+  const char* name = "ak_lmhead_logprobs_bwd_range";
+  if (v_begin < 0 || v_count <= 0 || v_begin > vocab - v_count)
+    return ak_set_error(AK_ERR_INVALID_ARG, "%s: vocab range [%lld, %lld + %lld) outside [0, %lld)", name,
+                        (long long)v_begin, (long long)v_begin, (long long)v_count, (long long)vocab);
+  const int rc = ak::check_logprobs(name, hidden, weight, n_rows, vocab, v_count, d, ld_h, ld_w, temperature, softcap, dtype);
+  if (rc) return rc;
+  if (!coefs || !grad_logits) return ak_set_error(AK_ERR_INVALID_ARG, "%s: null pointer", name);
+  if (!ak::aligned16(coefs) || (reinterpret_cast<uintptr_t>(grad_logits) & 1u))
+    return ak_set_error(AK_ERR_INVALID_ARG, "%s: coefs must be 16-byte aligned, grad_logits element-aligned", name);
+  if (ld_gl < v_count) return ak_set_error(AK_ERR_INVALID_ARG, "%s: grad_logits pitch must be >= the range's width", name);
+  ak::GradArgs ga{};
+  ga.dz = grad_logits;
+  ga.ld_dz = ld_gl;
+  ga.ignore_index = ignore_index;
+  ga.cap = softcap;
+  ga.v0 = v_begin;
+  ga.vocab_total = vocab;
+  ga.c2 = (float)(1.4426950408889634 / (double)temperature);
+  ga.coefs = reinterpret_cast<const ak::f32x4_t*>(coefs);
+  hipStream_t s = ak_stream(stream);
+  // the range's weight rows start at v_begin (16-byte aligned: ld_w is a multiple of 8)
+  const void* wr = static_cast<const char*>(weight) + (size_t)v_begin * (size_t)ld_w * 2;
+  if (dtype == AK_DTYPE_BF16)
+    ak::launch_logprobs_bwd<ak::bf16>(hidden, wr, tokens, ga, (int)n_rows, (int)v_count, (int)d, ld_h, ld_w, s);
+  else
+    ak::launch_logprobs_bwd<ak::f16>(hidden, wr, tokens, ga, (int)n_rows, (int)v_count, (int)d, ld_h, ld_w, s);
+  return ak_check_launch(name);
+}
 
 extern "C" size_t ak_lmhead_ce_workspace_bytes(int64_t n_rows, int64_t vocab) {
   if (n_rows <= 0 || vocab <= 0) return 0;
@@ -987,7 +1335,7 @@ extern "C" int ak_lmhead_ce_bwd_range(const void* hidden, const void* weight,
   const int64_t n_tiles = ((v_count + ak::kTV - 1) / ak::kTV) * ((n_rows + ak::kTT - 1) / ak::kTT);
   if (n_tiles > 0x7FFFFFFF) return ak_set_error(AK_ERR_INVALID_ARG, "%s: too many tiles", name);
   ak::GradArgs ga{lse, targets, grad_loss, denom, grad_logits, ld_gl, ignore_index, softcap,
-                  label_smoothing, nullptr, v_begin, vocab};
+                  label_smoothing, nullptr, v_begin, vocab, 0.0f, nullptr};
   hipStream_t s = ak_stream(stream);
   // the range's weight rows start at v_begin (16-byte aligned: ld_w is a multiple of 8)
   const void* wr = static_cast<const char*>(weight) + (size_t)v_begin * (size_t)ld_w * 2;

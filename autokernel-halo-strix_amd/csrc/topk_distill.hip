@@ -315,6 +315,7 @@ extern "C" int ak_topk_distill_fwd(const void* logits, const void* teacher_logit
   if (rc) return rc;
   if (!loss != !scale || (rows > 0 && (!losses || !stats))) return ak_set_error(AK_ERR_INVALID_ARG, "%s: null pointer", name);
   if (stats && !ak::aligned16(stats)) return ak_set_error(AK_ERR_INVALID_ARG, "%s: stats must be 16-byte aligned", name);
+  if (rows == 0 && !loss) return AK_OK;
   hipStream_t s = ak_stream(stream);
   if (rows > 0) {
     const ak::ScorePlan pl = ak::score_plan(rows, vocab, 16 / ak_dtype_size(dtype), 0);

@@ -83,6 +83,10 @@ _SIGNATURES = {
     "ak_lmhead_ce_fwd_denom": [_c_void_p] * 9 + [ctypes.c_size_t] + [_i64] * 6 + [_f32, _f32, _int, _c_void_p],
     "ak_lmhead_ce_bwd": [_c_void_p] * 7 + [_i64] * 7 + [_f32, _f32, _int, _c_void_p],
     "ak_lmhead_ce_bwd_range": [_c_void_p] * 7 + [_i64] * 9 + [_f32, _f32, _int, _c_void_p],
+    "ak_lmhead_logprobs_workspace_bytes": [_i64, _i64],
+    "ak_lmhead_logprobs_fwd": [_c_void_p] * 7 + [ctypes.c_size_t] + [_i64] * 5 + [_f32, _f32, _i64, _int, _c_void_p],
+    "ak_lmhead_logprobs_coefs": [_c_void_p] * 5 + [_i64, _i64, _f32, _i64, _c_void_p],
+    "ak_lmhead_logprobs_bwd_range": [_c_void_p] * 5 + [_i64] * 8 + [_f32, _f32, _i64, _int, _c_void_p],
     "ak_lmhead_grad_workspace_bytes": [_i64, _i64, _i64],
     "ak_lmhead_grad_hidden": [_c_void_p, _i64, _c_void_p, _i64, _c_void_p, _i64, _i64, _i64, _i64,
                               _int, _c_void_p, ctypes.c_size_t, _int, _c_void_p],
@@ -105,6 +109,7 @@ _RESTYPES = {
     "ak_token_logprobs_workspace_bytes": ctypes.c_size_t,
     "ak_topk_distill_workspace_bytes": ctypes.c_size_t,
     "ak_lmhead_ce_workspace_bytes": ctypes.c_size_t,
+    "ak_lmhead_logprobs_workspace_bytes": ctypes.c_size_t,
     "ak_lmhead_grad_workspace_bytes": ctypes.c_size_t,
     "ak_rmsnorm_bwd_workspace_bytes": ctypes.c_size_t,
     "ak_diag_scan_bwd_workspace_bytes": ctypes.c_size_t,
@@ -623,6 +628,55 @@ def lmhead_ce_bwd_range(hidden: torch.Tensor, weight: torch.Tensor, targets: tor
             _rows_view(weight, "weight"), int(ignore_index), float(softcap),
             float(label_smoothing), dtype_code(hidden.dtype), _stream(hidden))
     _check(rc, "ak_lmhead_ce_bwd_range")
+
+
+def lmhead_logprobs(hidden: torch.Tensor, weight: torch.Tensor, tokens: Optional[torch.Tensor],
+                    logprobs: Optional[torch.Tensor], entropy: torch.Tensor, stats: Optional[torch.Tensor],
+                    temperature: float, softcap: float, ignore_index: int) -> None:
+    """Log probabilities of ``tokens`` (int64) and entropies of ``softmax(hidden
+    @ weight^T)`` (fp32 ``[n_rows]``); ``stats`` fp32 ``[n_rows, 2]`` is for the
+    backward."""
+    require_device(hidden, weight, tokens, logprobs, entropy, stats)
+    n_rows, d = hidden.shape
+    vocab = weight.shape[0]
+    lib = load()
+    nbytes = int(lib.ak_lmhead_logprobs_workspace_bytes(n_rows, vocab))
+    with _on_device(hidden):
+        ws = _workspace(nbytes, hidden.device)
+        rc = lib.ak_lmhead_logprobs_fwd(
+            _ptr(hidden), _ptr(weight), _ptr(tokens), _ptr(logprobs), _ptr(entropy), _ptr(stats), _ptr(ws), nbytes,
+            n_rows, vocab, d, _rows_view(hidden, "hidden"), _rows_view(weight, "weight"), float(temperature),
+            float(softcap), int(ignore_index), dtype_code(hidden.dtype), _stream(hidden))
+    _check(rc, "ak_lmhead_logprobs_fwd")
+
+
+def lmhead_logprobs_coefs(tokens: Optional[torch.Tensor], stats: torch.Tensor, grad_logprobs: Optional[torch.Tensor],
+                          grad_entropy: Optional[torch.Tensor], coefs: torch.Tensor, vocab: int, temperature: float,
+                          ignore_index: int) -> None:
+    """The row coefficients ``coefs`` (fp32 ``[n_rows, 4]``) that
+    :func:`lmhead_logprobs_bwd_range` takes, from the upstream gradients."""
+    require_device(tokens, stats, grad_logprobs, grad_entropy, coefs)
+    with _on_device(stats):
+        rc = load().ak_lmhead_logprobs_coefs(_ptr(tokens), _ptr(stats), _ptr(grad_logprobs), _ptr(grad_entropy),
+                                             _ptr(coefs), stats.shape[0], int(vocab), float(temperature),
+                                             int(ignore_index), _stream(stats))
+    _check(rc, "ak_lmhead_logprobs_coefs")
+
+
+def lmhead_logprobs_bwd_range(hidden: torch.Tensor, weight: torch.Tensor, tokens: Optional[torch.Tensor],
+                              coefs: torch.Tensor, grad_logits: torch.Tensor, v_begin: int, temperature: float,
+                              softcap: float, ignore_index: int) -> None:
+    """The logits' gradient for the vocab columns ``[v_begin, v_begin +
+    grad_logits.shape[1])`` of the full ``weight``'s vocabulary."""
+    require_device(hidden, weight, tokens, coefs, grad_logits)
+    n_rows, d = hidden.shape
+    with _on_device(hidden):
+        rc = load().ak_lmhead_logprobs_bwd_range(
+            _ptr(hidden), _ptr(weight), _ptr(tokens), _ptr(coefs), _ptr(grad_logits),
+            _rows_view(grad_logits, "grad_logits"), n_rows, weight.shape[0], int(v_begin), grad_logits.shape[1], d,
+            _rows_view(hidden, "hidden"), _rows_view(weight, "weight"), float(temperature), float(softcap),
+            int(ignore_index), dtype_code(hidden.dtype), _stream(hidden))
+    _check(rc, "ak_lmhead_logprobs_bwd_range")
 
 
 # out_mode of the lm-head gradient GEMMs

@@ -185,32 +185,14 @@ def _vocab_ranges(n: int, vocab: int, elem: int, cus: int):
     return [(cuts[i], cuts[i + 1]) for i in range(count)]
 
 
-def lmhead_ce_backward(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor,
-                       lse: torch.Tensor, denom: torch.Tensor, grad_loss: torch.Tensor,
-                       ignore_index: int = -100, need_hidden: bool = True,
-                       need_weight: bool = True, softcap: float = 0.0,
-                       label_smoothing: float = 0.0):
-    """Fused backward of :func:`lmhead_ce_forward`'s mean loss.
-
-    ``lse`` is the forward's logsumexp, ``denom`` the number of counted rows
-    (a 0-d or 1-element fp32 tensor, clamped to >= 1) and ``grad_loss`` the
-    upstream gradient of the loss, ``softcap`` and ``label_smoothing`` the
-    forward's.
-    Returns ``(grad_hidden, grad_weight)`` in the input dtype (``None`` where
-    not requested).
-    """
-    _lib.require_device(hidden, weight, targets, lse, denom, grad_loss)
-    d_in = hidden.shape[1]
-    hidden, weight = _kernel_operands(hidden, weight)
-    targets = _row_targets(targets, hidden.shape[0])
+def gradients_by_ranges(hidden: torch.Tensor, weight: torch.Tensor, write_range, d_in: int, need_hidden: bool,
+                        need_weight: bool):
+    """``(grad_hidden, grad_weight)`` of ``_kernel_operands``, cut back to
+    ``d_in`` columns: for each vocab range ``write_range(g, v0)`` writes the
+    logits' gradient for columns from ``v0`` on into ``g [n, width]``, and the two
+    gradient GEMMs read it (``None`` where not requested)."""
     n, d = hidden.shape
     vocab = weight.shape[0]
-    if n == 0:
-        return (torch.empty((0, d_in), dtype=hidden.dtype, device=hidden.device) if need_hidden else None,
-                torch.zeros((vocab, d_in), dtype=weight.dtype, device=weight.device) if need_weight else None)
-    g1 = grad_loss.reshape(1).to(torch.float32).contiguous()
-    den1 = denom.reshape(1).to(torch.float32).contiguous()
-    lse = lse.contiguous()
     # the CU count only shapes the plan (a CPU tensor reaches here only from
     # the tests' fake backend: MI355X's 256)
     cus = (torch.cuda.get_device_properties(hidden.device).multi_processor_count
@@ -236,8 +218,7 @@ def lmhead_ce_backward(hidden: torch.Tensor, weight: torch.Tensor, targets: torc
         grad_hidden = None
     for v0, v1 in ranges:
         g = gp[:, :v1 - v0]  # lmhead_grad_hidden zeroes its K padding
-        _lib.lmhead_ce_bwd_range(hidden, weight, targets, lse, g1, den1, g, v0, ignore_index,
-                                 softcap, label_smoothing)
+        write_range(g, v0)
         if need_weight:
             _lib.lmhead_grad_weight(g, hidden, grad_weight[v0:v1], _lib.GEMM_OUT_DTYPE, ws)
         if need_hidden:
@@ -249,6 +230,39 @@ def lmhead_ce_backward(hidden: torch.Tensor, weight: torch.Tensor, targets: torc
         grad_hidden = grad_hidden[:, :d_in].contiguous() if need_hidden else None
         grad_weight = grad_weight[:, :d_in].contiguous() if need_weight else None
     return grad_hidden, grad_weight
+
+
+def lmhead_ce_backward(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor,
+                       lse: torch.Tensor, denom: torch.Tensor, grad_loss: torch.Tensor,
+                       ignore_index: int = -100, need_hidden: bool = True,
+                       need_weight: bool = True, softcap: float = 0.0,
+                       label_smoothing: float = 0.0):
+    """Fused backward of :func:`lmhead_ce_forward`'s mean loss.
+
+    ``lse`` is the forward's logsumexp, ``denom`` the number of counted rows
+    (a 0-d or 1-element fp32 tensor, clamped to >= 1) and ``grad_loss`` the
+    upstream gradient of the loss, ``softcap`` and ``label_smoothing`` the
+    forward's.
+    Returns ``(grad_hidden, grad_weight)`` in the input dtype (``None`` where
+    not requested).
+    """
+    _lib.require_device(hidden, weight, targets, lse, denom, grad_loss)
+    d_in = hidden.shape[1]
+    hidden, weight = _kernel_operands(hidden, weight)
+    targets = _row_targets(targets, hidden.shape[0])
+    n, vocab = hidden.shape[0], weight.shape[0]
+    if n == 0:
+        return (torch.empty((0, d_in), dtype=hidden.dtype, device=hidden.device) if need_hidden else None,
+                torch.zeros((vocab, d_in), dtype=weight.dtype, device=weight.device) if need_weight else None)
+    g1 = grad_loss.reshape(1).to(torch.float32).contiguous()
+    den1 = denom.reshape(1).to(torch.float32).contiguous()
+    lse = lse.contiguous()
+
+    def write_range(g, v0):
+        _lib.lmhead_ce_bwd_range(hidden, weight, targets, lse, g1, den1, g, v0, ignore_index, softcap,
+                                 label_smoothing)
+
+    return gradients_by_ranges(hidden, weight, write_range, d_in, need_hidden, need_weight)
 
 
 def _chunked_forward(hidden, weight, targets, chunk_size, softcap, ignore_index, label_smoothing):

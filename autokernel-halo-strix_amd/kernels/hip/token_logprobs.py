@@ -34,7 +34,6 @@ import os
 from typing import NamedTuple, Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from kernels.hip import _lib
 
@@ -69,6 +68,13 @@ def whole_numbers(t: torch.Tensor, name: str, shape) -> torch.Tensor:
     if tuple(t.shape) != tuple(shape):
         raise ValueError(f"{name} shape {tuple(t.shape)} != {tuple(shape)}")
     return t.to(torch.int64).contiguous()
+
+
+def differentiable_once(name: str) -> None:
+    """Refuse a backward that is itself to be differentiated (its kernels' results
+    carry no graph: what should have a gradient would pass as a constant)."""
+    if torch.is_grad_enabled():
+        raise RuntimeError(f"{name} is differentiable once: its backward takes no create_graph=True")
 
 
 def row_gradient(g: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
@@ -113,8 +119,8 @@ class _TokenLogprobs(torch.autograd.Function):
         return tuple(out)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g_logprobs, g_entropy, *unused):
+        differentiable_once(KERNEL_TYPE)
         rows2d, tokens, stats = ctx.saved_tensors
         grad = torch.empty(ctx.shape, dtype=rows2d.dtype, device=rows2d.device)
         if grad.numel():

@@ -32,10 +32,10 @@ No counterpart in the reference.
 import os
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from kernels.hip import _lib
-from kernels.hip.token_logprobs import check_scale, check_vocab, row_gradient, whole_numbers
+from kernels.hip.token_logprobs import (check_scale, check_vocab, differentiable_once, row_gradient,
+                                        whole_numbers)
 
 KERNEL_TYPE = "topk_distillation"
 BACKEND = "hip"
@@ -66,8 +66,8 @@ class _TopkDistillation(torch.autograd.Function):
         return loss
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g_loss):
+        differentiable_once(KERNEL_TYPE)
         rows2d, teacher, ids, stats, scale = ctx.saved_tensors
         grad = torch.empty(ctx.shape, dtype=rows2d.dtype, device=rows2d.device)
         if grad.numel():

@@ -396,6 +396,41 @@ int ak_lmhead_ce_bwd_range(const void* hidden, const void* weight, const int64_t
                            float label_smoothing, int dtype, void* stream);
 
 /*
+ * Log probabilities of given tokens and entropies straight from hidden
+ * [n_rows, d] and weight [vocab, d]: as ak_token_logprobs_fwd over the logits
+ * hidden @ weight^T (fp32 accumulation), which are never written to memory.
+ * tokens (and then logprobs), entropy and stats may be NULL; a row whose token
+ * is ignore_index has logprob and entropy 0, a token outside [0, vocab) that is
+ * not ignore_index logprob NaN. stats [n_rows, 2] fp32, 8-byte aligned, is what
+ * ak_lmhead_logprobs_coefs takes. Shape rules as for ak_lmhead_ce_fwd. No
+ * counterpart in the reference, whose chunked loss
+ * (kernels/hip/chunked_linear_cross_entropy.py:55-148) returns the mean only.
+ */
+size_t ak_lmhead_logprobs_workspace_bytes(int64_t n_rows, int64_t vocab);
+int ak_lmhead_logprobs_fwd(const void* hidden, const void* weight, const int64_t* tokens,
+                           float* logprobs, float* entropy, float* stats, void* workspace,
+                           size_t workspace_bytes, int64_t n_rows, int64_t vocab, int64_t d,
+                           int64_t ld_h, int64_t ld_w, float temperature, float softcap,
+                           int64_t ignore_index, int dtype, void* stream);
+
+/*
+ * Its backward, first half: the row coefficients (coefs [n_rows, 4] fp32,
+ * 16-byte aligned) from the upstream gradients (fp32 [n_rows]; NULL: none), and
+ * then the gradient of the logits over the vocab columns [v_begin, v_begin +
+ * v_count), as ak_token_logprobs_bwd gives it, in the element type (grad_logits
+ * and ranges as for ak_lmhead_ce_bwd_range). The two products after it are
+ * ak_lmhead_grad_hidden and ak_lmhead_grad_weight.
+ */
+int ak_lmhead_logprobs_coefs(const int64_t* tokens, const float* stats, const float* grad_logprobs,
+                             const float* grad_entropy, float* coefs, int64_t n_rows, int64_t vocab,
+                             float temperature, int64_t ignore_index, void* stream);
+int ak_lmhead_logprobs_bwd_range(const void* hidden, const void* weight, const int64_t* tokens,
+                                 const float* coefs, void* grad_logits, int64_t ld_gl, int64_t n_rows,
+                                 int64_t vocab, int64_t v_begin, int64_t v_count, int64_t d,
+                                 int64_t ld_h, int64_t ld_w, float temperature, float softcap,
+                                 int64_t ignore_index, int dtype, void* stream);
+
+/*
  * Gradient GEMMs of the lm-head + CE backward, from the dlogits written by
  * ak_lmhead_ce_bwd / ak_lmhead_ce_bwd_range (hand-written MFMA kernels,
  * fp32 accumulation). They replace the two torch.mm calls of the

@@ -46,8 +46,29 @@ def scoring_backend(monkeypatch):
         assert g.numel() == (1 if scale is not None else x.shape[0])
         grad.copy_(scoring.distill_grad_rows(x, t, ids, up.expand(x.shape[0]), temperature, softcap, ignore)[0])
 
+    def lmhead(h, w, tok, lp, ent, stats, temperature, softcap, ignore):
+        assert h.shape[1] % 64 == 0 and h.is_contiguous() and w.is_contiguous()
+        logprobs(h.double() @ w.double().t(), tok, lp, ent, stats, None, None, temperature, softcap, ignore)
+
+    saved = {}
+
+    def coefs(tok, stats, gl, ge, out, vocab, temperature, ignore):
+        saved.update(gl=gl, ge=ge)
+
+    def lmhead_bwd(h, w, tok, co, grad, v0, temperature, softcap, ignore):
+        full = scoring.logprob_grad_rows(h.double() @ w.double().t(), tok, saved["gl"], saved["ge"], temperature,
+                                         softcap, ignore)[0]
+        grad.copy_(full[:, v0:v0 + grad.shape[1]])
+
+    def add(out, value, mode):
+        out.copy_(value + (out.double() if mode == 2 else 0))
+
     for name, fn in (("token_logprobs", logprobs), ("token_logprobs_bwd", logprobs_bwd), ("topk_distill", distill),
-                     ("topk_distill_bwd", distill_bwd), ("require_device", lambda *t: None)):
+                     ("topk_distill_bwd", distill_bwd), ("require_device", lambda *t: None),
+                     ("lmhead_logprobs", lmhead), ("lmhead_logprobs_coefs", coefs),
+                     ("lmhead_logprobs_bwd_range", lmhead_bwd), ("lmhead_grad_workspace_bytes", lambda n, v, d: 256),
+                     ("lmhead_grad_hidden", lambda g, w, out, mode, ws: add(out, g.double() @ w.double(), mode)),
+                     ("lmhead_grad_weight", lambda g, h, out, mode, ws: add(out, g.double().t() @ h.double(), mode))):
         monkeypatch.setattr(_lib, name, fn)
 
 
@@ -88,9 +109,8 @@ def test_gradients_of_one_output_and_broadcast_upstream(scoring_backend):
     r = tl.kernel_fn(x, tok)
     (g,) = torch.autograd.grad(r.entropy.sum(), x, retain_graph=True)  # an expanded upstream gradient
     assert torch.allclose(g.double(), scoring.logprob_grad_rows(x.detach(), tok, None, torch.ones(4))[0], atol=1e-6)
-    (g,) = torch.autograd.grad(r.logprobs.double().sum(), x, create_graph=True)
-    with pytest.raises(RuntimeError, match="once_differentiable"):
-        g.sum().backward()
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(r.logprobs.double().sum(), x, create_graph=True)
 
 
 def test_distillation_contract(scoring_backend):
@@ -102,8 +122,8 @@ def test_distillation_contract(scoring_backend):
     ids[1, 1, 2:] = -100
     loss = td.kernel_fn(x, t, ids, temperature=2.0)
     rows = td.kernel_fn(x, t, ids, temperature=2.0, reduction="none")
-    assert loss.shape == () and rows.shape == (2, 3) and float(rows[0, 0]) == 0
-    assert float(loss) == pytest.approx(float(rows.sum()) / 5, rel=1e-6)
+    assert loss.shape == () and rows.shape == (2, 3) and float(rows.detach()[0, 0]) == 0
+    assert float(loss.detach()) == pytest.approx(float(rows.detach().sum()) / 5, rel=1e-6)
     (gx,) = torch.autograd.grad(loss, x, torch.tensor(0.5))
     (gr,) = torch.autograd.grad(rows, x, torch.full((2, 3), 0.1))
     assert torch.allclose(gx, gr, atol=1e-7)
@@ -113,6 +133,65 @@ def test_distillation_contract(scoring_backend):
     assert td.kernel_fn(x[:0], t[:0], ids[:0], reduction="none").shape == (0, 3)
     # a teacher that requires a gradient is a constant
     assert not td.kernel_fn(x.detach(), t.clone().requires_grad_(), ids).requires_grad
+
+
+@pytest.mark.parametrize("dtype,budget", [(torch.bfloat16, 4 << 30), (torch.float16, 6 * 256 * 2), (torch.float32, 0)])
+def test_lmhead_contract(scoring_backend, monkeypatch, dtype, budget):
+    """Padded hidden sizes, vocab ranges, fp32 row chunks, gradients of either operand."""
+    from kernels.hip import chunked_linear_cross_entropy as clce
+    from kernels.hip.lmhead_logprobs import kernel_fn
+    monkeypatch.setattr(clce, "GRAD_LOGITS_BUDGET", budget)
+    g = torch.Generator().manual_seed(3)
+    h = torch.randn(2, 3, 70, generator=g).to(dtype).requires_grad_()
+    w = (0.2 * torch.randn(600, 70, generator=g)).to(dtype).requires_grad_()
+    tok = torch.tensor([[5, -100, 599], [0, 1, 300]])
+    kw = dict(temperature=0.8, softcap=10.0, chunk_size=4)
+    r = kernel_fn(h, w, tok, **kw)
+    x = (h.double().reshape(6, 70) @ w.double().t()).detach()
+    lp, ent = scoring.logprob_rows(x, tok.reshape(-1), 0.8, 10.0)
+    assert r.logprobs.shape == r.entropy.shape == (2, 3)
+    assert torch.allclose(r.logprobs.double().reshape(-1), lp, atol=1e-5)
+    assert torch.allclose(r.entropy.double().reshape(-1), ent, atol=1e-5)
+    gl, ge = torch.randn(2, 3, generator=g), torch.randn(2, 3, generator=g)
+    gh, gw = torch.autograd.grad((r.logprobs, r.entropy), (h, w), (gl, ge), retain_graph=True)
+    dz = scoring.logprob_grad_rows(x, tok.reshape(-1), gl.reshape(-1), ge.reshape(-1), 0.8, 10.0)[0]
+    tol = 3e-2 if dtype != torch.float32 else 1e-5
+    assert gh.dtype == gw.dtype == dtype and gh.shape == h.shape
+    for got, want in ((gh.reshape(6, 70), dz @ w.double()), (gw, dz.t() @ h.double().reshape(6, 70))):
+        assert float((got.double() - want).norm() / want.norm()) < tol
+    (gh2,) = torch.autograd.grad(r.entropy, h, ge, retain_graph=True)
+    assert gh2.shape == h.shape
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(r.logprobs.sum(), h, create_graph=True)
+    # no tokens, no rows, a weight of another type, one row
+    assert kernel_fn(h.detach(), w.detach()).logprobs is None
+    assert kernel_fn(h.detach()[0, 0], w.detach().float(), torch.tensor(7)).logprobs.shape == ()
+    e = kernel_fn(h[:0], w, tok[:0])
+    assert e.logprobs.shape == (0, 3)
+    assert torch.equal(torch.autograd.grad(e.entropy.sum(), w)[0], torch.zeros_like(w))
+
+
+def test_lmhead_refusals(scoring_backend):
+    from kernels.hip.lmhead_logprobs import kernel_fn
+    h, w, tok = torch.randn(3, 64), torch.randn(9, 64), torch.zeros(3, dtype=torch.int64)
+    with pytest.raises(ValueError, match="go with"):
+        kernel_fn(h, w[:, :63], tok)
+    with pytest.raises(ValueError, match="go with"):
+        kernel_fn(h, w[0], tok)
+    with pytest.raises(ValueError, match="empty"):
+        kernel_fn(h, w[:0], tok)
+    with pytest.raises(ValueError, match="tokens"):
+        kernel_fn(h, w, tok[:2])
+    with pytest.raises(TypeError, match="whole"):
+        kernel_fn(h, w, tok.float())
+    with pytest.raises(TypeError, match="dtype"):
+        kernel_fn(h.double(), w, tok)
+    with pytest.raises(ValueError, match="temperature"):
+        kernel_fn(h, w, tok, temperature=0)
+    with pytest.raises(ValueError, match="softcap"):
+        kernel_fn(h, w, tok, softcap=-1)
+    with pytest.raises(ValueError, match="chunk_size"):
+        kernel_fn(h, w, tok, chunk_size=0)
 
 
 def test_refusals(scoring_backend):
@@ -193,7 +272,9 @@ def test_library_refusals(lib):
     assert fwd(stats=8) == -1 and says(b"aligned")
     need = lib.ak_token_logprobs_workspace_bytes(2, 50257, 20, 0)
     assert need > 0 and lib.ak_token_logprobs_workspace_bytes(4096, 50257, 20, 2) == 0
-    assert fwd(rows=2, vocab=50257, ld=50257, nbytes=need - 1, ws=256) == -4 or need == 0
+    plain = lib.ak_token_logprobs_workspace_bytes(2, 50257, 0, 0)
+    assert fwd(rows=2, vocab=50257, ld=50257, nbytes=plain - 1, ws=256) == -4 and says(b"workspace")
+    assert fwd(rows=2, vocab=50257, ld=50257, nbytes=plain) == -4 and 0 < plain < need
     assert fwd(rows=2, vocab=50257, ld=50257, top=20, tv=16, ti=16, nbytes=need, ws=8) == -4 and says(b"workspace")
     assert fwd(rows=0, logits=None) == 0
 
@@ -231,3 +312,42 @@ def test_workspace_covers_every_shape(lib, ve):
             if rows >= 256:
                 assert (a > 0) == (segs_least > 1)
             assert a >= (rows * segs_least * 16 if segs_least > 1 else 0) and (b > 0 or segs_least == 1)
+
+
+def test_library_refusals_of_the_head(lib):
+    def says(word):
+        return word in lib.ak_last_error()
+
+    def fwd(h=16, w=16, tok=None, lp=None, stats=None, ws=None, nbytes=0, n=8, v=16, d=64, ldh=64, ldw=64, t=1.0,
+            cap=0.0, dtype=2):
+        return lib.ak_lmhead_logprobs_fwd(h, w, tok, lp, None, stats, ws, nbytes, n, v, d, ldh, ldw, t, cap, -100, dtype,
+                                          None)
+
+    assert fwd(dtype=0) == -2 and says(b"bf16")
+    assert fwd(d=100, ldh=104, ldw=104) == -2 and says(b"multiple")
+    assert fwd(n=0) == -1 and fwd(v=0) == -1 and fwd(n=1 << 31) == -1 and says(b"shape")
+    assert fwd(ldh=63) == -1 and fwd(ldw=65) == -1 and fwd(ldh=1 << 23) == -1 and says(b"pitch")
+    assert fwd(h=None) == -1 and fwd(tok=16) == -1 and says(b"null")
+    assert fwd(h=8) == -1 and fwd(w=24) == -1 and says(b"aligned")
+    assert fwd(stats=4) == -1 and says(b"aligned")
+    assert fwd(t=0.0) == -1 and fwd(t=math.nan) == -1 and says(b"temperature")
+    assert fwd(cap=-1.0) == -1 and fwd(cap=math.inf) == -1 and says(b"softcap")
+    need = lib.ak_lmhead_logprobs_workspace_bytes(8, 16)
+    assert need >= 2 * 8 * 12 and fwd(nbytes=need - 1, ws=16) == -4 and fwd(nbytes=need) == -4
+    assert fwd(nbytes=need, ws=24) == -4 and says(b"workspace")
+
+    def bwd(co=16, gl=16, ldg=16, v0=0, vn=16):
+        return lib.ak_lmhead_logprobs_bwd_range(16, 16, None, co, gl, ldg, 8, 16, v0, vn, 64, 64, 64, 1.0, 0.0, -100, 2,
+                                                None)
+
+    assert bwd(v0=-1) == -1 and bwd(v0=1) == -1 and bwd(vn=0) == -1 and says(b"range")
+    assert bwd(co=None) == -1 and bwd(gl=None) == -1 and says(b"null")
+    assert bwd(co=8) == -1 and bwd(gl=17) == -1 and says(b"aligned")
+    assert bwd(ldg=15) == -1 and says(b"pitch")
+
+    def coefs(stats=16, co=16, n=8, v=16, t=1.0):
+        return lib.ak_lmhead_logprobs_coefs(None, stats, None, None, co, n, v, t, -100, None)
+
+    assert coefs(stats=None) == -1 and coefs(co=None) == -1 and says(b"null")
+    assert coefs(stats=4) == -1 and coefs(co=8) == -1 and says(b"aligned")
+    assert coefs(n=-1) == -1 and coefs(v=0) == -1 and coefs(t=0.0) == -1 and coefs(n=0, stats=None) == 0
