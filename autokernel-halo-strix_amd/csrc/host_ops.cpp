@@ -35,7 +35,11 @@ using Maybe = std::optional<Tensor>;
   X(ak_diag_scan_bwd_workspace_bytes) X(ak_diag_scan_bwd) X(ak_selective_scan_fwd_ws) X(ak_selective_scan_fwd_workspace_bytes)                 \
   X(ak_selective_scan_bwd_workspace_bytes) X(ak_selective_scan_bwd)                                \
   X(ak_lmhead_ce_workspace_bytes) X(ak_lmhead_ce_fwd_denom) X(ak_lmhead_ce_bwd_range)                    \
-  X(ak_lmhead_grad_workspace_bytes) X(ak_lmhead_grad_hidden) X(ak_lmhead_grad_weight)
+  X(ak_lmhead_grad_workspace_bytes) X(ak_lmhead_grad_hidden) X(ak_lmhead_grad_weight)                          \
+  X(ak_token_logprobs_workspace_bytes) X(ak_token_logprobs_fwd) X(ak_token_logprobs_bwd)                       \
+  X(ak_topk_distill_workspace_bytes) X(ak_topk_distill_fwd) X(ak_topk_distill_bwd)                             \
+  X(ak_lmhead_logprobs_workspace_bytes) X(ak_lmhead_logprobs_fwd) X(ak_lmhead_logprobs_coefs)                  \
+  X(ak_lmhead_logprobs_bwd_range)
 
 #define AK_FIELD(n) decltype(&::n) n = nullptr;
 struct Api { AK_ENTRIES(AK_FIELD) } api;
@@ -538,6 +542,37 @@ bool at16(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 
 bool dense16(const Tensor& t) { return t.dim() == 2 && t.is_contiguous() && at16(t); }
 Tensor realigned(const Tensor& t) { return at16(t) ? t : t.clone(); }
 
+// Room for the logits' gradient [n, v]: the pitch covers whole 64-column K
+// blocks and stays off powers of two, whose rows would all start in the same
+// memory channels.
+Tensor logit_gradient(const Tensor& h, int64_t v) {
+  const int64_t padded = (v + 63) / 64 * 64;
+  return at::empty({h.size(0), (padded & (padded - 1)) == 0 ? padded + 64 : padded}, h.options());
+}
+
+// (grad_hidden, grad_weight) from the logits' gradient gl.
+std::pair<Tensor, Tensor> head_gradients(const Tensor& gl, const Tensor& h, const Tensor& w, bool need_h, bool need_w) {
+  const int64_t n = h.size(0), d = h.size(1), v = w.size(0), pitch = gl.size(1), padded = (v + 63) / 64 * 64;
+  const int code = code_of(h.scalar_type());
+  void* st = stream_of(h);
+  const size_t bytes = api.ak_lmhead_grad_workspace_bytes(n, v, d);
+  Tensor ws = bytes ? bytes_like(h, bytes) : Tensor();
+  Tensor gh, gw;
+  if (need_w) {
+    gw = at::empty(w.sizes(), w.options());
+    check(api.ak_lmhead_grad_weight(gl.data_ptr(), pitch, h.data_ptr(), d, gw.data_ptr(), d, n, v, d, 0, ptr(ws), bytes, code,
+                                    st), "ak_lmhead_grad_weight");
+  }
+  if (need_h) {
+    // the K padding meets weight rows that load as zeros, but NaN x 0 is NaN
+    if (padded > v) gl.slice(1, v, padded).zero_();
+    gh = at::empty(h.sizes(), h.options());
+    check(api.ak_lmhead_grad_hidden(gl.data_ptr(), pitch, w.data_ptr(), d, gh.data_ptr(), d, n, v, d, 0, ptr(ws), bytes, code,
+                                    st), "ak_lmhead_grad_hidden");
+  }
+  return {gh, gw};
+}
+
 struct LmHead : torch::autograd::Function<LmHead> {
   static Tensor forward(AutogradContext* ctx, const Tensor& h, const Tensor& w, const Tensor& t, int64_t ignore, double cap,
                         double smoothing) {
@@ -567,28 +602,11 @@ struct LmHead : torch::autograd::Function<LmHead> {
     const int64_t n = h.size(0), d = h.size(1), v = w.size(0);
     const int code = code_of(h.scalar_type());
     void* st = stream_of(h);
-    // dlogits: the pitch covers whole 64-column K blocks and stays off powers
-    // of two, whose rows would all start in the same memory channels
-    const int64_t padded = (v + 63) / 64 * 64;
-    const int64_t pitch = (padded & (padded - 1)) == 0 ? padded + 64 : padded;
-    Tensor gl = at::empty({n, pitch}, h.options());
+    Tensor gl = logit_gradient(h, v);
+    const int64_t pitch = gl.size(1);
     check(api.ak_lmhead_ce_bwd_range(h.data_ptr(), w.data_ptr(), i64p(t), f32p(lse), f32p(up), f32p(denom), gl.data_ptr(), pitch,
                                      n, v, 0, v, d, d, d, ignore, (float)p[0], (float)p[1], code, st), "ak_lmhead_ce_bwd_range");
-    const size_t bytes = api.ak_lmhead_grad_workspace_bytes(n, v, d);
-    Tensor ws = bytes ? bytes_like(h, bytes) : Tensor();
-    Tensor gh, gw;
-    if (need_w) {
-      gw = at::empty(w.sizes(), w.options());
-      check(api.ak_lmhead_grad_weight(gl.data_ptr(), pitch, h.data_ptr(), d, gw.data_ptr(), d, n, v, d, 0, ptr(ws), bytes, code,
-                                      st), "ak_lmhead_grad_weight");
-    }
-    if (need_h) {
-      // the K padding meets weight rows that load as zeros, but NaN x 0 is NaN
-      if (padded > v) gl.slice(1, v, padded).zero_();
-      gh = at::empty(h.sizes(), h.options());
-      check(api.ak_lmhead_grad_hidden(gl.data_ptr(), pitch, w.data_ptr(), d, gh.data_ptr(), d, n, v, d, 0, ptr(ws), bytes, code,
-                                      st), "ak_lmhead_grad_hidden");
-    }
+    auto [gh, gw] = head_gradients(gl, h, w, need_h, need_w);
     return {gh, gw, Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };
@@ -601,6 +619,236 @@ Maybe lmhead_ce(const Tensor& h, const Tensor& w, const Tensor& t, int64_t ignor
     return std::nullopt;
   if (records({&h, &w}) && 2.0 * h.size(0) * ((w.size(0) + 255) / 256 * 256) > budget) return std::nullopt;  // vocab ranges
   return LmHead::apply(h, w, t, ignore, cap, smoothing);
+}
+
+// ---------------------------------------------------------------------------
+// Token log probabilities, distillation from a teacher's top logits
+// ---------------------------------------------------------------------------
+constexpr int64_t kMaxScoreVocab = 1 << 20;
+constexpr int64_t kMaxTopEntries = 256;
+
+bool scale_args(double temperature, double softcap) {
+  return temperature >= 1e-18 && temperature <= 1e18 && softcap >= 0.0 && std::isfinite(softcap);
+}
+
+bool score_args(const Tensor& x, double temperature, double softcap) {
+  return x.dim() >= 1 && x.is_contiguous() && x.numel() > 0 && x.size(-1) <= kMaxScoreVocab &&
+         code_of(x.scalar_type()) >= 0 && scale_args(temperature, softcap);
+}
+
+// whole numbers of the leading shape of x (its shape but the last dimension)
+bool leading_i64(const Tensor& t, const Tensor& x) {
+  return t.scalar_type() == at::kLong && t.is_contiguous() && t.sizes() == x.sizes().slice(0, x.dim() - 1);
+}
+
+// An upstream gradient of a row each as the kernels take it.
+Tensor row_gradient(const Tensor& g) { return g.defined() ? g.detach().to(at::kFloat).contiguous() : g; }
+
+// The kernels' results carry no graph: what should have a gradient would pass as a constant.
+void differentiable_once(const char* name) {
+  TORCH_CHECK(!at::GradMode::is_enabled(), name, " is differentiable once: its backward takes no create_graph=True");
+}
+
+struct Tops {
+  Tensor logprobs, ids;  // no outputs of the node, as in CrossEntropy
+};
+
+// {entropy} or {entropy, logprobs}
+variable_list run_logprobs(const Tensor& x, const Tensor& t, double temperature, double softcap, int64_t ignore, int64_t top,
+                           const Tensor& stats, Tops* tops) {
+  const int64_t v = x.size(-1), n = x.numel() / v;
+  const auto lead = x.sizes().slice(0, x.dim() - 1);
+  const int code = code_of(x.scalar_type());
+  variable_list out{f32_like(x, lead)};
+  if (t.defined()) out.push_back(f32_like(x, lead));
+  if (top) {
+    std::vector<int64_t> shape = lead.vec();
+    shape.push_back(top);
+    tops->logprobs = f32_like(x, shape);
+    tops->ids = at::empty(shape, x.options().dtype(at::kLong));
+  }
+  const size_t bytes = api.ak_token_logprobs_workspace_bytes(n, v, (int)top, code);
+  const Tensor ws = bytes ? bytes_like(x, bytes) : Tensor();
+  check(api.ak_token_logprobs_fwd(x.data_ptr(), t.defined() ? i64p(t) : nullptr, t.defined() ? f32p(out[1]) : nullptr,
+                                  f32p(out[0]), f32p(stats), f32p(tops->logprobs),
+                                  static_cast<int64_t*>(ptr(tops->ids)), ptr(ws), bytes, n, v, v, (int)top,
+                                  (float)temperature, (float)softcap, ignore, code, stream_of(x)), "ak_token_logprobs_fwd");
+  return out;
+}
+
+struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Maybe& t_, double temperature, double softcap,
+                               int64_t ignore, int64_t top, Tops* tops) {
+    const Tensor t = t_.value_or(Tensor());
+    const Tensor stats = f32_like(x, {x.numel() / x.size(-1), 4});
+    variable_list out = run_logprobs(x, t, temperature, softcap, ignore, top, stats, tops);
+    ctx->save_for_backward({x, t, stats});
+    ctx->saved_data["p"] = std::vector<double>{temperature, softcap};
+    ctx->saved_data["ignore"] = ignore;
+    ctx->set_materialize_grads(false);
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    differentiable_once("token_logprobs");
+    const auto s = ctx->get_saved_variables();
+    const auto p = ctx->saved_data["p"].toDoubleVector();
+    const Tensor x = s[0].contiguous(), t = saved_as(s[1], at::kLong), stats = saved_as(s[2], at::kFloat);
+    const Tensor ge = row_gradient(g[0]), gl = g.size() > 1 ? row_gradient(g[1]) : Tensor();
+    const int64_t v = x.size(-1), n = x.numel() / v;
+    Tensor grad = at::empty(x.sizes(), x.options());
+    check(api.ak_token_logprobs_bwd(x.data_ptr(), t.defined() ? i64p(t) : nullptr, f32p(stats), f32p(gl), f32p(ge),
+                                    grad.data_ptr(), n, v, v, v, (float)p[0], (float)p[1],
+                                    ctx->saved_data["ignore"].toInt(), code_of(x.scalar_type()), stream_of(x)),
+          "ak_token_logprobs_bwd");
+    return {grad, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+// (logprobs, entropy, top_logprobs, top_ids), undefined (None) where not asked for
+std::optional<std::tuple<Tensor, Tensor, Tensor, Tensor>> token_logprobs(const Tensor& x, const Maybe& t, double temperature,
+                                                                         double softcap, int64_t ignore, int64_t top) {
+  if (!ours(x) || !ours_if(t, x) || !score_args(x, temperature, softcap) || (t && !leading_i64(*t, x)) || top < 0 ||
+      top > std::min(kMaxTopEntries, x.size(-1)))
+    return std::nullopt;
+  Tops tops;
+  const variable_list out =
+      records({&x}) ? TokenLogprobs::apply(x, t, temperature, softcap, ignore, top, &tops)
+                    : run_logprobs(x, t.value_or(Tensor()), temperature, softcap, ignore, top, Tensor(), &tops);
+  return std::make_tuple(t ? out[1] : Tensor(), out[0], tops.logprobs, tops.ids);
+}
+
+struct Distill {
+  Tensor losses, stats, loss, scale;
+};
+
+Distill run_distill(const Tensor& x, const Tensor& teacher, const Tensor& ids, double temperature, double softcap,
+                    int64_t ignore, bool mean) {
+  const int64_t v = x.size(-1), n = x.numel() / v, k = ids.size(-1);
+  const int code = code_of(x.scalar_type());
+  Distill r;
+  r.losses = f32_like(x, x.sizes().slice(0, x.dim() - 1));
+  r.stats = f32_like(x, {n, 4});
+  if (mean) {
+    r.loss = f32_like(x, {});
+    r.scale = f32_like(x, {1});
+  }
+  const size_t bytes = api.ak_topk_distill_workspace_bytes(n, v, code);
+  const Tensor ws = bytes ? bytes_like(x, bytes) : Tensor();
+  check(api.ak_topk_distill_fwd(x.data_ptr(), teacher.data_ptr(), i64p(ids), f32p(r.losses), f32p(r.stats), f32p(r.loss),
+                                f32p(r.scale), ptr(ws), bytes, n, v, k, v, k, k, (float)temperature, (float)softcap, ignore,
+                                code, code_of(teacher.scalar_type()), stream_of(x)), "ak_topk_distill_fwd");
+  return r;
+}
+
+struct TopkDistillation : torch::autograd::Function<TopkDistillation> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& teacher, const Tensor& ids, double temperature,
+                        double softcap, int64_t ignore, bool mean) {
+    const Distill r = run_distill(x, teacher, ids, temperature, softcap, ignore, mean);
+    ctx->save_for_backward({x, teacher, ids, r.stats, r.scale});
+    ctx->saved_data["p"] = std::vector<double>{temperature, softcap};
+    ctx->saved_data["ignore"] = ignore;
+    return mean ? r.loss : r.losses;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    differentiable_once("topk_distillation");
+    const auto s = ctx->get_saved_variables();
+    const auto p = ctx->saved_data["p"].toDoubleVector();
+    const Tensor x = s[0].contiguous(), teacher = s[1].contiguous(), ids = saved_as(s[2], at::kLong);
+    const Tensor stats = saved_as(s[3], at::kFloat), scale = saved_as(s[4], at::kFloat), up = row_gradient(g[0]);
+    const int64_t v = x.size(-1), n = x.numel() / v, k = ids.size(-1);
+    Tensor grad = at::empty(x.sizes(), x.options());
+    check(api.ak_topk_distill_bwd(x.data_ptr(), teacher.data_ptr(), i64p(ids), f32p(stats), f32p(up), scale.defined() ? 0 : 1,
+                                  f32p(scale), grad.data_ptr(), n, v, k, v, k, k, v, (float)p[0], (float)p[1],
+                                  ctx->saved_data["ignore"].toInt(), code_of(x.scalar_type()),
+                                  code_of(teacher.scalar_type()), stream_of(x)), "ak_topk_distill_bwd");
+    return {grad, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+Maybe topk_distillation(const Tensor& x, const Tensor& teacher, const Tensor& ids, double temperature, double softcap,
+                        int64_t ignore, bool mean) {
+  if (!ours(x, teacher, ids) || !score_args(x, temperature, softcap) || teacher.dim() != x.dim() || !teacher.is_contiguous() ||
+      code_of(teacher.scalar_type()) < 0 || teacher.sizes().slice(0, x.dim() - 1) != x.sizes().slice(0, x.dim() - 1) ||
+      teacher.size(-1) < 1 || teacher.size(-1) > kMaxTopEntries || ids.scalar_type() != at::kLong || !ids.is_contiguous() ||
+      ids.sizes() != teacher.sizes())
+    return std::nullopt;
+  const Tensor constant = teacher.requires_grad() ? teacher.detach() : teacher;
+  if (records({&x})) return TopkDistillation::apply(x, constant, ids, temperature, softcap, ignore, mean);
+  const Distill r = run_distill(x, constant, ids, temperature, softcap, ignore, mean);
+  return mean ? r.loss : r.losses;
+}
+
+// ---------------------------------------------------------------------------
+// lm-head log probabilities
+// ---------------------------------------------------------------------------
+variable_list run_lmhead_logprobs(const Tensor& h, const Tensor& w, const Tensor& t, double temperature, double softcap,
+                                  int64_t ignore, const Tensor& stats) {
+  const int64_t n = h.size(0), d = h.size(1), v = w.size(0);
+  variable_list out{f32_like(h, {n})};
+  if (t.defined()) out.push_back(f32_like(h, {n}));
+  const size_t bytes = api.ak_lmhead_logprobs_workspace_bytes(n, v);
+  const Tensor ws = bytes_like(h, bytes);
+  check(api.ak_lmhead_logprobs_fwd(h.data_ptr(), w.data_ptr(), t.defined() ? i64p(t) : nullptr,
+                                   t.defined() ? f32p(out[1]) : nullptr, f32p(out[0]), f32p(stats), ws.data_ptr(), bytes, n, v,
+                                   d, d, d, (float)temperature, (float)softcap, ignore, code_of(h.scalar_type()), stream_of(h)),
+        "ak_lmhead_logprobs_fwd");
+  return out;
+}
+
+struct LmheadLogprobs : torch::autograd::Function<LmheadLogprobs> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& h, const Tensor& w, const Maybe& t_, double temperature,
+                               double softcap, int64_t ignore) {
+    const Tensor t = t_.value_or(Tensor());
+    const Tensor stats = f32_like(h, {h.size(0), 2});
+    variable_list out = run_lmhead_logprobs(h, w, t, temperature, softcap, ignore, stats);
+    ctx->save_for_backward({h, w, t, stats});
+    ctx->saved_data["p"] = std::vector<double>{temperature, softcap};
+    ctx->saved_data["ignore"] = ignore;
+    ctx->set_materialize_grads(false);
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    differentiable_once("lmhead_logprobs");
+    const auto s = ctx->get_saved_variables();
+    const auto p = ctx->saved_data["p"].toDoubleVector();
+    const int64_t ignore = ctx->saved_data["ignore"].toInt();
+    const bool need_h = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1);
+    const Tensor h = realigned(s[0].contiguous()), w = realigned(saved_as(s[1], h.scalar_type()));
+    const Tensor t = saved_as(s[2], at::kLong), stats = saved_as(s[3], at::kFloat);
+    const Tensor ge = row_gradient(g[0]), gl = g.size() > 1 ? row_gradient(g[1]) : Tensor();
+    const int64_t n = h.size(0), d = h.size(1), v = w.size(0);
+    const int64_t* tp = t.defined() ? i64p(t) : nullptr;
+    const Tensor coefs = f32_like(h, {n, 4});
+    check(api.ak_lmhead_logprobs_coefs(tp, f32p(stats), f32p(gl), f32p(ge), f32p(coefs), n, v, (float)p[0], ignore, stream_of(h)),
+          "ak_lmhead_logprobs_coefs");
+    const Tensor dz = logit_gradient(h, v);
+    check(api.ak_lmhead_logprobs_bwd_range(h.data_ptr(), w.data_ptr(), tp, f32p(coefs), dz.data_ptr(), dz.size(1), n, v, 0, v, d,
+                                           d, d, (float)p[0], (float)p[1], ignore, code_of(h.scalar_type()), stream_of(h)),
+          "ak_lmhead_logprobs_bwd_range");
+    auto [gh, gw] = head_gradients(dz, h, w, need_h, need_w);
+    return {gh, gw, Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+// (logprobs or None, entropy). budget: as in lmhead_ce.
+std::optional<std::tuple<Tensor, Tensor>> lmhead_logprobs(const Tensor& h, const Tensor& w, const Maybe& t, double temperature,
+                                                          double softcap, int64_t ignore, double budget) {
+  if (!ours(h, w) || !ours_if(t, h) || !scale_args(temperature, softcap) || h.dim() < 1 || !h.is_contiguous() || !at16(h) ||
+      !dense16(w) || h.scalar_type() != w.scalar_type() || h.numel() == 0 || w.size(0) == 0 ||
+      (h.scalar_type() != at::kHalf && h.scalar_type() != at::kBFloat16) || h.size(-1) != w.size(1) || w.size(1) % 64 ||
+      (t && !leading_i64(*t, h)))
+    return std::nullopt;
+  const int64_t d = w.size(1);
+  const bool rec = records({&h, &w});
+  if (rec && 2.0 * (h.numel() / d) * ((w.size(0) + 255) / 256 * 256) > budget) return std::nullopt;  // vocab ranges
+  const bool flat = h.dim() == 2;
+  const Tensor h2 = flat ? h : h.view({-1, d});
+  const Maybe t2 = t && !flat ? Maybe(t->view({-1})) : t;
+  variable_list out = rec ? LmheadLogprobs::apply(h2, w, t2, temperature, softcap, ignore)
+                          : run_lmhead_logprobs(h2, w, t2.value_or(Tensor()), temperature, softcap, ignore, Tensor());
+  if (!flat)
+    for (Tensor& o : out) o = o.view(h.sizes().slice(0, h.dim() - 1));
+  return std::make_tuple(t ? out[1] : Tensor(), out[0]);
 }
 
 }  // namespace
@@ -621,4 +869,7 @@ PYBIND11_MODULE(_host_ops, m) {
   m.def("diag_scan_op", &diag_scan_op, nogil());
   m.def("selective_scan", &selective_scan, nogil());
   m.def("lmhead_ce", &lmhead_ce, nogil());
+  m.def("token_logprobs", &token_logprobs, nogil());
+  m.def("topk_distillation", &topk_distillation, nogil());
+  m.def("lmhead_logprobs", &lmhead_logprobs, nogil());
 }

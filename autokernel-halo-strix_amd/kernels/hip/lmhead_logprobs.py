@@ -27,6 +27,7 @@ import torch
 import torch.nn.functional as F
 
 from kernels.hip import _lib
+from kernels.hip import chunked_linear_cross_entropy as clce
 from kernels.hip.chunked_linear_cross_entropy import _fused_ok, _kernel_operands, gradients_by_ranges
 from kernels.hip.token_logprobs import check_scale, differentiable_once, row_gradient, whole_numbers
 
@@ -131,6 +132,13 @@ def kernel_fn(hidden: torch.Tensor, weight: torch.Tensor, tokens: Optional[torch
             have to be finite where ``weight``'s gradient is asked for).
         chunk_size: rows per chunk of the fp32 path's GEMMs.
     """
+    temperature, softcap, ignore_index, chunk_size = float(temperature), float(softcap), int(ignore_index), int(chunk_size)
+    host = _lib.native(hidden, weight) if tokens is None else _lib.native(hidden, weight, tokens)
+    if host is not None and chunk_size > 0:
+        out = host.lmhead_logprobs(hidden, weight, tokens, temperature, softcap, ignore_index,
+                                   float(clce.GRAD_LOGITS_BUDGET))
+        if out is not None:
+            return LmheadLogprobs(*out)
     _lib.require_device(hidden, weight, tokens)
     _lib.dtype_code(hidden.dtype)
     if hidden.dim() == 0 or weight.dim() != 2 or weight.shape[1] != hidden.shape[-1]:
@@ -140,7 +148,6 @@ def kernel_fn(hidden: torch.Tensor, weight: torch.Tensor, tokens: Optional[torch
         raise ValueError(f"weight must not be empty, got shape {tuple(weight.shape)}")
     if hidden.dtype == torch.float32 and vocab > _lib.MAX_SCORE_VOCAB:
         raise ValueError(f"fp32 takes a vocab of at most {_lib.MAX_SCORE_VOCAB}, got {vocab}")
-    temperature, softcap, ignore_index, chunk_size = float(temperature), float(softcap), int(ignore_index), int(chunk_size)
     check_scale(temperature, softcap)
     if chunk_size < 1:
         raise ValueError(f"chunk_size must be at least 1, got {chunk_size}")

@@ -143,10 +143,15 @@ def kernel_fn(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, *, te
         ignore_index: token value of rows to leave out.
         top_k: alternatives of each row, 0 to min(256, vocab).
     """
+    temperature, softcap, ignore_index, top_k = float(temperature), float(softcap), int(ignore_index), int(top_k)
+    host = _lib.native(logits) if tokens is None else _lib.native(logits, tokens)
+    if host is not None:
+        out = host.token_logprobs(logits, tokens, temperature, softcap, ignore_index, top_k)
+        if out is not None:
+            return TokenLogprobs(*out)
     _lib.require_device(logits, tokens)
     vocab = check_vocab(logits)
     lead = logits.shape[:-1]
-    temperature, softcap, ignore_index, top_k = float(temperature), float(softcap), int(ignore_index), int(top_k)
     check_scale(temperature, softcap)
     if not 0 <= top_k <= min(_lib.MAX_TOP, vocab):
         raise ValueError(f"top_k must be 0 to min({_lib.MAX_TOP}, vocab), got {top_k}")

@@ -92,6 +92,13 @@ def kernel_fn(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_ids: t
         reduction: ``"mean"`` over the rows that have entries (a 0-d tensor),
             or ``"none"`` (one loss a row).
     """
+    temperature, softcap, ignore_index = float(temperature), float(softcap), int(ignore_index)
+    host = _lib.native(logits, teacher_logits, teacher_ids)
+    if host is not None and reduction in ("mean", "none"):
+        loss = host.topk_distillation(logits, teacher_logits, teacher_ids, temperature, softcap, ignore_index,
+                                      reduction == "mean")
+        if loss is not None:
+            return loss
     _lib.require_device(logits, teacher_logits, teacher_ids)
     vocab = check_vocab(logits)
     if reduction not in ("mean", "none"):
@@ -104,7 +111,6 @@ def kernel_fn(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_ids: t
     k = teacher_logits.shape[-1]
     if not 1 <= k <= _lib.MAX_TOP:
         raise ValueError(f"1 to {_lib.MAX_TOP} teacher entries a row are taken, got {k}")
-    temperature, softcap, ignore_index = float(temperature), float(softcap), int(ignore_index)
     check_scale(temperature, softcap)
     ids = whole_numbers(teacher_ids, "teacher_ids", teacher_logits.shape).view(-1, k)
     teacher = _lib.as_rows(teacher_logits.detach(), k)
