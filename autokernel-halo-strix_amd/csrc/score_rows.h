@@ -100,6 +100,31 @@ __device__ __forceinline__ RowStats wave_join(const ScoreParams& p, RowStats st)
   return st;
 }
 
+// The largest element of a vector. In assembly, since fmaxf first quiets each
+// operand that it does not know to be quiet (an instruction an element). A
+// signalling NaN makes the result NaN, a quiet one is passed over; a row that
+// holds either has a NaN sum. (The caller's next use is no lane permutation,
+// which would need wait states that the compiler does not see here.)
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float m;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(m) : "v"(a), "v"(b), "v"(c));
+  return m;
+}
+__device__ __forceinline__ float vec_max(const Vec16<float>& v) { return max3(max3(v.e[0], v.e[1], v.e[2]), v.e[3], v.e[3]); }
+__device__ __forceinline__ float vec_max(const Vec16<bf16>& v) {
+  auto lo = [&](int i) { return __builtin_bit_cast(float, v.u[i] << 16); };
+  auto hi = [&](int i) { return __builtin_bit_cast(float, v.u[i] & 0xFFFF0000u); };
+  return max3(max3(max3(max3(lo(0), hi(0), lo(1)), hi(1), lo(2)), hi(2), lo(3)), hi(3), hi(3));
+}
+__device__ __forceinline__ float vec_max(const Vec16<f16>& v) {
+  uint32_t a, b;
+  asm("v_pk_max_f16 %0, %1, %2" : "=v"(a) : "v"(v.u[0]), "v"(v.u[1]));
+  asm("v_pk_max_f16 %0, %1, %2" : "=v"(b) : "v"(v.u[2]), "v"(v.u[3]));
+  asm("v_pk_max_f16 %0, %1, %2" : "=v"(a) : "v"(a), "v"(b));
+  const f16x2_t m = __builtin_bit_cast(f16x2_t, a);
+  return max3((float)m[0], (float)m[1], (float)m[1]);
+}
+
 // A segment of a row in registers: TPR threads, VPT vectors each, and the
 // elements around the row's vectors (at most 14, with the first segment) one
 // to a thread.
@@ -158,13 +183,59 @@ struct Segment {
     float m = t < nx ? to_f32(xe) : -INFINITY;
 #pragma unroll
     for (int k = 0; k < VPT; ++k) {
-      if (t + k * TPR < nv) {
+      const float vm = vec_max(raw[k]);
+      m = fmaxf(m, t + k * TPR < nv ? vm : -INFINITY);
+      keep_packed(raw[k]);
+    }
+    return m;
+  }
+
+  // The same, and the maxima of the segment's groups of 2^SHIFT vectors, joined
+  // over as many lanes. maxima: the segment's first group's place; group: what
+  // this thread stores of them (store_groups): lane l of a group's lanes those
+  // of the vectors l, l + 2^SHIFT, ...
+  template <int SHIFT>
+  static constexpr int kStored = SHIFT > 0 ? (VPT + (1 << SHIFT) - 1) >> SHIFT : 1;
+
+  template <int SHIFT>
+  __device__ __forceinline__ float largest_of_groups(float* __restrict__ maxima, float (&group)[kStored<SHIFT>]) {
+    const int t = thread();
+    float m = t < nx ? to_f32(xe) : -INFINITY;
+    const int l = t & ((1 << SHIFT) - 1);
 #pragma unroll
-        for (int e = 0; e < VE; ++e) m = fmaxf(m, to_f32(raw[k].e[e]));
+    for (int k = 0; k < VPT; ++k) {
+      const bool in = t + k * TPR < nv;
+      float vm = vec_max(raw[k]);
+      vm = in ? vm : -INFINITY;
+      m = fmaxf(m, vm);
+      if constexpr (SHIFT >= 3) {
+        vm = fmaxf(vm, dpp<kDppXor1>(vm));
+        vm = fmaxf(vm, dpp<kDppXor2>(vm));
+        vm = fmaxf(vm, dpp<kDppHalfMirror>(vm));
+      }
+      if constexpr (SHIFT == 6) {
+        vm = fmaxf(vm, dpp<kDppMirror>(vm));
+        vm = fmaxf(vm, __shfl_xor(vm, 16, 64));
+        vm = fmaxf(vm, __shfl_xor(vm, 32, 64));
+      }
+      if constexpr (SHIFT == 0) {
+        if (in) maxima[t + k * TPR] = vm;
+      } else {
+        group[k >> SHIFT] = (k & ((1 << SHIFT) - 1)) == l ? vm : group[k >> SHIFT];
       }
       keep_packed(raw[k]);
     }
     return m;
+  }
+
+  template <int SHIFT>
+  __device__ __forceinline__ void store_groups(float* __restrict__ maxima, const float (&group)[kStored<SHIFT>]) const {
+    const int t = thread(), l = t & ((1 << SHIFT) - 1);
+#pragma unroll
+    for (int i = 0; i < kStored<SHIFT>; ++i) {
+      const int k = (i << SHIFT) + l, v = (t & ~((1 << SHIFT) - 1)) + k * TPR;  // the group's first vector
+      if (k < VPT && v < nv) maxima[v >> SHIFT] = group[i];
+    }
   }
 
   // This thread's part of s and, with ENT, of u.
@@ -187,38 +258,34 @@ struct ScorePlan {
   int segs, span;  // segments a row, vectors a segment
 };
 
-constexpr int kSegVectors = 8192;            // most vectors of a segment: 1024 threads x 8
+constexpr int kSegVectors = 8192;            // most vectors of a segment: 512 threads x 16
 constexpr int64_t kScoreVocab = 1 << 20;     // widest row
 constexpr int kMaxTop = 256;                 // most alternatives
-constexpr int kJoinKeys = 8192;              // most keys that the join holds in LDS
 
 // One segment a row where there are rows for every CU. Fewer rows are cut so
 // that about two workgroups a CU share the work, in segments of at least 256
-// vectors (one a thread), and with `top` alternatives in at most kJoinKeys /
-// 2 keys for the join.
-inline ScorePlan score_plan(int64_t rows, int64_t vocab, int ve, int top) {
+// vectors (one a thread), whole multiples of 64.
+inline ScorePlan score_plan(int64_t rows, int64_t vocab, int ve) {
   const int64_t nvec = std::max<int64_t>(1, vocab / ve);
   const int64_t least = (nvec + kSegVectors - 1) / kSegVectors;
   int64_t segs = least;
-  if (rows < 256) {
-    segs = std::max(segs, std::min((512 + rows - 1) / rows, nvec / 256));
-    if (top > 0) segs = std::max(least, std::min<int64_t>(segs, kJoinKeys / 2 / top));
-  }
-  const int64_t span = (nvec + segs - 1) / segs;
+  if (rows < 256) segs = std::max(segs, std::min((512 + rows - 1) / rows, nvec / 256));
+  const int64_t span = ((nvec + segs - 1) / segs + 63) / 64 * 64;
   return {(int)((nvec + span - 1) / span), (int)span};
 }
 
-// kernel<VPT, TPR> for a segment of `span` vectors: the fewest vectors a
-// thread that the workgroup sizes allow.
-#define AK_SEGMENT_DISPATCH(span, GO) \
-  do {                                \
-    if ((span) <= 256) GO(1, 256);    \
+// kernel<VPT, TPR> for a segment of `span` vectors.
+#define AK_SEGMENT_DISPATCH(span, GO)    \
+  do {                                   \
+    if ((span) <= 256) GO(1, 256);       \
     else if ((span) <= 512) GO(2, 256);  \
     else if ((span) <= 1024) GO(4, 256); \
-    else if ((span) <= 2048) GO(4, 512); \
-    else if ((span) <= 4096) GO(8, 512); \
-    else GO(8, 1024);                 \
+    else if ((span) <= 2048) GO(8, 256); \
+    else if ((span) <= 4096) GO(16, 256);\
+    else GO(16, 512);                    \
   } while (0)
+// (waves a SIMD that the register budget is set for)
+#define AK_SEGMENT_WAVES(VPT) ((VPT) == 16 ? 4 : (VPT) == 8 ? 6 : 1)
 
 // ---------------------------------------------------------------------------
 // Gradients: rows written whole from their statistics

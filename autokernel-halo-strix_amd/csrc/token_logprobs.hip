@@ -10,19 +10,23 @@
 // HBM-bound: the forward reads the logits once (score_rows.h), the backward
 // reads them once and writes the gradient once.
 //
-// Alternatives. Every thread has the largest of the (at most 64) logits it
-// holds from the max pass. The top_k-th largest of these group maxima is a
-// lower bound of the row's top_k-th logit, since top_k groups reach it; few
-// other logits do (for random rows about G ln(G / (G - K)) of them reach the
-// bound of G groups: 66 for 64 of 1024). So the threshold comes from one
-// wave's search over the maxima while the others form their exponentials, the
-// logits that reach it are gathered in LDS, and each finds its place by
-// counting the larger ones. Rows of which too many reach the threshold
-// (thousands of equal logits) and rows with NaN find the exact bound by
-// bisection over the whole segment (exact_top). A key holds the logit's place among the
-// numbers above the complement of its column, so keys are unique, equal logits
-// go by column and the result depends on neither the gathering's order nor
-// the row's split. -0 equals +0; NaN comes first.
+// Alternatives. The first kernel, which has the logits in registers, also
+// writes the maximum of each group of consecutive logits (128 bytes of the row
+// as a rule: 8 vectors, joined over 8 lanes). The row's top_k largest logits lie
+// in the top_k groups of the largest maxima, and in the few logits around the
+// row's vectors: each of those groups has a logit at or above the top_k-th
+// maximum, and where maxima are equal the groups of lower columns have the
+// lower columns. So a second kernel, one wave a row, bisects for the top_k-th
+// maximum, reads those groups again (one line each), gathers what passes the
+// maximum, and as many logits equal to it as are still wanted, in the order of
+// their columns, and places each by counting the larger ones. Keys hold a
+// logit's place among the numbers above the complement of its column, so they
+// are unique and the result depends on neither the gathering's order nor the
+// row's split. -0 equals +0; NaN comes first. Rows with NaN, and rows of which
+// more logits pass the bound than LDS holds, are bisected whole (exact_top).
+// (With the search, the gathering and the placing in the first kernel, [4096,
+// 32768] bf16 with 64 alternatives took 78 to 90 us, where the statistics alone
+// take 48: the phases between its barriers left too few loads in flight.)
 #include <type_traits>
 
 #include "score_rows.h"
@@ -45,9 +49,6 @@ __device__ __forceinline__ u64 key_of(float x, int col) { return (u64)place_of(x
 __device__ __forceinline__ int key_col(u64 key) { return (int)~(uint32_t)key; }
 __device__ __forceinline__ float key_logit(u64 key) { return float_at((uint32_t)(key >> 32)); }
 
-constexpr int kCandVectors = 512;  // vectors and keys gathered before the exact bound is searched
-constexpr int kCand = 1024;
-
 struct LogprobArgs {
   const int64_t* tokens;  // nullable
   float* logprobs;        // with tokens
@@ -55,9 +56,9 @@ struct LogprobArgs {
   f32x4_t* stats;         // nullable: (m, log2 s, H, -) for the backward
   float* top_logprobs;    // with top > 0
   int64_t* top_ids;
-  f32x4_t* part;          // segs > 1: (m, s, u, -) of each segment
-  u64* keys;              // segs > 1 and top > 0: its top keys, descending, 0 where it has none
-  int top, vocab;
+  f32x4_t* part;          // segs > 1 or top > 0: (m, s, u, -) of each segment
+  float* maxima;          // top > 0: [rows, groups] maxima of 2^shift vectors each
+  int top, vocab, groups, shift;
 };
 
 // The row's results but the alternatives, by one thread.
@@ -91,48 +92,183 @@ __device__ __forceinline__ void store_top(const ScoreParams& p, const LogprobArg
   a.top_ids[row * a.top + r] = key_col(key);
 }
 
-// Lower bound of the `top`-th largest of the n places in LDS, by one wave:
-// its first 20 bits, the rest zero. 0 where fewer than `top` are above 0.
-template <int MAXN>
-__device__ __forceinline__ uint32_t nth_place(const uint32_t* places, int n, int top) {
-  constexpr int PER = MAXN / 64;
-  uint32_t v[PER];
+// One workgroup per segment (units by grid stride; the loop bound is uniform).
+// SHIFT: kHere where the results are formed here, kPart where they are the
+// join's to form, or what 2^SHIFT vectors the groups of alternatives have.
+constexpr int kHere = -2, kPart = -1;
+
+template <typename T, int VPT, int TPR, bool CAP, int SHIFT>
+__global__ void __launch_bounds__(TPR, AK_SEGMENT_WAVES(VPT))
+logprob_segment_kernel(const T* __restrict__ logits, int64_t rows, int64_t ld, int segs, int span, ScoreParams p,
+                       LogprobArgs a) {
+  constexpr int W = TPR / 64;
+  constexpr bool PART = SHIFT != kHere;
+  __shared__ float part_m[W], part_s[W], part_u[W];
+  for (int64_t unit = blockIdx.x; unit < rows * segs; unit += gridDim.x) {
+    const int64_t row = segs == 1 ? unit : unit / segs;
+    const int seg = segs == 1 ? 0 : (int)(unit - row * segs);
+    const T* x = logits + row * ld;
+    int64_t tok = p.ignore_index;
+    float x_tok = 0.0f;
+    if (!PART && threadIdx.x == 0 && a.tokens) {
+      tok = a.tokens[row];
+      if (tok != p.ignore_index && tok >= 0 && tok < a.vocab) x_tok = to_f32(x[tok]);
+    }
+    Segment<T, VPT, TPR> sg(x, a.vocab, seg, span);
+    float m, group[Segment<T, VPT, TPR>::template kStored<(SHIFT > 0 ? SHIFT : 0)>] = {};
+    float* const maxima = SHIFT >= 0 ? a.maxima + row * a.groups + seg * (span >> (SHIFT > 0 ? SHIFT : 0)) : nullptr;
+    if constexpr (SHIFT >= 0) m = sg.template largest_of_groups<SHIFT>(maxima, group);
+    else m = sg.largest();
+    m = wave_max(m);
+    if ((threadIdx.x & 63) == 0) part_m[threadIdx.x / 64] = m;
+    __syncthreads();
 #pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int j = i * 64 + (threadIdx.x & 63);
-    v[i] = j < n ? places[j] : 0u;
-  }
-  uint32_t bound = 0;
-  for (int bit = 31; bit >= 12; --bit) {
-    const uint32_t at = bound | 1u << bit;
-    int c = 0;
+    for (int i = 0; i < W; ++i) m = fmaxf(m, part_m[i]);
+    RowStats st;
+    st.m = CAP ? score<CAP>(p, m) : m;
+    sg.template sums<CAP, true>(p, st.m, st.s, st.u);
+    st.s = wave_sum(st.s);
+    st.u = wave_sum(st.u);
+    if ((threadIdx.x & 63) == 0) {
+      part_s[threadIdx.x / 64] = st.s;
+      part_u[threadIdx.x / 64] = st.u;
+    }
+    __syncthreads();  // part_m has been read by all, so the next unit may write it
+    if (threadIdx.x == 0) {
+      st.s = part_s[0];
+      st.u = part_u[0];
 #pragma unroll
-    for (int i = 0; i < PER; ++i) c += __popcll(__ballot(v[i] >= at));
-    if (c >= top) bound = at;
+      for (int i = 1; i < W; ++i) {
+        st.s += part_s[i];
+        st.u += part_u[i];
+      }
+      if (PART) a.part[unit] = f32x4_t{st.m, st.s, st.u, 0.0f};
+      else finish_row<CAP>(p, a, row, st, tok, x_tok);
+    }
+    __syncthreads();  // part_s / part_u are rewritten for the workgroup's next unit
+    // (behind the barriers, which would wait for the store)
+    if constexpr (SHIFT > 0) sg.template store_groups<SHIFT>(maxima, group);
   }
-  return bound;
 }
 
-// The keys of a segment's `top` largest logits (all where it has fewer),
-// gathered in any order: a search by two bits at a time for the top-th largest
-// place, then for the column up to which logits of that place belong to the
-// top, the segment read again for each step. For rows of which too many logits
-// reach the threshold, and for rows with NaN; element by element, so that the
-// kernel's registers are those of its common rows. Reached by the whole
-// workgroup; part: 64 bits a wave.
-template <typename T, int TPR>
-__device__ int exact_top(const T* __restrict__ row, int vocab, int seg, int span, int top, u64* cand, int* count,
-                         u64* part) {
-  constexpr int VE = Vec16<T>::VE;
-  const RowSplit<T> sp(row, vocab);
-  const int v0 = seg * span, t = threadIdx.x;
-  const int end = sp.head + sp.nvec * VE;
-  // the segment's columns [lo, hi), and with the first one the row's last [end, vocab)
-  const int lo = seg == 0 ? 0 : sp.head + v0 * VE, hi = min(sp.head + (v0 + span) * VE, end);
+// A row's statistics from its segments, by one wave, in a fixed order.
+__device__ __forceinline__ RowStats join_row(const ScoreParams& p, const f32x4_t* part, int segs) {
+  RowStats st{-INFINITY, 0.0f, 0.0f};
+  if (segs == 1) {
+    const f32x4_t q = part[0];
+    return RowStats{q[0], q[1], q[2]};
+  }
+  for (int i = threadIdx.x & 63; i < segs; i += 64) {
+    const f32x4_t q = part[i];
+    st = join_stats(p, st, RowStats{q[0], q[1], q[2]});
+  }
+  return wave_join(p, st);
+}
+
+// Rows without alternatives from their segments, one wave a row.
+template <typename T, bool CAP>
+__global__ void __launch_bounds__(64)
+logprob_join_kernel(const T* __restrict__ logits, int64_t ld, int segs, ScoreParams p, LogprobArgs a) {
+  const int64_t row = blockIdx.x;
+  int64_t tok = p.ignore_index;
+  float x_tok = 0.0f;
+  if (threadIdx.x == 0 && a.tokens) {
+    tok = a.tokens[row];
+    if (tok != p.ignore_index && tok >= 0 && tok < a.vocab) x_tok = to_f32(logits[row * ld + tok]);
+  }
+  const RowStats st = join_row(p, a.part + row * segs, segs);
+  if (threadIdx.x == 0) finish_row<CAP>(p, a, row, st, tok, x_tok);
+}
+
+// The bits of a place that tell logits of type T apart.
+template <typename T>
+constexpr uint32_t kPlaceBits = std::is_same<T, float>::value ? 0xFFFFFFFFu : std::is_same<T, f16>::value ? 0xFFFFE000u : 0xFFFF0000u;
+
+// How many of these lanes are below the calling one.
+__device__ __forceinline__ int lanes_before(u64 lanes) {
+  return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(lanes >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)lanes, 0));
+}
+
+// What one row's alternatives are chosen from.
+struct Groups {
+  const uint16_t* list;  // the chosen groups, ascending
+  int n, shift;          // their number; 2^shift vectors a group
+};
+
+// Sum of v over the lanes below the calling one, and over all lanes.
+__device__ __forceinline__ int lanes_sum_before(int v, int& all) {
+  int c = v;  // inclusive: within rows of 16 lanes, then across them
+  c += __builtin_amdgcn_update_dpp(0, c, 0x111, 0xF, 0xF, false);  // row_shr 1
+  c += __builtin_amdgcn_update_dpp(0, c, 0x112, 0xF, 0xF, false);  // row_shr 2
+  c += __builtin_amdgcn_update_dpp(0, c, 0x114, 0xF, 0xF, false);  // row_shr 4
+  c += __builtin_amdgcn_update_dpp(0, c, 0x118, 0xF, 0xF, false);  // row_shr 8
+  c += __builtin_amdgcn_update_dpp(0, c, 0x142, 0xA, 0xF, false);  // row_bcast 15, into rows 1 and 3
+  c += __builtin_amdgcn_update_dpp(0, c, 0x143, 0xC, 0xF, false);  // row_bcast 31, into rows 2 and 3
+  all = __builtin_amdgcn_readlane(c, 63);
+  return c - v;
+}
+
+// Gathers the keys of the logits of the chosen groups that `passes` takes, in
+// any order; the loads of eight vectors a thread are in flight before the first
+// is used. Reached by whole waves; what `count` passes CAND by is left out.
+template <typename T, int TT, int CAND, typename F>
+__device__ __forceinline__ void gather_chosen(const T* __restrict__ row, const RowSplit<T>& sp, const Groups& g, u64* cand,
+                                              int* count, F passes) {
+  constexpr int VE = Vec16<T>::VE, U = 8;
+  const int total = g.n << g.shift, lane = threadIdx.x & 63;
+  for (int i0 = threadIdx.x - lane; i0 < total; i0 += U * TT) {
+    Vec16<T> q[U];
+    int col[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + lane + u * TT;
+      const int v = i < total ? (g.list[i >> g.shift] << g.shift) + (i & ((1 << g.shift) - 1)) : sp.nvec;
+      col[u] = v < sp.nvec ? sp.head + v * VE : -1;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (col[u] >= 0) q[u] = load16_any(row + col[u]);
+    uint32_t mask[U];  // bit e: element e of vector u passes
+    int mine = 0;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int e = 0; e < VE; ++e) m |= passes(to_f32(q[u].e[e])) ? 1u << e : 0u;
+      mask[u] = col[u] >= 0 ? m : 0u;
+      mine += __popc(mask[u]);
+    }
+    int all, to = lanes_sum_before(mine, all);
+    if (all == 0) continue;
+    int base = 0;
+    if (lane == 0) base = atomicAdd(count, all);
+    to += __builtin_amdgcn_readfirstlane(base);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (mask[u]) {
+#pragma unroll
+        for (int e = 0; e < VE; ++e) {
+          if (mask[u] >> e & 1) {
+            if (to < CAND) cand[to] = key_of(to_f32(q[u].e[e]), col[u] + e);
+            ++to;
+          }
+        }
+      }
+    }
+  }
+}
+
+// The keys of a row's `top` largest logits, gathered in any order: a search by
+// two bits at a time for the top-th largest place, then for the column up to
+// which logits of that place belong to the top, the row read again for each
+// step. For rows with NaN, and rows of which too many logits pass the bound.
+// Reached by the whole workgroup; part: 64 bits a wave.
+template <typename T, int TT>
+__device__ int exact_top(const T* __restrict__ row, int vocab, int top, u64* cand, int* count, u64* part) {
+  const int t = threadIdx.x;
   auto each = [&](auto f) {
 #pragma unroll 4
-    for (int i = lo + t; i < hi; i += TPR) f(place_of(to_f32(row[i])), i);
-    if (seg == 0 && end + t < vocab) f(place_of(to_f32(row[end + t])), end + t);
+    for (int i = t; i < vocab; i += TT) f(place_of(to_f32(row[i])), i);
   };
   // which(place, column): up to three counts of 21 bits
   auto total = [&](auto which) {
@@ -143,8 +279,7 @@ __device__ int exact_top(const T* __restrict__ row, int vocab, int seg, int span
     if ((t & 63) == 0) part[t / 64] = c;
     __syncthreads();
     c = 0;
-#pragma unroll 4
-    for (int i = 0; i < TPR / 64; ++i) c += part[i];
+    for (int i = 0; i < TT / 64; ++i) c += part[i];
     return c;
   };
   auto of = [](u64 c, int j) { return (int)(c >> (21 * (j - 1))) & 0x1FFFFF; };
@@ -180,204 +315,195 @@ __device__ int exact_top(const T* __restrict__ row, int vocab, int seg, int span
   return *count;
 }
 
-// One workgroup per segment (units by grid stride; the loop bound is uniform).
-template <typename T, int VPT, int TPR, bool CAP, bool TOP>
-__global__ void __launch_bounds__(TPR, VPT == 8 ? 8 : 1)
-logprob_segment_kernel(const T* __restrict__ logits, int64_t rows, int64_t ld, int segs, int span, ScoreParams p,
-                       LogprobArgs a) {
-  constexpr int W = TPR / 64;
-  __shared__ float part_m[W], part_s[W], part_u[W];
-  __shared__ uint32_t places[TOP ? TPR : 1];
-  __shared__ u32x4 vectors[TOP ? kCandVectors : 1];
-  __shared__ int columns[TOP ? kCandVectors : 1];
-  __shared__ u64 cand[TOP ? kCand : 1];
-  __shared__ int count[2];  // vectors, keys
-  __shared__ u64 totals[TOP ? W : 1];
-  __shared__ uint32_t bound;
-  for (int64_t unit = blockIdx.x; unit < rows * segs; unit += gridDim.x) {
-    const int64_t row = segs == 1 ? unit : unit / segs;
-    const int seg = segs == 1 ? 0 : (int)(unit - row * segs);
-    const T* x = logits + row * ld;
-    int64_t tok = p.ignore_index;
-    float x_tok = 0.0f;
-    if (segs == 1 && threadIdx.x == 0 && a.tokens) {
-      tok = a.tokens[row];
-      if (tok != p.ignore_index && tok >= 0 && tok < a.vocab) x_tok = to_f32(x[tok]);
-    }
-    Segment<T, VPT, TPR> sg(x, a.vocab, seg, span);
+// Groups that may be chosen beyond top: the search ends some bits earlier.
+constexpr int kSpare = 16;
 
-    const float tm = sg.largest();
-    float m = wave_max(tm);
-    if ((threadIdx.x & 63) == 0) part_m[threadIdx.x / 64] = m;
-    int fold = 1;
-    if constexpr (TOP) {
-      // groups of 1, 2 or 4 threads: the fewest of at least 4 top groups
-      float g = tm;
-      if (TPR / 2 >= 4 * a.top) {
-        g = fmaxf(g, dpp<kDppXor1>(g));
-        fold = 2;
-      }
-      if (TPR / 4 >= 4 * a.top) {
-        g = fmaxf(g, dpp<kDppXor2>(g));
-        fold = 4;
-      }
-      // (a group that holds nothing, or -inf alone, stays below every bound)
-      if (threadIdx.x % fold == 0) places[threadIdx.x / fold] = g == -INFINITY ? 0u : place_of(g);
-      if (threadIdx.x < 2) count[threadIdx.x] = 0;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < W; ++i) m = fmaxf(m, part_m[i]);
-    if constexpr (TOP) {
-      if (threadIdx.x < 64) {
-        const uint32_t b = fold == 4 ? nth_place<TPR / 4>(places, TPR / 4, a.top) : nth_place<TPR>(places, TPR / fold, a.top);
-        if (threadIdx.x == 0) bound = b;
-      }
-    }
-    RowStats st;
-    st.m = CAP ? score<CAP>(p, m) : m;
-    sg.template sums<CAP, true>(p, st.m, st.s, st.u);
-    st.s = wave_sum(st.s);
-    st.u = wave_sum(st.u);
-    if ((threadIdx.x & 63) == 0) {
-      part_s[threadIdx.x / 64] = st.s;
-      part_u[threadIdx.x / 64] = st.u;
-    }
-    __syncthreads();
-    st.s = part_s[0];
-    st.u = part_u[0];
-#pragma unroll
-    for (int i = 1; i < W; ++i) {
-      st.s += part_s[i];
-      st.u += part_u[i];
-    }
-    if (threadIdx.x == 0) {
-      if (segs == 1) finish_row<CAP>(p, a, row, st, tok, x_tok);
-      else a.part[unit] = f32x4_t{st.m, st.s, st.u, 0.0f};
-    }
-
-    if constexpr (TOP) {
-      constexpr int VE = Vec16<T>::VE;
-      auto keep = [&](u64 key) {
-        const int at = atomicAdd(&count[1], 1);
-        if (at < kCand) cand[at] = key;
-      };
-      // vectors with a logit that reaches the threshold go to LDS whole, so
-      // that their elements are looked at by as many threads
-      const float least = bound == 0 ? -INFINITY : float_at(bound);
-      if (tm >= least) {
-        const int t = sg.thread();
-#pragma unroll
-        for (int k = 0; k < VPT; ++k) {
-          float vm = to_f32(sg.raw[k].e[0]);
-#pragma unroll
-          for (int e = 1; e < VE; ++e) vm = fmaxf(vm, to_f32(sg.raw[k].e[e]));
-          if (vm >= least && t + k * TPR < sg.nv) {
-            const int at = atomicAdd(&count[0], 1);
-            if (at < kCandVectors) {
-              vectors[at] = sg.raw[k].u;
-              columns[at] = sg.col0 + (t + k * TPR) * VE;
-            }
-          }
-        }
-        if (t < sg.nx && to_f32(sg.xe) >= least) keep(key_of(to_f32(sg.xe), sg.sp.extra(t)));
-      }
-      __syncthreads();
-      const int nvectors = count[0];
-#pragma unroll 1
-      for (int i = threadIdx.x; i < min(nvectors, kCandVectors) * VE; i += TPR) {
-        const float v = to_f32(reinterpret_cast<const T*>(vectors)[i]);
-        if (v >= least) keep(key_of(v, columns[i / VE] + i % VE));
-      }
-      __syncthreads();
-      int n = count[1];
-      if (n > kCand || nvectors > kCandVectors || st.s != st.s) {  // uniform
-        n = exact_top<T, TPR>(x, a.vocab, seg, span, a.top, cand, &count[1], totals);
-      }
-#pragma unroll 1
-      for (int c = threadIdx.x; c < n; c += TPR) {
-        const u64 key = cand[c];
-        int r = 0;
-#pragma unroll 4
-        for (int j = 0; j < n; ++j) r += cand[j] > key;
-        if (r < a.top) {
-          if (segs == 1) store_top<CAP>(p, a, row, r, key, st);
-          else a.keys[unit * a.top + r] = key;
-        }
-      }
-      if (segs > 1)
-        for (int r = n + threadIdx.x; r < a.top; r += TPR) a.keys[unit * a.top + r] = 0;
-    }
-    __syncthreads();  // the shared arrays are rewritten for the workgroup's next unit
-  }
-}
-
-// Joins a row's segments: wave 0 folds the statistics in a fixed order; with
-// alternatives, the top-th largest key among the segments' j-th keys, j the
-// fewest that make top of them, bounds the row's top from below, and what
-// reaches it is placed by counting.
-constexpr int kJoinThreads = 256;
-
-template <typename T, bool CAP>
-__global__ void __launch_bounds__(kJoinThreads)
-logprob_join_kernel(const T* __restrict__ logits, int64_t ld, int segs, ScoreParams p, LogprobArgs a) {
+// A row's results from its segments' statistics and its groups' maxima. TT
+// threads a row: one wave where there are rows enough, four where there are few.
+// MAXG, CAND: room for the maxima and for the keys of what passes the bound.
+template <typename T, bool CAP, int TT, int MAXG, int CAND>
+__global__ void __launch_bounds__(TT)
+logprob_top_kernel(const T* __restrict__ logits, int64_t ld, int segs, ScoreParams p, LogprobArgs a) {
+  constexpr int VE = Vec16<T>::VE;
+  static_assert(MAXG <= 65536 && MAXG % TT == 0 && CAND >= kMaxTop, "groups in 16 bits, whole rounds");
+  __shared__ u64 cand[CAND + 1];
+  __shared__ uint16_t list[kMaxTop + kSpare];
+  __shared__ u64 totals[TT / 64];
   __shared__ RowStats whole;
-  __shared__ u64 cand[kJoinKeys];
-  __shared__ int count;
-  __shared__ u64 low;
+  __shared__ uint32_t counts[2][TT / 64];
+  __shared__ int above_of[TT / 64], at_of[TT / 64], count;
   const int64_t row = blockIdx.x;
-  const int t = threadIdx.x;
-  if (t == 0) {
-    count = 0;
-    low = 0;
+  const T* x = logits + row * ld;
+  const RowSplit<T> sp(x, a.vocab);
+  const int t = threadIdx.x, lane = t & 63;
+  const int64_t tok = t == 0 && a.tokens ? a.tokens[row] : p.ignore_index;
+  // (with an address off the 16-byte grid a row may have one vector less than its groups hold)
+  const int groups = (sp.nvec + (1 << a.shift) - 1) >> a.shift;
+  // wave w has the groups from w PER 64 on, 64 at a time
+  constexpr int W = TT / 64, PER = MAXG / TT;
+  const int wave = t / 64, first = wave * PER * 64 + lane;
+  uint32_t q[PER];  // places, 0 behind the last group (no logit has place 0)
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int at = first + i * 64;
+    q[i] = at < groups ? place_of(a.maxima[row * a.groups + at]) & kPlaceBits<T> : 0u;
   }
+  float x_tok = 0.0f;
+  if (tok != p.ignore_index && tok >= 0 && tok < a.vocab) x_tok = to_f32(x[tok]);
+  // the sum over the waves of a wave-uniform value (or the largest): two buffers in turn, one barrier each
+  int turn = 0;
+  auto over_waves = [&](uint32_t v, bool sum) {
+    if constexpr (W == 1) return v;
+    if (lane == 0) counts[turn][wave] = v;
+    __syncthreads();
+    v = counts[turn][0];
+#pragma unroll
+    for (int i = 1; i < W; ++i) v = sum ? v + counts[turn][i] : max(v, counts[turn][i]);
+    turn ^= 1;
+    return v;
+  };
+  auto number = [&](auto which) {
+    uint32_t c = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) c += __popcll(__ballot(which(q[i])));
+    return c;
+  };
+  const uint32_t top = a.top;
+  const uint32_t least_place = place_of(-INFINITY) & kPlaceBits<T>;
+  uint32_t b = least_place;
+  bool all = false;  // whether few more than top maxima reach b: all those are chosen then
+  if (groups > a.top) {
+    uint32_t high = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) high = max(high, q[i]);
+    for (int off = 32; off >= 1; off >>= 1) high = max(high, (uint32_t)__shfl_xor((int)high, off, 64));
+    high = over_waves(high, false);
+    b = 0;
+    // the top-th largest maximum, bit by bit (those above the largest's first are 0 in every place)
+    for (int bit = 31 - __builtin_clz(high | 1u); bit >= __builtin_ctz(kPlaceBits<T>) && !all; --bit) {
+      const uint32_t at = b | 1u << bit;
+      const uint32_t c = over_waves(number([&](uint32_t v) { return v >= at; }), true);
+      if (c >= top) b = at;
+      all = c >= top && c <= top + kSpare;
+    }
+    b = max(b, least_place);  // (every maximum reaches it: below it are no numbers)
+  }
+  // the chosen groups, ascending: those above b, and of those at it as many as are wanted
+  const int n_above = number([&](uint32_t v) { return v > b; }), n_at = number([&](uint32_t v) { return v == b; });
+  if (lane == 0) {
+    above_of[wave] = n_above;
+    at_of[wave] = n_at;
+  }
+  if (t == 0) count = 0;
+  __syncthreads();
+  int all_above = 0, all_at = 0, above_before = 0, at_before = 0;
+#pragma unroll
+  for (int i = 0; i < W; ++i) {
+    above_before += i < wave ? above_of[i] : 0;
+    at_before += i < wave ? at_of[i] : 0;
+    all_above += above_of[i];
+    all_at += at_of[i];
+  }
+  const int wanted = all ? all_at : min(all_at, a.top - all_above);
+  int left = max(0, wanted - at_before), to = above_before + min(at_before, wanted);
+  if (all) {  // uniform
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const u64 taken = __ballot(q[i] >= b);
+      if (q[i] >= b) list[to + lanes_before(taken)] = (uint16_t)(first + i * 64);
+      to += __popcll(taken);
+    }
+  } else {
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const u64 ties = __ballot(q[i] == b);
+    const bool take = q[i] > b || (q[i] == b && lanes_before(ties) < left);
+    const u64 taken = __ballot(take);
+    if (take) list[to + lanes_before(taken)] = (uint16_t)(first + i * 64);
+    to += __popcll(taken);
+    left = max(0, left - (int)__popcll(ties));
+  }
+  }
+  __syncthreads();
+  const Groups g{list, all_above + wanted, a.shift};
+  const float least = float_at(b < 0x80000000u ? b | ~kPlaceBits<T> : b);  // (a negative number's low bits are set)
+  // what reaches the bound in the chosen groups, or what passes it
+  bool above = false;
+  auto passes = [&](float v) { return above ? v > least : v >= least; };
+  auto gather = [&]() {
+    gather_chosen<T, TT, CAND>(x, sp, g, cand, &count, passes);
+    if (t < sp.nx && passes(to_f32(x[sp.extra(t)]))) {
+      const int at = atomicAdd(&count, 1);
+      if (at < CAND) cand[at] = key_of(to_f32(x[sp.extra(t)]), sp.extra(t));
+    }
+    __syncthreads();
+  };
   if (t < 64) {
-    int64_t tok = p.ignore_index;
-    float x_tok = 0.0f;
-    if (t == 0 && a.tokens) {
-      tok = a.tokens[row];
-      if (tok != p.ignore_index && tok >= 0 && tok < a.vocab) x_tok = to_f32(logits[row * ld + tok]);
-    }
-    RowStats st{-INFINITY, 0.0f, 0.0f};
-    for (int i = t; i < segs; i += 64) {
-      const f32x4_t q = a.part[row * segs + i];
-      st = join_stats(p, st, RowStats{q[0], q[1], q[2]});
-    }
-    st = wave_join(p, st);
+    const RowStats st = join_row(p, a.part + row * segs, segs);
     if (t == 0) {
       whole = st;
       finish_row<CAP>(p, a, row, st, tok, x_tok);
     }
   }
-  if (a.top == 0) return;
-  __syncthreads();
+  gather();
   const RowStats st = whole;
-  const u64* keys = a.keys + row * segs * a.top;
-  const int j = (a.top - 1) / segs;
-  for (int i = t; i < segs; i += kJoinThreads) cand[i] = keys[i * a.top + j];
-  __syncthreads();
-  // the rank of the bound among the segs keys: the (j + 1) segs' worth of keys above or at it number top at least
-  const int rank = (a.top - 1) / (j + 1);
-  for (int i = t; i < segs; i += kJoinThreads) {
-    const u64 key = cand[i];
-    int r = 0;
-    for (int k = 0; k < segs; ++k) r += cand[k] > key || (cand[k] == key && k < i);
-    if (r == rank) low = key;
+  int n = count;
+  const bool nan = st.s != st.s;
+  if (n > CAND && !nan) {  // uniform, as below
+    // many logits equal to the bound: those above it, and of the equal ones as
+    // many as are still wanted, by column: those before the row's vectors,
+    // those of the chosen groups, those behind
+    __syncthreads();
+    if (t == 0) count = 0;
+    above = true;
+    __syncthreads();
+    gather();
+    if (t < 64 && count < a.top) {
+      int at = count;
+      auto in_order = [&](bool equal, int col) {
+        const u64 lanes = __ballot(equal);
+        const int i = at + lanes_before(lanes);
+        if (equal && i < a.top) cand[i] = key_of(least, col);
+        at = min(a.top, at + (int)__popcll(lanes));
+      };
+      const bool ex = t < sp.nx && to_f32(x[sp.extra(t)]) == least;
+      in_order(ex && t < sp.head, t);
+      const int total = g.n << g.shift;
+      for (int i0 = 0; i0 < total && at < a.top; i0 += 64) {
+        const int i = i0 + lane, v = i < total ? (g.list[i >> g.shift] << g.shift) + (i & ((1 << g.shift) - 1)) : sp.nvec;
+        uint32_t equal = 0;  // bit e: element e of this lane's vector
+        if (v < sp.nvec) {
+          const Vec16<T> q = load16_any(x + sp.head + v * VE);
+#pragma unroll
+          for (int e = 0; e < VE; ++e) equal |= (uint32_t)(to_f32(q.e[e]) == least) << e;
+        }
+        // lanes are in the order of columns, a lane's elements follow each other
+        int before = 0, sum = 0;
+#pragma unroll
+        for (int e = 0; e < VE; ++e) {
+          const u64 lanes = __ballot(equal >> e & 1);
+          before += lanes_before(lanes);
+          sum += __popcll(lanes);
+        }
+        int k = at + before;
+        for (uint32_t rest = equal; rest && k < a.top; rest &= rest - 1, ++k)
+          cand[k] = key_of(least, sp.head + v * VE + __builtin_ctz(rest));
+        at = min(a.top, at + sum);
+      }
+      in_order(ex && t >= sp.head, sp.extra(t));
+      if (t == 0) count = at;
+    }
+    __syncthreads();
+    n = count;
   }
+  if (n > CAND || nan) n = exact_top<T, TT>(x, a.vocab, a.top, cand, &count, totals);
+  if (t == 0) cand[n] = 0;
   __syncthreads();
-  const u64 least = low;
-  for (int i = t; i < segs * a.top; i += kJoinThreads) {
-    const u64 key = keys[i];
-    if (key >= least && key != 0) cand[atomicAdd(&count, 1)] = key;
-  }
-  __syncthreads();
-  const int n = count;
-#pragma unroll 1
-  for (int c = t; c < n; c += kJoinThreads) {
+  for (int c = t; c < n; c += TT) {
     const u64 key = cand[c];
     int r = 0;
 #pragma unroll 4
-    for (int k = 0; k < n; ++k) r += cand[k] > key;
+    for (int i = 0; i < n; i += 2) r += (cand[i] > key) + (cand[i + 1] > key);
     if (r < a.top) store_top<CAP>(p, a, row, r, key, st);
   }
 }
@@ -429,16 +555,32 @@ logprob_grad_kernel(const T* __restrict__ logits, const int64_t* __restrict__ to
   }
 }
 
+// The groups of a row whose maxima are kept: 64 vectors where that leaves
+// twice the alternatives and 256 of them, else 8 (one line) where that leaves
+// twice the alternatives, else single vectors. Up to kMaxGroups.
+constexpr int kMaxGroups = 4096;
+
+int group_shift(int64_t nvec, int top) {
+  if (nvec / 64 >= std::max(2 * top, 256)) return 6;
+  return nvec / 8 >= 2 * top ? 3 : 0;
+}
+
 struct Workspace {
-  size_t part, keys, total;
+  int shift, groups;
+  size_t part, maxima, total;
 };
 
-Workspace workspace(int64_t rows, const ScorePlan& pl, int top) {
+Workspace workspace(int64_t rows, int64_t vocab, int ve, const ScorePlan& pl, int top) {
   auto up = [](size_t v) { return (v + 255) & ~(size_t)255; };
-  Workspace w{0, 0, 0};
-  if (pl.segs == 1 || rows <= 0) return w;
-  w.keys = up((size_t)rows * pl.segs * sizeof(f32x4_t));
-  w.total = w.keys + up((size_t)rows * pl.segs * top * sizeof(u64));
+  Workspace w{0, 0, 0, 0, 0};
+  if ((pl.segs == 1 && top == 0) || rows <= 0) return w;
+  w.maxima = w.total = up((size_t)rows * pl.segs * sizeof(f32x4_t));
+  if (top > 0) {
+    const int64_t nvec = std::max<int64_t>(1, vocab / ve);
+    w.shift = group_shift(nvec, top);
+    w.groups = (int)((nvec + (1 << w.shift) - 1) >> w.shift);
+    w.total += up((size_t)rows * w.groups * sizeof(float));
+  }
   return w;
 }
 
@@ -446,13 +588,27 @@ template <typename T, bool CAP>
 void launch_fwd(const void* logits, int64_t rows, int64_t ld, const ScorePlan& pl, const ScoreParams& p,
                 const LogprobArgs& a, hipStream_t s) {
   const T* x = static_cast<const T*>(logits);
-  const dim3 grid(row_grid(rows * pl.segs));
-#define GO(VPT, TPR)                                                                                           \
-  (a.top ? logprob_segment_kernel<T, VPT, TPR, CAP, true><<<grid, dim3(TPR), 0, s>>>(x, rows, ld, pl.segs, pl.span, p, a) \
-         : logprob_segment_kernel<T, VPT, TPR, CAP, false><<<grid, dim3(TPR), 0, s>>>(x, rows, ld, pl.segs, pl.span, p, a))
-  AK_SEGMENT_DISPATCH(pl.span, GO);
+  const dim3 grid(row_grid(rows * pl.segs)), each((unsigned)rows);
+  auto segments = [&](auto shift) {
+    constexpr int SHIFT = decltype(shift)::value;
+#define GO(VPT, TPR) logprob_segment_kernel<T, VPT, TPR, CAP, SHIFT><<<grid, dim3(TPR), 0, s>>>(x, rows, ld, pl.segs, pl.span, p, a)
+    AK_SEGMENT_DISPATCH(pl.span, GO);
 #undef GO
-  if (pl.segs > 1) logprob_join_kernel<T, CAP><<<dim3((unsigned)rows), dim3(a.top ? kJoinThreads : 64), 0, s>>>(x, ld, pl.segs, p, a);
+  };
+  if (!a.part) segments(std::integral_constant<int, kHere>());
+  else if (a.top == 0) segments(std::integral_constant<int, kPart>());
+  else if (a.shift == 0) segments(std::integral_constant<int, 0>());
+  else if (a.shift == 3) segments(std::integral_constant<int, 3>());
+  else segments(std::integral_constant<int, 6>());
+  if (!a.part) return;
+  const bool small = a.top <= 128 && a.groups <= 1024 && a.groups >= 2 * a.top;
+#define TOP(TT, MAXG, CAND) logprob_top_kernel<T, CAP, TT, MAXG, CAND><<<each, dim3(TT), 0, s>>>(x, ld, pl.segs, p, a)
+  if (a.top == 0) logprob_join_kernel<T, CAP><<<each, dim3(64), 0, s>>>(x, ld, pl.segs, p, a);
+  else if (rows >= 512 && small && a.groups <= 512) TOP(64, 512, 512);
+  else if (rows >= 512 && small) TOP(64, 1024, 512);
+  else if (small) TOP(256, 1024, 512);
+  else TOP(256, kMaxGroups, 2048);
+#undef TOP
 }
 
 template <typename T, bool CAP>
@@ -478,7 +634,7 @@ void launch_bwd(const void* logits, const int64_t* tokens, const float* stats, c
 extern "C" size_t ak_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int top_k, int dtype) {
   const int esz = ak_dtype_size(dtype);
   if (rows <= 0 || vocab <= 0 || vocab > ak::kScoreVocab || top_k < 0 || top_k > ak::kMaxTop || esz == 0) return 0;
-  return ak::workspace(rows, ak::score_plan(rows, vocab, 16 / esz, top_k), top_k).total;
+  return ak::workspace(rows, vocab, 16 / esz, ak::score_plan(rows, vocab, 16 / esz), top_k).total;
 }
 
 extern "C" int ak_token_logprobs_fwd(const void* logits, const int64_t* tokens, float* logprobs, float* entropy,
@@ -495,13 +651,15 @@ extern "C" int ak_token_logprobs_fwd(const void* logits, const int64_t* tokens, 
   if (!logits || (tokens && !logprobs) || (top_k > 0 && (!top_logprobs || !top_ids)))
     return ak_set_error(AK_ERR_INVALID_ARG, "%s: null pointer", name);
   if (stats && !ak::aligned16(stats)) return ak_set_error(AK_ERR_INVALID_ARG, "%s: stats must be 16-byte aligned", name);
-  const ak::ScorePlan pl = ak::score_plan(rows, vocab, 16 / ak_dtype_size(dtype), top_k);
-  const ak::Workspace w = ak::workspace(rows, pl, top_k);
+  const int ve = 16 / ak_dtype_size(dtype);
+  const ak::ScorePlan pl = ak::score_plan(rows, vocab, ve);
+  const ak::Workspace w = ak::workspace(rows, vocab, ve, pl, top_k);
   if (workspace_bytes < w.total || (w.total && (!workspace || !ak::aligned16(workspace))))
     return ak_set_error(AK_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed (16-byte aligned)", name, workspace_bytes, w.total);
   char* ws = static_cast<char*>(workspace);
   const ak::LogprobArgs a{tokens, logprobs, entropy, reinterpret_cast<ak::f32x4_t*>(stats), top_logprobs, top_ids,
-                          reinterpret_cast<ak::f32x4_t*>(ws), reinterpret_cast<ak::u64*>(ws + w.keys), top_k, (int)vocab};
+                          w.total ? reinterpret_cast<ak::f32x4_t*>(ws) : nullptr, reinterpret_cast<float*>(ws + w.maxima),
+                          top_k, (int)vocab, w.groups, w.shift};
   const ak::ScoreParams p = ak::score_params(temperature, softcap, ignore_index);
   hipStream_t s = ak_stream(stream);
   auto go = [&](auto t) {

@@ -104,7 +104,7 @@ __device__ __forceinline__ void finish_row(const ScoreParams& p, const TeacherAr
 
 // One workgroup per segment (units by grid stride; the loop bound is uniform).
 template <typename T, int VPT, int TPR, bool CAP>
-__global__ void __launch_bounds__(TPR, VPT == 8 ? 8 : 1)
+__global__ void __launch_bounds__(TPR, AK_SEGMENT_WAVES(VPT))
 distill_segment_kernel(const T* __restrict__ logits, int64_t rows, int64_t ld, int segs, int span, ScoreParams p,
                        TeacherArgs a, float* __restrict__ losses, f32x4_t* __restrict__ stats,
                        f32x4_t* __restrict__ part) {
@@ -301,7 +301,7 @@ int check(const char* name, const void* logits, const void* teacher, const int64
 extern "C" size_t ak_topk_distill_workspace_bytes(int64_t rows, int64_t vocab, int dtype) {
   const int esz = ak_dtype_size(dtype);
   if (rows <= 0 || vocab <= 0 || vocab > ak::kScoreVocab || esz == 0) return 0;
-  return ak::part_bytes(rows, ak::score_plan(rows, vocab, 16 / esz, 0));
+  return ak::part_bytes(rows, ak::score_plan(rows, vocab, 16 / esz));
 }
 
 extern "C" int ak_topk_distill_fwd(const void* logits, const void* teacher_logits, const int64_t* teacher_ids,
@@ -318,7 +318,7 @@ extern "C" int ak_topk_distill_fwd(const void* logits, const void* teacher_logit
   if (rows == 0 && !loss) return AK_OK;
   hipStream_t s = ak_stream(stream);
   if (rows > 0) {
-    const ak::ScorePlan pl = ak::score_plan(rows, vocab, 16 / ak_dtype_size(dtype), 0);
+    const ak::ScorePlan pl = ak::score_plan(rows, vocab, 16 / ak_dtype_size(dtype));
     const size_t need = ak::part_bytes(rows, pl);
     if (workspace_bytes < need || (need && (!workspace || !ak::aligned16(workspace))))
       return ak_set_error(AK_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed (16-byte aligned)", name, workspace_bytes, need);

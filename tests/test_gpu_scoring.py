@@ -141,6 +141,27 @@ def test_logprobs_temperature_and_softcap(rows, temperature, softcap):
     check_logprobs(x, t, temperature, softcap, top_k=10)
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("vocab,top_k", [(2500, 7), (5003, 100), (9000, 256), (17001, 64), (33000, 5), (60000, 128), (70001, 256)])
+def test_logprobs_top_of_many_rows(dtype, vocab, top_k):
+    """Uncut rows of every width: each way a thread holds a row, and its groups' maxima."""
+    need_gpu()
+    say("logprobs many", dtype, vocab, top_k)
+    from kernels.hip.token_logprobs import kernel_fn
+    x = logits_of(600, vocab, dtype, vocab)
+    x[1] = x[1].round()  # many ties
+    t = torch.randint(0, vocab, (600,), generator=torch.Generator().manual_seed(7)).to(DEV)
+    for rows in (600, 300):  # one wave a row, four
+        r = kernel_fn(x[:rows], t[:rows], top_k=top_k)
+        # exact ids of all rows: the logit's place among the numbers, then the column
+        bits = (x[:rows].float() + 0.0).view(torch.int32).to(torch.int64)
+        key = (torch.where(bits < 0, bits ^ 0x7FFFFFFF, bits) << 32) - torch.arange(vocab, device=DEV)
+        assert torch.equal(r.top_ids, key.topk(top_k, dim=1).indices)
+        logp = torch.log_softmax(x[:rows].double(), 1)
+        close(r.top_logprobs, logp.gather(1, r.top_ids).cpu(), 2 * ROW, "top_logprobs")
+        close(r.logprobs, logp.gather(1, t[:rows, None])[:, 0].cpu(), 2 * ROW, "logprobs")
+
+
 def test_logprobs_without_tokens():
     need_gpu()
     check_logprobs(logits_of(6, 3000, torch.float32, 1), None, top_k=4)

@@ -271,7 +271,7 @@ def test_library_refusals(lib):
     assert fwd(tokens=16) == -1 and fwd(top=2) == -1 and says(b"null")
     assert fwd(stats=8) == -1 and says(b"aligned")
     need = lib.ak_token_logprobs_workspace_bytes(2, 50257, 20, 0)
-    assert need > 0 and lib.ak_token_logprobs_workspace_bytes(4096, 50257, 20, 2) == 0
+    assert need > 0 and lib.ak_token_logprobs_workspace_bytes(4096, 50257, 0, 2) == 0
     plain = lib.ak_token_logprobs_workspace_bytes(2, 50257, 0, 0)
     assert fwd(rows=2, vocab=50257, ld=50257, nbytes=plain - 1, ws=256) == -4 and says(b"workspace")
     assert fwd(rows=2, vocab=50257, ld=50257, nbytes=plain) == -4 and 0 < plain < need
