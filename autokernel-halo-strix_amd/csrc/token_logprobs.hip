@@ -35,6 +35,7 @@ namespace ak {
 namespace {
 
 typedef unsigned long long u64;
+typedef u64 u64x2 __attribute__((ext_vector_type(2)));
 
 // Places of floats among the numbers, as unsigned integers; NaN first.
 __device__ __forceinline__ uint32_t place_of(float x) {
@@ -209,12 +210,12 @@ __device__ __forceinline__ int lanes_sum_before(int v, int& all) {
 }
 
 // Gathers the keys of the logits of the chosen groups that `passes` takes, in
-// any order; the loads of eight vectors a thread are in flight before the first
-// is used. Reached by whole waves; what `count` passes CAND by is left out.
+// any order; where a wave has the row alone, the loads of eight vectors a thread
+// are in flight before the first is used. Reached by whole waves; what `count` passes CAND by is left out.
 template <typename T, int TT, int CAND, typename F>
 __device__ __forceinline__ void gather_chosen(const T* __restrict__ row, const RowSplit<T>& sp, const Groups& g, u64* cand,
                                               int* count, F passes) {
-  constexpr int VE = Vec16<T>::VE, U = 8;
+  constexpr int VE = Vec16<T>::VE, U = TT > 64 ? 2 : 8;
   const int total = g.n << g.shift, lane = threadIdx.x & 63;
   for (int i0 = threadIdx.x - lane; i0 < total; i0 += U * TT) {
     Vec16<T> q[U];
@@ -325,108 +326,86 @@ template <typename T, bool CAP, int TT, int MAXG, int CAND>
 __global__ void __launch_bounds__(TT)
 logprob_top_kernel(const T* __restrict__ logits, int64_t ld, int segs, ScoreParams p, LogprobArgs a) {
   constexpr int VE = Vec16<T>::VE;
-  static_assert(MAXG <= 65536 && MAXG % TT == 0 && CAND >= kMaxTop, "groups in 16 bits, whole rounds");
-  __shared__ u64 cand[CAND + 1];
+  static_assert(MAXG <= 65536 && MAXG % 64 == 0 && CAND >= kMaxTop, "groups in 16 bits, whole rounds");
+  __shared__ __attribute__((aligned(16))) u64 cand[CAND + 2];
   __shared__ uint16_t list[kMaxTop + kSpare];
   __shared__ u64 totals[TT / 64];
   __shared__ RowStats whole;
-  __shared__ uint32_t counts[2][TT / 64];
-  __shared__ int above_of[TT / 64], at_of[TT / 64], count;
+  __shared__ uint32_t bound;
+  __shared__ int count, chosen;
   const int64_t row = blockIdx.x;
   const T* x = logits + row * ld;
   const RowSplit<T> sp(x, a.vocab);
   const int t = threadIdx.x, lane = t & 63;
-  const int64_t tok = t == 0 && a.tokens ? a.tokens[row] : p.ignore_index;
   // (with an address off the 16-byte grid a row may have one vector less than its groups hold)
   const int groups = (sp.nvec + (1 << a.shift) - 1) >> a.shift;
-  // wave w has the groups from w PER 64 on, 64 at a time
-  constexpr int W = TT / 64, PER = MAXG / TT;
-  const int wave = t / 64, first = wave * PER * 64 + lane;
-  uint32_t q[PER];  // places, 0 behind the last group (no logit has place 0)
-#pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int at = first + i * 64;
-    q[i] = at < groups ? place_of(a.maxima[row * a.groups + at]) & kPlaceBits<T> : 0u;
-  }
-  float x_tok = 0.0f;
-  if (tok != p.ignore_index && tok >= 0 && tok < a.vocab) x_tok = to_f32(x[tok]);
-  // the sum over the waves of a wave-uniform value (or the largest): two buffers in turn, one barrier each
-  int turn = 0;
-  auto over_waves = [&](uint32_t v, bool sum) {
-    if constexpr (W == 1) return v;
-    if (lane == 0) counts[turn][wave] = v;
-    __syncthreads();
-    v = counts[turn][0];
-#pragma unroll
-    for (int i = 1; i < W; ++i) v = sum ? v + counts[turn][i] : max(v, counts[turn][i]);
-    turn ^= 1;
-    return v;
-  };
-  auto number = [&](auto which) {
-    uint32_t c = 0;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) c += __popcll(__ballot(which(q[i])));
-    return c;
-  };
-  const uint32_t top = a.top;
   const uint32_t least_place = place_of(-INFINITY) & kPlaceBits<T>;
-  uint32_t b = least_place;
-  bool all = false;  // whether few more than top maxima reach b: all those are chosen then
-  if (groups > a.top) {
-    uint32_t high = 0;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) high = max(high, q[i]);
-    for (int off = 32; off >= 1; off >>= 1) high = max(high, (uint32_t)__shfl_xor((int)high, off, 64));
-    high = over_waves(high, false);
-    b = 0;
-    // the top-th largest maximum, bit by bit (those above the largest's first are 0 in every place)
-    for (int bit = 31 - __builtin_clz(high | 1u); bit >= __builtin_ctz(kPlaceBits<T>) && !all; --bit) {
-      const uint32_t at = b | 1u << bit;
-      const uint32_t c = over_waves(number([&](uint32_t v) { return v >= at; }), true);
-      if (c >= top) b = at;
-      all = c >= top && c <= top + kSpare;
-    }
-    b = max(b, least_place);  // (every maximum reaches it: below it are no numbers)
-  }
-  // the chosen groups, ascending: those above b, and of those at it as many as are wanted
-  const int n_above = number([&](uint32_t v) { return v > b; }), n_at = number([&](uint32_t v) { return v == b; });
-  if (lane == 0) {
-    above_of[wave] = n_above;
-    at_of[wave] = n_at;
-  }
-  if (t == 0) count = 0;
-  __syncthreads();
-  int all_above = 0, all_at = 0, above_before = 0, at_before = 0;
-#pragma unroll
-  for (int i = 0; i < W; ++i) {
-    above_before += i < wave ? above_of[i] : 0;
-    at_before += i < wave ? at_of[i] : 0;
-    all_above += above_of[i];
-    all_at += at_of[i];
-  }
-  const int wanted = all ? all_at : min(all_at, a.top - all_above);
-  int left = max(0, wanted - at_before), to = above_before + min(at_before, wanted);
-  if (all) {  // uniform
+  constexpr int kStatsWave = TT > 64 ? 64 : 0;  // the threads that fold the statistics, meanwhile where there are others
+  if (t < 64) {
+    constexpr int PER = MAXG / 64;
+    uint32_t q[PER];  // places, 0 behind the last group (no logit has place 0)
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const u64 taken = __ballot(q[i] >= b);
-      if (q[i] >= b) list[to + lanes_before(taken)] = (uint16_t)(first + i * 64);
-      to += __popcll(taken);
+      const int at = i * 64 + lane;
+      q[i] = at < groups ? __builtin_bit_cast(uint32_t, a.maxima[row * a.groups + at]) : 0u;
     }
-  } else {
+    uint32_t high = 0;
 #pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const u64 ties = __ballot(q[i] == b);
-    const bool take = q[i] > b || (q[i] == b && lanes_before(ties) < left);
-    const u64 taken = __ballot(take);
-    if (take) list[to + lanes_before(taken)] = (uint16_t)(first + i * 64);
-    to += __popcll(taken);
-    left = max(0, left - (int)__popcll(ties));
+    for (int i = 0; i < PER; ++i) {
+      q[i] = i * 64 + lane < groups ? place_of(__builtin_bit_cast(float, q[i])) & kPlaceBits<T> : 0u;
+      high = max(high, q[i]);
+    }
+    auto number = [&](auto which) {
+      int c = 0;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) c += __popcll(__ballot(which(q[i])));
+      return c;
+    };
+    uint32_t b = least_place;
+    bool all = false;  // whether few more than top maxima reach b: all those are chosen then
+    if (groups > a.top) {
+      for (int off = 32; off >= 1; off >>= 1) high = max(high, (uint32_t)__shfl_xor((int)high, off, 64));
+      b = 0;
+      // the top-th largest maximum, bit by bit (those above the largest's first are 0 in every place)
+      for (int bit = 31 - __builtin_clz(high | 1u); bit >= __builtin_ctz(kPlaceBits<T>) && !all; --bit) {
+        const uint32_t at = b | 1u << bit;
+        const int c = number([&](uint32_t v) { return v >= at; });
+        if (c >= a.top) b = at;
+        all = c >= a.top && c <= a.top + kSpare;
+      }
+      b = max(b, least_place);  // (every maximum reaches it: below it are no numbers)
+    }
+    // the chosen groups, ascending: those that reach b, or those above it and as
+    // many of those at it as are wanted
+    int left = all ? MAXG : a.top - number([&](uint32_t v) { return v > b; }), to = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const u64 ties = __ballot(q[i] == b);
+      const bool take = q[i] > b || (q[i] == b && lanes_before(ties) < left);
+      const u64 taken = __ballot(take);
+      if (take) list[to + lanes_before(taken)] = (uint16_t)(i * 64 + lane);
+      to += __popcll(taken);
+      left = max(0, left - (int)__popcll(ties));
+    }
+    if (lane == 0) {
+      chosen = to;
+      bound = b;
+      count = 0;
+    }
   }
+  if (t >= kStatsWave && t < kStatsWave + 64) {
+    const int64_t tok = lane == 0 && a.tokens ? a.tokens[row] : p.ignore_index;
+    float x_tok = 0.0f;
+    if (tok != p.ignore_index && tok >= 0 && tok < a.vocab) x_tok = to_f32(x[tok]);
+    const RowStats st = join_row(p, a.part + row * segs, segs);
+    if (lane == 0) {
+      whole = st;
+      finish_row<CAP>(p, a, row, st, tok, x_tok);
+    }
   }
   __syncthreads();
-  const Groups g{list, all_above + wanted, a.shift};
-  const float least = float_at(b < 0x80000000u ? b | ~kPlaceBits<T> : b);  // (a negative number's low bits are set)
+  const Groups g{list, chosen, a.shift};
+  const float least = float_at(bound < 0x80000000u ? bound | ~kPlaceBits<T> : bound);  // (a negative number's low bits are set)
   // what reaches the bound in the chosen groups, or what passes it
   bool above = false;
   auto passes = [&](float v) { return above ? v > least : v >= least; };
@@ -438,13 +417,6 @@ logprob_top_kernel(const T* __restrict__ logits, int64_t ld, int segs, ScorePara
     }
     __syncthreads();
   };
-  if (t < 64) {
-    const RowStats st = join_row(p, a.part + row * segs, segs);
-    if (t == 0) {
-      whole = st;
-      finish_row<CAP>(p, a, row, st, tok, x_tok);
-    }
-  }
   gather();
   const RowStats st = whole;
   int n = count;
@@ -497,13 +469,16 @@ logprob_top_kernel(const T* __restrict__ logits, int64_t ld, int segs, ScorePara
     n = count;
   }
   if (n > CAND || nan) n = exact_top<T, TT>(x, a.vocab, a.top, cand, &count, totals);
-  if (t == 0) cand[n] = 0;
+  if (t < 2) cand[n + t] = 0;
   __syncthreads();
   for (int c = t; c < n; c += TT) {
     const u64 key = cand[c];
     int r = 0;
 #pragma unroll 4
-    for (int i = 0; i < n; i += 2) r += (cand[i] > key) + (cand[i + 1] > key);
+    for (int i = 0; i < n; i += 2) {
+      const u64x2 two = *reinterpret_cast<const u64x2*>(cand + i);
+      r += (two[0] > key) + (two[1] > key);
+    }
     if (r < a.top) store_top<CAP>(p, a, row, r, key, st);
   }
 }
@@ -601,13 +576,23 @@ void launch_fwd(const void* logits, int64_t rows, int64_t ld, const ScorePlan& p
   else if (a.shift == 3) segments(std::integral_constant<int, 3>());
   else segments(std::integral_constant<int, 6>());
   if (!a.part) return;
-  const bool small = a.top <= 128 && a.groups <= 1024 && a.groups >= 2 * a.top;
 #define TOP(TT, MAXG, CAND) logprob_top_kernel<T, CAP, TT, MAXG, CAND><<<each, dim3(TT), 0, s>>>(x, ld, pl.segs, p, a)
-  if (a.top == 0) logprob_join_kernel<T, CAP><<<each, dim3(64), 0, s>>>(x, ld, pl.segs, p, a);
-  else if (rows >= 512 && small && a.groups <= 512) TOP(64, 512, 512);
-  else if (rows >= 512 && small) TOP(64, 1024, 512);
-  else if (small) TOP(256, 1024, 512);
-  else TOP(256, kMaxGroups, 2048);
+  if (a.top == 0) {
+    logprob_join_kernel<T, CAP><<<each, dim3(64), 0, s>>>(x, ld, pl.segs, p, a);
+    return;
+  }
+  // Room for the keys that reach the bound: about 1.4 top of twice top groups,
+  // fewer of more; where a row has less than twice top groups (single vectors
+  // then) all of its at most 4096 logits may. One wave a row where every CU has
+  // two, four waves for fewer rows and the widest.
+  const bool few = rows < 512;
+  if (a.groups < 2 * a.top || a.groups > 2048) TOP(256, kMaxGroups, 2048);
+  else if (a.groups > 1024 || a.top > 128) {
+    if (few) TOP(256, 2048, 1024);
+    else TOP(64, 2048, 1024);
+  } else if (few) TOP(256, 1024, 512);
+  else if (a.groups > 512) TOP(64, 1024, 512);
+  else TOP(64, 512, 512);
 #undef TOP
 }
 
