@@ -28,6 +28,7 @@ typedef float f32x4_t __attribute__((ext_vector_type(4)));
 // What the statistics mean: the capped, tempered logits.
 struct ScoreParams {
   float cap, inv_cap;  // softcap (with CAP)
+  float k2;            // 2 log2(e) / softcap
   float c2;            // log2(e) / temperature
   float inv_t;         // 1 / temperature
   int64_t ignore_index;
@@ -37,6 +38,7 @@ inline ScoreParams score_params(float temperature, float softcap, int64_t ignore
   ScoreParams p;
   p.cap = softcap;
   p.inv_cap = softcap > 0.0f ? 1.0f / softcap : 0.0f;
+  p.k2 = softcap > 0.0f ? (float)(2.8853900817779268 / (double)softcap) : 0.0f;
   p.c2 = (float)(1.4426950408889634 / (double)temperature);
   p.inv_t = 1.0f / temperature;
   p.ignore_index = ignore_index;
@@ -46,6 +48,18 @@ inline ScoreParams score_params(float temperature, float softcap, int64_t ignore
 template <bool CAP>
 __device__ __forceinline__ float score(const ScoreParams& p, float x) {
   return CAP ? p.cap * tanh_f32(x * p.inv_cap) : x;
+}
+
+// The score of one of a row's many logits of type T. Half-precision logits are
+// rounded to 2^-9 or 2^-12 of themselves already, so their cap takes the short
+// form cap - 2 cap r, r = 1 / (1 + exp(2 x / cap)), within 2^-22 cap of the exact
+// one (5 instructions for tanh_f32's 14: [4096, 50257] bf16 with a softcap
+// SHORT_FORM_US).
+template <typename T, bool CAP>
+__device__ __forceinline__ float many_score(const ScoreParams& p, float x) {
+  if constexpr (CAP && !std::is_same<T, float>::value)
+    return fmaf(-2.0f * p.cap, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * p.k2)), p.cap);
+  return score<CAP>(p, x);
 }
 
 // (m, s, u) of a row or a segment of one.
@@ -244,7 +258,7 @@ struct Segment {
     const float off = m == -INFINITY ? 0.0f : m;
     s = u = 0.0f;
     each([&](float x, int) {
-      const float t = (score<CAP>(p, x) - off) * p.c2;
+      const float t = (many_score<T, CAP>(p, x) - off) * p.c2;
       const float e = __builtin_amdgcn_exp2f(t);
       s += e;
       // 2^t is 0 from -150 on, and t may be -inf there
@@ -292,9 +306,14 @@ inline ScorePlan score_plan(int64_t rows, int64_t vocab, int ve) {
 // ---------------------------------------------------------------------------
 constexpr int kGradThreads = 256;
 
-// d(score / temperature) / d(logit), and the score.
-template <bool CAP>
+// d(score / temperature) / d(logit), and the score (as many_score).
+template <typename T, bool CAP>
 __device__ __forceinline__ float score_and_slope(const ScoreParams& p, float x, float& slope) {
+  if constexpr (CAP && !std::is_same<T, float>::value) {
+    const float r = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * p.k2));
+    slope = 4.0f * p.inv_t * r * (1.0f - r);
+    return fmaf(-2.0f * p.cap, r, p.cap);
+  }
   if constexpr (CAP) {
     const float th = tanh_f32(x * p.inv_cap);
     slope = p.inv_t * (1.0f - th * th);
@@ -304,12 +323,13 @@ __device__ __forceinline__ float score_and_slope(const ScoreParams& p, float x, 
   return x;
 }
 
-// out[v] = f(x[v]) over the row's vectors [v0, v1) and, with `ends`, the
-// elements around the vectors; U vectors of a thread are loaded before the
-// first is used.
-template <typename T, bool NT, int U, typename F>
+// The gradient of the row's vectors [v0, v1) and, with `ends`, of the elements
+// around the vectors: g.many(x) of each logit, and g.patch(col, v - v0, o) may
+// change a vector of results; g.one(x, col, i) of single element i. U vectors of
+// a thread are loaded before the first is used.
+template <typename T, bool NT, int U, typename G>
 __device__ __forceinline__ void map_row(const T* __restrict__ row, T* __restrict__ out, int vocab, int v0, int v1,
-                                        bool ends, F f) {
+                                        bool ends, const G& g) {
   constexpr int VE = Vec16<T>::VE;
   const RowSplit<T> sp(row, vocab);
   const int t = threadIdx.x;
@@ -320,7 +340,8 @@ __device__ __forceinline__ void map_row(const T* __restrict__ row, T* __restrict
   auto one = [&](const Vec16<T>& x, int v) {
     Vec16<T> o;
 #pragma unroll
-    for (int e = 0; e < VE; ++e) o.e[e] = from_f32<T>(f(to_f32(x.e[e])));
+    for (int e = 0; e < VE; ++e) o.e[e] = from_f32<T>(g.many(to_f32(x.e[e])));
+    g.patch(x, sp.head + v * VE, v - v0, o);
     if (NT) store16_any_nt(ov + (int64_t)v * VE, o);
     else store16_any(ov + (int64_t)v * VE, o);
   };
@@ -335,31 +356,23 @@ __device__ __forceinline__ void map_row(const T* __restrict__ row, T* __restrict
   for (; v < v1; v += kGradThreads) one(ld(rv + (int64_t)v * VE), v);
   if (ends && t < sp.nx) {
     const int c = sp.extra(t);
-    out[c] = from_f32<T>(f(to_f32(row[c])));
+    out[c] = from_f32<T>(g.one(to_f32(row[c]), c, t));
   }
 }
 
-// Whether map_row wrote column c for these vectors.
-template <typename T>
-__device__ __forceinline__ bool wrote_column(const T* row, int vocab, int v0, int v1, bool ends, int c) {
-  const RowSplit<T> sp(row, vocab);
-  const int v = c - sp.head;
-  if (v < 0 || v >= sp.nvec * Vec16<T>::VE) return ends;
-  return v / Vec16<T>::VE >= v0 && v / Vec16<T>::VE < v1;
-}
-
-// Between map_row's stores and another thread's store to one of the same
-// elements: the workgroup's stores have left before any wave goes on.
-__device__ __forceinline__ void stores_done() {
-  __builtin_amdgcn_s_waitcnt(0);
-  __syncthreads();
-}
+// A row without a gradient, whatever it holds.
+struct ZeroRow {
+  __device__ __forceinline__ float many(float) const { return 0.0f; }
+  template <typename V>
+  __device__ __forceinline__ void patch(const V&, int, int, V&) const {}
+  __device__ __forceinline__ float one(float, int, int) const { return 0.0f; }
+};
 
 // Spans of the gradient's grid: rounds of four vectors a thread where a row is
 // that wide, so that few rows fill the GPU too.
 inline ScorePlan grad_plan(int64_t vocab, int ve) {
   const int64_t nvec = vocab / ve;
-  const int64_t n = std::max<int64_t>(1, nvec / (4 * kGradThreads));
+  const int64_t n = std::max<int64_t>(1, nvec / (4 * kGradThreads));  // (spans below 8 kGradThreads vectors)
   return {(int)n, (int)((nvec + n - 1) / n)};
 }
 

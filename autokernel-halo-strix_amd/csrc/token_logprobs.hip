@@ -483,9 +483,34 @@ logprob_top_kernel(const T* __restrict__ logits, int64_t ld, int segs, ScorePara
   }
 }
 
+// -(g + e (ln p + H)) = c0 + c1 log2 p, and g for the given token beside it.
+template <typename T, bool CAP>
+struct LogprobRow {
+  const ScoreParams& p;
+  float m, l2, c0, c1, g;
+  int token;
+  __device__ __forceinline__ float many(float x) const {
+    float slope;
+    const float y = score_and_slope<T, CAP>(p, x, slope);
+    const float lp = (y - m) * p.c2 - l2;
+    // p is 0 from -150 on, and log2 p may be -inf there
+    return __builtin_amdgcn_exp2f(lp) * fmaf(c1, fmaxf(lp, -1000.0f), c0) * slope;
+  }
+  __device__ __forceinline__ float one(float x, int col, int) const {
+    float slope;
+    score_and_slope<T, CAP>(p, x, slope);
+    return col == token ? fmaf(g, slope, many(x)) : many(x);
+  }
+  __device__ __forceinline__ void patch(const Vec16<T>& x, int col, int, Vec16<T>& o) const {
+    if ((unsigned)(token - col) >= (unsigned)Vec16<T>::VE) return;
+#pragma unroll
+    for (int e = 0; e < Vec16<T>::VE; ++e)
+      if (col + e == token) o.e[e] = from_f32<T>(one(to_f32(x.e[e]), col + e, 0));
+  }
+};
+
 // The gradient from the forward's statistics; blockIdx.y takes `span` vectors
-// of the row. The given token's entry is written again, with its own term,
-// once the row's others have left.
+// of the row.
 template <typename T, bool CAP, bool NT, int U>
 __global__ void __launch_bounds__(kGradThreads)
 logprob_grad_kernel(const T* __restrict__ logits, const int64_t* __restrict__ tokens, const f32x4_t* __restrict__ stats,
@@ -501,32 +526,14 @@ logprob_grad_kernel(const T* __restrict__ logits, const int64_t* __restrict__ to
     const bool ignored = tokens && tok == p.ignore_index;
     const bool bad = tokens && !ignored && (tok < 0 || tok >= vocab);
     const bool empty = st[0] == -INFINITY && st[1] == 0.0f;
-    if (ignored || empty) {  // whatever the row holds
-      map_row<T, NT, 1>(x, gx, vocab, v0, v1, ends, [](float) { return 0.0f; });
+    if (ignored || empty) {
+      map_row<T, NT, 1>(x, gx, vocab, v0, v1, ends, ZeroRow());
       continue;
     }
     const float g = bad ? NAN : (tokens && g_logprobs ? g_logprobs[row] : 0.0f);
     const float e = g_entropy ? g_entropy[row] : 0.0f;
-    const float m = st[0], l2 = st[1];
-    // -(g + e (ln p + H)) = c0 + c1 log2 p
-    const float c0 = -fmaf(e, st[2], g), c1 = -e * kLn2;
-    auto dense = [&](float v) {
-      float slope;
-      const float y = score_and_slope<CAP>(p, v, slope);
-      const float lp = (y - m) * p.c2 - l2;
-      // p is 0 from -150 on, and log2 p may be -inf there
-      return __builtin_amdgcn_exp2f(lp) * fmaf(c1, fmaxf(lp, -1000.0f), c0) * slope;
-    };
-    map_row<T, NT, U>(x, gx, vocab, v0, v1, ends, dense);
-    if (tokens && !bad && wrote_column(x, vocab, v0, v1, ends, (int)tok)) {  // uniform
-      stores_done();
-      if (threadIdx.x == 0) {
-        float slope;
-        const float v = to_f32(x[tok]);
-        score_and_slope<CAP>(p, v, slope);
-        gx[tok] = from_f32<T>(fmaf(g, slope, dense(v)));
-      }
-    }
+    const LogprobRow<T, CAP> f{p, st[0], st[1], -fmaf(e, st[2], g), -e * kLn2, g, tokens && !bad ? (int)tok : -1};
+    map_row<T, NT, U>(x, gx, vocab, v0, v1, ends, f);
   }
 }
 

@@ -36,27 +36,40 @@ __device__ __forceinline__ float teacher_logit(const TeacherArgs& a, int64_t row
   return to_f32(static_cast<const bf16*>(a.logits)[at]);
 }
 
-// One row's entries in one wave: -inf where there is none.
-struct Entries {
+// One row's entries in one wave. The loads are issued where it is made, and
+// used in `entries` and `student`, so that a row's own loads may come between.
+struct RawEntries {
   float t[kPerLane];
-  int id[kPerLane];
-  bool bad;  // an id outside the vocabulary
-  __device__ __forceinline__ Entries(const TeacherArgs& a, int64_t row, int64_t ignore_index) {
+  int64_t id[kPerLane];
+  __device__ __forceinline__ RawEntries(const TeacherArgs& a, int64_t row, int top) {
+#pragma unroll
+    for (int i = 0; i < kPerLane; ++i) {
+      const int k = (threadIdx.x & 63) + 64 * i;
+      if (64 * i >= top) continue;  // uniform
+      id[i] = a.ids[row * a.ld_ids + min(k, top - 1)];
+      t[i] = teacher_logit(a, row, min(k, top - 1));
+    }
+  }
+};
+
+// -inf where there is no entry.
+template <typename T>
+struct Entries {
+  float t[kPerLane], x[kPerLane];  // the teacher's logits, the student's
+  bool bad;                        // an id outside the vocabulary
+  __device__ __forceinline__ Entries(const TeacherArgs& a, const RawEntries& r, const T* __restrict__ row, int64_t ignore_index,
+                                     int top) {
     bad = false;
-    const int lane = threadIdx.x & 63;
 #pragma unroll
     for (int i = 0; i < kPerLane; ++i) {
       t[i] = -INFINITY;
-      id[i] = 0;
-      const int k = lane + 64 * i;
-      if (k >= a.top) continue;
-      const int64_t c = a.ids[row * a.ld_ids + k];
-      if (c == ignore_index) continue;
-      if (c < 0 || c >= a.vocab) bad = true;
-      else {
-        id[i] = (int)c;
-        t[i] = teacher_logit(a, row, k);
-      }
+      x[i] = 0.0f;
+      if (64 * i >= top) continue;  // uniform
+      const bool here = (int)(threadIdx.x & 63) + 64 * i < top && r.id[i] != ignore_index;
+      const bool in = r.id[i] >= 0 && r.id[i] < a.vocab;
+      bad |= here && !in;
+      t[i] = here && in ? r.t[i] : -INFINITY;
+      x[i] = to_f32(row[here && in ? r.id[i] : 0]);
     }
   }
 };
@@ -64,9 +77,9 @@ struct Entries {
 // Loss of a row, by one wave. out: (m, log2 s, the largest teacher logit, log2
 // of the sum of 2^((t - largest) c2)) for the backward; m is NaN where the
 // loss is.
-template <bool CAP>
+template <typename T, bool CAP>
 __device__ __forceinline__ void finish_row(const ScoreParams& p, const TeacherArgs& a, int64_t row, const RowStats& st,
-                                           const Entries& en, const float* x, float* __restrict__ losses,
+                                           const Entries<T>& en, float* __restrict__ losses,
                                            f32x4_t* __restrict__ out) {
   float tm = -INFINITY;
 #pragma unroll
@@ -91,7 +104,7 @@ __device__ __forceinline__ void finish_row(const ScoreParams& p, const TeacherAr
     for (int i = 0; i < kPerLane; ++i) {
       const float lq = (en.t[i] - tm) * p.c2 - tl;
       const float q = __builtin_amdgcn_exp2f(lq);
-      if (q != 0.0f) loss += q * (kLn2 * lq - log_prob(p, score<CAP>(p, x[i]), st.m, l2));
+      if (q != 0.0f) loss += q * (kLn2 * lq - log_prob(p, score<CAP>(p, en.x[i]), st.m, l2));
     }
     loss = wave_sum(loss) * a.t2;
     if (loss != loss) m = NAN;
@@ -114,7 +127,11 @@ distill_segment_kernel(const T* __restrict__ logits, int64_t rows, int64_t ld, i
     const int64_t row = segs == 1 ? unit : unit / segs;
     const int seg = segs == 1 ? 0 : (int)(unit - row * segs);
     const T* x = logits + row * ld;
+    // (the other waves' loads of the entries hit the same lines)
+    const int entries = segs == 1 ? a.top : 0;
+    const RawEntries raw(a, row, entries);
     Segment<T, VPT, TPR> sg(x, a.vocab, seg, span);
+    const Entries<T> en(a, raw, x, p.ignore_index, entries);
     float m = wave_max(sg.largest());
     if ((threadIdx.x & 63) == 0) part_m[threadIdx.x / 64] = m;
     __syncthreads();
@@ -132,11 +149,7 @@ distill_segment_kernel(const T* __restrict__ logits, int64_t rows, int64_t ld, i
     if (segs > 1) {
       if (threadIdx.x == 0) part[unit] = f32x4_t{st.m, st.s, 0.0f, 0.0f};
     } else if (threadIdx.x < 64) {
-      const Entries en(a, row, p.ignore_index);
-      float xs[kPerLane];
-#pragma unroll
-      for (int i = 0; i < kPerLane; ++i) xs[i] = to_f32(x[en.id[i]]);
-      finish_row<CAP>(p, a, row, st, en, xs, losses, stats);
+      finish_row<T, CAP>(p, a, row, st, en, losses, stats);
     }
     __syncthreads();  // part_s is rewritten for the workgroup's next unit
   }
@@ -148,17 +161,14 @@ __global__ void __launch_bounds__(64)
 distill_join_kernel(const T* __restrict__ logits, int64_t ld, int segs, ScoreParams p, TeacherArgs a,
                     float* __restrict__ losses, f32x4_t* __restrict__ stats, const f32x4_t* __restrict__ part) {
   const int64_t row = blockIdx.x;
-  const Entries en(a, row, p.ignore_index);
-  float xs[kPerLane];
-#pragma unroll
-  for (int i = 0; i < kPerLane; ++i) xs[i] = to_f32(logits[row * ld + en.id[i]]);
+  const Entries<T> en(a, RawEntries(a, row, a.top), logits + row * ld, p.ignore_index, a.top);
   RowStats st{-INFINITY, 0.0f, 0.0f};
   for (int i = threadIdx.x; i < segs; i += 64) {
     const f32x4_t q = part[row * segs + i];
     st = join_stats(p, st, RowStats{q[0], q[1], 0.0f});
   }
   st = wave_join(p, st);
-  finish_row<CAP>(p, a, row, st, en, xs, losses, stats);
+  finish_row<T, CAP>(p, a, row, st, en, losses, stats);
 }
 
 // loss[0] = sum of losses / max(1, #rows with entries), scale[0] = 1 / that
@@ -195,16 +205,55 @@ distill_mean_kernel(const float* __restrict__ losses, const f32x4_t* __restrict_
   }
 }
 
-// The gradient from the forward's statistics; blockIdx.y takes `span` vectors
-// of the row. The entries' columns are written again, with their terms, once
-// the row's others have left; the same id twice writes the same value twice.
+constexpr int kSpanVectors = 8 * kGradThreads;  // no span has more (grad_plan)
+constexpr int kSlots = kSpanVectors + 16;       // and the elements around the vectors
+
+// (p_v - q_v) c. In LDS: for each vector of the span, and each single element,
+// 1 + the first of its entries, or 0; each entry's column, gradient and the
+// vector's next entry.
+template <typename T, bool CAP>
+struct DistillRow {
+  const ScoreParams& p;
+  float m, l2, c;
+  const uint32_t* first;
+  const int* ids;
+  const float* grads;
+  const uint32_t* next;
+  __device__ __forceinline__ float value(float x, float q) const {
+    float slope;
+    const float y = score_and_slope<T, CAP>(p, x, slope);
+    return (__builtin_amdgcn_exp2f((y - m) * p.c2 - l2) - q) * (c * slope);
+  }
+  __device__ __forceinline__ float many(float x) const { return value(x, 0.0f); }
+  __device__ __forceinline__ float one(float x, int, int i) const {
+    const uint32_t k = first[kSpanVectors + i];
+    return k ? grads[k - 1] : value(x, 0.0f);
+  }
+  __device__ __forceinline__ void patch(const Vec16<T>&, int col, int v, Vec16<T>& o) const {
+    for (uint32_t k = first[v]; k; k = next[k - 1]) {
+      const int at = ids[k - 1] - col;
+      const T g = from_f32<T>(grads[k - 1]);
+#pragma unroll
+      for (int e = 0; e < Vec16<T>::VE; ++e) o.e[e] = e == at ? g : o.e[e];
+    }
+  }
+};
+
+// The gradient from the forward's statistics; blockIdx.y takes `span` vectors of
+// the row. The entries of the span are worked out first, a thread each, and put
+// into their vectors' results on the way out. (Written over the stored row
+// instead, they cost [4096, 50257] bf16 with 64 entries 50 us behind a barrier
+// that waits for all stores, 30 us in a launch of their own, and 40 us where
+// each vector's thread works its entries out.)
 template <typename T, bool CAP, bool NT, int U>
 __global__ void __launch_bounds__(kGradThreads)
 distill_grad_kernel(const T* __restrict__ logits, const f32x4_t* __restrict__ stats, const float* __restrict__ g_loss,
                     int64_t g_stride, const float* __restrict__ scale, T* __restrict__ grad, int64_t rows,
                     int64_t ld, int64_t ld_g, int span, ScoreParams p, TeacherArgs a) {
-  __shared__ int sid[kMaxTop];
-  __shared__ float sq[kMaxTop];
+  constexpr int VE = Vec16<T>::VE;
+  __shared__ uint32_t first[kSlots], next[kMaxTop];
+  __shared__ int ids[kMaxTop];
+  __shared__ float qs[kMaxTop], grads[kMaxTop];
   const int v0 = blockIdx.y * span, v1 = v0 + span;
   const bool ends = blockIdx.y == 0;
   const int t = threadIdx.x;
@@ -214,33 +263,38 @@ distill_grad_kernel(const T* __restrict__ logits, const f32x4_t* __restrict__ st
     T* gx = grad + row * ld_g;
     const f32x4_t st = stats[row];
     if (st[2] == -INFINITY) {  // no entries
-      map_row<T, NT, 1>(x, gx, a.vocab, v0, v1, ends, [](float) { return 0.0f; });
+      map_row<T, NT, 1>(x, gx, a.vocab, v0, v1, ends, ZeroRow());
       continue;
     }
+    const RowSplit<T> sp(x, a.vocab);
+    int slot = -1;  // of this thread's entry, if this workgroup writes its column
+    float xv = 0.0f;
     if (t < a.top) {
-      const int64_t c = a.ids[row * a.ld_ids + t];
-      const bool there = c != p.ignore_index && c >= 0 && c < a.vocab;
-      sid[t] = there ? (int)c : -1;
-      sq[t] = there ? __builtin_amdgcn_exp2f((teacher_logit(a, row, t) - st[2]) * p.c2 - st[3]) : 0.0f;
-    }
-    const float m = st[0] == -INFINITY ? 0.0f : st[0], l2 = st[1];
-    const float c = g_loss[row * g_stride] * (scale ? scale[0] : 1.0f) * a.t2;
-    auto term = [&](float v, float q) {
-      float slope;
-      const float y = score_and_slope<CAP>(p, v, slope);
-      return (__builtin_amdgcn_exp2f((y - m) * p.c2 - l2) - q) * (c * slope);
-    };
-    map_row<T, NT, U>(x, gx, a.vocab, v0, v1, ends, [&](float v) { return term(v, 0.0f); });
-    stores_done();
-    if (t < a.top) {
-      const int id = sid[t];
-      if (id >= 0 && wrote_column(x, a.vocab, v0, v1, ends, id)) {
-        float q = 0.0f;
-        for (int k = 0; k < a.top; ++k) q += sid[k] == id ? sq[k] : 0.0f;
-        gx[id] = from_f32<T>(term(to_f32(x[id]), q));
+      const int64_t id = a.ids[row * a.ld_ids + t];
+      const bool there = id != p.ignore_index && id >= 0 && id < a.vocab;
+      qs[t] = __builtin_amdgcn_exp2f((teacher_logit(a, row, t) - st[2]) * p.c2 - st[3]);
+      ids[t] = there ? (int)id : -1;
+      if (there) {
+        const int c = (int)id - sp.head, v = c / VE;
+        if (c < 0 || v >= sp.nvec) slot = ends ? kSpanVectors + (c < 0 ? (int)id : (int)id - sp.nvec * VE) : -1;
+        else if (v >= v0 && v < v1) slot = v - v0;
+        if (slot >= 0) xv = to_f32(x[id]);
       }
     }
-    __syncthreads();  // sid / sq are rewritten for the workgroup's next row
+    for (int i = t; i < span; i += kGradThreads) first[i] = 0;
+    if (t < 16) first[kSpanVectors + t] = 0;
+    __syncthreads();
+    const DistillRow<T, CAP> f{p, st[0] == -INFINITY ? 0.0f : st[0], st[1],
+                               g_loss[row * g_stride] * (scale ? scale[0] : 1.0f) * a.t2, first, ids, grads, next};
+    if (slot >= 0) {
+      float q = 0.0f;  // in the order of the entries: of equal ids each has the same sum
+      for (int k = 0; k < a.top; ++k) q += ids[k] == ids[t] ? qs[k] : 0.0f;
+      grads[t] = f.value(xv, q);
+      next[t] = atomicExch(&first[slot], (uint32_t)t + 1);
+    }
+    __syncthreads();
+    map_row<T, NT, U>(x, gx, a.vocab, v0, v1, ends, f);
+    __syncthreads();  // the arrays are rewritten for the workgroup's next row
   }
 }
 
