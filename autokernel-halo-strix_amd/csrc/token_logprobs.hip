@@ -509,16 +509,17 @@ struct LogprobRow {
   }
 };
 
-// The gradient from the forward's statistics; blockIdx.y takes `span` vectors
-// of the row.
+// The gradient from the forward's statistics; a workgroup takes `span` vectors
+// of a row.
 template <typename T, bool CAP, bool NT, int U>
 __global__ void __launch_bounds__(kGradThreads)
 logprob_grad_kernel(const T* __restrict__ logits, const int64_t* __restrict__ tokens, const f32x4_t* __restrict__ stats,
                     const float* __restrict__ g_logprobs, const float* __restrict__ g_entropy, T* __restrict__ grad,
-                    int64_t rows, int vocab, int64_t ld, int64_t ld_g, int span, ScoreParams p) {
-  const int v0 = blockIdx.y * span, v1 = v0 + span;
-  const bool ends = blockIdx.y == 0;
-  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+                    int64_t rows, int vocab, int64_t ld, int64_t ld_g, int spans, int span, ScoreParams p) {
+  for (int64_t unit = blockIdx.x; unit < rows * spans; unit += gridDim.x) {
+    const int64_t row = unit / spans;
+    const int v0 = (int)(unit - row * spans) * span, v1 = v0 + span;
+    const bool ends = v0 == 0;
     const T* x = logits + row * ld;
     T* gx = grad + row * ld_g;
     const f32x4_t st = stats[row];
@@ -608,16 +609,16 @@ void launch_bwd(const void* logits, const int64_t* tokens, const float* stats, c
                 void* grad, int64_t rows, int vocab, int64_t ld, int64_t ld_g, const ScoreParams& p, hipStream_t s) {
   constexpr int VE = Vec16<T>::VE;
   const ScorePlan pl = grad_plan(vocab, VE);
-  const dim3 grid(row_grid(rows), pl.segs), block(kGradThreads);
+  const dim3 grid(row_grid(rows * pl.segs)), block(kGradThreads);
   const T* x = static_cast<const T*>(logits);
   T* g = static_cast<T*>(grad);
   const f32x4_t* st = reinterpret_cast<const f32x4_t*>(stats);
   if (vocab / VE < 4 * kGradThreads)
-    logprob_grad_kernel<T, CAP, false, 1><<<grid, block, 0, s>>>(x, tokens, st, gl, ge, g, rows, vocab, ld, ld_g, pl.span, p);
+    logprob_grad_kernel<T, CAP, false, 1><<<grid, block, 0, s>>>(x, tokens, st, gl, ge, g, rows, vocab, ld, ld_g, pl.segs, pl.span, p);
   else if (score_past_cache(2 * rows * vocab * (int64_t)sizeof(T)))
-    logprob_grad_kernel<T, CAP, true, 4><<<grid, block, 0, s>>>(x, tokens, st, gl, ge, g, rows, vocab, ld, ld_g, pl.span, p);
+    logprob_grad_kernel<T, CAP, true, 4><<<grid, block, 0, s>>>(x, tokens, st, gl, ge, g, rows, vocab, ld, ld_g, pl.segs, pl.span, p);
   else
-    logprob_grad_kernel<T, CAP, false, 4><<<grid, block, 0, s>>>(x, tokens, st, gl, ge, g, rows, vocab, ld, ld_g, pl.span, p);
+    logprob_grad_kernel<T, CAP, false, 4><<<grid, block, 0, s>>>(x, tokens, st, gl, ge, g, rows, vocab, ld, ld_g, pl.segs, pl.span, p);
 }
 
 }  // namespace

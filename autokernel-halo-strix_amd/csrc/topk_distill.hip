@@ -205,8 +205,7 @@ distill_mean_kernel(const float* __restrict__ losses, const f32x4_t* __restrict_
   }
 }
 
-constexpr int kSpanVectors = 8 * kGradThreads;  // no span has more (grad_plan)
-constexpr int kSlots = kSpanVectors + 16;       // and the elements around the vectors
+constexpr int kSlots = kSpan + 16;  // a span's vectors, and the elements around the vectors
 
 // (p_v - q_v) c. In LDS: for each vector of the span, and each single element,
 // 1 + the first of its entries, or 0; each entry's column, gradient and the
@@ -226,7 +225,7 @@ struct DistillRow {
   }
   __device__ __forceinline__ float many(float x) const { return value(x, 0.0f); }
   __device__ __forceinline__ float one(float x, int, int i) const {
-    const uint32_t k = first[kSpanVectors + i];
+    const uint32_t k = first[kSpan + i];
     return k ? grads[k - 1] : value(x, 0.0f);
   }
   __device__ __forceinline__ void patch(const Vec16<T>&, int col, int v, Vec16<T>& o) const {
@@ -239,8 +238,8 @@ struct DistillRow {
   }
 };
 
-// The gradient from the forward's statistics; blockIdx.y takes `span` vectors of
-// the row. The entries of the span are worked out first, a thread each, and put
+// The gradient from the forward's statistics; a workgroup takes `span` vectors of
+// a row. The entries of the span are worked out first, a thread each, and put
 // into their vectors' results on the way out. (Written over the stored row
 // instead, they cost [4096, 50257] bf16 with 64 entries 50 us behind a barrier
 // that waits for all stores, 30 us in a launch of their own, and 40 us where
@@ -249,16 +248,17 @@ template <typename T, bool CAP, bool NT, int U>
 __global__ void __launch_bounds__(kGradThreads)
 distill_grad_kernel(const T* __restrict__ logits, const f32x4_t* __restrict__ stats, const float* __restrict__ g_loss,
                     int64_t g_stride, const float* __restrict__ scale, T* __restrict__ grad, int64_t rows,
-                    int64_t ld, int64_t ld_g, int span, ScoreParams p, TeacherArgs a) {
+                    int64_t ld, int64_t ld_g, int spans, int span, ScoreParams p, TeacherArgs a) {
   constexpr int VE = Vec16<T>::VE;
   __shared__ uint32_t first[kSlots], next[kMaxTop];
   __shared__ int ids[kMaxTop];
   __shared__ float qs[kMaxTop], grads[kMaxTop];
-  const int v0 = blockIdx.y * span, v1 = v0 + span;
-  const bool ends = blockIdx.y == 0;
   const int t = threadIdx.x;
   static_assert(kMaxTop <= kGradThreads, "an entry a thread");
-  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+  for (int64_t unit = blockIdx.x; unit < rows * spans; unit += gridDim.x) {
+    const int64_t row = unit / spans;
+    const int v0 = (int)(unit - row * spans) * span, v1 = v0 + span;
+    const bool ends = v0 == 0;
     const T* x = logits + row * ld;
     T* gx = grad + row * ld_g;
     const f32x4_t st = stats[row];
@@ -276,21 +276,28 @@ distill_grad_kernel(const T* __restrict__ logits, const f32x4_t* __restrict__ st
       ids[t] = there ? (int)id : -1;
       if (there) {
         const int c = (int)id - sp.head, v = c / VE;
-        if (c < 0 || v >= sp.nvec) slot = ends ? kSpanVectors + (c < 0 ? (int)id : (int)id - sp.nvec * VE) : -1;
+        if (c < 0 || v >= sp.nvec) slot = ends ? kSpan + (c < 0 ? (int)id : (int)id - sp.nvec * VE) : -1;
         else if (v >= v0 && v < v1) slot = v - v0;
         if (slot >= 0) xv = to_f32(x[id]);
       }
     }
     for (int i = t; i < span; i += kGradThreads) first[i] = 0;
-    if (t < 16) first[kSpanVectors + t] = 0;
+    if (t < 16) first[kSpan + t] = 0;
     __syncthreads();
     const DistillRow<T, CAP> f{p, st[0] == -INFINITY ? 0.0f : st[0], st[1],
                                g_loss[row * g_stride] * (scale ? scale[0] : 1.0f) * a.t2, first, ids, grads, next};
+    if (slot >= 0) next[t] = atomicExch(&first[slot], (uint32_t)t + 1);
+    __syncthreads();
     if (slot >= 0) {
-      float q = 0.0f;  // in the order of the entries: of equal ids each has the same sum
-      for (int k = 0; k < a.top; ++k) q += ids[k] == ids[t] ? qs[k] : 0.0f;
+      // equal ids are in one list: their sum, in the order of the entries, whatever the list's
+      float q = 0.0f;
+      for (uint32_t last = 0, least; last <= kMaxTop; last = least) {
+        least = kMaxTop + 1;
+        for (uint32_t k = first[slot]; k; k = next[k - 1])
+          if (k > last && ids[k - 1] == ids[t]) least = min(least, k);
+        if (least <= kMaxTop) q += qs[least - 1];
+      }
       grads[t] = f.value(xv, q);
-      next[t] = atomicExch(&first[slot], (uint32_t)t + 1);
     }
     __syncthreads();
     map_row<T, NT, U>(x, gx, a.vocab, v0, v1, ends, f);
@@ -322,16 +329,16 @@ void launch_bwd(const void* logits, const float* stats, const float* g_loss, int
                 hipStream_t s) {
   constexpr int VE = Vec16<T>::VE;
   const ScorePlan pl = grad_plan(a.vocab, VE);
-  const dim3 grid(row_grid(rows), pl.segs), block(kGradThreads);
+  const dim3 grid(row_grid(rows * pl.segs)), block(kGradThreads);
   const T* x = static_cast<const T*>(logits);
   T* g = static_cast<T*>(grad);
   const f32x4_t* st = reinterpret_cast<const f32x4_t*>(stats);
   if (a.vocab / VE < 4 * kGradThreads)
-    distill_grad_kernel<T, CAP, false, 1><<<grid, block, 0, s>>>(x, st, g_loss, g_stride, scale, g, rows, ld, ld_g, pl.span, p, a);
+    distill_grad_kernel<T, CAP, false, 1><<<grid, block, 0, s>>>(x, st, g_loss, g_stride, scale, g, rows, ld, ld_g, pl.segs, pl.span, p, a);
   else if (score_past_cache(2 * rows * a.vocab * (int64_t)sizeof(T)))
-    distill_grad_kernel<T, CAP, true, 4><<<grid, block, 0, s>>>(x, st, g_loss, g_stride, scale, g, rows, ld, ld_g, pl.span, p, a);
+    distill_grad_kernel<T, CAP, true, 4><<<grid, block, 0, s>>>(x, st, g_loss, g_stride, scale, g, rows, ld, ld_g, pl.segs, pl.span, p, a);
   else
-    distill_grad_kernel<T, CAP, false, 4><<<grid, block, 0, s>>>(x, st, g_loss, g_stride, scale, g, rows, ld, ld_g, pl.span, p, a);
+    distill_grad_kernel<T, CAP, false, 4><<<grid, block, 0, s>>>(x, st, g_loss, g_stride, scale, g, rows, ld, ld_g, pl.segs, pl.span, p, a);
 }
 
 int check(const char* name, const void* logits, const void* teacher, const int64_t* ids, int64_t rows, int64_t vocab,
