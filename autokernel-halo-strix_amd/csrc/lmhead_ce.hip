@@ -901,6 +901,41 @@ lmhead_logprob_rows_kernel(const T* __restrict__ H, const T* __restrict__ W, con
   const int row0 = blockIdx.x * kRowsPerBlock, row = row0 + r;
   constexpr int kWaves = kRowsPerBlock * kRowGroups / 64;
   constexpr int kInFlight = 8;
+  // the given tokens' scores, kRowsPerBlock / kWaves of them a wave, their loads together
+  if (tokens) {
+    constexpr int kPer = kRowsPerBlock / kWaves;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x / 64;
+    int64_t t[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) t[i] = tokens[min(row0 + wave * kPer + i, n_rows - 1)];
+    const T* hp[kPer];
+    const T* wp[kPer];
+    float acc[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const bool in = t[i] != ignore_index && t[i] >= 0 && t[i] < vocab;
+      hp[i] = H + (int64_t)min(row0 + wave * kPer + i, n_rows - 1) * ldh;
+      wp[i] = W + (in ? t[i] : 0) * ldw;
+      acc[i] = 0.0f;
+    }
+    for (int c = lane; c < d / 8; c += 64) {
+      Vec16<T> x[kPer], y[kPer];
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        x[i] = load16<T>(hp[i] + 8 * c);
+        y[i] = load16<T>(wp[i] + 8 * c);
+      }
+#pragma unroll
+      for (int i = 0; i < kPer; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) acc[i] = fmaf(to_f32(x[i].e[e]), to_f32(y[i].e[e]), acc[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const float z = wave_sum(acc[i]);
+      if (lane == 0) tl[wave * kPer + i] = z;
+    }
+  }
   MSU st{-INFINITY, 0.0f, 0.0f};
   if (row < n_rows) {
     for (int v0 = grp; v0 < n_part; v0 += kInFlight * kRowGroups) {
@@ -912,21 +947,23 @@ lmhead_logprob_rows_kernel(const T* __restrict__ H, const T* __restrict__ W, con
         a[i] = part[at];
         u[i] = usum[at];
       }
+      // of these eight at their largest maximum, then one merge
+      MSU one{-INFINITY, 0.0f, 0.0f};
 #pragma unroll
       for (int i = 0; i < kInFlight; ++i)
-        if (v0 + i * kRowGroups < n_part) st = msu_merge(st, MSU{a[i].m, a[i].s, u[i]}, c2);
+        if (v0 + i * kRowGroups < n_part) one.m = fmaxf(one.m, a[i].m);
+#pragma unroll
+      for (int i = 0; i < kInFlight; ++i) {
+        if (v0 + i * kRowGroups < n_part && a[i].s != 0.0f) {
+          const float dm = (a[i].m - one.m) * c2, f = __builtin_amdgcn_exp2f(dm);
+          one.s += f * a[i].s;
+          one.u += f * (u[i] + fmaxf(dm, -1000.0f) * a[i].s);
+        }
+      }
+      st = msu_merge(st, one, c2);
     }
   }
   red[grp][r] = st;
-  if (tokens) {
-    for (int i = threadIdx.x / 64; i < kRowsPerBlock; i += kWaves) {
-      const int q = row0 + i;
-      const int64_t t = q < n_rows ? tokens[q] : -1;
-      float z = 0.0f;
-      if (t != ignore_index && t >= 0 && t < vocab) z = wave_dot(H + (int64_t)q * ldh, W + t * ldw, d);  // wave-uniform
-      if ((threadIdx.x & 63) == 0) tl[i] = z;
-    }
-  }
   __syncthreads();
   if (grp != 0 || row >= n_rows) return;
   for (int g = 1; g < kRowGroups; ++g) st = msu_merge(st, red[g][r], c2);
