@@ -799,7 +799,7 @@ struct LmheadLogprobs : torch::autograd::Function<LmheadLogprobs> {
   static variable_list forward(AutogradContext* ctx, const Tensor& h, const Tensor& w, const Maybe& t_, double temperature,
                                double softcap, int64_t ignore) {
     const Tensor t = t_.value_or(Tensor());
-    const Tensor stats = f32_like(h, {h.size(0), 2});
+    const Tensor stats = f32_like(h, {h.size(0), 4});
     variable_list out = run_lmhead_logprobs(h, w, t, temperature, softcap, ignore, stats);
     ctx->save_for_backward({h, w, t, stats});
     ctx->saved_data["p"] = std::vector<double>{temperature, softcap};
@@ -833,7 +833,7 @@ struct LmheadLogprobs : torch::autograd::Function<LmheadLogprobs> {
 // (logprobs or None, entropy). budget: as in lmhead_ce.
 std::optional<std::tuple<Tensor, Tensor>> lmhead_logprobs(const Tensor& h, const Tensor& w, const Maybe& t, double temperature,
                                                           double softcap, int64_t ignore, double budget) {
-  if (!ours(h, w) || !ours_if(t, h) || !scale_args(temperature, softcap) || h.dim() < 1 || !h.is_contiguous() || !at16(h) ||
+  if (!ours(h, w) || !ours_if(t, h) || !scale_args(temperature, softcap) || temperature < 1e-3 || h.dim() < 1 || !h.is_contiguous() || !at16(h) ||
       !dense16(w) || h.scalar_type() != w.scalar_type() || h.numel() == 0 || w.size(0) == 0 ||
       (h.scalar_type() != at::kHalf && h.scalar_type() != at::kBFloat16) || h.size(-1) != w.size(1) || w.size(1) % 64 ||
       (t && !leading_i64(*t, h)))

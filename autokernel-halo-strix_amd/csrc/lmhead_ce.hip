@@ -576,8 +576,12 @@ lmhead_ce_tile_kernel(const T* __restrict__ H, const T* __restrict__ W, MSPair* 
         float s = (s4[0] + s4[1]) + (s4[2] + s4[3]);
         s += __shfl_xor(s, 32, 64);
         if constexpr (kEnt) {
-          const float u = (u4[0] + u4[1]) + (u4[2] + u4[3]);
-          zres[tb] = u + __shfl_xor(u, 32, 64);
+          float u = (u4[0] + u4[1]) + (u4[2] + u4[3]);
+          u += __shfl_xor(u, 32, 64);
+          // ms is m c2 rounded: every exponent is off by the same rest, taken out here
+          const float rest = m == -INFINITY ? 0.0f : fmaf(m, c2, -ms), f = __builtin_amdgcn_exp2f(-rest);
+          zres[tb] = f * (u - rest * s);
+          s *= f;
         }
         res[tb] = MSPair{m, s};
         __builtin_amdgcn_sched_barrier(0);  // one token block's values live at a time
@@ -886,13 +890,13 @@ __device__ __forceinline__ MSU msu_merge(MSU a, MSU b, float c2) {
 // Rows from the tile partials: a 512-thread workgroup owns 32 tokens, 16
 // threads a token fold every 16th partial and are joined in a fixed order; the
 // workgroup's waves form the given tokens' scores as their own dot products
-// meanwhile. stats: (lse2, entropy) of each row for the backward, lse2 = m c2 +
-// log2 s.
+// meanwhile. stats: (lse2, entropy, rest, -) of each row for the backward, lse2 =
+// m c2 + log2 s rounded and the rest that it lacks.
 template <typename T>
 __global__ void __launch_bounds__(kRowsPerBlock * kRowGroups)
 lmhead_logprob_rows_kernel(const T* __restrict__ H, const T* __restrict__ W, const MSPair* __restrict__ part,
                            const float* __restrict__ usum, const int64_t* __restrict__ tokens,
-                           float* __restrict__ logprobs, float* __restrict__ entropy, f32x2_t* __restrict__ stats,
+                           float* __restrict__ logprobs, float* __restrict__ entropy, f32x4_t* __restrict__ stats,
                            int n_rows, int vocab, int d, int64_t ldh, int64_t ldw, int n_part, int64_t ignore_index,
                            float cap, float c2, float inv_t) {
   __shared__ MSU red[kRowGroups][kRowsPerBlock];
@@ -970,7 +974,8 @@ lmhead_logprob_rows_kernel(const T* __restrict__ H, const T* __restrict__ W, con
   const float l2 = __builtin_amdgcn_logf(st.s);
   float h = kLn2 * (l2 - st.u / st.s);
   if (h < 0.0f) h = 0.0f;  // one rounding below zero where one token holds all
-  if (stats) stats[row] = f32x2_t{fmaf(st.m, c2, l2), h};
+  const float lse2 = fmaf(st.m, c2, l2);
+  if (stats) stats[row] = f32x4_t{lse2, h, fmaf(st.m, c2, -lse2) + l2, 0.0f};
   if (tokens) {
     const int64_t t = tokens[row];
     float lp = (capped(tl[r], cap) - st.m) * inv_t - kLn2 * l2;
@@ -984,12 +989,12 @@ lmhead_logprob_rows_kernel(const T* __restrict__ H, const T* __restrict__ W, con
 // Row coefficients of the backward from the upstream gradients g and e:
 // -(g + e (ln p + H)) / T = c0 + c1 log2 p.
 __global__ void __launch_bounds__(256)
-lmhead_logprob_coef_kernel(const int64_t* __restrict__ tokens, const f32x2_t* __restrict__ stats,
+lmhead_logprob_coef_kernel(const int64_t* __restrict__ tokens, const f32x4_t* __restrict__ stats,
                            const float* __restrict__ g_logprobs, const float* __restrict__ g_entropy,
                            f32x4_t* __restrict__ coefs, int n_rows, int vocab, int64_t ignore_index, float inv_t) {
   const int row = blockIdx.x * 256 + threadIdx.x;
   if (row >= n_rows) return;
-  const f32x2_t st = stats[row];
+  const f32x4_t st = stats[row];
   float g = tokens && g_logprobs ? g_logprobs[row] : 0.0f, e = g_entropy ? g_entropy[row] : 0.0f;
   if (tokens) {
     const int64_t t = tokens[row];
@@ -998,7 +1003,10 @@ lmhead_logprob_coef_kernel(const int64_t* __restrict__ tokens, const f32x2_t* __
   }
   g *= inv_t;
   e *= inv_t;
-  coefs[row] = f32x4_t{st[0], g == 0.0f && e == 0.0f ? 0.0f : -fmaf(e, st[1], g), -e * kLn2, g};
+  // with t = z' c2 - lse2 in place of log2 p = t - rest, p = 2^t 2^-rest
+  const float f = __builtin_amdgcn_exp2f(-st[2]), c1 = -e * kLn2;
+  const float c0 = g == 0.0f && e == 0.0f ? 0.0f : -fmaf(e, st[1], g) - c1 * st[2];
+  coefs[row] = f32x4_t{st[0], c0 * f, c1 * f, g};
 }
 
 // The given tokens' entries, from their own dot products: what the tile kernel
@@ -1147,7 +1155,7 @@ void launch_logprobs(const void* h, const void* w, const int64_t* tokens, float*
   else
     launch_tiles_fwd<T, false, false, true>(hp, wp, part, n_rows, vocab, d, ldh, ldw, n_vt, n_tt, ga, gd, bd, s);
   lmhead_logprob_rows_kernel<T><<<dim3((n_rows + kRowsPerBlock - 1) / kRowsPerBlock), dim3(kRowsPerBlock * kRowGroups), 0, s>>>(
-      hp, wp, part, ga.zsum, tokens, logprobs, entropy, reinterpret_cast<f32x2_t*>(stats), n_rows, vocab, d, ldh, ldw,
+      hp, wp, part, ga.zsum, tokens, logprobs, entropy, reinterpret_cast<f32x4_t*>(stats), n_rows, vocab, d, ldh, ldw,
       2 * n_vt, ignore_index, cap, ga.c2, 1.0f / temperature);
 }
 
@@ -1166,11 +1174,15 @@ void launch_logprobs_bwd(const void* h, const void* w, const int64_t* tokens, co
     lmhead_logprob_grad_token_kernel<T><<<dim3((n_rows + 3) / 4), dim3(256), 0, s>>>(hp, wp, tokens, ga, n_rows, vocab, d, ldh, ldw);
 }
 
+// Below this the exponents' products in the tiles, z' c2, lose the scores' last
+// bits to their own size.
+constexpr float kLeastTemperature = 1e-3f;
+
 // What the log-probability entry points ask of their operands.
 int check_logprobs(const char* name, const void* hidden, const void* weight, int64_t n_rows, int64_t vocab, int64_t v_count,
                    int64_t d, int64_t ld_h, int64_t ld_w, float temperature, float softcap, int dtype) {
-  if (!(temperature >= 1e-18f && temperature <= 1e18f))
-    return ak_set_error(AK_ERR_INVALID_ARG, "%s: temperature must be between 1e-18 and 1e18", name);
+  if (!(temperature >= kLeastTemperature && temperature <= 1e18f))
+    return ak_set_error(AK_ERR_INVALID_ARG, "%s: temperature must be between 1e-3 and 1e18", name);
   if (!(softcap >= 0.0f) || softcap == INFINITY)
     return ak_set_error(AK_ERR_INVALID_ARG, "%s: softcap must be finite and >= 0", name);
   if (dtype != AK_DTYPE_BF16 && dtype != AK_DTYPE_F16)
@@ -1205,7 +1217,7 @@ extern "C" int ak_lmhead_logprobs_fwd(const void* hidden, const void* weight, co
   const int rc = ak::check_logprobs(name, hidden, weight, n_rows, vocab, vocab, d, ld_h, ld_w, temperature, softcap, dtype);
   if (rc) return rc;
   if (tokens && !logprobs) return ak_set_error(AK_ERR_INVALID_ARG, "%s: null pointer", name);
-  if (reinterpret_cast<uintptr_t>(stats) & 7u) return ak_set_error(AK_ERR_INVALID_ARG, "%s: stats must be 8-byte aligned", name);
+  if (!ak::aligned16(stats)) return ak_set_error(AK_ERR_INVALID_ARG, "%s: stats must be 16-byte aligned", name);
   const size_t need = ak::logprob_ws(n_rows, vocab).total;
   if (workspace_bytes < need || !workspace || !ak::aligned16(workspace))
     return ak_set_error(AK_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed (16-byte aligned)", name, workspace_bytes, need);
@@ -1223,14 +1235,14 @@ extern "C" int ak_lmhead_logprobs_coefs(const int64_t* tokens, const float* stat
   const char* name = "ak_lmhead_logprobs_coefs";
   if (n_rows < 0 || n_rows > (1 << 30) || vocab <= 0 || vocab > (1 << 30))
     return ak_set_error(AK_ERR_INVALID_ARG, "%s: bad shape n_rows=%lld vocab=%lld", name, (long long)n_rows, (long long)vocab);
-  if (!(temperature >= 1e-18f && temperature <= 1e18f))
-    return ak_set_error(AK_ERR_INVALID_ARG, "%s: temperature must be between 1e-18 and 1e18", name);
+  if (!(temperature >= ak::kLeastTemperature && temperature <= 1e18f))
+    return ak_set_error(AK_ERR_INVALID_ARG, "%s: temperature must be between 1e-3 and 1e18", name);
   if (n_rows == 0) return AK_OK;
   if (!stats || !coefs) return ak_set_error(AK_ERR_INVALID_ARG, "%s: null pointer", name);
-  if ((reinterpret_cast<uintptr_t>(stats) & 7u) || !ak::aligned16(coefs))
-    return ak_set_error(AK_ERR_INVALID_ARG, "%s: stats must be 8-byte and coefs 16-byte aligned", name);
+  if (!ak::aligned16(stats) || !ak::aligned16(coefs))
+    return ak_set_error(AK_ERR_INVALID_ARG, "%s: stats and coefs must be 16-byte aligned", name);
   ak::lmhead_logprob_coef_kernel<<<dim3((unsigned)((n_rows + 255) / 256)), dim3(256), 0, ak_stream(stream)>>>(
-      tokens, reinterpret_cast<const ak::f32x2_t*>(stats), grad_logprobs, grad_entropy, reinterpret_cast<ak::f32x4_t*>(coefs),
+      tokens, reinterpret_cast<const ak::f32x4_t*>(stats), grad_logprobs, grad_entropy, reinterpret_cast<ak::f32x4_t*>(coefs),
       (int)n_rows, (int)vocab, ignore_index, 1.0f / temperature);
   return ak_check_launch(name);
 }

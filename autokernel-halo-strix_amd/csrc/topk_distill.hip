@@ -13,7 +13,10 @@
 // more and writes the gradient once. Writing the gradient in the forward would
 // save that read where the upstream gradient is exactly 1, but such a loss is
 // weighted against another (or scaled, in fp16): the stored gradient would
-// then be read, scaled, rounded a second time and written again.
+// then be read, scaled, rounded a second time and written again. Measured (a copy
+// of 1 GiB here: 5.1 TB/s): [4096, 32768] bf16 with 64 entries 51 us forward and
+// 85 us backward, 5.2 and 6.3 TB/s; [1999, 50257] fp32 with 128 entries and a
+// softcap 90 and 130 us.
 #include "score_rows.h"
 
 namespace ak {
@@ -158,9 +161,9 @@ distill_segment_kernel(const T* __restrict__ logits, int64_t rows, int64_t ld, i
 // Joins a row's segments, one wave a row.
 template <typename T, bool CAP>
 __global__ void __launch_bounds__(64)
-distill_join_kernel(const T* __restrict__ logits, int64_t ld, int segs, ScoreParams p, TeacherArgs a,
+distill_join_kernel(const T* __restrict__ logits, int64_t row0, int64_t ld, int segs, ScoreParams p, TeacherArgs a,
                     float* __restrict__ losses, f32x4_t* __restrict__ stats, const f32x4_t* __restrict__ part) {
-  const int64_t row = blockIdx.x;
+  const int64_t row = row0 + blockIdx.x;
   const Entries<T> en(a, RawEntries(a, row, a.top), logits + row * ld, p.ignore_index, a.top);
   RowStats st{-INFINITY, 0.0f, 0.0f};
   for (int i = threadIdx.x; i < segs; i += 64) {
@@ -320,7 +323,8 @@ void launch_fwd(const void* logits, int64_t rows, int64_t ld, const ScorePlan& p
   distill_segment_kernel<T, VPT, TPR, CAP><<<grid, dim3(TPR), 0, s>>>(x, rows, ld, pl.segs, pl.span, p, a, losses, st, part)
   AK_SEGMENT_DISPATCH(pl.span, GO);
 #undef GO
-  if (pl.segs > 1) distill_join_kernel<T, CAP><<<dim3((unsigned)rows), dim3(64), 0, s>>>(x, ld, pl.segs, p, a, losses, st, part);
+  for (int64_t row0 = 0; pl.segs > 1 && row0 < rows; row0 += kMaxRowGrid)
+    distill_join_kernel<T, CAP><<<dim3(row_grid(rows - row0)), dim3(64), 0, s>>>(x, row0, ld, pl.segs, p, a, losses, st, part);
 }
 
 template <typename T, bool CAP>

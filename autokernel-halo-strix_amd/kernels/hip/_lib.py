@@ -634,7 +634,7 @@ def lmhead_logprobs(hidden: torch.Tensor, weight: torch.Tensor, tokens: Optional
                     logprobs: Optional[torch.Tensor], entropy: torch.Tensor, stats: Optional[torch.Tensor],
                     temperature: float, softcap: float, ignore_index: int) -> None:
     """Log probabilities of ``tokens`` (int64) and entropies of ``softmax(hidden
-    @ weight^T)`` (fp32 ``[n_rows]``); ``stats`` fp32 ``[n_rows, 2]`` is for the
+    @ weight^T)`` (fp32 ``[n_rows]``); ``stats`` fp32 ``[n_rows, 4]`` is for the
     backward."""
     require_device(hidden, weight, tokens, logprobs, entropy, stats)
     n_rows, d = hidden.shape

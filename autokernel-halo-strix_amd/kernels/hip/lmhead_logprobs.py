@@ -54,7 +54,7 @@ def _forward(hidden, weight, tokens, temperature, softcap, ignore_index, chunk_s
     f32 = dict(dtype=torch.float32, device=hidden.device)
     logprobs = torch.empty(n, **f32) if tokens is not None else None
     entropy = torch.empty(n, **f32)
-    stats = torch.empty((n, 2 if fused else 4), **f32) if keep else None
+    stats = torch.empty((n, 4), **f32) if keep else None
     if n and fused:
         h, w = _kernel_operands(hidden, weight)
         _lib.lmhead_logprobs(h, w, tokens, logprobs, entropy, stats, temperature, softcap, ignore_index)
@@ -126,7 +126,7 @@ def kernel_fn(hidden: torch.Tensor, weight: torch.Tensor, tokens: Optional[torch
         hidden: ``[..., d]`` fp16, bf16 or fp32.
         weight: ``[vocab, d]``; another type is converted to hidden's.
         tokens: whole numbers of the leading shape, or None (no ``logprobs``).
-        temperature: divides the (capped) logits.
+        temperature: divides the (capped) logits; at least 1e-3.
         softcap: logit softcap (0 = off).
         ignore_index: token value of rows to leave out (their hidden states
             have to be finite where ``weight``'s gradient is asked for).
@@ -148,7 +148,7 @@ def kernel_fn(hidden: torch.Tensor, weight: torch.Tensor, tokens: Optional[torch
         raise ValueError(f"weight must not be empty, got shape {tuple(weight.shape)}")
     if hidden.dtype == torch.float32 and vocab > _lib.MAX_SCORE_VOCAB:
         raise ValueError(f"fp32 takes a vocab of at most {_lib.MAX_SCORE_VOCAB}, got {vocab}")
-    check_scale(temperature, softcap)
+    check_scale(temperature, softcap, least=1e-3)
     if chunk_size < 1:
         raise ValueError(f"chunk_size must be at least 1, got {chunk_size}")
     lead = hidden.shape[:-1]

@@ -53,10 +53,10 @@ class TokenLogprobs(NamedTuple):
     top_ids: Optional[torch.Tensor]
 
 
-def check_scale(temperature: float, softcap: float) -> None:
+def check_scale(temperature: float, softcap: float, least: float = 1e-18) -> None:
     """The temperature and softcap that the scoring kernels take."""
-    if not 1e-18 <= temperature <= 1e18:
-        raise ValueError(f"temperature must be between 1e-18 and 1e18, got {temperature}")
+    if not least <= temperature <= 1e18:
+        raise ValueError(f"temperature must be between {least:g} and 1e18, got {temperature}")
     if not 0.0 <= softcap < math.inf:
         raise ValueError(f"softcap must be finite and >= 0, got {softcap}")
 

@@ -247,8 +247,9 @@ int ak_scale_inplace(void* x, int64_t n, const float* scale, int dtype, void* st
  * not ignore_index has logprob NaN. A row of -inf alone has logprob -inf and
  * entropy 0; a row that holds a NaN or +inf has NaN results. stats [rows, 4]
  * fp32, 16-byte aligned, is what ak_token_logprobs_bwd takes. top_k is at most
- * 256 and vocab, vocab at most 2^20. workspace: as many bytes as the query says
- * (0 for most calls; few or very wide rows are cut into segments), 16-byte
+ * 256 and vocab, vocab at most 2^20, temperature between 1e-18 and 1e18. workspace: as many bytes as the query says
+ * (0 without alternatives for most calls; few or very wide rows are cut into
+ * segments), 16-byte
  * aligned. No counterpart in the reference, whose cross-entropy
  * (kernels/ce_fused.py:122-382) gives the loss of given tokens only.
  */
@@ -401,8 +402,8 @@ int ak_lmhead_ce_bwd_range(const void* hidden, const void* weight, const int64_t
  * hidden @ weight^T (fp32 accumulation), which are never written to memory.
  * tokens (and then logprobs), entropy and stats may be NULL; a row whose token
  * is ignore_index has logprob and entropy 0, a token outside [0, vocab) that is
- * not ignore_index logprob NaN. stats [n_rows, 2] fp32, 8-byte aligned, is what
- * ak_lmhead_logprobs_coefs takes. Shape rules as for ak_lmhead_ce_fwd. No
+ * not ignore_index logprob NaN. stats [n_rows, 4] fp32, 16-byte aligned, is what
+ * ak_lmhead_logprobs_coefs takes. temperature is at least 1e-3. Shape rules as for ak_lmhead_ce_fwd. No
  * counterpart in the reference, whose chunked loss
  * (kernels/hip/chunked_linear_cross_entropy.py:55-148) returns the mean only.
  */

@@ -101,6 +101,13 @@ def test_lmhead_temperature_and_softcap(dtype, temperature, softcap):
     check(*operands(300, 1000, 128, dtype, 3), temperature, softcap)
 
 
+@pytest.mark.parametrize("temperature", [1e-3, 0.01, 50.0])
+def test_lmhead_far_temperatures(temperature):
+    """Scores in the thousands: each tile's offset is rounded, and its rest taken out again."""
+    need_gpu()
+    check(*operands(40, 700, 64, torch.bfloat16, 9, scale=8.0), temperature)
+
+
 def test_lmhead_fp32():
     need_gpu()
     check(*operands(70, 1001, 48, torch.float32, 4), 0.8, 20.0)
@@ -151,7 +158,7 @@ def test_lmhead_graph_replays():
     from kernels.hip import _lib
     h, w, t = (a.to(DEV) for a in operands(300, 1001, 128, torch.bfloat16, 8))
     f = lambda *s: torch.empty(*s, device=DEV)
-    lp, ent, st, co = f(300), f(300), f(300, 2), f(300, 4)
+    lp, ent, st, co = f(300), f(300), f(300, 4), f(300, 4)
     up = torch.randn(300, generator=torch.Generator().manual_seed(1)).to(DEV)
     dz = torch.zeros(300, 1088, dtype=torch.bfloat16, device=DEV)[:, :1001]
 

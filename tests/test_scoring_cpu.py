@@ -186,8 +186,9 @@ def test_lmhead_refusals(scoring_backend):
         kernel_fn(h, w, tok.float())
     with pytest.raises(TypeError, match="dtype"):
         kernel_fn(h.double(), w, tok)
-    with pytest.raises(ValueError, match="temperature"):
-        kernel_fn(h, w, tok, temperature=0)
+    for bad in (0, 1e-4, 1e20):
+        with pytest.raises(ValueError, match="temperature"):
+            kernel_fn(h, w, tok, temperature=bad)
     with pytest.raises(ValueError, match="softcap"):
         kernel_fn(h, w, tok, softcap=-1)
     with pytest.raises(ValueError, match="chunk_size"):
@@ -330,7 +331,7 @@ def test_library_refusals_of_the_head(lib):
     assert fwd(h=None) == -1 and fwd(tok=16) == -1 and says(b"null")
     assert fwd(h=8) == -1 and fwd(w=24) == -1 and says(b"aligned")
     assert fwd(stats=4) == -1 and says(b"aligned")
-    assert fwd(t=0.0) == -1 and fwd(t=math.nan) == -1 and says(b"temperature")
+    assert fwd(t=1e-4) == -1 and fwd(t=math.nan) == -1 and says(b"temperature")
     assert fwd(cap=-1.0) == -1 and fwd(cap=math.inf) == -1 and says(b"softcap")
     need = lib.ak_lmhead_logprobs_workspace_bytes(8, 16)
     assert need >= 2 * 8 * 12 and fwd(nbytes=need - 1, ws=16) == -4 and fwd(nbytes=need) == -4
