@@ -68,6 +68,12 @@ def check(h, w, t, temperature=1.0, softcap=0.0, grads=True):
         # relative error of a term: its exponent's, and the chains' of lse and entropy; fp16 also steps of its subnormals
         rel = 4 * terr + 2 * ROW
         term = dz.abs() * eps + size * rel + (2.0 ** -25 if dtype == torch.float16 else 0.0)
+        # the hardware exponential is 0 below fp32's smallest normal number: a term
+        # p (g + e (ln p + H)) / T with p < 2^-126 is lost whole; p |ln p| rises with p
+        # there, so it is at most 2^-126 (|g| + |e| (88 + ln V)) / T, 88 > 126 ln 2. (At
+        # T = 0.01 three rows of the vocab have their largest p at 2^-127, 2^-130, 2^-134.)
+        gsum = sum(u.abs() * f for u, f in ((pair[0], 1.0), (pair[1], 88.0 + lnv)) if u is not None)
+        term = term + (gsum * 2.0 ** -126 / temperature).double()[:, None]
         if pair[1] is not None:
             # -e p (ln p + H): ln p and H are off by absolute amounts (the tolerances above),
             # also where both are 0 and the term's size with them (one token holding all)
