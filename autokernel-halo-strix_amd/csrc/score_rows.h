@@ -397,8 +397,9 @@ inline int check_score_rows(const char* name, int64_t rows, int64_t vocab, int64
     return ak_set_error(AK_ERR_INVALID_ARG, "%s: rows=%lld x pitch exceed 64-bit addressing", name, (long long)rows);
   if (!(temperature >= 1e-18f && temperature <= 1e18f))  // its square is a float, too
     return ak_set_error(AK_ERR_INVALID_ARG, "%s: temperature must be between 1e-18 and 1e18", name);
-  if (!(softcap >= 0.0f) || softcap == INFINITY)
-    return ak_set_error(AK_ERR_INVALID_ARG, "%s: softcap must be finite and >= 0", name);
+  // the cap's tanh is within 2^-22 of 1: of a larger cap that is more than the logits' own rounding
+  if (!(softcap == 0.0f || (softcap >= 1e-3f && softcap <= 1e4f)))
+    return ak_set_error(AK_ERR_INVALID_ARG, "%s: softcap must be 0 or between 1e-3 and 1e4", name);
   return AK_OK;
 }
 

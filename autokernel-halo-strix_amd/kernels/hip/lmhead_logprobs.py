@@ -127,7 +127,7 @@ def kernel_fn(hidden: torch.Tensor, weight: torch.Tensor, tokens: Optional[torch
         weight: ``[vocab, d]``; another type is converted to hidden's.
         tokens: whole numbers of the leading shape, or None (no ``logprobs``).
         temperature: divides the (capped) logits; at least 1e-3.
-        softcap: logit softcap (0 = off).
+        softcap: logit softcap, 1e-3 to 1e4 (0 = off), as in ``token_logprobs``.
         ignore_index: token value of rows to leave out (their hidden states
             have to be finite where ``weight``'s gradient is asked for).
         chunk_size: rows per chunk of the fp32 path's GEMMs.

@@ -29,7 +29,6 @@ No counterpart in the reference, whose cross-entropy
 (``kernels/ce_fused.py:557-785``) gives the loss of given tokens only.
 """
 
-import math
 import os
 from typing import NamedTuple, Optional
 
@@ -57,8 +56,8 @@ def check_scale(temperature: float, softcap: float, least: float = 1e-18) -> Non
     """The temperature and softcap that the scoring kernels take."""
     if not least <= temperature <= 1e18:
         raise ValueError(f"temperature must be between {least:g} and 1e18, got {temperature}")
-    if not 0.0 <= softcap < math.inf:
-        raise ValueError(f"softcap must be finite and >= 0, got {softcap}")
+    if softcap != 0.0 and not 1e-3 <= softcap <= 1e4:
+        raise ValueError(f"softcap must be 0 (off) or between 1e-3 and 1e4, got {softcap}")
 
 
 def whole_numbers(t: torch.Tensor, name: str, shape) -> torch.Tensor:
@@ -139,7 +138,8 @@ def kernel_fn(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, *, te
         logits: ``[..., vocab]`` fp32, fp16 or bf16, vocab at most 2^20.
         tokens: whole numbers of the leading shape, or None (no ``logprobs``).
         temperature: divides the (capped) logits.
-        softcap: logit softcap (0 = off).
+        softcap: logit softcap, 1e-3 to 1e4 (0 = off); scores are exact to
+            ``2^-22 softcap / temperature`` under it.
         ignore_index: token value of rows to leave out.
         top_k: alternatives of each row, 0 to min(256, vocab).
     """

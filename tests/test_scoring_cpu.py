@@ -8,6 +8,7 @@ import pytest
 import torch
 
 from kernels.hip import _lib
+from kernels.hip import lmhead_logprobs as ll
 from kernels.hip import token_logprobs as tl
 from kernels.hip import topk_distillation as td
 from oracle import scoring
@@ -352,3 +353,25 @@ def test_library_refusals_of_the_head(lib):
     assert coefs(stats=None) == -1 and coefs(co=None) == -1 and says(b"null")
     assert coefs(stats=4) == -1 and coefs(co=8) == -1 and says(b"aligned")
     assert coefs(n=-1) == -1 and coefs(v=0) == -1 and coefs(t=0.0) == -1 and coefs(n=0, stats=None) == 0
+
+
+def test_softcaps_out_of_range(scoring_backend):
+    """Caps whose tanh, within 2^-22 of 1, would say less than the logits (or nothing: 1e-50 is 0 in fp32)."""
+    x, tok, ids = torch.randn(3, 8), torch.zeros(3, dtype=torch.int64), torch.zeros(3, 2, dtype=torch.int64)
+    for bad in (1e-50, 9e-4, 2e4, 1e38):
+        with pytest.raises(ValueError, match="softcap"):
+            tl.kernel_fn(x, tok, softcap=bad)
+        with pytest.raises(ValueError, match="softcap"):
+            td.kernel_fn(x, x[:, :2], ids, softcap=bad)
+        with pytest.raises(ValueError, match="softcap"):
+            ll.kernel_fn(torch.randn(3, 64), torch.randn(8, 64), tok, softcap=bad)
+    for good in (1e-3, 1e4):
+        tl.kernel_fn(x, tok, softcap=good)
+
+
+@pytest.mark.parametrize("cap", [1e-40, 9e-4, 2e4, 3e38])
+def test_library_refuses_softcaps_out_of_range(lib, cap):
+    for rc in (lib.ak_token_logprobs_fwd(16, None, None, None, None, None, None, None, 0, 600, 8, 8, 0, 1.0, cap, -100, 0, None),
+               lib.ak_topk_distill_fwd(16, 16, 16, 16, 16, None, None, None, 0, 600, 8, 2, 8, 2, 2, 1.0, cap, -100, 0, 0, None),
+               lib.ak_lmhead_logprobs_fwd(16, 16, None, None, None, None, None, 0, 8, 16, 64, 64, 64, 1.0, cap, -100, 2, None)):
+        assert rc == -1 and b"softcap" in lib.ak_last_error()
