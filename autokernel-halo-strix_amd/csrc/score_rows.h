@@ -309,18 +309,20 @@ inline ScorePlan score_plan(int64_t rows, int64_t vocab, int ve) {
 // ---------------------------------------------------------------------------
 constexpr int kGradThreads = 256;
 
-// d(score / temperature) / d(logit), and the score (as many_score).
+// d(score / temperature) / d(logit), and the score (as many_score). The slope 1 -
+// tanh^2 as 4 q / (1 + q)^2 with q = exp(2 x / cap): a difference from 1 would
+// have nothing left where the cap is near.
 template <typename T, bool CAP>
 __device__ __forceinline__ float score_and_slope(const ScoreParams& p, float x, float& slope) {
   if constexpr (CAP && !std::is_same<T, float>::value) {
-    const float r = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * p.k2));
-    slope = 4.0f * p.inv_t * r * (1.0f - r);
+    const float q = __builtin_amdgcn_exp2f(x * p.k2), r = __builtin_amdgcn_rcpf(1.0f + q);
+    slope = 4.0f * p.inv_t * r * (r * fminf(q, 1e30f));  // (q may be inf, r 0 then)
     return fmaf(-2.0f * p.cap, r, p.cap);
   }
   if constexpr (CAP) {
-    const float th = tanh_f32(x * p.inv_cap);
-    slope = p.inv_t * (1.0f - th * th);
-    return p.cap * th;
+    const float a = x * p.inv_cap, q = fast_exp(-2.0f * fabsf(a)), r = __builtin_amdgcn_rcpf(1.0f + q);
+    slope = 4.0f * p.inv_t * r * (r * q);
+    return p.cap * tanh_f32(a);  // (the same exponential and reciprocal)
   }
   slope = p.inv_t;
   return x;

@@ -70,7 +70,7 @@ def logprob_grad_rows(x, tokens, g_logprobs, g_entropy, temperature=1.0, softcap
     entropy = -_plogp(logp).sum(-1, keepdim=True)
     slope = torch.full_like(z, 1.0 / temperature)
     if softcap > 0:
-        slope = slope * (1 - torch.tanh(x.double() / softcap) ** 2)
+        slope = slope * torch.cosh(x.double() / softcap) ** -2
     grad, size = torch.zeros_like(z), torch.zeros_like(z)
     for r in range(x.shape[0]):
         t = None if tokens is None else int(tokens[r])
@@ -127,7 +127,7 @@ def distill_grad_rows(x, teacher, ids, upstream, temperature=1.0, softcap=0.0, i
     _, q, counted = distill_rows(x, teacher, ids, temperature, softcap, ignore_index)
     slope = torch.full_like(z, temperature)
     if softcap > 0:
-        slope = slope * (1 - torch.tanh(x.double() / softcap) ** 2)
+        slope = slope * torch.cosh(x.double() / softcap) ** -2
     by = upstream.double().reshape(-1, 1) * slope * counted[:, None]
     grad = torch.where(counted[:, None], (p - q) * by, torch.zeros_like(z))
     return grad, torch.where(counted[:, None], (p + q) * by.abs(), torch.zeros_like(z))

@@ -403,3 +403,20 @@ def test_runs_are_bitwise_the_same():
         got = [*r, g]
         first = first or got
         assert all(torch.equal(a, b) for a, b in zip(got, first))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("softcap", [1e-3, 1.0, 2.0, 1e4])
+def test_gradients_near_and_far_from_the_cap(dtype, softcap):
+    """Logits beyond a small cap, whose slope 1 - tanh^2 goes down to e^-30 (its
+    exponent 2 |x| / cap is rounded to 2 u of it, within ROW), and a cap beyond all logits."""
+    need_gpu()
+    say("softcap", dtype, softcap)
+    x = logits_of(9, 1500, dtype, 31)
+    if softcap < 1.0:
+        x.mul_(softcap)  # (x / cap up to 15; of fp16's subnormals each is exact)
+    else:
+        x.clamp_(-15 * softcap, 15 * softcap)
+    t = torch.randint(0, 1500, (9,), generator=torch.Generator().manual_seed(5)).to(DEV)
+    check_logprobs(x, t, 1.0, softcap, top_k=4)
+    check_distill(x, *teacher_of(x, 20, 6), softcap=softcap)
