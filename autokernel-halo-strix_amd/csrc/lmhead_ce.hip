@@ -440,7 +440,7 @@ lmhead_ce_tile_kernel(const T* __restrict__ H, const T* __restrict__ W, MSPair* 
                 } else {
                   t = fmaf(z, ga.c2, -lse2);
                 }
-                e[j] = __builtin_amdgcn_exp2f(t) * fmaf(c1, t, c0) * slope;
+                e[j] = __builtin_amdgcn_exp2f(t) * fmaf(c1, fmaxf(t, -1000.0f), c0) * slope;
               } else if constexpr (kCap) {
                 // softmax(z')_v * s_t * dz'/dz
                 const Cap cp(ga.cap);
@@ -562,7 +562,7 @@ lmhead_ce_tile_kernel(const T* __restrict__ H, const T* __restrict__ W, MSPair* 
         float m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
         m = fmaxf(m, __shfl_xor(m, 32, 64));
         const float c2 = kEnt ? ga.c2 : kLog2e;
-        const float ms = m * c2;
+        const float ms = kEnt && m == -INFINITY ? 0.0f : m * c2;  // logits past fp32's range: s = u = 0
         float s4[4] = {0.0f, 0.0f, 0.0f, 0.0f}, u4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int vb = 0; vb < 4; ++vb)
@@ -571,7 +571,7 @@ lmhead_ce_tile_kernel(const T* __restrict__ H, const T* __restrict__ W, MSPair* 
             const float t = fmaf(x[vb][r], c2, -ms);
             const float e = __builtin_amdgcn_exp2f(t);
             s4[r & 3] += e;
-            if constexpr (kEnt) u4[r & 3] = fmaf(e, kTail ? fmaxf(t, -1000.0f) : t, u4[r & 3]);
+            if constexpr (kEnt) u4[r & 3] = fmaf(e, fmaxf(t, -1000.0f), u4[r & 3]);  // (2^t is 0 there)
           }
         float s = (s4[0] + s4[1]) + (s4[2] + s4[3]);
         s += __shfl_xor(s, 32, 64);
@@ -891,7 +891,7 @@ __device__ __forceinline__ MSU msu_merge(MSU a, MSU b, float c2) {
 // threads a token fold every 16th partial and are joined in a fixed order; the
 // workgroup's waves form the given tokens' scores as their own dot products
 // meanwhile. stats: (lse2, entropy, rest, -) of each row for the backward, lse2 =
-// m c2 + log2 s rounded and the rest that it lacks.
+// m c2 + log2 s rounded and the rest that it lacks; lse2 = inf where every logit is -inf.
 template <typename T>
 __global__ void __launch_bounds__(kRowsPerBlock * kRowGroups)
 lmhead_logprob_rows_kernel(const T* __restrict__ H, const T* __restrict__ W, const MSPair* __restrict__ part,
@@ -971,14 +971,15 @@ lmhead_logprob_rows_kernel(const T* __restrict__ H, const T* __restrict__ W, con
   __syncthreads();
   if (grp != 0 || row >= n_rows) return;
   for (int g = 1; g < kRowGroups; ++g) st = msu_merge(st, red[g][r], c2);
-  const float l2 = __builtin_amdgcn_logf(st.s);
-  float h = kLn2 * (l2 - st.u / st.s);
+  const bool empty = st.m == -INFINITY && st.s == 0.0f;  // every logit is -inf
+  const float l2 = empty ? 0.0f : __builtin_amdgcn_logf(st.s);
+  float h = empty ? 0.0f : kLn2 * (l2 - st.u / st.s);
   if (h < 0.0f) h = 0.0f;  // one rounding below zero where one token holds all
-  const float lse2 = fmaf(st.m, c2, l2);
-  if (stats) stats[row] = f32x4_t{lse2, h, fmaf(st.m, c2, -lse2) + l2, 0.0f};
+  const float lse2 = empty ? INFINITY : fmaf(st.m, c2, l2);
+  if (stats) stats[row] = f32x4_t{lse2, h, empty ? 0.0f : fmaf(st.m, c2, -lse2) + l2, 0.0f};
   if (tokens) {
     const int64_t t = tokens[row];
-    float lp = (capped(tl[r], cap) - st.m) * inv_t - kLn2 * l2;
+    float lp = empty ? -INFINITY : (capped(tl[r], cap) - st.m) * inv_t - kLn2 * l2;
     if (t == ignore_index) lp = h = 0.0f;
     else if (t < 0 || t >= vocab) lp = NAN;
     logprobs[row] = lp;
@@ -996,9 +997,11 @@ lmhead_logprob_coef_kernel(const int64_t* __restrict__ tokens, const f32x4_t* __
   if (row >= n_rows) return;
   const f32x4_t st = stats[row];
   float g = tokens && g_logprobs ? g_logprobs[row] : 0.0f, e = g_entropy ? g_entropy[row] : 0.0f;
+  const bool empty = st[0] == INFINITY;  // no gradient, t = -inf
+  if (empty) g = e = 0.0f;
   if (tokens) {
     const int64_t t = tokens[row];
-    if (t == ignore_index) g = e = 0.0f;
+    if (t == ignore_index || empty) g = e = 0.0f;
     else if (t < 0 || t >= vocab) g = NAN;
   }
   g *= inv_t;
@@ -1029,7 +1032,7 @@ lmhead_logprob_grad_token_kernel(const T* __restrict__ H, const T* __restrict__ 
     slope = q < INFINITY ? 4.0f * q * r * r : 0.0f;
   }
   static_cast<T*>(ga.dz)[(int64_t)tok * ga.ld_dz + tl] =
-      from_f32<T>(fmaf(__builtin_amdgcn_exp2f(t), fmaf(co[2], t, co[1]), co[3]) * slope);
+      from_f32<T>(fmaf(__builtin_amdgcn_exp2f(t), fmaf(co[2], fmaxf(t, -1000.0f), co[1]), co[3]) * slope);
 }
 
 size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }

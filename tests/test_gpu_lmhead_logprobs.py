@@ -194,3 +194,41 @@ def test_lmhead_graph_replays():
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip((lp, ent, dz), ref))
         run()
+
+
+@pytest.mark.parametrize("n,vocab,live", [(5, 700, 3), (300, 1024, 200), (300, 1153, 300), (260, 600, 599)])
+def test_lmhead_logits_past_fp32(n, vocab, live):
+    """In bf16 (fp16's products stay in fp32's range). Weight rows whose products pass fp32 to -inf mask their tokens, tiles of
+    them alone too; a hidden row for which all are such has no distribution.
+    The live tokens' logits are 0, so ln p = -ln(live) and the entropy ln(live)."""
+    need_gpu()
+    from kernels.hip.lmhead_logprobs import kernel_fn
+    say("lmhead past fp32", n, vocab, live)
+    g = torch.Generator().manual_seed(8)
+    w = torch.zeros(vocab, 64, dtype=torch.bfloat16)
+    w[:, 0] = -1e30
+    at = torch.randperm(vocab, generator=g)[:live]
+    w[at, 0] = 0.0
+    w[:, 1] = -1e30
+    h = torch.zeros(n, 64, dtype=torch.bfloat16)
+    h[:, 0] = 1e30
+    h[1] = 0.0
+    h[1, 1] = 1e30  # all -inf
+    t = at[torch.randint(0, live, (n,), generator=g)]
+    masked = (w[:, 0] != 0).nonzero().flatten()
+    t[2] = masked[0]
+    hd, wd, td = h.to(DEV).requires_grad_(), w.to(DEV), t.to(DEV)
+    r = kernel_fn(hd, wd, td)
+    lp, ent = r.logprobs.double().cpu(), r.entropy.double().cpu()
+    rows = torch.ones(n, dtype=torch.bool)
+    rows[1] = False
+    assert float((ent[rows] - math.log(live)).abs().max()) <= ROW * (1 + 2 * math.log(live)) and ent[1] == 0
+    assert lp[1] == -math.inf and lp[2] == -math.inf
+    rows[2] = False
+    assert float((lp[rows] + math.log(live)).abs().max()) <= ROW + 4 * U * math.log(live)
+    # the gradient's rows of the weight: sum over rows of dz h, 0 but in column 0 (and nothing from row 1)
+    wl = w.to(DEV).requires_grad_()
+    (gw,) = torch.autograd.grad(kernel_fn(h.to(DEV), wl, td).entropy.sum(), wl)
+    assert bool((gw[:, 1:] == 0).all()) and bool((gw[masked.to(DEV)] == 0).all())
+    (gh,) = torch.autograd.grad(r.entropy.sum(), hd)
+    assert bool((gh[1] == 0).all()) and not bool(torch.isnan(gh).any())
