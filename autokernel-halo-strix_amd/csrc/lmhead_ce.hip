@@ -887,6 +887,27 @@ __device__ __forceinline__ MSU msu_merge(MSU a, MSU b, float c2) {
   return r;
 }
 
+// A row's results from its statistics and its token's score z, by one thread.
+__device__ __forceinline__ void finish_logprob_row(MSU st, float z, int row, const int64_t* __restrict__ tokens,
+                                                   float* __restrict__ logprobs, float* __restrict__ entropy,
+                                                   f32x4_t* __restrict__ stats, int vocab, int64_t ignore_index, float cap,
+                                                   float c2, float inv_t) {
+  const bool empty = st.m == -INFINITY && st.s == 0.0f;  // every logit is -inf
+  const float l2 = empty ? 0.0f : __builtin_amdgcn_logf(st.s);
+  float h = empty ? 0.0f : kLn2 * (l2 - st.u / st.s);
+  if (h < 0.0f) h = 0.0f;  // one rounding below zero where one token holds all
+  const float lse2 = empty ? INFINITY : fmaf(st.m, c2, l2);
+  if (stats) stats[row] = f32x4_t{lse2, h, empty ? 0.0f : fmaf(st.m, c2, -lse2) + l2, 0.0f};
+  if (tokens) {
+    const int64_t t = tokens[row];
+    float lp = empty ? -INFINITY : (capped(z, cap) - st.m) * inv_t - kLn2 * l2;
+    if (t == ignore_index) lp = h = 0.0f;
+    else if (t < 0 || t >= vocab) lp = NAN;
+    logprobs[row] = lp;
+  }
+  if (entropy) entropy[row] = h;
+}
+
 // Rows from the tile partials: a 512-thread workgroup owns 32 tokens, 16
 // threads a token fold every 16th partial and are joined in a fixed order; the
 // workgroup's waves form the given tokens' scores as their own dot products
@@ -971,20 +992,154 @@ lmhead_logprob_rows_kernel(const T* __restrict__ H, const T* __restrict__ W, con
   __syncthreads();
   if (grp != 0 || row >= n_rows) return;
   for (int g = 1; g < kRowGroups; ++g) st = msu_merge(st, red[g][r], c2);
-  const bool empty = st.m == -INFINITY && st.s == 0.0f;  // every logit is -inf
-  const float l2 = empty ? 0.0f : __builtin_amdgcn_logf(st.s);
-  float h = empty ? 0.0f : kLn2 * (l2 - st.u / st.s);
-  if (h < 0.0f) h = 0.0f;  // one rounding below zero where one token holds all
-  const float lse2 = empty ? INFINITY : fmaf(st.m, c2, l2);
-  if (stats) stats[row] = f32x4_t{lse2, h, empty ? 0.0f : fmaf(st.m, c2, -lse2) + l2, 0.0f};
-  if (tokens) {
-    const int64_t t = tokens[row];
-    float lp = empty ? -INFINITY : (capped(tl[r], cap) - st.m) * inv_t - kLn2 * l2;
-    if (t == ignore_index) lp = h = 0.0f;
-    else if (t < 0 || t >= vocab) lp = NAN;
-    logprobs[row] = lp;
+  finish_logprob_row(st, tl[r], row, tokens, logprobs, entropy, stats, vocab, ignore_index, cap, c2, inv_t);
+}
+
+// Few tokens (at most kFewTokens). The tile kernel above is 256 tokens wide, so fewer
+// take as long as 256, and it feeds on the ring's full rate of both operands;
+// here the weight, read once, is all there is to move. Each of four waves forms
+// 32 of its workgroup's 128 vocab rows x 32 TB tokens: the weight goes from
+// memory straight into the matrix cores' layout, a K chunk ahead; the hidden
+// states' chunk, which the waves share, through LDS (rows 16 bytes longer than
+// the chunk, so that 16 lanes' reads meet all banks once). One partial (m, s, u)
+// per 128 vocab rows and token. The whole forward, 64 tokens here and 65 in the
+// tile above: 50257 x 768 28 and 39 us, 32768 x 768 18 and 32, 32768 x 4096 67 and
+// 101, 128000 x 2048 120 and 144 (4.4 TB/s of weight); four blocks of 32 tokens lost
+// to the tile at 50257 x 768 (43 us for 38) and 128000 x 2048 (171 for 147), and
+// chunks of 256 columns, whose registers leave no room to read LDS ahead, took 31
+// us for 28.
+constexpr int kFewTokens = 64;
+constexpr int kFewK = 128;              // columns a chunk
+constexpr int kFewPitch = kFewK + 8;
+
+template <typename T, bool kCap, int TB>
+__global__ void __launch_bounds__(256, 2)
+lmhead_logprob_few_kernel(const T* __restrict__ H, const T* __restrict__ W, MSPair* __restrict__ part,
+                          float* __restrict__ usum, int n_rows, int vocab, int d, int64_t ldh, int64_t ldw, float cap,
+                          float c2) {
+  __shared__ __attribute__((aligned(16))) T hs[TB * 32 * kFewPitch];
+  __shared__ MSU red[4][TB * 32];
+  constexpr int kSteps = kFewK / 16, kStage = TB * 32 * (kFewK / 8) / 256;
+  const int t = threadIdx.x, lane = t & 63, wave = t / 64, fr = lane & 31, khalf = lane >> 5;
+  const int v0 = blockIdx.x * 128 + wave * 32;
+  const T* wrow = W + (int64_t)min(v0 + fr, vocab - 1) * ldw;
+  u32x4 w[kSteps], h[kStage];
+  // (past the last column: its last 8, never used)
+  auto load_w = [&](int k0) {
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) w[i] = load16<T>(wrow + min(k0 + 16 * i + 8 * khalf, d - 8)).u;
+  };
+  auto load_h = [&](int k0) {
+#pragma unroll
+    for (int i = 0; i < kStage; ++i) {
+      const int c = t + 256 * i;
+      h[i] = load16<T>(H + (int64_t)min(c / (kFewK / 8), n_rows - 1) * ldh + min(k0 + c % (kFewK / 8) * 8, d - 8)).u;
+    }
+  };
+  f32x16_t acc[TB] = {};
+  load_h(0);
+  load_w(0);
+#pragma unroll 1
+  for (int k0 = 0; k0 < d; k0 += kFewK) {
+#pragma unroll
+    for (int i = 0; i < kStage; ++i) {
+      const int c = t + 256 * i;
+      *reinterpret_cast<u32x4*>(hs + c / (kFewK / 8) * kFewPitch + c % (kFewK / 8) * 8) = h[i];
+    }
+    u32x4 a[kSteps];
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) a[i] = w[i];
+    if (k0 + kFewK < d) {
+      load_h(k0 + kFewK);
+      load_w(k0 + kFewK);
+    }
+    __builtin_amdgcn_s_waitcnt(waitcnt_vm_lgkm0(63));  // the stores to LDS alone
+    ring_barrier();
+#pragma unroll
+    for (int q = 0; q < kSteps; q += 4) {
+      if (k0 + 16 * q < d) {  // uniform: d is whole blocks of 64
+#pragma unroll
+        for (int i = q; i < q + 4; ++i)
+#pragma unroll
+          for (int tb = 0; tb < TB; ++tb)
+            acc[tb] = mfma32(T(), a[i], *reinterpret_cast<const u32x4*>(hs + (tb * 32 + fr) * kFewPitch + 16 * i + 8 * khalf), acc[tb]);
+      }
+    }
+    __builtin_amdgcn_s_waitcnt(waitcnt_vm_lgkm0(63));  // this wave's reads of the chunk are done
+    ring_barrier();
   }
-  if (entropy) entropy[row] = h;
+#pragma unroll
+  for (int tb = 0; tb < TB; ++tb) {
+    float x[16], m = -INFINITY;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      x[r] = v0 + 8 * (r >> 2) + (r & 3) + 4 * khalf < vocab ? (kCap ? capped(acc[tb][r], cap) : acc[tb][r]) : -INFINITY;
+      m = fmaxf(m, x[r]);
+    }
+    m = fmaxf(m, __shfl_xor(m, 32, 64));
+    const float off = m == -INFINITY ? 0.0f : m;
+    float s = 0.0f, u = 0.0f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const float q = (x[r] - off) * c2, e = __builtin_amdgcn_exp2f(q);
+      s += e;
+      u = fmaf(e, fmaxf(q, -1000.0f), u);  // (2^q is 0 there)
+    }
+    s += __shfl_xor(s, 32, 64);
+    u += __shfl_xor(u, 32, 64);
+    if (khalf == 0) red[wave][tb * 32 + fr] = MSU{m, s, u};
+  }
+  __syncthreads();
+  if (t < TB * 32 && t < n_rows) {
+    MSU st = red[0][t];
+    for (int i = 1; i < 4; ++i) st = msu_merge(st, red[i][t], c2);
+    part[(int64_t)blockIdx.x * n_rows + t] = MSPair{st.m, st.s};
+    usum[(int64_t)blockIdx.x * n_rows + t] = st.u;
+  }
+}
+
+// Its rows, one workgroup each: all threads fold the partials and form the
+// given token's dot product, joined in a fixed order.
+template <typename T>
+__global__ void __launch_bounds__(256)
+lmhead_logprob_few_rows_kernel(const T* __restrict__ H, const T* __restrict__ W, const MSPair* __restrict__ part,
+                               const float* __restrict__ usum, const int64_t* __restrict__ tokens,
+                               float* __restrict__ logprobs, float* __restrict__ entropy, f32x4_t* __restrict__ stats,
+                               int n_rows, int vocab, int d, int64_t ldh, int64_t ldw, int n_part, int64_t ignore_index,
+                               float cap, float c2, float inv_t) {
+  __shared__ MSU red[4];
+  __shared__ float dots[4];
+  const int t = threadIdx.x, row = blockIdx.x;
+  float z = 0.0f;
+  if (tokens) {
+    const int64_t tok = tokens[row];
+    const T* hp = H + (int64_t)row * ldh;
+    const T* wp = W + (tok >= 0 && tok < vocab ? tok : 0) * ldw;
+    for (int c = t; c < d / 8; c += 256) {
+      const Vec16<T> a = load16<T>(hp + 8 * c), b = load16<T>(wp + 8 * c);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) z = fmaf(to_f32(a.e[e]), to_f32(b.e[e]), z);
+    }
+    z = wave_sum(z);
+  }
+  MSU st{-INFINITY, 0.0f, 0.0f};
+  for (int i = t; i < n_part; i += 256) {
+    const MSPair q = part[(int64_t)i * n_rows + row];
+    st = msu_merge(st, MSU{q.m, q.s, usum[(int64_t)i * n_rows + row]}, c2);
+  }
+  for (int off = 1; off < 64; off <<= 1)
+    st = msu_merge(st, MSU{__shfl_xor(st.m, off, 64), __shfl_xor(st.s, off, 64), __shfl_xor(st.u, off, 64)}, c2);
+  if ((t & 63) == 0) {
+    red[t / 64] = st;
+    dots[t / 64] = z;
+  }
+  __syncthreads();
+  if (t != 0) return;
+  for (int i = 1; i < 4; ++i) {
+    st = msu_merge(st, red[i], c2);
+    z += dots[i];
+  }
+  finish_logprob_row(st, z, row, tokens, logprobs, entropy, stats, vocab, ignore_index, cap, c2, inv_t);
 }
 
 // Row coefficients of the backward from the upstream gradients g and e:
@@ -1152,6 +1307,22 @@ void launch_logprobs(const void* h, const void* w, const int64_t* tokens, float*
   ga.cap = cap;
   ga.c2 = (float)(1.4426950408889634 / (double)temperature);
   ga.zsum = reinterpret_cast<float*>(base + L.usum);
+  if (n_rows <= kFewTokens) {
+    const int n_part = (vocab + 127) / 128;  // (at most the 2 n_vt that the workspace has room for)
+#define FEW(CAP, TB) lmhead_logprob_few_kernel<T, CAP, TB><<<dim3(n_part), dim3(256), 0, s>>>(hp, wp, part, ga.zsum, n_rows, vocab, d, ldh, ldw, cap, ga.c2)
+    if (cap > 0.0f) {
+      if (n_rows <= 32) FEW(true, 1);
+      else FEW(true, 2);
+    } else {
+      if (n_rows <= 32) FEW(false, 1);
+      else FEW(false, 2);
+    }
+#undef FEW
+    lmhead_logprob_few_rows_kernel<T><<<dim3(n_rows), dim3(256), 0, s>>>(
+        hp, wp, part, ga.zsum, tokens, logprobs, entropy, reinterpret_cast<f32x4_t*>(stats), n_rows, vocab, d, ldh, ldw,
+        n_part, ignore_index, cap, ga.c2, 1.0f / temperature);
+    return;
+  }
   const dim3 gd(min(n_vt * n_tt, cu_count())), bd(kLThreads);
   if (cap > 0.0f)
     launch_tiles_fwd<T, true, false, true>(hp, wp, part, n_rows, vocab, d, ldh, ldw, n_vt, n_tt, ga, gd, bd, s);

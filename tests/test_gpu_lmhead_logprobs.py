@@ -232,3 +232,14 @@ def test_lmhead_logits_past_fp32(n, vocab, live):
     assert bool((gw[:, 1:] == 0).all()) and bool((gw[masked.to(DEV)] == 0).all())
     (gh,) = torch.autograd.grad(r.entropy.sum(), hd)
     assert bool((gh[1] == 0).all()) and not bool(torch.isnan(gh).any())
+
+
+@pytest.mark.parametrize("dtype", HALF, ids=str)
+@pytest.mark.parametrize("n,vocab,d,softcap", [(32, 513, 320, 0.0), (33, 129, 64, 30.0), (64, 2000, 832, 0.0), (65, 777, 256, 0.0),
+                                               (128, 1153, 576, 30.0), (129, 1153, 576, 30.0)])
+def test_lmhead_few_tokens(dtype, n, vocab, d, softcap):
+    """Both sides of the token blocks, last K chunks of one to four blocks, vocab rows left in the last group."""
+    need_gpu()
+    say("lmhead few", dtype, n, vocab, d, softcap)
+    check(*operands(n, vocab, d, dtype, n + d), 0.9, softcap)
+    check(*operands(n, vocab, d, dtype, n + d + 1)[:2], None, 1.0, softcap)
