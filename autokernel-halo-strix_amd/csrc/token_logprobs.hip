@@ -7,7 +7,8 @@
 // and backward, with g and e the gradients of logp and H:
 //   dx_v = (g ([v == token] - p_v) - e p_v (ln p_v + H)) (1 - tanh^2) / temperature.
 //
-// HBM-bound: the forward reads the logits once (score_rows.h), the backward
+// HBM-bound: the forward reads the logits once (score_rows.h; of many rows, not
+// those of an ignored token), the backward
 // reads them once and writes the gradient once. Measured (a copy of 1 GiB here:
 // 5.1 TB/s): [8192, 50304] bf16 forward 145 us, 5.7 TB/s; [4096, 50257] bf16
 // forward and backward 79 + 130 us, 5.9 TB/s of the three passes; [8, 50257]
@@ -65,6 +66,12 @@ struct LogprobArgs {
   f32x4_t* part;          // segs > 1 or top > 0: (m, s, u, -) of each segment
   float* maxima;          // top > 0: [rows, groups] maxima of 2^shift vectors each
   int top, vocab, groups, shift;
+  // Whether rows of an ignored token are left unread. The token is then waited for
+  // before the row: [8192, 50304] bf16 153 to 160 us (152 without), a quarter of it
+  // ignored 118 (146), [4096, 50257] 81 (81) and 63 (80), [2000, 50257] fp32 67 (65)
+  // and 53 (65). Few rows, which wait for
+  // latency alone, are read.
+  bool skip;
 };
 
 // The row's results but the alternatives, by one thread.
@@ -116,9 +123,16 @@ logprob_segment_kernel(const T* __restrict__ logits, int64_t rows, int64_t ld, i
     const T* x = logits + row * ld;
     int64_t tok = p.ignore_index;
     float x_tok = 0.0f;
-    if (!PART && threadIdx.x == 0 && a.tokens) {
+    if (SHIFT < 0 && a.tokens && (!PART || a.skip)) {
       tok = a.tokens[row];
-      if (tok != p.ignore_index && tok >= 0 && tok < a.vocab) x_tok = to_f32(x[tok]);
+      if (a.skip && tok == p.ignore_index) {  // (the whole workgroup) 0 whatever the row holds
+        if (threadIdx.x == 0) {
+          if (PART) a.part[unit] = f32x4_t{-INFINITY, 0.0f, 0.0f, 0.0f};
+          else finish_row<CAP>(p, a, row, RowStats{-INFINITY, 0.0f, 0.0f}, tok, 0.0f);
+        }
+        continue;
+      }
+      if (!PART && threadIdx.x == 0 && tok != p.ignore_index && tok >= 0 && tok < a.vocab) x_tok = to_f32(x[tok]);
     }
     Segment<T, VPT, TPR> sg(x, a.vocab, seg, span);
     float m, group[Segment<T, VPT, TPR>::template kStored<(SHIFT > 0 ? SHIFT : 0)>] = {};
@@ -656,7 +670,7 @@ extern "C" int ak_token_logprobs_fwd(const void* logits, const int64_t* tokens, 
   char* ws = static_cast<char*>(workspace);
   const ak::LogprobArgs a{tokens, logprobs, entropy, reinterpret_cast<ak::f32x4_t*>(stats), top_logprobs, top_ids,
                           w.total ? reinterpret_cast<ak::f32x4_t*>(ws) : nullptr, reinterpret_cast<float*>(ws + w.maxima),
-                          top_k, (int)vocab, w.groups, w.shift};
+                          top_k, (int)vocab, w.groups, w.shift, rows >= 256 && top_k == 0};
   const ak::ScoreParams p = ak::score_params(temperature, softcap, ignore_index);
   hipStream_t s = ak_stream(stream);
   auto go = [&](auto t) {

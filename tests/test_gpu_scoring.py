@@ -420,3 +420,40 @@ def test_gradients_near_and_far_from_the_cap(dtype, softcap):
     t = torch.randint(0, 1500, (9,), generator=torch.Generator().manual_seed(5)).to(DEV)
     check_logprobs(x, t, 1.0, softcap, top_k=4)
     check_distill(x, *teacher_of(x, 20, 6), softcap=softcap)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_ignored_rows_among_many(dtype):
+    """Whole rows (256 and more), every third ignored and some of those NaN: nothing of them
+    reaches their results, their gradients or their neighbours; all ignored; ignored with alternatives."""
+    need_gpu()
+    from kernels.hip.token_logprobs import kernel_fn
+    say("ignored", dtype)
+    x = logits_of(300, 1031, dtype, 41)
+    t = torch.randint(0, 1031, (300,), generator=torch.Generator().manual_seed(4))
+    t[::3] = -100
+    check_logprobs(x, t.to(DEV))
+    check_logprobs(x, t.to(DEV), top_k=3)
+    y = x.clone()
+    y[::6] = math.nan
+    for a, b in zip(kernel_fn(x, t.to(DEV))[:2], kernel_fn(y, t.to(DEV))[:2]):
+        assert torch.equal(a, b)
+    leaf = y.requires_grad_()
+    r = kernel_fn(leaf, t.to(DEV))
+    (g,) = torch.autograd.grad(r.logprobs.sum() + r.entropy.sum(), leaf)
+    assert bool((g[::3] == 0).all()) and bool(torch.isfinite(g).all())
+    r = kernel_fn(x, torch.full((300,), -100, device=DEV))
+    assert bool((r.logprobs == 0).all()) and bool((r.entropy == 0).all())
+    # rows of several segments
+    x = logits_of(257, 70001, dtype, 42)
+    t = torch.randint(0, 70001, (257,), generator=torch.Generator().manual_seed(4))
+    t[::3] = -100
+    x[::6] = math.nan
+    leaf = x.requires_grad_()
+    r = kernel_fn(leaf, t.to(DEV))
+    lp, h = scoring.logprob_rows(x[1:5].detach().cpu(), t[1:5])
+    close(r.logprobs[1:5], lp, ROW + 4 * U * lp.abs(), "logprobs")
+    close(r.entropy[1:5], h, ROW * (1 + 2 * math.log(70001)), "entropy")
+    assert bool((r.logprobs[::3] == 0).all()) and bool((r.entropy[::3] == 0).all()) and bool(torch.isfinite(r.logprobs).all())
+    (g,) = torch.autograd.grad(r.logprobs.sum() + r.entropy.sum(), leaf)
+    assert bool((g[::3] == 0).all()) and bool(torch.isfinite(g).all())
