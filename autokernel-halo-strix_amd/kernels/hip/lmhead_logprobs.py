@@ -14,7 +14,8 @@ tiles again, writes the logits' gradient in the input type (one rounding, as
 both products after it take that type) for as much of the vocabulary at a time
 as ``GRAD_LOGITS_BUDGET`` of the loss allows, and runs the loss's two gradient
 GEMMs on it. For fp32 the logits of ``chunk_size`` rows at a time come from a
-GEMM and go through the row kernels. The backward is differentiable once.
+GEMM and go through the row kernels (under autocast too: operands keep their
+type). The backward is differentiable once.
 
 No counterpart in the reference, whose chunked loss
 (``kernels/hip/chunked_linear_cross_entropy.py:50-175``) returns the mean only.
@@ -47,6 +48,14 @@ def _rows(t, start, end):
     return t[start:end] if t is not None else None
 
 
+def _own_types(t):
+    """GEMMs in the operands' type whatever autocast is in force: the backward
+    forms the logits again, often behind the autocast block that the forward ran
+    in, and its probabilities sum to 1 only over the logits that the statistics
+    are of."""
+    return torch.autocast(t.device.type, enabled=False)
+
+
 def _forward(hidden, weight, tokens, temperature, softcap, ignore_index, chunk_size, keep):
     """``(logprobs, entropy, stats)``."""
     n = hidden.shape[0]
@@ -59,11 +68,12 @@ def _forward(hidden, weight, tokens, temperature, softcap, ignore_index, chunk_s
         h, w = _kernel_operands(hidden, weight)
         _lib.lmhead_logprobs(h, w, tokens, logprobs, entropy, stats, temperature, softcap, ignore_index)
     elif n:
-        for start in range(0, n, chunk_size):
-            end = min(start + chunk_size, n)
-            _lib.token_logprobs(F.linear(hidden[start:end], weight), _rows(tokens, start, end),
-                                _rows(logprobs, start, end), entropy[start:end], _rows(stats, start, end), None, None,
-                                temperature, softcap, ignore_index)
+        with _own_types(hidden):
+            for start in range(0, n, chunk_size):
+                end = min(start + chunk_size, n)
+                _lib.token_logprobs(F.linear(hidden[start:end], weight), _rows(tokens, start, end),
+                                    _rows(logprobs, start, end), entropy[start:end], _rows(stats, start, end), None,
+                                    None, temperature, softcap, ignore_index)
     return logprobs, entropy, stats
 
 
@@ -104,16 +114,17 @@ class _LmheadLogprobs(torch.autograd.Function):
             stats = stats.contiguous()
             gh = torch.empty_like(h) if need_h else None
             gw = torch.zeros(weight.shape, dtype=torch.float32, device=weight.device) if need_w else None
-            for start in range(0, n, ctx.chunk_size):
-                end = min(start + ctx.chunk_size, n)
-                logits = F.linear(h[start:end], w)
-                grad = torch.empty_like(logits)  # (the row kernel reads the logits again behind its stores)
-                _lib.token_logprobs_bwd(logits, _rows(tokens, start, end), stats[start:end], _rows(gl, start, end),
-                                        _rows(ge, start, end), grad, *ctx.params)
-                if need_h:
-                    gh[start:end] = grad @ w
-                if need_w:
-                    gw.addmm_(grad.t(), h[start:end])
+            with _own_types(h):
+                for start in range(0, n, ctx.chunk_size):
+                    end = min(start + ctx.chunk_size, n)
+                    logits = F.linear(h[start:end], w)
+                    grad = torch.empty_like(logits)  # (the row kernel reads the logits again behind its stores)
+                    _lib.token_logprobs_bwd(logits, _rows(tokens, start, end), stats[start:end],
+                                            _rows(gl, start, end), _rows(ge, start, end), grad, *ctx.params)
+                    if need_h:
+                        gh[start:end] = grad @ w
+                    if need_w:
+                        gw.addmm_(grad.t(), h[start:end])
         return gh, gw, None, None, None, None, None
 
 

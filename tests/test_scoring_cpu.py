@@ -375,3 +375,31 @@ def test_library_refuses_softcaps_out_of_range(lib, cap):
                lib.ak_topk_distill_fwd(16, 16, 16, 16, 16, None, None, None, 0, 600, 8, 2, 8, 2, 2, 1.0, cap, -100, 0, 0, None),
                lib.ak_lmhead_logprobs_fwd(16, 16, None, None, None, None, None, 0, 8, 16, 64, 64, 64, 1.0, cap, -100, 2, None)):
         assert rc == -1 and b"softcap" in lib.ak_last_error()
+
+
+@pytest.mark.parametrize("inside", [True, False])
+def test_lmhead_fp32_keeps_its_type_under_autocast(scoring_backend, monkeypatch, inside):
+    """The logits of the forward and those that the backward forms again are fp32, and
+    results and gradients are those without autocast, inside the block and behind it."""
+    seen = []
+    for name in ("token_logprobs", "token_logprobs_bwd"):
+        fn = getattr(_lib, name)
+        monkeypatch.setattr(_lib, name, lambda x, *a, fn=fn: (seen.append(x.dtype), fn(x, *a))[1])
+    g = torch.Generator().manual_seed(1)
+    h, w = torch.randn(5, 40, generator=g, requires_grad=True), torch.randn(30, 40, generator=g, requires_grad=True)
+    tok = torch.tensor([1, 29, -100, 3, 4])
+
+    def call():
+        r = ll.kernel_fn(h, w, tok, chunk_size=2)
+        return list(r), r.logprobs.sum() + 0.5 * r.entropy.sum()
+
+    outs, total = call()
+    want = [*outs, *torch.autograd.grad(total, (h, w))]
+    with torch.autocast("cpu", dtype=torch.bfloat16):
+        outs, total = call()
+        if inside:
+            grads = torch.autograd.grad(total, (h, w))
+    if not inside:
+        grads = torch.autograd.grad(total, (h, w))
+    assert set(seen) == {torch.float32} and len(seen) == 12
+    assert all(torch.equal(a, b) for a, b in zip([*outs, *grads], want))
