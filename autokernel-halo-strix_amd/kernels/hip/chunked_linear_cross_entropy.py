@@ -24,7 +24,7 @@ every dot product) and the gradients are cut back to ``d`` columns.
 
 For fp32 inputs the forward runs the reference's row-chunked algorithm: per
 ``chunk_size`` rows a GEMM (``torch.nn.functional.linear``) feeds the gfx950
-CE row kernel.
+CE row kernel (under autocast too: operands keep their type).
 
 Backward (the fused forward's conditions): ``ak_lmhead_ce_bwd``
 recomputes the logits tile by tile on the matrix cores from the saved
@@ -265,6 +265,14 @@ def lmhead_ce_backward(hidden: torch.Tensor, weight: torch.Tensor, targets: torc
     return gradients_by_ranges(hidden, weight, write_range, d_in, need_hidden, need_weight)
 
 
+def own_types(t: torch.Tensor):
+    """GEMMs in the operands' type whatever autocast is in force: a backward
+    forms the logits again, often behind the autocast block that the forward ran
+    in, and its probabilities sum to 1 only over the logits that the statistics
+    are of."""
+    return torch.autocast(t.device.type, enabled=False)
+
+
 def _chunked_forward(hidden, weight, targets, chunk_size, softcap, ignore_index, label_smoothing):
     """Row-chunked GEMM + CE row kernel; returns (loss_sum, lse, n_valid float tensor)."""
     from kernels.ce_fused import _get_fwd_module
@@ -274,7 +282,8 @@ def _chunked_forward(hidden, weight, targets, chunk_size, softcap, ignore_index,
     loss_sum = torch.zeros((), dtype=torch.float32, device=hidden.device)
     for start in range(0, n, chunk_size):
         end = min(start + chunk_size, n)
-        logits = F.linear(hidden[start:end], weight)
+        with own_types(hidden):
+            logits = F.linear(hidden[start:end], weight)
         t = targets[start:end]
         losses, lse_c, _, _, _ = mod.cross_entropy_fwd_hip(
             logits, t, float(softcap), int(ignore_index), float(label_smoothing), 0, 0, 1.0)
@@ -327,18 +336,19 @@ class _ChunkedLinearCrossEntropy(torch.autograd.Function):
             w = weight.contiguous()
             h = hidden.contiguous()
             n = h.shape[0]
-            for start in range(0, n, ctx.chunk_size):
-                end = min(start + ctx.chunk_size, n)
-                logits = F.linear(h[start:end], w)
-                # softmax = exp(x - lse) / 1: lse as the row max and 1 as the row sum
-                glog = torch.empty_like(logits)
-                _lib.ce_bwd_tiny(logits, targets[start:end], lse[start:end], ones[start:end], glog,
-                                 ctx.softcap, ctx.ignore_index, ctx.label_smoothing, 1.0,
-                                 scale_dev=scale)
-                if need_h:
-                    grad_hidden[start:end] = glog @ w
-                if need_w:
-                    grad_weight.addmm_(glog.t().to(torch.float32), h[start:end].to(torch.float32))
+            with own_types(h):
+                for start in range(0, n, ctx.chunk_size):
+                    end = min(start + ctx.chunk_size, n)
+                    logits = F.linear(h[start:end], w)
+                    # softmax = exp(x - lse) / 1: lse as the row max and 1 as the row sum
+                    glog = torch.empty_like(logits)
+                    _lib.ce_bwd_tiny(logits, targets[start:end], lse[start:end], ones[start:end], glog,
+                                     ctx.softcap, ctx.ignore_index, ctx.label_smoothing, 1.0,
+                                     scale_dev=scale)
+                    if need_h:
+                        grad_hidden[start:end] = glog @ w
+                    if need_w:
+                        grad_weight.addmm_(glog.t().to(torch.float32), h[start:end].to(torch.float32))
             if need_w:
                 grad_weight = grad_weight.to(weight.dtype)
         return grad_hidden, grad_weight, None, None, None, None, None, None

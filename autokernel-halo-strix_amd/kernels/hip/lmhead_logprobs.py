@@ -29,7 +29,7 @@ import torch.nn.functional as F
 
 from kernels.hip import _lib
 from kernels.hip import chunked_linear_cross_entropy as clce
-from kernels.hip.chunked_linear_cross_entropy import _fused_ok, _kernel_operands, gradients_by_ranges
+from kernels.hip.chunked_linear_cross_entropy import _fused_ok, _kernel_operands, gradients_by_ranges, own_types
 from kernels.hip.token_logprobs import check_scale, differentiable_once, row_gradient, whole_numbers
 
 KERNEL_TYPE = "lmhead_logprobs"
@@ -48,13 +48,6 @@ def _rows(t, start, end):
     return t[start:end] if t is not None else None
 
 
-def _own_types(t):
-    """GEMMs in the operands' type whatever autocast is in force: the backward
-    forms the logits again, often behind the autocast block that the forward ran
-    in, and its probabilities sum to 1 only over the logits that the statistics
-    are of."""
-    return torch.autocast(t.device.type, enabled=False)
-
 
 def _forward(hidden, weight, tokens, temperature, softcap, ignore_index, chunk_size, keep):
     """``(logprobs, entropy, stats)``."""
@@ -68,7 +61,7 @@ def _forward(hidden, weight, tokens, temperature, softcap, ignore_index, chunk_s
         h, w = _kernel_operands(hidden, weight)
         _lib.lmhead_logprobs(h, w, tokens, logprobs, entropy, stats, temperature, softcap, ignore_index)
     elif n:
-        with _own_types(hidden):
+        with own_types(hidden):
             for start in range(0, n, chunk_size):
                 end = min(start + chunk_size, n)
                 _lib.token_logprobs(F.linear(hidden[start:end], weight), _rows(tokens, start, end),
@@ -114,7 +107,7 @@ class _LmheadLogprobs(torch.autograd.Function):
             stats = stats.contiguous()
             gh = torch.empty_like(h) if need_h else None
             gw = torch.zeros(weight.shape, dtype=torch.float32, device=weight.device) if need_w else None
-            with _own_types(h):
+            with own_types(h):
                 for start in range(0, n, ctx.chunk_size):
                     end = min(start + ctx.chunk_size, n)
                     logits = F.linear(h[start:end], w)

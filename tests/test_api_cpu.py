@@ -661,3 +661,23 @@ def test_lmhead_backward_vocab_range_plan(monkeypatch):
         assert all((v1 - v0) % 256 == 0 for v0, v1 in r[:-1])
         assert max(-(-(v1 - v0) // 256) for v0, v1 in r) <= cap
         assert len(r) == -(-tiles // cap)
+
+
+@pytest.mark.parametrize("inside", [True, False])
+def test_chunked_loss_keeps_its_type_under_autocast(fake_backend, inside):
+    """fp32 operands: the logits of the forward and those that the backward forms
+    again are fp32, inside an autocast block and behind it."""
+    from kernels.hip.chunked_linear_cross_entropy import ChunkedLinearCrossEntropyLoss
+    g = torch.Generator().manual_seed(1)
+    h, w = torch.randn(9, 40, generator=g, requires_grad=True), torch.randn(30, 40, generator=g, requires_grad=True)
+    t = torch.tensor([1, 29, -100, 3, 4, 0, 0, 7, 8])
+    fn = ChunkedLinearCrossEntropyLoss(chunk_size=4)
+    loss = fn(h, w, t)
+    want = [loss, *torch.autograd.grad(loss, (h, w))]
+    with torch.autocast("cpu", dtype=torch.bfloat16):
+        loss = fn(h, w, t)
+        if inside:
+            grads = torch.autograd.grad(loss, (h, w))
+    if not inside:
+        grads = torch.autograd.grad(loss, (h, w))
+    assert all(torch.equal(a, b) for a, b in zip([loss, *grads], want))
