@@ -416,6 +416,8 @@ lmhead_ce_tile_kernel(const T* __restrict__ H, const T* __restrict__ W, MSPair* 
         const float lse2 = kEnt ? pre_co[tb][0] : pre_lse[tb] * kLog2e;
         const float cl2 = kCap ? ga.cap * (kEnt ? ga.c2 : kLog2e) - lse2 : 0.0f;  // log2 of exp(cap - lse)
         const float c0 = kEnt ? pre_co[tb][1] : 0.0f, c1 = kEnt ? pre_co[tb][2] : 0.0f;
+        // a row without a gradient stores zeros whatever its logits are (NaN times 0 is NaN)
+        const bool still = kEnt && c0 == 0.0f && c1 == 0.0f;
         const int64_t tg = kEnt ? 0 : pre_tg[tb];
         const float st = tg == ga.ignore_index ? 0.0f : ((tg < 0 || tg >= ga.vocab_total) ? NAN : gs);
         const float nls = kEnt ? 0.0f : -(ga.ls / (float)ga.vocab_total) * st;  // label smoothing's uniform term
@@ -454,7 +456,10 @@ lmhead_ce_tile_kernel(const T* __restrict__ H, const T* __restrict__ W, MSPair* 
             }
             const int x0 = vb * 32 + 8 * g4;  // row of e[0] in the half, as counted by lo / hi
 #pragma unroll
-            for (int j = 0; j < 2; ++j) pk[g4][j] = pack2<T>(e[2 * j], e[2 * j + 1]);
+            for (int j = 0; j < 2; ++j) {
+              pk[g4][j] = pack2<T>(e[2 * j], e[2 * j + 1]);
+              if constexpr (kEnt) pk[g4][j] = still ? 0u : pk[g4][j];
+            }
             if constexpr (kEdge) {
               T* const q = drow + 4 * khalf + x0;
               if (tok_ok && x0 >= lo && x0 + 4 <= hi) {
@@ -462,7 +467,7 @@ lmhead_ce_tile_kernel(const T* __restrict__ H, const T* __restrict__ W, MSPair* 
               } else if (tok_ok) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                  if (x0 + j >= lo && x0 + j < hi) q[j] = from_f32<T>(e[j]);
+                  if (x0 + j >= lo && x0 + j < hi) q[j] = from_f32<T>(still ? 0.0f : e[j]);
               }
             }
           }
@@ -1152,13 +1157,12 @@ lmhead_logprob_coef_kernel(const int64_t* __restrict__ tokens, const f32x4_t* __
   if (row >= n_rows) return;
   const f32x4_t st = stats[row];
   float g = tokens && g_logprobs ? g_logprobs[row] : 0.0f, e = g_entropy ? g_entropy[row] : 0.0f;
-  const bool empty = st[0] == INFINITY;  // no gradient, t = -inf
-  if (empty) g = e = 0.0f;
-  if (tokens) {
-    const int64_t t = tokens[row];
-    if (t == ignore_index || empty) g = e = 0.0f;
-    else if (t < 0 || t >= vocab) g = NAN;
+  const int64_t t = tokens ? tokens[row] : 0;
+  if (st[0] == INFINITY || (tokens && t == ignore_index)) {  // no distribution, or ignored: no gradient
+    coefs[row] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};            // (an ignored row's statistics may be NaN)
+    return;
   }
+  if (tokens && (t < 0 || t >= vocab)) g = NAN;
   g *= inv_t;
   e *= inv_t;
   // with t = z' c2 - lse2 in place of log2 p = t - rest, p = 2^t 2^-rest
@@ -1180,6 +1184,7 @@ lmhead_logprob_grad_token_kernel(const T* __restrict__ H, const T* __restrict__ 
   const float z = wave_dot(H + (int64_t)tok * ldh, W + tl * ldw, d);
   if ((threadIdx.x & 63) != 0) return;
   const f32x4_t co = ga.coefs[tok];
+  if (co[1] == 0.0f && co[2] == 0.0f && co[3] == 0.0f) return;  // no gradient: the tile's 0 stays
   const float t = fmaf(capped(z, ga.cap), ga.c2, -co[0]);
   float slope = 1.0f;
   if (ga.cap > 0.0f) {

@@ -132,8 +132,9 @@ def kernel_fn(hidden: torch.Tensor, weight: torch.Tensor, tokens: Optional[torch
         tokens: whole numbers of the leading shape, or None (no ``logprobs``).
         temperature: divides the (capped) logits; at least 1e-3.
         softcap: logit softcap, 1e-3 to 1e4 (0 = off), as in ``token_logprobs``.
-        ignore_index: token value of rows to leave out (their hidden states
-            have to be finite where ``weight``'s gradient is asked for).
+        ignore_index: token value of rows to leave out, whatever they and
+            their logits hold; but ``weight``'s gradient sums 0 times their
+            hidden states, which have to be finite where it is asked for.
         chunk_size: rows per chunk of the fp32 path's GEMMs.
     """
     temperature, softcap, ignore_index, chunk_size = float(temperature), float(softcap), int(ignore_index), int(chunk_size)

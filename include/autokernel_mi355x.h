@@ -418,7 +418,8 @@ int ak_lmhead_logprobs_fwd(const void* hidden, const void* weight, const int64_t
  * Its backward, first half: the row coefficients (coefs [n_rows, 4] fp32,
  * 16-byte aligned) from the upstream gradients (fp32 [n_rows]; NULL: none), and
  * then the gradient of the logits over the vocab columns [v_begin, v_begin +
- * v_count), as ak_token_logprobs_bwd gives it, in the element type (grad_logits
+ * v_count), as ak_token_logprobs_bwd gives it (zeros for rows of an ignored token
+ * and rows of -inf alone, whatever they hold), in the element type (grad_logits
  * and ranges as for ak_lmhead_ce_bwd_range). The two products after it are
  * ak_lmhead_grad_hidden and ak_lmhead_grad_weight.
  */

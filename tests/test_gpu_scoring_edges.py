@@ -6,6 +6,8 @@ Tolerances are those of the row and head tests, whose derivation stands there;
 what is added here is derived at its test.
 """
 
+import math
+
 import pytest
 import torch
 
@@ -40,3 +42,43 @@ def test_head_in_fp32_under_autocast(inside):
     if not inside:
         got = torch.autograd.grad(total, (h, w))
     assert all(torch.equal(a, b) for a, b in zip([*r, *got], want))
+
+
+@pytest.mark.parametrize("n", [40, 300])
+@pytest.mark.parametrize("softcap", [0.0, 5.0])
+@pytest.mark.parametrize("every", [3, 1])
+def test_head_ignored_rows_hold_anything(n, softcap, every):
+    """Ignored rows of NaN, of infinities and of finite values whose logits pass
+    fp32: results and hidden states' gradients 0, everything else as without them.
+    ``every``: every third row, or a run of rows in front."""
+    need_gpu()
+    from kernels.hip.lmhead_logprobs import kernel_fn
+    say("head ignored", n, softcap, every)
+    h, w, t = operands(n, 1153, 64, torch.bfloat16, 23)
+    gone = torch.zeros(n, dtype=torch.bool)
+    gone[::3] = every == 3
+    gone[:n // 3] |= every == 1
+    t[1:4] = 7
+    t[gone] = -100
+    at = gone.nonzero().flatten()
+    up = torch.randn(2, n, generator=torch.Generator().manual_seed(2)).to(DEV)
+
+    def run(h, need_w):
+        hl, wl = h.to(DEV).requires_grad_(), w.to(DEV).requires_grad_(need_w)
+        r = kernel_fn(hl, wl, t.to(DEV), temperature=0.7, softcap=softcap)
+        return [*r, *torch.autograd.grad([r.logprobs, r.entropy], [hl, wl][:1 + need_w], list(up))]
+
+    calm = h.clone()
+    calm[at] = 0.0
+    want = run(calm, True)
+    assert all(bool(torch.isfinite(a).all()) for a in want)
+    past = h.clone()  # finite, with logits of either infinity and of both at once
+    past[at] = 3e38 * h[at].sign().where(h[at] != 0, torch.ones((), dtype=h.dtype))
+    wild = h.clone()
+    wild[at[::2]] = math.nan
+    wild[at[1::2]] = math.inf
+    for x, need_w in ((past, True), (wild, False)):
+        got = run(x, need_w)
+        assert bool((got[0][at] == 0).all()) and bool((got[1][at] == 0).all()) and bool((got[2][at] == 0).all())
+        # the other rows' tiles do not see them; the weight's gradient has zeros of them
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
