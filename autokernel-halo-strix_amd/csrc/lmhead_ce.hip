@@ -145,6 +145,9 @@ struct Cap {
   float k2, nc;
   __device__ __forceinline__ explicit Cap(float cap) : k2(2.0f * kLog2e / cap), nc(-2.0f * cap * kLog2e) {}
   __device__ __forceinline__ float q(float z) const { return __builtin_amdgcn_exp2f(z * k2); }
+  // 1 - tanh^2 = 4 q r^2, without 4 q = inf on the way to 0: q is held at 2^125
+  // (z = 43 cap), beyond which r^2 falls as q^-2 or is 0.
+  static __device__ __forceinline__ float slope(float q, float r) { return 4.0f * fminf(q, 0x1p125f) * r * r; }
 };
 
 // Partial of vocab tile vt, vocab half h (0/1), token t: part[(2 vt + h) * n_rows + t].
@@ -438,7 +441,7 @@ lmhead_ce_tile_kernel(const T* __restrict__ H, const T* __restrict__ W, MSPair* 
                   const float q = cp.q(z);
                   const float r = __builtin_amdgcn_rcpf(q + 1.0f);
                   t = fmaf(-2.0f * ga.cap * ga.c2, r, cl2);
-                  slope = q < INFINITY ? 4.0f * q * r * r : 0.0f;
+                  slope = Cap::slope(q, r);
                 } else {
                   t = fmaf(z, ga.c2, -lse2);
                 }
@@ -1189,7 +1192,7 @@ lmhead_logprob_grad_token_kernel(const T* __restrict__ H, const T* __restrict__ 
   float slope = 1.0f;
   if (ga.cap > 0.0f) {
     const float q = Cap(ga.cap).q(z), r = __builtin_amdgcn_rcpf(q + 1.0f);
-    slope = q < INFINITY ? 4.0f * q * r * r : 0.0f;
+    slope = Cap::slope(q, r);
   }
   static_cast<T*>(ga.dz)[(int64_t)tok * ga.ld_dz + tl] =
       from_f32<T>(fmaf(__builtin_amdgcn_exp2f(t), fmaf(co[2], fmaxf(t, -1000.0f), co[1]), co[3]) * slope);

@@ -12,7 +12,7 @@ import pytest
 import torch
 
 from gpu_util import gpu, need_gpu, say
-from test_gpu_lmhead_logprobs import operands
+from test_gpu_lmhead_logprobs import HALF, check, operands
 from test_gpu_scoring import DEV
 
 pytestmark = gpu
@@ -42,6 +42,28 @@ def test_head_in_fp32_under_autocast(inside):
     if not inside:
         got = torch.autograd.grad(total, (h, w))
     assert all(torch.equal(a, b) for a, b in zip([*r, *got], want))
+
+
+def saturated(n, dtype, sign):
+    """Hidden states and weights whose logits are sign * (38, 38.25, ..., 53.75) on
+    vocab rows 0..63 and small elsewhere: with a cap of 1, exp(2 z) leaves fp32."""
+    h, w, t = operands(n, 300, 64, dtype, 17, scale=0.5)
+    h[:, 0] = 1.0
+    w[:, 0] = 0.0
+    w[:64] = 0.0
+    w[:64, 0] = sign * (38.0 + 0.25 * torch.arange(64.0))
+    t[:] = torch.arange(n) % 64
+    return h, w, t
+
+
+@pytest.mark.parametrize("dtype", HALF, ids=str)
+@pytest.mark.parametrize("n", [5, 300])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_head_gradients_of_saturated_caps(dtype, n, sign):
+    """The cap's slope goes to e^-108 without passing an infinity on the way."""
+    need_gpu()
+    say("saturated", dtype, n, sign)
+    check(*saturated(n, dtype, sign), 1.0, 1.0)
 
 
 @pytest.mark.parametrize("n", [40, 300])
