@@ -452,7 +452,7 @@ lmhead_ce_tile_kernel(const T* __restrict__ H, const T* __restrict__ W, MSPair* 
                 const float q = cp.q(z);
                 const float r = __builtin_amdgcn_rcpf(q + 1.0f);
                 const float p = __builtin_amdgcn_exp2f(fmaf(cp.nc, r, cl2));
-                e[j] = fmaf(p, st, nls) * (4.0f * q * r * r);
+                e[j] = fmaf(p, st, nls) * Cap::slope(q, r);
               } else {
                 e[j] = fmaf(__builtin_amdgcn_exp2f(fmaf(z, kLog2e, -lse2)), st, nls);
               }
@@ -843,7 +843,7 @@ lmhead_ce_grad_target_kernel(const T* __restrict__ H, const T* __restrict__ W, G
       const float q = cp.q(acc);
       const float r = __builtin_amdgcn_rcpf(q + 1.0f);
       const float p = __builtin_amdgcn_exp2f(fmaf(cp.nc, r, (ga.cap - ga.lse[tok]) * kLog2e));
-      g = (p - (1.0f - ga.ls) - ga.ls / (float)ga.vocab_total) * gs * (4.0f * q * r * r);
+      g = (p - (1.0f - ga.ls) - ga.ls / (float)ga.vocab_total) * gs * Cap::slope(q, r);
     } else {
       const float p = __builtin_amdgcn_exp2f((acc - ga.lse[tok]) * kLog2e);
       g = (p - (1.0f - ga.ls) - ga.ls / (float)ga.vocab_total) * gs;

@@ -13,7 +13,7 @@ import torch
 
 from gpu_util import gpu, need_gpu, say
 from test_gpu_lmhead_logprobs import HALF, check, operands
-from test_gpu_scoring import DEV
+from test_gpu_scoring import DEV, TINY
 
 pytestmark = gpu
 
@@ -64,6 +64,34 @@ def test_head_gradients_of_saturated_caps(dtype, n, sign):
     need_gpu()
     say("saturated", dtype, n, sign)
     check(*saturated(n, dtype, sign), 1.0, 1.0)
+
+
+@pytest.mark.parametrize("n", [5, 300])
+@pytest.mark.parametrize("dtype", HALF, ids=str)
+def test_loss_gradients_of_saturated_caps(dtype, n):
+    """The same of the head's loss: dz = (p - [target]) / n (1 - tanh^2), within one
+    rounding of the type and 2e-6 of the scale 1 / n, as its other tests."""
+    need_gpu()
+    from kernels.hip import _lib
+    from kernels.hip.chunked_linear_cross_entropy import ChunkedLinearCrossEntropyLoss, lmhead_ce_forward
+    say("saturated loss", dtype, n)
+    for sign, size in ((1, 1.0), (-1, 1.0), (1, 16.0)):  # (and far past the range)
+        h, w, t = saturated(n, dtype, sign)
+        w[:64] *= size
+        hd, wd, td = h.to(DEV), w.to(DEV), t.to(DEV)
+        _, lse, nv = lmhead_ce_forward(hd, wd, td, softcap=1.0)
+        dz = torch.empty(n, 300, dtype=dtype, device=DEV)
+        _lib.lmhead_ce_bwd(hd, wd, td, lse, torch.ones(1, device=DEV), nv.float(), dz, -100, 1.0)
+        x = h.double() @ w.double().t()
+        p = torch.softmax(torch.tanh(x), 1)
+        p[torch.arange(n), t] -= 1
+        ref = p / torch.cosh(x.clamp(-300, 300)) ** 2 / n
+        got = dz.double().cpu()
+        tol = torch.finfo(dtype).eps / 2 * ref.abs() + 2e-6 / n + TINY[dtype]
+        assert bool(((got - ref).abs() <= tol).all())
+        hl, wl = hd.clone().requires_grad_(), wd.clone().requires_grad_()
+        gh, gw = torch.autograd.grad(ChunkedLinearCrossEntropyLoss(softcap=1.0)(hl, wl, td), (hl, wl))
+        assert bool(torch.isfinite(gh).all()) and bool(torch.isfinite(gw).all())
 
 
 @pytest.mark.parametrize("n", [40, 300])
