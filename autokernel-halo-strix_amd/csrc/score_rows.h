@@ -311,12 +311,13 @@ constexpr int kGradThreads = 256;
 
 // d(score / temperature) / d(logit), and the score (as many_score). The slope 1 -
 // tanh^2 as 4 q / (1 + q)^2 with q = exp(2 x / cap): a difference from 1 would
-// have nothing left where the cap is near.
+// have nothing left where the cap is near. (q may be inf, r 0 then: q is held at
+// 2^125, up to which r q is 1 and the slope keeps its digits.)
 template <typename T, bool CAP>
 __device__ __forceinline__ float score_and_slope(const ScoreParams& p, float x, float& slope) {
   if constexpr (CAP && !std::is_same<T, float>::value) {
     const float q = __builtin_amdgcn_exp2f(x * p.k2), r = __builtin_amdgcn_rcpf(1.0f + q);
-    slope = 4.0f * p.inv_t * r * (r * fminf(q, 1e30f));  // (q may be inf, r 0 then)
+    slope = 4.0f * p.inv_t * r * (r * fminf(q, 0x1p125f));
     return fmaf(-2.0f * p.cap, r, p.cap);
   }
   if constexpr (CAP) {

@@ -12,8 +12,9 @@ import pytest
 import torch
 
 from gpu_util import gpu, need_gpu, say
+from oracle import scoring
 from test_gpu_lmhead_logprobs import HALF, check, operands
-from test_gpu_scoring import DEV, TINY
+from test_gpu_scoring import DEV, DTYPES, ROW, TINY, close
 
 pytestmark = gpu
 
@@ -92,6 +93,24 @@ def test_loss_gradients_of_saturated_caps(dtype, n):
         hl, wl = hd.clone().requires_grad_(), wd.clone().requires_grad_()
         gh, gw = torch.autograd.grad(ChunkedLinearCrossEntropyLoss(softcap=1.0)(hl, wl, td), (hl, wl))
         assert bool(torch.isfinite(gh).all()) and bool(torch.isfinite(gw).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_row_gradients_of_saturated_caps(dtype):
+    """The slope keeps its relative accuracy down to the smallest normal number: with
+    the given token beside the cap, dx = (1 - p) 4 e^-2a, a = x / cap up to 43; the
+    exponent 2 a is rounded to u of it, 43 * 2 u < ROW."""
+    need_gpu()
+    from kernels.hip.token_logprobs import kernel_fn
+    say("row slopes", dtype)
+    a = torch.arange(30.0, 43.0, 0.25)
+    x = torch.zeros(len(a), 700)
+    x[:, 5] = a
+    t = torch.full((len(a),), 5)
+    leaf = x.to(dtype).to(DEV).requires_grad_()
+    (g,) = torch.autograd.grad(kernel_fn(leaf, t.to(DEV), softcap=1.0).logprobs.sum(), leaf)
+    ref, size = scoring.logprob_grad_rows(x.to(dtype), t, torch.ones(len(a)), None, 1.0, 1.0)
+    close(g, ref, (2 * ROW + torch.finfo(dtype).eps / 2) * size * 1.001 + TINY[dtype] + 1e-45, "gradient")
 
 
 @pytest.mark.parametrize("n", [40, 300])
