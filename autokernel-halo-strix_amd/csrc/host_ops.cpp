@@ -645,8 +645,11 @@ bool leading_i64(const Tensor& t, const Tensor& x) {
 Tensor row_gradient(const Tensor& g) { return g.defined() ? g.detach().to(at::kFloat).contiguous() : g; }
 
 // The kernels' results carry no graph: what should have a gradient would pass as a constant.
-void differentiable_once(const char* name) {
+void differentiable_once(const char* name, const variable_list& upstream) {
   TORCH_CHECK(!at::GradMode::is_enabled(), name, " is differentiable once: its backward takes no create_graph=True");
+  for (const Tensor& g : upstream)
+    TORCH_CHECK(!g.defined() || !g._fw_grad(0).defined(), name,
+                " has no forward-mode derivative: its backward is the derivative there is");
 }
 
 struct Tops {
@@ -689,7 +692,7 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
     return out;
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
-    differentiable_once("token_logprobs");
+    differentiable_once("token_logprobs", g);
     const auto s = ctx->get_saved_variables();
     const auto p = ctx->saved_data["p"].toDoubleVector();
     const Tensor x = s[0].contiguous(), t = saved_as(s[1], at::kLong), stats = saved_as(s[2], at::kFloat);
@@ -750,7 +753,7 @@ struct TopkDistillation : torch::autograd::Function<TopkDistillation> {
     return mean ? r.loss : r.losses;
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
-    differentiable_once("topk_distillation");
+    differentiable_once("topk_distillation", g);
     const auto s = ctx->get_saved_variables();
     const auto p = ctx->saved_data["p"].toDoubleVector();
     const Tensor x = s[0].contiguous(), teacher = s[1].contiguous(), ids = saved_as(s[2], at::kLong);
@@ -808,7 +811,7 @@ struct LmheadLogprobs : torch::autograd::Function<LmheadLogprobs> {
     return out;
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
-    differentiable_once("lmhead_logprobs");
+    differentiable_once("lmhead_logprobs", g);
     const auto s = ctx->get_saved_variables();
     const auto p = ctx->saved_data["p"].toDoubleVector();
     const int64_t ignore = ctx->saved_data["ignore"].toInt();

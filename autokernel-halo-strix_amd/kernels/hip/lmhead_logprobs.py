@@ -30,7 +30,8 @@ import torch.nn.functional as F
 from kernels.hip import _lib
 from kernels.hip import chunked_linear_cross_entropy as clce
 from kernels.hip.chunked_linear_cross_entropy import _fused_ok, _kernel_operands, gradients_by_ranges, own_types
-from kernels.hip.token_logprobs import check_scale, differentiable_once, row_gradient, whole_numbers
+from kernels.hip.token_logprobs import (check_scale, differentiable_once, refuse_tangents, row_gradient,
+                                        whole_numbers)
 
 KERNEL_TYPE = "lmhead_logprobs"
 BACKEND = "hip"
@@ -83,7 +84,7 @@ class _LmheadLogprobs(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, g_logprobs, g_entropy):
-        differentiable_once(KERNEL_TYPE)
+        differentiable_once(KERNEL_TYPE, g_logprobs, g_entropy)
         hidden, weight, tokens, stats = ctx.saved_tensors
         need_h, need_w = ctx.needs_input_grad[:2]
         gl, ge = row_gradient(g_logprobs), row_gradient(g_entropy)
@@ -145,6 +146,7 @@ def kernel_fn(hidden: torch.Tensor, weight: torch.Tensor, tokens: Optional[torch
         if out is not None:
             return LmheadLogprobs(*out)
     _lib.require_device(hidden, weight, tokens)
+    refuse_tangents(KERNEL_TYPE, hidden, weight)
     _lib.dtype_code(hidden.dtype)
     if hidden.dim() == 0 or weight.dim() != 2 or weight.shape[1] != hidden.shape[-1]:
         raise ValueError(f"hidden shape {tuple(hidden.shape)} does not go with weight {tuple(weight.shape)}")

@@ -33,6 +33,7 @@ import os
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from kernels.hip import _lib
 
@@ -69,11 +70,18 @@ def whole_numbers(t: torch.Tensor, name: str, shape) -> torch.Tensor:
     return t.to(torch.int64).contiguous()
 
 
-def differentiable_once(name: str) -> None:
+def refuse_tangents(name: str, *tensors: Optional[torch.Tensor]) -> None:
+    """Refuse forward mode: the kernels would drop a tangent without a word."""
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f"{name} has no forward-mode derivative: its backward is the derivative there is")
+
+
+def differentiable_once(name: str, *upstream: Optional[torch.Tensor]) -> None:
     """Refuse a backward that is itself to be differentiated (its kernels' results
     carry no graph: what should have a gradient would pass as a constant)."""
     if torch.is_grad_enabled():
         raise RuntimeError(f"{name} is differentiable once: its backward takes no create_graph=True")
+    refuse_tangents(name, *upstream)
 
 
 def row_gradient(g: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
@@ -119,7 +127,7 @@ class _TokenLogprobs(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, g_logprobs, g_entropy, *unused):
-        differentiable_once(KERNEL_TYPE)
+        differentiable_once(KERNEL_TYPE, g_logprobs, g_entropy)
         rows2d, tokens, stats = ctx.saved_tensors
         grad = torch.empty(ctx.shape, dtype=rows2d.dtype, device=rows2d.device)
         if grad.numel():
@@ -150,6 +158,7 @@ def kernel_fn(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, *, te
         if out is not None:
             return TokenLogprobs(*out)
     _lib.require_device(logits, tokens)
+    refuse_tangents(KERNEL_TYPE, logits)
     vocab = check_vocab(logits)
     lead = logits.shape[:-1]
     check_scale(temperature, softcap)

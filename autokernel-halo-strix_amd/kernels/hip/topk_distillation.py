@@ -34,8 +34,8 @@ import os
 import torch
 
 from kernels.hip import _lib
-from kernels.hip.token_logprobs import (check_scale, check_vocab, differentiable_once, row_gradient,
-                                        whole_numbers)
+from kernels.hip.token_logprobs import (check_scale, check_vocab, differentiable_once, refuse_tangents,
+                                        row_gradient, whole_numbers)
 
 KERNEL_TYPE = "topk_distillation"
 BACKEND = "hip"
@@ -67,7 +67,7 @@ class _TopkDistillation(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, g_loss):
-        differentiable_once(KERNEL_TYPE)
+        differentiable_once(KERNEL_TYPE, g_loss)
         rows2d, teacher, ids, stats, scale = ctx.saved_tensors
         grad = torch.empty(ctx.shape, dtype=rows2d.dtype, device=rows2d.device)
         if grad.numel():
@@ -100,6 +100,7 @@ def kernel_fn(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_ids: t
         if loss is not None:
             return loss
     _lib.require_device(logits, teacher_logits, teacher_ids)
+    refuse_tangents(KERNEL_TYPE, logits)
     vocab = check_vocab(logits)
     if reduction not in ("mean", "none"):
         raise ValueError(f"reduction must be 'mean' or 'none', got {reduction!r}")

@@ -151,3 +151,40 @@ def test_head_ignored_rows_hold_anything(n, softcap, every):
         assert bool((got[0][at] == 0).all()) and bool((got[1][at] == 0).all()) and bool((got[2][at] == 0).all())
         # the other rows' tiles do not see them; the weight's gradient has zeros of them
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def entry_points():
+    from kernels.hip import lmhead_logprobs, token_logprobs, topk_distillation
+    g = torch.Generator().manual_seed(1)
+    x = (3 * torch.randn(2, 5, 301, generator=g)).to(DEV)
+    t = torch.randint(0, 301, (2, 5), generator=g).to(DEV)
+    t[0, 1] = -100
+    tv, ti = torch.randn(2, 5, 20, generator=g).to(DEV), torch.randint(0, 301, (2, 5, 20), generator=g).to(DEV)
+    h, w = torch.randn(2, 5, 128, generator=g).to(DEV), (0.1 * torch.randn(301, 128, generator=g)).to(DEV)
+    head = lambda h, w: lmhead_logprobs.kernel_fn(h, w, t, softcap=30.0)
+    return {
+        "logprobs": ((x,), lambda x: token_logprobs.kernel_fn(x, t, temperature=0.7, top_k=9)[:2]),
+        "distill": ((x.bfloat16(),), lambda x: [topk_distillation.kernel_fn(x, tv, ti, temperature=2.0)]),
+        "head": ((h.bfloat16(), w.bfloat16()), head),
+        "head fp32": ((h, w), head),
+    }
+
+
+@pytest.mark.parametrize("name", ["logprobs", "distill", "head", "head fp32"])
+def test_forward_mode_is_refused(name):
+    need_gpu()
+    import torch.autograd.forward_ad as fw
+    leaves, fn = entry_points()[name]
+    say("forward mode", name)
+    for i in range(len(leaves)):
+        for grad_mode in (True, False):
+            with fw.dual_level(), torch.set_grad_enabled(grad_mode):
+                args = list(leaves)
+                args[i] = fw.make_dual(args[i], torch.ones_like(args[i]))
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    fn(*args)
+    out = fn(*[a.requires_grad_() for a in leaves])[0]
+    with fw.dual_level():
+        up = fw.make_dual(torch.ones_like(out), torch.ones_like(out))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            out.backward(up)

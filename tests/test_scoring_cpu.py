@@ -403,3 +403,29 @@ def test_lmhead_fp32_keeps_its_type_under_autocast(scoring_backend, monkeypatch,
         grads = torch.autograd.grad(total, (h, w))
     assert set(seen) == {torch.float32} and len(seen) == 12
     assert all(torch.equal(a, b) for a, b in zip([*outs, *grads], want))
+
+
+def test_forward_mode_is_refused(scoring_backend):
+    """A tangent is not dropped, with gradients recorded or not; a teacher is a constant, its tangent too."""
+    import torch.autograd.forward_ad as fw
+    x, tok, ids = torch.randn(3, 8), torch.zeros(3, dtype=torch.int64), torch.zeros(3, 2, dtype=torch.int64)
+    h, w = torch.randn(3, 64), torch.randn(8, 64)
+    dual = lambda t: fw.make_dual(t, torch.ones_like(t))
+    for record in (True, False):
+        with fw.dual_level(), torch.set_grad_enabled(record):
+            for call in (lambda: tl.kernel_fn(dual(x), tok), lambda: tl.kernel_fn(dual(x), top_k=2),
+                         lambda: td.kernel_fn(dual(x), x[:, :2], ids), lambda: ll.kernel_fn(dual(h), w, tok),
+                         lambda: ll.kernel_fn(h, dual(w)), lambda: ll.kernel_fn(h.bfloat16(), dual(w), tok)):
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    call()
+            assert fw.unpack_dual(td.kernel_fn(x, dual(x[:, :2]), ids)).tangent is None
+            assert tl.kernel_fn(x, tok).logprobs.shape == (3,)  # others as ever
+    # an upstream gradient's tangent
+    leaf = x.clone().requires_grad_()
+    outs = [tl.kernel_fn(leaf, tok).logprobs, td.kernel_fn(leaf, x[:, :2], ids, reduction="none"),
+            ll.kernel_fn(h, w.clone().requires_grad_(), tok).entropy]
+    for out in outs:
+        with fw.dual_level():
+            up = dual(torch.ones(3))
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                out.backward(up)
