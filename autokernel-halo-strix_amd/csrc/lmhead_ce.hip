@@ -909,6 +909,7 @@ __device__ __forceinline__ void finish_logprob_row(MSU st, float z, int row, con
   if (tokens) {
     const int64_t t = tokens[row];
     float lp = empty ? -INFINITY : (capped(z, cap) - st.m) * inv_t - kLn2 * l2;
+    if (lp > 0.0f) lp = 0.0f;  // z and the row's sum come from two orders of additions (NaN stays)
     if (t == ignore_index) lp = h = 0.0f;
     else if (t < 0 || t >= vocab) lp = NAN;
     logprobs[row] = lp;

@@ -80,9 +80,11 @@ __device__ __forceinline__ float log2_sum(const RowStats& r) {
 }
 
 // ln p of a score; l2: log2_sum. (In natural units: a mask of the type's
-// lowest value stays in fp32's range, which its product with c2 would leave.)
+// lowest value stays in fp32's range, which its product with c2 would leave.) At
+// most 0: under a softcap y and the row's sum come from two forms of the tanh.
 __device__ __forceinline__ float log_prob(const ScoreParams& p, float y, float m, float l2) {
-  return m == -INFINITY && y == -INFINITY ? y - l2 : (y - m) * p.inv_t - kLn2 * l2;
+  const float lp = m == -INFINITY && y == -INFINITY ? y - l2 : (y - m) * p.inv_t - kLn2 * l2;
+  return lp > 0.0f ? 0.0f : lp;  // (NaN stays)
 }
 
 __device__ __forceinline__ float row_entropy(const RowStats& r) {

@@ -14,7 +14,7 @@ import torch
 from gpu_util import gpu, need_gpu, say
 from oracle import scoring
 from test_gpu_lmhead_logprobs import HALF, check, operands
-from test_gpu_scoring import DEV, DTYPES, ROW, TINY, close
+from test_gpu_scoring import DEV, DTYPES, ROW, TINY, close, logits_of
 
 pytestmark = gpu
 
@@ -151,6 +151,37 @@ def test_head_ignored_rows_hold_anything(n, softcap, every):
         assert bool((got[0][at] == 0).all()) and bool((got[1][at] == 0).all()) and bool((got[2][at] == 0).all())
         # the other rows' tiles do not see them; the weight's gradient has zeros of them
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype", HALF, ids=str)
+@pytest.mark.parametrize("n", [64, 512])
+@pytest.mark.parametrize("temperature", [1e-3, 0.02, 1.0])
+def test_head_log_probabilities_are_at_most_zero(dtype, n, temperature):
+    """The given token holds all of the row: its own dot product and the tiles' logits
+    differ by their roundings, divided by the temperature."""
+    need_gpu()
+    from kernels.hip.lmhead_logprobs import kernel_fn
+    say("head bound", dtype, n, temperature)
+    h, w, _ = operands(n, 600, 832, dtype, 29, scale=12.0)
+    t = (h.double() @ w.double().t()).argmax(1)
+    lp = kernel_fn(h.to(DEV), w.to(DEV), t.to(DEV), temperature=temperature).logprobs
+    assert bool((lp <= 0).all()), float(lp.max())
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("rows", [40, 300])
+def test_row_log_probabilities_are_at_most_zero(dtype, rows):
+    """The same with a softcap, whose tanh the sums take in a shorter form."""
+    need_gpu()
+    from kernels.hip.token_logprobs import kernel_fn
+    say("row bound", dtype, rows)
+    x = logits_of(rows, 3001, dtype, 33)
+    x[:, 11] = 20.0 + 0.125 * torch.arange(rows, device=DEV)
+    t = torch.full((rows,), 11, device=DEV)
+    for temperature in (0.01, 0.3):
+        r = kernel_fn(x, t, temperature=temperature, softcap=30.0, top_k=2)
+        assert bool((r.logprobs <= 0).all()) and bool((r.top_logprobs <= 0).all()), float(r.logprobs.max())
+        assert bool((kernel_fn(x, t, temperature=temperature, softcap=30.0).logprobs <= 0).all())
 
 
 def entry_points():
