@@ -507,27 +507,21 @@ lmhead_ce_tile_kernel(const T* __restrict__ H, const T* __restrict__ W, MSPair* 
       for (int tb = 0; tb < 4; ++tb) {
         // this token block's 64 logits of the lane, read once from the AGPRs
         float x[4][16];
+        const Cap cap(kCap ? ga.cap : 1.0f);
 #pragma unroll
         for (int vb = 0; vb < 4; ++vb)
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             x[vb][r] = acc_read(acc[vb][tb][r]);
+            // with a temperature the scores may lie far below cap / T: capped before
+            // their maximum, and before the mask (a logit of -inf is -cap, a
+            // column outside is none)
+            if constexpr (kEnt && kCap) x[vb][r] = fmaf(-2.0f * ga.cap, __builtin_amdgcn_rcpf(cap.q(x[vb][r]) + 1.0f), ga.cap);
             if (kTail) {
               const int o = vb * 32 + 8 * (r >> 2) + (r & 3);
               x[vb][r] = (o >= lo && o < hi) ? x[vb][r] : -INFINITY;
             }
           }
-        if constexpr (kEnt && kCap) {
-          // with a temperature the scores may lie far below cap / T: their own maximum
-          const Cap cp(ga.cap);
-#pragma unroll
-          for (int vb = 0; vb < 4; ++vb)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-              const float z = fmaf(-2.0f * ga.cap, __builtin_amdgcn_rcpf(cp.q(x[vb][r]) + 1.0f), ga.cap);
-              x[vb][r] = kTail && x[vb][r] == -INFINITY ? -INFINITY : z;
-            }
-        }
         if constexpr (kCap && !kEnt) {
           // (cap, sum exp(z' - cap)) with exp(z' - cap) = exp2(nc r); masked
           // rows (x = -inf) would give exp(-2 cap) and are dropped. With label

@@ -14,7 +14,7 @@ import torch
 from gpu_util import gpu, need_gpu, say
 from oracle import scoring
 from test_gpu_lmhead_logprobs import HALF, check, operands
-from test_gpu_scoring import DEV, DTYPES, ROW, TINY, close, logits_of
+from test_gpu_scoring import DEV, DTYPES, ROW, TINY, U, close, logits_of
 
 pytestmark = gpu
 
@@ -182,6 +182,34 @@ def test_row_log_probabilities_are_at_most_zero(dtype, rows):
         r = kernel_fn(x, t, temperature=temperature, softcap=30.0, top_k=2)
         assert bool((r.logprobs <= 0).all()) and bool((r.top_logprobs <= 0).all()), float(r.logprobs.max())
         assert bool((kernel_fn(x, t, temperature=temperature, softcap=30.0).logprobs <= 0).all())
+
+
+@pytest.mark.parametrize("n,vocab,live", [(5, 700, 3), (300, 700, 3), (300, 1024, 200), (300, 1153, 600), (260, 600, 599)])
+def test_head_softcap_of_infinite_logits(n, vocab, live):
+    """A logit of -inf is -softcap, wherever its column is in a tile. The live tokens'
+    logits are 0, so with k = V - live capped ones s = live + k e^(-cap / T)."""
+    need_gpu()
+    from kernels.hip.lmhead_logprobs import kernel_fn
+    say("head capped -inf", n, vocab, live)
+    g = torch.Generator().manual_seed(8)
+    w = torch.zeros(vocab, 64, dtype=torch.bfloat16)
+    w[:, 0] = -1e30
+    at = torch.randperm(vocab, generator=g)[:live]
+    w[at, 0] = 0.0
+    h = torch.zeros(n, 64, dtype=torch.bfloat16)
+    h[:, 0] = 1e30
+    t = at[torch.randint(0, live, (n,), generator=g)]
+    t[::2] = (w[:, 0] != 0).nonzero().flatten()[torch.randint(0, vocab - live, (len(t[::2]),), generator=g)]
+    x = torch.where(w[:, 0] == 0, 0.0, -math.inf).double().expand(n, vocab)
+    lp, ent = scoring.logprob_rows(x, t, 2.0, 3.0)
+    r = kernel_fn(h.to(DEV), w.to(DEV), t.to(DEV), temperature=2.0, softcap=3.0)
+    tol = ROW + 2 * 8 * U * 3.0 / 2.0
+    close(r.logprobs, lp, tol + 4 * U * lp.abs(), "logprobs")
+    close(r.entropy, ent, tol * (1 + 2 * math.log(vocab)), "entropy")
+    # saturated: no gradient but of the live tokens' columns
+    wl = w.to(DEV).requires_grad_()
+    (gw,) = torch.autograd.grad(kernel_fn(h.to(DEV), wl, t.to(DEV), temperature=2.0, softcap=3.0).entropy.sum(), wl)
+    assert bool((gw[(w[:, 0] != 0).to(DEV)] == 0).all()) and bool(torch.isfinite(gw).all())
 
 
 def entry_points():
