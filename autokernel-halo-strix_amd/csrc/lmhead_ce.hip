@@ -137,6 +137,20 @@ struct GradArgs {
   const f32x4_t* coefs;
 };
 
+// A row of ga.coefs: dz = 2^t (c0 + c1 t) with t = z' c2 - lse2. Without a softcap
+// (-inf, c0, m, g) stands for t = z' - m, and c1 = 0, where m c2 leaves fp32.
+template <bool kCap>
+struct RowCoefs {
+  float lse2, c0, c1, c2;
+  __device__ __forceinline__ RowCoefs(const f32x4_t& co, float c2_) : lse2(co[0]), c0(co[1]), c1(co[2]), c2(c2_) {
+    if (!kCap && co[0] == -INFINITY) {
+      lse2 = co[2];
+      c1 = 0.0f;
+      c2 = 1.0f;
+    }
+  }
+};
+
 // Logit softcap z' = cap * tanh(z / cap), evaluated without cancellation
 // through q = exp(2 z / cap) and r = 1 / (q + 1):
 //   z' - cap = -2 cap r,   1 - tanh^2 = 4 q r^2.
@@ -149,6 +163,11 @@ struct Cap {
   // (z = 43 cap), beyond which r^2 falls as q^-2 or is 0.
   static __device__ __forceinline__ float slope(float q, float r) { return 4.0f * fminf(q, 0x1p125f) * r * r; }
 };
+
+// c2, or 1 where m c2 leaves fp32 (a mask of bf16's lowest value fills a tile):
+// beside such an m any other logit is 2^80 and more away, so that 2^t is 1 at m
+// and 0 elsewhere with either factor.
+__device__ __forceinline__ float exponent_factor(float m, float c2) { return fabsf(m * c2) < INFINITY ? c2 : 1.0f; }
 
 // Partial of vocab tile vt, vocab half h (0/1), token t: part[(2 vt + h) * n_rows + t].
 //
@@ -416,9 +435,10 @@ lmhead_ce_tile_kernel(const T* __restrict__ H, const T* __restrict__ W, MSPair* 
         const int tok = t_first + wt * 128 + tb * 32 + fr;
         const int tok_c = min(tok, n_rows - 1);
         const bool tok_ok = tok >= t_own && tok < n_rows;
-        const float lse2 = kEnt ? pre_co[tb][0] : pre_lse[tb] * kLog2e;
+        const RowCoefs<kCap> rc(kEnt ? pre_co[tb] : f32x4_t{}, ga.c2);
+        const float lse2 = kEnt ? rc.lse2 : pre_lse[tb] * kLog2e;
         const float cl2 = kCap ? ga.cap * (kEnt ? ga.c2 : kLog2e) - lse2 : 0.0f;  // log2 of exp(cap - lse)
-        const float c0 = kEnt ? pre_co[tb][1] : 0.0f, c1 = kEnt ? pre_co[tb][2] : 0.0f;
+        const float c0 = rc.c0, c1 = rc.c1;
         // a row without a gradient stores zeros whatever its logits are (NaN times 0 is NaN)
         const bool still = kEnt && c0 == 0.0f && c1 == 0.0f;
         const int64_t tg = kEnt ? 0 : pre_tg[tb];
@@ -443,7 +463,7 @@ lmhead_ce_tile_kernel(const T* __restrict__ H, const T* __restrict__ W, MSPair* 
                   t = fmaf(-2.0f * ga.cap * ga.c2, r, cl2);
                   slope = Cap::slope(q, r);
                 } else {
-                  t = fmaf(z, ga.c2, -lse2);
+                  t = fmaf(z, rc.c2, -lse2);
                 }
                 e[j] = __builtin_amdgcn_exp2f(t) * fmaf(c1, fmaxf(t, -1000.0f), c0) * slope;
               } else if constexpr (kCap) {
@@ -563,7 +583,7 @@ lmhead_ce_tile_kernel(const T* __restrict__ H, const T* __restrict__ W, MSPair* 
           for (int r = 0; r < 16; ++r) m4[r & 3] = fmaxf(m4[r & 3], x[vb][r]);
         float m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
         m = fmaxf(m, __shfl_xor(m, 32, 64));
-        const float c2 = kEnt ? ga.c2 : kLog2e;
+        const float c2 = kEnt && !kCap ? exponent_factor(m, ga.c2) : kEnt ? ga.c2 : kLog2e;
         const float ms = kEnt && m == -INFINITY ? 0.0f : m * c2;  // logits past fp32's range: s = u = 0
         float s4[4] = {0.0f, 0.0f, 0.0f, 0.0f}, u4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -898,8 +918,13 @@ __device__ __forceinline__ void finish_logprob_row(MSU st, float z, int row, con
   const float l2 = empty ? 0.0f : __builtin_amdgcn_logf(st.s);
   float h = empty ? 0.0f : kLn2 * (l2 - st.u / st.s);
   if (h < 0.0f) h = 0.0f;  // one rounding below zero where one token holds all
-  const float lse2 = empty ? INFINITY : fmaf(st.m, c2, l2);
-  if (stats) stats[row] = f32x4_t{lse2, h, empty ? 0.0f : fmaf(st.m, c2, -lse2) + l2, 0.0f};
+  if (stats) {
+    const float lse2 = fmaf(st.m, c2, l2);
+    const bool far = fabsf(st.m) < INFINITY && exponent_factor(st.m, c2) != c2;
+    stats[row] = empty ? f32x4_t{INFINITY, h, 0.0f, 0.0f}
+                 : far ? f32x4_t{-INFINITY, h, l2, st.m}
+                       : f32x4_t{lse2, h, fmaf(st.m, c2, -lse2) + l2, 0.0f};
+  }
   if (tokens) {
     const int64_t t = tokens[row];
     float lp = empty ? -INFINITY : (capped(z, cap) - st.m) * inv_t - kLn2 * l2;
@@ -915,7 +940,8 @@ __device__ __forceinline__ void finish_logprob_row(MSU st, float z, int row, con
 // threads a token fold every 16th partial and are joined in a fixed order; the
 // workgroup's waves form the given tokens' scores as their own dot products
 // meanwhile. stats: (lse2, entropy, rest, -) of each row for the backward, lse2 =
-// m c2 + log2 s rounded and the rest that it lacks; lse2 = inf where every logit is -inf.
+// m c2 + log2 s rounded and the rest that it lacks; lse2 = inf where every logit is
+// -inf; (-inf, entropy, log2 s, m) where m c2 leaves fp32.
 template <typename T>
 __global__ void __launch_bounds__(kRowsPerBlock * kRowGroups)
 lmhead_logprob_rows_kernel(const T* __restrict__ H, const T* __restrict__ W, const MSPair* __restrict__ part,
@@ -1166,7 +1192,8 @@ lmhead_logprob_coef_kernel(const int64_t* __restrict__ tokens, const f32x4_t* __
   // with t = z' c2 - lse2 in place of log2 p = t - rest, p = 2^t 2^-rest
   const float f = __builtin_amdgcn_exp2f(-st[2]), c1 = -e * kLn2;
   const float c0 = g == 0.0f && e == 0.0f ? 0.0f : -fmaf(e, st[1], g) - c1 * st[2];
-  coefs[row] = f32x4_t{st[0], c0 * f, c1 * f, g};
+  // (where m c2 leaves fp32 only logits of m have a p, and t = 0: m in c1's place)
+  coefs[row] = f32x4_t{st[0], c0 * f, st[0] == -INFINITY ? st[3] : c1 * f, g};
 }
 
 // The given tokens' entries, from their own dot products: what the tile kernel
@@ -1182,15 +1209,16 @@ lmhead_logprob_grad_token_kernel(const T* __restrict__ H, const T* __restrict__ 
   const float z = wave_dot(H + (int64_t)tok * ldh, W + tl * ldw, d);
   if ((threadIdx.x & 63) != 0) return;
   const f32x4_t co = ga.coefs[tok];
-  if (co[1] == 0.0f && co[2] == 0.0f && co[3] == 0.0f) return;  // no gradient: the tile's 0 stays
-  const float t = fmaf(capped(z, ga.cap), ga.c2, -co[0]);
+  const RowCoefs<false> rc(co, ga.c2);
+  if (rc.c0 == 0.0f && rc.c1 == 0.0f && co[3] == 0.0f) return;  // no gradient: the tile's 0 stays
+  const float t = fmaf(capped(z, ga.cap), rc.c2, -rc.lse2);
   float slope = 1.0f;
   if (ga.cap > 0.0f) {
     const float q = Cap(ga.cap).q(z), r = __builtin_amdgcn_rcpf(q + 1.0f);
     slope = Cap::slope(q, r);
   }
   static_cast<T*>(ga.dz)[(int64_t)tok * ga.ld_dz + tl] =
-      from_f32<T>(fmaf(__builtin_amdgcn_exp2f(t), fmaf(co[2], fmaxf(t, -1000.0f), co[1]), co[3]) * slope);
+      from_f32<T>(fmaf(__builtin_amdgcn_exp2f(t), fmaf(rc.c1, fmaxf(t, -1000.0f), rc.c0), co[3]) * slope);
 }
 
 size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }

@@ -212,6 +212,55 @@ def test_head_softcap_of_infinite_logits(n, vocab, live):
     assert bool((gw[(w[:, 0] != 0).to(DEV)] == 0).all()) and bool(torch.isfinite(gw).all())
 
 
+@pytest.mark.parametrize("n", [6, 70, 300])
+@pytest.mark.parametrize("temperature", [0.25, 1.0])
+def test_head_masks_of_the_lowest_value(n, temperature):
+    """A constant hidden feature and a weight column of bf16's lowest value mask most of
+    the vocabulary with finite logits of -3.39e38, whole tiles of it, as -inf does;
+    a row of which every logit is that value is uniform."""
+    need_gpu()
+    from kernels.hip import _lib
+    from kernels.hip.lmhead_logprobs import kernel_fn
+    say("head lowest", n, temperature)
+    h, w, t = operands(n, 1153, 64, torch.bfloat16, 31)
+    low = torch.finfo(torch.bfloat16).min
+    h[:, :2], w[:, :2] = 0.0, 0.0
+    keep = torch.zeros(1153, dtype=torch.bool)
+    keep[[3, 400, 401, 1150]] = True
+    h[:, 0] = 1.0
+    w[~keep, 0] = low
+    w[:, 1] = low
+    h[2] = 0.0
+    h[2, 1] = 1.0  # nothing left: uniform
+    t[:] = torch.tensor([3, 400, 401, 1150])[torch.arange(n) % 4]
+    t[3] = 9       # masked
+    x = h.double() @ w.double().t()
+    lp, ent = scoring.logprob_rows(x, t, temperature)
+    hd, wd, td = h.to(DEV), w.to(DEV), t.to(DEV)
+    r = kernel_fn(hd, wd, td, temperature=temperature)
+    terr = (72 * U * 40 + 2 * U * 40) / temperature  # (the kept logits are sums of |h w| below 40)
+    assert float((h[:, 2:].double().abs() @ w[:, 2:].double().abs().t()).max()) < 40
+    far = lp < -1e30
+    assert far.tolist() == [i == 3 for i in range(n)] and float(r.logprobs[3]) < -1e37
+    close(r.logprobs.cpu()[~far], lp[~far], ROW + 2 * terr + 4 * U * lp[~far].abs(), "logprobs")
+    close(r.entropy, ent, (ROW + 2 * terr) * (1 + 2 * math.log(1153)), "entropy")
+    # the logits' gradient
+    f = lambda *s: torch.empty(*s, device=DEV)
+    lp2, ent2, st, co = f(n), f(n), f(n, 4), f(n, 4)
+    up = torch.randn(2, n, generator=torch.Generator().manual_seed(1))
+    dz = torch.zeros(n, 1280, dtype=torch.bfloat16, device=DEV)[:, :1153]
+    _lib.lmhead_logprobs(hd, wd, td, lp2, ent2, st, temperature, 0.0, -100)
+    _lib.lmhead_logprobs_coefs(td, st, up[0].to(DEV), up[1].to(DEV), co, 1153, temperature, -100)
+    _lib.lmhead_logprobs_bwd_range(hd, wd, td, co, dz, 0, temperature, 0.0, -100)
+    assert torch.equal(lp2, r.logprobs) and torch.equal(ent2, r.entropy)
+    ref, size = scoring.logprob_grad_rows(x, t, up[0], up[1], temperature)
+    # ln p and H are off by absolute amounts too (as in the head's other tests)
+    p = torch.softmax(scoring.scores(x, temperature), 1)
+    tol = size * (4 * terr + 2 * ROW) + p * up[1].abs()[:, None] * (ROW + 2 * terr) * (2 + 2 * math.log(1153)) / temperature
+    tol = tol + 1.01 * torch.finfo(dz.dtype).eps / 2 * ref.abs() + 2.0 ** -120
+    close(dz, ref, tol, "gradient")
+
+
 def entry_points():
     from kernels.hip import lmhead_logprobs, token_logprobs, topk_distillation
     g = torch.Generator().manual_seed(1)
