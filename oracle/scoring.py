@@ -75,6 +75,7 @@ def logprob_grad_rows(x, tokens, g_logprobs, g_entropy, temperature=1.0, softcap
     for r in range(x.shape[0]):
         t = None if tokens is None else int(tokens[r])
         if t == ignore_index or bool((z[r] == -math.inf).all()):
+            slope[r] = 0.0  # whatever the row holds (a NaN logit has a NaN slope)
             continue
         g = 0.0 if g_logprobs is None or t is None else float(g_logprobs[r])
         e = 0.0 if g_entropy is None else float(g_entropy[r])

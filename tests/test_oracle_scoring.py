@@ -80,3 +80,11 @@ def test_distillation_is_kl_div_and_differences(temperature, softcap):
     d = 1e-6 * torch.randn(5, 9, generator=g, dtype=torch.float64)
     change = value(x.detach() + d) - value(x.detach() - d)
     assert torch.allclose(change, 2 * (grad * d).sum(), rtol=1e-5, atol=1e-14)
+
+
+def test_ignored_rows_have_no_gradient_whatever_they_hold():
+    x = torch.tensor([[1.0, math.nan, 2.0], [math.inf, -math.inf, math.nan], [0.5, 1.0, -1.0]])
+    t = torch.tensor([-100, -100, 1])
+    for softcap in (0.0, 4.0):
+        grad, size = scoring.logprob_grad_rows(x, t, torch.ones(3), torch.ones(3), 0.7, softcap)
+        assert bool((grad[:2] == 0).all()) and bool((size[:2] == 0).all()) and bool(torch.isfinite(grad[2]).all())
