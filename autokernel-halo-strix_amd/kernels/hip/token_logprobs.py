@@ -20,10 +20,11 @@ Rules at the edges:
   gradient, whatever it holds (its alternatives are its own);
 * a token outside ``[0, vocab)`` that is not ``ignore_index`` gives a NaN
   logprob, and a NaN gradient row;
-* -inf masks a logit (with a softcap it becomes ``-softcap``, as any logit
-  does). A row of -inf alone has logprobs of -inf, entropy 0, a zero gradient;
-* a row that holds a NaN or +inf has NaN results, NaN first among its
-  alternatives.
+* -inf masks a logit. A row of -inf alone has logprobs of -inf, entropy 0, a zero
+  gradient. (With a softcap -inf is ``-softcap``, which masks nothing, and such
+  a row uniform.)
+* a row that holds a NaN, or without a softcap +inf (with one it becomes
+  ``softcap``), has NaN results, NaN first among its alternatives.
 
 No counterpart in the reference, whose cross-entropy
 (``kernels/ce_fused.py:557-785``) gives the loss of given tokens only.

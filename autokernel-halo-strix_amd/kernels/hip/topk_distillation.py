@@ -24,7 +24,8 @@ Rules at the edges:
 * an id outside ``[0, vocab)`` that is not ``ignore_index``, a NaN or +inf on
   either side give a NaN loss and a NaN gradient row;
 * an entry that the student masks (-inf) while the teacher has it makes the
-  row's loss +inf.
+  row's loss +inf;
+* with a softcap the student's infinities are ``softcap`` and ``-softcap``.
 
 No counterpart in the reference.
 """

@@ -245,10 +245,11 @@ int ak_scale_inplace(void* x, int64_t n, const float* scale, int dtype, void* st
  * tokens (and then logprobs), entropy and stats may be NULL. A row whose token
  * is ignore_index has logprob and entropy 0; a token outside [0, vocab) that is
  * not ignore_index has logprob NaN. A row of -inf alone has logprob -inf and
- * entropy 0; a row that holds a NaN or +inf has NaN results. stats [rows, 4]
- * fp32, 16-byte aligned, is what ak_token_logprobs_bwd takes. top_k is at most
- * 256 and vocab, vocab at most 2^20, temperature between 1e-18 and 1e18, softcap
- * 0 or between 1e-3 and 1e4. workspace: as many bytes as the query says (0
+ * entropy 0; a row that holds a NaN or +inf has NaN results (with a softcap
+ * infinities are +-softcap, and only NaN gives NaN). stats [rows, 4] fp32,
+ * 16-byte aligned, is what ak_token_logprobs_bwd takes. top_k is at most 256
+ * and vocab, vocab at most 2^20, temperature between 1e-18 and 1e18, softcap 0
+ * or between 1e-3 and 1e4. workspace: as many bytes as the query says (0
  * without alternatives for most calls; few or very wide rows are cut into
  * segments), 16-byte aligned. No counterpart in the reference, whose cross-entropy
  * (kernels/ce_fused.py:122-382) gives the loss of given tokens only.

@@ -14,7 +14,7 @@ import torch
 from gpu_util import gpu, need_gpu, say
 from oracle import scoring
 from test_gpu_lmhead_logprobs import HALF, check, operands
-from test_gpu_scoring import DEV, DTYPES, ROW, TINY, U, close, logits_of
+from test_gpu_scoring import DEV, DTYPES, ROW, TINY, U, check_distill, check_logprobs, close, logits_of, special_rows
 
 pytestmark = gpu
 
@@ -259,6 +259,30 @@ def test_head_masks_of_the_lowest_value(n, temperature):
     tol = size * (4 * terr + 2 * ROW) + p * up[1].abs()[:, None] * (ROW + 2 * terr) * (2 + 2 * math.log(1153)) / temperature
     tol = tol + 1.01 * torch.finfo(dz.dtype).eps / 2 * ref.abs() + 2.0 ** -120
     close(dz, ref, tol, "gradient")
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("vocab", [40, 3001, 40007])
+def test_special_rows_with_a_softcap(dtype, vocab):
+    """Under a softcap infinities are logits of +-softcap, a row of -inf alone is
+    uniform; NaN stay NaN."""
+    need_gpu()
+    say("special capped", dtype, vocab)
+    x = special_rows(vocab, dtype)
+    tok = torch.randint(0, vocab, (14,), generator=torch.Generator().manual_seed(2))
+    tok[1], tok[2], tok[5] = vocab // 2, vocab - 1, -100
+    r = check_logprobs(x.to(DEV), tok.to(DEV), 0.8, 7.0, top_k=min(20, vocab))
+    assert bool(torch.isfinite(r.entropy[[0, 1, 2, 3, 4, 6, 8, 9, 10, 11, 12]]).all())
+    many = x.repeat(20, 1).to(DEV)
+    from kernels.hip.token_logprobs import kernel_fn
+    whole = kernel_fn(many, tok.repeat(20).to(DEV), temperature=0.8, softcap=7.0)
+    lp, h = scoring.logprob_rows(x, tok, 0.8, 7.0)
+    close(whole.logprobs[-14:], lp, 2 * ROW + 4 * U * torch.nan_to_num(lp.abs()), "logprobs")
+    close(whole.entropy[-14:], h, 2 * ROW * (1 + 2 * math.log(vocab)), "entropy")
+    ids = torch.stack([torch.randperm(vocab, generator=torch.Generator().manual_seed(4))[:6] for _ in range(14)])
+    t = torch.randn(14, 6, generator=torch.Generator().manual_seed(5))
+    ids[8, 2], t[9, 1], t[12] = vocab, math.nan, -math.inf
+    check_distill(x.to(DEV), t.to(DEV), ids.to(DEV), 1.5, 7.0)
 
 
 def entry_points():
