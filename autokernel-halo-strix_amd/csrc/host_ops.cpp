@@ -628,7 +628,8 @@ constexpr int64_t kMaxScoreVocab = 1 << 20;
 constexpr int64_t kMaxTopEntries = 256;
 
 bool scale_args(double temperature, double softcap) {
-  return temperature >= 1e-18 && temperature <= 1e18 && (softcap == 0.0 || (softcap >= 1e-3 && softcap <= 1e4));
+  return temperature >= 1e-18 && temperature <= 1e18 &&
+         (softcap == 0.0 || (softcap >= 1e-3 && softcap <= 1e4 && softcap <= temperature * 1048576.0));
 }
 
 bool score_args(const Tensor& x, double temperature, double softcap) {

@@ -1390,6 +1390,8 @@ int check_logprobs(const char* name, const void* hidden, const void* weight, int
     return ak_set_error(AK_ERR_INVALID_ARG, "%s: temperature must be between 1e-3 and 1e18", name);
   if (!(softcap == 0.0f || (softcap >= 1e-3f && softcap <= 1e4f)))  // (as check_score_rows)
     return ak_set_error(AK_ERR_INVALID_ARG, "%s: softcap must be 0 or between 1e-3 and 1e4", name);
+  if (softcap > temperature * 0x1p20f)
+    return ak_set_error(AK_ERR_INVALID_ARG, "%s: softcap must be at most 2^20 temperatures", name);
   if (dtype != AK_DTYPE_BF16 && dtype != AK_DTYPE_F16)
     return ak_set_error(AK_ERR_UNSUPPORTED, "%s: dtype must be bf16 or fp16", name);
   if (n_rows <= 0 || vocab <= 0 || d <= 0 || n_rows > (1 << 30) || vocab > (1 << 30) || d > (1 << 20))

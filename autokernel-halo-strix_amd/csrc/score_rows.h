@@ -405,6 +405,10 @@ inline int check_score_rows(const char* name, int64_t rows, int64_t vocab, int64
   // the cap's tanh is within 2^-22 of 1: of a larger cap that is more than the logits' own rounding
   if (!(softcap == 0.0f || (softcap >= 1e-3f && softcap <= 1e4f)))
     return ak_set_error(AK_ERR_INVALID_ARG, "%s: softcap must be 0 or between 1e-3 and 1e4", name);
+  // the scores are off by that over the temperature: a quarter there, and further on
+  // an element's may pass the row's maximum by more than 2^t holds
+  if (softcap > temperature * 0x1p20f)
+    return ak_set_error(AK_ERR_INVALID_ARG, "%s: softcap must be at most 2^20 temperatures", name);
   return AK_OK;
 }
 

@@ -60,6 +60,9 @@ def check_scale(temperature: float, softcap: float, least: float = 1e-18) -> Non
         raise ValueError(f"temperature must be between {least:g} and 1e18, got {temperature}")
     if softcap != 0.0 and not 1e-3 <= softcap <= 1e4:
         raise ValueError(f"softcap must be 0 (off) or between 1e-3 and 1e4, got {softcap}")
+    # the capped scores are exact to 2^-22 softcap / temperature: a quarter there
+    if softcap > temperature * 2 ** 20:
+        raise ValueError(f"softcap must be at most 2^20 temperatures, got {softcap} and {temperature}")
 
 
 def whole_numbers(t: torch.Tensor, name: str, shape) -> torch.Tensor:
@@ -147,8 +150,9 @@ def kernel_fn(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, *, te
         logits: ``[..., vocab]`` fp32, fp16 or bf16, vocab at most 2^20.
         tokens: whole numbers of the leading shape, or None (no ``logprobs``).
         temperature: divides the (capped) logits.
-        softcap: logit softcap, 1e-3 to 1e4 (0 = off); scores are exact to
-            ``2^-22 softcap / temperature`` under it.
+        softcap: logit softcap, 1e-3 to 1e4 (0 = off) and at most ``2^20
+            temperature``; scores are exact to ``2^-22 softcap / temperature``
+            under it.
         ignore_index: token value of rows to leave out.
         top_k: alternatives of each row, 0 to min(256, vocab).
     """

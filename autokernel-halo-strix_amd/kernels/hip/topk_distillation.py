@@ -88,7 +88,7 @@ def kernel_fn(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_ids: t
         teacher_logits: ``[..., k]`` of any of these types, ``k`` from 1 to 256.
         teacher_ids: whole numbers ``[..., k]``, the columns of ``teacher_logits``.
         temperature: divides both sides' logits.
-        softcap: the student's logit softcap, 1e-3 to 1e4 (0 = off).
+        softcap: the student's logit softcap, as in ``token_logprobs``.
         ignore_index: id of entries that are not there.
         reduction: ``"mean"`` over the rows that have entries (a 0-d tensor),
             or ``"none"`` (one loss a row).

@@ -249,7 +249,8 @@ int ak_scale_inplace(void* x, int64_t n, const float* scale, int dtype, void* st
  * infinities are +-softcap, and only NaN gives NaN). stats [rows, 4] fp32,
  * 16-byte aligned, is what ak_token_logprobs_bwd takes. top_k is at most 256
  * and vocab, vocab at most 2^20, temperature between 1e-18 and 1e18, softcap 0
- * or between 1e-3 and 1e4. workspace: as many bytes as the query says (0
+ * or between 1e-3 and 1e4 and at most 2^20 temperatures (scores are exact to
+ * 2^-22 softcap / temperature). workspace: as many bytes as the query says (0
  * without alternatives for most calls; few or very wide rows are cut into
  * segments), 16-byte aligned. No counterpart in the reference, whose cross-entropy
  * (kernels/ce_fused.py:122-382) gives the loss of given tokens only.

@@ -14,7 +14,8 @@ import torch
 from gpu_util import gpu, need_gpu, say
 from oracle import scoring
 from test_gpu_lmhead_logprobs import HALF, check, operands
-from test_gpu_scoring import DEV, DTYPES, ROW, TINY, U, check_distill, check_logprobs, close, logits_of, special_rows
+from test_gpu_scoring import (DEV, DTYPES, ROW, TINY, U, check_distill, check_logprobs, close, logits_of,
+                              special_rows, teacher_of)
 
 pytestmark = gpu
 
@@ -283,6 +284,29 @@ def test_special_rows_with_a_softcap(dtype, vocab):
     t = torch.randn(14, 6, generator=torch.Generator().manual_seed(5))
     ids[8, 2], t[9, 1], t[12] = vocab, math.nan, -math.inf
     check_distill(x.to(DEV), t.to(DEV), ids.to(DEV), 1.5, 7.0)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_softcaps_that_temperatures_leave_without_digits(dtype):
+    """The cap's tanh is within 2^-22: up to 2^20 temperatures of it the scores keep
+    digits, and past that the calls are refused."""
+    need_gpu()
+    from kernels.hip.lmhead_logprobs import kernel_fn as head
+    from kernels.hip.token_logprobs import kernel_fn as logprobs
+    from kernels.hip.topk_distillation import kernel_fn as distill
+    say("cap and temperature", dtype)
+    x = logits_of(9, 1500, dtype, 31)
+    t = torch.randint(0, 1500, (9,), generator=torch.Generator().manual_seed(5)).to(DEV)
+    check_logprobs(x, t, 30 * 2.0 ** -20, 30.0, grads=False)
+    tv, ti = teacher_of(x, 20, 6)
+    h = torch.randn(9, 64, device=DEV).to(dtype)
+    for cap, temperature in ((1e4, 1e-3), (30.0, 1e-18), (30.0, 2.0 ** -16)):
+        with pytest.raises(ValueError, match="softcap"):
+            logprobs(x, t, softcap=cap, temperature=temperature)
+        with pytest.raises(ValueError, match="softcap"):
+            distill(x, tv, ti, softcap=cap, temperature=temperature)
+    with pytest.raises(ValueError, match="softcap"):
+        head(h, torch.randn(1500, 64, device=DEV).to(dtype), t, softcap=1e4, temperature=1e-3)
 
 
 def entry_points():

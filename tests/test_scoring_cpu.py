@@ -429,3 +429,28 @@ def test_forward_mode_is_refused(scoring_backend):
             up = dual(torch.ones(3))
             with pytest.raises(RuntimeError, match="forward-mode"):
                 out.backward(up)
+
+
+@pytest.mark.parametrize("cap,temperature", [(1e4, 1e-3), (30.0, 1e-18), (30.0, 2e-5)])
+def test_softcaps_that_the_temperature_leaves_without_digits(scoring_backend, cap, temperature):
+    """Capped scores are exact to 2^-22 cap / T: a cap over 2^20 temperatures is refused."""
+    x, tok, ids = torch.randn(3, 8), torch.zeros(3, dtype=torch.int64), torch.zeros(3, 2, dtype=torch.int64)
+    kw = dict(softcap=cap, temperature=temperature)
+    with pytest.raises(ValueError, match="softcap"):
+        tl.kernel_fn(x, tok, **kw)
+    with pytest.raises(ValueError, match="softcap"):
+        td.kernel_fn(x, x[:, :2], ids, **kw)
+    if temperature >= 1e-3:
+        with pytest.raises(ValueError, match="softcap"):
+            ll.kernel_fn(torch.randn(3, 64), torch.randn(8, 64), tok, **kw)
+    tl.kernel_fn(x, tok, softcap=cap, temperature=cap / 2 ** 20)
+
+
+@pytest.mark.parametrize("cap,t", [(1e4, 1e-3), (30.0, 2e-5)])
+def test_library_refuses_softcaps_of_too_many_temperatures(lib, cap, t):
+    calls = [lib.ak_token_logprobs_fwd(16, None, None, None, None, None, None, None, 0, 600, 8, 8, 0, t, cap, -100, 0, None),
+             lib.ak_token_logprobs_bwd(16, None, 16, None, None, 16, 4, 8, 8, 8, t, cap, -100, 0, None),
+             lib.ak_topk_distill_fwd(16, 16, 16, 16, 16, None, None, None, 0, 600, 8, 2, 8, 2, 2, t, cap, -100, 0, 0, None)]
+    if t >= 1e-3:
+        calls.append(lib.ak_lmhead_logprobs_fwd(16, 16, None, None, None, None, None, 0, 8, 16, 64, 64, 64, t, cap, -100, 2, None))
+    assert all(rc == -1 for rc in calls) and b"softcap" in lib.ak_last_error()
