@@ -14,12 +14,15 @@ import torch
 from gpu_util import gpu, need_gpu, say
 from oracle import scoring
 from test_gpu_lmhead_logprobs import HALF, check, operands
-from test_gpu_scoring import (DEV, DTYPES, ROW, TINY, U, check_distill, check_logprobs, close, logits_of,
+from test_gpu_scoring import (DEV, DTYPES, ROW, TINY, U, check_distill, check_logprobs, close, grad_tol, logits_of,
                               special_rows, teacher_of)
 
 pytestmark = gpu
 
 
+# ---------------------------------------------------------------------------
+# Autocast
+# ---------------------------------------------------------------------------
 @pytest.mark.parametrize("inside", [True, False])
 def test_head_in_fp32_under_autocast(inside):
     """fp32 operands keep their type under autocast: logits, and the gradient's
@@ -46,6 +49,9 @@ def test_head_in_fp32_under_autocast(inside):
     assert all(torch.equal(a, b) for a, b in zip([*r, *got], want))
 
 
+# ---------------------------------------------------------------------------
+# Saturated softcaps
+# ---------------------------------------------------------------------------
 def saturated(n, dtype, sign):
     """Hidden states and weights whose logits are sign * (38, 38.25, ..., 53.75) on
     vocab rows 0..63 and small elsewhere: with a cap of 1, exp(2 z) leaves fp32."""
@@ -114,6 +120,9 @@ def test_row_gradients_of_saturated_caps(dtype):
     close(g, ref, (2 * ROW + torch.finfo(dtype).eps / 2) * size * 1.001 + TINY[dtype] + 1e-45, "gradient")
 
 
+# ---------------------------------------------------------------------------
+# Ignored rows
+# ---------------------------------------------------------------------------
 @pytest.mark.parametrize("n", [40, 300])
 @pytest.mark.parametrize("softcap", [0.0, 5.0])
 @pytest.mark.parametrize("every", [3, 1])
@@ -154,6 +163,9 @@ def test_head_ignored_rows_hold_anything(n, softcap, every):
         assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+# ---------------------------------------------------------------------------
+# Log probabilities are at most 0
+# ---------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", HALF, ids=str)
 @pytest.mark.parametrize("n", [64, 512])
 @pytest.mark.parametrize("temperature", [1e-3, 0.02, 1.0])
@@ -185,6 +197,9 @@ def test_row_log_probabilities_are_at_most_zero(dtype, rows):
         assert bool((kernel_fn(x, t, temperature=temperature, softcap=30.0).logprobs <= 0).all())
 
 
+# ---------------------------------------------------------------------------
+# Infinities and lowest values
+# ---------------------------------------------------------------------------
 @pytest.mark.parametrize("n,vocab,live", [(5, 700, 3), (300, 700, 3), (300, 1024, 200), (300, 1153, 600), (260, 600, 599)])
 def test_head_softcap_of_infinite_logits(n, vocab, live):
     """A logit of -inf is -softcap, wherever its column is in a tile. The live tokens'
@@ -257,7 +272,8 @@ def test_head_masks_of_the_lowest_value(n, temperature):
     ref, size = scoring.logprob_grad_rows(x, t, up[0], up[1], temperature)
     # ln p and H are off by absolute amounts too (as in the head's other tests)
     p = torch.softmax(scoring.scores(x, temperature), 1)
-    tol = size * (4 * terr + 2 * ROW) + p * up[1].abs()[:, None] * (ROW + 2 * terr) * (2 + 2 * math.log(1153)) / temperature
+    tol = size * (4 * terr + 2 * ROW)
+    tol = tol + p * up[1].abs()[:, None] * (ROW + 2 * terr) * (2 + 2 * math.log(1153)) / temperature
     tol = tol + 1.01 * torch.finfo(dz.dtype).eps / 2 * ref.abs() + 2.0 ** -120
     close(dz, ref, tol, "gradient")
 
@@ -309,6 +325,9 @@ def test_softcaps_that_temperatures_leave_without_digits(dtype):
         head(h, torch.randn(1500, 64, device=DEV).to(dtype), t, softcap=1e4, temperature=1e-3)
 
 
+# ---------------------------------------------------------------------------
+# Forward mode, torch.compile, many rows
+# ---------------------------------------------------------------------------
 def entry_points():
     from kernels.hip import lmhead_logprobs, token_logprobs, topk_distillation
     g = torch.Generator().manual_seed(1)
@@ -344,3 +363,65 @@ def test_forward_mode_is_refused(name):
         up = fw.make_dual(torch.ones_like(out), torch.ones_like(out))
         with pytest.raises(RuntimeError, match="forward-mode"):
             out.backward(up)
+
+
+@pytest.mark.parametrize("name", ["logprobs", "distill", "head", "head fp32"])
+def test_under_torch_compile(name):
+    need_gpu()
+    import torch._dynamo
+    import torch._dynamo.compiled_autograd as compiled
+    leaves, fn = entry_points()[name]
+    say("compile", name)
+    leaves = [a.requires_grad_() for a in leaves]
+    outs = fn(*leaves)
+    want = [*outs, *torch.autograd.grad(sum(o.sum() for o in outs), leaves)]
+    torch._dynamo.reset()
+    outs = torch.compile(fn, backend="eager")(*leaves)
+    got = [*outs, *torch.autograd.grad(sum(o.sum() for o in outs), leaves)]
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    total = sum(o.sum() for o in fn(*leaves))
+    with compiled._enable(torch.compile(backend="eager")):
+        total.backward()
+    torch._dynamo.reset()
+    for a, b in zip(leaves, want[len(outs):]):
+        assert torch.equal(a.grad, b)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=str)
+def test_more_rows_than_workgroups(dtype):
+    """2^20 + 3 rows of a small vocabulary, and the last ones checked."""
+    need_gpu()
+    from kernels.hip.token_logprobs import kernel_fn as logprobs
+    from kernels.hip.topk_distillation import kernel_fn as distill
+    say("many rows", dtype)
+    n = (1 << 20) + 3
+    g = torch.Generator(device=DEV).manual_seed(3)
+    x = (2 * torch.randn(n, 8, generator=g, device=DEV)).to(dtype).requires_grad_()
+    t = torch.randint(0, 8, (n,), generator=g, device=DEV)
+    t[::5] = -100
+    r = logprobs(x, t, top_k=3)
+    part = slice(n - 9, n)
+    xc, tc = x.detach()[part].cpu(), t[part].cpu()
+    lp, h = scoring.logprob_rows(xc, tc)
+    tv, ti = scoring.top_rows(xc, 3)
+    close(r.logprobs[part], lp, ROW + 4 * U * lp.abs(), "logprobs")
+    close(r.entropy[part], h, ROW * (1 + 2 * math.log(8)), "entropy")
+    close(r.top_logprobs[part], tv, ROW + 4 * U * tv.abs(), "top_logprobs")
+    assert torch.equal(r.top_ids[part].cpu(), ti)
+    assert torch.equal(logprobs(x, t).logprobs, r.logprobs) and torch.equal(r.logprobs == 0, t == -100)
+    (gx,) = torch.autograd.grad(r.logprobs.sum() + 0.5 * r.entropy.sum(), x)
+    ref, size = scoring.logprob_grad_rows(xc, tc, torch.ones(9), 0.5 * torch.ones(9))
+    close(gx[part], ref, grad_tol(ref, size, dtype, 1.0, 0.0), "gradient")
+    ids, tl = torch.randint(0, 8, (n, 2), generator=g, device=DEV), torch.randn(n, 2, generator=g, device=DEV)
+    losses = distill(x, tl, ids, reduction="none")
+    want, _, _ = scoring.distill_rows(xc, tl[part].cpu(), ids[part].cpu())
+    close(losses[part], want, 2 * ROW + 24 * U * (1 + math.log(8) + 2 * xc.double().abs().amax(1)), "losses")
+    (gx,) = torch.autograd.grad(losses.sum(), x)
+    ref, size = scoring.distill_grad_rows(xc, tl[part].cpu(), ids[part].cpu(), torch.ones(9))
+    close(gx[part], ref, 2 * grad_tol(ref, size, dtype, 1.0, 0.0), "distillation gradient")
+
+
+def test_head_fp32_beyond_one_chunk():
+    need_gpu()
+    say("head fp32 chunks")
+    check(*operands(1100, 301, 40, torch.float32, 6), 1.2)
