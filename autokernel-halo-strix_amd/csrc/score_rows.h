@@ -13,11 +13,12 @@
 // A row is cut into `segs` segments of `span` 16-byte vectors. One workgroup
 // holds a segment in registers, packed, so that it crosses HBM once, 16 vectors
 // a thread where it is that wide: with 8 in twice the threads, the same bytes in
-// flight and twice the waves at each barrier, [8192, 50304] bf16 took 157 us
-// where it takes 145, and [4096, 32768] with the groups' maxima, whose registers
-// spilled, 70 us for 49. One segment a row where rows fill the GPU and a row fits a workgroup; otherwise
-// each segment leaves its (m, s, u) in a workspace and a second kernel joins
-// them, as a decode step's few rows need every CU (plan below).
+// flight and twice the waves at each barrier, [8192, 50304] bf16 takes 233 us
+// for 152 to 160, [4096, 50257] bf16 and fp16 123 for 84, the distillation step
+// of [1999, 50257] fp32 262 for 216, [4096, 32768] bf16 with 64 alternatives 80
+// for 76. One segment a row where rows fill the GPU and a row fits a workgroup;
+// otherwise each segment leaves its (m, s, u) in a workspace and a second kernel
+// joins them, as a decode step's few rows need every CU (plan below).
 #pragma once
 
 #include <algorithm>

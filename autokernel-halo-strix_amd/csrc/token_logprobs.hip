@@ -10,9 +10,11 @@
 // HBM-bound: the forward reads the logits once (score_rows.h; of many rows, not
 // those of an ignored token), the backward
 // reads them once and writes the gradient once. Measured (a copy of 1 GiB here:
-// 5.1 TB/s): [8192, 50304] bf16 forward 145 us, 5.7 TB/s; [4096, 50257] bf16
-// forward and backward 79 + 130 us, 5.9 TB/s of the three passes; [8, 50257]
-// with 20 alternatives, a decode step, 12 us, two launches of 3.6 and 8 us.
+// 5.1 TB/s): [8192, 50304] bf16 forward 152 to 160 us, 5.2 TB/s and more, 116 to
+// 122 with a quarter of the rows ignored, 136 to 143 for the entropy alone (no
+// token's logit to fetch); [4096, 50257] bf16, a quarter ignored, forward 65 us,
+// forward and backward 196, 5.2 TB/s over the three passes; [8, 50257] with 20
+// alternatives, a decode step, 12 us, two kernels of 3.8 and 9.7 us in a trace.
 //
 // Alternatives. The first kernel, which has the logits in registers, also
 // writes the maximum of each group of consecutive logits (128 bytes of the row
@@ -67,10 +69,10 @@ struct LogprobArgs {
   float* maxima;          // top > 0: [rows, groups] maxima of 2^shift vectors each
   int top, vocab, groups, shift;
   // Whether rows of an ignored token are left unread. The token is then waited for
-  // before the row: [8192, 50304] bf16 153 to 160 us (152 without), a quarter of it
-  // ignored 118 (146), [4096, 50257] 81 (81) and 63 (80), [2000, 50257] fp32 67 (65)
-  // and 53 (65). Few rows, which wait for
-  // latency alone, are read.
+  // before the row: [8192, 50304] bf16 152 to 156 us (154 to 157 without), a quarter
+  // of it ignored 116 to 119 (150 to 154), [4096, 50257] 82 to 85 (81 to 84) and 65
+  // (81), [2000, 50257] fp32 68 (66) and 54 (66). Few rows, which wait for latency
+  // alone, are read.
   bool skip;
 };
 

@@ -11,7 +11,8 @@ the logits on the matrix cores and folds each tile into a maximum, ``sum e^t``
 and ``sum e^t t`` of each token in registers; a row kernel joins them and adds
 the given tokens' scores as their own dot products. The backward forms the
 tiles again, writes the logits' gradient in the input type (one rounding, as
-both products after it take that type) for as much of the vocabulary at a time
+both products after it take that type; fp16 loses entries below 6e-8 unless the
+caller scales its loss) for as much of the vocabulary at a time
 as ``GRAD_LOGITS_BUDGET`` of the loss allows, and runs the loss's two gradient
 GEMMs on it. For fp32 the logits of ``chunk_size`` rows at a time come from a
 GEMM and go through the row kernels (under autocast too: operands keep their
