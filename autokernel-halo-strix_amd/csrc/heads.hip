@@ -1,0 +1,800 @@
+// Rotary positions, head norms and the paged cache's appends for gfx950.
+//
+// Per token and head of dim elements, in fp32 with one final rounding:
+//   n = x / sqrt(mean(x^2) + eps) * weight     (where the heads are normed)
+//   y = the pairs of n's first `rotary` elements turned by the token's angles,
+//       (y0, y1) = (n0 cos - n1 sin, n1 cos + n0 sin), the rest as it is
+// A pair is (i, i + rotary / 2), or interleaved (2 i, 2 i + 1). The cosines and
+// sines of a position are a row of an fp32 table ([positions][2][rotary / 2],
+// made once in float64): an angle of a far position in fp32 has lost the digits
+// that matter. Backward, with dz = dy turned back and r = 1 / rms:
+//   dx = r (g - n mean(g n)),  g = dz weight,  n = x r;  dweight = sum of dz n
+//
+// HBM-bound: every element is read once and written once, the table's rows
+// come from the caches. One head's row belongs to the fewest lanes (a power of
+// two) that hold it in units of two 16-byte vectors: the two vectors of a unit
+// hold the two halves of its pairs, so the turn needs no exchange between
+// lanes, and only the norm's sum crosses them (DPP).
+#include <algorithm>
+#include <utility>
+
+#include "heads.h"
+
+namespace ak {
+namespace {
+
+constexpr int kThreads = 256;
+
+// One of the tensors whose heads a call walks over: element strides, the last
+// dimension dense.
+struct HeadRows {
+  const void* x;
+  void* y;
+  const void* w;      // the norm's weight, or NULL
+  int64_t so, si, sh; // of x: outer, inner (token), head
+  int64_t yt, ys, yh; // of y: token and head; of a cache: page, slot and head
+  int64_t heads;
+};
+
+struct HeadArgs {
+  HeadRows r[3];      // queries, keys, values (the last two into the cache where there is one)
+  const float* table;
+  const void* positions;
+  int64_t tokens, inner, n_positions, table_rows;
+  int64_t all_heads, total;  // heads of all tensors, rows: tokens times them
+  int dim, rotary, lpr_log2;
+  int interleaved, inverse, pos64, zero_tail;
+  float eps;
+  // the cache
+  Sequences seq;
+  const int32_t* pages;
+  int64_t n_pages, page_size, max_pages, ld_pages;
+};
+
+__device__ __forceinline__ int64_t div_small(int64_t a, int64_t b) {
+  if (((a | b) >> 32) == 0) return (uint32_t)a / (uint32_t)b;
+  return a / b;
+}
+
+// The sum over the 2^log2 lanes of a row (aligned to their number).
+__device__ __forceinline__ float lanes_sum(float v, int log2) {
+  if (log2 > 0) v += dpp<kDppXor1>(v);
+  if (log2 > 1) v += dpp<kDppXor2>(v);
+  if (log2 > 2) v += dpp<kDppHalfMirror>(v);
+  if (log2 > 3) v += dpp<kDppMirror>(v);
+  if (log2 > 4) v += __shfl_xor(v, 16, kWave);
+  if (log2 > 5) v += __shfl_xor(v, 32, kWave);
+  return v;
+}
+
+// Where a unit's two vectors stand in the head, and whether they are turned.
+template <int VE>
+struct Unit {
+  int off0, off1;
+  bool turned, has0, has1;
+  __device__ __forceinline__ Unit(int u, const HeadArgs& a) {
+    const int ur = a.rotary / (2 * VE);
+    turned = u < ur;
+    if (turned) {
+      off0 = a.interleaved ? 2 * u * VE : u * VE;
+      off1 = a.interleaved ? off0 + VE : a.rotary / 2 + u * VE;
+    } else {
+      off0 = a.rotary + 2 * (u - ur) * VE;
+      off1 = off0 + VE;
+    }
+    has0 = off0 < a.dim;
+    has1 = off1 < a.dim;
+  }
+};
+
+// The angles of a unit's VE pairs: cosines and sines (negated for the way back).
+template <int VE>
+__device__ __forceinline__ void load_angles(const HeadArgs& a, int64_t pos, int u, float (&c)[VE], float (&s)[VE]) {
+  if (pos < 0 || pos >= a.table_rows) {
+#pragma unroll
+    for (int e = 0; e < VE; ++e) c[e] = s[e] = __builtin_nanf("");
+    return;
+  }
+  const float* row = a.table + pos * a.rotary + u * VE;
+#pragma unroll
+  for (int e = 0; e < VE; e += 4) {
+    const Vec16<float> cv = load16(row + e), sv = load16(row + a.rotary / 2 + e);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      c[e + i] = cv.e[i];
+      s[e + i] = a.inverse ? -sv.e[i] : sv.e[i];
+    }
+  }
+}
+
+template <int VE>
+__device__ __forceinline__ void turn(float (&p)[VE], float (&q)[VE], const float (&c)[VE], const float (&s)[VE],
+                                     bool interleaved) {
+  if (interleaved) {
+#pragma unroll
+    for (int e = 0; e < VE; e += 2) {
+      const float p0 = p[e], p1 = p[e + 1], q0 = q[e], q1 = q[e + 1];
+      const float pc = c[e / 2], ps = s[e / 2], qc = c[VE / 2 + e / 2], qs = s[VE / 2 + e / 2];
+      p[e] = p0 * pc - p1 * ps;
+      p[e + 1] = p1 * pc + p0 * ps;
+      q[e] = q0 * qc - q1 * qs;
+      q[e + 1] = q1 * qc + q0 * qs;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < VE; ++e) {
+      const float x0 = p[e], x1 = q[e];
+      p[e] = x0 * c[e] - x1 * s[e];
+      q[e] = x1 * c[e] + x0 * s[e];
+    }
+  }
+}
+
+__device__ __forceinline__ int64_t position_of(const HeadArgs& a, int64_t token) {
+  const int64_t i = token < a.n_positions ? token : token - div_small(token, a.n_positions) * a.n_positions;
+  if (a.positions == nullptr) return i;
+  return a.pos64 ? static_cast<const int64_t*>(a.positions)[i] : (int64_t)static_cast<const int32_t*>(a.positions)[i];
+}
+
+// What a row of the walk is: its tensor, token and head, where it is read and
+// written, and the position whose angles turn it.
+template <typename T>
+struct Row {
+  const T* x;
+  T* y;
+  const T* w;
+  int64_t pos;
+  bool write, zero, rotate;
+};
+
+// All lanes of a wave call this together, their rows in ascending order.
+template <typename T, bool APPEND>
+__device__ __forceinline__ Row<T> row_of(const HeadArgs& a, int64_t row, bool live) {
+  Row<T> o;
+  const int64_t token = div_small(row, a.all_heads);
+  int64_t h = row - token * a.all_heads;
+  int kind = 0;
+  if (h >= a.r[0].heads) {
+    h -= a.r[0].heads;
+    kind = 1;
+    if (APPEND && h >= a.r[1].heads) {
+      h -= a.r[1].heads;
+      kind = 2;
+    }
+  }
+  // (field by field: an index would put the arguments into scratch memory)
+#define AK_PICK(f) (kind == 0 ? a.r[0].f : kind == 1 ? a.r[1].f : a.r[2].f)
+  o.x = static_cast<const T*>(AK_PICK(x)) + h * AK_PICK(sh);
+  if (a.inner < a.tokens) {
+    const int64_t outer = div_small(token, a.inner);
+    o.x += outer * AK_PICK(so) + (token - outer * a.inner) * AK_PICK(si);
+  } else {
+    o.x += token * AK_PICK(si);
+  }
+  o.w = static_cast<const T*>(AK_PICK(w));
+  o.y = static_cast<T*>(AK_PICK(y)) + h * AK_PICK(yh);
+  o.rotate = kind < 2;
+  o.zero = false;
+  o.write = live;
+  if constexpr (!APPEND) {
+    o.pos = position_of(a, token);
+    o.y += token * AK_PICK(yt);
+  } else {
+    const int64_t b = sequence_of(a.seq, token);
+    o.pos = -1;
+    if (b >= 0) {
+      int64_t first, count;
+      sequence_tokens(a.seq, b, first, count);
+      o.pos = (int64_t)a.seq.lengths[b] - count + (token - first);
+    }
+    if (kind == 0) {
+      o.y += token * a.r[0].yt;
+      o.zero = b < 0;
+      o.write = live && (b >= 0 || a.zero_tail);
+    } else {
+      int64_t page = -1, slot = 0;
+      if (o.pos >= 0) {
+        const int64_t i = div_small(o.pos, a.page_size);
+        slot = o.pos - i * a.page_size;
+        if (i < a.max_pages) page = a.pages[b * a.ld_pages + i];
+      }
+      o.write = live && page >= 0 && page < a.n_pages;
+      if (o.write) o.y += page * AK_PICK(yt) + slot * AK_PICK(ys);
+    }
+  }
+#undef AK_PICK
+  return o;
+}
+
+// Rows of whole vectors: 16-byte aligned, dim a multiple of a vector and the
+// turned part one of two.
+template <typename T, bool NORM, bool APPEND>
+__global__ void __launch_bounds__(kThreads) heads_kernel(HeadArgs a) {
+  constexpr int VE = Vec16<T>::VE;
+  const int lpr = 1 << a.lpr_log2, per = kThreads >> a.lpr_log2;
+  const int u = threadIdx.x & (lpr - 1);
+  const Unit<VE> unit(u, a);
+  for (int64_t base = (int64_t)blockIdx.x * per; base < a.total; base += (int64_t)gridDim.x * per) {
+    const int64_t row = base + (threadIdx.x >> a.lpr_log2);
+    const Row<T> o = row_of<T, APPEND>(a, min(row, a.total - 1), row < a.total);
+    Vec16<T> v0, v1;
+    v0.u = v1.u = u32x4{0, 0, 0, 0};
+    if (unit.has0) v0 = load16(o.x + unit.off0);
+    if (unit.has1) v1 = load16(o.x + unit.off1);
+    if (!NORM && APPEND && !o.rotate) {  // values are copied
+      if (o.write && unit.has0) store16(o.y + unit.off0, v0);
+      if (o.write && unit.has1) store16(o.y + unit.off1, v1);
+      continue;
+    }
+    float p[VE], q[VE];
+#pragma unroll
+    for (int e = 0; e < VE; ++e) {
+      p[e] = to_f32(v0.e[e]);
+      q[e] = to_f32(v1.e[e]);
+    }
+    if constexpr (NORM) {
+      float ss = 0.0f;
+#pragma unroll
+      for (int e = 0; e < VE; ++e) ss = fmaf(p[e], p[e], fmaf(q[e], q[e], ss));
+      ss = lanes_sum(ss, a.lpr_log2);
+      if (o.w != nullptr) {
+        const float inv = 1.0f / sqrtf(ss / (float)a.dim + a.eps);
+        Vec16<T> w0, w1;
+        w0.u = w1.u = u32x4{0, 0, 0, 0};
+        if (unit.has0) w0 = load16(o.w + unit.off0);
+        if (unit.has1) w1 = load16(o.w + unit.off1);
+#pragma unroll
+        for (int e = 0; e < VE; ++e) {
+          p[e] = p[e] * inv * to_f32(w0.e[e]);
+          q[e] = q[e] * inv * to_f32(w1.e[e]);
+        }
+      }
+    }
+    if (unit.turned && o.rotate) {
+      float c[VE], s[VE];
+      load_angles<VE>(a, o.pos, u, c, s);
+      turn<VE>(p, q, c, s, a.interleaved);
+    }
+    if (o.write) {
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        v0.e[e] = o.zero ? from_f32<T>(0.0f) : from_f32<T>(p[e]);
+        v1.e[e] = o.zero ? from_f32<T>(0.0f) : from_f32<T>(q[e]);
+      }
+      if (unit.has0) store16(o.y + unit.off0, v0);
+      if (unit.has1) store16(o.y + unit.off1, v1);
+    }
+  }
+}
+
+// Element i of a head's pair list: its two places.
+__device__ __forceinline__ void pair_at(const HeadArgs& a, int i, int& e0, int& e1) {
+  e0 = a.interleaved ? 2 * i : i;
+  e1 = a.interleaved ? 2 * i + 1 : a.rotary / 2 + i;
+}
+
+__device__ __forceinline__ void angle_at(const HeadArgs& a, int64_t pos, int i, float& c, float& s) {
+  c = s = __builtin_nanf("");
+  if (pos >= 0 && pos < a.table_rows) {
+    c = a.table[pos * a.rotary + i];
+    s = a.table[pos * a.rotary + a.rotary / 2 + i];
+    if (a.inverse) s = -s;
+  }
+}
+
+// Every other row: a wave each, one element or pair a lane at a time.
+template <typename T, bool NORM, bool APPEND>
+__global__ void __launch_bounds__(kThreads) heads_any_kernel(HeadArgs a) {
+  const int lane = threadIdx.x & 63;
+  for (int64_t base = (int64_t)blockIdx.x * 4; base < a.total; base += (int64_t)gridDim.x * 4) {
+    const int64_t row = base + (threadIdx.x >> 6);
+    const Row<T> o = row_of<T, APPEND>(a, min(row, a.total - 1), row < a.total);
+    float inv = 1.0f;
+    const bool norm = NORM && o.w != nullptr;
+    if (norm) {
+      float ss = 0.0f;
+      for (int d = lane; d < a.dim; d += 64) {
+        const float x = to_f32(o.x[d]);
+        ss = fmaf(x, x, ss);
+      }
+      inv = 1.0f / sqrtf(wave_sum(ss) / (float)a.dim + a.eps);
+    }
+    if (!o.write) continue;
+    auto value = [&](int d) {
+      const float x = to_f32(o.x[d]);
+      return norm ? x * inv * to_f32(o.w[d]) : x;
+    };
+    const int turned = o.rotate ? a.rotary : 0;
+    for (int i = lane; i < turned / 2; i += 64) {
+      int e0, e1;
+      pair_at(a, i, e0, e1);
+      float c, s;
+      angle_at(a, o.pos, i, c, s);
+      const float x0 = value(e0), x1 = value(e1);
+      o.y[e0] = from_f32<T>(o.zero ? 0.0f : x0 * c - x1 * s);
+      o.y[e1] = from_f32<T>(o.zero ? 0.0f : x1 * c + x0 * s);
+    }
+    for (int d = turned + lane; d < a.dim; d += 64) o.y[d] = from_f32<T>(o.zero ? 0.0f : value(d));
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Backward of the norm with the rotation
+// ---------------------------------------------------------------------------
+struct GradRows {
+  const void *x, *g, *w;
+  void* dx;              // dense [tokens, heads, dim]
+  void* dw;              // [dim] of the element type, or NULL
+  int64_t so, si, sh;    // of x
+  int64_t go, gi, gh;    // of g
+  int64_t heads, rows;
+  int first_block, blocks;
+};
+
+struct GradArgs {
+  GradRows r[2];
+  HeadArgs h;            // the angles
+  float* part;           // [blocks of both][dim]
+};
+
+template <typename T>
+struct GradRow {
+  const T *x, *g;
+  int64_t pos;
+};
+
+template <typename T>
+__device__ __forceinline__ GradRow<T> grad_row_of(const HeadArgs& a, const GradRows& r, int64_t row) {
+  const int64_t token = div_small(row, r.heads), h = row - token * r.heads;
+  int64_t outer = 0, in = token;
+  if (a.inner < a.tokens) {
+    outer = div_small(token, a.inner);
+    in = token - outer * a.inner;
+  }
+  return {static_cast<const T*>(r.x) + outer * r.so + in * r.si + h * r.sh,
+          static_cast<const T*>(r.g) + outer * r.go + in * r.gi + h * r.gh, position_of(a, token)};
+}
+
+// A workgroup walks rows of one tensor; its lanes keep their unit, so the
+// weight's gradient gathers in registers, then over the workgroup's rows in LDS,
+// then over the workgroups in grad_weight_kernel: fixed orders throughout.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) heads_bwd_kernel(GradArgs ga) {
+  constexpr int VE = Vec16<T>::VE;
+  __shared__ float gather[kThreads * 2 * VE];
+  const HeadArgs& a = ga.h;
+  const bool second = (int)blockIdx.x >= ga.r[1].first_block;
+  const GradRows r = second ? ga.r[1] : ga.r[0];
+  const int lpr = 1 << a.lpr_log2, per = kThreads >> a.lpr_log2;
+  const int u = threadIdx.x & (lpr - 1), slot = threadIdx.x >> a.lpr_log2;
+  const Unit<VE> unit(u, a);
+  const T* w = static_cast<const T*>(r.w);
+  float w0[VE], w1[VE], d0[VE], d1[VE];
+  {
+    Vec16<T> v0, v1;
+    v0.u = v1.u = u32x4{0, 0, 0, 0};
+    if (unit.has0) v0 = load16(w + unit.off0);
+    if (unit.has1) v1 = load16(w + unit.off1);
+#pragma unroll
+    for (int e = 0; e < VE; ++e) {
+      w0[e] = to_f32(v0.e[e]);
+      w1[e] = to_f32(v1.e[e]);
+      d0[e] = d1[e] = 0.0f;
+    }
+  }
+  for (int64_t base = (int64_t)((int)blockIdx.x - r.first_block) * per; base < r.rows; base += (int64_t)r.blocks * per) {
+    const int64_t row = base + slot;
+    const bool live = row < r.rows;
+    const GradRow<T> o = grad_row_of<T>(a, r, min(row, r.rows - 1));
+    Vec16<T> x0, x1, g0, g1;
+    x0.u = x1.u = g0.u = g1.u = u32x4{0, 0, 0, 0};
+    if (live && unit.has0) {
+      x0 = load16(o.x + unit.off0);
+      g0 = load16(o.g + unit.off0);
+    }
+    if (live && unit.has1) {
+      x1 = load16(o.x + unit.off1);
+      g1 = load16(o.g + unit.off1);
+    }
+    float z0[VE], z1[VE];
+#pragma unroll
+    for (int e = 0; e < VE; ++e) {
+      z0[e] = to_f32(g0.e[e]);
+      z1[e] = to_f32(g1.e[e]);
+    }
+    if (unit.turned) {
+      float c[VE], s[VE];
+      load_angles<VE>(a, o.pos, u, c, s);
+      turn<VE>(z0, z1, c, s, a.interleaved);
+    }
+    float ss = 0.0f, gx = 0.0f;
+#pragma unroll
+    for (int e = 0; e < VE; ++e) {
+      const float a0 = to_f32(x0.e[e]), a1 = to_f32(x1.e[e]);
+      ss = fmaf(a0, a0, fmaf(a1, a1, ss));
+      gx = fmaf(z0[e] * w0[e], a0, fmaf(z1[e] * w1[e], a1, gx));
+    }
+    ss = lanes_sum(ss, a.lpr_log2);
+    gx = lanes_sum(gx, a.lpr_log2);
+    if (!live) continue;
+    const float inv = 1.0f / sqrtf(ss / (float)a.dim + a.eps);
+    const float back = inv * inv * (gx / (float)a.dim);
+    Vec16<T> y0, y1;
+#pragma unroll
+    for (int e = 0; e < VE; ++e) {
+      const float a0 = to_f32(x0.e[e]), a1 = to_f32(x1.e[e]);
+      y0.e[e] = from_f32<T>(inv * (z0[e] * w0[e] - a0 * back));
+      y1.e[e] = from_f32<T>(inv * (z1[e] * w1[e] - a1 * back));
+      d0[e] = fmaf(z0[e], a0 * inv, d0[e]);
+      d1[e] = fmaf(z1[e], a1 * inv, d1[e]);
+    }
+    T* y = static_cast<T*>(r.dx) + row * a.dim;
+    if (unit.has0) store16(y + unit.off0, y0);
+    if (unit.has1) store16(y + unit.off1, y1);
+  }
+  if (r.dw == nullptr) return;
+  // gather[element of the unit][thread]; then column by column over the row slots
+#pragma unroll
+  for (int e = 0; e < VE; ++e) {
+    gather[e * kThreads + threadIdx.x] = d0[e];
+    gather[(VE + e) * kThreads + threadIdx.x] = d1[e];
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < lpr * 2 * VE; i += kThreads) {
+    const int lane_u = i & (lpr - 1), e = i >> a.lpr_log2;
+    const Unit<VE> q(lane_u, a);
+    const int col = e < VE ? q.off0 + e : q.off1 + e - VE;
+    if (col >= a.dim) continue;
+    float sum = 0.0f;
+    for (int s = 0; s < per; ++s) sum += gather[e * kThreads + s * lpr + lane_u];
+    ga.part[(int64_t)blockIdx.x * a.dim + col] = sum;
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) heads_bwd_any_kernel(GradArgs ga) {
+  __shared__ float gather[4][kMaxHeadDim];
+  const HeadArgs& a = ga.h;
+  const bool second = (int)blockIdx.x >= ga.r[1].first_block;
+  const GradRows r = second ? ga.r[1] : ga.r[0];
+  const T* w = static_cast<const T*>(r.w);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  float* mine = gather[wave];
+  for (int d = lane; d < a.dim; d += 64) mine[d] = 0.0f;
+  __syncthreads();
+  for (int64_t row = (int64_t)((int)blockIdx.x - r.first_block) * 4 + wave; row < r.rows; row += (int64_t)r.blocks * 4) {
+    const GradRow<T> o = grad_row_of<T>(a, r, row);
+    // dz of pair i, or of the element rotary + (i - rotary / 2) past the pairs
+    auto pair = [&](int i, int& e0, int& e1, float& z0, float& z1) {
+      if (i < a.rotary / 2) {
+        pair_at(a, i, e0, e1);
+        float c, s;
+        angle_at(a, o.pos, i, c, s);
+        const float y0 = to_f32(o.g[e0]), y1 = to_f32(o.g[e1]);
+        z0 = y0 * c - y1 * s;
+        z1 = y1 * c + y0 * s;
+      } else {
+        e0 = a.rotary / 2 + i;
+        e1 = -1;
+        z0 = to_f32(o.g[e0]);
+        z1 = 0.0f;
+      }
+    };
+    const int n = a.dim - a.rotary / 2;
+    float ss = 0.0f, gx = 0.0f;
+    for (int i = lane; i < n; i += 64) {
+      int e0, e1;
+      float z0, z1;
+      pair(i, e0, e1, z0, z1);
+      const float x0 = to_f32(o.x[e0]), x1 = e1 >= 0 ? to_f32(o.x[e1]) : 0.0f, w1 = e1 >= 0 ? to_f32(w[e1]) : 0.0f;
+      ss = fmaf(x0, x0, fmaf(x1, x1, ss));
+      gx = fmaf(z0 * to_f32(w[e0]), x0, fmaf(z1 * w1, x1, gx));
+    }
+    ss = wave_sum(ss);
+    gx = wave_sum(gx);
+    const float inv = 1.0f / sqrtf(ss / (float)a.dim + a.eps);
+    const float back = inv * inv * (gx / (float)a.dim);
+    T* y = static_cast<T*>(r.dx) + row * a.dim;
+    for (int i = lane; i < n; i += 64) {
+      int e0, e1;
+      float z0, z1;
+      pair(i, e0, e1, z0, z1);
+      const float x0 = to_f32(o.x[e0]);
+      y[e0] = from_f32<T>(inv * (z0 * to_f32(w[e0]) - x0 * back));
+      mine[e0] = fmaf(z0, x0 * inv, mine[e0]);
+      if (e1 >= 0) {
+        const float x1 = to_f32(o.x[e1]);
+        y[e1] = from_f32<T>(inv * (z1 * to_f32(w[e1]) - x1 * back));
+        mine[e1] = fmaf(z1, x1 * inv, mine[e1]);
+      }
+    }
+  }
+  __syncthreads();
+  if (r.dw == nullptr) return;
+  for (int d = threadIdx.x; d < a.dim; d += kThreads)
+    ga.part[(int64_t)blockIdx.x * a.dim + d] = gather[0][d] + gather[1][d] + gather[2][d] + gather[3][d];
+}
+
+// The weights' gradients from the workgroups' parts: 32 columns a workgroup, 8
+// threads each.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) grad_weight_kernel(GradArgs ga) {
+  __shared__ float sums[8][32];
+  const int which = blockIdx.y;
+  const int first = which ? ga.r[1].first_block : ga.r[0].first_block, n = which ? ga.r[1].blocks : ga.r[0].blocks;
+  T* dw = static_cast<T*>(which ? ga.r[1].dw : ga.r[0].dw);
+  const int col = (int)blockIdx.x * 32 + (threadIdx.x & 31), group = threadIdx.x >> 5;
+  const int dim = ga.h.dim;
+  float sum = 0.0f;
+  if (dw != nullptr && col < dim) {
+    for (int i = group; i < n; i += 8) sum += ga.part[(int64_t)(first + i) * dim + col];
+  }
+  sums[group][threadIdx.x & 31] = sum;
+  __syncthreads();
+  if (group == 0 && dw != nullptr && col < dim) {
+    for (int i = 1; i < 8; ++i) sum += sums[i][threadIdx.x & 31];
+    dw[col] = from_f32<T>(sum);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+bool vec_ok(const void* p) { return p == nullptr || aligned16(p); }
+
+// Fewest lanes (a power of two) that hold a head in units; past 64 the head
+// takes the other kernels.
+int lanes_log2(int64_t dim, int64_t rotary, int ve) {
+  const int64_t units = rotary / (2 * ve) + (dim - rotary + 2 * ve - 1) / (2 * ve);
+  int l = 0;
+  while (((int64_t)1 << l) < units) ++l;
+  return l;
+}
+
+// Leading dimensions that fold into one: a token's place then needs no division.
+template <typename... Strides>
+void fold_tokens(int64_t& outer, int64_t& inner, Strides... so_si) {
+  const auto each = [&](auto fn) { (fn(*so_si.first, *so_si.second), ...); };
+  if (inner == 1) {
+    each([](int64_t& so, int64_t& si) { si = so; });
+    inner = outer;
+    outer = 1;
+  }
+  bool one = true;
+  each([&](int64_t& so, int64_t& si) { one = one && so == inner * si; });
+  if (one) {
+    inner *= outer;
+    outer = 1;
+  }
+}
+
+int check_heads(const char* name, int64_t dim, int64_t rotary, int64_t table_rows, const float* table, float eps, int dtype) {
+  if (ak_dtype_size(dtype) == 0) return ak_set_error(AK_ERR_UNSUPPORTED, "%s: unsupported dtype code %d", name, dtype);
+  if (dim < 1 || dim > kMaxHeadDim)
+    return ak_set_error(AK_ERR_UNSUPPORTED, "%s: head dim %lld is not 1 to %lld", name, (long long)dim, (long long)kMaxHeadDim);
+  if (rotary < 0 || rotary > dim || rotary % 2)
+    return ak_set_error(AK_ERR_INVALID_ARG, "%s: rotary %lld is not an even number up to dim", name, (long long)rotary);
+  if (rotary > 0 && (!table || table_rows < 1 || table_rows > INT64_MAX / 4 / rotary))
+    return ak_set_error(AK_ERR_INVALID_ARG, "%s: no table of angles", name);
+  if (!(eps >= 0.0f) || eps > 3.0e38f) return ak_set_error(AK_ERR_INVALID_ARG, "%s: eps must be finite and not negative", name);
+  return AK_OK;
+}
+
+template <typename T, bool NORM, bool APPEND>
+void launch_heads(HeadArgs& a, bool vec, hipStream_t s) {
+  constexpr int VE = Vec16<T>::VE;
+  a.lpr_log2 = lanes_log2(a.dim, a.rotary, VE);
+  for (const HeadRows& r : a.r) {
+    if (r.heads == 0) continue;
+    vec = vec && vec_ok(r.x) && vec_ok(r.y) && vec_ok(r.w) && r.so % VE == 0 && r.si % VE == 0 && r.sh % VE == 0 &&
+          r.yt % VE == 0 && r.ys % VE == 0 && r.yh % VE == 0;
+  }
+  vec = vec && a.dim % VE == 0 && a.rotary % (2 * VE) == 0 && vec_ok(a.table) && a.lpr_log2 <= 6;
+  const int64_t per = vec ? kThreads >> a.lpr_log2 : 4;
+  const dim3 grid(row_grid((a.total + per - 1) / per)), block(kThreads);
+  if (vec) heads_kernel<T, NORM, APPEND><<<grid, block, 0, s>>>(a);
+  else heads_any_kernel<T, NORM, APPEND><<<grid, block, 0, s>>>(a);
+}
+
+template <bool APPEND>
+void dispatch_heads(HeadArgs& a, bool norm, int dtype, hipStream_t s) {
+  auto go = [&](auto t) {
+    using T = decltype(t);
+    if (norm) launch_heads<T, true, APPEND>(a, true, s);
+    else launch_heads<T, false, APPEND>(a, true, s);
+  };
+  if (dtype == AK_DTYPE_F32) go(float());
+  else if (dtype == AK_DTYPE_F16) go(f16());
+  else go(bf16());
+}
+
+constexpr int64_t kGradBlocks = 1024;
+
+// Workgroups of the backward for queries and keys: by their heads, at least one
+// where there are any, at most one for each group of rows.
+void grad_blocks(int64_t tokens, int64_t q_heads, int64_t k_heads, int64_t* bq, int64_t* bk) {
+  const int64_t all = q_heads + k_heads;
+  auto share = [&](int64_t heads) {
+    if (heads == 0 || tokens == 0) return (int64_t)0;
+    const int64_t want = (int64_t)((double)kGradBlocks * (double)heads / (double)all + 0.5);
+    // (a workgroup of the vector form takes 4 rows at least)
+    const int64_t rows = tokens > (kGradBlocks * 4) / heads ? kGradBlocks * 4 : tokens * heads;
+    return std::max((int64_t)1, std::min(want, (rows + 3) / 4));
+  };
+  *bq = share(q_heads);
+  *bk = share(k_heads);
+}
+
+}  // namespace
+}  // namespace ak
+
+extern "C" int ak_qk_norm_rotary_fwd(const void* q, const void* k, const void* q_weight, const void* k_weight,
+                                     const float* table, const void* positions, void* q_out, void* k_out, int64_t outer,
+                                     int64_t inner, int64_t q_heads, int64_t k_heads, int64_t dim, int64_t rotary,
+                                     int64_t table_rows, int64_t n_positions, int64_t q_so, int64_t q_si, int64_t q_sh,
+                                     int64_t k_so, int64_t k_si, int64_t k_sh, float eps, int flags, int dtype, void* stream) {
+  const char* name = "ak_qk_norm_rotary_fwd";
+  int rc = ak::check_heads(name, dim, rotary, table_rows, table, eps, dtype);
+  if (rc) return rc;
+  const int esz = ak_dtype_size(dtype);
+  if (outer < 0 || inner < 0 || q_heads < 0 || k_heads < 0 || q_heads > INT32_MAX || k_heads > INT32_MAX ||
+      !ak::extent_ok(outer, q_so, inner, q_si, q_heads, q_sh, dim, esz) ||
+      !ak::extent_ok(outer, k_so, inner, k_si, k_heads, k_sh, dim, esz) ||
+      (__int128)outer * inner * (q_heads + k_heads) * dim > INT64_MAX / esz)
+    return ak_set_error(AK_ERR_INVALID_ARG, "%s: bad shape or strides", name);
+  const int64_t tokens = outer * inner;
+  if (tokens == 0 || q_heads + k_heads == 0) return AK_OK;
+  if (n_positions < 1) return ak_set_error(AK_ERR_INVALID_ARG, "%s: no positions", name);
+  if ((q_heads && (!q || !q_out)) || (k_heads && (!k || !k_out)) || (q_heads && k_heads && !q_weight != !k_weight))
+    return ak_set_error(AK_ERR_INVALID_ARG, "%s: null pointer", name);
+  ak::fold_tokens(outer, inner, std::make_pair(&q_so, &q_si), std::make_pair(&k_so, &k_si));
+  ak::HeadArgs a{};
+  a.r[0] = {q, q_out, q_weight, q_so, q_si, q_sh, q_heads * dim, 0, dim, q_heads};
+  a.r[1] = {k, k_out, k_weight, k_so, k_si, k_sh, k_heads * dim, 0, dim, k_heads};
+  a.table = table;
+  a.positions = positions;
+  a.tokens = tokens;
+  a.inner = inner;
+  a.n_positions = n_positions;
+  a.table_rows = table_rows;
+  a.all_heads = q_heads + k_heads;
+  a.total = tokens * a.all_heads;
+  a.dim = (int)dim;
+  a.rotary = (int)rotary;
+  a.interleaved = (flags & AK_ROTARY_INTERLEAVED) != 0;
+  a.inverse = (flags & AK_ROTARY_INVERSE) != 0;
+  a.pos64 = (flags & AK_POSITIONS_I64) != 0;
+  a.eps = eps;
+  ak::dispatch_heads<false>(a, (q_heads && q_weight) || (k_heads && k_weight), dtype, ak_stream(stream));
+  return ak_check_launch(name);
+}
+
+extern "C" size_t ak_qk_norm_rotary_bwd_workspace_bytes(int64_t tokens, int64_t q_heads, int64_t k_heads, int64_t dim) {
+  if (tokens <= 0 || q_heads < 0 || k_heads < 0 || dim <= 0) return 0;
+  int64_t bq, bk;
+  ak::grad_blocks(tokens, q_heads, k_heads, &bq, &bk);
+  return (size_t)(bq + bk) * (size_t)dim * sizeof(float);
+}
+
+extern "C" int ak_qk_norm_rotary_bwd(const void* q, const void* k, const void* q_weight, const void* k_weight,
+                                     const float* table, const void* positions, const void* grad_q_out,
+                                     const void* grad_k_out, void* grad_q, void* grad_k, void* grad_q_weight,
+                                     void* grad_k_weight, void* workspace, size_t workspace_bytes, int64_t outer,
+                                     int64_t inner, int64_t q_heads, int64_t k_heads, int64_t dim, int64_t rotary,
+                                     int64_t table_rows, int64_t n_positions, int64_t q_so, int64_t q_si, int64_t q_sh,
+                                     int64_t k_so, int64_t k_si, int64_t k_sh, int64_t gq_so, int64_t gq_si, int64_t gq_sh,
+                                     int64_t gk_so, int64_t gk_si, int64_t gk_sh, float eps, int flags, int dtype,
+                                     void* stream) {
+  const char* name = "ak_qk_norm_rotary_bwd";
+  int rc = ak::check_heads(name, dim, rotary, table_rows, table, eps, dtype);
+  if (rc) return rc;
+  const int esz = ak_dtype_size(dtype);
+  if (outer < 0 || inner < 0 || q_heads < 0 || k_heads < 0 || q_heads > INT32_MAX || k_heads > INT32_MAX ||
+      !ak::extent_ok(outer, q_so, inner, q_si, q_heads, q_sh, dim, esz) ||
+      !ak::extent_ok(outer, k_so, inner, k_si, k_heads, k_sh, dim, esz) ||
+      !ak::extent_ok(outer, gq_so, inner, gq_si, q_heads, gq_sh, dim, esz) ||
+      !ak::extent_ok(outer, gk_so, inner, gk_si, k_heads, gk_sh, dim, esz) ||
+      (__int128)outer * inner * (q_heads + k_heads) * dim > INT64_MAX / esz)
+    return ak_set_error(AK_ERR_INVALID_ARG, "%s: bad shape or strides", name);
+  const int64_t tokens = outer * inner;
+  if (tokens > 0 && n_positions < 1) return ak_set_error(AK_ERR_INVALID_ARG, "%s: no positions", name);
+  const bool some = tokens > 0;
+  if ((some && q_heads && (!q || !q_weight || !grad_q_out || !grad_q)) || (some && k_heads && (!k || !k_weight || !grad_k_out || !grad_k)))
+    return ak_set_error(AK_ERR_INVALID_ARG, "%s: null pointer", name);
+  const size_t need = ak_qk_norm_rotary_bwd_workspace_bytes(tokens, q_heads, k_heads, dim);
+  if (workspace_bytes < need || (need && (!workspace || !ak::aligned16(workspace))))
+    return ak_set_error(AK_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed (16-byte aligned)", name, workspace_bytes, need);
+  ak::fold_tokens(outer, inner, std::make_pair(&q_so, &q_si), std::make_pair(&k_so, &k_si),
+                  std::make_pair(&gq_so, &gq_si), std::make_pair(&gk_so, &gk_si));
+  ak::GradArgs g{};
+  int64_t bq, bk;
+  ak::grad_blocks(tokens, q_heads, k_heads, &bq, &bk);
+  g.r[0] = {q, grad_q_out, q_weight, grad_q, grad_q_weight, q_so, q_si, q_sh, gq_so, gq_si, gq_sh, q_heads,
+            tokens * q_heads, 0, (int)bq};
+  g.r[1] = {k, grad_k_out, k_weight, grad_k, grad_k_weight, k_so, k_si, k_sh, gk_so, gk_si, gk_sh, k_heads,
+            tokens * k_heads, (int)bq, (int)bk};
+  g.part = static_cast<float*>(workspace);
+  ak::HeadArgs& a = g.h;
+  a.table = table;
+  a.positions = positions;
+  a.tokens = tokens;
+  a.inner = inner;
+  a.n_positions = n_positions;
+  a.table_rows = table_rows;
+  a.dim = (int)dim;
+  a.rotary = (int)rotary;
+  a.interleaved = (flags & AK_ROTARY_INTERLEAVED) != 0;
+  a.inverse = 1;
+  a.pos64 = (flags & AK_POSITIONS_I64) != 0;
+  a.eps = eps;
+  hipStream_t s = ak_stream(stream);
+  auto go = [&](auto t) {
+    using T = decltype(t);
+    constexpr int VE = ak::Vec16<T>::VE;
+    a.lpr_log2 = ak::lanes_log2(dim, rotary, VE);
+    bool vec = dim % VE == 0 && rotary % (2 * VE) == 0 && ak::vec_ok(table) && a.lpr_log2 <= 6;
+    for (const ak::GradRows& r : g.r) {
+      if (r.heads == 0) continue;
+      for (const void* p : {r.x, r.g, r.w, (const void*)r.dx}) vec = vec && ak::vec_ok(p);
+      for (int64_t st : {r.so, r.si, r.sh, r.go, r.gi, r.gh}) vec = vec && st % VE == 0;
+    }
+    if (bq + bk > 0) {
+      if (vec) ak::heads_bwd_kernel<T><<<dim3((unsigned)(bq + bk)), dim3(ak::kThreads), 0, s>>>(g);
+      else ak::heads_bwd_any_kernel<T><<<dim3((unsigned)(bq + bk)), dim3(ak::kThreads), 0, s>>>(g);
+    }
+    if (grad_q_weight || grad_k_weight)
+      ak::grad_weight_kernel<T><<<dim3((unsigned)((dim + 31) / 32), 2), dim3(ak::kThreads), 0, s>>>(g);
+  };
+  if (dtype == AK_DTYPE_F32) go(float());
+  else if (dtype == AK_DTYPE_F16) go(ak::f16());
+  else go(ak::bf16());
+  return ak_check_launch(name);
+}
+
+extern "C" int ak_paged_append(const void* q, const void* k, const void* v, const void* q_weight, const void* k_weight,
+                               const float* table, void* q_out, void* k_cache, void* v_cache, const int32_t* page_table,
+                               const int32_t* lengths, const int32_t* starts, int64_t tokens, int64_t batch, int64_t q_heads,
+                               int64_t kv_heads, int64_t dim, int64_t rotary, int64_t table_rows, int64_t n_pages,
+                               int64_t page_size, int64_t max_pages, int64_t ld_pages, int64_t q_st, int64_t q_sh,
+                               int64_t k_st, int64_t k_sh, int64_t v_st, int64_t v_sh, int64_t qo_st, int64_t qo_sh,
+                               int64_t kc_sp, int64_t kc_ss, int64_t kc_sh, int64_t vc_sp, int64_t vc_ss, int64_t vc_sh,
+                               float eps, int flags, int dtype, void* stream) {
+  const char* name = "ak_paged_append";
+  int rc = ak::check_heads(name, dim, rotary, table_rows, table, eps, dtype);
+  if (rc) return rc;
+  const int esz = ak_dtype_size(dtype);
+  rc = ak::check_paged(name, tokens, batch, n_pages, page_size, max_pages, ld_pages, starts, lengths, page_table);
+  if (rc) return rc;
+  if (q_heads < 0 || kv_heads < 1 || q_heads > INT32_MAX / 4 || kv_heads > INT32_MAX / 4 ||
+      !ak::extent_ok(1, 0, tokens, q_st, q_heads, q_sh, dim, esz) || !ak::extent_ok(1, 0, tokens, qo_st, q_heads, qo_sh, dim, esz) ||
+      !ak::extent_ok(1, 0, tokens, k_st, kv_heads, k_sh, dim, esz) || !ak::extent_ok(1, 0, tokens, v_st, kv_heads, v_sh, dim, esz) ||
+      !ak::extent_ok(n_pages, kc_sp, page_size, kc_ss, kv_heads, kc_sh, dim, esz) ||
+      !ak::extent_ok(n_pages, vc_sp, page_size, vc_ss, kv_heads, vc_sh, dim, esz) ||
+      (__int128)tokens * (q_heads + 2 * kv_heads) > INT64_MAX / 4096)
+    return ak_set_error(AK_ERR_INVALID_ARG, "%s: bad shape or strides", name);
+  if (tokens == 0) return AK_OK;
+  if ((q_heads && (!q || !q_out)) || !k || !v || (n_pages && (!k_cache || !v_cache)))
+    return ak_set_error(AK_ERR_INVALID_ARG, "%s: null pointer", name);
+  ak::HeadArgs a{};
+  a.r[0] = {q, q_out, q_weight, 0, q_st, q_sh, qo_st, 0, qo_sh, q_heads};
+  a.r[1] = {k, k_cache, k_weight, 0, k_st, k_sh, kc_sp, kc_ss, kc_sh, kv_heads};
+  a.r[2] = {v, v_cache, nullptr, 0, v_st, v_sh, vc_sp, vc_ss, vc_sh, kv_heads};
+  a.table = table;
+  a.tokens = a.inner = a.n_positions = tokens;
+  a.table_rows = table_rows;
+  a.all_heads = q_heads + 2 * kv_heads;
+  a.total = tokens * a.all_heads;
+  a.dim = (int)dim;
+  a.rotary = (int)rotary;
+  a.interleaved = (flags & AK_ROTARY_INTERLEAVED) != 0;
+  a.zero_tail = (flags & AK_ZERO_OTHER_ROWS) != 0;
+  a.eps = eps;
+  a.seq = {starts, lengths, batch, tokens, starts ? 0 : tokens / batch};
+  a.pages = page_table;
+  a.n_pages = n_pages;
+  a.page_size = page_size;
+  a.max_pages = max_pages;
+  a.ld_pages = ld_pages;
+  ak::dispatch_heads<true>(a, (q_heads && q_weight) || k_weight, dtype, ak_stream(stream));
+  return ak_check_launch(name);
+}

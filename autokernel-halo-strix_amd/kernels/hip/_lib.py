@@ -76,6 +76,12 @@ _SIGNATURES = {
                                                                              _c_void_p],
     "ak_topk_distill_bwd": [_c_void_p] * 5 + [_i64, _c_void_p, _c_void_p] + [_i64] * 7
     + [_f32, _f32, _i64, _int, _int, _c_void_p],
+    "ak_qk_norm_rotary_fwd": [_c_void_p] * 8 + [_i64] * 14 + [_f32, _int, _int, _c_void_p],
+    "ak_qk_norm_rotary_bwd_workspace_bytes": [_i64] * 4,
+    "ak_qk_norm_rotary_bwd": [_c_void_p] * 13 + [ctypes.c_size_t] + [_i64] * 20 + [_f32, _int, _int, _c_void_p],
+    "ak_paged_append": [_c_void_p] * 12 + [_i64] * 25 + [_f32, _int, _int, _c_void_p],
+    "ak_paged_attention_workspace_bytes": [_i64] * 7 + [_int],
+    "ak_paged_attention": [_c_void_p] * 8 + [ctypes.c_size_t] + [_i64] * 20 + [_f32, _f32, _i64, _int, _int, _c_void_p],
     "ak_lmhead_ce_workspace_bytes": [_i64, _i64],
     "ak_lmhead_ce_fwd": [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
                          _c_void_p, ctypes.c_size_t, _i64, _i64, _i64, _i64, _i64, _i64, _f32, _f32,
@@ -108,6 +114,8 @@ _RESTYPES = {
     "ak_target_arch": ctypes.c_char_p,
     "ak_token_logprobs_workspace_bytes": ctypes.c_size_t,
     "ak_topk_distill_workspace_bytes": ctypes.c_size_t,
+    "ak_qk_norm_rotary_bwd_workspace_bytes": ctypes.c_size_t,
+    "ak_paged_attention_workspace_bytes": ctypes.c_size_t,
     "ak_lmhead_ce_workspace_bytes": ctypes.c_size_t,
     "ak_lmhead_logprobs_workspace_bytes": ctypes.c_size_t,
     "ak_lmhead_grad_workspace_bytes": ctypes.c_size_t,
@@ -878,3 +886,106 @@ def diag_scan_bwd(dA, dBx, C, D, x, grad_y, grad_dA, grad_dBx, grad_C, grad_D, g
                                   _ptr(grad_x), _ptr(ws), ws.numel(), batch, seqlen, d_inner,
                                   _stream(dA))
     _check(rc, "ak_diag_scan_bwd")
+
+
+# ---------------------------------------------------------------------------
+# Attention heads: rotary positions, head norms, the paged cache
+# ---------------------------------------------------------------------------
+
+ROTARY_INTERLEAVED, ROTARY_INVERSE, POSITIONS_I64, ZERO_OTHER_ROWS = 1, 2, 4, 8
+
+
+def _head_flags(positions, interleaved: bool, inverse: bool = False, zero: bool = False) -> int:
+    wide = positions is not None and positions.dtype == torch.int64
+    return interleaved * ROTARY_INTERLEAVED | inverse * ROTARY_INVERSE | wide * POSITIONS_I64 | zero * ZERO_OTHER_ROWS
+
+
+def _angles(table: Optional[torch.Tensor]) -> tuple:
+    """``(rotary, rows)`` of a table of angles."""
+    return (0, 0) if table is None else (table.shape[1], table.shape[0])
+
+
+def qk_norm_rotary(q, k, q_weight, k_weight, table, positions, n_positions: int, q_out: torch.Tensor,
+                   k_out: Optional[torch.Tensor], eps: float, interleaved: bool, inverse: bool) -> None:
+    """Norm and rotation of heads (``_heads.Heads``; k may be None) into contiguous outputs."""
+    kt = None if k is None else k.t
+    require_device(q.t, kt, q_weight, k_weight, table, positions, q_out, k_out)
+    rotary, rows = _angles(table)
+    with _on_device(q.t):
+        rc = load().ak_qk_norm_rotary_fwd(
+            _ptr(q.t), _ptr(kt), _ptr(q_weight), _ptr(k_weight), _ptr(table), _ptr(positions), _ptr(q_out), _ptr(k_out),
+            q.outer, q.inner, q.heads, k.heads if k else 0, q.dim, rotary, rows, n_positions, *q.strides,
+            *(k.strides if k else (0, 0, 0)), float(eps), _head_flags(positions, interleaved, inverse),
+            dtype_code(q.t.dtype), _stream(q.t))
+    _check(rc, "ak_qk_norm_rotary_fwd")
+
+
+def qk_norm_rotary_bwd_workspace_bytes(tokens: int, q_heads: int, k_heads: int, dim: int) -> int:
+    return int(load().ak_qk_norm_rotary_bwd_workspace_bytes(tokens, q_heads, k_heads, dim))
+
+
+def qk_norm_rotary_bwd(q, k, q_weight, k_weight, table, positions, n_positions: int, g_q, g_k, dq: torch.Tensor,
+                       dk: Optional[torch.Tensor], dq_weight: Optional[torch.Tensor], dk_weight: Optional[torch.Tensor],
+                       workspace: torch.Tensor, eps: float, interleaved: bool) -> None:
+    kt, gkt = (None, None) if k is None else (k.t, g_k.t)
+    require_device(q.t, kt, q_weight, k_weight, table, positions, g_q.t, gkt, dq, dk, dq_weight, dk_weight, workspace)
+    rotary, rows = _angles(table)
+    none = (0, 0, 0)
+    with _on_device(q.t):
+        rc = load().ak_qk_norm_rotary_bwd(
+            _ptr(q.t), _ptr(kt), _ptr(q_weight), _ptr(k_weight), _ptr(table), _ptr(positions), _ptr(g_q.t), _ptr(gkt),
+            _ptr(dq), _ptr(dk), _ptr(dq_weight), _ptr(dk_weight), _ptr(workspace), workspace.numel(), q.outer, q.inner,
+            q.heads, k.heads if k else 0, q.dim, rotary, rows, n_positions, *q.strides, *(k.strides if k else none),
+            *g_q.strides, *(g_k.strides if k else none), float(eps), _head_flags(positions, interleaved),
+            dtype_code(q.t.dtype), _stream(q.t))
+    _check(rc, "ak_qk_norm_rotary_bwd")
+
+
+def _page_args(batch, cache: torch.Tensor) -> tuple:
+    """``(n_pages, page_size, max_pages, ld_pages)``."""
+    pages = batch.pages
+    ld = pages.stride(0) if pages.shape[0] > 1 else pages.shape[1]
+    return cache.shape[0], cache.shape[1], pages.shape[1], ld
+
+
+def paged_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, q_weight: Optional[torch.Tensor],
+                 k_weight: Optional[torch.Tensor], table: Optional[torch.Tensor], q_out: Optional[torch.Tensor],
+                 k_cache: torch.Tensor, v_cache: torch.Tensor, batch, eps: float, interleaved: bool, zero: bool) -> None:
+    """``batch``: a ``_heads.Batch``."""
+    require_device(q, k, v, q_weight, k_weight, table, q_out, k_cache, v_cache, *batch)
+    rotary, rows = _angles(table)
+    tokens, heads, dim = k.shape
+    with _on_device(k):
+        rc = load().ak_paged_append(
+            _ptr(q), _ptr(k), _ptr(v), _ptr(q_weight), _ptr(k_weight), _ptr(table), _ptr(q_out), _ptr(k_cache),
+            _ptr(v_cache), _ptr(batch.pages), _ptr(batch.lengths), _ptr(batch.starts), tokens, batch.lengths.shape[0],
+            0 if q is None else q.shape[1], heads, dim, rotary, rows, *_page_args(batch, k_cache),
+            *((0, 0) if q is None else q.stride()[:2]), *k.stride()[:2], *v.stride()[:2],
+            *((0, 0) if q is None else q_out.stride()[:2]), *k_cache.stride()[:3], *v_cache.stride()[:3], float(eps),
+            _head_flags(None, interleaved, zero=zero), dtype_code(k.dtype), _stream(k))
+    _check(rc, "ak_paged_append")
+
+
+def paged_attention_workspace_bytes(tokens: int, batch: int, q_heads: int, kv_heads: int, dim: int, max_keys: int,
+                                    max_chunk: int, dtype: torch.dtype) -> int:
+    return int(load().ak_paged_attention_workspace_bytes(tokens, batch, q_heads, kv_heads, dim, max_keys, max_chunk,
+                                                         dtype_code(dtype)))
+
+
+def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, batch, out: torch.Tensor,
+                    max_chunk: int, scale: float, softcap: float, window: int, zero: bool) -> None:
+    """``batch``: a ``_heads.Batch``."""
+    require_device(q, k_cache, v_cache, out, *batch)
+    tokens, heads, dim = q.shape
+    n = batch.lengths.shape[0]
+    page_args = _page_args(batch, k_cache)
+    size = paged_attention_workspace_bytes(tokens, n, heads, k_cache.shape[2], dim, page_args[1] * page_args[2], max_chunk,
+                                           q.dtype)
+    ws = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
+    with _on_device(q):
+        rc = load().ak_paged_attention(
+            _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(batch.pages), _ptr(batch.lengths), _ptr(batch.starts), _ptr(out),
+            _ptr(ws), size, tokens, n, heads, k_cache.shape[2], dim, *page_args, max_chunk, *q.stride()[:2],
+            *out.stride()[:2], *k_cache.stride()[:3], *v_cache.stride()[:3], float(scale), float(softcap), window,
+            _head_flags(None, False, zero=zero), dtype_code(q.dtype), _stream(q))
+    _check(rc, "ak_paged_attention")

@@ -43,6 +43,12 @@ extern "C" {
 /* ak_selective_scan_bwd_workspace_bytes only: the size for a complex A */
 #define AK_SCAN_A_COMPLEX 4
 
+/* ak_qk_norm_rotary_*, ak_paged_*: flags */
+#define AK_ROTARY_INTERLEAVED 1
+#define AK_ROTARY_INVERSE 2
+#define AK_POSITIONS_I64 4
+#define AK_ZERO_OTHER_ROWS 8
+
 #define AK_OK 0
 #define AK_ERR_INVALID_ARG (-1)
 #define AK_ERR_UNSUPPORTED (-2)
@@ -650,6 +656,88 @@ int ak_diag_scan_bwd(const float* dA, const float* dBx, const float* C, const fl
                      float* grad_dA, float* grad_dBx, float* grad_C, float* grad_D,
                      float* grad_x, void* workspace, size_t workspace_bytes,
                      int64_t batch, int64_t seqlen, int64_t d_inner, void* stream);
+
+/*
+ * Rotary positions and head norms of queries [outer, inner, q_heads, dim] and
+ * keys (element strides so, si, sh; the last dimension dense). Per token and head,
+ * in fp32 with one rounding:
+ *   n = x / sqrt(mean(x^2) + eps) * weight        (x itself where the weights are NULL)
+ *   the pairs of n's first `rotary` elements, (i, i + rotary / 2) or with
+ *   AK_ROTARY_INTERLEAVED (2 i, 2 i + 1), turned by the token's angles:
+ *   (n0 cos - n1 sin, n1 cos + n0 sin); AK_ROTARY_INVERSE turns them back.
+ * table [table_rows, rotary] holds a position's cosines, then its sines. Token t
+ * (of outer * inner) has position positions[t % n_positions] (int32, or int64 with
+ * AK_POSITIONS_I64; NULL: t % n_positions itself); outside the table its turned
+ * elements are NaN. Outputs are dense [outer, inner, heads, dim]. rotary 0 (table
+ * NULL) only norms. dim is at most 2048. No counterpart among the reference's kernels
+ * that this library covers.
+ */
+int ak_qk_norm_rotary_fwd(const void* q, const void* k, const void* q_weight, const void* k_weight,
+                          const float* table, const void* positions, void* q_out, void* k_out,
+                          int64_t outer, int64_t inner, int64_t q_heads, int64_t k_heads, int64_t dim,
+                          int64_t rotary, int64_t table_rows, int64_t n_positions,
+                          int64_t q_so, int64_t q_si, int64_t q_sh, int64_t k_so, int64_t k_si,
+                          int64_t k_sh, float eps, int flags, int dtype, void* stream);
+
+/*
+ * Backward of ak_qk_norm_rotary_fwd with weights (without them it is the forward
+ * of the gradients with AK_ROTARY_INVERSE). grad_q and grad_k are dense; the
+ * weights' gradients [dim], of the element type, are summed in fp32 in a fixed
+ * order (NULL: not wanted).
+ */
+size_t ak_qk_norm_rotary_bwd_workspace_bytes(int64_t tokens, int64_t q_heads, int64_t k_heads, int64_t dim);
+int ak_qk_norm_rotary_bwd(const void* q, const void* k, const void* q_weight, const void* k_weight,
+                          const float* table, const void* positions, const void* grad_q_out,
+                          const void* grad_k_out, void* grad_q, void* grad_k, void* grad_q_weight,
+                          void* grad_k_weight, void* workspace, size_t workspace_bytes,
+                          int64_t outer, int64_t inner, int64_t q_heads, int64_t k_heads, int64_t dim,
+                          int64_t rotary, int64_t table_rows, int64_t n_positions,
+                          int64_t q_so, int64_t q_si, int64_t q_sh, int64_t k_so, int64_t k_si, int64_t k_sh,
+                          int64_t gq_so, int64_t gq_si, int64_t gq_sh, int64_t gk_so, int64_t gk_si,
+                          int64_t gk_sh, float eps, int flags, int dtype, void* stream);
+
+/*
+ * New keys and values [tokens, kv_heads, dim] into a paged cache. Sequence b's new
+ * tokens are rows [starts[b], starts[b + 1]) (starts NULL: tokens / batch each) and
+ * the last of its lengths[b] positions; position p lives in slot p % page_size of
+ * page page_table[b][p / page_size]. Keys (and queries, which go to q_out; q_heads 0
+ * without) are normed and turned as in ak_qk_norm_rotary_fwd at their positions.
+ * Nothing is written for a token of no sequence, at a negative position, past the
+ * table's max_pages or on a page outside [0, n_pages); its q_out row stays as it is,
+ * or is zeroed with AK_ZERO_OTHER_ROWS, where the token has no sequence. Two new
+ * tokens must not share a slot. No counterpart in the reference.
+ */
+int ak_paged_append(const void* q, const void* k, const void* v, const void* q_weight, const void* k_weight,
+                    const float* table, void* q_out, void* k_cache, void* v_cache, const int32_t* page_table,
+                    const int32_t* lengths, const int32_t* starts, int64_t tokens, int64_t batch,
+                    int64_t q_heads, int64_t kv_heads, int64_t dim, int64_t rotary, int64_t table_rows,
+                    int64_t n_pages, int64_t page_size, int64_t max_pages, int64_t ld_pages,
+                    int64_t q_st, int64_t q_sh, int64_t k_st, int64_t k_sh, int64_t v_st, int64_t v_sh,
+                    int64_t qo_st, int64_t qo_sh, int64_t kc_sp, int64_t kc_ss, int64_t kc_sh,
+                    int64_t vc_sp, int64_t vc_ss, int64_t vc_sh, float eps, int flags, int dtype, void* stream);
+
+/*
+ * Attention of the new tokens q [tokens, q_heads, dim] (sequences as in
+ * ak_paged_append, whose cache holds the tokens' own keys and values too) over
+ * their sequences' cached keys. The token at position p sees the keys j <= p below
+ * lengths[b], with window > 0 those above p - window, on pages inside [0, n_pages):
+ *   s_j = scale q . k_j  (softcap > 0: softcap tanh(s_j / softcap)),
+ *   out = sum_j softmax(s)_j v_j
+ * in fp32 (fp16 / bf16: the probabilities are rounded once, for the matrix cores). A
+ * token that sees no key, or only scores of -inf, gives 0. Query head h reads key
+ * head h * kv_heads / q_heads. max_chunk: the most new tokens of a sequence, as far as
+ * the caller knows (it chooses the kernel; results hold for any). out rows of no
+ * sequence: as in ak_paged_append. dim is at most 1024. No counterpart in the reference.
+ */
+size_t ak_paged_attention_workspace_bytes(int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads,
+                                          int64_t dim, int64_t max_keys, int64_t max_chunk, int dtype);
+int ak_paged_attention(const void* q, const void* k_cache, const void* v_cache, const int32_t* page_table,
+                       const int32_t* lengths, const int32_t* starts, void* out, void* workspace,
+                       size_t workspace_bytes, int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads,
+                       int64_t dim, int64_t n_pages, int64_t page_size, int64_t max_pages, int64_t ld_pages,
+                       int64_t max_chunk, int64_t q_st, int64_t q_sh, int64_t o_st, int64_t o_sh,
+                       int64_t kc_sp, int64_t kc_ss, int64_t kc_sh, int64_t vc_sp, int64_t vc_ss, int64_t vc_sh,
+                       float scale, float softcap, int64_t window, int flags, int dtype, void* stream);
 
 #ifdef __cplusplus
 }
