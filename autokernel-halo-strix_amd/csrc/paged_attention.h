@@ -1,0 +1,59 @@
+// Shared pieces of the kernels of attention over a paged cache.
+#pragma once
+
+#include "heads.h"
+
+namespace ak {
+
+constexpr int64_t kMaxAttendDim = 1024;
+constexpr float kNegInf = -__builtin_inff();
+
+struct AttendArgs {
+  const void *q, *k, *v;
+  void* out;
+  float* part;
+  Sequences seq;
+  const int32_t* pages;
+  int64_t n_pages, page_size, max_pages, ld_pages;
+  int64_t q_st, q_sh, o_st, o_sh;
+  int64_t kp, ks, kh, vp, vs, vh;  // cache strides: page, slot, head
+  int64_t window;                  // 0: none
+  int q_heads, kv_heads, dim, zero_other;
+  int splits;
+  float scale, softcap;
+};
+
+// The keys that a token at `pos` of a sequence may see: [lo, hi).
+__device__ __forceinline__ void keys_of(const AttendArgs& a, int64_t length, int64_t pos, int64_t& lo, int64_t& hi) {
+  hi = min(pos + 1, min(length, a.max_pages * a.page_size));
+  lo = a.window > 0 ? max(pos - a.window + 1, (int64_t)0) : 0;
+  if (hi < lo) hi = lo;
+}
+
+// The page of key j of sequence b, or -1 where there is none.
+__device__ __forceinline__ int64_t page_of(const AttendArgs& a, int64_t b, int64_t j, int64_t& slot) {
+  const int64_t i = (uint32_t)j / (uint32_t)a.page_size;
+  slot = j - i * a.page_size;
+  const int64_t page = a.pages[b * a.ld_pages + i];
+  return page >= 0 && page < a.n_pages ? page : -1;
+}
+
+__device__ __forceinline__ float score_of(const AttendArgs& a, float dot) {
+  const float s = dot * a.scale;
+  return a.softcap > 0.0f ? a.softcap * tanh_f32(s / a.softcap) : s;
+}
+
+// exp(s - m); beside a maximum of -inf (nothing seen yet, or NaN alone, which the
+// maximum passes over) 0 or that NaN.
+__device__ __forceinline__ float weight_of(float s, float m) {
+  return m == kNegInf ? (s == s ? 0.0f : s) : fast_exp(s - m);
+}
+
+// The kernels on the matrix cores (paged_attention_tiles.hip): fp16 / bf16 of head
+// dims up to 256 in whole 16-byte vectors, fp32 the same.
+bool attend_tiles_take(const AttendArgs& a, int dtype);
+size_t attend_tiles_workspace_bytes(int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t dim,
+                                    int64_t max_keys, int64_t max_chunk, int dtype);
+void attend_tiles(const AttendArgs& a, int64_t max_chunk, int dtype, void* workspace, hipStream_t s);
+
+}  // namespace ak

@@ -10,54 +10,10 @@
 // scores of -inf, is 0.
 #include <algorithm>
 
-#include "heads.h"
+#include "paged_attention.h"
 
 namespace ak {
 namespace {
-
-constexpr int64_t kMaxAttendDim = 1024;
-constexpr float kNegInf = -__builtin_inff();
-
-struct AttendArgs {
-  const void *q, *k, *v;
-  void* out;
-  float* part;
-  Sequences seq;
-  const int32_t* pages;
-  int64_t n_pages, page_size, max_pages, ld_pages;
-  int64_t q_st, q_sh, o_st, o_sh;
-  int64_t kp, ks, kh, vp, vs, vh;  // cache strides: page, slot, head
-  int64_t window;                  // 0: none
-  int q_heads, kv_heads, dim, zero_other;
-  int splits;
-  float scale, softcap;
-};
-
-// The keys that a token at `pos` of a sequence may see: [lo, hi).
-__device__ __forceinline__ void keys_of(const AttendArgs& a, int64_t length, int64_t pos, int64_t& lo, int64_t& hi) {
-  hi = min(pos + 1, min(length, a.max_pages * a.page_size));
-  lo = a.window > 0 ? max(pos - a.window + 1, (int64_t)0) : 0;
-  if (hi < lo) hi = lo;
-}
-
-// The page of key j of sequence b, or -1 where there is none.
-__device__ __forceinline__ int64_t page_of(const AttendArgs& a, int64_t b, int64_t j, int64_t& slot) {
-  const int64_t i = (uint32_t)j / (uint32_t)a.page_size;
-  slot = j - i * a.page_size;
-  const int64_t page = a.pages[b * a.ld_pages + i];
-  return page >= 0 && page < a.n_pages ? page : -1;
-}
-
-__device__ __forceinline__ float score_of(const AttendArgs& a, float dot) {
-  const float s = dot * a.scale;
-  return a.softcap > 0.0f ? a.softcap * tanh_f32(s / a.softcap) : s;
-}
-
-// exp(s - m); beside a maximum of -inf (nothing seen yet, or NaN alone, which the
-// maximum passes over) 0 or that NaN.
-__device__ __forceinline__ float weight_of(float s, float m) {
-  return m == kNegInf ? (s == s ? 0.0f : s) : fast_exp(s - m);
-}
 
 // Any type, head dim and alignment: a workgroup for a row (token and query head)
 // and a cut of its keys. A wave takes 64 keys at a time: a lane each for the
@@ -200,10 +156,14 @@ int any_splits(int64_t rows, int64_t max_keys) {
 
 extern "C" size_t ak_paged_attention_workspace_bytes(int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads,
                                                      int64_t dim, int64_t max_keys, int64_t max_chunk, int dtype) {
-  if (tokens <= 0 || batch <= 0 || q_heads <= 0 || kv_heads <= 0 || dim <= 0) return 0;
+  if (tokens <= 0 || batch <= 0 || q_heads <= 0 || kv_heads <= 0 || dim <= 0 || max_keys < 0) return 0;
+  max_chunk = std::max(max_chunk, (int64_t)1);
+  // of the kernel that the call takes: by its pointers' alignment it may be either
   const int64_t rows = tokens * q_heads;
   const int splits = ak::any_splits(rows, max_keys);
-  return splits > 1 ? (size_t)(rows * splits * (dim + 2)) * sizeof(float) : 0;
+  const size_t any = splits > 1 ? (size_t)(rows * splits * (dim + 2)) * sizeof(float) : 0;
+  if (q_heads % kv_heads || dim > 256 || ak_dtype_size(dtype) == 0 || dim % (16 / ak_dtype_size(dtype))) return any;
+  return std::max(any, ak::attend_tiles_workspace_bytes(tokens, batch, q_heads, kv_heads, dim, max_keys, max_chunk, dtype));
 }
 
 extern "C" int ak_paged_attention(const void* q, const void* k_cache, const void* v_cache, const int32_t* page_table,
@@ -231,7 +191,7 @@ extern "C" int ak_paged_attention(const void* q, const void* k_cache, const void
   if (tokens == 0) return AK_OK;
   if (!q || !out || (n_pages && (!k_cache || !v_cache))) return ak_set_error(AK_ERR_INVALID_ARG, "%s: null pointer", name);
   const int64_t max_keys = max_pages * page_size;
-  const size_t need = ak_paged_attention_workspace_bytes(tokens, batch, q_heads, kv_heads, dim, max_keys, max_chunk, dtype);
+  const size_t need = ak_paged_attention_workspace_bytes(tokens, batch, q_heads, kv_heads, dim, max_keys, std::max(max_chunk, (int64_t)1), dtype);
   if (workspace_bytes < need || (need && (!workspace || !ak::aligned16(workspace))))
     return ak_set_error(AK_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed (16-byte aligned)", name, workspace_bytes, need);
   ak::AttendArgs a{};
@@ -256,6 +216,10 @@ extern "C" int ak_paged_attention(const void* q, const void* k_cache, const void
   a.scale = scale;
   a.softcap = softcap;
   hipStream_t s = ak_stream(stream);
+  if (batch > 0 && ak::attend_tiles_take(a, dtype)) {
+    ak::attend_tiles(a, std::max(max_chunk, (int64_t)1), dtype, workspace, s);
+    return ak_check_launch(name);
+  }
   const int64_t rows = tokens * q_heads;
   a.splits = batch > 0 ? ak::any_splits(rows, max_keys) : 1;
   auto go = [&](auto t) {
