@@ -515,25 +515,30 @@ __global__ void __launch_bounds__(kThreads) heads_bwd_any_kernel(GradArgs ga) {
     ga.part[(int64_t)blockIdx.x * a.dim + d] = gather[0][d] + gather[1][d] + gather[2][d] + gather[3][d];
 }
 
-// The weights' gradients from the workgroups' parts: 32 columns a workgroup, 8
+// The weights' gradients from the workgroups' parts: 16 columns a workgroup, 64
 // threads each.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) grad_weight_kernel(GradArgs ga) {
-  __shared__ float sums[8][32];
+__global__ void __launch_bounds__(1024) grad_weight_kernel(GradArgs ga) {
+  __shared__ float sums[64][17];
   const int which = blockIdx.y;
   const int first = which ? ga.r[1].first_block : ga.r[0].first_block, n = which ? ga.r[1].blocks : ga.r[0].blocks;
   T* dw = static_cast<T*>(which ? ga.r[1].dw : ga.r[0].dw);
-  const int col = (int)blockIdx.x * 32 + (threadIdx.x & 31), group = threadIdx.x >> 5;
+  if (dw == nullptr) return;
+  const int c = threadIdx.x & 15, col = (int)blockIdx.x * 16 + c, group = threadIdx.x >> 4;
   const int dim = ga.h.dim;
   float sum = 0.0f;
-  if (dw != nullptr && col < dim) {
-    for (int i = group; i < n; i += 8) sum += ga.part[(int64_t)(first + i) * dim + col];
+  if (col < dim) {
+#pragma unroll 4
+    for (int i = group; i < n; i += 64) sum += ga.part[(int64_t)(first + i) * dim + col];
   }
-  sums[group][threadIdx.x & 31] = sum;
+  sums[group][c] = sum;
   __syncthreads();
-  if (group == 0 && dw != nullptr && col < dim) {
-    for (int i = 1; i < 8; ++i) sum += sums[i][threadIdx.x & 31];
-    dw[col] = from_f32<T>(sum);
+  if (threadIdx.x < 256) {  // four groups each, then the 16 sums of a column, which a wave holds
+    sum = 0.0f;
+    for (int i = 0; i < 4; ++i) sum += sums[4 * (threadIdx.x & 15) + i][threadIdx.x >> 4];
+    sum = row16_sum(sum);
+    const int out = (int)blockIdx.x * 16 + (threadIdx.x >> 4);
+    if ((threadIdx.x & 15) == 0 && out < dim) dw[out] = from_f32<T>(sum);
   }
 }
 
@@ -743,7 +748,7 @@ extern "C" int ak_qk_norm_rotary_bwd(const void* q, const void* k, const void* q
       else ak::heads_bwd_any_kernel<T><<<dim3((unsigned)(bq + bk)), dim3(ak::kThreads), 0, s>>>(g);
     }
     if (grad_q_weight || grad_k_weight)
-      ak::grad_weight_kernel<T><<<dim3((unsigned)((dim + 31) / 32), 2), dim3(ak::kThreads), 0, s>>>(g);
+      ak::grad_weight_kernel<T><<<dim3((unsigned)((dim + 15) / 16), 2), dim3(1024), 0, s>>>(g);
   };
   if (dtype == AK_DTYPE_F32) go(float());
   else if (dtype == AK_DTYPE_F16) go(ak::f16());

@@ -14,6 +14,9 @@
 // whose path the loader passes in, so there is one copy of them in the process.
 #include <dlfcn.h>
 
+#include <algorithm>
+#include <array>
+
 #include <c10/hip/HIPStream.h>
 #include <hip/hip_runtime_api.h>
 #include <torch/csrc/autograd/engine.h>
@@ -39,7 +42,9 @@ using Maybe = std::optional<Tensor>;
   X(ak_token_logprobs_workspace_bytes) X(ak_token_logprobs_fwd) X(ak_token_logprobs_bwd)                       \
   X(ak_topk_distill_workspace_bytes) X(ak_topk_distill_fwd) X(ak_topk_distill_bwd)                             \
   X(ak_lmhead_logprobs_workspace_bytes) X(ak_lmhead_logprobs_fwd) X(ak_lmhead_logprobs_coefs)                  \
-  X(ak_lmhead_logprobs_bwd_range)
+  X(ak_lmhead_logprobs_bwd_range)                                                                              \
+  X(ak_qk_norm_rotary_fwd) X(ak_qk_norm_rotary_bwd_workspace_bytes) X(ak_qk_norm_rotary_bwd)                   \
+  X(ak_paged_append) X(ak_paged_attention_workspace_bytes) X(ak_paged_attention)
 
 #define AK_FIELD(n) decltype(&::n) n = nullptr;
 struct Api { AK_ENTRIES(AK_FIELD) } api;
@@ -855,6 +860,310 @@ std::optional<std::tuple<Tensor, Tensor>> lmhead_logprobs(const Tensor& h, const
   return std::make_tuple(t ? out[1] : Tensor(), out[0]);
 }
 
+// ---------------------------------------------------------------------------
+// Attention heads: rotary positions, head norms, the paged cache
+// ---------------------------------------------------------------------------
+constexpr int64_t kMaxHeadDim = 2048, kMaxAttendDim = 1024;
+
+// [..., heads, dim] as the kernels take it (heads 0: not there).
+struct Heads {
+  int64_t outer = 1, inner = 1, heads = 0, dim = 0, so = 0, si = 0, sh = 0;
+};
+
+// False where the last dimension is not dense or the leading ones but the last do not fold.
+bool heads_of(const Tensor& t, Heads& h) {
+  const int64_t n = t.dim();
+  if (n < 2) return false;
+  h.heads = t.size(n - 2);
+  h.dim = t.size(n - 1);
+  h.sh = t.stride(n - 2);
+  if (h.dim > 1 && t.stride(n - 1) != 1) return false;
+  if (n > 2) {
+    h.inner = t.size(n - 3);
+    h.si = t.stride(n - 3);
+  }
+  if (n > 3) {
+    h.so = t.stride(n - 4);
+    for (int64_t i = 0; i < n - 3; ++i) {
+      h.outer *= t.size(i);
+      if (i + 1 < n - 3 && t.stride(i) != t.size(i + 1) * t.stride(i + 1)) return false;
+    }
+  }
+  return true;
+}
+
+// A gradient or saved tensor of a node the same way, copied where it has to be.
+Tensor heads_as(const Tensor& t, at::ScalarType type, Heads& h) {
+  Tensor r = t.to(type);
+  Heads x;
+  if (!heads_of(r, x)) {
+    r = r.contiguous();
+    x = Heads();
+    heads_of(r, x);
+  }
+  h = x;
+  return r;
+}
+
+bool dense_places(const Tensor& t) {
+  std::array<std::pair<int64_t, int64_t>, 4> d;
+  int n = 0;
+  for (int64_t i = 0; i < t.dim(); ++i)
+    if (t.size(i) > 1) d[n++] = {t.stride(i), t.size(i)};
+  std::sort(d.begin(), d.begin() + n);
+  int64_t reach = 1;
+  for (int i = 0; i < n; ++i) {
+    if (d[i].first < reach) return false;
+    reach += d[i].first * (d[i].second - 1);
+  }
+  return true;
+}
+
+bool table_ok(const Tensor& t, int64_t dim) {
+  return t.dim() == 2 && dense_f32(t) && t.size(0) > 0 && t.size(1) >= 2 && t.size(1) % 2 == 0 && t.size(1) <= dim &&
+         !t.requires_grad();
+}
+
+bool weight_ok(const Tensor& w, const Tensor& x) {
+  return w.dim() == 1 && w.size(0) == x.size(-1) && w.is_contiguous() && w.scalar_type() == x.scalar_type();
+}
+
+// Positions of the leading shape's last dimensions, as they are.
+bool positions_ok(const Tensor& p, const Tensor& q) {
+  const int64_t lead = q.dim() - 2, n = p.dim();
+  return (p.scalar_type() == at::kInt || p.scalar_type() == at::kLong) && p.is_contiguous() && n <= lead &&
+         p.sizes() == q.sizes().slice(lead - n, n) && p.numel() > 0;
+}
+
+int head_flags(const Tensor& positions, bool interleaved, bool inverse, bool zero) {
+  return (interleaved ? AK_ROTARY_INTERLEAVED : 0) | (inverse ? AK_ROTARY_INVERSE : 0) | (zero ? AK_ZERO_OTHER_ROWS : 0) |
+         (positions.defined() && positions.scalar_type() == at::kLong ? AK_POSITIONS_I64 : 0);
+}
+
+int64_t rotary_of(const Tensor& table) { return table.defined() ? table.size(1) : 0; }
+int64_t rows_in(const Tensor& table) { return table.defined() ? table.size(0) : 0; }
+
+struct Turn {
+  Tensor table, positions;
+  double eps;
+  bool interleaved;
+};
+
+int64_t n_positions(const Turn& t, const Heads& h) { return t.positions.defined() ? t.positions.numel() : h.inner; }
+
+// {q'} or {q', k'}; weights undefined: no norm
+variable_list run_heads(const Tensor& q, const Tensor& k, const Tensor& qw, const Tensor& kw, const Turn& t, bool inverse) {
+  Heads a, b;
+  const Tensor qr = heads_as(q, q.scalar_type(), a);
+  Tensor kr;
+  variable_list out{at::empty(q.sizes(), q.options())};
+  if (k.defined()) {
+    kr = heads_as(k, k.scalar_type(), b);
+    out.push_back(at::empty(k.sizes(), k.options()));
+  }
+  check(api.ak_qk_norm_rotary_fwd(ptr(qr), ptr(kr), ptr(qw), ptr(kw), f32p(t.table), ptr(t.positions), ptr(out[0]),
+                                  k.defined() ? ptr(out[1]) : nullptr, a.outer, a.inner, a.heads, b.heads, a.dim,
+                                  rotary_of(t.table), rows_in(t.table), n_positions(t, a), a.so, a.si, a.sh, b.so, b.si, b.sh,
+                                  (float)t.eps, head_flags(t.positions, t.interleaved, inverse, false),
+                                  code_of(q.scalar_type()), stream_of(q)), "ak_qk_norm_rotary_fwd");
+  return out;
+}
+
+void save_turn(AutogradContext* ctx, const Turn& t) {
+  ctx->saved_data["eps"] = t.eps;
+  ctx->saved_data["interleaved"] = t.interleaved;
+}
+
+Turn saved_turn(AutogradContext* ctx, const Tensor& table, const Tensor& positions) {
+  return {saved_as(table, at::kFloat), positions.defined() ? positions.contiguous() : positions,
+          ctx->saved_data["eps"].toDouble(), ctx->saved_data["interleaved"].toBool()};
+}
+
+Maybe given(const Tensor& t) { return t.defined() ? Maybe(t) : std::nullopt; }
+
+// Linear in q and k: its backward is itself, turned the other way.
+struct Rotary : torch::autograd::Function<Rotary> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const Maybe& k_, const Tensor& table,
+                               const Maybe& positions_, bool interleaved, bool inverse) {
+    const Tensor k = k_.value_or(Tensor()), positions = positions_.value_or(Tensor());
+    const Turn t{table, positions, 0.0, interleaved};
+    ctx->save_for_backward({table, positions});
+    save_turn(ctx, t);
+    ctx->saved_data["inverse"] = inverse;
+    return run_heads(q, k, Tensor(), Tensor(), t, inverse);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const auto s = ctx->get_saved_variables();
+    const Turn t = saved_turn(ctx, s[0], s[1]);
+    const bool inverse = !ctx->saved_data["inverse"].toBool();
+    for (const Tensor& x : g)
+      TORCH_CHECK(!x.defined() || !x._fw_grad(0).defined(),
+                  "rotary has no forward-mode derivative: its backward is the derivative there is");
+    const Tensor gk = g.size() > 1 ? g[1] : Tensor();
+    variable_list r = records({&g[0], &gk}) ? Rotary::apply(g[0], given(gk), t.table, given(t.positions), t.interleaved, inverse)
+                                            : run_heads(g[0], gk, Tensor(), Tensor(), t, inverse);
+    return {r[0], gk.defined() ? r[1] : Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+struct QkNormRotary : torch::autograd::Function<QkNormRotary> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const Maybe& k_, const Tensor& qw, const Maybe& kw_,
+                               const Maybe& table_, const Maybe& positions_, double eps, bool interleaved) {
+    const Tensor k = k_.value_or(Tensor()), kw = kw_.value_or(Tensor()), table = table_.value_or(Tensor()),
+                 positions = positions_.value_or(Tensor());
+    const Turn t{table, positions, eps, interleaved};
+    ctx->save_for_backward({q, k, qw, kw, table, positions});
+    save_turn(ctx, t);
+    ctx->saved_data["qw"] = qw.requires_grad();
+    ctx->saved_data["kw"] = kw.defined() && kw.requires_grad();
+    return run_heads(q, k, qw, kw, t, false);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    differentiable_once("qk_norm_rotary", g);
+    const auto s = ctx->get_saved_variables();
+    const Turn t = saved_turn(ctx, s[4], s[5]);
+    const at::ScalarType type = s[0].scalar_type();
+    Heads a, b, ga, gb;
+    const Tensor q = heads_as(s[0], type, a), gq = heads_as(g[0], type, ga), qw = saved_as(s[2], type), kw = saved_as(s[3], type);
+    Tensor k, gk, dk, dqw, dkw;
+    const Tensor dq = at::empty(q.sizes(), q.options());
+    if (s[1].defined()) {
+      k = heads_as(s[1], type, b);
+      gk = heads_as(g[1], type, gb);
+      dk = at::empty(k.sizes(), k.options());
+    }
+    if (ctx->saved_data["qw"].toBool()) dqw = at::empty({a.dim}, q.options());
+    if (ctx->saved_data["kw"].toBool()) dkw = at::empty({a.dim}, q.options());
+    const size_t bytes = api.ak_qk_norm_rotary_bwd_workspace_bytes(a.outer * a.inner, a.heads, b.heads, a.dim);
+    const Tensor ws = bytes_like(q, bytes);
+    check(api.ak_qk_norm_rotary_bwd(ptr(q), ptr(k), ptr(qw), ptr(kw), f32p(t.table), ptr(t.positions), ptr(gq), ptr(gk), ptr(dq),
+                                    ptr(dk), ptr(dqw), ptr(dkw), ptr(ws), bytes, a.outer, a.inner, a.heads, b.heads, a.dim,
+                                    rotary_of(t.table), rows_in(t.table), n_positions(t, a), a.so, a.si, a.sh, b.so, b.si, b.sh,
+                                    ga.so, ga.si, ga.sh, gb.so, gb.si, gb.sh, (float)t.eps,
+                                    head_flags(t.positions, t.interleaved, false, false), code_of(type), stream_of(q)),
+          "ak_qk_norm_rotary_bwd");
+    return {dq, dk, dqw, dkw, Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+using Two = std::optional<std::tuple<Tensor, Tensor>>;
+
+// The tensors of a call of either operator in their plain form.
+bool heads_args(const Tensor& q, const Maybe& k, const Maybe& table, const Maybe& positions) {
+  Heads a, b;
+  if (code_of(q.scalar_type()) < 0 || !heads_of(q, a) || a.dim < 1 || a.dim > kMaxHeadDim || q.numel() == 0) return false;
+  if (k && (k->scalar_type() != q.scalar_type() || !heads_of(*k, b) || k->dim() != q.dim() || b.dim != a.dim || k->numel() == 0 ||
+            k->sizes().slice(0, k->dim() - 2) != q.sizes().slice(0, q.dim() - 2)))
+    return false;
+  return (!table || table_ok(*table, a.dim)) && (!positions || positions_ok(*positions, q));
+}
+
+Two pair_of(const variable_list& v) { return std::make_tuple(v[0], v.size() > 1 ? v[1] : Tensor()); }
+
+Two rotary(const Tensor& q, const Maybe& k, const Tensor& table, const Maybe& positions, bool interleaved) {
+  if (!ours(q, table) || !ours_if(k, q) || !ours_if(positions, q) || !heads_args(q, k, table, positions)) return std::nullopt;
+  const Tensor kk = k.value_or(Tensor()), p = positions.value_or(Tensor());
+  if (records({&q, &kk})) return pair_of(Rotary::apply(q, k, table, positions, interleaved, false));
+  return pair_of(run_heads(q, kk, Tensor(), Tensor(), Turn{table, p, 0.0, interleaved}, false));
+}
+
+Two qk_norm_rotary(const Tensor& q, const Maybe& k, const Tensor& qw, const Maybe& kw, const Maybe& table, const Maybe& positions,
+                   double eps, bool interleaved) {
+  if (!ours(q, qw) || !ours_if(k, q) || !ours_if(kw, q) || !ours_if(table, q) || !ours_if(positions, q) ||
+      !heads_args(q, k, table, positions) || !weight_ok(qw, q) || k.has_value() != kw.has_value() || (kw && !weight_ok(*kw, q)) ||
+      (positions && !table))
+    return std::nullopt;
+  const Tensor kk = k.value_or(Tensor()), kkw = kw.value_or(Tensor()), t = table.value_or(Tensor()),
+               p = positions.value_or(Tensor());
+  if (records({&q, &kk, &qw, &kkw})) return pair_of(QkNormRotary::apply(q, k, qw, kw, table, positions, eps, interleaved));
+  return pair_of(run_heads(q, kk, qw, kkw, Turn{t, p, eps, interleaved}, false));
+}
+
+// The cache and the batch of a call on them, as the kernels take them.
+bool paged_args(const Tensor& k_cache, const Tensor& v_cache, const Tensor& pages, const Tensor& lengths, const Maybe& starts,
+                int64_t heads, int64_t dim, at::ScalarType type, int64_t tokens) {
+  const auto cache = [&](const Tensor& c) {
+    return c.dim() == 4 && c.scalar_type() == type && c.size(1) > 0 && c.size(2) == heads && c.size(3) == dim &&
+           (dim == 1 || c.stride(3) == 1);
+  };
+  const auto i32 = [](const Tensor& t, int64_t n) { return t.scalar_type() == at::kInt && t.dim() == 1 && t.size(0) == n && t.is_contiguous(); };
+  if (!cache(k_cache) || !cache(v_cache) || k_cache.sizes() != v_cache.sizes() || pages.scalar_type() != at::kInt || pages.dim() != 2)
+    return false;
+  const int64_t batch = pages.size(0), width = pages.size(1);
+  return i32(lengths, batch) && (width <= 1 || pages.stride(1) == 1) && (batch <= 1 || pages.stride(0) >= width) && batch > 0 &&
+         (starts ? i32(*starts, batch + 1) : tokens % batch == 0);
+}
+
+int32_t* i32p(const Tensor& t) { return static_cast<int32_t*>(ptr(t)); }
+int64_t page_pitch(const Tensor& pages) { return pages.size(0) > 1 ? pages.stride(0) : pages.size(1); }
+
+bool rows3(const Tensor& t, at::ScalarType type) { return t.dim() == 3 && t.scalar_type() == type && (t.size(2) == 1 || t.stride(2) == 1); }
+
+void wrote(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
+// (done, q'): q' undefined (None) without q
+std::optional<std::tuple<bool, Tensor>> paged_append(const Tensor& k, const Tensor& v, const Tensor& k_cache, const Tensor& v_cache,
+                                                     const Tensor& pages, const Tensor& lengths, const Maybe& starts, const Maybe& q,
+                                                     const Maybe& q_weight, const Maybe& k_weight, double eps, const Maybe& table,
+                                                     bool interleaved, const Maybe& q_out) {
+  if (!ours(k, v, k_cache, v_cache, pages, lengths) || !ours_if(starts, k) || !ours_if(q, k) || !ours_if(q_weight, k) ||
+      !ours_if(k_weight, k) || !ours_if(table, k) || !ours_if(q_out, k))
+    return std::nullopt;
+  const at::ScalarType type = k.scalar_type();
+  if (code_of(type) < 0 || !rows3(k, type) || !rows3(v, type) || k.sizes() != v.sizes() || k.numel() == 0) return std::nullopt;
+  const int64_t tokens = k.size(0), heads = k.size(1), dim = k.size(2);
+  if (dim > kMaxHeadDim || !paged_args(k_cache, v_cache, pages, lengths, starts, heads, dim, type, tokens) || !dense_places(k_cache) ||
+      !dense_places(v_cache) || (q ? !rows3(*q, type) || q->size(0) != tokens || q->size(2) != dim : q_weight || q_out) ||
+      (q_out && (!rows3(*q_out, type) || q_out->sizes() != q->sizes() || !dense_places(*q_out))) || (q_weight && !weight_ok(*q_weight, k)) ||
+      (k_weight && !weight_ok(*k_weight, k)) || (table && !table_ok(*table, dim)))
+    return std::nullopt;
+  const Tensor qq = q.value_or(Tensor()), qw = q_weight.value_or(Tensor()), kw = k_weight.value_or(Tensor()),
+               t = table.value_or(Tensor()), st = starts.value_or(Tensor());
+  Tensor out = q_out.value_or(Tensor());
+  if (records({&k, &v, &k_cache, &v_cache, &qq, &qw, &kw, &out})) return std::nullopt;
+  if (q && !q_out) out = at::empty(q->sizes(), q->options());
+  const auto row = [](const Tensor& x, int i) { return x.defined() ? x.stride(i) : 0; };
+  check(api.ak_paged_append(ptr(qq), ptr(k), ptr(v), ptr(qw), ptr(kw), f32p(t), ptr(out), ptr(k_cache), ptr(v_cache), i32p(pages),
+                            i32p(lengths), i32p(st), tokens, pages.size(0), q ? q->size(1) : 0, heads, dim, rotary_of(t), rows_in(t),
+                            k_cache.size(0), k_cache.size(1), pages.size(1), page_pitch(pages), row(qq, 0), row(qq, 1), k.stride(0),
+                            k.stride(1), v.stride(0), v.stride(1), row(out, 0), row(out, 1), k_cache.stride(0), k_cache.stride(1),
+                            k_cache.stride(2), v_cache.stride(0), v_cache.stride(1), v_cache.stride(2), (float)eps,
+                            head_flags(Tensor(), interleaved, false, !q_out), code_of(type), stream_of(k)), "ak_paged_append");
+  wrote(k_cache);
+  wrote(v_cache);
+  if (q_out) wrote(out);
+  return std::make_tuple(true, out);
+}
+
+Maybe paged_attention(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, const Tensor& pages, const Tensor& lengths,
+                      const Maybe& starts, double scale, double softcap, int64_t window, int64_t max_chunk, const Maybe& out_) {
+  if (!ours(q, k_cache, v_cache, pages, lengths) || !ours_if(starts, q) || !ours_if(out_, q)) return std::nullopt;
+  const at::ScalarType type = q.scalar_type();
+  if (code_of(type) < 0 || !rows3(q, type) || q.numel() == 0 || k_cache.dim() != 4) return std::nullopt;
+  const int64_t tokens = q.size(0), heads = q.size(1), dim = q.size(2), kv = k_cache.size(2);
+  if (dim > kMaxAttendDim || kv < 1 || heads % kv || !paged_args(k_cache, v_cache, pages, lengths, starts, kv, dim, type, tokens) ||
+      (out_ && (!rows3(*out_, type) || out_->sizes() != q.sizes() || !dense_places(*out_))))
+    return std::nullopt;
+  const Tensor st = starts.value_or(Tensor());
+  Tensor out = out_.value_or(Tensor());
+  if (records({&q, &k_cache, &v_cache, &out})) return std::nullopt;
+  if (!out_) out = at::empty(q.sizes(), q.options());
+  const int64_t batch = pages.size(0), keys = pages.size(1) * k_cache.size(1);
+  const int code = code_of(type);
+  const int64_t chunk = starts ? std::min(max_chunk, tokens) : tokens / batch;
+  const size_t bytes = api.ak_paged_attention_workspace_bytes(tokens, batch, heads, kv, dim, keys, chunk, code);
+  const Tensor ws = bytes ? bytes_like(q, bytes) : Tensor();
+  check(api.ak_paged_attention(ptr(q), ptr(k_cache), ptr(v_cache), i32p(pages), i32p(lengths), i32p(st), ptr(out), ptr(ws), bytes,
+                               tokens, batch, heads, kv, dim, k_cache.size(0), k_cache.size(1), pages.size(1), page_pitch(pages),
+                               chunk, q.stride(0), q.stride(1), out.stride(0), out.stride(1), k_cache.stride(0), k_cache.stride(1),
+                               k_cache.stride(2), v_cache.stride(0), v_cache.stride(1), v_cache.stride(2), (float)scale,
+                               (float)softcap, window, out_ ? 0 : AK_ZERO_OTHER_ROWS, code, stream_of(q)), "ak_paged_attention");
+  if (out_) wrote(out);
+  return out;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_host_ops, m) {
@@ -876,4 +1185,8 @@ PYBIND11_MODULE(_host_ops, m) {
   m.def("token_logprobs", &token_logprobs, nogil());
   m.def("topk_distillation", &topk_distillation, nogil());
   m.def("lmhead_logprobs", &lmhead_logprobs, nogil());
+  m.def("rotary", &rotary, nogil());
+  m.def("qk_norm_rotary", &qk_norm_rotary, nogil());
+  m.def("paged_append", &paged_append, nogil());
+  m.def("paged_attention", &paged_attention, nogil());
 }

@@ -829,28 +829,79 @@ __global__ void __launch_bounds__(256) attend_join_kernel(TileArgs g) {
   const int parts = (int)(w1 - w0 + 1);
   const float* first = g.part + (2 * w0 + (begin_of(w0, total, n) < p.begin)) * one;
   const float* rest = g.part + 2 * (w0 + 1) * one;  // part i > 0: two slots further each
-  for (int row = blockIdx.y * 4 + wave; row < rows; row += 4 * gridDim.y) {
-    auto part = [&](int i) { return (i == 0 ? first : rest + (int64_t)(i - 1) * 2 * one) + (int64_t)row * (DB + 2); };
-    float top = kNegInf, sum = 0.0f;
-    for (int i = lane; i < parts; i += 64) top = fmaxf(top, part(i)[DB]);
-    top = wave_max(top);
-    auto factor = [&](float m) { return top == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(m - top); };
-    for (int i = lane; i < parts; i += 64) sum += factor(part(i)[DB]) * part(i)[DB + 1];
-    sum = wave_sum(sum);
-    float acc[kVals] = {};
-#pragma unroll 4
-    for (int i = 0; i < parts; ++i) {
-      const float* x = part(i);
-      const float f = factor(x[DB]);
+  auto part = [&](int i, int row) { return (i == 0 ? first : rest + (int64_t)(i - 1) * 2 * one) + (int64_t)row * (DB + 2); };
+  // R rows of the parts begin, begin + step, ..: their maxima, sums, products of the values
+  auto gather = [&](auto rows_tag, int row0, int begin, int step, float* inv, float (*acc)[kVals]) {
+    constexpr int R = decltype(rows_tag)::value, kUnroll = R > 1 ? 2 : 8;
+    float top[R], sum[R];
 #pragma unroll
-      for (int v = 0; v < kVals; ++v) acc[v] = fmaf(f, x[64 * v + lane], acc[v]);
+    for (int k = 0; k < R; ++k) {
+      const int row = min(row0 + k, rows - 1);
+      top[k] = kNegInf;
+      for (int i = lane; i < parts; i += 64) top[k] = fmaxf(top[k], part(i, row)[DB]);
     }
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    auto factor = [&](float m, int k) { return top[k] == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(m - top[k]); };
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      const int row = min(row0 + k, rows - 1);
+      top[k] = wave_max(top[k]);
+      sum[k] = 0.0f;
+      for (int i = lane; i < parts; i += 64) sum[k] += factor(part(i, row)[DB], k) * part(i, row)[DB + 1];
+#pragma unroll
+      for (int v = 0; v < kVals; ++v) acc[k][v] = 0.0f;
+    }
+#pragma unroll kUnroll
+    for (int i = begin; i < parts; i += step) {
+#pragma unroll
+      for (int k = 0; k < R; ++k) {
+        const float* x = part(i, min(row0 + k, rows - 1));
+        const float f = factor(x[DB], k);
+#pragma unroll
+        for (int v = 0; v < kVals; ++v) acc[k][v] = fmaf(f, x[64 * v + lane], acc[k][v]);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      sum[k] = wave_sum(sum[k]);
+      inv[k] = sum[k] == 0.0f ? 0.0f : 1.0f / sum[k];
+    }
+  };
+  auto store = [&](int row, const float* acc, float inv) {
     const int i = row / g.group;
     T* out = static_cast<T*>(g.a.out) + (p.s.first + t0 + i) * g.a.o_st + (int64_t)(p.h * g.group + row - i * g.group) * g.a.o_sh;
 #pragma unroll
     for (int v = 0; v < kVals; ++v)
       if (64 * v + lane < g.a.dim) out[64 * v + lane] = from_f32<T>(acc[v] * inv);
+  };
+  if (g.rows > kRows) {
+    // many rows in few parts: 8 rows a wave at a time, their loads together
+    constexpr int R = 8;
+    for (int row = (blockIdx.y * 4 + wave) * R; row < rows; row += 4 * R * gridDim.y) {
+      float inv[R], acc[R][kVals];
+      gather(std::integral_constant<int, R>(), row, 0, 1, inv, acc);
+#pragma unroll
+      for (int k = 0; k < R; ++k)
+        if (row + k < rows) store(row + k, acc[k], inv[k]);
+    }
+  } else {
+    // few rows in many parts: a row at a time, the parts over the waves
+    __shared__ float sums[4][DB];
+    for (int row = blockIdx.y; row < rows; row += gridDim.y) {
+      float inv[1], acc[1][kVals];
+      gather(std::integral_constant<int, 1>(), row, wave, 4, inv, acc);
+#pragma unroll
+      for (int v = 0; v < kVals; ++v) sums[wave][64 * v + lane] = acc[0][v];
+      __syncthreads();
+      if (wave == 0) {
+#pragma unroll
+        for (int v = 0; v < kVals; ++v) {
+          const int d = 64 * v + lane;
+          acc[0][v] = (sums[0][d] + sums[1][d]) + (sums[2][d] + sums[3][d]);
+        }
+        store(row, acc[0], inv[0]);
+      }
+      __syncthreads();
+    }
   }
 }
 
@@ -903,7 +954,7 @@ void launch_tiles(const TileArgs& g, const Plan& p, hipStream_t s) {
     attend_many_kernel<T, DB, kWaves, kUnit, LANE><<<dim3((unsigned)p.workers), dim3(64 * kWaves), 0, s>>>(g);
   }
   if (p.workers > 1) {
-    const unsigned slices = p.rows > 4 ? (p.rows > 32 ? 8 : 2) : 1;
+    const unsigned slices = (unsigned)(p.rows > kRows ? (p.rows + 31) / 32 : std::min(p.rows, 4));
     attend_join_kernel<T, DB><<<dim3((unsigned)(p.workers - 1), slices), dim3(256), 0, s>>>(g);
   }
 }

@@ -207,6 +207,11 @@ def native(*tensors):
     return _host or host()  # (which looks at the other tensors' devices itself)
 
 
+def given(*tensors) -> tuple:
+    """Those of some optional tensors that are there."""
+    return tuple(t for t in tensors if t is not None)
+
+
 def is_available() -> bool:
     return os.path.exists(lib_path())
 

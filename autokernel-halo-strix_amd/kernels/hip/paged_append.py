@@ -57,6 +57,12 @@ def kernel_fn(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: 
             q itself; None: a new tensor (with zeros there).
     """
     eps, interleaved = check_eps(eps), bool(interleaved)
+    host = _lib.native(k, v, k_cache, v_cache, page_table, lengths, *_lib.given(starts, q, q_weight, k_weight, table, q_out))
+    if host is not None:
+        done = host.paged_append(k, v, k_cache, v_cache, page_table, lengths, starts, q, q_weight, k_weight, eps, table,
+                                 interleaved, q_out)
+        if done is not None:
+            return q_out if q_out is not None else done[1]
     _lib.require_device(k, v, k_cache, v_cache, page_table, lengths, starts, q, q_weight, k_weight, table, q_out)
     _heads.no_gradient(KERNEL_TYPE, k, v, k_cache, v_cache, q, q_weight, k_weight, q_out)
     _lib.dtype_code(k.dtype)

@@ -70,6 +70,15 @@ def kernel_fn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, pag
         out: where the result goes (rows of no sequence stay as they are); None: a new
             tensor (with zeros there).
     """
+    host = _lib.native(q, k_cache, v_cache, page_table, lengths, *_lib.given(starts, out))
+    if host is not None and q.dim() == 3 and q.shape[2]:
+        numbers = check_scores(scale, softcap, window, q.shape[2])
+        if max_chunk is not None and int(max_chunk) < 1:
+            raise ValueError(f"max_chunk must be positive, got {max_chunk}")
+        done = host.paged_attention(q, k_cache, v_cache, page_table, lengths, starts, *numbers,
+                                    q.shape[0] if max_chunk is None else int(max_chunk), out)
+        if done is not None:
+            return done if out is None else out
     _lib.require_device(q, k_cache, v_cache, page_table, lengths, starts, out)
     _heads.no_gradient(KERNEL_TYPE, q, k_cache, v_cache, out)
     _lib.dtype_code(q.dtype)

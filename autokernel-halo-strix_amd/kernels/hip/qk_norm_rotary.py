@@ -97,6 +97,11 @@ def kernel_fn(q: torch.Tensor, k: Optional[torch.Tensor], q_weight: torch.Tensor
         eps: added to the mean square.
     """
     eps, interleaved = check_eps(eps), bool(interleaved)
+    host = _lib.native(q, *_lib.given(k, q_weight, k_weight, table, positions))
+    if host is not None and q_weight is not None:
+        out = host.qk_norm_rotary(q, k, q_weight, k_weight, table, positions, eps, interleaved)
+        if out is not None:
+            return out
     _lib.require_device(q, k, q_weight, k_weight, table, positions)
     refuse_tangents(KERNEL_TYPE, q, k, q_weight, k_weight)
     check_pair(q, k)

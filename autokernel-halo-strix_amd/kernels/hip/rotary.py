@@ -167,6 +167,11 @@ def kernel_fn(q: torch.Tensor, k: Optional[torch.Tensor], table: torch.Tensor, p
         interleaved: pairs of neighbours instead of halves.
     """
     interleaved = bool(interleaved)
+    host = _lib.native(q, *_lib.given(k, table, positions))
+    if host is not None:
+        out = host.rotary(q, k, table, positions, interleaved)
+        if out is not None:
+            return out
     _lib.require_device(q, k, table, positions)
     refuse_tangents(KERNEL_TYPE, q, k)
     check_pair(q, k)

@@ -404,3 +404,69 @@ def test_streams_and_graphs():
             if j >= len(outs) - 2:
                 a, b = a[b.abs().sum(-1) > 0], b[b.abs().sum(-1) > 0]
             assert torch.equal(a, b), (i, j)
+
+
+def test_host_forms():
+    """The native host side and the Python one give the same bits, with the same autograd contract."""
+    need_gpu()
+    from kernels.hip import _lib, paged_append, paged_attention, qk_norm_rotary, rotary
+    g = torch.Generator().manual_seed(16)
+    dtype = torch.bfloat16
+    q, k = randn(g, 2, 9, 4, 64).to(dtype).to(DEV), randn(g, 2, 9, 2, 64).to(dtype).to(DEV)
+    wq, wk = (1 + 0.1 * randn(g, 64)).to(dtype).to(DEV), (1 + 0.1 * randn(g, 64)).to(dtype).to(DEV)
+    table, pos = table_of(32, 40).to(DEV), torch.randint(0, 40, (2, 9), generator=g).to(DEV)
+    pages, lens, starts, total = (t.to(DEV) if isinstance(t, torch.Tensor) else t for t in make_batch([12, 6], [20, 6], 8, 17))
+    caches = [torch.zeros(total, 8, 2, 64, dtype=dtype, device=DEV) for _ in range(2)]
+    ups = [randn(g, 2, 9, 4, 64).to(dtype).to(DEV), randn(g, 2, 9, 2, 64).to(dtype).to(DEV)]
+
+    def run():
+        out = []
+        leaves = [t.detach().requires_grad_() for t in (q, k, wq, wk)]
+        for p in (pos, None):
+            y = rotary.kernel_fn(*leaves[:2], table, p, interleaved=True)
+            out += [*y, *torch.autograd.grad(y, leaves[:2], ups)]
+            y = qk_norm_rotary.kernel_fn(*leaves, table, p)
+            out += [*y, *torch.autograd.grad(y, leaves, ups)]
+        y, none = qk_norm_rotary.kernel_fn(leaves[0], None, leaves[2], None)
+        assert none is None
+        out += [y, *torch.autograd.grad(y, (leaves[0], leaves[2]), ups[0])]
+        y = rotary.kernel_fn(leaves[0], None, table)[0]
+        # (an expanded gradient, and a transposed one)
+        out += [*torch.autograd.grad(y.sum(), leaves[0], retain_graph=True),
+                *torch.autograd.grad((y.transpose(1, 3) * ups[0].transpose(1, 3).contiguous()).sum(), leaves[0])]
+        flat_q, flat_k = q.view(18, 4, 64), k.view(18, 2, 64)
+        with torch.no_grad():
+            r = paged_append.kernel_fn(flat_k, flat_k, *caches, pages, lens, starts, q=flat_q, q_weight=wq, k_weight=wk, table=table)
+        out += [r, *(c.clone() for c in caches)]
+        out.append(paged_attention.kernel_fn(r, *caches, pages, lens, starts, window=7, softcap=9.0))
+        assert not any(t.requires_grad for t in out[-4:])
+        return out
+
+    say("native")
+    native = run()
+    real = _lib.native
+    try:
+        _lib.native = lambda *t: None
+        say("python")
+        python = run()
+    finally:
+        _lib.native = real
+    assert len(native) == len(python)
+    assert all(torch.equal(a, b) and a.requires_grad == b.requires_grad for a, b in zip(native, python))
+    x = q.detach().requires_grad_()
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(qk_norm_rotary.kernel_fn(x, None, wq, None)[0].float().square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        paged_attention.kernel_fn(x.view(18, 4, 64), *caches, pages, lens, starts)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        paged_append.kernel_fn(k.view(18, 2, 64).requires_grad_(), k.view(18, 2, 64), *caches, pages, lens, starts)
+    with torch.autograd.forward_ad.dual_level():
+        d = torch.autograd.forward_ad.make_dual(q.detach(), torch.ones_like(q))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            rotary.kernel_fn(d, None, table)
+    with torch.inference_mode():
+        flat_k = k.view(18, 2, 64).clone()
+        paged_append.kernel_fn(flat_k, flat_k, *(c.clone() for c in caches), pages, lens, starts)
+    version = caches[0]._version
+    paged_append.kernel_fn(k.detach().view(18, 2, 64), k.detach().view(18, 2, 64), *caches, pages, lens, starts)
+    assert caches[0]._version > version
