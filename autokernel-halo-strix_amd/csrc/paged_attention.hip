@@ -181,7 +181,7 @@ extern "C" int ak_paged_attention(const void* q, const void* k_cache, const void
   int rc = ak::check_paged(name, tokens, batch, n_pages, page_size, max_pages, ld_pages, starts, lengths, page_table);
   if (rc) return rc;
   if (q_heads < 1 || kv_heads < 1 || q_heads % kv_heads || q_heads > 65536 || tokens > INT32_MAX / q_heads ||
-      (__int128)max_pages * page_size > INT32_MAX || !ak::extent_ok(1, 0, tokens, q_st, q_heads, q_sh, dim, esz) ||
+      (__int128)max_pages * page_size > INT32_MAX - 4096 || !ak::extent_ok(1, 0, tokens, q_st, q_heads, q_sh, dim, esz) ||
       !ak::extent_ok(1, 0, tokens, o_st, q_heads, o_sh, dim, esz) ||
       !ak::extent_ok(n_pages, kc_sp, page_size, kc_ss, kv_heads, kc_sh, dim, esz) ||
       !ak::extent_ok(n_pages, vc_sp, page_size, vc_ss, kv_heads, vc_sh, dim, esz))

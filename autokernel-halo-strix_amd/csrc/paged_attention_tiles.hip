@@ -27,6 +27,13 @@ constexpr int kPlanBatch = 1024;   // sequences that a workgroup lines up by its
 typedef float f32x4_v __attribute__((ext_vector_type(4)));
 typedef const int32_t __attribute__((address_space(4)))* ConstI32;
 
+// What the joining kernel does for a worker: the rows of its last tile, whose first part
+// is the worker's own.
+struct Job {
+  int64_t token, first;  // the tile's first token of the call; its part's slot
+  int head, rows, parts, pad;  // its first query head; rows 0: nothing
+};
+
 struct TileArgs {
   AttendArgs a;
   int group, per_tile;             // heads of a group, tokens of a tile
@@ -34,6 +41,7 @@ struct TileArgs {
   int unit, rows;                  // keys of a unit, rows of a tile
   int workers, min_units;
   int64_t* line;                   // [batch + 1]: the units before each sequence
+  Job* jobs;                       // [workers]
   float* part;                     // [2 workers][rows][DB + 2]: sums of products, maximum, sum
   float c, cap_in, cap_out;        // scores in base 2: s c, or cap_out tanh(s cap_in)
 };
@@ -471,6 +479,20 @@ __device__ __forceinline__ void rows_end(const TileArgs& g, const Place& p, int 
     }
 }
 
+// The job that a worker leaves, given the part of its last tile that it has begun but not ended (or none).
+__device__ __forceinline__ void leave_job(const TileArgs& g, int64_t worker, const Place* p, int64_t slot, int64_t total, int64_t n) {
+  Job j{};
+  if (p != nullptr) {
+    const int t0 = p->t * g.per_tile;
+    j.token = p->s.first + t0;
+    j.first = slot;
+    j.head = p->h * g.group;
+    j.rows = min(g.per_tile, p->s.count - t0) * g.group;
+    j.parts = (int)(worker_of(p->begin + (p->k.u1 - p->k.u0) - 1, total, n) - worker) + 1;
+  }
+  g.jobs[worker] = j;
+}
+
 // Zeros for the rows of no sequence, a token a wave at a time.
 template <typename T>
 __device__ __forceinline__ void zero_other_rows(const TileArgs& g, int64_t wave, int64_t waves) {
@@ -485,78 +507,75 @@ __device__ __forceinline__ void zero_other_rows(const TileArgs& g, int64_t wave,
   }
 }
 
-// The K and V rows of up to 64 keys, as N loads of a wave each: load i takes rows
-// first + i * stride .. + kPerLoad - 1 from key0 on. LANE: pages that are no multiple of
-// a load's rows, looked up lane by lane; else they are scalar work.
-template <typename T, int DB, int N, bool LANE>
+// The pages of a unit's keys, a key a lane (its 32 or 64 rows): looked up while the unit
+// before it is loaded.
+template <int UNIT, int GROUP>
+struct Pages {
+  int page, slot;  // page -1: no key of the tile
+
+  // GROUP rows are loaded together, seen by some row of the tile or not.
+  __device__ __forceinline__ void look_up(const TileArgs& g, const Place& p, int key0) {
+    const int key = key0 + (threadIdx.x & (UNIT - 1));
+    page = -1;
+    slot = 0;
+    if (key >= (p.k.lo & -GROUP) && key < p.k.hi) {
+      uint32_t at, in;
+      key_place(g, (uint32_t)key, at, in);
+      slot = (int)in;
+      page = g.a.pages[p.b * g.a.ld_pages + at];
+    }
+  }
+  __device__ __forceinline__ bool there(const TileArgs& g, int pg) const { return pg >= 0 && pg < (int)g.a.n_pages; }
+  // The keys that are there, by row.
+  __device__ __forceinline__ uint64_t seen(const TileArgs& g) const {
+    const uint64_t all = __ballot(there(g, page));
+    return UNIT == 64 ? all : all & 0xFFFFFFFFu;
+  }
+};
+
+// The K and V rows of a unit, as N loads of a wave each: load i takes rows first + i *
+// stride .. + kPerLoad - 1. LANE: pages that are no multiple of a load's rows, so that a
+// load's rows are on pages of their own; else its address is scalar work.
+template <typename T, int DB, int N, int UNIT, bool LANE>
 struct Loads {
   using S = Shape<T, DB>;
+  using P = Pages<UNIT, LANE ? 1 : S::kPerLoad>;
   u32x4 k[N], v[N];
 
-  // Returns the bits (by row) of the keys that are there, of this wave's rows.
-  __device__ __forceinline__ uint64_t issue(const TileArgs& g, const Place& p, int key0, int first, int stride) {
+  __device__ __forceinline__ void issue(const TileArgs& g, const Place& p, const P& pg, int first, int stride) {
     const int lane = threadIdx.x & 63;
     const int in = lane / S::kChunks, d = (lane % S::kChunks) * S::VE;
-    uint64_t there = 0;
     const T* k0 = static_cast<const T*>(g.a.k) + (int64_t)p.h * g.a.kh;
     const T* v0 = static_cast<const T*>(g.a.v) + (int64_t)p.h * g.a.vh;
     if constexpr (LANE) {
-      int64_t page[N];
-      uint32_t slot[N];
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const int row = first + i * stride + in, key = key0 + row;
-        page[i] = -1;
-        slot[i] = 0;
-        if (key >= p.k.lo && key < p.k.hi) {
-          uint32_t at;
-          key_place(g, (uint32_t)key, at, slot[i]);
-          page[i] = g.a.pages[p.b * g.a.ld_pages + at];
-          if (page[i] >= g.a.n_pages) page[i] = -1;
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
+        const int page = __shfl(pg.page, first + i * stride + in), slot = __shfl(pg.slot, first + i * stride + in);
         k[i] = v[i] = u32x4{0, 0, 0, 0};
-        const uint64_t ok = __ballot(page[i] >= 0);
-#pragma unroll
-        for (int x = 0; x < S::kPerLoad; ++x)
-          there |= ((ok >> (x * S::kChunks)) & 1) << (first + i * stride + x);
-        if (page[i] >= 0 && d < g.a.dim) {
-          k[i] = *reinterpret_cast<const u32x4*>(k0 + page[i] * g.a.kp + (int64_t)slot[i] * g.a.ks + d);
-          v[i] = *reinterpret_cast<const u32x4*>(v0 + page[i] * g.a.vp + (int64_t)slot[i] * g.a.vs + d);
+        if (pg.there(g, page) && d < g.a.dim) {
+          k[i] = *reinterpret_cast<const u32x4*>(k0 + (int64_t)page * g.a.kp + (int64_t)slot * g.a.ks + d);
+          v[i] = *reinterpret_cast<const u32x4*>(v0 + (int64_t)page * g.a.vp + (int64_t)slot * g.a.vs + d);
         }
       }
     } else {
-      const ConstI32 pages = (ConstI32)(uintptr_t)(g.a.pages + p.b * g.a.ld_pages);
       const int64_t ko = (int64_t)in * g.a.ks + d, vo = (int64_t)in * g.a.vs + d;
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const int row = first + i * stride, key = key0 + row;
+        // (rows of the load past the tile's keys are memory of the same page, hidden below)
+        const int page = __builtin_amdgcn_readlane(pg.page, first + i * stride);
+        const int slot = __builtin_amdgcn_readlane(pg.slot, first + i * stride);
         k[i] = v[i] = u32x4{0, 0, 0, 0};
-        // a load's rows share a page: there if any of them is to be seen (the rest of
-        // them is memory of the page, hidden below)
-        if (key + S::kPerLoad > p.k.lo && key < p.k.hi) {
-          uint32_t at, slot;
-          key_place(g, (uint32_t)key, at, slot);
-          const int64_t page = pages[at];
-          if (page >= 0 && page < g.a.n_pages) {
-            there |= ((1ull << S::kPerLoad) - 1) << row;
-            if (d < g.a.dim) {
-              k[i] = *reinterpret_cast<const u32x4*>(k0 + page * g.a.kp + (int64_t)slot * g.a.ks + ko);
-              v[i] = *reinterpret_cast<const u32x4*>(v0 + page * g.a.vp + (int64_t)slot * g.a.vs + vo);
-            }
-          }
+        if (pg.there(g, page) && d < g.a.dim) {
+          k[i] = *reinterpret_cast<const u32x4*>(k0 + ((int64_t)page * g.a.kp + (int64_t)slot * g.a.ks) + ko);
+          v[i] = *reinterpret_cast<const u32x4*>(v0 + ((int64_t)page * g.a.vp + (int64_t)slot * g.a.vs) + vo);
         }
       }
     }
-    return there;
   }
 
   // Into LDS. edge: the unit holds keys outside the tile's, whose values become 0; clean:
   // values that are not finite do, too. Returns whether this lane had some.
-  __device__ __forceinline__ bool store(const TileArgs& g, const Place& p, int key0, int first, int stride, char* kl, char* vl,
-                                        bool edge, bool clean) {
+  __device__ __forceinline__ bool store(const Place& p, int key0, int first, int stride, char* kl, char* vl, bool edge, bool clean) {
     const int lane = threadIdx.x & 63;
     const int in = lane / S::kChunks, chunk = lane % S::kChunks;
     uint32_t found = 0;
@@ -657,10 +676,6 @@ __global__ void __launch_bounds__(64 * kFewWaves, DB * sizeof(T) <= 256 ? 2 : 1)
           found[w][2] = mine[i];
         }
       }
-      if (blockIdx.x == 0 && b < batch) {  // for the kernel that joins
-        if (b == 0) g.line[0] = 0;
-        g.line[b + 1] = before + mine[i];
-      }
       before += mine[i];
     }
     __syncthreads();
@@ -670,7 +685,10 @@ __global__ void __launch_bounds__(64 * kFewWaves, DB * sizeof(T) <= 256 ? 2 : 1)
     units = found[wave][2];
   }
   zero_other_rows<T>(g, worker, (int64_t)gridDim.x * kFewWaves);
-  if (total == 0 || worker >= n_workers) return;
+  if (total == 0 || worker >= n_workers) {
+    if (lane == 0) leave_job(g, worker, nullptr, 0, 0, 0);
+    return;
+  }
   u1 = begin_of(worker + 1, total, n_workers);
   p.b = ((int64_t)__builtin_amdgcn_readfirstlane((int)(p.b >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((int)p.b);
   place_in_sequence(g, p, u0, at, units);
@@ -678,22 +696,31 @@ __global__ void __launch_bounds__(64 * kFewWaves, DB * sizeof(T) <= 256 ? 2 : 1)
 
   char* kl = lds[wave];
   char* vl = lds[wave] + 32 * S::kPitch;
-  Loads<T, DB, N, LANE> x;
+  Loads<T, DB, N, 32, LANE> x;
+  typename Loads<T, DB, N, 32, LANE>::P pg;
   Rows<T, DB> r;
   for (int64_t u = u0; u < u1;) {
     const int64_t tile_end = p.begin + (p.k.u1 - p.k.u0);
     const int64_t stop = min(tile_end, u1);
     const bool whole = u == p.begin && stop == tile_end;
     const int tokens = min(g.per_tile, p.s.count - p.t * g.per_tile);
-    rows_begin<T, DB>(g, p, 0, r);
     int key0 = __builtin_amdgcn_readfirstlane((p.k.u0 + (int)(u - p.begin)) * 32);
-    uint32_t there = (uint32_t)x.issue(g, p, key0, 0, S::kPerLoad);
-    for (; u < stop; ++u, key0 += 32) {
+    const int key1 = __builtin_amdgcn_readfirstlane(key0 + 32 * (int)(stop - u));
+    pg.look_up(g, p, key0);
+    rows_begin<T, DB>(g, p, 0, r);
+    x.issue(g, p, pg, 0, S::kPerLoad);
+    uint32_t next = (uint32_t)pg.seen(g);
+    pg.look_up(g, p, key0 + 32);
+    for (; key0 < key1; key0 += 32) {
+      const uint32_t seen = next;
       const bool edge = key0 < p.k.lo || key0 + 32 > p.k.hi;
-      const bool mask = key0 < r.low || key0 + 32 > r.top || there != 0xFFFFFFFFu;
-      const bool bad = x.store(g, p, key0, 0, S::kPerLoad, kl, vl, edge, mask && tokens > 1);
-      const uint32_t seen = there;
-      if (u + 1 < stop) there = (uint32_t)x.issue(g, p, key0 + 32, 0, S::kPerLoad);
+      const bool mask = key0 < r.low || key0 + 32 > r.top || seen != 0xFFFFFFFFu;
+      const bool bad = x.store(p, key0, 0, S::kPerLoad, kl, vl, edge, mask && tokens > 1);
+      if (key0 + 32 < key1) {
+        x.issue(g, p, pg, 0, S::kPerLoad);
+        next = (uint32_t)pg.seen(g);
+        pg.look_up(g, p, key0 + 64);
+      }
       f32x16_t s[1];
       s[0] = scores32<T, DB>(g, r, kl, 0);
       if (mask) hide32<T, DB>(r, s[0], key0, seen);
@@ -702,10 +729,13 @@ __global__ void __launch_bounds__(64 * kFewWaves, DB * sizeof(T) <= 256 ? 2 : 1)
       values32<T, DB>(r, s[0], vl, 0);
       if (__any(bad)) add_not_finite<T, DB>(g, p, r, key0, seen);
     }
+    u = stop;
     float* part = nullptr;
-    if (!whole) part = g.part + (2 * worker + (p.begin != first_begin)) * g.rows * (DB + 2);
+    const int64_t slot = 2 * worker + (p.begin != first_begin);
+    if (!whole) part = g.part + slot * g.rows * (DB + 2);
     rows_end<T, DB>(g, p, 0, r, part);
     if (u < u1) next_place(g, p);
+    else if (lane == 0) leave_job(g, worker, p.begin >= u0 && !whole ? &p : nullptr, slot, total, n_workers);
   }
 }
 
@@ -719,15 +749,18 @@ __global__ void __launch_bounds__(64 * WAVES) attend_many_kernel(TileArgs g) {
   static_assert(N >= 1 && N * S::kPerLoad * WAVES == UNIT, "a unit is whole loads of every wave");
   constexpr int kV = UNIT * S::kPitch;
   __shared__ __attribute__((aligned(16))) char lds[2][UNIT * (S::kPitch + S::vPitch)];  // two units' K and V
-  __shared__ uint32_t bits[2][3][8];  // of each wave's rows: there (two words); values that are not finite
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  __shared__ uint32_t bad[2];  // the unit (by count) whose values are not all finite
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // neighbours in the line, which share keys, go to one XCD
   const int64_t nb = gridDim.x;
   const int64_t worker = nb % 8 == 0 ? (int64_t)(blockIdx.x % 8) * (nb / 8) + blockIdx.x / 8 : blockIdx.x;
   const int64_t total = g.line[g.a.seq.batch];
   const int64_t n_workers = active_workers(g, total);
   zero_other_rows<T>(g, worker * WAVES + wave, nb * WAVES);
-  if (total == 0 || worker >= n_workers) return;
+  if (total == 0 || worker >= n_workers) {
+    if (threadIdx.x == 0) leave_job(g, worker, nullptr, 0, 0, 0);
+    return;
+  }
   const int64_t u0 = begin_of(worker, total, n_workers), u1 = begin_of(worker + 1, total, n_workers);
   Place p;
   p.b = sequence_at(g.line, g.a.seq.batch, u0);
@@ -736,172 +769,167 @@ __global__ void __launch_bounds__(64 * WAVES) attend_many_kernel(TileArgs g) {
   const int64_t first_begin = p.begin;
   const int row0 = wave * kRows, first = wave * S::kPerLoad;
   constexpr int stride = WAVES * S::kPerLoad;
-  if (threadIdx.x < 48) (&bits[0][0][0])[threadIdx.x] = 0;
+  if (threadIdx.x < 2) bad[threadIdx.x] = 0;
   __syncthreads();
 
-  Loads<T, DB, N, LANE> x;
+  Loads<T, DB, N, UNIT, LANE> x;
+  typename Loads<T, DB, N, UNIT, LANE>::P pg;
   Rows<T, DB> r;
   int buf = 0;
+  uint32_t serial = 0;
   for (int64_t u = u0; u < u1;) {
     const int64_t tile_end = p.begin + (p.k.u1 - p.k.u0);
     const int64_t stop = min(tile_end, u1);
     const bool whole = u == p.begin && stop == tile_end;
     const int t0 = p.t * g.per_tile, tokens = min(g.per_tile, p.s.count - t0);
+    int key0 = __builtin_amdgcn_readfirstlane((p.k.u0 + (int)(u - p.begin)) * UNIT);
+    const int key1 = __builtin_amdgcn_readfirstlane(key0 + UNIT * (int)(stop - u));
+    pg.look_up(g, p, key0);
     rows_begin<T, DB>(g, p, row0, r);
     // the keys that some row of this wave sees (none without rows), and that every row of the tile does
     const int w0 = row0 / g.group, w1 = min((row0 + kRows - 1) / g.group, tokens - 1);
     const int end = w0 < tokens ? __builtin_amdgcn_readfirstlane(min(p.s.pos0 + t0 + w1 + 1, p.s.length)) : 0;
-    const int all_top = p.s.pos0 + t0 + 1;
+    const int all_top = __builtin_amdgcn_readfirstlane(p.s.pos0 + t0 + 1);
     int beg = 0, all_low = 0;
     if (g.a.window > 0) {
       beg = __builtin_amdgcn_readfirstlane((int)max((int64_t)p.s.pos0 + t0 + w0 + 1 - g.a.window, (int64_t)0));
-      all_low = (int)max((int64_t)p.s.pos0 + t0 + tokens - g.a.window, (int64_t)0);
+      all_low = __builtin_amdgcn_readfirstlane((int)max((int64_t)p.s.pos0 + t0 + tokens - g.a.window, (int64_t)0));
     }
-    int key0 = __builtin_amdgcn_readfirstlane((p.k.u0 + (int)(u - p.begin)) * UNIT);
-    auto put = [&](int key, uint64_t there, int to) {
+    auto put = [&](int key, int to) {
       const bool edge = key < p.k.lo || key + UNIT > p.k.hi;
       const bool clean = tokens > 1 && (key < all_low || key + UNIT > all_top);
-      const bool bad = __any(x.store(g, p, key, first, stride, lds[to], lds[to] + kV, edge, clean));
-      if (lane == 0) {
-        bits[to][0][wave] = (uint32_t)there;
-        if (UNIT > 32) bits[to][1][wave] = (uint32_t)(there >> 32);
-        bits[to][2][wave] = bad;
-      }
+      ++serial;
+      if (x.store(p, key, first, stride, lds[to], lds[to] + kV, edge, clean)) bad[to] = serial;
     };
-    uint64_t there = x.issue(g, p, key0, first, stride);
-    put(key0, there, buf);
+    x.issue(g, p, pg, first, stride);
+    uint64_t next = pg.seen(g);
+    pg.look_up(g, p, key0 + UNIT);
+    put(key0, buf);
     __syncthreads();
-    for (; u < stop; ++u, key0 += UNIT, buf ^= 1) {
-      const bool more = u + 1 < stop;
-      if (more) there = x.issue(g, p, key0 + UNIT, first, stride);
+    for (; key0 < key1; key0 += UNIT, buf ^= 1) {
+      const bool more = key0 + UNIT < key1;
+      const uint64_t seen = next;
+      const uint32_t now = serial;
+      if (more) {
+        x.issue(g, p, pg, first, stride);
+        next = pg.seen(g);
+        pg.look_up(g, p, key0 + 2 * UNIT);
+      }
       if (key0 < end && key0 + UNIT > beg) {
-        // the words of the waves, joined in groups of 8 lanes
-        uint32_t word = lane < 24 ? (&bits[buf][0][0])[lane] : 0u;
-        word |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)word, kDppXor1, 0xF, 0xF, false);
-        word |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)word, kDppXor2, 0xF, 0xF, false);
-        word |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)word, kDppHalfMirror, 0xF, 0xF, false);
-        const bool bad = __builtin_amdgcn_readlane(word, 16) != 0;
 #pragma unroll
         for (int n = 0; n < UNIT / 32; ++n) {
           const int key = key0 + 32 * n;
           if (n > 0 && key >= end) break;
-          const uint32_t seen = (uint32_t)__builtin_amdgcn_readlane(word, 8 * n);
+          const uint32_t bits = (uint32_t)(seen >> (32 * n));
           f32x16_t s[1];
           s[0] = scores32<T, DB>(g, r, lds[buf], 32 * n);
-          if (key < r.low || key + 32 > r.top || seen != 0xFFFFFFFFu) hide32<T, DB>(r, s[0], key, seen);
+          if (key < r.low || key + 32 > r.top || bits != 0xFFFFFFFFu) hide32<T, DB>(r, s[0], key, bits);
           new_maximum<T, DB, 1>(g, r, s);
           weights32<T, DB>(g, r, s[0]);
           values32<T, DB>(r, s[0], lds[buf] + kV, 32 * n);
-          if (bad) add_not_finite<T, DB>(g, p, r, key, seen);
+          if (__builtin_amdgcn_readfirstlane(bad[buf]) == now) add_not_finite<T, DB>(g, p, r, key, bits);
         }
       }
-      if (more) put(key0 + UNIT, there, buf ^ 1);
+      if (more) put(key0 + UNIT, buf ^ 1);
       __syncthreads();
     }
+    u = stop;
     float* part = nullptr;
-    if (!whole) part = g.part + (2 * worker + (p.begin != first_begin)) * g.rows * (DB + 2);
+    const int64_t slot = 2 * worker + (p.begin != first_begin);
+    if (!whole) part = g.part + slot * g.rows * (DB + 2);
     rows_end<T, DB>(g, p, row0, r, part);
     if (u < u1) next_place(g, p);
+    else if (threadIdx.x == 0) leave_job(g, worker, p.begin >= u0 && !whole ? &p : nullptr, slot, total, n_workers);
   }
 }
 
 // ---------------------------------------------------------------------------
-// Joining the parts: a workgroup for each border of two workers
+// Joining the parts: a job for each worker whose last tile goes on in the next one
 // ---------------------------------------------------------------------------
 template <typename T, int DB>
 __global__ void __launch_bounds__(256) attend_join_kernel(TileArgs g) {
   constexpr int kVals = DB / 64;
+  __shared__ float sums[4][DB];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t total = g.line[g.a.seq.batch], n = active_workers(g, total);
-  const int64_t w = (int64_t)blockIdx.x + 1;
-  if (total == 0 || w >= n) return;
-  const int64_t u = begin_of(w, total, n);
-  Place p;
-  p.b = sequence_at(g.line, g.a.seq.batch, u);
-  const int64_t at = g.line[p.b];
-  place_in_sequence(g, p, u, at, g.line[p.b + 1] - at);
-  if (p.begin == u) return;  // the border is a tile's, too
-  const int64_t w0 = worker_of(p.begin, total, n);
-  if (w0 != w - 1) return;   // the tile's first border joins it
-  const int64_t w1 = worker_of(p.begin + (p.k.u1 - p.k.u0) - 1, total, n);
-  const int t0 = p.t * g.per_tile, rows = min(g.per_tile, p.s.count - t0) * g.group;
+  const Job job = g.jobs[blockIdx.x];
+  const int rows = job.rows, parts = job.parts;
+  if (rows == 0) return;
   const int64_t one = (int64_t)g.rows * (DB + 2);
-  const int parts = (int)(w1 - w0 + 1);
-  const float* first = g.part + (2 * w0 + (begin_of(w0, total, n) < p.begin)) * one;
-  const float* rest = g.part + 2 * (w0 + 1) * one;  // part i > 0: two slots further each
+  const float* first = g.part + job.first * one;
+  const float* rest = g.part + 2 * ((int64_t)blockIdx.x + 1) * one;  // part i > 0: two slots further each
   auto part = [&](int i, int row) { return (i == 0 ? first : rest + (int64_t)(i - 1) * 2 * one) + (int64_t)row * (DB + 2); };
-  // R rows of the parts begin, begin + step, ..: their maxima, sums, products of the values
-  auto gather = [&](auto rows_tag, int row0, int begin, int step, float* inv, float (*acc)[kVals]) {
-    constexpr int R = decltype(rows_tag)::value, kUnroll = R > 1 ? 2 : 8;
-    float top[R], sum[R];
-#pragma unroll
-    for (int k = 0; k < R; ++k) {
-      const int row = min(row0 + k, rows - 1);
-      top[k] = kNegInf;
-      for (int i = lane; i < parts; i += 64) top[k] = fmaxf(top[k], part(i, row)[DB]);
-    }
-    auto factor = [&](float m, int k) { return top[k] == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(m - top[k]); };
-#pragma unroll
-    for (int k = 0; k < R; ++k) {
-      const int row = min(row0 + k, rows - 1);
-      top[k] = wave_max(top[k]);
-      sum[k] = 0.0f;
-      for (int i = lane; i < parts; i += 64) sum[k] += factor(part(i, row)[DB], k) * part(i, row)[DB + 1];
-#pragma unroll
-      for (int v = 0; v < kVals; ++v) acc[k][v] = 0.0f;
-    }
-#pragma unroll kUnroll
-    for (int i = begin; i < parts; i += step) {
-#pragma unroll
-      for (int k = 0; k < R; ++k) {
-        const float* x = part(i, min(row0 + k, rows - 1));
-        const float f = factor(x[DB], k);
-#pragma unroll
-        for (int v = 0; v < kVals; ++v) acc[k][v] = fmaf(f, x[64 * v + lane], acc[k][v]);
-      }
-    }
-#pragma unroll
-    for (int k = 0; k < R; ++k) {
-      sum[k] = wave_sum(sum[k]);
-      inv[k] = sum[k] == 0.0f ? 0.0f : 1.0f / sum[k];
-    }
-  };
   auto store = [&](int row, const float* acc, float inv) {
-    const int i = row / g.group;
-    T* out = static_cast<T*>(g.a.out) + (p.s.first + t0 + i) * g.a.o_st + (int64_t)(p.h * g.group + row - i * g.group) * g.a.o_sh;
+    const int i = (uint32_t)row / (uint32_t)g.group;
+    T* out = static_cast<T*>(g.a.out) + (job.token + i) * g.a.o_st + (int64_t)(job.head + row - i * g.group) * g.a.o_sh;
 #pragma unroll
     for (int v = 0; v < kVals; ++v)
       if (64 * v + lane < g.a.dim) out[64 * v + lane] = from_f32<T>(acc[v] * inv);
   };
-  if (g.rows > kRows) {
-    // many rows in few parts: 8 rows a wave at a time, their loads together
-    constexpr int R = 8;
-    for (int row = (blockIdx.y * 4 + wave) * R; row < rows; row += 4 * R * gridDim.y) {
-      float inv[R], acc[R][kVals];
-      gather(std::integral_constant<int, R>(), row, 0, 1, inv, acc);
+  typedef float f32x2_a __attribute__((ext_vector_type(2), aligned(8)));
+  const auto factor = [](float m, float top) { return top == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(m - top); };
+  if (parts <= 8) {
+    // R rows a wave, their loads together; a row's maxima and sums in every lane
+    constexpr int R = 4;
+    for (int row0 = (blockIdx.y * 4 + wave) * R; row0 < rows; row0 += 4 * R * gridDim.y) {
+      float top[R], sum[R], acc[R][kVals];
+#pragma unroll
+      for (int k = 0; k < R; ++k) {
+        top[k] = kNegInf;
+        sum[k] = 0.0f;
+#pragma unroll
+        for (int v = 0; v < kVals; ++v) acc[k][v] = 0.0f;
+      }
+      for (int i = 0; i < parts; ++i) {
+        f32x2_a ml[R];
+        float x[R][kVals];
+#pragma unroll
+        for (int k = 0; k < R; ++k) {
+          const float* src = part(i, min(row0 + k, rows - 1));
+          ml[k] = *reinterpret_cast<const f32x2_a*>(src + DB);
+#pragma unroll
+          for (int v = 0; v < kVals; ++v) x[k][v] = src[64 * v + lane];
+        }
+#pragma unroll
+        for (int k = 0; k < R; ++k) {
+          const float now = fmaxf(top[k], ml[k][0]), keep = factor(top[k], now), f = factor(ml[k][0], now);
+          top[k] = now;
+          sum[k] = sum[k] * keep + ml[k][1] * f;
+#pragma unroll
+          for (int v = 0; v < kVals; ++v) acc[k][v] = acc[k][v] * keep + x[k][v] * f;
+        }
+      }
 #pragma unroll
       for (int k = 0; k < R; ++k)
-        if (row + k < rows) store(row + k, acc[k], inv[k]);
+        if (row0 + k < rows) store(row0 + k, acc[k], sum[k] == 0.0f ? 0.0f : 1.0f / sum[k]);
     }
-  } else {
-    // few rows in many parts: a row at a time, the parts over the waves
-    __shared__ float sums[4][DB];
-    for (int row = blockIdx.y; row < rows; row += gridDim.y) {
-      float inv[1], acc[1][kVals];
-      gather(std::integral_constant<int, 1>(), row, wave, 4, inv, acc);
+    return;
+  }
+  // many parts: a row at a time, its parts over the waves
+  for (int row = blockIdx.y; row < rows; row += gridDim.y) {
+    float top = kNegInf, sum = 0.0f, acc[kVals] = {};
+    for (int i = lane; i < parts; i += 64) top = fmaxf(top, part(i, row)[DB]);
+    top = wave_max(top);
+    for (int i = lane; i < parts; i += 64) sum += factor(part(i, row)[DB], top) * part(i, row)[DB + 1];
+    sum = wave_sum(sum);
+#pragma unroll 8
+    for (int i = wave; i < parts; i += 4) {
+      const float* x = part(i, row);
+      const float f = factor(x[DB], top);
 #pragma unroll
-      for (int v = 0; v < kVals; ++v) sums[wave][64 * v + lane] = acc[0][v];
-      __syncthreads();
-      if (wave == 0) {
+      for (int v = 0; v < kVals; ++v) acc[v] = fmaf(f, x[64 * v + lane], acc[v]);
+    }
 #pragma unroll
-        for (int v = 0; v < kVals; ++v) {
-          const int d = 64 * v + lane;
-          acc[0][v] = (sums[0][d] + sums[1][d]) + (sums[2][d] + sums[3][d]);
-        }
-        store(row, acc[0], inv[0]);
+    for (int v = 0; v < kVals; ++v) sums[wave][64 * v + lane] = acc[v];
+    __syncthreads();
+    if (wave == 0) {
+#pragma unroll
+      for (int v = 0; v < kVals; ++v) {
+        const int d = 64 * v + lane;
+        acc[v] = (sums[0][d] + sums[1][d]) + (sums[2][d] + sums[3][d]);
       }
-      __syncthreads();
+      store(row, acc, sum == 0.0f ? 0.0f : 1.0f / sum);
     }
+    __syncthreads();
   }
 }
 
@@ -909,10 +937,10 @@ __global__ void __launch_bounds__(256) attend_join_kernel(TileArgs g) {
 // Host side
 // ---------------------------------------------------------------------------
 struct Plan {
-  bool few, lined;
+  bool few, lined, cut;
   int padded, waves, unit, per_tile, rows, min_units;
   int64_t workers;
-  size_t line_bytes, part_bytes;
+  size_t line_bytes, job_bytes, part_bytes;
 };
 
 Plan plan_of(int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t dim, int64_t max_keys, int64_t max_chunk,
@@ -938,7 +966,9 @@ Plan plan_of(int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads, i
   const int64_t useful = most > 1e9 ? (int64_t)1 << 30 : (int64_t)most / p.min_units + 1;
   p.workers = std::min(groups * (p.few ? kFewWaves : 1), useful);
   if (p.few) p.workers = (p.workers + kFewWaves - 1) / kFewWaves * kFewWaves;
+  p.cut = p.workers > 8 * kv_heads * (tokens / p.per_tile);
   p.line_bytes = (size_t)(batch + 2) / 2 * 16;
+  p.job_bytes = (size_t)p.workers * sizeof(Job);
   p.part_bytes = (size_t)p.workers * 2 * (size_t)p.rows * (size_t)(p.padded + 2) * sizeof(float);
   return p;
 }
@@ -954,7 +984,8 @@ void launch_tiles(const TileArgs& g, const Plan& p, hipStream_t s) {
     attend_many_kernel<T, DB, kWaves, kUnit, LANE><<<dim3((unsigned)p.workers), dim3(64 * kWaves), 0, s>>>(g);
   }
   if (p.workers > 1) {
-    const unsigned slices = (unsigned)(p.rows > kRows ? (p.rows + 31) / 32 : std::min(p.rows, 4));
+    // (of few rows in many parts a row a workgroup, of many rows 16)
+    const unsigned slices = (unsigned)(p.rows > kRows ? (p.rows + 15) / 16 : p.cut ? std::min(p.rows, 4) : 1);
     attend_join_kernel<T, DB><<<dim3((unsigned)(p.workers - 1), slices), dim3(256), 0, s>>>(g);
   }
 }
@@ -985,7 +1016,7 @@ bool attend_tiles_take(const AttendArgs& a, int dtype) {
 size_t attend_tiles_workspace_bytes(int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t dim,
                                     int64_t max_keys, int64_t max_chunk, int dtype) {
   const Plan p = plan_of(tokens, batch, q_heads, kv_heads, dim, max_keys, max_chunk, dtype);
-  return p.line_bytes + p.part_bytes;
+  return p.line_bytes + p.job_bytes + p.part_bytes;
 }
 
 void attend_tiles(const AttendArgs& a, int64_t max_chunk, int dtype, void* workspace, hipStream_t s) {
@@ -1000,7 +1031,8 @@ void attend_tiles(const AttendArgs& a, int64_t max_chunk, int dtype, void* works
   g.workers = (int)p.workers;
   g.min_units = p.min_units;
   g.line = static_cast<int64_t*>(workspace);
-  g.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + p.line_bytes);
+  g.jobs = reinterpret_cast<Job*>(static_cast<char*>(workspace) + p.line_bytes);
+  g.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + p.line_bytes + p.job_bytes);
   if (a.softcap > 0.0f) {
     g.cap_in = a.scale / a.softcap;
     g.cap_out = a.softcap * kLog2e;
