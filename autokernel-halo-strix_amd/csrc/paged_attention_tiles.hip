@@ -25,13 +25,13 @@ constexpr int kRows = 32;          // rows of a wave
 constexpr int kPlanBatch = 1024;   // sequences that a workgroup lines up by itself
 
 typedef float f32x4_v __attribute__((ext_vector_type(4)));
-typedef const int32_t __attribute__((address_space(4)))* ConstI32;
 
 // What the joining kernel does for a worker: the rows of its last tile, whose first part
 // is the worker's own.
 struct Job {
-  int64_t token, first;  // the tile's first token of the call; its part's slot
-  int head, rows, parts, pad;  // its first query head; rows 0: nothing
+  int64_t first;         // the part's slot
+  int token, head;       // the tile's first token of the call, its first query head
+  int rows, parts;       // rows 0: nothing
 };
 
 struct TileArgs {
@@ -40,39 +40,63 @@ struct TileArgs {
   uint32_t page_magic;             // floor(2^32 / page_size), at most 2^32 - 1
   int unit, rows;                  // keys of a unit, rows of a tile
   int workers, min_units;
+  uint32_t kp, ks, vp, vs;         // cache strides in bytes: page, slot
   int64_t* line;                   // [batch + 1]: the units before each sequence
   Job* jobs;                       // [workers]
   float* part;                     // [2 workers][rows][DB + 2]: sums of products, maximum, sum
   float c, cap_in, cap_out;        // scores in base 2: s c, or cap_out tanh(s cap_in)
 };
 
-// Where a key lives.
-__device__ __forceinline__ void key_place(const TileArgs& g, uint32_t key, uint32_t& page, uint32_t& slot) {
-  const uint32_t d = (uint32_t)g.a.page_size;
-  page = __umulhi(key, g.page_magic);  // the quotient or one less
-  slot = key - page * d;
-  if (slot >= d) {
-    slot -= d;
-    ++page;
-  }
+// The kernels' argument where the launch left it. Held in registers all of it would crowd
+// out what the loops need (100 scalars went through vector registers there, a quarter of the
+// instructions): what a tile's ends need is read anew for each, through fresh().
+typedef const TileArgs __attribute__((address_space(4)))* Args;
+
+__device__ __forceinline__ Args kernel_args() { return (Args)__builtin_amdgcn_kernarg_segment_ptr(); }
+__device__ __forceinline__ Args fresh(Args g) {
+  asm volatile("" : "+s"(g));
+  return g;
 }
+
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// Where a key lives.
+struct PageMath {
+  uint32_t size, magic;
+  __device__ __forceinline__ void place(uint32_t key, uint32_t& page, uint32_t& slot) const {
+    page = __umulhi(key, magic);  // the quotient or one less
+    slot = key - page * size;
+    if (slot >= size) {
+      slot -= size;
+      ++page;
+    }
+  }
+};
+__device__ __forceinline__ PageMath page_math(Args g) { return {(uint32_t)g->a.page_size, g->page_magic}; }
 
 // A sequence's part in the line.
 struct Seq {
-  int64_t first;      // its first new token
-  int count, length;  // new tokens, positions that can have keys
-  int pos0;           // position of the first new token
+  int first, count;   // its new tokens
+  int length, pos0;   // positions that can have keys, position of the first new token
 };
 
-__device__ __forceinline__ Seq seq_at(const TileArgs& g, int64_t b) {
+__device__ __forceinline__ Seq seq_at(Args g, int b) {
   Seq s;
+  const int tokens = (int)g->a.seq.tokens;
   int64_t count;
-  sequence_tokens(g.a.seq, b, s.first, count);
-  const int length = g.a.seq.lengths[b];
+  if (g->a.seq.starts == nullptr) {
+    s.first = b * (int)g->a.seq.per;
+    count = g->a.seq.per;
+  } else {
+    const int a = g->a.seq.starts[b], e = g->a.seq.starts[b + 1];
+    s.first = min(max(a, 0), tokens);
+    count = max(min(e, tokens) - s.first, 0);
+  }
+  const int length = g->a.seq.lengths[b];
   s.count = (int)count;
   // (far below 0 all the same once it is: no key)
   s.pos0 = (int)max((int64_t)length - count, (int64_t)INT32_MIN / 2);
-  s.length = (int)min((int64_t)length, g.a.max_pages * g.a.page_size);
+  s.length = (int)min((int64_t)length, g->a.max_pages * g->a.page_size);
   return s;
 }
 
@@ -81,22 +105,22 @@ struct Span {
   int lo, hi, u0, u1;
 };
 
-__device__ __forceinline__ Span span_of(const TileArgs& g, const Seq& s, int t) {
-  const int t0 = t * g.per_tile, t1 = min(t0 + g.per_tile, s.count);
+__device__ __forceinline__ Span span_of(Args g, const Seq& s, int t) {
+  const int t0 = t * g->per_tile, t1 = min(t0 + g->per_tile, s.count);
   Span r;
   r.hi = max(min(s.pos0 + t1, s.length), 0);
   r.lo = 0;
-  if (g.a.window > 0) r.lo = (int)min(max((int64_t)s.pos0 + t0 + 1 - g.a.window, (int64_t)0), (int64_t)r.hi);
-  r.u0 = (uint32_t)r.lo / (uint32_t)g.unit;
-  r.u1 = max((int)(((uint32_t)r.hi + g.unit - 1) / (uint32_t)g.unit), r.u0 + 1);
+  if (g->a.window > 0) r.lo = (int)min(max((int64_t)s.pos0 + t0 + 1 - g->a.window, (int64_t)0), (int64_t)r.hi);
+  r.u0 = (uint32_t)r.lo / (uint32_t)g->unit;
+  r.u1 = max((int)(((uint32_t)r.hi + g->unit - 1) / (uint32_t)g->unit), r.u0 + 1);
   return r;
 }
 
-__device__ __forceinline__ int tiles_of(const TileArgs& g, const Seq& s) { return (s.count + g.per_tile - 1) / g.per_tile; }
+__device__ __forceinline__ int tiles_of(Args g, const Seq& s) { return (s.count + g->per_tile - 1) / g->per_tile; }
 
 // Workers that a line of `total` units keeps busy; worker w has [begin(w), begin(w + 1)).
-__device__ __forceinline__ int64_t active_workers(const TileArgs& g, int64_t total) {
-  return max(min((int64_t)g.workers, total / g.min_units), (int64_t)1);
+__device__ __forceinline__ int64_t active_workers(Args g, int64_t total) {
+  return max(min((int64_t)g->workers, total / g->min_units), (int64_t)1);
 }
 __device__ __forceinline__ int64_t begin_of(int64_t w, int64_t total, int64_t n) { return w * total / n; }
 __device__ __forceinline__ int64_t worker_of(int64_t u, int64_t total, int64_t n) { return ((u + 1) * n - 1) / total; }
@@ -107,24 +131,21 @@ __device__ __forceinline__ int64_t wave_sum64(int64_t v) {
   return v;
 }
 
-// The tile of a line's unit.
+// A tile of the line, and which of its units come first and end (a worker's share of it).
 struct Place {
-  int64_t b;
-  int h, t;        // key head, tile of the sequence
-  int64_t begin;   // the tile's first unit in the line
+  int b, h, t;     // sequence, key head, tile of the sequence
   Seq s;
   Span k;
 };
 
-// Which head and tile of sequence b unit u is in; the sequence's units begin at `at`.
-// All lanes of a wave together.
-__device__ __forceinline__ void place_in_sequence(const TileArgs& g, Place& p, int64_t u, int64_t at, int64_t units) {
+// The tile of a sequence's unit `rest` (counted from the sequence's first); `rest` becomes
+// the unit of the tile. All lanes of a wave together.
+__device__ __forceinline__ void place_in_sequence(Args g, Place& p, int64_t& rest, int64_t units) {
   const int lane = threadIdx.x & 63;
   p.s = seq_at(g, p.b);
-  const int64_t each = units / g.a.kv_heads;
-  int64_t rest = u - at;
-  p.h = (int)(rest / each);
-  rest -= (int64_t)p.h * each;
+  const int64_t each = units / g->a.kv_heads;
+  const int h = (int)(rest / each);
+  rest -= (int64_t)h * each;
   const int n = tiles_of(g, p.s);
   int t = 0;
   if (n > 1) {
@@ -151,29 +172,47 @@ __device__ __forceinline__ void place_in_sequence(const TileArgs& g, Place& p, i
       rest -= all;
     }
   }
-  p.t = __builtin_amdgcn_readfirstlane(t);
-  p.h = __builtin_amdgcn_readfirstlane(p.h);
-  p.begin = u - rest;
+  p.t = uniform(t);
+  p.h = uniform(h);
+  p.k = span_of(g, p.s, p.t);
+}
+
+// The tile after p.
+__device__ __forceinline__ void next_place(Args g, Place& p) {
+  if (++p.t == tiles_of(g, p.s)) {
+    p.t = 0;
+    if (++p.h == g->a.kv_heads) {
+      p.h = 0;
+      do {
+        ++p.b;
+        p.s = seq_at(g, p.b);
+      } while (p.s.count == 0 && p.b + 1 < (int)g->a.seq.batch);
+      p.s.first = uniform(p.s.first);
+      p.s.count = uniform(p.s.count);
+      p.s.length = uniform(p.s.length);
+      p.s.pos0 = uniform(p.s.pos0);
+    }
+  }
   p.k = span_of(g, p.s, p.t);
 }
 
 // The sequence of unit u from the line in memory: 64 entries at a time.
-__device__ __forceinline__ int64_t sequence_at(const int64_t* line, int64_t batch, int64_t u) {
+__device__ __forceinline__ int sequence_at(const int64_t* line, int batch, int64_t u) {
   const int lane = threadIdx.x & 63;
-  int64_t lo = 0, n = batch;
+  int lo = 0, n = batch;
   while (n > 1) {
-    const int64_t step = (n + 63) / 64;
-    const bool le = lane * step < n && line[lo + lane * step] <= u;
+    const int step = (n + 63) / 64;
+    const bool le = (int64_t)lane * step < n && line[lo + lane * step] <= u;
     const int last = 63 - __builtin_clzll(__ballot(le) | 1);
-    const int64_t next = lo + last * step;
+    const int next = lo + last * step;
     n = min(step, lo + n - next);
     lo = next;
   }
   // (sequences without units begin where the next one does: the last of them is ours)
-  return lo;
+  return uniform(lo);
 }
 
-__device__ __forceinline__ int64_t units_of(const TileArgs& g, const Seq& s, int first_tile, int step) {
+__device__ __forceinline__ int64_t units_of(Args g, const Seq& s, int first_tile, int step) {
   int64_t sum = 0;
   const int n = tiles_of(g, s);
   for (int t = first_tile; t < n; t += step) {
@@ -184,20 +223,22 @@ __device__ __forceinline__ int64_t units_of(const TileArgs& g, const Seq& s, int
 }
 
 // Lines up the units of all sequences: a wave each, then their sums.
-__global__ void __launch_bounds__(1024) attend_line_kernel(TileArgs g) {
+__global__ void __launch_bounds__(1024) attend_line_kernel(TileArgs) {
   __shared__ int64_t sums[16];
+  const Args g = kernel_args();
+  int64_t* const line = g->line;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t batch = g.a.seq.batch;
+  const int64_t batch = g->a.seq.batch;
   for (int64_t b = wave; b < batch; b += 16) {
-    const int64_t n = wave_sum64(units_of(g, seq_at(g, b), lane, 64));
-    if (lane == 0) g.line[b + 1] = n * g.a.kv_heads;
+    const int64_t n = wave_sum64(units_of(g, seq_at(g, (int)b), lane, 64));
+    if (lane == 0) line[b + 1] = n * g->a.kv_heads;
   }
-  if (threadIdx.x == 0) g.line[0] = 0;
+  if (threadIdx.x == 0) line[0] = 0;
   __syncthreads();
   int64_t before = 0;
   for (int64_t b0 = 0; b0 < batch; b0 += 1024) {
     const int64_t b = b0 + threadIdx.x;
-    int64_t upto = b < batch ? g.line[b + 1] : 0;
+    int64_t upto = b < batch ? line[b + 1] : 0;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
       const int64_t o = __shfl_up(upto, d);
@@ -210,7 +251,7 @@ __global__ void __launch_bounds__(1024) attend_line_kernel(TileArgs g) {
       if (w < wave) add += sums[w];
       before += sums[w];
     }
-    if (b < batch) g.line[b + 1] = upto + add;
+    if (b < batch) line[b + 1] = upto + add;
     __syncthreads();
   }
 }
@@ -282,33 +323,48 @@ struct Rows {
   float m, l;     // the running maximum (base 2; the lane's query) and this half's sum
   int lo, hi;     // the keys that the query sees
   int top, low;   // of the wave's rows: the least hi, the largest lo
-  bool live;
+  int beg, end;   // of the wave's rows: the keys that some of them see
 };
+
+// Scores in base 2.
+struct ScoreMath {
+  float c, cap_in, cap_out;
+  bool cap;
+};
+__device__ __forceinline__ ScoreMath score_math(Args g) { return {g->c, g->cap_in, g->cap_out, g->cap_out > 0.0f}; }
 
 // Loads the queries of rows [row0, row0 + 32) of a tile and starts their sums.
 template <typename T, int DB>
-__device__ __forceinline__ void rows_begin(const TileArgs& g, const Place& p, int row0, Rows<T, DB>& r) {
+__device__ __forceinline__ void rows_begin(Args g0, const Place& p, int row0, Rows<T, DB>& r) {
   using S = Shape<T, DB>;
+  const Args g = fresh(g0);
   const int lane = threadIdx.x & 63, half = lane >> 5;
-  const int t0 = p.t * g.per_tile, tokens = min(g.per_tile, p.s.count - t0);
+  const int t0 = p.t * g->per_tile, tokens = min(g->per_tile, p.s.count - t0), group = g->group, dim = g->a.dim;
   const int row = row0 + (lane & 31);
-  const int i = (uint32_t)row / (uint32_t)g.group;  // token of the tile
-  r.live = i < tokens && row < g.rows;
+  const int i = (uint32_t)row / (uint32_t)group;  // token of the tile
+  const bool live = i < tokens;
   const int tok = min(i, tokens - 1);
   const int pos = p.s.pos0 + t0 + tok;
-  r.hi = r.live ? max(min(pos + 1, p.s.length), 0) : 0;
-  r.lo = g.a.window > 0 ? (int)max((int64_t)pos + 1 - g.a.window, (int64_t)0) : 0;
+  const int64_t window = g->a.window;
+  r.hi = live ? max(min(pos + 1, p.s.length), 0) : 0;
+  r.lo = window > 0 ? (int)max((int64_t)pos + 1 - window, (int64_t)0) : 0;
   // (rows past the tile's see what its last token does: nothing of theirs is kept, and they mask nothing)
-  const int last = min((int)((uint32_t)(row0 + 31) / (uint32_t)g.group), tokens - 1), fst = min((int)((uint32_t)row0 / (uint32_t)g.group), tokens - 1);
-  r.top = __builtin_amdgcn_readfirstlane(max(min(p.s.pos0 + t0 + fst + 1, p.s.length), 0));
-  r.low = g.a.window > 0 ? __builtin_amdgcn_readfirstlane((int)max((int64_t)p.s.pos0 + t0 + last + 1 - g.a.window, (int64_t)0)) : 0;
-  const T* q = static_cast<const T*>(g.a.q) + (p.s.first + t0 + tok) * g.a.q_st +
-               (int64_t)(p.h * g.group + (row - i * g.group)) * g.a.q_sh;
+  const int i0 = (uint32_t)row0 / (uint32_t)group, i1 = min((int)((uint32_t)(row0 + 31) / (uint32_t)group), tokens - 1);
+  const int pos_0 = p.s.pos0 + t0 + min(i0, tokens - 1), pos_1 = p.s.pos0 + t0 + i1;
+  r.top = uniform(max(min(pos_0 + 1, p.s.length), 0));
+  r.end = i0 < tokens ? uniform(min(pos_1 + 1, p.s.length)) : 0;
+  r.low = r.beg = 0;
+  if (window > 0) {
+    r.low = uniform((int)max((int64_t)pos_1 + 1 - window, (int64_t)0));
+    r.beg = uniform((int)max((int64_t)pos_0 + 1 - window, (int64_t)0));
+  }
+  const T* q = static_cast<const T*>(g->a.q) + (int64_t)(p.s.first + t0 + tok) * g->a.q_st +
+               (int64_t)(p.h * group + (row - i * group)) * g->a.q_sh;
 #pragma unroll
   for (int k = 0; k < S::kSteps; ++k) {
     r.q[k] = u32x4{0, 0, 0, 0};
     const int d = (2 * k + half) * S::VE;
-    if (r.live && d < g.a.dim) r.q[k] = *reinterpret_cast<const u32x4*>(q + d);
+    if (live && d < dim) r.q[k] = *reinterpret_cast<const u32x4*>(q + d);
   }
 #pragma unroll
   for (int b = 0; b < S::kBlocks; ++b) r.o[b] = f32x16_t{};
@@ -316,21 +372,21 @@ __device__ __forceinline__ void rows_begin(const TileArgs& g, const Place& p, in
   r.l = 0.0f;
 }
 
-// 32 keys from `key0` on, their K and V at kl and vl in LDS (rows row0 .. row0 + 31
-// there). edge: some row does not see all of them; seen: their bits that exist.
+// Scores of the 32 keys whose K is at row0 on in LDS.
 template <typename T, int DB>
-__device__ __forceinline__ f32x16_t scores32(const TileArgs& g, const Rows<T, DB>& r, const char* kl, int row0) {
+__device__ __forceinline__ f32x16_t scores32(const ScoreMath& sm, const Rows<T, DB>& r, const char* kl, int row0) {
   using S = Shape<T, DB>;
   const int lane = threadIdx.x & 63, half = lane >> 5, row = row0 + (lane & 31);
   const char* base = kl + row * S::kPitch + 16 * half;
   f32x16_t s{};
 #pragma unroll
   for (int k = 0; k < S::kSteps; ++k) s = mfma_step(T(), *reinterpret_cast<const u32x4*>(base + 32 * k), r.q[k], s);
-  if (g.cap_out > 0.0f) {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) s[i] = g.cap_out * tanh_f32(s[i] * g.cap_in);
-  }
   return s;
+}
+
+__device__ __forceinline__ void cap32(const ScoreMath& sm, f32x16_t& s) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) s[i] = sm.cap_out * tanh_f32(s[i] * sm.cap_in);
 }
 
 template <typename T, int DB>
@@ -343,17 +399,22 @@ __device__ __forceinline__ void hide32(const Rows<T, DB>& r, f32x16_t& s, int ke
   }
 }
 
-// The running maximum over N x 32 new scores, and everything so far brought to it.
+// The maximum that the weights are taken beside, over N x 32 new scores. It follows the
+// true one at a distance of up to 2^kLag: weights of up to 2^kLag are as exact as weights
+// of up to 1, and most units then leave what is summed up alone (raised at every new
+// maximum, [4, 4096 ..] prompts took 709 us, with the lag LAGUS).
+constexpr float kLag = 8.0f;
+
 template <typename T, int DB, int N>
-__device__ __forceinline__ void new_maximum(const TileArgs& g, Rows<T, DB>& r, const f32x16_t (&s)[N]) {
+__device__ __forceinline__ void new_maximum(const ScoreMath& sm, Rows<T, DB>& r, const f32x16_t (&s)[N]) {
   float top = s[0][0];
 #pragma unroll
   for (int n = 0; n < N; ++n)
 #pragma unroll
     for (int i = 0; i < 16; ++i) top = fmaxf(top, s[n][i]);
   top = other_half_max(top);
-  const float scaled = g.cap_out > 0.0f ? top : top * g.c;
-  if (__any(scaled > r.m)) {
+  const float scaled = top * sm.c;
+  if (__any(scaled > r.m + kLag)) {
     const float m = fmaxf(r.m, scaled);
     const float keep = r.m == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(r.m - m);
     r.m = m;
@@ -363,22 +424,37 @@ __device__ __forceinline__ void new_maximum(const TileArgs& g, Rows<T, DB>& r, c
   }
 }
 
-// The weights of 32 keys: s becomes p, the sum grows.
+// The weights of 32 keys as the operand of their product: 16 bit rounded once, two to a
+// register; fp32 as they are.
+template <typename T>
+struct Weights {
+  u32x4 w[sizeof(T) == 2 ? 2 : 4];
+};
+
 template <typename T, int DB>
-__device__ __forceinline__ void weights32(const TileArgs& g, Rows<T, DB>& r, f32x16_t& s) {
-  const float c = g.cap_out > 0.0f ? 1.0f : g.c;
+__device__ __forceinline__ Weights<T> weights32(const ScoreMath& sm, Rows<T, DB>& r, const f32x16_t& s) {
   // (nothing seen yet: every score is -inf or NaN, and the weight 0 or NaN)
   const float m = r.m == kNegInf ? 0.0f : r.m;
+  float p[16];
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
-    s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, -m));
-    r.l += s[i];
+    p[i] = __builtin_amdgcn_exp2f(fmaf(s[i], sm.c, -m));
+    r.l += p[i];
   }
+  Weights<T> w;
+  if constexpr (sizeof(T) == 2) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w.w[i / 4][i % 4] = pack2<T>(p[2 * i], p[2 * i + 1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) w.w[i / 4][i % 4] = __float_as_uint(p[i]);
+  }
+  return w;
 }
 
 // O^T += V^T P^T of 32 keys.
 template <typename T, int DB>
-__device__ __forceinline__ void values32(Rows<T, DB>& r, const f32x16_t& p, const char* vl, int row0) {
+__device__ __forceinline__ void values32(Rows<T, DB>& r, const Weights<T>& p, const char* vl, int row0) {
   using S = Shape<T, DB>;
   const int lane = threadIdx.x & 63, half = lane >> 5;
   if constexpr (sizeof(T) == 2) {
@@ -387,14 +463,11 @@ __device__ __forceinline__ void values32(Rows<T, DB>& r, const f32x16_t& p, cons
     const char* base = vl + (row0 + 4 * half + (j >> 2)) * S::vPitch + 32 * ((lane >> 4) & 1) + 8 * (j & 3);
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
-      u32x4 b;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) b[i] = pack2<T>(p[8 * kb + 2 * i], p[8 * kb + 2 * i + 1]);
 #pragma unroll
       for (int blk = 0; blk < S::kBlocks; ++blk) {
         const u32x2 x = lds_tr(base + 16 * kb * S::vPitch + 64 * blk);
         const u32x2 y = lds_tr(base + (16 * kb + 8) * S::vPitch + 64 * blk);
-        r.o[blk] = mfma32(T(), u32x4{x[0], x[1], y[0], y[1]}, b, r.o[blk]);
+        r.o[blk] = mfma32(T(), u32x4{x[0], x[1], y[0], y[1]}, p.w[kb], r.o[blk]);
       }
     }
   } else {
@@ -404,7 +477,7 @@ __device__ __forceinline__ void values32(Rows<T, DB>& r, const f32x16_t& p, cons
 #pragma unroll
       for (int blk = 0; blk < S::kBlocks; ++blk) {
         const float v = *reinterpret_cast<const float*>(base + (8 * (i / 4) + i % 4) * S::vPitch + 128 * blk);
-        r.o[blk] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, p[i], r.o[blk], 0, 0, 0);
+        r.o[blk] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, __uint_as_float(p.w[i / 4][i % 4]), r.o[blk], 0, 0, 0);
       }
     }
   }
@@ -413,23 +486,25 @@ __device__ __forceinline__ void values32(Rows<T, DB>& r, const f32x16_t& p, cons
 // What values that are not finite (left out of LDS where only some rows see them) do to
 // the rows that see their keys.
 template <typename T, int DB>
-__device__ __forceinline__ void add_not_finite(const TileArgs& g, const Place& p, Rows<T, DB>& r, int key0, uint32_t seen) {
-  const int half = (threadIdx.x & 63) >> 5;
-  const T* v0 = static_cast<const T*>(g.a.v) + (int64_t)p.h * g.a.vh;
+__device__ __forceinline__ void add_not_finite(Args g0, const Place& p, Rows<T, DB>& r, int key0, uint32_t seen) {
+  const Args g = fresh(g0);
+  const int half = (threadIdx.x & 63) >> 5, dim = g->a.dim;
+  const PageMath math = page_math(g);
+  const T* v0 = static_cast<const T*>(g->a.v) + (int64_t)p.h * g->a.vh;
   for (int j = 0; j < 32; ++j) {
     if (!((seen >> j) & 1)) continue;
     const int key = key0 + j;
     uint32_t i, slot;
-    key_place(g, (uint32_t)key, i, slot);
-    const int64_t page = g.a.pages[p.b * g.a.ld_pages + i];  // (there: its bit is set)
-    const T* v = v0 + page * g.a.vp + (int64_t)slot * g.a.vs;
+    math.place((uint32_t)key, i, slot);
+    const int64_t page = g->a.pages[(int64_t)p.b * g->a.ld_pages + i];  // (there: its bit is set)
+    const T* v = v0 + page * g->a.vp + (int64_t)slot * g->a.vs;
     const bool sees = key < r.hi && key >= r.lo;
 #pragma unroll
     for (int blk = 0; blk < Shape<T, DB>::kBlocks; ++blk)
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         const int d = 32 * blk + 8 * c + 4 * half;
-        if (d < g.a.dim) {
+        if (d < dim) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const float x = to_f32(v[d + e]);
@@ -441,15 +516,17 @@ __device__ __forceinline__ void add_not_finite(const TileArgs& g, const Place& p
   }
 }
 
-// A row's results: to the output where the worker had all its units, else to its part.
+// A row's results: to the output where the worker had all its units, else to a part's slot (-1: none).
 template <typename T, int DB>
-__device__ __forceinline__ void rows_end(const TileArgs& g, const Place& p, int row0, Rows<T, DB>& r, float* part) {
+__device__ __forceinline__ void rows_end(Args g0, const Place& p, int row0, Rows<T, DB>& r, int64_t slot) {
   using S = Shape<T, DB>;
+  const Args g = fresh(g0);
   const int lane = threadIdx.x & 63, half = lane >> 5, row = row0 + (lane & 31);
   const float l = both_halves(r.l);
-  if (!r.live) return;
-  if (part != nullptr) {
-    float* x = part + (int64_t)row * (DB + 2);
+  const int t0 = p.t * g->per_tile, tokens = min(g->per_tile, p.s.count - t0), group = g->group;
+  if (row >= tokens * group) return;
+  if (slot >= 0) {
+    float* x = g->part + (slot * g->rows + row) * (DB + 2);
 #pragma unroll
     for (int b = 0; b < S::kBlocks; ++b)
 #pragma unroll
@@ -464,46 +541,49 @@ __device__ __forceinline__ void rows_end(const TileArgs& g, const Place& p, int 
     return;
   }
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  const int i = (uint32_t)row / (uint32_t)g.group;
-  T* out = static_cast<T*>(g.a.out) + (p.s.first + p.t * g.per_tile + i) * g.a.o_st +
-           (int64_t)(p.h * g.group + (row - i * g.group)) * g.a.o_sh;
+  const int i = (uint32_t)row / (uint32_t)group, dim = g->a.dim;
+  T* out = static_cast<T*>(g->a.out) + (int64_t)(p.s.first + t0 + i) * g->a.o_st +
+           (int64_t)(p.h * group + (row - i * group)) * g->a.o_sh;
 #pragma unroll
   for (int b = 0; b < S::kBlocks; ++b)
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
       const int d = 32 * b + 8 * c + 4 * half;
-      if (d >= g.a.dim) continue;
+      if (d >= dim) continue;
       const float x0 = r.o[b][4 * c] * inv, x1 = r.o[b][4 * c + 1] * inv, x2 = r.o[b][4 * c + 2] * inv, x3 = r.o[b][4 * c + 3] * inv;
       if constexpr (sizeof(T) == 2) *reinterpret_cast<u32x2*>(out + d) = u32x2{pack2<T>(x0, x1), pack2<T>(x2, x3)};
       else *reinterpret_cast<f32x4_v*>(out + d) = f32x4_v{x0, x1, x2, x3};
     }
 }
 
-// The job that a worker leaves, given the part of its last tile that it has begun but not ended (or none).
-__device__ __forceinline__ void leave_job(const TileArgs& g, int64_t worker, const Place* p, int64_t slot, int64_t total, int64_t n) {
+// The job that a worker leaves, given its last tile where it has begun that but not ended it.
+__device__ __forceinline__ void leave_job(Args g0, int worker, const Place* p, int64_t slot, int parts) {
+  const Args g = fresh(g0);
   Job j{};
   if (p != nullptr) {
-    const int t0 = p->t * g.per_tile;
-    j.token = p->s.first + t0;
+    const int t0 = p->t * g->per_tile;
     j.first = slot;
-    j.head = p->h * g.group;
-    j.rows = min(g.per_tile, p->s.count - t0) * g.group;
-    j.parts = (int)(worker_of(p->begin + (p->k.u1 - p->k.u0) - 1, total, n) - worker) + 1;
+    j.token = p->s.first + t0;
+    j.head = p->h * g->group;
+    j.rows = min(g->per_tile, p->s.count - t0) * g->group;
+    j.parts = parts;
   }
-  g.jobs[worker] = j;
+  g->jobs[worker] = j;
 }
 
 // Zeros for the rows of no sequence, a token a wave at a time.
 template <typename T>
-__device__ __forceinline__ void zero_other_rows(const TileArgs& g, int64_t wave, int64_t waves) {
-  const Sequences& s = g.a.seq;
-  if (!g.a.zero_other || s.starts == nullptr || (s.starts[0] <= 0 && s.starts[s.batch] >= s.tokens)) return;
+__device__ __forceinline__ void zero_other_rows(Args g, int wave, int waves) {
+  if (!g->a.zero_other || g->a.seq.starts == nullptr ||
+      (g->a.seq.starts[0] <= 0 && g->a.seq.starts[g->a.seq.batch] >= g->a.seq.tokens))
+    return;
+  const Sequences s{g->a.seq.starts, g->a.seq.lengths, g->a.seq.batch, g->a.seq.tokens, g->a.seq.per};
   const int lane = threadIdx.x & 63;
   for (int64_t t = wave; t < s.tokens; t += waves) {
     if (sequence_of(s, t) >= 0) continue;
-    T* out = static_cast<T*>(g.a.out) + t * g.a.o_st;
-    for (int h = 0; h < g.a.q_heads; ++h)
-      for (int d = lane; d < g.a.dim; d += 64) out[h * g.a.o_sh + d] = from_f32<T>(0.0f);
+    T* out = static_cast<T*>(g->a.out) + t * g->a.o_st;
+    for (int h = 0; h < g->a.q_heads; ++h)
+      for (int d = lane; d < g->a.dim; d += 64) out[h * g->a.o_sh + d] = from_f32<T>(0.0f);
   }
 }
 
@@ -511,108 +591,116 @@ __device__ __forceinline__ void zero_other_rows(const TileArgs& g, int64_t wave,
 // before it is loaded.
 template <int UNIT, int GROUP>
 struct Pages {
-  int page, slot;  // page -1: no key of the tile
+  int page, slot;    // page -1: no key of the tile
+  int key, lo, hi;   // the unit's first key, the tile's
+  int h;
+  bool clean;        // only some of the tile's rows see some of the keys
 
   // GROUP rows are loaded together, seen by some row of the tile or not.
-  __device__ __forceinline__ void look_up(const TileArgs& g, const Place& p, int key0) {
-    const int key = key0 + (threadIdx.x & (UNIT - 1));
+  __device__ __forceinline__ void look_up(Args g, const PageMath& math, const Place& p, int key0) {
+    const int at_key = key0 + (threadIdx.x & (UNIT - 1));
     page = -1;
     slot = 0;
-    if (key >= (p.k.lo & -GROUP) && key < p.k.hi) {
+    key = key0;
+    lo = p.k.lo;
+    hi = p.k.hi;
+    h = p.h;
+    if (at_key >= (p.k.lo & -GROUP) && at_key < p.k.hi) {
       uint32_t at, in;
-      key_place(g, (uint32_t)key, at, in);
+      math.place((uint32_t)at_key, at, in);
       slot = (int)in;
-      page = g.a.pages[p.b * g.a.ld_pages + at];
+      page = g->a.pages[(int64_t)p.b * g->a.ld_pages + at];
     }
+    const int t0 = p.t * g->per_tile, tokens = min(g->per_tile, p.s.count - t0);
+    clean = tokens > 1 && key0 + UNIT > p.s.pos0 + t0 + 1;
+    if (g->a.window > 0) clean = clean || (tokens > 1 && key0 < (int64_t)p.s.pos0 + t0 + tokens - g->a.window);
   }
-  __device__ __forceinline__ bool there(const TileArgs& g, int pg) const { return pg >= 0 && pg < (int)g.a.n_pages; }
   // The keys that are there, by row.
-  __device__ __forceinline__ uint64_t seen(const TileArgs& g) const {
-    const uint64_t all = __ballot(there(g, page));
+  __device__ __forceinline__ uint64_t seen(uint32_t n_pages) const {
+    const uint64_t all = __ballot((uint32_t)page < n_pages);
     return UNIT == 64 ? all : all & 0xFFFFFFFFu;
   }
 };
 
+// Where the cache is: bases of this lane's chunk, strides in bytes.
+struct Cache {
+  const char *k, *v;
+  int64_t kh, vh;          // head strides in bytes
+  uint32_t kp, ks, vp, vs, n_pages;
+  bool on;                 // the lane's chunk is one of a row
+};
+
+template <typename T, int DB>
+__device__ __forceinline__ Cache cache_of(Args g) {
+  using S = Shape<T, DB>;
+  const int d = (threadIdx.x & 63) % S::kChunks * 16;
+  return {static_cast<const char*>(g->a.k) + d, static_cast<const char*>(g->a.v) + d, g->a.kh * (int64_t)sizeof(T),
+          g->a.vh * (int64_t)sizeof(T), g->kp, g->ks, g->vp, g->vs, (uint32_t)g->a.n_pages, d < g->a.dim * (int)sizeof(T)};
+}
+
 // The K and V rows of a unit, as N loads of a wave each: load i takes rows first + i *
 // stride .. + kPerLoad - 1. LANE: pages that are no multiple of a load's rows, so that a
-// load's rows are on pages of their own; else its address is scalar work.
+// load's rows are on pages of their own; else the page and slot are scalars. Keys that no
+// row of the tile sees are zeros.
 template <typename T, int DB, int N, int UNIT, bool LANE>
 struct Loads {
   using S = Shape<T, DB>;
   using P = Pages<UNIT, LANE ? 1 : S::kPerLoad>;
   u32x4 k[N], v[N];
+  bool clean;
 
-  __device__ __forceinline__ void issue(const TileArgs& g, const Place& p, const P& pg, int first, int stride) {
-    const int lane = threadIdx.x & 63;
-    const int in = lane / S::kChunks, d = (lane % S::kChunks) * S::VE;
-    const T* k0 = static_cast<const T*>(g.a.k) + (int64_t)p.h * g.a.kh;
-    const T* v0 = static_cast<const T*>(g.a.v) + (int64_t)p.h * g.a.vh;
-    if constexpr (LANE) {
+  __device__ __forceinline__ void issue(const Cache& c, const P& pg, int first, int stride) {
+    const int in = (threadIdx.x & 63) / S::kChunks;
+    const char* kb = c.k + pg.h * c.kh;
+    const char* vb = c.v + pg.h * c.vh;
+    clean = pg.clean;
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const int page = __shfl(pg.page, first + i * stride + in), slot = __shfl(pg.slot, first + i * stride + in);
-        k[i] = v[i] = u32x4{0, 0, 0, 0};
-        if (pg.there(g, page) && d < g.a.dim) {
-          k[i] = *reinterpret_cast<const u32x4*>(k0 + (int64_t)page * g.a.kp + (int64_t)slot * g.a.ks + d);
-          v[i] = *reinterpret_cast<const u32x4*>(v0 + (int64_t)page * g.a.vp + (int64_t)slot * g.a.vs + d);
+    for (int i = 0; i < N; ++i) {
+      k[i] = v[i] = u32x4{0, 0, 0, 0};
+      const int row = first + i * stride;
+      if constexpr (LANE) {
+        const uint32_t page = __shfl(pg.page, row + in), slot = __shfl(pg.slot, row + in);
+        if (page < c.n_pages && c.on) {
+          k[i] = *reinterpret_cast<const u32x4*>(kb + (uint64_t)page * c.kp + (uint64_t)slot * c.ks);
+          v[i] = *reinterpret_cast<const u32x4*>(vb + (uint64_t)page * c.vp + (uint64_t)slot * c.vs);
         }
-      }
-    } else {
-      const int64_t ko = (int64_t)in * g.a.ks + d, vo = (int64_t)in * g.a.vs + d;
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        // (rows of the load past the tile's keys are memory of the same page, hidden below)
-        const int page = __builtin_amdgcn_readlane(pg.page, first + i * stride);
-        const int slot = __builtin_amdgcn_readlane(pg.slot, first + i * stride);
-        k[i] = v[i] = u32x4{0, 0, 0, 0};
-        if (pg.there(g, page) && d < g.a.dim) {
-          k[i] = *reinterpret_cast<const u32x4*>(k0 + ((int64_t)page * g.a.kp + (int64_t)slot * g.a.ks) + ko);
-          v[i] = *reinterpret_cast<const u32x4*>(v0 + ((int64_t)page * g.a.vp + (int64_t)slot * g.a.vs) + vo);
+      } else {
+        // (a row of the load past the tile's keys may be first: its page is the others')
+        const uint32_t page = __builtin_amdgcn_readlane(pg.page, row), slot = __builtin_amdgcn_readlane(pg.slot, row) + in;
+        if (page < c.n_pages && c.on && pg.key + row + in >= pg.lo && pg.key + row + in < pg.hi) {
+          k[i] = *reinterpret_cast<const u32x4*>(kb + (uint64_t)page * c.kp + (uint64_t)slot * c.ks);
+          v[i] = *reinterpret_cast<const u32x4*>(vb + (uint64_t)page * c.vp + (uint64_t)slot * c.vs);
         }
       }
     }
   }
 
-  // Into LDS. edge: the unit holds keys outside the tile's, whose values become 0; clean:
-  // values that are not finite do, too. Returns whether this lane had some.
-  __device__ __forceinline__ bool store(const Place& p, int key0, int first, int stride, char* kl, char* vl, bool edge, bool clean) {
+  // Into LDS; where the unit is to be clean, with 0 for values that are not finite. Returns
+  // whether this lane had some.
+  __device__ __forceinline__ bool store(int first, int stride, char* kl, char* vl) {
     const int lane = threadIdx.x & 63;
-    const int in = lane / S::kChunks, chunk = lane % S::kChunks;
+    const int row = first + lane / S::kChunks, chunk = lane % S::kChunks;
+    char* kd = kl + row * S::kPitch + 16 * chunk;
+    char* vd = vl + row * S::vPitch + 16 * chunk;
     uint32_t found = 0;
+    if (clean) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int row = first + i * stride + in;
-      if (edge && (key0 + row < p.k.lo || key0 + row >= p.k.hi)) v[i] = u32x4{0, 0, 0, 0};
-      if (clean) {
+      for (int i = 0; i < N; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const uint32_t bad = not_finite<T>(v[i][e]);
           found |= bad;
           v[i][e] = finite_only<T>(v[i][e], bad);
         }
-      }
-      *reinterpret_cast<u32x4*>(kl + row * S::kPitch + 16 * chunk) = k[i];
-      *reinterpret_cast<u32x4*>(vl + row * S::vPitch + 16 * chunk) = v[i];
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      *reinterpret_cast<u32x4*>(kd + i * stride * S::kPitch) = k[i];
+      *reinterpret_cast<u32x4*>(vd + i * stride * S::vPitch) = v[i];
     }
     return found != 0;
   }
 };
-
-// The next tile of the line after p.
-__device__ __forceinline__ void next_place(const TileArgs& g, Place& p) {
-  p.begin += p.k.u1 - p.k.u0;
-  if (++p.t == tiles_of(g, p.s)) {
-    p.t = 0;
-    if (++p.h == g.a.kv_heads) {
-      p.h = 0;
-      do {
-        ++p.b;
-        p.s = seq_at(g, p.b);
-      } while (p.s.count == 0 && p.b + 1 < g.a.seq.batch);
-    }
-  }
-  p.k = span_of(g, p.s, p.t);
-}
 
 // ---------------------------------------------------------------------------
 // Few rows: a wave is a worker
@@ -620,33 +708,35 @@ __device__ __forceinline__ void next_place(const TileArgs& g, Place& p) {
 constexpr int kFewWaves = 4;
 
 template <typename T, int DB, bool LANE>
-__global__ void __launch_bounds__(64 * kFewWaves, DB * sizeof(T) <= 256 ? 2 : 1) attend_few_kernel(TileArgs g, bool lined) {
+__global__ void __launch_bounds__(64 * kFewWaves, DB * sizeof(T) <= 256 ? 2 : 1) attend_few_kernel(TileArgs, bool lined) {
   using S = Shape<T, DB>;
   constexpr int N = 32 / S::kPerLoad;
   __shared__ __attribute__((aligned(16))) char lds[kFewWaves][32 * (S::kPitch + S::vPitch)];
   __shared__ int64_t sums[kFewWaves];
   __shared__ int64_t found[kFewWaves][3];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t worker = (int64_t)blockIdx.x * kFewWaves + wave;
-  const int64_t batch = g.a.seq.batch;
+  const Args g = kernel_args();
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  const int worker = blockIdx.x * kFewWaves + wave;
+  const int batch = (int)g->a.seq.batch;
   int64_t total, n_workers, u0, u1, at = 0, units = 0;
   Place p;
   if (lined) {
-    total = g.line[batch];
+    total = g->line[batch];
     n_workers = active_workers(g, total);
     u0 = begin_of(worker, total, n_workers);
     if (total > 0 && worker < n_workers) {
-      p.b = sequence_at(g.line, batch, u0);
-      at = g.line[p.b];
-      units = g.line[p.b + 1] - at;
+      p.b = sequence_at(g->line, batch, u0);
+      at = g->line[p.b];
+      units = g->line[p.b + 1] - at;
     }
   } else {
     // every workgroup lines the sequences up: 4 a thread, at most
-    int64_t mine[kPlanBatch / (64 * kFewWaves)], sum = 0;
+    constexpr int kEach = kPlanBatch / (64 * kFewWaves);
+    int64_t mine[kEach], sum = 0;
 #pragma unroll
-    for (int i = 0; i < kPlanBatch / (64 * kFewWaves); ++i) {
-      const int64_t b = (int64_t)threadIdx.x * (kPlanBatch / (64 * kFewWaves)) + i;
-      mine[i] = b < batch ? units_of(g, seq_at(g, b), 0, 1) * g.a.kv_heads : 0;
+    for (int i = 0; i < kEach; ++i) {
+      const int b = (int)threadIdx.x * kEach + i;
+      mine[i] = b < batch ? units_of(g, seq_at(g, b), 0, 1) * g->a.kv_heads : 0;
       sum += mine[i];
     }
     int64_t upto = sum;
@@ -665,13 +755,15 @@ __global__ void __launch_bounds__(64 * kFewWaves, DB * sizeof(T) <= 256 ? 2 : 1)
       total += sums[w];
     }
     n_workers = active_workers(g, total);
+    int64_t begins[kFewWaves];
 #pragma unroll
-    for (int i = 0; i < kPlanBatch / (64 * kFewWaves); ++i) {
-      const int64_t b = (int64_t)threadIdx.x * (kPlanBatch / (64 * kFewWaves)) + i;
+    for (int w = 0; w < kFewWaves; ++w) begins[w] = begin_of((int64_t)blockIdx.x * kFewWaves + w, total, n_workers);
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+#pragma unroll
       for (int w = 0; w < kFewWaves; ++w) {
-        const int64_t x = begin_of((int64_t)blockIdx.x * kFewWaves + w, total, n_workers);
-        if (x >= before && x < before + mine[i]) {
-          found[w][0] = b;
+        if (begins[w] >= before && begins[w] < before + mine[i]) {
+          found[w][0] = (int)threadIdx.x * kEach + i;
           found[w][1] = before;
           found[w][2] = mine[i];
         }
@@ -680,166 +772,231 @@ __global__ void __launch_bounds__(64 * kFewWaves, DB * sizeof(T) <= 256 ? 2 : 1)
     }
     __syncthreads();
     u0 = begin_of(worker, total, n_workers);
-    p.b = found[wave][0];
+    p.b = uniform((int)found[wave][0]);
     at = found[wave][1];
     units = found[wave][2];
   }
-  zero_other_rows<T>(g, worker, (int64_t)gridDim.x * kFewWaves);
+  zero_other_rows<T>(g, worker, (int)gridDim.x * kFewWaves);
   if (total == 0 || worker >= n_workers) {
-    if (lane == 0) leave_job(g, worker, nullptr, 0, 0, 0);
+    if (lane == 0) leave_job(g, worker, nullptr, 0, 0);
     return;
   }
   u1 = begin_of(worker + 1, total, n_workers);
-  p.b = ((int64_t)__builtin_amdgcn_readfirstlane((int)(p.b >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((int)p.b);
-  place_in_sequence(g, p, u0, at, units);
-  const int64_t first_begin = p.begin;
+  int64_t in_tile = u0 - at;
+  place_in_sequence(g, p, in_tile, units);
 
-  char* kl = lds[wave];
-  char* vl = lds[wave] + 32 * S::kPitch;
+  char* const kl = lds[wave];
+  char* const vl = lds[wave] + 32 * S::kPitch;
+  const PageMath math = page_math(g);
+  const ScoreMath sm = score_math(g);
+  const Cache cache = cache_of<T, DB>(g);
   Loads<T, DB, N, 32, LANE> x;
   typename Loads<T, DB, N, 32, LANE>::P pg;
   Rows<T, DB> r;
-  for (int64_t u = u0; u < u1;) {
-    const int64_t tile_end = p.begin + (p.k.u1 - p.k.u0);
-    const int64_t stop = min(tile_end, u1);
-    const bool whole = u == p.begin && stop == tile_end;
-    const int tokens = min(g.per_tile, p.s.count - p.t * g.per_tile);
-    int key0 = __builtin_amdgcn_readfirstlane((p.k.u0 + (int)(u - p.begin)) * 32);
-    const int key1 = __builtin_amdgcn_readfirstlane(key0 + 32 * (int)(stop - u));
-    pg.look_up(g, p, key0);
+  int unit = uniform((int)in_tile), left = uniform((int)min(u1 - u0, (int64_t)INT32_MAX));
+  for (int tile = 0;; ++tile) {
+    const int begin = unit, tile_units = p.k.u1 - p.k.u0, n = min(tile_units - unit, left);
+    int key0 = uniform((p.k.u0 + unit) * 32);
+    const int key1 = key0 + 32 * n;
+    pg.look_up(g, math, p, key0);
+    typename Loads<T, DB, N, 32, LANE>::P pg1;
+    pg1.look_up(g, math, p, key0 + 32);
     rows_begin<T, DB>(g, p, 0, r);
-    x.issue(g, p, pg, 0, S::kPerLoad);
-    uint32_t next = (uint32_t)pg.seen(g);
-    pg.look_up(g, p, key0 + 32);
+    x.issue(cache, pg, 0, S::kPerLoad);
+    uint32_t next = (uint32_t)pg.seen(cache.n_pages);
+    pg = pg1;
     for (; key0 < key1; key0 += 32) {
       const uint32_t seen = next;
-      const bool edge = key0 < p.k.lo || key0 + 32 > p.k.hi;
-      const bool mask = key0 < r.low || key0 + 32 > r.top || seen != 0xFFFFFFFFu;
-      const bool bad = x.store(p, key0, 0, S::kPerLoad, kl, vl, edge, mask && tokens > 1);
+      const bool bad = x.store(0, S::kPerLoad, kl, vl);
       if (key0 + 32 < key1) {
-        x.issue(g, p, pg, 0, S::kPerLoad);
-        next = (uint32_t)pg.seen(g);
-        pg.look_up(g, p, key0 + 64);
+        x.issue(cache, pg, 0, S::kPerLoad);
+        next = (uint32_t)pg.seen(cache.n_pages);
+        pg.look_up(g, math, p, key0 + 64);
       }
       f32x16_t s[1];
-      s[0] = scores32<T, DB>(g, r, kl, 0);
-      if (mask) hide32<T, DB>(r, s[0], key0, seen);
-      new_maximum<T, DB, 1>(g, r, s);
-      weights32<T, DB>(g, r, s[0]);
-      values32<T, DB>(r, s[0], vl, 0);
+      s[0] = scores32<T, DB>(sm, r, kl, 0);
+      if (sm.cap) cap32(sm, s[0]);
+      if (key0 < r.low || key0 + 32 > r.top || seen != 0xFFFFFFFFu) hide32<T, DB>(r, s[0], key0, seen);
+      new_maximum<T, DB, 1>(sm, r, s);
+      values32<T, DB>(r, weights32<T, DB>(sm, r, s[0]), vl, 0);
       if (__any(bad)) add_not_finite<T, DB>(g, p, r, key0, seen);
     }
-    u = stop;
-    float* part = nullptr;
-    const int64_t slot = 2 * worker + (p.begin != first_begin);
-    if (!whole) part = g.part + slot * g.rows * (DB + 2);
-    rows_end<T, DB>(g, p, 0, r, part);
-    if (u < u1) next_place(g, p);
-    else if (lane == 0) leave_job(g, worker, p.begin >= u0 && !whole ? &p : nullptr, slot, total, n_workers);
+    left -= n;
+    unit += n;
+    const bool ended = unit == tile_units;
+    const int64_t slot = begin == 0 && ended ? -1 : 2 * (int64_t)worker + (tile > 0);
+    rows_end<T, DB>(g, p, 0, r, slot);
+    if (left == 0) {
+      if (lane == 0) {
+        const int parts = ended ? 0 : (int)(worker_of(u1 + (tile_units - unit) - 1, total, n_workers) - worker) + 1;
+        leave_job(g, worker, begin == 0 && !ended ? &p : nullptr, slot, parts);
+      }
+      return;
+    }
+    unit = 0;
+    next_place(g, p);
   }
 }
 
 // ---------------------------------------------------------------------------
 // Many rows: a workgroup is a worker, its waves share the units' keys and values
 // ---------------------------------------------------------------------------
+// A worker's units go through a ring of LDS slots one after the other, whatever tile they
+// are of: looked up four steps, loaded three and stored two before their scores are taken.
+// A wave's step has two phases: the matrix cores' (O^T += of the unit before, the scores of
+// this one; a tile's end and the next one's beginning between them) and the vector units'
+// (the weights of this unit; the stores and loads of those ahead). Half of the waves, one on
+// each SIMD, runs a phase late, so that on every SIMD one wave feeds the matrix cores while
+// the other computes weights.
 template <typename T, int DB, int WAVES, int UNIT, bool LANE>
-__global__ void __launch_bounds__(64 * WAVES) attend_many_kernel(TileArgs g) {
+__global__ void __launch_bounds__(64 * WAVES) attend_many_kernel(TileArgs) {
   using S = Shape<T, DB>;
   constexpr int N = UNIT / S::kPerLoad / WAVES;  // loads of a wave, UNIT rows over all waves
+  constexpr int NB = UNIT / 32;
   static_assert(N >= 1 && N * S::kPerLoad * WAVES == UNIT, "a unit is whole loads of every wave");
-  constexpr int kV = UNIT * S::kPitch;
-  __shared__ __attribute__((aligned(16))) char lds[2][UNIT * (S::kPitch + S::vPitch)];  // two units' K and V
-  __shared__ uint32_t bad[2];  // the unit (by count) whose values are not all finite
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // Units that are stored before they are used (one where the rows are too long for more);
+  // K is read in the step of its scores, V in the next one, by the late waves a phase later.
+  constexpr int kAhead = S::kRowBytes > 512 ? 1 : 2;
+  constexpr int kSlots = kAhead + (WAVES == 8), vSlots = kSlots + 1;
+  __shared__ __attribute__((aligned(16))) char kl[kSlots][UNIT * S::kPitch];
+  __shared__ __attribute__((aligned(16))) char vl[vSlots][UNIT * S::vPitch];
+  __shared__ int bad[vSlots];                    // the unit (by count) whose values are not all finite
+  const Args g = kernel_args();
+  const int wave = uniform(threadIdx.x >> 6);
+  const bool late = WAVES == 8 && wave >= 4;
   // neighbours in the line, which share keys, go to one XCD
-  const int64_t nb = gridDim.x;
-  const int64_t worker = nb % 8 == 0 ? (int64_t)(blockIdx.x % 8) * (nb / 8) + blockIdx.x / 8 : blockIdx.x;
-  const int64_t total = g.line[g.a.seq.batch];
+  const int nb = (int)gridDim.x;
+  const int worker = nb % 8 == 0 ? (int)(blockIdx.x % 8) * (nb / 8) + (int)blockIdx.x / 8 : (int)blockIdx.x;
+  const int64_t total = g->line[g->a.seq.batch];
   const int64_t n_workers = active_workers(g, total);
   zero_other_rows<T>(g, worker * WAVES + wave, nb * WAVES);
   if (total == 0 || worker >= n_workers) {
-    if (threadIdx.x == 0) leave_job(g, worker, nullptr, 0, 0, 0);
+    if (threadIdx.x == 0) leave_job(g, worker, nullptr, 0, 0);
     return;
   }
   const int64_t u0 = begin_of(worker, total, n_workers), u1 = begin_of(worker + 1, total, n_workers);
+  const int n = uniform((int)min(u1 - u0, (int64_t)INT32_MAX));
   Place p;
-  p.b = sequence_at(g.line, g.a.seq.batch, u0);
-  const int64_t at = g.line[p.b];
-  place_in_sequence(g, p, u0, at, g.line[p.b + 1] - at);
-  const int64_t first_begin = p.begin;
+  p.b = sequence_at(g->line, (int)g->a.seq.batch, u0);
+  int64_t in_tile = u0 - g->line[p.b];
+  place_in_sequence(g, p, in_tile, g->line[p.b + 1] - g->line[p.b]);
   const int row0 = wave * kRows, first = wave * S::kPerLoad;
   constexpr int stride = WAVES * S::kPerLoad;
-  if (threadIdx.x < 2) bad[threadIdx.x] = 0;
-  __syncthreads();
+  const PageMath math = page_math(g);
+  const ScoreMath sm = score_math(g);
+  const Cache cache = cache_of<T, DB>(g);
 
+  // the units' way into LDS: the tile and unit that are looked up next, how many are left
   Loads<T, DB, N, UNIT, LANE> x;
   typename Loads<T, DB, N, UNIT, LANE>::P pg;
-  Rows<T, DB> r;
-  int buf = 0;
-  uint32_t serial = 0;
-  for (int64_t u = u0; u < u1;) {
-    const int64_t tile_end = p.begin + (p.k.u1 - p.k.u0);
-    const int64_t stop = min(tile_end, u1);
-    const bool whole = u == p.begin && stop == tile_end;
-    const int t0 = p.t * g.per_tile, tokens = min(g.per_tile, p.s.count - t0);
-    int key0 = __builtin_amdgcn_readfirstlane((p.k.u0 + (int)(u - p.begin)) * UNIT);
-    const int key1 = __builtin_amdgcn_readfirstlane(key0 + UNIT * (int)(stop - u));
-    pg.look_up(g, p, key0);
-    rows_begin<T, DB>(g, p, row0, r);
-    // the keys that some row of this wave sees (none without rows), and that every row of the tile does
-    const int w0 = row0 / g.group, w1 = min((row0 + kRows - 1) / g.group, tokens - 1);
-    const int end = w0 < tokens ? __builtin_amdgcn_readfirstlane(min(p.s.pos0 + t0 + w1 + 1, p.s.length)) : 0;
-    const int all_top = __builtin_amdgcn_readfirstlane(p.s.pos0 + t0 + 1);
-    int beg = 0, all_low = 0;
-    if (g.a.window > 0) {
-      beg = __builtin_amdgcn_readfirstlane((int)max((int64_t)p.s.pos0 + t0 + w0 + 1 - g.a.window, (int64_t)0));
-      all_low = __builtin_amdgcn_readfirstlane((int)max((int64_t)p.s.pos0 + t0 + tokens - g.a.window, (int64_t)0));
+  Place lp = p;
+  int l_unit = uniform((int)in_tile), l_left = n;
+  auto look_up = [&](auto& to) {
+    if (l_left == 0) return;
+    to.look_up(g, math, lp, uniform((lp.k.u0 + l_unit) * UNIT));
+    --l_left;
+    if (++l_unit == lp.k.u1 - lp.k.u0 && l_left > 0) {
+      l_unit = 0;
+      next_place(fresh(g), lp);
     }
-    auto put = [&](int key, int to) {
-      const bool edge = key < p.k.lo || key + UNIT > p.k.hi;
-      const bool clean = tokens > 1 && (key < all_low || key + UNIT > all_top);
-      ++serial;
-      if (x.store(p, key, first, stride, lds[to], lds[to] + kV, edge, clean)) bad[to] = serial;
-    };
-    x.issue(g, p, pg, first, stride);
-    uint64_t next = pg.seen(g);
-    pg.look_up(g, p, key0 + UNIT);
-    put(key0, buf);
-    __syncthreads();
-    for (; key0 < key1; key0 += UNIT, buf ^= 1) {
-      const bool more = key0 + UNIT < key1;
-      const uint64_t seen = next;
-      const uint32_t now = serial;
-      if (more) {
-        x.issue(g, p, pg, first, stride);
-        next = pg.seen(g);
-        pg.look_up(g, p, key0 + 2 * UNIT);
-      }
-      if (key0 < end && key0 + UNIT > beg) {
+  };
+  int kput = 0, vput = 0, puts = 0;  // the slots that are stored next
+  auto put = [&]() {
+    ++puts;
+    if (x.store(first, stride, kl[kput], vl[vput])) bad[vput] = puts;
+    kput = kput + 1 == kSlots ? 0 : kput + 1;
+    vput = vput + 1 == vSlots ? 0 : vput + 1;
+  };
+  uint64_t seen[kAhead + 2];  // of the units j - 1, j, .. j + kAhead (their keys that are there)
 #pragma unroll
-        for (int n = 0; n < UNIT / 32; ++n) {
-          const int key = key0 + 32 * n;
-          if (n > 0 && key >= end) break;
-          const uint32_t bits = (uint32_t)(seen >> (32 * n));
-          f32x16_t s[1];
-          s[0] = scores32<T, DB>(g, r, lds[buf], 32 * n);
-          if (key < r.low || key + 32 > r.top || bits != 0xFFFFFFFFu) hide32<T, DB>(r, s[0], key, bits);
-          new_maximum<T, DB, 1>(g, r, s);
-          weights32<T, DB>(g, r, s[0]);
-          values32<T, DB>(r, s[0], lds[buf] + kV, 32 * n);
-          if (__builtin_amdgcn_readfirstlane(bad[buf]) == now) add_not_finite<T, DB>(g, p, r, key, bits);
-        }
+  for (int a = 0; a < kAhead + 2; ++a) seen[a] = 0;
+  if (threadIdx.x < vSlots) bad[threadIdx.x] = 0;
+  __syncthreads();
+  {
+    typename Loads<T, DB, N, UNIT, LANE>::P all[kAhead + 2];
+#pragma unroll
+    for (int a = 0; a < kAhead + 2; ++a) look_up(all[a]);
+#pragma unroll
+    for (int a = 0; a <= kAhead; ++a) {
+      if (a < n) {
+        x.issue(cache, all[a], first, stride);
+        seen[a + 1] = all[a].seen(cache.n_pages);
+        if (a < kAhead) put();
       }
-      if (more) put(key0 + UNIT, buf ^ 1);
-      __syncthreads();
     }
-    u = stop;
-    float* part = nullptr;
-    const int64_t slot = 2 * worker + (p.begin != first_begin);
-    if (!whole) part = g.part + slot * g.rows * (DB + 2);
-    rows_end<T, DB>(g, p, row0, r, part);
-    if (u < u1) next_place(g, p);
-    else if (threadIdx.x == 0) leave_job(g, worker, p.begin >= u0 && !whole ? &p : nullptr, slot, total, n_workers);
+    pg = all[kAhead + 1];
+  }
+  __syncthreads();
+  if (late) __syncthreads();
+
+  int kget = 0, vget = vSlots - 1;  // the slots of unit j's keys and of unit j - 1's values
+  bool before = false;              // this wave has weights of unit j - 1
+  int unit = uniform((int)in_tile), begin = unit, tiles = 0;  // of the tile: unit j, this worker's first
+  int key = uniform((p.k.u0 + unit) * UNIT);
+  Rows<T, DB> r;
+  rows_begin<T, DB>(g, p, row0, r);
+  f32x16_t s[NB];
+  Weights<T> w[NB];
+  for (int j = 0;; ++j) {
+    if (before) {
+#pragma unroll
+      for (int b = 0; b < NB; ++b) values32<T, DB>(r, w[b], vl[vget], 32 * b);
+      if (uniform(bad[vget]) == j) {
+        for (int b = 0; b < NB; ++b) add_not_finite<T, DB>(g, p, r, key - UNIT + 32 * b, (uint32_t)(seen[0] >> (32 * b)));
+      }
+    }
+    const bool ended = j > 0 && unit == p.k.u1 - p.k.u0;
+    if (ended || j == n) {
+      const int64_t slot = begin == 0 && ended ? -1 : 2 * (int64_t)worker + (tiles > 0);
+      rows_end<T, DB>(g, p, row0, r, slot);
+      if (j == n) {
+        if (threadIdx.x == 0) {
+          const int parts = ended ? 0 : (int)(worker_of(u1 + (p.k.u1 - p.k.u0 - unit) - 1, total, n_workers) - worker) + 1;
+          leave_job(g, worker, begin == 0 && !ended ? &p : nullptr, slot, parts);
+        }
+        break;
+      }
+      next_place(fresh(g), p);
+      unit = begin = 0;
+      ++tiles;
+      key = uniform(p.k.u0 * UNIT);
+      rows_begin<T, DB>(g, p, row0, r);
+    }
+    const bool now = key < r.end && key + UNIT > r.beg;
+    if (now) {
+#pragma unroll
+      for (int b = 0; b < NB; ++b) s[b] = scores32<T, DB>(sm, r, kl[kget], 32 * b);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int a = 0; a <= kAhead; ++a) seen[a] = seen[a + 1];
+    if (j + kAhead < n) {
+      put();
+      if (j + kAhead + 1 < n) {
+        x.issue(cache, pg, first, stride);
+        seen[kAhead + 1] = pg.seen(cache.n_pages);
+        look_up(pg);
+      }
+    }
+    if (now) {
+      if (sm.cap) {
+#pragma unroll
+        for (int b = 0; b < NB; ++b) cap32(sm, s[b]);
+      }
+      if (key < r.low || key + UNIT > r.top || seen[0] != (UNIT == 64 ? ~0ull : 0xFFFFFFFFull)) {
+#pragma unroll
+        for (int b = 0; b < NB; ++b) hide32<T, DB>(r, s[b], key + 32 * b, (uint32_t)(seen[0] >> (32 * b)));
+      }
+      new_maximum<T, DB, NB>(sm, r, s);
+#pragma unroll
+      for (int b = 0; b < NB; ++b) w[b] = weights32<T, DB>(sm, r, s[b]);
+    }
+    before = now;
+    ++unit;
+    key += UNIT;
+    kget = kget + 1 == kSlots ? 0 : kget + 1;
+    vget = vget + 1 == vSlots ? 0 : vget + 1;
+    __syncthreads();
   }
 }
 
@@ -847,23 +1004,24 @@ __global__ void __launch_bounds__(64 * WAVES) attend_many_kernel(TileArgs g) {
 // Joining the parts: a job for each worker whose last tile goes on in the next one
 // ---------------------------------------------------------------------------
 template <typename T, int DB>
-__global__ void __launch_bounds__(256) attend_join_kernel(TileArgs g) {
+__global__ void __launch_bounds__(256) attend_join_kernel(TileArgs) {
   constexpr int kVals = DB / 64;
+  const Args g = kernel_args();
   __shared__ float sums[4][DB];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const Job job = g.jobs[blockIdx.x];
+  const Job job = g->jobs[blockIdx.x];
   const int rows = job.rows, parts = job.parts;
   if (rows == 0) return;
-  const int64_t one = (int64_t)g.rows * (DB + 2);
-  const float* first = g.part + job.first * one;
-  const float* rest = g.part + 2 * ((int64_t)blockIdx.x + 1) * one;  // part i > 0: two slots further each
+  const int64_t one = (int64_t)g->rows * (DB + 2);
+  const float* first = g->part + job.first * one;
+  const float* rest = g->part + 2 * ((int64_t)blockIdx.x + 1) * one;  // part i > 0: two slots further each
   auto part = [&](int i, int row) { return (i == 0 ? first : rest + (int64_t)(i - 1) * 2 * one) + (int64_t)row * (DB + 2); };
   auto store = [&](int row, const float* acc, float inv) {
-    const int i = (uint32_t)row / (uint32_t)g.group;
-    T* out = static_cast<T*>(g.a.out) + (job.token + i) * g.a.o_st + (int64_t)(job.head + row - i * g.group) * g.a.o_sh;
+    const int i = (uint32_t)row / (uint32_t)g->group;
+    T* out = static_cast<T*>(g->a.out) + (int64_t)(job.token + i) * g->a.o_st + (int64_t)(job.head + row - i * g->group) * g->a.o_sh;
 #pragma unroll
     for (int v = 0; v < kVals; ++v)
-      if (64 * v + lane < g.a.dim) out[64 * v + lane] = from_f32<T>(acc[v] * inv);
+      if (64 * v + lane < g->a.dim) out[64 * v + lane] = from_f32<T>(acc[v] * inv);
   };
   typedef float f32x2_a __attribute__((ext_vector_type(2), aligned(8)));
   const auto factor = [](float m, float top) { return top == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(m - top); };
@@ -1010,6 +1168,7 @@ bool attend_tiles_take(const AttendArgs& a, int dtype) {
   bool ok = a.dim <= 256 && a.dim % ve == 0 && group <= kRows * (a.dim > 128 || (a.dim > 64 && ve == 4) ? 4 : 8);
   for (const void* x : {a.q, a.k, a.v, (const void*)a.out}) ok = ok && aligned16(x);
   for (int64_t st : {a.q_st, a.q_sh, a.o_st, a.o_sh, a.kp, a.ks, a.kh, a.vp, a.vs, a.vh}) ok = ok && st % ve == 0;
+  for (int64_t st : {a.kp, a.ks, a.vp, a.vs}) ok = ok && st <= (int64_t)UINT32_MAX / 4;  // (bytes are multiplied in 32 x 32 bits)
   return ok;
 }
 
@@ -1030,6 +1189,11 @@ void attend_tiles(const AttendArgs& a, int64_t max_chunk, int dtype, void* works
   g.rows = p.rows;
   g.workers = (int)p.workers;
   g.min_units = p.min_units;
+  const uint32_t esz = (uint32_t)ak_dtype_size(dtype);
+  g.kp = (uint32_t)a.kp * esz;
+  g.ks = (uint32_t)a.ks * esz;
+  g.vp = (uint32_t)a.vp * esz;
+  g.vs = (uint32_t)a.vs * esz;
   g.line = static_cast<int64_t*>(workspace);
   g.jobs = reinterpret_cast<Job*>(static_cast<char*>(workspace) + p.line_bytes);
   g.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + p.line_bytes + p.job_bytes);
