@@ -524,8 +524,9 @@ __device__ __forceinline__ void rows_end(Args g0, const Place& p, int row0, Rows
   const int lane = threadIdx.x & 63, half = lane >> 5, row = row0 + (lane & 31);
   const float l = both_halves(r.l);
   const int t0 = p.t * g->per_tile, tokens = min(g->per_tile, p.s.count - t0), group = g->group;
-  if (row >= tokens * group) return;
+  const bool mine = row < tokens * group;
   if (slot >= 0) {
+    if (!mine) return;
     float* x = g->part + (slot * g->rows + row) * (DB + 2);
 #pragma unroll
     for (int b = 0; b < S::kBlocks; ++b)
@@ -547,12 +548,21 @@ __device__ __forceinline__ void rows_end(Args g0, const Place& p, int row0, Rows
 #pragma unroll
   for (int b = 0; b < S::kBlocks; ++b)
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const int d = 32 * b + 8 * c + 4 * half;
-      if (d >= dim) continue;
-      const float x0 = r.o[b][4 * c] * inv, x1 = r.o[b][4 * c + 1] * inv, x2 = r.o[b][4 * c + 2] * inv, x3 = r.o[b][4 * c + 3] * inv;
-      if constexpr (sizeof(T) == 2) *reinterpret_cast<u32x2*>(out + d) = u32x2{pack2<T>(x0, x1), pack2<T>(x2, x3)};
-      else *reinterpret_cast<f32x4_v*>(out + d) = f32x4_v{x0, x1, x2, x3};
+    for (int c = 0; c < 4; c += 2) {
+      float y[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] = r.o[b][4 * c + e] * inv;
+      if constexpr (sizeof(T) == 2) {
+        // the lane's 4 values of c and of c + 1 for 8 neighbours, with the other half's
+        const auto lo = __builtin_amdgcn_permlane32_swap(pack2<T>(y[0], y[1]), pack2<T>(y[4], y[5]), false, false);
+        const auto hi = __builtin_amdgcn_permlane32_swap(pack2<T>(y[2], y[3]), pack2<T>(y[6], y[7]), false, false);
+        const int d = 32 * b + 8 * (c + half);
+        if (mine && d < dim) *reinterpret_cast<u32x4*>(out + d) = u32x4{lo[0], hi[0], lo[1], hi[1]};
+      } else {
+        const int d = 32 * b + 8 * c + 4 * half;
+        if (mine && d < dim) *reinterpret_cast<f32x4_v*>(out + d) = f32x4_v{y[0], y[1], y[2], y[3]};
+        if (mine && d + 8 < dim) *reinterpret_cast<f32x4_v*>(out + d + 8) = f32x4_v{y[4], y[5], y[6], y[7]};
+      }
     }
 }
 
@@ -587,46 +597,9 @@ __device__ __forceinline__ void zero_other_rows(Args g, int wave, int waves) {
   }
 }
 
-// The pages of a unit's keys, a key a lane (its 32 or 64 rows): looked up while the unit
-// before it is loaded.
-template <int UNIT, int GROUP>
-struct Pages {
-  int page, slot;    // page -1: no key of the tile
-  int key, lo, hi;   // the unit's first key, the tile's
-  int h;
-  bool clean;        // only some of the tile's rows see some of the keys
-
-  // GROUP rows are loaded together, seen by some row of the tile or not.
-  __device__ __forceinline__ void look_up(Args g, const PageMath& math, const Place& p, int key0) {
-    const int at_key = key0 + (threadIdx.x & (UNIT - 1));
-    page = -1;
-    slot = 0;
-    key = key0;
-    lo = p.k.lo;
-    hi = p.k.hi;
-    h = p.h;
-    if (at_key >= (p.k.lo & -GROUP) && at_key < p.k.hi) {
-      uint32_t at, in;
-      math.place((uint32_t)at_key, at, in);
-      slot = (int)in;
-      page = g->a.pages[(int64_t)p.b * g->a.ld_pages + at];
-    }
-    const int t0 = p.t * g->per_tile, tokens = min(g->per_tile, p.s.count - t0);
-    clean = tokens > 1 && key0 + UNIT > p.s.pos0 + t0 + 1;
-    if (g->a.window > 0) clean = clean || (tokens > 1 && key0 < (int64_t)p.s.pos0 + t0 + tokens - g->a.window);
-  }
-  // The keys that are there, by row.
-  __device__ __forceinline__ uint64_t seen(uint32_t n_pages) const {
-    const uint64_t all = __ballot((uint32_t)page < n_pages);
-    return UNIT == 64 ? all : all & 0xFFFFFFFFu;
-  }
-};
-
-// Where the cache is: bases of this lane's chunk, strides in bytes.
+// Where the cache is: bases of this lane's chunk.
 struct Cache {
   const char *k, *v;
-  int64_t kh, vh;          // head strides in bytes
-  uint32_t kp, ks, vp, vs, n_pages;
   bool on;                 // the lane's chunk is one of a row
 };
 
@@ -634,50 +607,73 @@ template <typename T, int DB>
 __device__ __forceinline__ Cache cache_of(Args g) {
   using S = Shape<T, DB>;
   const int d = (threadIdx.x & 63) % S::kChunks * 16;
-  return {static_cast<const char*>(g->a.k) + d, static_cast<const char*>(g->a.v) + d, g->a.kh * (int64_t)sizeof(T),
-          g->a.vh * (int64_t)sizeof(T), g->kp, g->ks, g->vp, g->vs, (uint32_t)g->a.n_pages, d < g->a.dim * (int)sizeof(T)};
+  return {static_cast<const char*>(g->a.k) + d, static_cast<const char*>(g->a.v) + d, d < g->a.dim * (int)sizeof(T)};
+}
+
+// Looking a key's row up, in two steps some units apart: its page is loaded (without a
+// condition: a merge behind one would wait for it), then its K and V rows' byte offsets, or
+// kNoRow, go into a table in LDS. The loops that read the table need nothing else of the
+// sequence, head or page.
+constexpr uint32_t kNoRow = 0xFFFFFFFFu;  // in the high half of K's offset
+
+struct LookUp {
+  int page, slot, h;
+  bool of_tile;
+
+  __device__ __forceinline__ void start(Args g0, const Place& p, int key) {
+    const Args g = fresh(g0);
+    of_tile = key >= p.k.lo && key < p.k.hi;
+    uint32_t at, in;
+    page_math(g).place((uint32_t)max(min(max(key, p.k.lo), p.k.hi - 1), 0), at, in);
+    slot = (int)in;
+    h = p.h;
+    page = g->a.pages[(int64_t)p.b * g->a.ld_pages + at];
+  }
+  // Returns whether the key is there.
+  template <typename T>
+  __device__ __forceinline__ bool finish(Args g0, u32x4* to) const {
+    const Args g = fresh(g0);
+    const bool there = of_tile && (uint32_t)page < (uint32_t)g->a.n_pages;
+    const uint64_t k = (uint64_t)(uint32_t)page * g->kp + (uint64_t)(uint32_t)slot * g->ks + (uint64_t)h * (uint64_t)(g->a.kh * (int64_t)sizeof(T));
+    const uint64_t v = (uint64_t)(uint32_t)page * g->vp + (uint64_t)(uint32_t)slot * g->vs + (uint64_t)h * (uint64_t)(g->a.vh * (int64_t)sizeof(T));
+    *to = u32x4{(uint32_t)k, there ? (uint32_t)(k >> 32) : kNoRow, (uint32_t)v, (uint32_t)(v >> 32)};
+    return there;
+  }
+};
+
+// Whether only some of a tile's rows see some of the unit's keys.
+__device__ __forceinline__ bool partly_seen(Args g, const Place& p, int key0, int unit) {
+  const int t0 = p.t * g->per_tile, tokens = min(g->per_tile, p.s.count - t0);
+  bool some = tokens > 1 && key0 + unit > p.s.pos0 + t0 + 1;
+  if (g->a.window > 0) some = some || (tokens > 1 && key0 < (int64_t)p.s.pos0 + t0 + tokens - g->a.window);
+  return some;
 }
 
 // The K and V rows of a unit, as N loads of a wave each: load i takes rows first + i *
-// stride .. + kPerLoad - 1. LANE: pages that are no multiple of a load's rows, so that a
-// load's rows are on pages of their own; else the page and slot are scalars. Keys that no
-// row of the tile sees are zeros.
-template <typename T, int DB, int N, int UNIT, bool LANE>
+// stride .. + kPerLoad - 1. Keys that are not there are zeros.
+template <typename T, int DB, int N>
 struct Loads {
   using S = Shape<T, DB>;
-  using P = Pages<UNIT, LANE ? 1 : S::kPerLoad>;
   u32x4 k[N], v[N];
-  bool clean;
 
-  __device__ __forceinline__ void issue(const Cache& c, const P& pg, int first, int stride) {
+  __device__ __forceinline__ void issue(const Cache& c, const u32x4* table, int first, int stride) {
     const int in = (threadIdx.x & 63) / S::kChunks;
-    const char* kb = c.k + pg.h * c.kh;
-    const char* vb = c.v + pg.h * c.vh;
-    clean = pg.clean;
+    u32x4 at[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) at[i] = table[first + i * stride + in];
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       k[i] = v[i] = u32x4{0, 0, 0, 0};
-      const int row = first + i * stride;
-      if constexpr (LANE) {
-        const uint32_t page = __shfl(pg.page, row + in), slot = __shfl(pg.slot, row + in);
-        if (page < c.n_pages && c.on) {
-          k[i] = *reinterpret_cast<const u32x4*>(kb + (uint64_t)page * c.kp + (uint64_t)slot * c.ks);
-          v[i] = *reinterpret_cast<const u32x4*>(vb + (uint64_t)page * c.vp + (uint64_t)slot * c.vs);
-        }
-      } else {
-        // (a row of the load past the tile's keys may be first: its page is the others')
-        const uint32_t page = __builtin_amdgcn_readlane(pg.page, row), slot = __builtin_amdgcn_readlane(pg.slot, row) + in;
-        if (page < c.n_pages && c.on && pg.key + row + in >= pg.lo && pg.key + row + in < pg.hi) {
-          k[i] = *reinterpret_cast<const u32x4*>(kb + (uint64_t)page * c.kp + (uint64_t)slot * c.ks);
-          v[i] = *reinterpret_cast<const u32x4*>(vb + (uint64_t)page * c.vp + (uint64_t)slot * c.vs);
-        }
+      if (at[i][1] != kNoRow && c.on) {
+        k[i] = *reinterpret_cast<const u32x4*>(c.k + ((uint64_t)at[i][1] << 32 | at[i][0]));
+        v[i] = *reinterpret_cast<const u32x4*>(c.v + ((uint64_t)at[i][3] << 32 | at[i][2]));
       }
     }
   }
 
   // Into LDS; where the unit is to be clean, with 0 for values that are not finite. Returns
   // whether this lane had some.
-  __device__ __forceinline__ bool store(int first, int stride, char* kl, char* vl) {
+  __device__ __forceinline__ bool store(int first, int stride, char* kl, char* vl, bool clean) {
     const int lane = threadIdx.x & 63;
     const int row = first + lane / S::kChunks, chunk = lane % S::kChunks;
     char* kd = kl + row * S::kPitch + 16 * chunk;
@@ -707,11 +703,12 @@ struct Loads {
 // ---------------------------------------------------------------------------
 constexpr int kFewWaves = 4;
 
-template <typename T, int DB, bool LANE>
+template <typename T, int DB>
 __global__ void __launch_bounds__(64 * kFewWaves, DB * sizeof(T) <= 256 ? 2 : 1) attend_few_kernel(TileArgs, bool lined) {
   using S = Shape<T, DB>;
   constexpr int N = 32 / S::kPerLoad;
   __shared__ __attribute__((aligned(16))) char lds[kFewWaves][32 * (S::kPitch + S::vPitch)];
+  __shared__ u32x4 tables[kFewWaves][2][64];  // the rows of two pairs of units
   __shared__ int64_t sums[kFewWaves];
   __shared__ int64_t found[kFewWaves][3];
   const Args g = kernel_args();
@@ -787,39 +784,38 @@ __global__ void __launch_bounds__(64 * kFewWaves, DB * sizeof(T) <= 256 ? 2 : 1)
 
   char* const kl = lds[wave];
   char* const vl = lds[wave] + 32 * S::kPitch;
-  const PageMath math = page_math(g);
   const ScoreMath sm = score_math(g);
   const Cache cache = cache_of<T, DB>(g);
-  Loads<T, DB, N, 32, LANE> x;
-  typename Loads<T, DB, N, 32, LANE>::P pg;
+  Loads<T, DB, N> x;
+  LookUp next;
   Rows<T, DB> r;
   int unit = uniform((int)in_tile), left = uniform((int)min(u1 - u0, (int64_t)INT32_MAX));
   for (int tile = 0;; ++tile) {
     const int begin = unit, tile_units = p.k.u1 - p.k.u0, n = min(tile_units - unit, left);
-    int key0 = uniform((p.k.u0 + unit) * 32);
-    const int key1 = key0 + 32 * n;
-    pg.look_up(g, math, p, key0);
-    typename Loads<T, DB, N, 32, LANE>::P pg1;
-    pg1.look_up(g, math, p, key0 + 32);
+    int key = uniform((p.k.u0 + unit) * 32);
+    // units are looked up in pairs: this one's are in the table, the next one's on their way
+    next.start(g, p, key + lane);
     rows_begin<T, DB>(g, p, 0, r);
-    x.issue(cache, pg, 0, S::kPerLoad);
-    uint32_t next = (uint32_t)pg.seen(cache.n_pages);
-    pg = pg1;
-    for (; key0 < key1; key0 += 32) {
-      const uint32_t seen = next;
-      const bool bad = x.store(0, S::kPerLoad, kl, vl);
-      if (key0 + 32 < key1) {
-        x.issue(cache, pg, 0, S::kPerLoad);
-        next = (uint32_t)pg.seen(cache.n_pages);
-        pg.look_up(g, math, p, key0 + 64);
+    uint64_t seen = __ballot(next.finish<T>(g, &tables[wave][0][lane]));
+    next.start(g, p, key + 64 + lane);
+    x.issue(cache, tables[wave][0], 0, S::kPerLoad);
+    for (int i = 0; i < n; ++i, key += 32) {
+      const uint32_t now = (uint32_t)seen;
+      const bool mask = key < r.low || key + 32 > r.top || now != 0xFFFFFFFFu;
+      const bool bad = x.store(0, S::kPerLoad, kl, vl, mask && (r.top < r.end || r.low > r.beg));
+      seen >>= 32;
+      if (i & 1) {
+        seen = __ballot(next.finish<T>(g, &tables[wave][((i + 1) >> 1) & 1][lane]));
+        next.start(g, p, key + 96 + lane);
       }
+      if (i + 1 < n) x.issue(cache, &tables[wave][((i + 1) >> 1) & 1][((i + 1) & 1) * 32], 0, S::kPerLoad);
       f32x16_t s[1];
       s[0] = scores32<T, DB>(sm, r, kl, 0);
       if (sm.cap) cap32(sm, s[0]);
-      if (key0 < r.low || key0 + 32 > r.top || seen != 0xFFFFFFFFu) hide32<T, DB>(r, s[0], key0, seen);
+      if (mask) hide32<T, DB>(r, s[0], key, now);
       new_maximum<T, DB, 1>(sm, r, s);
       values32<T, DB>(r, weights32<T, DB>(sm, r, s[0]), vl, 0);
-      if (__any(bad)) add_not_finite<T, DB>(g, p, r, key0, seen);
+      if (__any(bad)) add_not_finite<T, DB>(g, p, r, key, now);
     }
     left -= n;
     unit += n;
@@ -842,13 +838,14 @@ __global__ void __launch_bounds__(64 * kFewWaves, DB * sizeof(T) <= 256 ? 2 : 1)
 // Many rows: a workgroup is a worker, its waves share the units' keys and values
 // ---------------------------------------------------------------------------
 // A worker's units go through a ring of LDS slots one after the other, whatever tile they
-// are of: looked up four steps, loaded three and stored two before their scores are taken.
-// A wave's step has two phases: the matrix cores' (O^T += of the unit before, the scores of
-// this one; a tile's end and the next one's beginning between them) and the vector units'
-// (the weights of this unit; the stores and loads of those ahead). Half of the waves, one on
-// each SIMD, runs a phase late, so that on every SIMD one wave feeds the matrix cores while
-// the other computes weights.
-template <typename T, int DB, int WAVES, int UNIT, bool LANE>
+// are of. In a round of WAVES units each wave looks one of the next round's units up; a unit
+// is loaded three and stored two steps before its scores are taken. A wave's step has two
+// phases: the matrix cores' (O^T += of the unit before, the scores of this one; a tile's end
+// and the next one's beginning between them) and the vector units' (the weights of this
+// unit; the stores, loads and look-ups of those ahead). Half of the waves, one on each SIMD,
+// runs a phase late, so that on every SIMD one wave feeds the matrix cores while the other
+// computes weights.
+template <typename T, int DB, int WAVES, int UNIT>
 __global__ void __launch_bounds__(64 * WAVES) attend_many_kernel(TileArgs) {
   using S = Shape<T, DB>;
   constexpr int N = UNIT / S::kPerLoad / WAVES;  // loads of a wave, UNIT rows over all waves
@@ -858,11 +855,16 @@ __global__ void __launch_bounds__(64 * WAVES) attend_many_kernel(TileArgs) {
   // K is read in the step of its scores, V in the next one, by the late waves a phase later.
   constexpr int kAhead = S::kRowBytes > 512 ? 1 : 2;
   constexpr int kSlots = kAhead + (WAVES == 8), vSlots = kSlots + 1;
+  // The rows' table holds 16 units: the rounds that are used and kLead more.
+  constexpr int kTable = 16, kLead = WAVES == 8 ? 1 : 2, kFinish = 2;
+  static_assert(WAVES == 8 || WAVES == 4, "rounds divide the table");
   __shared__ __attribute__((aligned(16))) char kl[kSlots][UNIT * S::kPitch];
   __shared__ __attribute__((aligned(16))) char vl[vSlots][UNIT * S::vPitch];
+  __shared__ u32x4 table[kTable][UNIT];
+  __shared__ uint32_t there[2 * kTable][4];      // of a unit: the bits of its keys that are there; whether it is partly seen
   __shared__ int bad[vSlots];                    // the unit (by count) whose values are not all finite
   const Args g = kernel_args();
-  const int wave = uniform(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const bool late = WAVES == 8 && wave >= 4;
   // neighbours in the line, which share keys, go to one XCD
   const int nb = (int)gridDim.x;
@@ -882,49 +884,69 @@ __global__ void __launch_bounds__(64 * WAVES) attend_many_kernel(TileArgs) {
   place_in_sequence(g, p, in_tile, g->line[p.b + 1] - g->line[p.b]);
   const int row0 = wave * kRows, first = wave * S::kPerLoad;
   constexpr int stride = WAVES * S::kPerLoad;
-  const PageMath math = page_math(g);
   const ScoreMath sm = score_math(g);
   const Cache cache = cache_of<T, DB>(g);
 
-  // the units' way into LDS: the tile and unit that are looked up next, how many are left
-  Loads<T, DB, N, UNIT, LANE> x;
-  typename Loads<T, DB, N, UNIT, LANE>::P pg;
+  // this wave's units on their way: the one that it looks up next
+  LookUp next;
   Place lp = p;
-  int l_unit = uniform((int)in_tile), l_left = n;
-  auto look_up = [&](auto& to) {
-    if (l_left == 0) return;
-    to.look_up(g, math, lp, uniform((lp.k.u0 + l_unit) * UNIT));
-    --l_left;
-    if (++l_unit == lp.k.u1 - lp.k.u0 && l_left > 0) {
-      l_unit = 0;
-      next_place(fresh(g), lp);
+  int l_unit = uniform((int)in_tile), l_at = 0;
+  auto advance = [&](int by) {
+    l_at += by;
+    while (by > 0 && l_at < n) {
+      const int rest = lp.k.u1 - lp.k.u0 - l_unit, go = min(by, rest);
+      l_unit += go;
+      by -= go;
+      if (go == rest) {
+        l_unit = 0;
+        next_place(fresh(g), lp);
+      }
     }
   };
-  int kput = 0, vput = 0, puts = 0;  // the slots that are stored next
-  auto put = [&]() {
-    ++puts;
-    if (x.store(first, stride, kl[kput], vl[vput])) bad[vput] = puts;
+  auto start = [&]() {
+    if (l_at < n) next.start(g, lp, (lp.k.u0 + l_unit) * UNIT + (lane & (UNIT - 1)));
+  };
+  auto finish = [&]() {
+    if (l_at < n) {
+      const int at = l_at % (2 * kTable);
+      const bool key_there = lane < UNIT && next.finish<T>(g, &table[at % kTable][lane & (UNIT - 1)]);
+      const uint64_t bits = __ballot(key_there);
+      const bool some = partly_seen(fresh(g), lp, (lp.k.u0 + l_unit) * UNIT, UNIT);
+      if (lane == 0) {
+        there[at][0] = (uint32_t)bits;
+        there[at][1] = (uint32_t)(bits >> 32);
+        there[at][2] = some;
+      }
+      advance(WAVES);
+    }
+  };
+  auto seen_of = [&](int j) {
+    const uint32_t* t = there[j % (2 * kTable)];
+    return (uint64_t)(uint32_t)uniform(t[1]) << 32 | (uint32_t)uniform(t[0]);
+  };
+  Loads<T, DB, N> x;
+  int kput = 0, vput = 0;  // the slots that are stored next
+  auto put = [&](int j) {
+    const bool clean = uniform(there[j % (2 * kTable)][2]) != 0;
+    if (x.store(first, stride, kl[kput], vl[vput], clean)) bad[vput] = j + 1;
     kput = kput + 1 == kSlots ? 0 : kput + 1;
     vput = vput + 1 == vSlots ? 0 : vput + 1;
   };
-  uint64_t seen[kAhead + 2];  // of the units j - 1, j, .. j + kAhead (their keys that are there)
-#pragma unroll
-  for (int a = 0; a < kAhead + 2; ++a) seen[a] = 0;
   if (threadIdx.x < vSlots) bad[threadIdx.x] = 0;
+  advance(wave);
+  for (int a = 0; a < kLead; ++a) {
+    start();
+    finish();
+  }
+  Rows<T, DB> r;
+  rows_begin<T, DB>(g, p, row0, r);
   __syncthreads();
-  {
-    typename Loads<T, DB, N, UNIT, LANE>::P all[kAhead + 2];
 #pragma unroll
-    for (int a = 0; a < kAhead + 2; ++a) look_up(all[a]);
-#pragma unroll
-    for (int a = 0; a <= kAhead; ++a) {
-      if (a < n) {
-        x.issue(cache, all[a], first, stride);
-        seen[a + 1] = all[a].seen(cache.n_pages);
-        if (a < kAhead) put();
-      }
+  for (int a = 0; a <= kAhead; ++a) {
+    if (a < n) {
+      x.issue(cache, table[a], first, stride);
+      if (a < kAhead) put(a);
     }
-    pg = all[kAhead + 1];
   }
   __syncthreads();
   if (late) __syncthreads();
@@ -932,9 +954,7 @@ __global__ void __launch_bounds__(64 * WAVES) attend_many_kernel(TileArgs) {
   int kget = 0, vget = vSlots - 1;  // the slots of unit j's keys and of unit j - 1's values
   bool before = false;              // this wave has weights of unit j - 1
   int unit = uniform((int)in_tile), begin = unit, tiles = 0;  // of the tile: unit j, this worker's first
-  int key = uniform((p.k.u0 + unit) * UNIT);
-  Rows<T, DB> r;
-  rows_begin<T, DB>(g, p, row0, r);
+  int key = uniform((p.k.u0 + unit) * UNIT), units = uniform(p.k.u1 - p.k.u0);
   f32x16_t s[NB];
   Weights<T> w[NB];
   for (int j = 0;; ++j) {
@@ -942,16 +962,19 @@ __global__ void __launch_bounds__(64 * WAVES) attend_many_kernel(TileArgs) {
 #pragma unroll
       for (int b = 0; b < NB; ++b) values32<T, DB>(r, w[b], vl[vget], 32 * b);
       if (uniform(bad[vget]) == j) {
-        for (int b = 0; b < NB; ++b) add_not_finite<T, DB>(g, p, r, key - UNIT + 32 * b, (uint32_t)(seen[0] >> (32 * b)));
+        const uint64_t seen = seen_of(j - 1);
+        for (int b = 0; b < NB; ++b) add_not_finite<T, DB>(g, p, r, key - UNIT + 32 * b, (uint32_t)(seen >> (32 * b)));
       }
     }
-    const bool ended = j > 0 && unit == p.k.u1 - p.k.u0;
+    const bool ended = j > 0 && unit == units;
     if (ended || j == n) {
       const int64_t slot = begin == 0 && ended ? -1 : 2 * (int64_t)worker + (tiles > 0);
       rows_end<T, DB>(g, p, row0, r, slot);
       if (j == n) {
         if (threadIdx.x == 0) {
-          const int parts = ended ? 0 : (int)(worker_of(u1 + (p.k.u1 - p.k.u0 - unit) - 1, total, n_workers) - worker) + 1;
+          const int64_t all = fresh(g)->line[fresh(g)->a.seq.batch], count = active_workers(fresh(g), all);
+          const int64_t end = begin_of(worker + 1, all, count);
+          const int parts = ended ? 0 : (int)(worker_of(end + (units - unit) - 1, all, count) - worker) + 1;
           leave_job(g, worker, begin == 0 && !ended ? &p : nullptr, slot, parts);
         }
         break;
@@ -960,6 +983,7 @@ __global__ void __launch_bounds__(64 * WAVES) attend_many_kernel(TileArgs) {
       unit = begin = 0;
       ++tiles;
       key = uniform(p.k.u0 * UNIT);
+      units = uniform(p.k.u1 - p.k.u0);
       rows_begin<T, DB>(g, p, row0, r);
     }
     const bool now = key < r.end && key + UNIT > r.beg;
@@ -968,24 +992,21 @@ __global__ void __launch_bounds__(64 * WAVES) attend_many_kernel(TileArgs) {
       for (int b = 0; b < NB; ++b) s[b] = scores32<T, DB>(sm, r, kl[kget], 32 * b);
     }
     __syncthreads();
-#pragma unroll
-    for (int a = 0; a <= kAhead; ++a) seen[a] = seen[a + 1];
     if (j + kAhead < n) {
-      put();
-      if (j + kAhead + 1 < n) {
-        x.issue(cache, pg, first, stride);
-        seen[kAhead + 1] = pg.seen(cache.n_pages);
-        look_up(pg);
-      }
+      put(j + kAhead);
+      if (j + kAhead + 1 < n) x.issue(cache, table[(j + kAhead + 1) % kTable], first, stride);
     }
+    if (j % WAVES == 0) start();
+    if (j % WAVES == kFinish) finish();
     if (now) {
       if (sm.cap) {
 #pragma unroll
         for (int b = 0; b < NB; ++b) cap32(sm, s[b]);
       }
-      if (key < r.low || key + UNIT > r.top || seen[0] != (UNIT == 64 ? ~0ull : 0xFFFFFFFFull)) {
+      const uint64_t seen = seen_of(j);
+      if (key < r.low || key + UNIT > r.top || seen != (UNIT == 64 ? ~0ull : 0xFFFFFFFFull)) {
 #pragma unroll
-        for (int b = 0; b < NB; ++b) hide32<T, DB>(r, s[b], key + 32 * b, (uint32_t)(seen[0] >> (32 * b)));
+        for (int b = 0; b < NB; ++b) hide32<T, DB>(r, s[b], key + 32 * b, (uint32_t)(seen >> (32 * b)));
       }
       new_maximum<T, DB, NB>(sm, r, s);
 #pragma unroll
@@ -1131,15 +1152,15 @@ Plan plan_of(int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads, i
   return p;
 }
 
-template <typename T, int DB, bool LANE>
+template <typename T, int DB>
 void launch_tiles(const TileArgs& g, const Plan& p, hipStream_t s) {
   if (p.lined) attend_line_kernel<<<dim3(1), dim3(1024), 0, s>>>(g);
   if constexpr (DB < 256) {
-    if (p.few) attend_few_kernel<T, DB, LANE><<<dim3((unsigned)(p.workers / kFewWaves)), dim3(64 * kFewWaves), 0, s>>>(g, p.lined);
+    if (p.few) attend_few_kernel<T, DB><<<dim3((unsigned)(p.workers / kFewWaves)), dim3(64 * kFewWaves), 0, s>>>(g, p.lined);
   }
   if (!p.few) {
     constexpr int kWaves = DB * sizeof(T) > 256 ? 4 : 8, kUnit = DB * sizeof(T) > 256 ? 32 : 64;
-    attend_many_kernel<T, DB, kWaves, kUnit, LANE><<<dim3((unsigned)p.workers), dim3(64 * kWaves), 0, s>>>(g);
+    attend_many_kernel<T, DB, kWaves, kUnit><<<dim3((unsigned)p.workers), dim3(64 * kWaves), 0, s>>>(g);
   }
   if (p.workers > 1) {
     // (of few rows in many parts a row a workgroup, of many rows 16)
@@ -1150,11 +1171,7 @@ void launch_tiles(const TileArgs& g, const Plan& p, hipStream_t s) {
 
 template <typename T>
 void launch_type(TileArgs& g, const Plan& p, hipStream_t s) {
-  auto go = [&](auto db) {
-    constexpr int DB = decltype(db)::value;
-    if (g.a.page_size % Shape<T, DB>::kPerLoad) launch_tiles<T, DB, true>(g, p, s);
-    else launch_tiles<T, DB, false>(g, p, s);
-  };
+  auto go = [&](auto db) { launch_tiles<T, decltype(db)::value>(g, p, s); };
   if (p.padded == 64) go(std::integral_constant<int, 64>());
   else if (p.padded == 128) go(std::integral_constant<int, 128>());
   else go(std::integral_constant<int, 256>());
@@ -1165,7 +1182,7 @@ void launch_type(TileArgs& g, const Plan& p, hipStream_t s) {
 bool attend_tiles_take(const AttendArgs& a, int dtype) {
   const int ve = 16 / ak_dtype_size(dtype);
   const int64_t group = a.q_heads / a.kv_heads;
-  bool ok = a.dim <= 256 && a.dim % ve == 0 && group <= kRows * (a.dim > 128 || (a.dim > 64 && ve == 4) ? 4 : 8);
+  bool ok = a.max_pages > 0 && a.n_pages > 0 && a.dim <= 256 && a.dim % ve == 0 && group <= kRows * (a.dim > 128 || (a.dim > 64 && ve == 4) ? 4 : 8);
   for (const void* x : {a.q, a.k, a.v, (const void*)a.out}) ok = ok && aligned16(x);
   for (int64_t st : {a.q_st, a.q_sh, a.o_st, a.o_sh, a.kp, a.ks, a.kh, a.vp, a.vs, a.vh}) ok = ok && st % ve == 0;
   for (int64_t st : {a.kp, a.ks, a.vp, a.vs}) ok = ok && st <= (int64_t)UINT32_MAX / 4;  // (bytes are multiplied in 32 x 32 bits)
