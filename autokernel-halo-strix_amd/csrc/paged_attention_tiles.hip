@@ -43,7 +43,7 @@ struct TileArgs {
   uint32_t kp, ks, vp, vs;         // cache strides in bytes: page, slot
   int64_t* line;                   // [batch + 1]: the units before each sequence
   Job* jobs;                       // [workers]
-  float* part;                     // [2 workers][rows][DB + 2]: sums of products, maximum, sum
+  float* part;                     // [2 workers]: sums of products, maxima, sums of a tile's rows
   float c, cap_in, cap_out;        // scores in base 2: s c, or cap_out tanh(s cap_in)
 };
 
@@ -333,13 +333,33 @@ struct ScoreMath {
 };
 __device__ __forceinline__ ScoreMath score_math(Args g) { return {g->c, g->cap_in, g->cap_out, g->cap_out > 0.0f}; }
 
-// Loads the queries of rows [row0, row0 + 32) of a tile and starts their sums.
+// Loads the queries of rows [row0, row0 + 32) of a tile.
 template <typename T, int DB>
-__device__ __forceinline__ void rows_begin(Args g0, const Place& p, int row0, Rows<T, DB>& r) {
+__device__ __forceinline__ void rows_load(Args g0, const Place& p, int row0, Rows<T, DB>& r) {
   using S = Shape<T, DB>;
   const Args g = fresh(g0);
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int t0 = p.t * g->per_tile, tokens = min(g->per_tile, p.s.count - t0), group = g->group, dim = g->a.dim;
+  const int row = row0 + (lane & 31);
+  const int i = (uint32_t)row / (uint32_t)group;  // token of the tile
+  const bool live = i < tokens;
+  const T* q = static_cast<const T*>(g->a.q) + (int64_t)(p.s.first + t0 + min(i, tokens - 1)) * g->a.q_st +
+               (int64_t)(p.h * group + (row - i * group)) * g->a.q_sh;
+#pragma unroll
+  for (int k = 0; k < S::kSteps; ++k) {
+    r.q[k] = u32x4{0, 0, 0, 0};
+    const int d = (2 * k + half) * S::VE;
+    if (live && d < dim) r.q[k] = *reinterpret_cast<const u32x4*>(q + d);
+  }
+}
+
+// Starts the sums of rows [row0, row0 + 32) of a tile.
+template <typename T, int DB>
+__device__ __forceinline__ void rows_begin(Args g0, const Place& p, int row0, Rows<T, DB>& r) {
+  using S = Shape<T, DB>;
+  const Args g = fresh(g0);
+  const int lane = threadIdx.x & 63;
+  const int t0 = p.t * g->per_tile, tokens = min(g->per_tile, p.s.count - t0), group = g->group;
   const int row = row0 + (lane & 31);
   const int i = (uint32_t)row / (uint32_t)group;  // token of the tile
   const bool live = i < tokens;
@@ -357,14 +377,6 @@ __device__ __forceinline__ void rows_begin(Args g0, const Place& p, int row0, Ro
   if (window > 0) {
     r.low = uniform((int)max((int64_t)pos_1 + 1 - window, (int64_t)0));
     r.beg = uniform((int)max((int64_t)pos_0 + 1 - window, (int64_t)0));
-  }
-  const T* q = static_cast<const T*>(g->a.q) + (int64_t)(p.s.first + t0 + tok) * g->a.q_st +
-               (int64_t)(p.h * group + (row - i * group)) * g->a.q_sh;
-#pragma unroll
-  for (int k = 0; k < S::kSteps; ++k) {
-    r.q[k] = u32x4{0, 0, 0, 0};
-    const int d = (2 * k + half) * S::VE;
-    if (live && d < dim) r.q[k] = *reinterpret_cast<const u32x4*>(q + d);
   }
 #pragma unroll
   for (int b = 0; b < S::kBlocks; ++b) r.o[b] = f32x16_t{};
@@ -516,42 +528,20 @@ __device__ __forceinline__ void add_not_finite(Args g0, const Place& p, Rows<T, 
   }
 }
 
-// A row's results: to the output where the worker had all its units, else to a part's slot (-1: none).
+// Results of a wave's rows to the output.
 template <typename T, int DB>
-__device__ __forceinline__ void rows_end(Args g0, const Place& p, int row0, Rows<T, DB>& r, int64_t slot) {
-  using S = Shape<T, DB>;
-  const Args g = fresh(g0);
-  const int lane = threadIdx.x & 63, half = lane >> 5, row = row0 + (lane & 31);
-  const float l = both_halves(r.l);
-  const int t0 = p.t * g->per_tile, tokens = min(g->per_tile, p.s.count - t0), group = g->group;
-  const bool mine = row < tokens * group;
-  if (slot >= 0) {
-    if (!mine) return;
-    float* x = g->part + (slot * g->rows + row) * (DB + 2);
-#pragma unroll
-    for (int b = 0; b < S::kBlocks; ++b)
-#pragma unroll
-      for (int i = 0; i < 16; i += 2) {
-        typedef float f32x2_u __attribute__((ext_vector_type(2), aligned(8)));
-        *reinterpret_cast<f32x2_u*>(x + 32 * b + 8 * (i / 4) + 4 * half + i % 4) = f32x2_u{r.o[b][i], r.o[b][i + 1]};
-      }
-    if (half == 0) {
-      x[DB] = r.m;
-      x[DB + 1] = l;
-    }
-    return;
-  }
+__device__ __forceinline__ void rows_out(Args g, int token, int head, int row, bool mine, const f32x16_t* o, float l) {
+  const int half = (threadIdx.x & 63) >> 5;
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  const int i = (uint32_t)row / (uint32_t)group, dim = g->a.dim;
-  T* out = static_cast<T*>(g->a.out) + (int64_t)(p.s.first + t0 + i) * g->a.o_st +
-           (int64_t)(p.h * group + (row - i * group)) * g->a.o_sh;
+  const int group = g->group, i = (uint32_t)row / (uint32_t)group, dim = g->a.dim;
+  T* out = static_cast<T*>(g->a.out) + (int64_t)(token + i) * g->a.o_st + (int64_t)(head + (row - i * group)) * g->a.o_sh;
 #pragma unroll
-  for (int b = 0; b < S::kBlocks; ++b)
+  for (int b = 0; b < Shape<T, DB>::kBlocks; ++b)
 #pragma unroll
     for (int c = 0; c < 4; c += 2) {
       float y[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) y[e] = r.o[b][4 * c + e] * inv;
+      for (int e = 0; e < 8; ++e) y[e] = o[b][4 * c + e] * inv;
       if constexpr (sizeof(T) == 2) {
         // the lane's 4 values of c and of c + 1 for 8 neighbours, with the other half's
         const auto lo = __builtin_amdgcn_permlane32_swap(pack2<T>(y[0], y[1]), pack2<T>(y[4], y[5]), false, false);
@@ -564,6 +554,52 @@ __device__ __forceinline__ void rows_end(Args g0, const Place& p, int row0, Rows
         if (mine && d + 8 < dim) *reinterpret_cast<f32x4_v*>(out + d + 8) = f32x4_v{y[4], y[5], y[6], y[7]};
       }
     }
+}
+
+// A part of many rows holds its waves' registers as they are, four of a lane together: 1 KB
+// a store (rows in order, as a part of few rows has them, took 14 us a tile of 256).
+template <int DB>
+__device__ __forceinline__ float* wave_part(Args g, int64_t slot, int wave) {
+  return g->part + (slot * ((g->rows + 31) / 32) + wave) * (32 * (DB + 4));
+}
+
+// A row's results: to the output where the worker had all its units, else to a part's slot (-1: none).
+template <typename T, int DB, bool MANY>
+__device__ __forceinline__ void rows_end(Args g0, const Place& p, int row0, Rows<T, DB>& r, int64_t slot) {
+  using S = Shape<T, DB>;
+  const Args g = fresh(g0);
+  const int lane = threadIdx.x & 63, half = lane >> 5, row = row0 + (lane & 31);
+  const float l = both_halves(r.l);
+  const int t0 = p.t * g->per_tile, tokens = min(g->per_tile, p.s.count - t0);
+  const bool mine = row < tokens * g->group;
+  if (slot < 0) {
+    rows_out<T, DB>(g, p.s.first + t0, p.h * g->group, row, mine, r.o, l);
+    return;
+  }
+  if (!mine) return;
+  if constexpr (MANY) {
+    float* x = wave_part<DB>(g, slot, row0 / kRows);
+#pragma unroll
+    for (int b = 0; b < S::kBlocks; ++b)
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        *reinterpret_cast<f32x4_v*>(x + ((b * 4 + c) * 64 + lane) * 4) = f32x4_v{r.o[b][4 * c], r.o[b][4 * c + 1], r.o[b][4 * c + 2], r.o[b][4 * c + 3]};
+    typedef float f32x2_v __attribute__((ext_vector_type(2)));
+    *reinterpret_cast<f32x2_v*>(x + 32 * DB + 2 * lane) = f32x2_v{r.m, l};
+  } else {
+    float* x = g->part + (slot * g->rows + row) * (DB + 2);
+#pragma unroll
+    for (int b = 0; b < S::kBlocks; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; i += 2) {
+        typedef float f32x2_u __attribute__((ext_vector_type(2), aligned(8)));
+        *reinterpret_cast<f32x2_u*>(x + 32 * b + 8 * (i / 4) + 4 * half + i % 4) = f32x2_u{r.o[b][i], r.o[b][i + 1]};
+      }
+    if (half == 0) {
+      x[DB] = r.m;
+      x[DB + 1] = l;
+    }
+  }
 }
 
 // The job that a worker leaves, given its last tile where it has begun that but not ended it.
@@ -795,6 +831,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, DB * sizeof(T) <= 256 ? 2 : 1)
     int key = uniform((p.k.u0 + unit) * 32);
     // units are looked up in pairs: this one's are in the table, the next one's on their way
     next.start(g, p, key + lane);
+    rows_load<T, DB>(g, p, 0, r);
     rows_begin<T, DB>(g, p, 0, r);
     uint64_t seen = __ballot(next.finish<T>(g, &tables[wave][0][lane]));
     next.start(g, p, key + 64 + lane);
@@ -821,7 +858,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, DB * sizeof(T) <= 256 ? 2 : 1)
     unit += n;
     const bool ended = unit == tile_units;
     const int64_t slot = begin == 0 && ended ? -1 : 2 * (int64_t)worker + (tile > 0);
-    rows_end<T, DB>(g, p, 0, r, slot);
+    rows_end<T, DB, false>(g, p, 0, r, slot);
     if (left == 0) {
       if (lane == 0) {
         const int parts = ended ? 0 : (int)(worker_of(u1 + (tile_units - unit) - 1, total, n_workers) - worker) + 1;
@@ -841,10 +878,11 @@ __global__ void __launch_bounds__(64 * kFewWaves, DB * sizeof(T) <= 256 ? 2 : 1)
 // are of. In a round of WAVES units each wave looks one of the next round's units up; a unit
 // is loaded three and stored two steps before its scores are taken. A wave's step has two
 // phases: the matrix cores' (O^T += of the unit before, the scores of this one; a tile's end
-// and the next one's beginning between them) and the vector units' (the weights of this
-// unit; the stores, loads and look-ups of those ahead). Half of the waves, one on each SIMD,
+// and the next one's beginning between them; the stores and loads of units ahead) and the
+// vector units' (the weights of this unit, look-ups). Half of the waves, one on each SIMD,
 // runs a phase late, so that on every SIMD one wave feeds the matrix cores while the other
-// computes weights.
+// computes weights. (Four waves of long rows have a SIMD each: all in one phase, and the
+// stores after the barrier, which saves a slot.)
 template <typename T, int DB, int WAVES, int UNIT>
 __global__ void __launch_bounds__(64 * WAVES) attend_many_kernel(TileArgs) {
   using S = Shape<T, DB>;
@@ -893,6 +931,10 @@ __global__ void __launch_bounds__(64 * WAVES) attend_many_kernel(TileArgs) {
   int l_unit = uniform((int)in_tile), l_at = 0;
   auto advance = [&](int by) {
     l_at += by;
+    if (l_unit + by < lp.k.u1 - lp.k.u0) {
+      l_unit += by;
+      return;
+    }
     while (by > 0 && l_at < n) {
       const int rest = lp.k.u1 - lp.k.u0 - l_unit, go = min(by, rest);
       l_unit += go;
@@ -932,6 +974,12 @@ __global__ void __launch_bounds__(64 * WAVES) attend_many_kernel(TileArgs) {
     kput = kput + 1 == kSlots ? 0 : kput + 1;
     vput = vput + 1 == vSlots ? 0 : vput + 1;
   };
+  // unit j into LDS, the next one on its way
+  auto bring = [&](int j) {
+    if (j >= n) return;
+    put(j);
+    if (j + 1 < n) x.issue(cache, table[(j + 1) % kTable], first, stride);
+  };
   if (threadIdx.x < vSlots) bad[threadIdx.x] = 0;
   advance(wave);
   for (int a = 0; a < kLead; ++a) {
@@ -939,6 +987,7 @@ __global__ void __launch_bounds__(64 * WAVES) attend_many_kernel(TileArgs) {
     finish();
   }
   Rows<T, DB> r;
+  rows_load<T, DB>(g, p, row0, r);
   rows_begin<T, DB>(g, p, row0, r);
   __syncthreads();
 #pragma unroll
@@ -955,6 +1004,7 @@ __global__ void __launch_bounds__(64 * WAVES) attend_many_kernel(TileArgs) {
   bool before = false;              // this wave has weights of unit j - 1
   int unit = uniform((int)in_tile), begin = unit, tiles = 0;  // of the tile: unit j, this worker's first
   int key = uniform((p.k.u0 + unit) * UNIT), units = uniform(p.k.u1 - p.k.u0);
+  Place following = p;
   f32x16_t s[NB];
   Weights<T> w[NB];
   for (int j = 0;; ++j) {
@@ -969,7 +1019,7 @@ __global__ void __launch_bounds__(64 * WAVES) attend_many_kernel(TileArgs) {
     const bool ended = j > 0 && unit == units;
     if (ended || j == n) {
       const int64_t slot = begin == 0 && ended ? -1 : 2 * (int64_t)worker + (tiles > 0);
-      rows_end<T, DB>(g, p, row0, r, slot);
+      rows_end<T, DB, true>(g, p, row0, r, slot);
       if (j == n) {
         if (threadIdx.x == 0) {
           const int64_t all = fresh(g)->line[fresh(g)->a.seq.batch], count = active_workers(fresh(g), all);
@@ -979,7 +1029,7 @@ __global__ void __launch_bounds__(64 * WAVES) attend_many_kernel(TileArgs) {
         }
         break;
       }
-      next_place(fresh(g), p);
+      p = following;
       unit = begin = 0;
       ++tiles;
       key = uniform(p.k.u0 * UNIT);
@@ -991,10 +1041,13 @@ __global__ void __launch_bounds__(64 * WAVES) attend_many_kernel(TileArgs) {
 #pragma unroll
       for (int b = 0; b < NB; ++b) s[b] = scores32<T, DB>(sm, r, kl[kget], 32 * b);
     }
+    if (WAVES == 8) bring(j + kAhead);
     __syncthreads();
-    if (j + kAhead < n) {
-      put(j + kAhead);
-      if (j + kAhead + 1 < n) x.issue(cache, table[(j + kAhead + 1) % kTable], first, stride);
+    if (WAVES != 8) bring(j + kAhead);
+    if (unit + 1 == units && j + 1 < n) {  // the next tile's queries, in the registers that the last scores have left
+      following = p;
+      next_place(fresh(g), following);
+      rows_load<T, DB>(g, following, row0, r);
     }
     if (j % WAVES == 0) start();
     if (j % WAVES == kFinish) finish();
@@ -1024,6 +1077,40 @@ __global__ void __launch_bounds__(64 * WAVES) attend_many_kernel(TileArgs) {
 // ---------------------------------------------------------------------------
 // Joining the parts: a job for each worker whose last tile goes on in the next one
 // ---------------------------------------------------------------------------
+template <typename T, int DB>
+__global__ void __launch_bounds__(256) attend_join_many_kernel(TileArgs) {
+  const Args g = kernel_args();
+  const int lane = threadIdx.x & 63, wave = blockIdx.y * 4 + uniform(threadIdx.x >> 6);
+  const Job job = g->jobs[blockIdx.x];
+  const int row = wave * kRows + (lane & 31);
+  if (wave * kRows >= job.rows) return;
+  const bool mine = row < job.rows;
+  f32x16_t o[DB / 32];
+#pragma unroll
+  for (int b = 0; b < DB / 32; ++b) o[b] = f32x16_t{};
+  float top = kNegInf, sum = 0.0f;
+  for (int i = 0; i < job.parts; ++i) {
+    const float* x = wave_part<DB>(g, i == 0 ? job.first : 2 * ((int64_t)blockIdx.x + i), wave);
+    typedef float f32x2_v __attribute__((ext_vector_type(2)));
+    f32x2_v ml = {kNegInf, 0.0f};  // (lanes without a row left nothing)
+    if (mine) ml = *reinterpret_cast<const f32x2_v*>(x + 32 * DB + 2 * lane);
+    const float now = fmaxf(top, ml[0]);
+    const float keep = now == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(top - now), f = now == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(ml[0] - now);
+    top = now;
+    sum = sum * keep + ml[1] * f;
+#pragma unroll
+    for (int b = 0; b < DB / 32; ++b)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        f32x4_v v = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (mine) v = *reinterpret_cast<const f32x4_v*>(x + ((b * 4 + c) * 64 + lane) * 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[b][4 * c + e] = o[b][4 * c + e] * keep + v[e] * f;
+      }
+  }
+  rows_out<T, DB>(g, job.token, job.head, row, mine, o, sum);
+}
+
 template <typename T, int DB>
 __global__ void __launch_bounds__(256) attend_join_kernel(TileArgs) {
   constexpr int kVals = DB / 64;
@@ -1148,7 +1235,8 @@ Plan plan_of(int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads, i
   p.cut = p.workers > 8 * kv_heads * (tokens / p.per_tile);
   p.line_bytes = (size_t)(batch + 2) / 2 * 16;
   p.job_bytes = (size_t)p.workers * sizeof(Job);
-  p.part_bytes = (size_t)p.workers * 2 * (size_t)p.rows * (size_t)(p.padded + 2) * sizeof(float);
+  const size_t part = p.few ? (size_t)p.rows * (size_t)(p.padded + 2) : (size_t)((p.rows + 31) / 32) * 32 * (size_t)(p.padded + 4);
+  p.part_bytes = (size_t)p.workers * 2 * part * sizeof(float);
   return p;
 }
 
@@ -1163,9 +1251,10 @@ void launch_tiles(const TileArgs& g, const Plan& p, hipStream_t s) {
     attend_many_kernel<T, DB, kWaves, kUnit><<<dim3((unsigned)p.workers), dim3(64 * kWaves), 0, s>>>(g);
   }
   if (p.workers > 1) {
-    // (of few rows in many parts a row a workgroup, of many rows 16)
-    const unsigned slices = (unsigned)(p.rows > kRows ? (p.rows + 15) / 16 : p.cut ? std::min(p.rows, 4) : 1);
-    attend_join_kernel<T, DB><<<dim3((unsigned)(p.workers - 1), slices), dim3(256), 0, s>>>(g);
+    const unsigned jobs = (unsigned)(p.workers - 1);
+    if (!p.few) attend_join_many_kernel<T, DB><<<dim3(jobs, (unsigned)((p.rows + 127) / 128)), dim3(256), 0, s>>>(g);
+    // (of few rows in many parts a row a workgroup)
+    else attend_join_kernel<T, DB><<<dim3(jobs, (unsigned)(p.cut ? std::min(p.rows, 4) : 1)), dim3(256), 0, s>>>(g);
   }
 }
 
