@@ -495,6 +495,72 @@ __device__ __forceinline__ void values32(Rows<T, DB>& r, const Weights<T>& p, co
   }
 }
 
+// The same for a unit of NB x 32 keys, for the matrix phase of the many-row kernel: the
+// operands of a group of four MFMAs are read while the group before runs, and the compiler is
+// kept from moving the reads back to their uses (it reads two operands, waits for them and
+// uses them: [4, 4096 ..] prompts PINUS and UNPINUS us).
+__device__ __forceinline__ void pinned() { __builtin_amdgcn_sched_barrier(0); }
+
+template <typename T, int DB, int NB>
+__device__ __forceinline__ void scores_unit(const Rows<T, DB>& r, const char* kl, f32x16_t (&s)[NB]) {
+  using S = Shape<T, DB>;
+  constexpr int G = 4, kGroups = NB * S::kSteps / G;
+  const int lane = threadIdx.x & 63;
+  const char* base = kl + (lane & 31) * S::kPitch + 16 * (lane >> 5);
+  u32x4 k[2][G];
+  auto read = [&](int g) {
+#pragma unroll
+    for (int i = 0; i < G; ++i) {
+      const int at = g * G + i;
+      k[g % 2][i] = *reinterpret_cast<const u32x4*>(base + (at / S::kSteps) * 32 * S::kPitch + 32 * (at % S::kSteps));
+    }
+  };
+  read(0);
+  pinned();
+#pragma unroll
+  for (int g = 0; g < kGroups; ++g) {
+    if (g + 1 < kGroups) read(g + 1);
+#pragma unroll
+    for (int i = 0; i < G; ++i) {
+      const int at = g * G + i, b = at / S::kSteps, step = at % S::kSteps;
+      s[b] = mfma_step(T(), k[g % 2][i], r.q[step], step == 0 ? f32x16_t{} : s[b]);
+    }
+    pinned();
+  }
+}
+
+template <typename T, int DB, int NB>
+__device__ __forceinline__ void values_unit(Rows<T, DB>& r, const Weights<T> (&p)[NB], const char* vl) {
+  using S = Shape<T, DB>;
+  static_assert(sizeof(T) == 2, "fp32 takes values32");
+  constexpr int G = S::kBlocks < 4 ? S::kBlocks : 4, kGroups = NB * 2 * S::kBlocks / G;
+  const int lane = threadIdx.x & 63, j = lane & 15;
+  const char* base = vl + (4 * (lane >> 5) + (j >> 2)) * S::vPitch + 32 * ((lane >> 4) & 1) + 8 * (j & 3);
+  u32x2 x[2][G], y[2][G];
+  auto read = [&](int g) {
+#pragma unroll
+    for (int i = 0; i < G; ++i) {
+      const int at = g * G + i;
+      const char* from = base + 16 * (at / S::kBlocks) * S::vPitch + 64 * (at % S::kBlocks);
+      x[g % 2][i] = lds_tr(from);
+      y[g % 2][i] = lds_tr(from + 8 * S::vPitch);
+    }
+  };
+  read(0);
+  pinned();
+#pragma unroll
+  for (int g = 0; g < kGroups; ++g) {
+    if (g + 1 < kGroups) read(g + 1);
+#pragma unroll
+    for (int i = 0; i < G; ++i) {
+      const int at = g * G + i, kb = at / S::kBlocks, blk = at % S::kBlocks;
+      const u32x2 a = x[g % 2][i], b = y[g % 2][i];
+      r.o[blk] = mfma32(T(), u32x4{a[0], a[1], b[0], b[1]}, p[kb / 2].w[kb % 2], r.o[blk]);
+    }
+    pinned();
+  }
+}
+
 // What values that are not finite (left out of LDS where only some rows see them) do to
 // the rows that see their keys.
 template <typename T, int DB>
@@ -686,35 +752,46 @@ __device__ __forceinline__ bool partly_seen(Args g, const Place& p, int key0, in
 }
 
 // The K and V rows of a unit, as N loads of a wave each: load i takes rows first + i *
-// stride .. + kPerLoad - 1. Keys that are not there are zeros.
+// stride .. + kPerLoad - 1. Rows that are not there are loaded from the cache's first place:
+// their keys are hidden, their values become zeros on the way into LDS.
 template <typename T, int DB, int N>
 struct Loads {
   using S = Shape<T, DB>;
+  u32x4 at[N];      // the rows' places, read from the table before they are needed
   u32x4 k[N], v[N];
 
-  __device__ __forceinline__ void issue(const Cache& c, const u32x4* table, int first, int stride) {
+  __device__ __forceinline__ void places(const u32x4* table, int first, int stride) {
     const int in = (threadIdx.x & 63) / S::kChunks;
-    u32x4 at[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) at[i] = table[first + i * stride + in];
+  }
+
+  // (lanes of chunks past the head's end load nothing: their part of LDS stays zeros)
+  __device__ __forceinline__ void issue(const Cache& c) {
+    if (!c.on) return;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      k[i] = v[i] = u32x4{0, 0, 0, 0};
-      if (at[i][1] != kNoRow && c.on) {
-        k[i] = *reinterpret_cast<const u32x4*>(c.k + ((uint64_t)at[i][1] << 32 | at[i][0]));
-        v[i] = *reinterpret_cast<const u32x4*>(c.v + ((uint64_t)at[i][3] << 32 | at[i][2]));
-      }
+      const bool row = at[i][1] != kNoRow;
+      k[i] = *reinterpret_cast<const u32x4*>(c.k + (row ? (uint64_t)at[i][1] << 32 | at[i][0] : 0));
+      v[i] = *reinterpret_cast<const u32x4*>(c.v + (row ? (uint64_t)at[i][3] << 32 | at[i][2] : 0));
     }
   }
 
-  // Into LDS; where the unit is to be clean, with 0 for values that are not finite. Returns
-  // whether this lane had some.
-  __device__ __forceinline__ bool store(int first, int stride, char* kl, char* vl, bool clean) {
+  // Into LDS. gaps: not all rows of the unit are there (its table is given once more); clean:
+  // values that are not finite become 0. Returns whether this lane had some of those.
+  __device__ __forceinline__ bool store(const Cache& c, int first, int stride, char* kl, char* vl, bool gaps, const u32x4* table,
+                                        bool clean) {
+    if (!c.on) return false;
     const int lane = threadIdx.x & 63;
     const int row = first + lane / S::kChunks, chunk = lane % S::kChunks;
     char* kd = kl + row * S::kPitch + 16 * chunk;
     char* vd = vl + row * S::vPitch + 16 * chunk;
     uint32_t found = 0;
+    if (gaps) {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (table[row + i * stride][1] == kNoRow) v[i] = u32x4{0, 0, 0, 0};
+    }
     if (clean) {
 #pragma unroll
       for (int i = 0; i < N; ++i)
@@ -733,6 +810,11 @@ struct Loads {
     return found != 0;
   }
 };
+
+// Zeros into LDS from all of a workgroup's (or wave's) threads.
+__device__ __forceinline__ void clear_lds(char* to, int bytes, int thread, int threads) {
+  for (int i = thread * 16; i < bytes; i += threads * 16) *reinterpret_cast<u32x4*>(to + i) = u32x4{0, 0, 0, 0};
+}
 
 // ---------------------------------------------------------------------------
 // Few rows: a wave is a worker
@@ -825,6 +907,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, DB * sizeof(T) <= 256 ? 2 : 1)
   Loads<T, DB, N> x;
   LookUp next;
   Rows<T, DB> r;
+  clear_lds(kl, 32 * (S::kPitch + S::vPitch), lane, 64);
   int unit = uniform((int)in_tile), left = uniform((int)min(u1 - u0, (int64_t)INT32_MAX));
   for (int tile = 0;; ++tile) {
     const int begin = unit, tile_units = p.k.u1 - p.k.u0, n = min(tile_units - unit, left);
@@ -835,17 +918,22 @@ __global__ void __launch_bounds__(64 * kFewWaves, DB * sizeof(T) <= 256 ? 2 : 1)
     rows_begin<T, DB>(g, p, 0, r);
     uint64_t seen = __ballot(next.finish<T>(g, &tables[wave][0][lane]));
     next.start(g, p, key + 64 + lane);
-    x.issue(cache, tables[wave][0], 0, S::kPerLoad);
+    x.places(tables[wave][0], 0, S::kPerLoad);
+    x.issue(cache);
     for (int i = 0; i < n; ++i, key += 32) {
       const uint32_t now = (uint32_t)seen;
       const bool mask = key < r.low || key + 32 > r.top || now != 0xFFFFFFFFu;
-      const bool bad = x.store(0, S::kPerLoad, kl, vl, mask && (r.top < r.end || r.low > r.beg));
+      const bool bad = x.store(cache, 0, S::kPerLoad, kl, vl, now != 0xFFFFFFFFu, &tables[wave][(i >> 1) & 1][(i & 1) * 32],
+                               mask && (r.top < r.end || r.low > r.beg));
       seen >>= 32;
       if (i & 1) {
         seen = __ballot(next.finish<T>(g, &tables[wave][((i + 1) >> 1) & 1][lane]));
         next.start(g, p, key + 96 + lane);
       }
-      if (i + 1 < n) x.issue(cache, &tables[wave][((i + 1) >> 1) & 1][((i + 1) & 1) * 32], 0, S::kPerLoad);
+      if (i + 1 < n) {
+        x.places(&tables[wave][((i + 1) >> 1) & 1][((i + 1) & 1) * 32], 0, S::kPerLoad);
+        x.issue(cache);
+      }
       f32x16_t s[1];
       s[0] = scores32<T, DB>(sm, r, kl, 0);
       if (sm.cap) cap32(sm, s[0]);
@@ -899,7 +987,7 @@ __global__ void __launch_bounds__(64 * WAVES) attend_many_kernel(TileArgs) {
   __shared__ __attribute__((aligned(16))) char kl[kSlots][UNIT * S::kPitch];
   __shared__ __attribute__((aligned(16))) char vl[vSlots][UNIT * S::vPitch];
   __shared__ u32x4 table[kTable][UNIT];
-  __shared__ uint32_t there[2 * kTable][4];      // of a unit: the bits of its keys that are there; whether it is partly seen
+  __shared__ uint32_t there[2 * kTable][4];      // of a unit: the bits of its keys that are there; 1: partly seen, 2: not all there
   __shared__ int bad[vSlots];                    // the unit (by count) whose values are not all finite
   const Args g = kernel_args();
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
@@ -957,7 +1045,7 @@ __global__ void __launch_bounds__(64 * WAVES) attend_many_kernel(TileArgs) {
       if (lane == 0) {
         there[at][0] = (uint32_t)bits;
         there[at][1] = (uint32_t)(bits >> 32);
-        there[at][2] = some;
+        there[at][2] = some | (bits != (UNIT == 64 ? ~0ull : 0xFFFFFFFFull)) * 2u;
       }
       advance(WAVES);
     }
@@ -968,19 +1056,29 @@ __global__ void __launch_bounds__(64 * WAVES) attend_many_kernel(TileArgs) {
   };
   Loads<T, DB, N> x;
   int kput = 0, vput = 0;  // the slots that are stored next
-  auto put = [&](int j) {
-    const bool clean = uniform(there[j % (2 * kTable)][2]) != 0;
-    if (x.store(first, stride, kl[kput], vl[vput], clean)) bad[vput] = j + 1;
-    kput = kput + 1 == kSlots ? 0 : kput + 1;
-    vput = vput + 1 == vSlots ? 0 : vput + 1;
+  uint32_t flags = 0;      // of the unit that is stored next
+  auto prepare = [&](int j) {
+    x.places(table[j % kTable], first, stride);
+    flags = there[(j + 2 * kTable - 1) % (2 * kTable)][2];
   };
-  // unit j into LDS, the next one on its way
+  // Unit j into LDS, the next one on its way, the one after it made ready: nothing here waits
+  // for what it has asked for itself.
   auto bring = [&](int j) {
     if (j >= n) return;
-    put(j);
-    if (j + 1 < n) x.issue(cache, table[(j + 1) % kTable], first, stride);
+    const int f = uniform(flags);
+    if (x.store(cache, first, stride, kl[kput], vl[vput], f & 2, table[j % kTable], f & 1)) bad[vput] = j + 1;
+    kput = kput + 1 == kSlots ? 0 : kput + 1;
+    vput = vput + 1 == vSlots ? 0 : vput + 1;
+    if (j + 1 < n) {
+      x.issue(cache);
+      prepare(j + 2);
+    }
   };
   if (threadIdx.x < vSlots) bad[threadIdx.x] = 0;
+  if (g->a.dim < DB) {
+    clear_lds(kl[0], sizeof(kl), threadIdx.x, 64 * WAVES);
+    clear_lds(vl[0], sizeof(vl), threadIdx.x, 64 * WAVES);
+  }
   advance(wave);
   for (int a = 0; a < kLead; ++a) {
     start();
@@ -990,13 +1088,10 @@ __global__ void __launch_bounds__(64 * WAVES) attend_many_kernel(TileArgs) {
   rows_load<T, DB>(g, p, row0, r);
   rows_begin<T, DB>(g, p, row0, r);
   __syncthreads();
-#pragma unroll
-  for (int a = 0; a <= kAhead; ++a) {
-    if (a < n) {
-      x.issue(cache, table[a], first, stride);
-      if (a < kAhead) put(a);
-    }
-  }
+  prepare(0);
+  x.issue(cache);
+  prepare(1);
+  for (int a = 0; a < kAhead; ++a) bring(a);
   __syncthreads();
   if (late) __syncthreads();
 
@@ -1005,17 +1100,27 @@ __global__ void __launch_bounds__(64 * WAVES) attend_many_kernel(TileArgs) {
   int unit = uniform((int)in_tile), begin = unit, tiles = 0;  // of the tile: unit j, this worker's first
   int key = uniform((p.k.u0 + unit) * UNIT), units = uniform(p.k.u1 - p.k.u0);
   Place following = p;
-  f32x16_t s[NB];
   Weights<T> w[NB];
   for (int j = 0;; ++j) {
+    __builtin_amdgcn_s_setprio(1);  // the matrix cores' wave first
     if (before) {
+      if constexpr (sizeof(T) == 2) {
+        values_unit<T, DB, NB>(r, w, vl[vget]);
+      } else {
 #pragma unroll
-      for (int b = 0; b < NB; ++b) values32<T, DB>(r, w[b], vl[vget], 32 * b);
+        for (int b = 0; b < NB; ++b) values32<T, DB>(r, w[b], vl[vget], 32 * b);
+      }
       if (uniform(bad[vget]) == j) {
         const uint64_t seen = seen_of(j - 1);
         for (int b = 0; b < NB; ++b) add_not_finite<T, DB>(g, p, r, key - UNIT + 32 * b, (uint32_t)(seen >> (32 * b)));
       }
     }
+    // Queries that may be on their way are waited for here, where the unit's loads are, too:
+    // before the scores the wait would include the loads that `bring` has just sent out.
+#pragma unroll
+    for (int k = 0; k < S::kSteps; ++k) asm volatile("" : "+v"(r.q[k]));
+    // (ahead of a tile's stores, whose end the wait for the loads would include)
+    if (WAVES == 8) bring(j + kAhead);
     const bool ended = j > 0 && unit == units;
     if (ended || j == n) {
       const int64_t slot = begin == 0 && ended ? -1 : 2 * (int64_t)worker + (tiles > 0);
@@ -1037,11 +1142,9 @@ __global__ void __launch_bounds__(64 * WAVES) attend_many_kernel(TileArgs) {
       rows_begin<T, DB>(g, p, row0, r);
     }
     const bool now = key < r.end && key + UNIT > r.beg;
-    if (now) {
-#pragma unroll
-      for (int b = 0; b < NB; ++b) s[b] = scores32<T, DB>(sm, r, kl[kget], 32 * b);
-    }
-    if (WAVES == 8) bring(j + kAhead);
+    f32x16_t s[NB];  // (of this step alone: set where it is read, in no other registers)
+    if (now) scores_unit<T, DB, NB>(r, kl[kget], s);
+    __builtin_amdgcn_s_setprio(0);
     __syncthreads();
     if (WAVES != 8) bring(j + kAhead);
     if (unit + 1 == units && j + 1 < n) {  // the next tile's queries, in the registers that the last scores have left
