@@ -24,6 +24,11 @@ namespace ak {
 namespace {
 
 constexpr int kThreads = 256;
+// Results that the eight L2s of 4 MiB cannot hold are stored past them: 84 MB of
+// queries and keys turned there and back in 65 us (5.2 TB/s), through them in 79
+// (normed too, in 85 and 93). Smaller ones stay for their reader; so does what
+// goes into a cache, 67 us for 133 MB of appended prompts, past the L2s 66.
+constexpr int64_t kL2Bytes = 32 << 20;
 
 // One of the tensors whose heads a call walks over: element strides, the last
 // dimension dense.
@@ -44,6 +49,7 @@ struct HeadArgs {
   int64_t all_heads, total;  // heads of all tensors, rows: tokens times them
   int dim, rotary, lpr_log2;
   int interleaved, inverse, pos64, zero_tail;
+  int past;           // results go past the L2s
   float eps;
   // the cache
   Sequences seq;
@@ -75,13 +81,9 @@ struct Unit {
   __device__ __forceinline__ Unit(int u, const HeadArgs& a) {
     const int ur = a.rotary / (2 * VE);
     turned = u < ur;
-    if (turned) {
-      off0 = a.interleaved ? 2 * u * VE : u * VE;
-      off1 = a.interleaved ? off0 + VE : a.rotary / 2 + u * VE;
-    } else {
-      off0 = a.rotary + 2 * (u - ur) * VE;
-      off1 = off0 + VE;
-    }
+    const bool halves = turned & !a.interleaved;  // else its two vectors are neighbours
+    off0 = halves ? u * VE : 2 * u * VE;
+    off1 = off0 + (halves ? a.rotary / 2 : VE);
     has0 = off0 < a.dim;
     has1 = off1 < a.dim;
   }
@@ -90,20 +92,22 @@ struct Unit {
 // The angles of a unit's VE pairs: cosines and sines (negated for the way back).
 template <int VE>
 __device__ __forceinline__ void load_angles(const HeadArgs& a, int64_t pos, int u, float (&c)[VE], float (&s)[VE]) {
-  if (pos < 0 || pos >= a.table_rows) {
+  Vec16<float> cv[VE / 4], sv[VE / 4];
+  constexpr uint32_t kNaN = 0x7fc00000u;
 #pragma unroll
-    for (int e = 0; e < VE; ++e) c[e] = s[e] = __builtin_nanf("");
-    return;
-  }
-  const float* row = a.table + pos * a.rotary + u * VE;
+  for (int i = 0; i < VE / 4; ++i) cv[i].u = sv[i].u = u32x4{kNaN, kNaN, kNaN, kNaN};
+  if (pos >= 0 && pos < a.table_rows) {
+    const float* row = a.table + pos * a.rotary + u * VE;
 #pragma unroll
-  for (int e = 0; e < VE; e += 4) {
-    const Vec16<float> cv = load16(row + e), sv = load16(row + a.rotary / 2 + e);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      c[e + i] = cv.e[i];
-      s[e + i] = a.inverse ? -sv.e[i] : sv.e[i];
+    for (int i = 0; i < VE / 4; ++i) {
+      cv[i] = load16(row + 4 * i);
+      sv[i] = load16(row + a.rotary / 2 + 4 * i);
     }
+  }
+#pragma unroll
+  for (int e = 0; e < VE; ++e) {
+    c[e] = cv[e / 4].e[e % 4];
+    s[e] = a.inverse ? -sv[e / 4].e[e % 4] : sv[e / 4].e[e % 4];
   }
 }
 
@@ -136,23 +140,23 @@ __device__ __forceinline__ int64_t position_of(const HeadArgs& a, int64_t token)
   return a.pos64 ? static_cast<const int64_t*>(a.positions)[i] : (int64_t)static_cast<const int32_t*>(a.positions)[i];
 }
 
-// What a row of the walk is: its tensor, token and head, where it is read and
-// written, and the position whose angles turn it.
+// What a row of the walk is: its tensor, token and head, and where it is read.
 template <typename T>
 struct Row {
   const T* x;
-  T* y;
   const T* w;
-  int64_t pos;
-  bool write, zero, rotate;
+  int64_t token, h;
+  int kind;
 };
 
-// All lanes of a wave call this together, their rows in ascending order.
+// (field by field: an index would put the arguments into scratch memory)
+#define AK_PICK(f) (kind == 0 ? a.r[0].f : kind == 1 ? a.r[1].f : a.r[2].f)
+
 template <typename T, bool APPEND>
-__device__ __forceinline__ Row<T> row_of(const HeadArgs& a, int64_t row, bool live) {
+__device__ __forceinline__ Row<T> row_of(const HeadArgs& a, int64_t row) {
   Row<T> o;
-  const int64_t token = div_small(row, a.all_heads);
-  int64_t h = row - token * a.all_heads;
+  o.token = div_small(row, a.all_heads);
+  int64_t h = row - o.token * a.all_heads;
   int kind = 0;
   if (h >= a.r[0].heads) {
     h -= a.r[0].heads;
@@ -162,33 +166,49 @@ __device__ __forceinline__ Row<T> row_of(const HeadArgs& a, int64_t row, bool li
       kind = 2;
     }
   }
-  // (field by field: an index would put the arguments into scratch memory)
-#define AK_PICK(f) (kind == 0 ? a.r[0].f : kind == 1 ? a.r[1].f : a.r[2].f)
+  o.h = h;
+  o.kind = kind;
   o.x = static_cast<const T*>(AK_PICK(x)) + h * AK_PICK(sh);
   if (a.inner < a.tokens) {
-    const int64_t outer = div_small(token, a.inner);
-    o.x += outer * AK_PICK(so) + (token - outer * a.inner) * AK_PICK(si);
+    const int64_t outer = div_small(o.token, a.inner);
+    o.x += outer * AK_PICK(so) + (o.token - outer * a.inner) * AK_PICK(si);
   } else {
-    o.x += token * AK_PICK(si);
+    o.x += o.token * AK_PICK(si);
   }
   o.w = static_cast<const T*>(AK_PICK(w));
-  o.y = static_cast<T*>(AK_PICK(y)) + h * AK_PICK(yh);
+  return o;
+}
+
+// Where it is written, and the position whose angles turn it.
+template <typename T>
+struct Target {
+  T* y;
+  int64_t pos;
+  bool write, zero, rotate;
+};
+
+// All lanes of a wave call this together, their rows in ascending order.
+template <typename T, bool APPEND>
+__device__ __forceinline__ Target<T> target_of(const HeadArgs& a, const Row<T>& r, bool live) {
+  Target<T> o;
+  const int kind = r.kind;
+  o.y = static_cast<T*>(AK_PICK(y)) + r.h * AK_PICK(yh);
   o.rotate = kind < 2;
   o.zero = false;
   o.write = live;
   if constexpr (!APPEND) {
-    o.pos = position_of(a, token);
-    o.y += token * AK_PICK(yt);
+    o.pos = position_of(a, r.token);
+    o.y += r.token * AK_PICK(yt);
   } else {
-    const int64_t b = sequence_of(a.seq, token);
+    const int64_t b = sequence_of(a.seq, r.token);
     o.pos = -1;
     if (b >= 0) {
       int64_t first, count;
       sequence_tokens(a.seq, b, first, count);
-      o.pos = (int64_t)a.seq.lengths[b] - count + (token - first);
+      o.pos = (int64_t)a.seq.lengths[b] - count + (r.token - first);
     }
     if (kind == 0) {
-      o.y += token * a.r[0].yt;
+      o.y += r.token * a.r[0].yt;
       o.zero = b < 0;
       o.write = live && (b >= 0 || a.zero_tail);
     } else {
@@ -202,9 +222,9 @@ __device__ __forceinline__ Row<T> row_of(const HeadArgs& a, int64_t row, bool li
       if (o.write) o.y += page * AK_PICK(yt) + slot * AK_PICK(ys);
     }
   }
-#undef AK_PICK
   return o;
 }
+#undef AK_PICK
 
 // Rows of whole vectors: 16-byte aligned, dim a multiple of a vector and the
 // turned part one of two.
@@ -216,11 +236,12 @@ __global__ void __launch_bounds__(kThreads) heads_kernel(HeadArgs a) {
   const Unit<VE> unit(u, a);
   for (int64_t base = (int64_t)blockIdx.x * per; base < a.total; base += (int64_t)gridDim.x * per) {
     const int64_t row = base + (threadIdx.x >> a.lpr_log2);
-    const Row<T> o = row_of<T, APPEND>(a, min(row, a.total - 1), row < a.total);
+    const Row<T> from = row_of<T, APPEND>(a, min(row, a.total - 1));
     Vec16<T> v0, v1;
     v0.u = v1.u = u32x4{0, 0, 0, 0};
-    if (unit.has0) v0 = load16(o.x + unit.off0);
-    if (unit.has1) v1 = load16(o.x + unit.off1);
+    if (unit.has0) v0 = load16(from.x + unit.off0);
+    if (unit.has1) v1 = load16(from.x + unit.off1);
+    const Target<T> o = target_of<T, APPEND>(a, from, row < a.total);  // (its searches while the loads are on their way)
     if (!NORM && APPEND && !o.rotate) {  // values are copied
       if (o.write && unit.has0) store16(o.y + unit.off0, v0);
       if (o.write && unit.has1) store16(o.y + unit.off1, v1);
@@ -237,12 +258,12 @@ __global__ void __launch_bounds__(kThreads) heads_kernel(HeadArgs a) {
 #pragma unroll
       for (int e = 0; e < VE; ++e) ss = fmaf(p[e], p[e], fmaf(q[e], q[e], ss));
       ss = lanes_sum(ss, a.lpr_log2);
-      if (o.w != nullptr) {
+      if (from.w != nullptr) {
         const float inv = 1.0f / sqrtf(ss / (float)a.dim + a.eps);
         Vec16<T> w0, w1;
         w0.u = w1.u = u32x4{0, 0, 0, 0};
-        if (unit.has0) w0 = load16(o.w + unit.off0);
-        if (unit.has1) w1 = load16(o.w + unit.off1);
+        if (unit.has0) w0 = load16(from.w + unit.off0);
+        if (unit.has1) w1 = load16(from.w + unit.off1);
 #pragma unroll
         for (int e = 0; e < VE; ++e) {
           p[e] = p[e] * inv * to_f32(w0.e[e]);
@@ -261,8 +282,13 @@ __global__ void __launch_bounds__(kThreads) heads_kernel(HeadArgs a) {
         v0.e[e] = o.zero ? from_f32<T>(0.0f) : from_f32<T>(p[e]);
         v1.e[e] = o.zero ? from_f32<T>(0.0f) : from_f32<T>(q[e]);
       }
-      if (unit.has0) store16(o.y + unit.off0, v0);
-      if (unit.has1) store16(o.y + unit.off1, v1);
+      if (!APPEND && a.past) {
+        if (unit.has0) store16_nt(o.y + unit.off0, v0);
+        if (unit.has1) store16_nt(o.y + unit.off1, v1);
+      } else {
+        if (unit.has0) store16(o.y + unit.off0, v0);
+        if (unit.has1) store16(o.y + unit.off1, v1);
+      }
     }
   }
 }
@@ -288,21 +314,22 @@ __global__ void __launch_bounds__(kThreads) heads_any_kernel(HeadArgs a) {
   const int lane = threadIdx.x & 63;
   for (int64_t base = (int64_t)blockIdx.x * 4; base < a.total; base += (int64_t)gridDim.x * 4) {
     const int64_t row = base + (threadIdx.x >> 6);
-    const Row<T> o = row_of<T, APPEND>(a, min(row, a.total - 1), row < a.total);
+    const Row<T> from = row_of<T, APPEND>(a, min(row, a.total - 1));
+    const Target<T> o = target_of<T, APPEND>(a, from, row < a.total);
     float inv = 1.0f;
-    const bool norm = NORM && o.w != nullptr;
+    const bool norm = NORM && from.w != nullptr;
     if (norm) {
       float ss = 0.0f;
       for (int d = lane; d < a.dim; d += 64) {
-        const float x = to_f32(o.x[d]);
+        const float x = to_f32(from.x[d]);
         ss = fmaf(x, x, ss);
       }
       inv = 1.0f / sqrtf(wave_sum(ss) / (float)a.dim + a.eps);
     }
     if (!o.write) continue;
     auto value = [&](int d) {
-      const float x = to_f32(o.x[d]);
-      return norm ? x * inv * to_f32(o.w[d]) : x;
+      const float x = to_f32(from.x[d]);
+      return norm ? x * inv * to_f32(from.w[d]) : x;
     };
     const int turned = o.rotate ? a.rotary : 0;
     for (int i = lane; i < turned / 2; i += 64) {
@@ -355,11 +382,13 @@ __device__ __forceinline__ GradRow<T> grad_row_of(const HeadArgs& a, const GradR
           static_cast<const T*>(r.g) + outer * r.go + in * r.gi + h * r.gh, position_of(a, token)};
 }
 
-// A workgroup walks rows of one tensor; its lanes keep their unit, so the
+// A workgroup walks rows of one tensor (four workgroups a CU: the registers are
+// held to 128 for it, [8, 1024, 32 + 8, 128] bf16 forward and back 97 us, of three
+// 117); its lanes keep their unit, so the
 // weight's gradient gathers in registers, then over the workgroup's rows in LDS,
 // then over the workgroups in grad_weight_kernel: fixed orders throughout.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) heads_bwd_kernel(GradArgs ga) {
+__global__ void __launch_bounds__(kThreads, 4) heads_bwd_kernel(GradArgs ga) {
   constexpr int VE = Vec16<T>::VE;
   __shared__ float gather[kThreads * 2 * VE];
   const HeadArgs& a = ga.h;
@@ -429,8 +458,13 @@ __global__ void __launch_bounds__(kThreads) heads_bwd_kernel(GradArgs ga) {
       d1[e] = fmaf(z1[e], a1 * inv, d1[e]);
     }
     T* y = static_cast<T*>(r.dx) + row * a.dim;
-    if (unit.has0) store16(y + unit.off0, y0);
-    if (unit.has1) store16(y + unit.off1, y1);
+    if (a.past) {
+      if (unit.has0) store16_nt(y + unit.off0, y0);
+      if (unit.has1) store16_nt(y + unit.off1, y1);
+    } else {
+      if (unit.has0) store16(y + unit.off0, y0);
+      if (unit.has1) store16(y + unit.off1, y1);
+    }
   }
   if (r.dw == nullptr) return;
   // gather[element of the unit][thread]; then column by column over the row slots
@@ -595,6 +629,7 @@ void launch_heads(HeadArgs& a, bool vec, hipStream_t s) {
           r.yt % VE == 0 && r.ys % VE == 0 && r.yh % VE == 0;
   }
   vec = vec && a.dim % VE == 0 && a.rotary % (2 * VE) == 0 && vec_ok(a.table) && a.lpr_log2 <= 6;
+  a.past = a.total > kL2Bytes / (a.dim * (int64_t)sizeof(T));
   const int64_t per = vec ? kThreads >> a.lpr_log2 : 4;
   const dim3 grid(row_grid((a.total + per - 1) / per)), block(kThreads);
   if (vec) heads_kernel<T, NORM, APPEND><<<grid, block, 0, s>>>(a);
@@ -743,6 +778,7 @@ extern "C" int ak_qk_norm_rotary_bwd(const void* q, const void* k, const void* q
       for (const void* p : {r.x, r.g, r.w, (const void*)r.dx}) vec = vec && ak::vec_ok(p);
       for (int64_t st : {r.so, r.si, r.sh, r.go, r.gi, r.gh}) vec = vec && st % VE == 0;
     }
+    a.past = tokens * (q_heads + k_heads) > ak::kL2Bytes / (dim * (int64_t)sizeof(T));
     if (bq + bk > 0) {
       if (vec) ak::heads_bwd_kernel<T><<<dim3((unsigned)(bq + bk)), dim3(ak::kThreads), 0, s>>>(g);
       else ak::heads_bwd_any_kernel<T><<<dim3((unsigned)(bq + bk)), dim3(ak::kThreads), 0, s>>>(g);

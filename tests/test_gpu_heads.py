@@ -406,6 +406,58 @@ def test_streams_and_graphs():
             assert torch.equal(a, b), (i, j)
 
 
+def test_more_rows_than_a_grid():
+    """Past 2^20 workgroups' rows: positions 0 leave the heads as they are, others turn them."""
+    need_gpu()
+    from kernels.hip import rotary
+    n = 2 ** 22 + 9  # (four a workgroup)
+    say("many rows", n)
+    x = randn(torch.Generator().manual_seed(2), n, 1, 2).to(torch.bfloat16).to(DEV)
+    at = torch.zeros(n, dtype=torch.int32, device=DEV)
+    at[-3:] = 1
+    y = rotary.kernel_fn(x, None, table_of(2, 2).to(DEV), at)[0]
+    assert torch.equal(y[:-3], x[:-3])
+    want = oracle.turn(flat(x[-3:]), *oracle.from_table(table_of(2, 2), torch.ones(3, dtype=torch.long)))
+    close(flat(y[-3:]), want, turn_bound(want, flat(x[-3:]), 2, False, torch.bfloat16))
+
+
+def test_captured_backward():
+    """Forward and backward in one graph, replayed over new values with eager work between."""
+    need_gpu()
+    from kernels.hip import qk_norm_rotary, rotary
+    g = torch.Generator().manual_seed(12)
+    dtype = torch.bfloat16
+    q, k = randn(g, 70, 4, 64).to(dtype).to(DEV), randn(g, 70, 2, 64).to(dtype).to(DEV)
+    wq, wk = ((1 + 0.1 * randn(g, 64)).to(dtype).to(DEV) for _ in range(2))
+    gq, gk = randn(g, 70, 4, 64).to(dtype).to(DEV), randn(g, 70, 2, 64).to(dtype).to(DEV)
+    table = table_of(64, 70).to(DEV)
+    leaves = [t.requires_grad_() for t in (q, k, wq, wk)]
+
+    def step():
+        a, b = qk_norm_rotary.kernel_fn(*leaves, table)
+        c, d = rotary.kernel_fn(a, b, table)
+        return [c, d, *torch.autograd.grad((c, d), leaves, (gq, gk))]
+
+    say("warm")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for i in range(4):
+        say("replay", i)
+        with torch.no_grad():
+            q.copy_(randn(g, 70, 4, 64))
+            gk.copy_(randn(g, 70, 2, 64))
+        want = [t.detach().clone() for t in step()]
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(held, want)), i
+
+
 def test_host_forms():
     """The native host side and the Python one give the same bits, with the same autograd contract."""
     need_gpu()
