@@ -15,106 +15,109 @@
 namespace ak {
 namespace {
 
-// Any type, head dim and alignment: a workgroup for a row (token and query head)
-// and a cut of its keys. A wave takes 64 keys at a time: a lane each for the
-// scores, then a lane for every 64th element of the values' sum. Bound by the
-// strided reads of the keys; fp32 and odd heads come here.
+// What the tiles do not take, heads of more than 256 elements, rows that are not
+// of whole aligned vectors, very many query heads to a key head: a workgroup for
+// a row (token and query head) and a cut of its keys. A wave takes 64 keys at a
+// time: a lane each for the scores, then a lane for every 64th element of the
+// values' sum. Bound by the strided reads of the keys: ANYUS.
 template <typename T>
-__global__ void __launch_bounds__(256) attend_any_kernel(AttendArgs a) {
+__global__ void __launch_bounds__(256) attend_any_kernel(AttendArgs a, int64_t rows) {
   constexpr int kPer = kMaxAttendDim / 64;
   __shared__ float qf[kMaxAttendDim];
   __shared__ float prob[4][64];
   __shared__ float sums[4][kMaxAttendDim];
   __shared__ float stat[4][2];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t row = blockIdx.x;
-  const int64_t token = (uint32_t)row / (uint32_t)a.q_heads;
-  const int h = (int)(row - token * a.q_heads), kvh = h / (a.q_heads / a.kv_heads);
-  const int64_t b = sequence_of(a.seq, token);
-  int64_t lo = 0, hi = 0;
-  if (b >= 0) {
-    int64_t first, count;
-    sequence_tokens(a.seq, b, first, count);
-    const int64_t length = a.seq.lengths[b];
-    keys_of(a, length, length - count + (token - first), lo, hi);
-  }
-  // this workgroup's cut, in whole blocks of 64
-  const int64_t blocks = (hi - lo + 63) / 64;
-  const int64_t end = min(hi, lo + blocks * (blockIdx.y + 1) / a.splits * 64);
-  lo += blocks * blockIdx.y / a.splits * 64;
-  hi = end;
-  const T* q = static_cast<const T*>(a.q) + token * a.q_st + h * a.q_sh;
-  for (int d = threadIdx.x; d < a.dim; d += 256) qf[d] = to_f32(q[d]);
-  __syncthreads();
-  float m = kNegInf, l = 0.0f, acc[kPer];
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) acc[i] = 0.0f;
-  for (int64_t j0 = lo + wave * 64; j0 < hi; j0 += 256) {
-    const int64_t j = j0 + lane;
-    int64_t slot = 0, page = -1;
-    if (j < hi) page = page_of(a, b, j, slot);
-    float s = kNegInf;
-    if (page >= 0) {
-      const T* k = static_cast<const T*>(a.k) + page * a.kp + slot * a.ks + kvh * a.kh;
-      float dot = 0.0f;
-      for (int d = 0; d < a.dim; ++d) dot = fmaf(qf[d], to_f32(k[d]), dot);
-      s = score_of(a, dot);
+  // (a row's sums are read before the next row's first barrier, and written after it)
+  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+    const int64_t token = (uint32_t)row / (uint32_t)a.q_heads;
+    const int h = (int)(row - token * a.q_heads), kvh = h / (a.q_heads / a.kv_heads);
+    const int64_t b = sequence_of(a.seq, token);
+    int64_t lo = 0, hi = 0;
+    if (b >= 0) {
+      int64_t first, count;
+      sequence_tokens(a.seq, b, first, count);
+      const int64_t length = a.seq.lengths[b];
+      keys_of(a, length, length - count + (token - first), lo, hi);
     }
-    const float top = fmaxf(m, wave_max(s));
-    const float p = page >= 0 ? weight_of(s, top) : 0.0f;
-    const float keep = weight_of(m, top);
-    m = top;
-    l = l * keep + p;
-    prob[wave][lane] = p;
-    __builtin_amdgcn_wave_barrier();
+    // this workgroup's cut, in whole blocks of 64
+    const int64_t blocks = (hi - lo + 63) / 64;
+    const int64_t end = min(hi, lo + blocks * (blockIdx.y + 1) / a.splits * 64);
+    lo += blocks * blockIdx.y / a.splits * 64;
+    hi = end;
+    const T* q = static_cast<const T*>(a.q) + token * a.q_st + h * a.q_sh;
+    for (int d = threadIdx.x; d < a.dim; d += 256) qf[d] = to_f32(q[d]);
+    __syncthreads();
+    float m = kNegInf, l = 0.0f, acc[kPer];
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) acc[i] *= keep;
-    uint64_t seen = __ballot(page >= 0);  // masked values take no part, whatever they hold
-    while (seen) {
-      const int x = __builtin_ctzll(seen);
-      seen &= seen - 1;
-      const int64_t vpage = __shfl(page, x), vslot = __shfl(slot, x);
-      const T* v = static_cast<const T*>(a.v) + vpage * a.vp + vslot * a.vs + kvh * a.vh;
-      const float px = prob[wave][x];
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        if (i * 64 < a.dim && i * 64 + lane < a.dim) acc[i] = fmaf(px, to_f32(v[i * 64 + lane]), acc[i]);
+    for (int i = 0; i < kPer; ++i) acc[i] = 0.0f;
+    for (int64_t j0 = lo + wave * 64; j0 < hi; j0 += 256) {
+      const int64_t j = j0 + lane;
+      int64_t slot = 0, page = -1;
+      if (j < hi) page = page_of(a, b, j, slot);
+      float s = kNegInf;
+      if (page >= 0) {
+        const T* k = static_cast<const T*>(a.k) + page * a.kp + slot * a.ks + kvh * a.kh;
+        float dot = 0.0f;
+        for (int d = 0; d < a.dim; ++d) dot = fmaf(qf[d], to_f32(k[d]), dot);
+        s = score_of(a, dot);
       }
+      const float top = fmaxf(m, wave_max(s));
+      const float p = page >= 0 ? weight_of(s, top) : 0.0f;
+      const float keep = weight_of(m, top);
+      m = top;
+      l = l * keep + p;
+      prob[wave][lane] = p;
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) acc[i] *= keep;
+      uint64_t seen = __ballot(page >= 0);  // masked values take no part, whatever they hold
+      while (seen) {
+        const int x = __builtin_ctzll(seen);
+        seen &= seen - 1;
+        const int64_t vpage = __shfl(page, x), vslot = __shfl(slot, x);
+        const T* v = static_cast<const T*>(a.v) + vpage * a.vp + vslot * a.vs + kvh * a.vh;
+        const float px = prob[wave][x];
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+          if (i * 64 < a.dim && i * 64 + lane < a.dim) acc[i] = fmaf(px, to_f32(v[i * 64 + lane]), acc[i]);
+        }
+      }
+      __builtin_amdgcn_wave_barrier();
     }
-    __builtin_amdgcn_wave_barrier();
-  }
-  l = wave_sum(l);
+    l = wave_sum(l);
 #pragma unroll
-  for (int i = 0; i < kPer; ++i)
-    if (i * 64 + lane < a.dim) sums[wave][i * 64 + lane] = acc[i];
-  if (lane == 0) {
-    stat[wave][0] = m;
-    stat[wave][1] = l;
-  }
-  __syncthreads();
-  float top = kNegInf, total = 0.0f, f[4];
+    for (int i = 0; i < kPer; ++i)
+      if (i * 64 + lane < a.dim) sums[wave][i * 64 + lane] = acc[i];
+    if (lane == 0) {
+      stat[wave][0] = m;
+      stat[wave][1] = l;
+    }
+    __syncthreads();
+    float top = kNegInf, total = 0.0f, f[4];
 #pragma unroll
-  for (int w = 0; w < 4; ++w) top = fmaxf(top, stat[w][0]);
+    for (int w = 0; w < 4; ++w) top = fmaxf(top, stat[w][0]);
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    f[w] = weight_of(stat[w][0], top);
-    total += f[w] * stat[w][1];
-  }
-  if (a.splits > 1) {
-    float* part = a.part + (row * a.splits + blockIdx.y) * (a.dim + 2);
+    for (int w = 0; w < 4; ++w) {
+      f[w] = weight_of(stat[w][0], top);
+      total += f[w] * stat[w][1];
+    }
+    if (a.splits > 1) {
+      float* part = a.part + (row * a.splits + blockIdx.y) * (a.dim + 2);
+      for (int d = threadIdx.x; d < a.dim; d += 256)
+        part[d] = f[0] * sums[0][d] + f[1] * sums[1][d] + f[2] * sums[2][d] + f[3] * sums[3][d];
+      if (threadIdx.x == 0) {
+        part[a.dim] = top;
+        part[a.dim + 1] = total;
+      }
+      continue;
+    }
+    if (b < 0 && !a.zero_other) continue;
+    T* out = static_cast<T*>(a.out) + token * a.o_st + h * a.o_sh;
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
     for (int d = threadIdx.x; d < a.dim; d += 256)
-      part[d] = f[0] * sums[0][d] + f[1] * sums[1][d] + f[2] * sums[2][d] + f[3] * sums[3][d];
-    if (threadIdx.x == 0) {
-      part[a.dim] = top;
-      part[a.dim + 1] = total;
-    }
-    return;
+      out[d] = from_f32<T>((f[0] * sums[0][d] + f[1] * sums[1][d] + f[2] * sums[2][d] + f[3] * sums[3][d]) * inv);
   }
-  if (b < 0 && !a.zero_other) return;
-  T* out = static_cast<T*>(a.out) + token * a.o_st + h * a.o_sh;
-  const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-  for (int d = threadIdx.x; d < a.dim; d += 256)
-    out[d] = from_f32<T>((f[0] * sums[0][d] + f[1] * sums[1][d] + f[2] * sums[2][d] + f[3] * sums[3][d]) * inv);
 }
 
 // Joins a row's cuts, a wave a row.
@@ -224,7 +227,7 @@ extern "C" int ak_paged_attention(const void* q, const void* k_cache, const void
   a.splits = batch > 0 ? ak::any_splits(rows, max_keys) : 1;
   auto go = [&](auto t) {
     using T = decltype(t);
-    ak::attend_any_kernel<T><<<dim3((unsigned)rows, (unsigned)a.splits), dim3(256), 0, s>>>(a);
+    ak::attend_any_kernel<T><<<dim3(ak::row_grid(rows), (unsigned)a.splits), dim3(256), 0, s>>>(a, rows);
     if (a.splits > 1) ak::attend_any_join_kernel<T><<<dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s>>>(a, rows);
   };
   if (dtype == AK_DTYPE_F32) go(float());

@@ -32,6 +32,12 @@ CASES = [
     ([9, 1], [20, 31], 16, 2, 1, 66, 0, 0.0),         # heads off the vectors
     ([4], [19], 5, 2, 2, 320, 0, 0.0),                # wide heads
     ([1] * 130, [1 + (37 * i) % 90 for i in range(130)], 16, 4, 2, 64, 0, 0.0),
+    ([1] * 1500, [(7 * i) % 45 for i in range(1500)], 16, 2, 1, 64, 0, 0.0),   # more sequences than one workgroup lines up
+    ([1, 2], [70, 31], 16, 40, 1, 64, 0, 0.0),        # groups past one tile's 32 rows,
+    ([2, 1], [45, 9], 16, 130, 1, 256, 0, 0.0),       # past the tiles of wide heads,
+    ([1, 2], [45, 9], 16, 300, 1, 64, 0, 0.0),        # past every tile
+    ([1, 70], [1503, 901], 16, 4, 2, 64, 333, 20.0),  # a window over many units, cut among workers
+    ([4500], [4500], 16, 1, 1, 64, 40, 0.0),          # (with the hint 1: more tiles than sequences explain)
 ]
 
 
@@ -198,6 +204,26 @@ def test_scores_at_the_edges(dtype):
     k3[place[3]][:] = 0.0
     got = run(q3, k3, vc, scale=1.0)
     close(got, vc[place[3]].double().expand(4, 2, 64), torch.zeros(4, 2, 64), "lowest")
+
+
+@pytest.mark.parametrize("dim", [4, 8])
+def test_more_rows_than_a_grid(dim):
+    """Past 2^20 rows, of which each sees its own key alone: the values come back as they are."""
+    need_gpu()
+    from kernels.hip.paged_attention import kernel_fn
+    counts, page, dtype = [2 ** 20 + 77, 0, 300], 64, torch.bfloat16
+    say("many rows", dim)
+    pages, lens, starts, total = make_batch(counts, counts, page, 4)
+    g = torch.Generator().manual_seed(4)
+    q = torch.randn(sum(counts) + 1, 1, dim, generator=g).to(dtype).to(DEV)
+    kc, vc = (torch.randn(total, page, 1, dim, generator=g).to(dtype).to(DEV) for _ in range(2))
+    pages = pages.to(DEV)
+    got = kernel_fn(q, kc, vc, pages, lens.to(DEV), starts.to(DEV), window=1)
+    place = torch.arange(counts[0], device=DEV)
+    assert torch.equal(got[:counts[0]], vc[pages[0, place // page].long(), place % page])
+    place = torch.arange(counts[2], device=DEV)
+    assert torch.equal(got[counts[0]:-1], vc[pages[2, place // page].long(), place % page])
+    assert not got[-1].any()
 
 
 def test_bad_pages_and_batches():
