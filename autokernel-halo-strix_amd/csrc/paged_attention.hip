@@ -189,8 +189,8 @@ extern "C" int ak_paged_attention(const void* q, const void* k_cache, const void
       !ak::extent_ok(n_pages, kc_sp, page_size, kc_ss, kv_heads, kc_sh, dim, esz) ||
       !ak::extent_ok(n_pages, vc_sp, page_size, vc_ss, kv_heads, vc_sh, dim, esz))
     return ak_set_error(AK_ERR_INVALID_ARG, "%s: bad shape or strides", name);
-  if (!(scale > 0.0f) || scale > 1e18f || !(softcap >= 0.0f) || softcap > 1e18f || window < 0)
-    return ak_set_error(AK_ERR_INVALID_ARG, "%s: scale must be positive, softcap and window not negative", name);
+  if (!(scale >= 1e-18f && scale <= 1e18f) || !(softcap == 0.0f || (softcap >= 1e-3f && softcap <= 1e4f)) || window < 0)
+    return ak_set_error(AK_ERR_INVALID_ARG, "%s: scale must be 1e-18 to 1e18, softcap 0 or 1e-3 to 1e4, window not negative", name);
   if (tokens == 0) return AK_OK;
   if (!q || !out || (n_pages && (!k_cache || !v_cache))) return ak_set_error(AK_ERR_INVALID_ARG, "%s: null pointer", name);
   const int64_t max_keys = max_pages * page_size;

@@ -37,6 +37,10 @@ CASES = [
     ([2, 1], [45, 9], 16, 130, 1, 256, 0, 0.0),       # past the tiles of wide heads,
     ([1, 2], [45, 9], 16, 300, 1, 64, 0, 0.0),        # past every tile
     ([1, 70], [1503, 901], 16, 4, 2, 64, 333, 20.0),  # a window over many units, cut among workers
+    ([5, 1], [90, 33], 16, 2, 1, 128, 0, 0.001),      # caps from the smallest
+    ([5, 1], [90, 33], 16, 2, 1, 128, 0, 256.0),
+    ([5, 1], [90, 33], 16, 2, 1, 128, 0, 300.0),
+    ([5, 1], [90, 33], 16, 2, 1, 66, 0, 10000.0),     # to the largest
     ([4500], [4500], 16, 1, 1, 64, 40, 0.0),          # (with the hint 1: more tiles than sequences explain)
 ]
 
