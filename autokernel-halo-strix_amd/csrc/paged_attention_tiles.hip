@@ -400,7 +400,7 @@ __device__ __forceinline__ f32x16_t scores32(const ScoreMath& sm, const Rows<T, 
 // 2 softcap / (exp(2 x) + 1), whose first term a softmax does not see. Its error of up to
 // 4 softcap 2^-24 is absolute, 2^-14 at most, a quarter of a weight's rounding; others take
 // the form with small results' own precision. (16 sequences of up to 7000 keys, chunks of up
-// to 500 tokens, 32 + 8 heads of 128: 361 us, in the other form 458.)
+// to 500 tokens, 32 + 8 heads of 128: 361 us, in the other form 458 (each beside the other).)
 constexpr float kQuickCap = 256.0f;
 
 template <typename T>
@@ -414,20 +414,24 @@ __device__ __forceinline__ void cap32(const ScoreMath& sm, f32x16_t& s) {
   }
 }
 
+// The scores of keys that are not seen: the seen ones' bits first, then two operations a
+// score on constants (compared one by one, the places held 30 registers through the loop).
 template <typename T, int DB>
 __device__ __forceinline__ void hide32(const Rows<T, DB>& r, f32x16_t& s, int key0, uint32_t seen) {
   const int half = (threadIdx.x & 63) >> 5;
+  const auto below = [&](int key) { return (uint32_t)((1ull << max(0, min(key - key0, 32))) - 1); };
+  const uint32_t bits = (seen & below(r.hi) & ~below(r.lo)) >> (4 * half);
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
-    const int j = 8 * (i / 4) + 4 * half + i % 4, key = key0 + j;
-    if (key >= r.hi || key < r.lo || !((seen >> j) & 1)) s[i] = kNegInf;
+    const uint32_t keep = (uint32_t)((int32_t)(bits << (31 - (8 * (i / 4) + i % 4))) >> 31);
+    s[i] = __uint_as_float((__float_as_uint(s[i]) & keep) | (0xff800000u & ~keep));
   }
 }
 
 // The maximum that the weights are taken beside, over N x 32 new scores. It follows the
 // true one at a distance of up to 2^kLag: weights of up to 2^kLag are as exact as weights
 // of up to 1, and most units then leave what is summed up alone (raised at every new
-// maximum, [4, 4096 ..] prompts took 709 us, with the lag LAGUS).
+// maximum, [4, 4096 ..] prompts took 709 us, with the lag 663).
 constexpr float kLag = 8.0f;
 
 template <typename T, int DB, int N>
@@ -511,7 +515,7 @@ __device__ __forceinline__ void values32(Rows<T, DB>& r, const Weights<T>& p, co
 // The same for a unit of NB x 32 keys, for the matrix phase of the many-row kernel: the
 // operands of a group of four MFMAs are read while the group before runs, and the compiler is
 // kept from moving the reads back to their uses (it reads two operands, waits for them and
-// uses them: [4, 4096 ..] prompts PINUS and UNPINUS us).
+// uses them: [4, 4096 ..] prompts 531 us, left to the compiler 544).
 __device__ __forceinline__ void pinned() { __builtin_amdgcn_sched_barrier(0); }
 
 template <typename T, int DB, int NB>
@@ -1117,13 +1121,14 @@ __global__ void __launch_bounds__(64 * WAVES) attend_many_kernel(TileArgs) {
   for (int j = 0;; ++j) {
     __builtin_amdgcn_s_setprio(1);  // the matrix cores' wave first
     if (before) {
+      const int spoilt = bad[vget];  // (on its way during the products)
       if constexpr (sizeof(T) == 2) {
         values_unit<T, DB, NB>(r, w, vl[vget]);
       } else {
 #pragma unroll
         for (int b = 0; b < NB; ++b) values32<T, DB>(r, w[b], vl[vget], 32 * b);
       }
-      if (uniform(bad[vget]) == j) {
+      if (uniform(spoilt) == j) {
         const uint64_t seen = seen_of(j - 1);
         for (int b = 0; b < NB; ++b) add_not_finite<T, DB>(g, p, r, key - UNIT + 32 * b, (uint32_t)(seen >> (32 * b)));
       }
