@@ -19,42 +19,56 @@ struct Sequences {
 
 // The first new token of sequence b and the number of them, inside the call's
 // tokens whatever `starts` holds.
-__device__ __forceinline__ void sequence_tokens(const Sequences& s, int64_t b, int64_t& first, int64_t& count) {
+__device__ __forceinline__ void sequence_tokens(const Sequences& s, int b, int& first, int& count) {
   if (s.starts == nullptr) {
-    first = b * s.per;
-    count = s.per;
+    first = b * (int)s.per;
+    count = (int)s.per;
     return;
   }
-  const int64_t a = s.starts[b], e = s.starts[b + 1];
-  first = min(max(a, (int64_t)0), s.tokens);
-  count = max(min(e, s.tokens) - first, (int64_t)0);
+  const int tokens = (int)s.tokens;
+  first = min(max(s.starts[b], 0), tokens);
+  count = max(min(s.starts[b + 1], tokens) - first, 0);
 }
 
 // The sequence of token t (the last b with starts[b] <= t), or -1 where none has
 // it. All lanes of the wave search for their own t together: 64 starts at a time
 // narrow the lowest lane's sequence down, the others walk on from there (their
 // tokens follow it).
-__device__ __forceinline__ int64_t sequence_of(const Sequences& s, int64_t t) {
-  if (s.batch == 0) return -1;
+__device__ __forceinline__ int sequence_of(const Sequences& s, int t) {
+  const int batch = (int)s.batch;
+  if (batch == 0) return -1;
   if (s.starts == nullptr) return (uint32_t)t / (uint32_t)s.per;
   const int lane = threadIdx.x & 63;
-  const int64_t t0 = ((int64_t)__builtin_amdgcn_readfirstlane((int)(t >> 32)) << 32) |
-                     (uint32_t)__builtin_amdgcn_readfirstlane((int)t);
-  int64_t lo = 0, n = s.batch;  // starts[lo] <= t0 (or lo = 0), starts[lo + n] > t0 (or the end)
+  const int t0 = __builtin_amdgcn_readfirstlane(t);
+  uint32_t lo = 0, n = batch;  // starts[lo] <= t0 (or lo = 0), starts[lo + n] > t0 (or the end)
   while (n > 1) {
-    const int64_t step = (n + 63) / 64;
-    const int64_t i = lo + lane * step;
-    const bool le = lane * step < n && s.starts[i] <= t0;
+    const uint32_t step = (n + 63) / 64, at = lane * step;
+    const bool le = at < n && s.starts[lo + at] <= t0;
     const uint64_t hit = __ballot(le);
-    const int last = hit ? 63 - __builtin_clzll(hit) : 0;
-    const int64_t nlo = lo + last * step;
-    n = min(step, lo + n - nlo);
-    lo = nlo;
+    const uint32_t last = (hit ? 63 - __builtin_clzll(hit) : 0) * step;
+    lo += last;
+    n = min(step, n - last);
   }
-  int64_t b = lo;
-  while (b + 1 < s.batch && s.starts[b + 1] <= t) ++b;
-  return s.starts[b] <= t && t < s.starts[b + 1] ? b : -1;
+  int b = (int)lo;
+  int first = s.starts[b], next = s.starts[b + 1];
+  while (next <= t && b + 1 < batch) {
+    ++b;
+    first = next;
+    next = s.starts[b + 1];
+  }
+  return first <= t && t < next ? b : -1;
 }
+
+// Division by a number of up to 32 bits that a launch knows.
+struct Divisor {
+  uint32_t d, magic;  // 2^32 / d, rounded down
+  Divisor() = default;
+  explicit Divisor(int64_t n) : d((uint32_t)n), magic((uint32_t)(n < 2 ? UINT32_MAX : ((uint64_t)1 << 32) / (uint64_t)n)) {}
+  __device__ __forceinline__ uint32_t operator()(uint32_t x) const {
+    const uint32_t q = __umulhi(x, magic);  // the quotient or one less
+    return x - q * d >= d ? q + 1 : q;
+  }
+};
 
 // Whether (outer, inner, heads) rows of dim elements at these strides stay
 // addressable with signed 64-bit byte offsets.

@@ -47,20 +47,26 @@ struct HeadArgs {
   const void* positions;
   int64_t tokens, inner, n_positions, table_rows;
   int64_t all_heads, total;  // heads of all tensors, rows: tokens times them
+  Divisor by_heads, by_inner, by_positions, by_page;  // for whole vectors' rows, where all numbers have 32 bits
   int dim, rotary, lpr_log2;
   int interleaved, inverse, pos64, zero_tail;
   int past;           // results go past the L2s
-  float eps;
+  float eps, by_dim;  // by_dim: 1 / dim
   // the cache
   Sequences seq;
   const int32_t* pages;
   int64_t n_pages, page_size, max_pages, ld_pages;
 };
 
-__device__ __forceinline__ int64_t div_small(int64_t a, int64_t b) {
+// Rows are counted in 64 bits, or where the numbers allow it in 32: in 64 their places
+// took more than half of the instructions (appended prompts 67 us, in 32 53).
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b, const Divisor&) {
   if (((a | b) >> 32) == 0) return (uint32_t)a / (uint32_t)b;
   return a / b;
 }
+__device__ __forceinline__ uint32_t quotient(uint32_t a, int64_t, const Divisor& by) { return by(a); }
+__device__ __forceinline__ int64_t steps(int64_t n, int64_t stride) { return n * stride; }
+__device__ __forceinline__ int64_t steps(uint32_t n, int64_t stride) { return (int64_t)((uint64_t)n * (uint32_t)stride); }
 
 // The sum over the 2^log2 lanes of a row (aligned to their number).
 __device__ __forceinline__ float lanes_sum(float v, int log2) {
@@ -90,14 +96,14 @@ struct Unit {
 };
 
 // The angles of a unit's VE pairs: cosines and sines (negated for the way back).
-template <int VE>
+template <int VE, bool INVERSE>
 __device__ __forceinline__ void load_angles(const HeadArgs& a, int64_t pos, int u, float (&c)[VE], float (&s)[VE]) {
   Vec16<float> cv[VE / 4], sv[VE / 4];
   constexpr uint32_t kNaN = 0x7fc00000u;
 #pragma unroll
   for (int i = 0; i < VE / 4; ++i) cv[i].u = sv[i].u = u32x4{kNaN, kNaN, kNaN, kNaN};
   if (pos >= 0 && pos < a.table_rows) {
-    const float* row = a.table + pos * a.rotary + u * VE;
+    const float* row = a.table + steps((uint32_t)pos, a.rotary) + u * VE;
 #pragma unroll
     for (int i = 0; i < VE / 4; ++i) {
       cv[i] = load16(row + 4 * i);
@@ -107,7 +113,7 @@ __device__ __forceinline__ void load_angles(const HeadArgs& a, int64_t pos, int 
 #pragma unroll
   for (int e = 0; e < VE; ++e) {
     c[e] = cv[e / 4].e[e % 4];
-    s[e] = a.inverse ? -sv[e / 4].e[e % 4] : sv[e / 4].e[e % 4];
+    s[e] = INVERSE && a.inverse ? -sv[e / 4].e[e % 4] : sv[e / 4].e[e % 4];
   }
 }
 
@@ -134,46 +140,47 @@ __device__ __forceinline__ void turn(float (&p)[VE], float (&q)[VE], const float
   }
 }
 
-__device__ __forceinline__ int64_t position_of(const HeadArgs& a, int64_t token) {
-  const int64_t i = token < a.n_positions ? token : token - div_small(token, a.n_positions) * a.n_positions;
+template <typename I>
+__device__ __forceinline__ int64_t position_of(const HeadArgs& a, I token) {
+  const I n = (I)a.n_positions, i = token < n ? token : token - quotient(token, a.n_positions, a.by_positions) * n;
   if (a.positions == nullptr) return i;
   return a.pos64 ? static_cast<const int64_t*>(a.positions)[i] : (int64_t)static_cast<const int32_t*>(a.positions)[i];
 }
 
 // What a row of the walk is: its tensor, token and head, and where it is read.
-template <typename T>
+template <typename T, typename I>
 struct Row {
   const T* x;
   const T* w;
-  int64_t token, h;
+  I token, h;
   int kind;
 };
 
 // (field by field: an index would put the arguments into scratch memory)
 #define AK_PICK(f) (kind == 0 ? a.r[0].f : kind == 1 ? a.r[1].f : a.r[2].f)
 
-template <typename T, bool APPEND>
-__device__ __forceinline__ Row<T> row_of(const HeadArgs& a, int64_t row) {
-  Row<T> o;
-  o.token = div_small(row, a.all_heads);
-  int64_t h = row - o.token * a.all_heads;
+template <typename T, bool APPEND, typename I>
+__device__ __forceinline__ Row<T, I> row_of(const HeadArgs& a, I row) {
+  Row<T, I> o;
+  o.token = quotient(row, a.all_heads, a.by_heads);
+  I h = row - o.token * (I)a.all_heads;
   int kind = 0;
-  if (h >= a.r[0].heads) {
-    h -= a.r[0].heads;
+  if (h >= (I)a.r[0].heads) {
+    h -= (I)a.r[0].heads;
     kind = 1;
-    if (APPEND && h >= a.r[1].heads) {
-      h -= a.r[1].heads;
+    if (APPEND && h >= (I)a.r[1].heads) {
+      h -= (I)a.r[1].heads;
       kind = 2;
     }
   }
   o.h = h;
   o.kind = kind;
-  o.x = static_cast<const T*>(AK_PICK(x)) + h * AK_PICK(sh);
-  if (a.inner < a.tokens) {
-    const int64_t outer = div_small(o.token, a.inner);
-    o.x += outer * AK_PICK(so) + (o.token - outer * a.inner) * AK_PICK(si);
+  o.x = static_cast<const T*>(AK_PICK(x)) + steps(h, AK_PICK(sh));
+  if (!APPEND && a.inner < a.tokens) {
+    const I outer = quotient(o.token, a.inner, a.by_inner);
+    o.x += steps(outer, AK_PICK(so)) + steps(o.token - outer * (I)a.inner, AK_PICK(si));
   } else {
-    o.x += o.token * AK_PICK(si);
+    o.x += steps(o.token, AK_PICK(si));
   }
   o.w = static_cast<const T*>(AK_PICK(w));
   return o;
@@ -188,38 +195,40 @@ struct Target {
 };
 
 // All lanes of a wave call this together, their rows in ascending order.
-template <typename T, bool APPEND>
-__device__ __forceinline__ Target<T> target_of(const HeadArgs& a, const Row<T>& r, bool live) {
+template <typename T, bool APPEND, typename I>
+__device__ __forceinline__ Target<T> target_of(const HeadArgs& a, const Row<T, I>& r, bool live) {
   Target<T> o;
   const int kind = r.kind;
-  o.y = static_cast<T*>(AK_PICK(y)) + r.h * AK_PICK(yh);
+  o.y = static_cast<T*>(AK_PICK(y)) + steps(r.h, AK_PICK(yh));
   o.rotate = kind < 2;
   o.zero = false;
   o.write = live;
   if constexpr (!APPEND) {
     o.pos = position_of(a, r.token);
-    o.y += r.token * AK_PICK(yt);
+    o.y += steps(r.token, AK_PICK(yt));
   } else {
-    const int64_t b = sequence_of(a.seq, r.token);
-    o.pos = -1;
+    const int token = (int)r.token, b = sequence_of(a.seq, token);
+    int pos = -1;
     if (b >= 0) {
-      int64_t first, count;
+      int first, count;
       sequence_tokens(a.seq, b, first, count);
-      o.pos = (int64_t)a.seq.lengths[b] - count + (r.token - first);
+      pos = max(a.seq.lengths[b], 0) - (count - (token - first));
     }
+    o.pos = pos;
     if (kind == 0) {
-      o.y += r.token * a.r[0].yt;
+      o.y += steps(r.token, a.r[0].yt);
       o.zero = b < 0;
       o.write = live && (b >= 0 || a.zero_tail);
     } else {
-      int64_t page = -1, slot = 0;
-      if (o.pos >= 0) {
-        const int64_t i = div_small(o.pos, a.page_size);
-        slot = o.pos - i * a.page_size;
+      int page = -1;
+      uint32_t slot = 0;
+      if (pos >= 0) {
+        const uint32_t i = a.by_page(pos);
+        slot = pos - i * (uint32_t)a.page_size;
         if (i < a.max_pages) page = a.pages[b * a.ld_pages + i];
       }
       o.write = live && page >= 0 && page < a.n_pages;
-      if (o.write) o.y += page * AK_PICK(yt) + slot * AK_PICK(ys);
+      if (o.write) o.y += steps((I)page, AK_PICK(yt)) + steps((I)slot, AK_PICK(ys));
     }
   }
   return o;
@@ -234,14 +243,15 @@ __global__ void __launch_bounds__(kThreads) heads_kernel(HeadArgs a) {
   const int lpr = 1 << a.lpr_log2, per = kThreads >> a.lpr_log2;
   const int u = threadIdx.x & (lpr - 1);
   const Unit<VE> unit(u, a);
-  for (int64_t base = (int64_t)blockIdx.x * per; base < a.total; base += (int64_t)gridDim.x * per) {
-    const int64_t row = base + (threadIdx.x >> a.lpr_log2);
-    const Row<T> from = row_of<T, APPEND>(a, min(row, a.total - 1));
+  const uint32_t total = (uint32_t)a.total;  // (and a walk's step more stays in 32 bits)
+  for (uint32_t base = blockIdx.x * per; base < total; base += gridDim.x * per) {
+    const uint32_t row = base + (threadIdx.x >> a.lpr_log2);
+    const Row<T, uint32_t> from = row_of<T, APPEND>(a, min(row, total - 1));
     Vec16<T> v0, v1;
     v0.u = v1.u = u32x4{0, 0, 0, 0};
     if (unit.has0) v0 = load16(from.x + unit.off0);
     if (unit.has1) v1 = load16(from.x + unit.off1);
-    const Target<T> o = target_of<T, APPEND>(a, from, row < a.total);  // (its searches while the loads are on their way)
+    const Target<T> o = target_of<T, APPEND>(a, from, row < total);  // (its searches while the loads are on their way)
     if (!NORM && APPEND && !o.rotate) {  // values are copied
       if (o.write && unit.has0) store16(o.y + unit.off0, v0);
       if (o.write && unit.has1) store16(o.y + unit.off1, v1);
@@ -259,7 +269,7 @@ __global__ void __launch_bounds__(kThreads) heads_kernel(HeadArgs a) {
       for (int e = 0; e < VE; ++e) ss = fmaf(p[e], p[e], fmaf(q[e], q[e], ss));
       ss = lanes_sum(ss, a.lpr_log2);
       if (from.w != nullptr) {
-        const float inv = 1.0f / sqrtf(ss / (float)a.dim + a.eps);
+        const float inv = 1.0f / sqrtf(ss * a.by_dim + a.eps);
         Vec16<T> w0, w1;
         w0.u = w1.u = u32x4{0, 0, 0, 0};
         if (unit.has0) w0 = load16(from.w + unit.off0);
@@ -273,15 +283,16 @@ __global__ void __launch_bounds__(kThreads) heads_kernel(HeadArgs a) {
     }
     if (unit.turned && o.rotate) {
       float c[VE], s[VE];
-      load_angles<VE>(a, o.pos, u, c, s);
+      load_angles<VE, !APPEND>(a, o.pos, u, c, s);
       turn<VE>(p, q, c, s, a.interleaved);
     }
     if (o.write) {
 #pragma unroll
       for (int e = 0; e < VE; ++e) {
-        v0.e[e] = o.zero ? from_f32<T>(0.0f) : from_f32<T>(p[e]);
-        v1.e[e] = o.zero ? from_f32<T>(0.0f) : from_f32<T>(q[e]);
+        v0.e[e] = from_f32<T>(p[e]);
+        v1.e[e] = from_f32<T>(q[e]);
       }
+      if (APPEND && o.zero) v0.u = v1.u = u32x4{0, 0, 0, 0};
       if (!APPEND && a.past) {
         if (unit.has0) store16_nt(o.y + unit.off0, v0);
         if (unit.has1) store16_nt(o.y + unit.off1, v1);
@@ -314,7 +325,7 @@ __global__ void __launch_bounds__(kThreads) heads_any_kernel(HeadArgs a) {
   const int lane = threadIdx.x & 63;
   for (int64_t base = (int64_t)blockIdx.x * 4; base < a.total; base += (int64_t)gridDim.x * 4) {
     const int64_t row = base + (threadIdx.x >> 6);
-    const Row<T> from = row_of<T, APPEND>(a, min(row, a.total - 1));
+    const Row<T, int64_t> from = row_of<T, APPEND>(a, min(row, a.total - 1));
     const Target<T> o = target_of<T, APPEND>(a, from, row < a.total);
     float inv = 1.0f;
     const bool norm = NORM && from.w != nullptr;
@@ -356,6 +367,7 @@ struct GradRows {
   int64_t go, gi, gh;    // of g
   int64_t heads, rows;
   int first_block, blocks;
+  Divisor by_heads;
 };
 
 struct GradArgs {
@@ -370,16 +382,16 @@ struct GradRow {
   int64_t pos;
 };
 
-template <typename T>
-__device__ __forceinline__ GradRow<T> grad_row_of(const HeadArgs& a, const GradRows& r, int64_t row) {
-  const int64_t token = div_small(row, r.heads), h = row - token * r.heads;
-  int64_t outer = 0, in = token;
+template <typename T, typename I>
+__device__ __forceinline__ GradRow<T> grad_row_of(const HeadArgs& a, const GradRows& r, I row) {
+  const I token = quotient(row, r.heads, r.by_heads), h = row - token * (I)r.heads;
+  I outer = 0, in = token;
   if (a.inner < a.tokens) {
-    outer = div_small(token, a.inner);
-    in = token - outer * a.inner;
+    outer = quotient(token, a.inner, a.by_inner);
+    in = token - outer * (I)a.inner;
   }
-  return {static_cast<const T*>(r.x) + outer * r.so + in * r.si + h * r.sh,
-          static_cast<const T*>(r.g) + outer * r.go + in * r.gi + h * r.gh, position_of(a, token)};
+  return {static_cast<const T*>(r.x) + steps(outer, r.so) + steps(in, r.si) + steps(h, r.sh),
+          static_cast<const T*>(r.g) + steps(outer, r.go) + steps(in, r.gi) + steps(h, r.gh), position_of(a, token)};
 }
 
 // A workgroup walks rows of one tensor (four workgroups a CU: the registers are
@@ -411,10 +423,11 @@ __global__ void __launch_bounds__(kThreads, 4) heads_bwd_kernel(GradArgs ga) {
       d0[e] = d1[e] = 0.0f;
     }
   }
-  for (int64_t base = (int64_t)((int)blockIdx.x - r.first_block) * per; base < r.rows; base += (int64_t)r.blocks * per) {
-    const int64_t row = base + slot;
-    const bool live = row < r.rows;
-    const GradRow<T> o = grad_row_of<T>(a, r, min(row, r.rows - 1));
+  const uint32_t rows = (uint32_t)r.rows;
+  for (uint32_t base = (blockIdx.x - r.first_block) * per; base < rows; base += r.blocks * per) {
+    const uint32_t row = base + slot;
+    const bool live = row < rows;
+    const GradRow<T> o = grad_row_of<T>(a, r, min(row, rows - 1));
     Vec16<T> x0, x1, g0, g1;
     x0.u = x1.u = g0.u = g1.u = u32x4{0, 0, 0, 0};
     if (live && unit.has0) {
@@ -433,7 +446,7 @@ __global__ void __launch_bounds__(kThreads, 4) heads_bwd_kernel(GradArgs ga) {
     }
     if (unit.turned) {
       float c[VE], s[VE];
-      load_angles<VE>(a, o.pos, u, c, s);
+      load_angles<VE, true>(a, o.pos, u, c, s);
       turn<VE>(z0, z1, c, s, a.interleaved);
     }
     float ss = 0.0f, gx = 0.0f;
@@ -446,18 +459,18 @@ __global__ void __launch_bounds__(kThreads, 4) heads_bwd_kernel(GradArgs ga) {
     ss = lanes_sum(ss, a.lpr_log2);
     gx = lanes_sum(gx, a.lpr_log2);
     if (!live) continue;
-    const float inv = 1.0f / sqrtf(ss / (float)a.dim + a.eps);
-    const float back = inv * inv * (gx / (float)a.dim);
+    const float inv = 1.0f / sqrtf(ss * a.by_dim + a.eps);
+    const float back = inv * (gx * a.by_dim);  // (of order one, as n is, whatever the size of x)
     Vec16<T> y0, y1;
 #pragma unroll
     for (int e = 0; e < VE; ++e) {
-      const float a0 = to_f32(x0.e[e]), a1 = to_f32(x1.e[e]);
-      y0.e[e] = from_f32<T>(inv * (z0[e] * w0[e] - a0 * back));
-      y1.e[e] = from_f32<T>(inv * (z1[e] * w1[e] - a1 * back));
-      d0[e] = fmaf(z0[e], a0 * inv, d0[e]);
-      d1[e] = fmaf(z1[e], a1 * inv, d1[e]);
+      const float n0 = to_f32(x0.e[e]) * inv, n1 = to_f32(x1.e[e]) * inv;
+      y0.e[e] = from_f32<T>(inv * fmaf(z0[e], w0[e], -(n0 * back)));
+      y1.e[e] = from_f32<T>(inv * fmaf(z1[e], w1[e], -(n1 * back)));
+      d0[e] = fmaf(z0[e], n0, d0[e]);
+      d1[e] = fmaf(z1[e], n1, d1[e]);
     }
-    T* y = static_cast<T*>(r.dx) + row * a.dim;
+    T* y = static_cast<T*>(r.dx) + steps(row, a.dim);
     if (a.past) {
       if (unit.has0) store16_nt(y + unit.off0, y0);
       if (unit.has1) store16_nt(y + unit.off1, y1);
@@ -625,10 +638,18 @@ void launch_heads(HeadArgs& a, bool vec, hipStream_t s) {
   a.lpr_log2 = lanes_log2(a.dim, a.rotary, VE);
   for (const HeadRows& r : a.r) {
     if (r.heads == 0) continue;
+    for (int64_t st : {r.heads > 1 ? r.sh : 0, r.heads > 1 ? r.yh : 0, r.si, r.so, r.yt, r.ys}) vec = vec && st <= (int64_t)UINT32_MAX;
     vec = vec && vec_ok(r.x) && vec_ok(r.y) && vec_ok(r.w) && r.so % VE == 0 && r.si % VE == 0 && r.sh % VE == 0 &&
           r.yt % VE == 0 && r.ys % VE == 0 && r.yh % VE == 0;
   }
   vec = vec && a.dim % VE == 0 && a.rotary % (2 * VE) == 0 && vec_ok(a.table) && a.lpr_log2 <= 6;
+  // (2^30 rows, of 32 bytes at least, and the last step of a walk)
+  vec = vec && a.total <= 1 << 30 && a.table_rows <= INT32_MAX;
+  a.by_heads = Divisor(a.all_heads);
+  a.by_inner = Divisor(a.inner);
+  a.by_positions = Divisor(a.n_positions);
+  a.by_page = Divisor(a.page_size);
+  a.by_dim = 1.0f / (float)a.dim;
   a.past = a.total > kL2Bytes / (a.dim * (int64_t)sizeof(T));
   const int64_t per = vec ? kThreads >> a.lpr_log2 : 4;
   const dim3 grid(row_grid((a.total + per - 1) / per)), block(kThreads);
@@ -695,7 +716,7 @@ extern "C" int ak_qk_norm_rotary_fwd(const void* q, const void* k, const void* q
   a.positions = positions;
   a.tokens = tokens;
   a.inner = inner;
-  a.n_positions = n_positions;
+  a.n_positions = std::min(n_positions, tokens);
   a.table_rows = table_rows;
   a.all_heads = q_heads + k_heads;
   a.total = tokens * a.all_heads;
@@ -759,7 +780,7 @@ extern "C" int ak_qk_norm_rotary_bwd(const void* q, const void* k, const void* q
   a.positions = positions;
   a.tokens = tokens;
   a.inner = inner;
-  a.n_positions = n_positions;
+  a.n_positions = std::min(n_positions, tokens);
   a.table_rows = table_rows;
   a.dim = (int)dim;
   a.rotary = (int)rotary;
@@ -776,8 +797,14 @@ extern "C" int ak_qk_norm_rotary_bwd(const void* q, const void* k, const void* q
     for (const ak::GradRows& r : g.r) {
       if (r.heads == 0) continue;
       for (const void* p : {r.x, r.g, r.w, (const void*)r.dx}) vec = vec && ak::vec_ok(p);
-      for (int64_t st : {r.so, r.si, r.sh, r.go, r.gi, r.gh}) vec = vec && st % VE == 0;
+      for (int64_t st : {r.so, r.si, r.sh, r.go, r.gi, r.gh}) vec = vec && st % VE == 0 && st <= (int64_t)UINT32_MAX;
+      vec = vec && r.rows <= 1 << 30;
     }
+    for (ak::GradRows& r : g.r) r.by_heads = ak::Divisor(r.heads);
+    vec = vec && table_rows <= INT32_MAX;
+    a.by_inner = ak::Divisor(a.inner);
+    a.by_positions = ak::Divisor(a.n_positions);
+    a.by_dim = 1.0f / (float)dim;
     a.past = tokens * (q_heads + k_heads) > ak::kL2Bytes / (dim * (int64_t)sizeof(T));
     if (bq + bk > 0) {
       if (vec) ak::heads_bwd_kernel<T><<<dim3((unsigned)(bq + bk)), dim3(ak::kThreads), 0, s>>>(g);

@@ -32,10 +32,10 @@ __global__ void __launch_bounds__(256) attend_any_kernel(AttendArgs a, int64_t r
   for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
     const int64_t token = (uint32_t)row / (uint32_t)a.q_heads;
     const int h = (int)(row - token * a.q_heads), kvh = h / (a.q_heads / a.kv_heads);
-    const int64_t b = sequence_of(a.seq, token);
+    const int b = sequence_of(a.seq, (int)token);
     int64_t lo = 0, hi = 0;
     if (b >= 0) {
-      int64_t first, count;
+      int first, count;
       sequence_tokens(a.seq, b, first, count);
       const int64_t length = a.seq.lengths[b];
       keys_of(a, length, length - count + (token - first), lo, hi);
@@ -127,7 +127,7 @@ __global__ void __launch_bounds__(256) attend_any_join_kernel(AttendArgs a, int6
   const int64_t row = min((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), rows - 1);  // (the last row more than once)
   const int64_t token = (uint32_t)row / (uint32_t)a.q_heads;
   const int h = (int)(row - token * a.q_heads);
-  if (sequence_of(a.seq, token) < 0 && !a.zero_other) return;
+  if (sequence_of(a.seq, (int)token) < 0 && !a.zero_other) return;
   const float* part = a.part + row * a.splits * (a.dim + 2);
   float top = kNegInf, total = 0.0f;
   for (int s = 0; s < a.splits; ++s) top = fmaxf(top, part[(int64_t)s * (a.dim + 2) + a.dim]);

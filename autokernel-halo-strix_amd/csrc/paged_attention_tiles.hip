@@ -709,7 +709,7 @@ __device__ __forceinline__ void zero_other_rows(Args g, int wave, int waves) {
   const Sequences s{g->a.seq.starts, g->a.seq.lengths, g->a.seq.batch, g->a.seq.tokens, g->a.seq.per};
   const int lane = threadIdx.x & 63;
   for (int64_t t = wave; t < s.tokens; t += waves) {
-    if (sequence_of(s, t) >= 0) continue;
+    if (sequence_of(s, (int)t) >= 0) continue;
     T* out = static_cast<T*>(g->a.out) + t * g->a.o_st;
     for (int h = 0; h < g->a.q_heads; ++h)
       for (int d = lane; d < g->a.dim; d += 64) out[h * g->a.o_sh + d] = from_f32<T>(0.0f);

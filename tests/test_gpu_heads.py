@@ -421,6 +421,29 @@ def test_more_rows_than_a_grid():
     close(flat(y[-3:]), want, turn_bound(want, flat(x[-3:]), 2, False, torch.bfloat16))
 
 
+def test_strides_past_32_bits():
+    """Two tokens 2^32 + 8 elements apart, forward and back, against the same ones side by side."""
+    need_gpu()
+    from kernels.hip import qk_norm_rotary, rotary
+    say("far strides")
+    g = torch.Generator().manual_seed(3)
+    near = randn(g, 2, 1, 64).to(torch.bfloat16).to(DEV)
+    room = torch.empty(2 ** 32 + 8 + 64, dtype=torch.bfloat16, device=DEV)
+    far = room.as_strided((2, 1, 64), (2 ** 32 + 8, 64, 1))
+    far.copy_(near)
+    w, table = (1 + 0.1 * randn(g, 64)).to(torch.bfloat16).to(DEV), table_of(64, 2).to(DEV)
+    assert torch.equal(rotary.kernel_fn(far, None, table)[0], rotary.kernel_fn(near, None, table)[0])
+    grads = []
+    for x in (far, near):
+        x, w1 = x.detach().requires_grad_(), w.detach().requires_grad_()
+        y = qk_norm_rotary.kernel_fn(x, None, w1, None, table)[0]
+        grads.append([y.detach(), *torch.autograd.grad(y, (x, w1), x.detach())])
+    # (their sums are taken in another order: both are half a step from sums of up to 64 products
+    # of at most 32, a rounding in fp32 each)
+    for a, b in zip(*grads):
+        close(a, b.cpu(), 2.1 * half_eps(torch.bfloat16) * b.cpu().double().abs() + 2 * 64 * 32 * E)
+
+
 def test_captured_backward():
     """Forward and backward in one graph, replayed over new values with eager work between."""
     need_gpu()
