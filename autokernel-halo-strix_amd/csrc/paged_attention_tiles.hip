@@ -263,10 +263,12 @@ template <typename T, int DB>
 struct Shape {
   static constexpr int VE = Vec16<T>::VE;
   static constexpr int kChunks = DB / VE;            // 16-byte chunks of a row
-  // Rows in LDS are a chunk (K: a column of chunks is read) or two (V: two chunks of four
-  // rows are read together) longer than their values, which spreads them over the banks.
+  // Rows in LDS are a chunk (K: a column of chunks is read) or more (V: four chunks of four
+  // rows are read together) longer than their values, which spreads them over the banks: four
+  // leave V without conflicts, two with one in three reads twice as long, but room for two
+  // workgroups of few rows a CU (of many rows prompts 533 us with two, 524 with four).
   static constexpr int kRowBytes = DB * (int)sizeof(T);
-  static constexpr int kPitch = kRowBytes + 16, vPitch = kRowBytes + 32;
+  static constexpr int kPitch = kRowBytes + 16, vPitch = kRowBytes + 32, vWidePitch = kRowBytes + 64;
   static constexpr int kPerLoad = 64 / kChunks;      // rows of one load of a wave
   static constexpr int kSteps = DB / (2 * VE);       // operand steps of a score
   static constexpr int kBlocks = DB / 32;            // blocks of 32 values
@@ -482,30 +484,30 @@ __device__ __forceinline__ Weights<T> weights32(const ScoreMath& sm, Rows<T, DB>
 }
 
 // O^T += V^T P^T of 32 keys.
-template <typename T, int DB>
+template <typename T, int DB, int PITCH>
 __device__ __forceinline__ void values32(Rows<T, DB>& r, const Weights<T>& p, const char* vl, int row0) {
   using S = Shape<T, DB>;
   const int lane = threadIdx.x & 63, half = lane >> 5;
   if constexpr (sizeof(T) == 2) {
     // lane group q of 16 reads rows 4 (q / 2) + 0 .. 3 and 8 further on, columns 16 (q % 2) on
     const int j = lane & 15;
-    const char* base = vl + (row0 + 4 * half + (j >> 2)) * S::vPitch + 32 * ((lane >> 4) & 1) + 8 * (j & 3);
+    const char* base = vl + (row0 + 4 * half + (j >> 2)) * PITCH + 32 * ((lane >> 4) & 1) + 8 * (j & 3);
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
 #pragma unroll
       for (int blk = 0; blk < S::kBlocks; ++blk) {
-        const u32x2 x = lds_tr(base + 16 * kb * S::vPitch + 64 * blk);
-        const u32x2 y = lds_tr(base + (16 * kb + 8) * S::vPitch + 64 * blk);
+        const u32x2 x = lds_tr(base + 16 * kb * PITCH + 64 * blk);
+        const u32x2 y = lds_tr(base + (16 * kb + 8) * PITCH + 64 * blk);
         r.o[blk] = mfma32(T(), u32x4{x[0], x[1], y[0], y[1]}, p.w[kb], r.o[blk]);
       }
     }
   } else {
-    const char* base = vl + (row0 + 4 * half) * S::vPitch + 4 * (lane & 31);
+    const char* base = vl + (row0 + 4 * half) * PITCH + 4 * (lane & 31);
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
 #pragma unroll
       for (int blk = 0; blk < S::kBlocks; ++blk) {
-        const float v = *reinterpret_cast<const float*>(base + (8 * (i / 4) + i % 4) * S::vPitch + 128 * blk);
+        const float v = *reinterpret_cast<const float*>(base + (8 * (i / 4) + i % 4) * PITCH + 128 * blk);
         r.o[blk] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, __uint_as_float(p.w[i / 4][i % 4]), r.o[blk], 0, 0, 0);
       }
     }
@@ -552,15 +554,15 @@ __device__ __forceinline__ void values_unit(Rows<T, DB>& r, const Weights<T> (&p
   static_assert(sizeof(T) == 2, "fp32 takes values32");
   constexpr int G = S::kBlocks < 4 ? S::kBlocks : 4, kGroups = NB * 2 * S::kBlocks / G;
   const int lane = threadIdx.x & 63, j = lane & 15;
-  const char* base = vl + (4 * (lane >> 5) + (j >> 2)) * S::vPitch + 32 * ((lane >> 4) & 1) + 8 * (j & 3);
+  const char* base = vl + (4 * (lane >> 5) + (j >> 2)) * S::vWidePitch + 32 * ((lane >> 4) & 1) + 8 * (j & 3);
   u32x2 x[2][G], y[2][G];
   auto read = [&](int g) {
 #pragma unroll
     for (int i = 0; i < G; ++i) {
       const int at = g * G + i;
-      const char* from = base + 16 * (at / S::kBlocks) * S::vPitch + 64 * (at % S::kBlocks);
+      const char* from = base + 16 * (at / S::kBlocks) * S::vWidePitch + 64 * (at % S::kBlocks);
       x[g % 2][i] = lds_tr(from);
-      y[g % 2][i] = lds_tr(from + 8 * S::vPitch);
+      y[g % 2][i] = lds_tr(from + 8 * S::vWidePitch);
     }
   };
   read(0);
@@ -771,7 +773,7 @@ __device__ __forceinline__ bool partly_seen(Args g, const Place& p, int key0, in
 // The K and V rows of a unit, as N loads of a wave each: load i takes rows first + i *
 // stride .. + kPerLoad - 1. Rows that are not there are loaded from the cache's first place:
 // their keys are hidden, their values become zeros on the way into LDS.
-template <typename T, int DB, int N>
+template <typename T, int DB, int N, int PITCH>
 struct Loads {
   using S = Shape<T, DB>;
   u32x4 at[N];      // the rows' places, read from the table before they are needed
@@ -802,7 +804,7 @@ struct Loads {
     const int lane = threadIdx.x & 63;
     const int row = first + lane / S::kChunks, chunk = lane % S::kChunks;
     char* kd = kl + row * S::kPitch + 16 * chunk;
-    char* vd = vl + row * S::vPitch + 16 * chunk;
+    char* vd = vl + row * PITCH + 16 * chunk;
     uint32_t found = 0;
     if (gaps) {
 #pragma unroll
@@ -822,7 +824,7 @@ struct Loads {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       *reinterpret_cast<u32x4*>(kd + i * stride * S::kPitch) = k[i];
-      *reinterpret_cast<u32x4*>(vd + i * stride * S::vPitch) = v[i];
+      *reinterpret_cast<u32x4*>(vd + i * stride * PITCH) = v[i];
     }
     return found != 0;
   }
@@ -921,7 +923,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, DB * sizeof(T) <= 256 ? 2 : 1)
   char* const vl = lds[wave] + 32 * S::kPitch;
   const ScoreMath sm = score_math(g);
   const Cache cache = cache_of<T, DB>(g);
-  Loads<T, DB, N> x;
+  Loads<T, DB, N, S::vPitch> x;
   LookUp next;
   Rows<T, DB> r;
   if (g->a.dim < DB) clear_lds(kl, 32 * (S::kPitch + S::vPitch), lane, 64);
@@ -956,7 +958,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, DB * sizeof(T) <= 256 ? 2 : 1)
       if (sm.cap) cap32<T>(sm, s[0]);
       if (mask) hide32<T, DB>(r, s[0], key, now);
       new_maximum<T, DB, 1>(sm, r, s);
-      values32<T, DB>(r, weights32<T, DB>(sm, r, s[0]), vl, 0);
+      values32<T, DB, S::vPitch>(r, weights32<T, DB>(sm, r, s[0]), vl, 0);
       if (__any(bad)) add_not_finite<T, DB>(g, p, r, key, now);
     }
     left -= n;
@@ -1002,7 +1004,7 @@ __global__ void __launch_bounds__(64 * WAVES) attend_many_kernel(TileArgs) {
   constexpr int kTable = 16, kLead = WAVES == 8 ? 1 : 2, kFinish = 2;
   static_assert(WAVES == 8 || WAVES == 4, "rounds divide the table");
   __shared__ __attribute__((aligned(16))) char kl[kSlots][UNIT * S::kPitch];
-  __shared__ __attribute__((aligned(16))) char vl[vSlots][UNIT * S::vPitch];
+  __shared__ __attribute__((aligned(16))) char vl[vSlots][UNIT * S::vWidePitch];
   __shared__ u32x4 table[kTable][UNIT];
   __shared__ uint32_t there[2 * kTable][4];      // of a unit: the bits of its keys that are there; 1: partly seen, 2: not all there
   __shared__ int bad[vSlots];                    // the unit (by count) whose values are not all finite
@@ -1071,7 +1073,7 @@ __global__ void __launch_bounds__(64 * WAVES) attend_many_kernel(TileArgs) {
     const uint32_t* t = there[j % (2 * kTable)];
     return (uint64_t)(uint32_t)uniform(t[1]) << 32 | (uint32_t)uniform(t[0]);
   };
-  Loads<T, DB, N> x;
+  Loads<T, DB, N, S::vWidePitch> x;
   int kput = 0, vput = 0;  // the slots that are stored next
   uint32_t flags = 0;      // of the unit that is stored next
   auto prepare = [&](int j) {
@@ -1126,7 +1128,7 @@ __global__ void __launch_bounds__(64 * WAVES) attend_many_kernel(TileArgs) {
         values_unit<T, DB, NB>(r, w, vl[vget]);
       } else {
 #pragma unroll
-        for (int b = 0; b < NB; ++b) values32<T, DB>(r, w[b], vl[vget], 32 * b);
+        for (int b = 0; b < NB; ++b) values32<T, DB, S::vWidePitch>(r, w[b], vl[vget], 32 * b);
       }
       if (uniform(spoilt) == j) {
         const uint64_t seen = seen_of(j - 1);
