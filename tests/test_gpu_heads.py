@@ -545,3 +545,109 @@ def test_host_forms():
     version = caches[0]._version
     paged_append.kernel_fn(k.detach().view(18, 2, 64), k.detach().view(18, 2, 64), *caches, pages, lens, starts)
     assert caches[0]._version > version
+
+
+def training_calls():
+    from kernels.hip import qk_norm_rotary, rotary
+    g = torch.Generator().manual_seed(21)
+    dtype = torch.bfloat16
+    q, k = randn(g, 2, 9, 4, 64).to(dtype).to(DEV), randn(g, 2, 9, 2, 64).to(dtype).to(DEV)
+    wq, wk = ((1 + 0.1 * randn(g, 64)).to(dtype).to(DEV) for _ in range(2))
+    table, at = table_of(32, 40).to(DEV), torch.randint(0, 40, (2, 9), generator=g).to(DEV)
+    return {
+        "rotary": ((q, k), lambda q, k: rotary.kernel_fn(q, k, table, at)),
+        "rotary one": ((q,), lambda q: rotary.kernel_fn(q, None, table)[:1]),
+        "norm": ((q, k, wq, wk), lambda q, k, wq, wk: qk_norm_rotary.kernel_fn(q, k, wq, wk, table, at)),
+        "norm one": ((q, wq), lambda q, wq: qk_norm_rotary.kernel_fn(q, None, wq, None)[:1]),
+    }
+
+
+CALLS = ["rotary", "rotary one", "norm", "norm one"]
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_under_torch_compile(name):
+    need_gpu()
+    import torch._dynamo
+    import torch._dynamo.compiled_autograd as compiled
+    leaves, fn = training_calls()[name]
+    say("compile", name)
+    leaves = [a.requires_grad_() for a in leaves]
+    loss = lambda outs: sum((o.float() * o.detach().float()).sum() for o in outs)  # noqa: E731
+    outs = fn(*leaves)
+    want = [*outs, *torch.autograd.grad(loss(outs), leaves)]
+    torch._dynamo.reset()
+    outs = torch.compile(fn, backend="eager")(*leaves)
+    got = [*outs, *torch.autograd.grad(loss(outs), leaves)]
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    total = loss(fn(*leaves))
+    with compiled._enable(torch.compile(backend="eager")):
+        total.backward()
+    torch._dynamo.reset()
+    for a, b in zip(leaves, want[len(outs):]):
+        assert torch.equal(a.grad, b)
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_forward_mode_is_refused(name):
+    need_gpu()
+    import torch.autograd.forward_ad as fw
+    leaves, fn = training_calls()[name]
+    say("forward mode", name)
+    for i in range(len(leaves)):
+        for grad_mode in (True, False):
+            with fw.dual_level(), torch.set_grad_enabled(grad_mode):
+                args = list(leaves)
+                args[i] = fw.make_dual(args[i], torch.ones_like(args[i]))
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    fn(*args)
+
+
+@pytest.mark.parametrize("name", ["rotary", "norm"])
+def test_parts_of_the_gradient(name):
+    """A loss of one output, a gradient of one leaf, tensors saved on the host, two backward passes."""
+    need_gpu()
+    leaves, fn = training_calls()[name]
+    say("parts", name)
+    leaves = [a.requires_grad_() for a in leaves]
+    up = [torch.randn_like(a) for a in leaves[:2]]
+    outs = fn(*leaves)
+    both = torch.autograd.grad(outs, leaves, up, retain_graph=True)
+    for i in (0, 1):
+        alone = torch.autograd.grad(outs[i], leaves, up[i], retain_graph=True, allow_unused=True)
+        for j, (a, b) in enumerate(zip(alone, both)):
+            if j % 2 == i:
+                assert torch.equal(a, b)
+            else:
+                assert a is None or not a.any()
+    for i, leaf in enumerate(leaves):
+        assert torch.equal(torch.autograd.grad(outs, leaf, up, retain_graph=True)[0], both[i])
+        rest = [a.detach() if a is not leaf else a for a in leaves]
+        o = fn(*rest)
+        used = [(x, u) for x, u in zip(o, up) if x.requires_grad]
+        assert torch.equal(torch.autograd.grad([x for x, _ in used], leaf, [u for _, u in used])[0], both[i])
+    with torch.autograd.graph.save_on_cpu():
+        o = fn(*leaves)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(o, leaves, up), both))
+
+
+def test_serving_under_torch_compile():
+    need_gpu()
+    import torch._dynamo
+    from kernels.hip import paged_append, paged_attention
+    say("compile", "serving")
+    g = torch.Generator().manual_seed(22)
+    x = randn(g, 18, 8, 64).to(torch.bfloat16).to(DEV)
+    table = table_of(64, 40).to(DEV)
+    pages, lens, starts, total = (t.to(DEV) if isinstance(t, torch.Tensor) else t for t in make_batch([12, 6], [20, 6], 8, 17))
+
+    def step(x, kc, vc):
+        q = paged_append.kernel_fn(x[:, 4:6], x[:, 6:], kc, vc, pages, lens, starts, q=x[:, :4], table=table)
+        return paged_attention.kernel_fn(q, kc, vc, pages, lens, starts)
+
+    made = []
+    for fn in (step, torch.compile(step, backend="eager")):
+        caches = [torch.zeros(total, 8, 2, 64, dtype=x.dtype, device=DEV) for _ in range(2)]
+        made.append([fn(x, *caches), *caches])
+    torch._dynamo.reset()
+    assert all(torch.equal(a, b) for a, b in zip(*made))
