@@ -41,6 +41,7 @@ struct TileArgs {
   int unit, rows;                  // keys of a unit, rows of a tile
   int workers, min_units;
   uint32_t kp, ks, vp, vs;         // cache strides in bytes: page, slot
+  float join_cost;                 // of a part, in a unit's time, over the number of tiles
   int64_t* line;                   // [batch + 1]: the units before each sequence
   Job* jobs;                       // [workers]
   float* part;                     // [2 workers]: sums of products, maxima, sums of a tile's rows
@@ -118,9 +119,13 @@ __device__ __forceinline__ Span span_of(Args g, const Seq& s, int t) {
 
 __device__ __forceinline__ int tiles_of(Args g, const Seq& s) { return (s.count + g->per_tile - 1) / g->per_tile; }
 
-// Workers that a line of `total` units keeps busy; worker w has [begin(w), begin(w + 1)).
+// Workers that a line of `total` units keeps busy; worker w has [begin(w), begin(w + 1)). A
+// tile of n units takes n / parts of a unit's time and then parts times join_cost of it to be
+// joined, least at units of sqrt(n join_cost) a part: 7 tokens over 69571 keys of one head took
+// 226 us with a worker a unit, so 35; 4 tokens over 20284 keys 160 and 31.
 __device__ __forceinline__ int64_t active_workers(Args g, int64_t total) {
-  return max(min((int64_t)g->workers, total / g->min_units), (int64_t)1);
+  const int64_t least = max((int64_t)g->min_units, (int64_t)sqrtf((float)total * g->join_cost));
+  return max(min((int64_t)g->workers, total / least), (int64_t)1);
 }
 __device__ __forceinline__ int64_t begin_of(int64_t w, int64_t total, int64_t n) { return w * total / n; }
 __device__ __forceinline__ int64_t worker_of(int64_t u, int64_t total, int64_t n) { return ((u + 1) * n - 1) / total; }
@@ -838,6 +843,13 @@ __device__ __forceinline__ void clear_lds(char* to, int bytes, int thread, int t
 // ---------------------------------------------------------------------------
 // Few rows: a wave is a worker
 // ---------------------------------------------------------------------------
+// Bound by the cache's bytes, each read once: a wave loads a unit of 32 keys' K and V while
+// it works on the one before, whose rows it has looked up a unit earlier. Of a tile of up to
+// 32 rows the matrix cores do mostly nothing (a decode step has the group's heads), and are
+// free. [64 sequences of 2048 to 8192 keys, 32 + 8 heads of 128] bf16 264 us, 5.1 TB/s, where
+// reads alone reach 6.0; two of 130001 keys 180, 4.8 TB/s with the join. Rows of 512 bytes
+// leave registers for one workgroup a CU, and still: 25 x 1882 keys, 4 heads of 256, bf16 51
+// us, in tiles of many rows 70.
 constexpr int kFewWaves = 4;
 
 template <typename T, int DB>
@@ -990,6 +1002,14 @@ __global__ void __launch_bounds__(64 * kFewWaves, DB * sizeof(T) <= 256 ? 2 : 1)
 // runs a phase late, so that on every SIMD one wave feeds the matrix cores while the other
 // computes weights. (Four waves of long rows have a SIMD each: all in one phase, and the
 // stores after the barrier, which saves a slot.)
+//
+// Bound by what surrounds the products: prompts of up to 4096 tokens, 32 + 8 heads of 128 bf16,
+// 490 to 500 us, 750 TFLOP/s where a product of 8192^3 reaches 1420. Of a step's 5600 cycles
+// (1.9 GHz under this load) a SIMD's matrix cores take 2050. The matrix phase has 900 for O^T's
+// products, 750 for the stores, loads and places of units ahead, 300 for tiles' ends, 660 for
+// the scores, the vector phase 1340 for weights and 530 for look-ups. A first unit's operands
+// read before the barrier, loads sent out in the vector phase, tiles of 64 rows a wave, two
+// workgroups of four waves a CU: all the same or slower.
 template <typename T, int DB, int WAVES, int UNIT>
 __global__ void __launch_bounds__(64 * WAVES) attend_many_kernel(TileArgs) {
   using S = Shape<T, DB>;
@@ -1200,23 +1220,25 @@ __global__ void __launch_bounds__(64 * WAVES) attend_many_kernel(TileArgs) {
 // ---------------------------------------------------------------------------
 // Joining the parts: a job for each worker whose last tile goes on in the next one
 // ---------------------------------------------------------------------------
+// Of many rows: a workgroup for 32 of them, the parts over its waves, then wave 0 takes the
+// others' sums in their order.
 template <typename T, int DB>
 __global__ void __launch_bounds__(256) attend_join_many_kernel(TileArgs) {
+  typedef float f32x2_v __attribute__((ext_vector_type(2)));
+  __shared__ f32x4_v sums[3][DB / 8][64];
+  __shared__ f32x2_v stats[3][64];
   const Args g = kernel_args();
-  const int lane = threadIdx.x & 63, wave = blockIdx.y * 4 + uniform(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), block = blockIdx.y;
   const Job job = g->jobs[blockIdx.x];
-  const int row = wave * kRows + (lane & 31);
-  if (wave * kRows >= job.rows) return;
+  const int row = block * kRows + (lane & 31);
+  if (block * kRows >= job.rows) return;
   const bool mine = row < job.rows;
   f32x16_t o[DB / 32];
 #pragma unroll
   for (int b = 0; b < DB / 32; ++b) o[b] = f32x16_t{};
   float top = kNegInf, sum = 0.0f;
-  for (int i = 0; i < job.parts; ++i) {
-    const float* x = wave_part<DB>(g, i == 0 ? job.first : 2 * ((int64_t)blockIdx.x + i), wave);
-    typedef float f32x2_v __attribute__((ext_vector_type(2)));
-    f32x2_v ml = {kNegInf, 0.0f};  // (lanes without a row left nothing)
-    if (mine) ml = *reinterpret_cast<const f32x2_v*>(x + 32 * DB + 2 * lane);
+  // adds (ml, what `from` gives) to the sums
+  const auto add = [&](f32x2_v ml, auto from) {
     const float now = fmaxf(top, ml[0]);
     const float keep = now == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(top - now), f = now == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(ml[0] - now);
     top = now;
@@ -1225,12 +1247,30 @@ __global__ void __launch_bounds__(256) attend_join_many_kernel(TileArgs) {
     for (int b = 0; b < DB / 32; ++b)
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        f32x4_v v = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (mine) v = *reinterpret_cast<const f32x4_v*>(x + ((b * 4 + c) * 64 + lane) * 4);
+        const f32x4_v v = from(b * 4 + c);
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[b][4 * c + e] = o[b][4 * c + e] * keep + v[e] * f;
       }
+  };
+  for (int i = wave; i < job.parts; i += 4) {
+    const float* x = wave_part<DB>(g, i == 0 ? job.first : 2 * ((int64_t)blockIdx.x + i), block);
+    f32x2_v ml = {kNegInf, 0.0f};  // (lanes without a row left nothing)
+    if (mine) ml = *reinterpret_cast<const f32x2_v*>(x + 32 * DB + 2 * lane);
+    add(ml, [&](int at) {
+      f32x4_v v = {0.0f, 0.0f, 0.0f, 0.0f};
+      if (mine) v = *reinterpret_cast<const f32x4_v*>(x + (at * 64 + lane) * 4);
+      return v;
+    });
   }
+  if (wave > 0) {
+    stats[wave - 1][lane] = f32x2_v{top, sum};
+#pragma unroll
+    for (int at = 0; at < DB / 8; ++at)
+      sums[wave - 1][at][lane] = f32x4_v{o[at / 4][4 * (at % 4)], o[at / 4][4 * (at % 4) + 1], o[at / 4][4 * (at % 4) + 2], o[at / 4][4 * (at % 4) + 3]};
+  }
+  __syncthreads();
+  if (wave > 0) return;
+  for (int w = 0; w < min(job.parts - 1, 3); ++w) add(stats[w][lane], [&](int at) { return sums[w][at][lane]; });
   rows_out<T, DB>(g, job.token, job.head, row, mine, o, sum);
 }
 
@@ -1329,6 +1369,7 @@ struct Plan {
   bool few, lined, cut;
   int padded, waves, unit, per_tile, rows, min_units;
   int64_t workers;
+  float join_cost;
   size_t line_bytes, job_bytes, part_bytes;
 };
 
@@ -1340,7 +1381,7 @@ Plan plan_of(int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads, i
   p.padded = dim <= 64 ? 64 : dim <= 128 ? 128 : 256;
   max_chunk = std::min(max_chunk, tokens);
   const bool wide = p.padded * (f32 ? 4 : 2) > 256;  // rows past 256 bytes: half the waves and keys
-  p.few = max_chunk * group <= kRows && p.padded < 256;
+  p.few = max_chunk * group <= kRows && p.padded * (f32 ? 4 : 2) <= 512;
   p.waves = p.few || wide ? 4 : 8;
   p.unit = p.few || wide ? 32 : 64;
   const int64_t rows = p.few ? kRows : kRows * p.waves;
@@ -1357,7 +1398,11 @@ Plan plan_of(int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads, i
   const int64_t useful = most > 1e9 ? (int64_t)1 << 30 : (int64_t)most / p.min_units + 1;
   p.workers = std::min(groups * (p.few ? kFewWaves : 1), useful);
   if (p.few) p.workers = (p.workers + kFewWaves - 1) / kFewWaves * kFewWaves;
-  p.cut = p.workers > 8 * kv_heads * (tokens / p.per_tile);
+  const int64_t tiles = kv_heads * std::max(tokens / p.per_tile, (int64_t)1);
+  p.cut = p.workers > 8 * tiles;
+  // (measured: half and double of either cost do the same to drawn calls, on the average; units of
+  // fp32 take four times as long)
+  p.join_cost = (p.few ? 0.02f * (float)((p.rows + 15) / 16) : 0.2f) / (f32 ? 4.0f : 1.0f) / (float)tiles;
   p.line_bytes = (size_t)(batch + 2) / 2 * 16;
   p.job_bytes = (size_t)p.workers * sizeof(Job);
   const size_t part = p.few ? (size_t)p.rows * (size_t)(p.padded + 2) : (size_t)((p.rows + 31) / 32) * 32 * (size_t)(p.padded + 4);
@@ -1368,7 +1413,7 @@ Plan plan_of(int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads, i
 template <typename T, int DB>
 void launch_tiles(const TileArgs& g, const Plan& p, hipStream_t s) {
   if (p.lined) attend_line_kernel<<<dim3(1), dim3(1024), 0, s>>>(g);
-  if constexpr (DB < 256) {
+  if constexpr (DB * sizeof(T) <= 512) {
     if (p.few) attend_few_kernel<T, DB><<<dim3((unsigned)(p.workers / kFewWaves)), dim3(64 * kFewWaves), 0, s>>>(g, p.lined);
   }
   if (!p.few) {
@@ -1377,9 +1422,9 @@ void launch_tiles(const TileArgs& g, const Plan& p, hipStream_t s) {
   }
   if (p.workers > 1) {
     const unsigned jobs = (unsigned)(p.workers - 1);
-    if (!p.few) attend_join_many_kernel<T, DB><<<dim3(jobs, (unsigned)((p.rows + 127) / 128)), dim3(256), 0, s>>>(g);
-    // (of few rows in many parts a row a workgroup)
-    else attend_join_kernel<T, DB><<<dim3(jobs, (unsigned)(p.cut ? std::min(p.rows, 4) : 1)), dim3(256), 0, s>>>(g);
+    if (!p.few) attend_join_many_kernel<T, DB><<<dim3(jobs, (unsigned)((p.rows + 31) / 32)), dim3(256), 0, s>>>(g);
+    // (of few rows in many parts a row a workgroup, up to 16: with 4 the two calls above took 59 and 50 us)
+    else attend_join_kernel<T, DB><<<dim3(jobs, (unsigned)(p.cut ? std::min(p.rows, 16) : 1)), dim3(256), 0, s>>>(g);
   }
 }
 
@@ -1420,6 +1465,7 @@ void attend_tiles(const AttendArgs& a, int64_t max_chunk, int dtype, void* works
   g.rows = p.rows;
   g.workers = (int)p.workers;
   g.min_units = p.min_units;
+  g.join_cost = p.join_cost;
   const uint32_t esz = (uint32_t)ak_dtype_size(dtype);
   g.kp = (uint32_t)a.kp * esz;
   g.ks = (uint32_t)a.ks * esz;
