@@ -236,7 +236,10 @@ __device__ __forceinline__ Target<T> target_of(const HeadArgs& a, const Row<T, I
 #undef AK_PICK
 
 // Rows of whole vectors: 16-byte aligned, dim a multiple of a vector and the
-// turned part one of two.
+// turned part one of two. [8, 1024, 32 + 8, 128] bf16 turned 28 us (6.0 TB/s), normed
+// and turned 30 (5.6); prompts of 9730 tokens, 32 + 8 + 8 heads of 128 fp16, into a cache
+// 50 (4.9). A decode step is one launch of 4 us. Two or four rows a thread at a
+// time, or fewer workgroups that read a row ahead: the same or slower.
 template <typename T, bool NORM, bool APPEND>
 __global__ void __launch_bounds__(kThreads) heads_kernel(HeadArgs a) {
   constexpr int VE = Vec16<T>::VE;
@@ -319,14 +322,17 @@ __device__ __forceinline__ void angle_at(const HeadArgs& a, int64_t pos, int i, 
   }
 }
 
-// Every other row: a wave each, one element or pair a lane at a time.
-template <typename T, bool NORM, bool APPEND>
+// Every other row: a wave each, one element or pair a lane at a time. Bound by its narrow
+// loads: [8, 1024, 32 + 8, 128] bf16 with 44 elements turned takes 94 us, whole vectors (64
+// turned) 28; forward and back with the norm 541 and 88.
+template <typename T, bool NORM, bool APPEND, typename I>
 __global__ void __launch_bounds__(kThreads) heads_any_kernel(HeadArgs a) {
   const int lane = threadIdx.x & 63;
-  for (int64_t base = (int64_t)blockIdx.x * 4; base < a.total; base += (int64_t)gridDim.x * 4) {
-    const int64_t row = base + (threadIdx.x >> 6);
-    const Row<T, int64_t> from = row_of<T, APPEND>(a, min(row, a.total - 1));
-    const Target<T> o = target_of<T, APPEND>(a, from, row < a.total);
+  const I total = (I)a.total;
+  for (I base = (I)blockIdx.x * 4; base < total; base += (I)gridDim.x * 4) {
+    const I row = base + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // (places are the wave's: scalar work)
+    const Row<T, I> from = row_of<T, APPEND>(a, min(row, total - 1));
+    const Target<T> o = target_of<T, APPEND>(a, from, row < total);
     float inv = 1.0f;
     const bool norm = NORM && from.w != nullptr;
     if (norm) {
@@ -394,11 +400,11 @@ __device__ __forceinline__ GradRow<T> grad_row_of(const HeadArgs& a, const GradR
           static_cast<const T*>(r.g) + steps(outer, r.go) + steps(in, r.gi) + steps(h, r.gh), position_of(a, token)};
 }
 
-// A workgroup walks rows of one tensor (four workgroups a CU: the registers are
-// held to 128 for it, [8, 1024, 32 + 8, 128] bf16 forward and back 97 us, of three
-// 117); its lanes keep their unit, so the
-// weight's gradient gathers in registers, then over the workgroup's rows in LDS,
-// then over the workgroups in grad_weight_kernel: fixed orders throughout.
+// A workgroup walks rows of one tensor; its lanes keep their unit, so the weight's
+// gradient gathers in registers, then over the workgroup's rows in LDS, then over
+// the workgroups in grad_weight_kernel: fixed orders throughout. [8, 1024, 32 + 8,
+// 128] bf16 43 us (5.8 TB/s) and 4 for the weights, of 88 forward and back. The
+// registers are held to 128 for four workgroups a CU: with three it was 117 for 97.
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 4) heads_bwd_kernel(GradArgs ga) {
   constexpr int VE = Vec16<T>::VE;
@@ -505,7 +511,7 @@ __global__ void __launch_bounds__(kThreads) heads_bwd_any_kernel(GradArgs ga) {
   const bool second = (int)blockIdx.x >= ga.r[1].first_block;
   const GradRows r = second ? ga.r[1] : ga.r[0];
   const T* w = static_cast<const T*>(r.w);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   float* mine = gather[wave];
   for (int d = lane; d < a.dim; d += 64) mine[d] = 0.0f;
   __syncthreads();
@@ -633,18 +639,18 @@ int check_heads(const char* name, int64_t dim, int64_t rotary, int64_t table_row
 }
 
 template <typename T, bool NORM, bool APPEND>
-void launch_heads(HeadArgs& a, bool vec, hipStream_t s) {
+void launch_heads(HeadArgs& a, hipStream_t s) {
   constexpr int VE = Vec16<T>::VE;
+  // (2^30 rows, and the last step of a walk)
+  bool vec = true, narrow = a.total <= 1 << 30 && a.table_rows <= INT32_MAX;
   a.lpr_log2 = lanes_log2(a.dim, a.rotary, VE);
   for (const HeadRows& r : a.r) {
     if (r.heads == 0) continue;
-    for (int64_t st : {r.heads > 1 ? r.sh : 0, r.heads > 1 ? r.yh : 0, r.si, r.so, r.yt, r.ys}) vec = vec && st <= (int64_t)UINT32_MAX;
+    for (int64_t st : {r.heads > 1 ? r.sh : 0, r.heads > 1 ? r.yh : 0, r.si, r.so, r.yt, r.ys}) narrow = narrow && st <= (int64_t)UINT32_MAX;
     vec = vec && vec_ok(r.x) && vec_ok(r.y) && vec_ok(r.w) && r.so % VE == 0 && r.si % VE == 0 && r.sh % VE == 0 &&
           r.yt % VE == 0 && r.ys % VE == 0 && r.yh % VE == 0;
   }
-  vec = vec && a.dim % VE == 0 && a.rotary % (2 * VE) == 0 && vec_ok(a.table) && a.lpr_log2 <= 6;
-  // (2^30 rows, of 32 bytes at least, and the last step of a walk)
-  vec = vec && a.total <= 1 << 30 && a.table_rows <= INT32_MAX;
+  vec = vec && narrow && a.dim % VE == 0 && a.rotary % (2 * VE) == 0 && vec_ok(a.table) && a.lpr_log2 <= 6;
   a.by_heads = Divisor(a.all_heads);
   a.by_inner = Divisor(a.inner);
   a.by_positions = Divisor(a.n_positions);
@@ -654,15 +660,16 @@ void launch_heads(HeadArgs& a, bool vec, hipStream_t s) {
   const int64_t per = vec ? kThreads >> a.lpr_log2 : 4;
   const dim3 grid(row_grid((a.total + per - 1) / per)), block(kThreads);
   if (vec) heads_kernel<T, NORM, APPEND><<<grid, block, 0, s>>>(a);
-  else heads_any_kernel<T, NORM, APPEND><<<grid, block, 0, s>>>(a);
+  else if (narrow) heads_any_kernel<T, NORM, APPEND, uint32_t><<<grid, block, 0, s>>>(a);
+  else heads_any_kernel<T, NORM, APPEND, int64_t><<<grid, block, 0, s>>>(a);
 }
 
 template <bool APPEND>
 void dispatch_heads(HeadArgs& a, bool norm, int dtype, hipStream_t s) {
   auto go = [&](auto t) {
     using T = decltype(t);
-    if (norm) launch_heads<T, true, APPEND>(a, true, s);
-    else launch_heads<T, false, APPEND>(a, true, s);
+    if (norm) launch_heads<T, true, APPEND>(a, s);
+    else launch_heads<T, false, APPEND>(a, s);
   };
   if (dtype == AK_DTYPE_F32) go(float());
   else if (dtype == AK_DTYPE_F16) go(f16());
