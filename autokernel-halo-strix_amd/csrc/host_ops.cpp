@@ -1137,18 +1137,21 @@ std::optional<std::tuple<bool, Tensor>> paged_append(const Tensor& k, const Tens
   return std::make_tuple(true, out);
 }
 
-Maybe paged_attention(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, const Tensor& pages, const Tensor& lengths,
+Maybe paged_attention(const Tensor& q_, const Tensor& k_cache, const Tensor& v_cache, const Tensor& pages, const Tensor& lengths,
                       const Maybe& starts, double scale, double softcap, int64_t window, int64_t max_chunk, const Maybe& out_) {
-  if (!ours(q, k_cache, v_cache, pages, lengths) || !ours_if(starts, q) || !ours_if(out_, q)) return std::nullopt;
-  const at::ScalarType type = q.scalar_type();
-  if (code_of(type) < 0 || !rows3(q, type) || q.numel() == 0 || k_cache.dim() != 4) return std::nullopt;
-  const int64_t tokens = q.size(0), heads = q.size(1), dim = q.size(2), kv = k_cache.size(2);
+  if (!ours(q_, k_cache, v_cache, pages, lengths) || !ours_if(starts, q_) || !ours_if(out_, q_)) return std::nullopt;
+  const at::ScalarType type = q_.scalar_type();
+  if (code_of(type) < 0 || !rows3(q_, type) || q_.numel() == 0 || k_cache.dim() != 4) return std::nullopt;
+  const int64_t tokens = q_.size(0), heads = q_.size(1), dim = q_.size(2), kv = k_cache.size(2), esz = q_.element_size();
   if (dim > kMaxAttendDim || kv < 1 || heads % kv || !paged_args(k_cache, v_cache, pages, lengths, starts, kv, dim, type, tokens) ||
-      (out_ && (!rows3(*out_, type) || out_->sizes() != q.sizes() || !dense_places(*out_))))
+      (out_ && (!rows3(*out_, type) || out_->sizes() != q_.sizes() || !dense_places(*out_))))
     return std::nullopt;
   const Tensor st = starts.value_or(Tensor());
   Tensor out = out_.value_or(Tensor());
-  if (records({&q, &k_cache, &v_cache, &out})) return std::nullopt;
+  if (records({&q_, &k_cache, &v_cache, &out})) return std::nullopt;
+  // queries off the alignment are copied: without it the whole cache goes through the slow kernel
+  const bool off = (reinterpret_cast<uintptr_t>(ptr(q_)) | (uintptr_t)(q_.stride(0) * esz) | (uintptr_t)(q_.stride(1) * esz)) % 16 != 0;
+  const Tensor q = off && dim * esz % 16 == 0 ? q_.clone(at::MemoryFormat::Contiguous) : q_;
   if (!out_) out = at::empty(q.sizes(), q.options());
   const int64_t batch = pages.size(0), keys = pages.size(1) * k_cache.size(1);
   const int code = code_of(type);

@@ -393,7 +393,7 @@ __device__ __forceinline__ void rows_begin(Args g0, const Place& p, int row0, Ro
 
 // Scores of the 32 keys whose K is at row0 on in LDS.
 template <typename T, int DB>
-__device__ __forceinline__ f32x16_t scores32(const ScoreMath& sm, const Rows<T, DB>& r, const char* kl, int row0) {
+__device__ __forceinline__ f32x16_t scores32(const Rows<T, DB>& r, const char* kl, int row0) {
   using S = Shape<T, DB>;
   const int lane = threadIdx.x & 63, half = lane >> 5, row = row0 + (lane & 31);
   const char* base = kl + row * S::kPitch + 16 * half;
@@ -966,7 +966,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, DB * sizeof(T) <= 256 ? 2 : 1)
         x.issue(cache);
       }
       f32x16_t s[1];
-      s[0] = scores32<T, DB>(sm, r, kl, 0);
+      s[0] = scores32<T, DB>(r, kl, 0);
       if (sm.cap) cap32<T>(sm, s[0]);
       if (mask) hide32<T, DB>(r, s[0], key, now);
       new_maximum<T, DB, 1>(sm, r, s);

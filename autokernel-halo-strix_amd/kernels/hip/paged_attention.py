@@ -106,6 +106,9 @@ def kernel_fn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, pag
     else:
         _heads.check_out(out, "out", q)
     q = q if dim == 1 or q.stride(2) == 1 else q.contiguous()
+    size = q.element_size()
+    if dim * size % 16 == 0 and (q.data_ptr() | q.stride(0) * size | q.stride(1) * size) % 16:
+        q = q.clone(memory_format=torch.contiguous_format)  # off the alignment the whole cache goes through the slow kernel
     if tokens:
         _lib.paged_attention(q, k_cache, v_cache, batch, out, max(1, chunk), scale, softcap, window, zero)
     if not zero:
