@@ -1115,7 +1115,7 @@ std::optional<std::tuple<bool, Tensor>> paged_append(const Tensor& k, const Tens
   if (code_of(type) < 0 || !rows3(k, type) || !rows3(v, type) || k.sizes() != v.sizes() || k.numel() == 0) return std::nullopt;
   const int64_t tokens = k.size(0), heads = k.size(1), dim = k.size(2);
   if (dim > kMaxHeadDim || !paged_args(k_cache, v_cache, pages, lengths, starts, heads, dim, type, tokens) || !dense_places(k_cache) ||
-      !dense_places(v_cache) || (q ? !rows3(*q, type) || q->size(0) != tokens || q->size(2) != dim : q_weight || q_out) ||
+      !dense_places(v_cache) || ptr(k_cache) == ptr(v_cache) || (q ? !rows3(*q, type) || q->size(0) != tokens || q->size(2) != dim : q_weight || q_out) ||
       (q_out && (!rows3(*q_out, type) || q_out->sizes() != q->sizes() || !dense_places(*q_out))) || (q_weight && !weight_ok(*q_weight, k)) ||
       (k_weight && !weight_ok(*k_weight, k)) || (table && !table_ok(*table, dim)))
     return std::nullopt;

@@ -76,6 +76,8 @@ def kernel_fn(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: 
     _heads.check_cache(k_cache, v_cache, heads, dim, k.dtype)
     if not _heads.dense_places(k_cache) or not _heads.dense_places(v_cache):
         raise ValueError("two places of a cache share their memory")
+    if k_cache.numel() and k_cache.data_ptr() == v_cache.data_ptr():
+        raise ValueError("k_cache and v_cache begin at the same place")
     batch = _heads.check_batch(page_table, lengths, starts, tokens)
     if q is None:
         if q_weight is not None or q_out is not None:

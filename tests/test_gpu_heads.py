@@ -444,6 +444,33 @@ def test_strides_past_32_bits():
         close(a, b.cpu(), 2.1 * half_eps(torch.bfloat16) * b.cpu().double().abs() + 2 * 64 * 32 * E)
 
 
+def test_the_same_tensor_twice():
+    """One tensor as queries and keys, one weight for both: the gradients are the sums; one cache for both is refused."""
+    need_gpu()
+    from kernels.hip import paged_append, qk_norm_rotary, rotary
+    say("twice")
+    g = torch.Generator().manual_seed(31)
+    x, w = randn(g, 7, 4, 64).to(DEV), (1 + 0.1 * randn(g, 64)).to(DEV)
+    up = [randn(g, 7, 4, 64).to(DEV) for _ in range(2)]
+    table = table_of(64, 7).to(DEV)
+    x1, x2, w1, w2 = (t.clone().requires_grad_() for t in (x, x, w, w))
+    x, w = x.requires_grad_(), w.requires_grad_()
+    a, b = torch.autograd.grad(rotary.kernel_fn(x1, x2, table), (x1, x2), up)
+    assert torch.equal(torch.autograd.grad(rotary.kernel_fn(x, x, table), x, up)[0], a + b)
+    a, b, c, d = torch.autograd.grad(qk_norm_rotary.kernel_fn(x1, x2, w1, w2, table), (x1, x2, w1, w2), up)
+    dx, dw = torch.autograd.grad(qk_norm_rotary.kernel_fn(x, x, w, w, table), (x, w), up)
+    assert torch.equal(dx, a + b) and torch.equal(dw, c + d)
+    pages, lens, starts, total = (t.to(DEV) if isinstance(t, torch.Tensor) else t for t in make_batch([7], [7], 8, 1))
+    cache = torch.zeros(total, 8, 4, 64, device=DEV)
+    with pytest.raises(ValueError, match="same place"):
+        paged_append.kernel_fn(x.detach(), x.detach(), cache, cache, pages, lens, starts)
+    # the halves of one allocation are two caches; lengths and starts out of a wider table
+    both = torch.zeros(total, 2, 8, 4, 64, device=DEV)
+    wide = torch.stack([lens, lens + 1], 1)[:, 0], torch.stack([starts, starts], 1)[:, 0]
+    paged_append.kernel_fn(x.detach(), up[0], both[:, 0], both[:, 1], pages, *wide)
+    assert torch.equal(both[int(pages[0, 0]), 0, :7], x.detach()) and torch.equal(both[int(pages[0, 0]), 1, :7], up[0])
+
+
 def test_captured_backward():
     """Forward and backward in one graph, replayed over new values with eager work between."""
     need_gpu()

@@ -36,6 +36,10 @@ CASES = [
     ([1, 2], [70, 31], 16, 40, 1, 64, 0, 0.0),        # groups past one tile's 32 rows,
     ([2, 1], [45, 9], 16, 130, 1, 256, 0, 0.0),       # past the tiles of wide heads,
     ([1, 2], [45, 9], 16, 300, 1, 64, 0, 0.0),        # past every tile
+    ([1, 70], [3003, 2001], 16, 4, 2, 256, 0, 0.0),   # long rows, cut among workers: many of them,
+    ([1, 3, 2], [2500, 900, 1], 16, 8, 2, 192, 0, 30.0),   # few of them,
+    ([7], [9001], 64, 2, 1, 128, 0, 0.0),             # one tile in very many parts
+    ([98], [5000], 128, 1, 1, 256, 0, 0.0),
     ([1, 70], [1503, 901], 16, 4, 2, 64, 333, 20.0),  # a window over many units, cut among workers
     ([5, 1], [90, 33], 16, 2, 1, 128, 0, 0.001),      # caps from the smallest
     ([5, 1], [90, 33], 16, 2, 1, 128, 0, 256.0),

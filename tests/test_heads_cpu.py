@@ -297,6 +297,7 @@ def test_append_and_attend(heads_backend):
     (lambda c: c.update(k_cache=c["k_cache"][:, :0]), ValueError, "k_cache"),
     (lambda c: c.update(v_cache=c["v_cache"][1:]), ValueError, "differ"),
     (lambda c: c.update(v_cache=c["v_cache"][:1].expand_as(c["v_cache"])), ValueError, "share"),
+    (lambda c: c.update(v_cache=c["k_cache"]), ValueError, "same place"),
     (lambda c: c.update(k_cache=torch.zeros(*c["k_cache"].shape[:3], 12)[..., ::2]), ValueError, "dense"),
     (lambda c: c.update(page_table=c["page_table"].long()), TypeError, "int32"),
     (lambda c: c.update(page_table=c["page_table"][0]), ValueError, "page_table"),
