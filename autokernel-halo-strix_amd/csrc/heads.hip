@@ -68,6 +68,37 @@ __device__ __forceinline__ uint32_t quotient(uint32_t a, int64_t, const Divisor&
 __device__ __forceinline__ int64_t steps(int64_t n, int64_t stride) { return n * stride; }
 __device__ __forceinline__ int64_t steps(uint32_t n, int64_t stride) { return (int64_t)((uint64_t)n * (uint32_t)stride); }
 
+// N elements in one access of 16, 8 or 4 bytes.
+template <int BYTES>
+struct Word;
+template <>
+struct Word<16> { typedef u32x4 type; };
+template <>
+struct Word<8> { typedef uint32_t type __attribute__((ext_vector_type(2))); };
+template <>
+struct Word<4> { typedef uint32_t type; };
+
+template <typename T, int N>
+union Vec {
+  typedef typename Word<N * sizeof(T)>::type W;
+  W u;
+  T e[N];
+};
+
+template <int N, typename T>
+__device__ __forceinline__ Vec<T, N> load_vec(const T* p) {
+  Vec<T, N> v;
+  v.u = *reinterpret_cast<const typename Vec<T, N>::W*>(p);
+  return v;
+}
+
+template <typename T, int N>
+__device__ __forceinline__ void store_vec(T* p, const Vec<T, N>& v, bool past) {
+  auto* to = reinterpret_cast<typename Vec<T, N>::W*>(p);
+  if (past) __builtin_nontemporal_store(v.u, to);
+  else *to = v.u;
+}
+
 // The sum over the 2^log2 lanes of a row (aligned to their number).
 __device__ __forceinline__ float lanes_sum(float v, int log2) {
   if (log2 > 0) v += dpp<kDppXor1>(v);
@@ -98,22 +129,22 @@ struct Unit {
 // The angles of a unit's VE pairs: cosines and sines (negated for the way back).
 template <int VE, bool INVERSE>
 __device__ __forceinline__ void load_angles(const HeadArgs& a, int64_t pos, int u, float (&c)[VE], float (&s)[VE]) {
-  Vec16<float> cv[VE / 4], sv[VE / 4];
-  constexpr uint32_t kNaN = 0x7fc00000u;
+  constexpr int A = VE < 4 ? VE : 4;
+  Vec<float, A> cv[VE / A], sv[VE / A];
 #pragma unroll
-  for (int i = 0; i < VE / 4; ++i) cv[i].u = sv[i].u = u32x4{kNaN, kNaN, kNaN, kNaN};
+  for (int e = 0; e < VE; ++e) cv[e / A].e[e % A] = sv[e / A].e[e % A] = __builtin_nanf("");
   if (pos >= 0 && pos < a.table_rows) {
     const float* row = a.table + steps((uint32_t)pos, a.rotary) + u * VE;
 #pragma unroll
-    for (int i = 0; i < VE / 4; ++i) {
-      cv[i] = load16(row + 4 * i);
-      sv[i] = load16(row + a.rotary / 2 + 4 * i);
+    for (int i = 0; i < VE / A; ++i) {
+      cv[i] = load_vec<A>(row + A * i);
+      sv[i] = load_vec<A>(row + a.rotary / 2 + A * i);
     }
   }
 #pragma unroll
   for (int e = 0; e < VE; ++e) {
-    c[e] = cv[e / 4].e[e % 4];
-    s[e] = INVERSE && a.inverse ? -sv[e / 4].e[e % 4] : sv[e / 4].e[e % 4];
+    c[e] = cv[e / A].e[e % A];
+    s[e] = INVERSE && a.inverse ? -sv[e / A].e[e % A] : sv[e / A].e[e % A];
   }
 }
 
@@ -235,14 +266,15 @@ __device__ __forceinline__ Target<T> target_of(const HeadArgs& a, const Row<T, I
 }
 #undef AK_PICK
 
-// Rows of whole vectors: 16-byte aligned, dim a multiple of a vector and the
-// turned part one of two. [8, 1024, 32 + 8, 128] bf16 turned 28 us (6.0 TB/s), normed
-// and turned 30 (5.6); prompts of 9730 tokens, 32 + 8 + 8 heads of 128 fp16, into a cache
-// 50 (4.9). A decode step is one launch of 4 us. Two or four rows a thread at a
-// time, or fewer workgroups that read a row ahead: the same or slower.
-template <typename T, bool NORM, bool APPEND>
+// Rows of whole vectors of VE elements: aligned to them, dim a multiple of one and the
+// turned part of two. The widest that fits, 16, 8 or 4 bytes: of [8, 1024, 32 + 8, 128]
+// bf16 with all or 64, 56 and 44 elements turned 28 (6.0 TB/s), 34 and 57 us, a wave a
+// row 94; normed and back 88, 105 and 168 for 541. Prompts of 9730 tokens, 32 + 8 + 8
+// heads of 128 fp16, normed into a cache 50 us (4.9 TB/s). A decode step is one launch
+// of 4 us. Two or four rows a thread at a time, or fewer workgroups that read a row
+// ahead: the same or slower.
+template <typename T, int VE, bool NORM, bool APPEND>
 __global__ void __launch_bounds__(kThreads) heads_kernel(HeadArgs a) {
-  constexpr int VE = Vec16<T>::VE;
   const int lpr = 1 << a.lpr_log2, per = kThreads >> a.lpr_log2;
   const int u = threadIdx.x & (lpr - 1);
   const Unit<VE> unit(u, a);
@@ -250,14 +282,14 @@ __global__ void __launch_bounds__(kThreads) heads_kernel(HeadArgs a) {
   for (uint32_t base = blockIdx.x * per; base < total; base += gridDim.x * per) {
     const uint32_t row = base + (threadIdx.x >> a.lpr_log2);
     const Row<T, uint32_t> from = row_of<T, APPEND>(a, min(row, total - 1));
-    Vec16<T> v0, v1;
-    v0.u = v1.u = u32x4{0, 0, 0, 0};
-    if (unit.has0) v0 = load16(from.x + unit.off0);
-    if (unit.has1) v1 = load16(from.x + unit.off1);
+    Vec<T, VE> v0, v1;
+    v0.u = v1.u = typename Vec<T, VE>::W{};
+    if (unit.has0) v0 = load_vec<VE>(from.x + unit.off0);
+    if (unit.has1) v1 = load_vec<VE>(from.x + unit.off1);
     const Target<T> o = target_of<T, APPEND>(a, from, row < total);  // (its searches while the loads are on their way)
     if (!NORM && APPEND && !o.rotate) {  // values are copied
-      if (o.write && unit.has0) store16(o.y + unit.off0, v0);
-      if (o.write && unit.has1) store16(o.y + unit.off1, v1);
+      if (o.write && unit.has0) store_vec(o.y + unit.off0, v0, false);
+      if (o.write && unit.has1) store_vec(o.y + unit.off1, v1, false);
       continue;
     }
     float p[VE], q[VE];
@@ -273,10 +305,10 @@ __global__ void __launch_bounds__(kThreads) heads_kernel(HeadArgs a) {
       ss = lanes_sum(ss, a.lpr_log2);
       if (from.w != nullptr) {
         const float inv = 1.0f / sqrtf(ss * a.by_dim + a.eps);
-        Vec16<T> w0, w1;
-        w0.u = w1.u = u32x4{0, 0, 0, 0};
-        if (unit.has0) w0 = load16(from.w + unit.off0);
-        if (unit.has1) w1 = load16(from.w + unit.off1);
+        Vec<T, VE> w0, w1;
+        w0.u = w1.u = typename Vec<T, VE>::W{};
+        if (unit.has0) w0 = load_vec<VE>(from.w + unit.off0);
+        if (unit.has1) w1 = load_vec<VE>(from.w + unit.off1);
 #pragma unroll
         for (int e = 0; e < VE; ++e) {
           p[e] = p[e] * inv * to_f32(w0.e[e]);
@@ -295,14 +327,9 @@ __global__ void __launch_bounds__(kThreads) heads_kernel(HeadArgs a) {
         v0.e[e] = from_f32<T>(p[e]);
         v1.e[e] = from_f32<T>(q[e]);
       }
-      if (APPEND && o.zero) v0.u = v1.u = u32x4{0, 0, 0, 0};
-      if (!APPEND && a.past) {
-        if (unit.has0) store16_nt(o.y + unit.off0, v0);
-        if (unit.has1) store16_nt(o.y + unit.off1, v1);
-      } else {
-        if (unit.has0) store16(o.y + unit.off0, v0);
-        if (unit.has1) store16(o.y + unit.off1, v1);
-      }
+      if (APPEND && o.zero) v0.u = v1.u = typename Vec<T, VE>::W{};
+      if (unit.has0) store_vec(o.y + unit.off0, v0, !APPEND && a.past);
+      if (unit.has1) store_vec(o.y + unit.off1, v1, !APPEND && a.past);
     }
   }
 }
@@ -323,8 +350,8 @@ __device__ __forceinline__ void angle_at(const HeadArgs& a, int64_t pos, int i, 
 }
 
 // Every other row: a wave each, one element or pair a lane at a time. Bound by its narrow
-// loads: [8, 1024, 32 + 8, 128] bf16 with 44 elements turned takes 94 us, whole vectors (64
-// turned) 28; forward and back with the norm 541 and 88.
+// loads: [8, 1024, 32 + 8, 66] bf16 with 22 elements turned takes 89 us, forward and back with
+// the norm 405.
 template <typename T, bool NORM, bool APPEND, typename I>
 __global__ void __launch_bounds__(kThreads) heads_any_kernel(HeadArgs a) {
   const int lane = threadIdx.x & 63;
@@ -405,9 +432,8 @@ __device__ __forceinline__ GradRow<T> grad_row_of(const HeadArgs& a, const GradR
 // the workgroups in grad_weight_kernel: fixed orders throughout. [8, 1024, 32 + 8,
 // 128] bf16 43 us (5.8 TB/s) and 4 for the weights, of 88 forward and back. The
 // registers are held to 128 for four workgroups a CU: with three it was 117 for 97.
-template <typename T>
+template <typename T, int VE>
 __global__ void __launch_bounds__(kThreads, 4) heads_bwd_kernel(GradArgs ga) {
-  constexpr int VE = Vec16<T>::VE;
   __shared__ float gather[kThreads * 2 * VE];
   const HeadArgs& a = ga.h;
   const bool second = (int)blockIdx.x >= ga.r[1].first_block;
@@ -418,10 +444,10 @@ __global__ void __launch_bounds__(kThreads, 4) heads_bwd_kernel(GradArgs ga) {
   const T* w = static_cast<const T*>(r.w);
   float w0[VE], w1[VE], d0[VE], d1[VE];
   {
-    Vec16<T> v0, v1;
-    v0.u = v1.u = u32x4{0, 0, 0, 0};
-    if (unit.has0) v0 = load16(w + unit.off0);
-    if (unit.has1) v1 = load16(w + unit.off1);
+    Vec<T, VE> v0, v1;
+    v0.u = v1.u = typename Vec<T, VE>::W{};
+    if (unit.has0) v0 = load_vec<VE>(w + unit.off0);
+    if (unit.has1) v1 = load_vec<VE>(w + unit.off1);
 #pragma unroll
     for (int e = 0; e < VE; ++e) {
       w0[e] = to_f32(v0.e[e]);
@@ -434,15 +460,15 @@ __global__ void __launch_bounds__(kThreads, 4) heads_bwd_kernel(GradArgs ga) {
     const uint32_t row = base + slot;
     const bool live = row < rows;
     const GradRow<T> o = grad_row_of<T>(a, r, min(row, rows - 1));
-    Vec16<T> x0, x1, g0, g1;
-    x0.u = x1.u = g0.u = g1.u = u32x4{0, 0, 0, 0};
+    Vec<T, VE> x0, x1, g0, g1;
+    x0.u = x1.u = g0.u = g1.u = typename Vec<T, VE>::W{};
     if (live && unit.has0) {
-      x0 = load16(o.x + unit.off0);
-      g0 = load16(o.g + unit.off0);
+      x0 = load_vec<VE>(o.x + unit.off0);
+      g0 = load_vec<VE>(o.g + unit.off0);
     }
     if (live && unit.has1) {
-      x1 = load16(o.x + unit.off1);
-      g1 = load16(o.g + unit.off1);
+      x1 = load_vec<VE>(o.x + unit.off1);
+      g1 = load_vec<VE>(o.g + unit.off1);
     }
     float z0[VE], z1[VE];
 #pragma unroll
@@ -467,7 +493,7 @@ __global__ void __launch_bounds__(kThreads, 4) heads_bwd_kernel(GradArgs ga) {
     if (!live) continue;
     const float inv = 1.0f / sqrtf(ss * a.by_dim + a.eps);
     const float back = inv * (gx * a.by_dim);  // (of order one, as n is, whatever the size of x)
-    Vec16<T> y0, y1;
+    Vec<T, VE> y0, y1;
 #pragma unroll
     for (int e = 0; e < VE; ++e) {
       const float n0 = to_f32(x0.e[e]) * inv, n1 = to_f32(x1.e[e]) * inv;
@@ -477,13 +503,8 @@ __global__ void __launch_bounds__(kThreads, 4) heads_bwd_kernel(GradArgs ga) {
       d1[e] = fmaf(z1[e], n1, d1[e]);
     }
     T* y = static_cast<T*>(r.dx) + steps(row, a.dim);
-    if (a.past) {
-      if (unit.has0) store16_nt(y + unit.off0, y0);
-      if (unit.has1) store16_nt(y + unit.off1, y1);
-    } else {
-      if (unit.has0) store16(y + unit.off0, y0);
-      if (unit.has1) store16(y + unit.off1, y1);
-    }
+    if (unit.has0) store_vec(y + unit.off0, y0, a.past);
+    if (unit.has1) store_vec(y + unit.off1, y1, a.past);
   }
   if (r.dw == nullptr) return;
   // gather[element of the unit][thread]; then column by column over the row slots
@@ -598,7 +619,7 @@ __global__ void __launch_bounds__(1024) grad_weight_kernel(GradArgs ga) {
 // ---------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------
-bool vec_ok(const void* p) { return p == nullptr || aligned16(p); }
+bool on(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 
 // Fewest lanes (a power of two) that hold a head in units; past 64 the head
 // takes the other kernels.
@@ -640,26 +661,33 @@ int check_heads(const char* name, int64_t dim, int64_t rotary, int64_t table_row
 
 template <typename T, bool NORM, bool APPEND>
 void launch_heads(HeadArgs& a, hipStream_t s) {
-  constexpr int VE = Vec16<T>::VE;
   // (2^30 rows, and the last step of a walk)
-  bool vec = true, narrow = a.total <= 1 << 30 && a.table_rows <= INT32_MAX;
-  a.lpr_log2 = lanes_log2(a.dim, a.rotary, VE);
-  for (const HeadRows& r : a.r) {
-    if (r.heads == 0) continue;
+  bool narrow = a.total <= 1 << 30 && a.table_rows <= INT32_MAX;
+  for (const HeadRows& r : a.r)
     for (int64_t st : {r.heads > 1 ? r.sh : 0, r.heads > 1 ? r.yh : 0, r.si, r.so, r.yt, r.ys}) narrow = narrow && st <= (int64_t)UINT32_MAX;
-    vec = vec && vec_ok(r.x) && vec_ok(r.y) && vec_ok(r.w) && r.so % VE == 0 && r.si % VE == 0 && r.sh % VE == 0 &&
-          r.yt % VE == 0 && r.ys % VE == 0 && r.yh % VE == 0;
-  }
-  vec = vec && narrow && a.dim % VE == 0 && a.rotary % (2 * VE) == 0 && vec_ok(a.table) && a.lpr_log2 <= 6;
+  const auto fits = [&](int w) {
+    bool ok = a.dim % w == 0 && a.rotary % (2 * w) == 0 && on(a.table, std::min(w, 4) * 4) && lanes_log2(a.dim, a.rotary, w) <= 6;
+    for (const HeadRows& r : a.r) {
+      if (r.heads == 0) continue;
+      for (const void* p : {r.x, (const void*)r.y, r.w}) ok = ok && on(p, w * (int)sizeof(T));
+      for (int64_t st : {r.so, r.si, r.sh, r.yt, r.ys, r.yh}) ok = ok && st % w == 0;
+    }
+    return ok;
+  };
+  constexpr int VE = Vec16<T>::VE;
+  const int w = !narrow ? 0 : fits(VE) ? VE : fits(VE / 2) ? VE / 2 : VE > 4 && fits(VE / 4) ? VE / 4 : 0;
+  a.lpr_log2 = w ? lanes_log2(a.dim, a.rotary, w) : 6;
   a.by_heads = Divisor(a.all_heads);
   a.by_inner = Divisor(a.inner);
   a.by_positions = Divisor(a.n_positions);
   a.by_page = Divisor(a.page_size);
   a.by_dim = 1.0f / (float)a.dim;
   a.past = a.total > kL2Bytes / (a.dim * (int64_t)sizeof(T));
-  const int64_t per = vec ? kThreads >> a.lpr_log2 : 4;
+  const int64_t per = kThreads >> a.lpr_log2;
   const dim3 grid(row_grid((a.total + per - 1) / per)), block(kThreads);
-  if (vec) heads_kernel<T, NORM, APPEND><<<grid, block, 0, s>>>(a);
+  if (w == VE) heads_kernel<T, VE, NORM, APPEND><<<grid, block, 0, s>>>(a);
+  else if (w == VE / 2) heads_kernel<T, VE / 2, NORM, APPEND><<<grid, block, 0, s>>>(a);
+  else if (VE > 4 && w == VE / 4) heads_kernel<T, (VE > 4 ? VE / 4 : 2), NORM, APPEND><<<grid, block, 0, s>>>(a);
   else if (narrow) heads_any_kernel<T, NORM, APPEND, uint32_t><<<grid, block, 0, s>>>(a);
   else heads_any_kernel<T, NORM, APPEND, int64_t><<<grid, block, 0, s>>>(a);
 }
@@ -798,24 +826,34 @@ extern "C" int ak_qk_norm_rotary_bwd(const void* q, const void* k, const void* q
   hipStream_t s = ak_stream(stream);
   auto go = [&](auto t) {
     using T = decltype(t);
-    constexpr int VE = ak::Vec16<T>::VE;
-    a.lpr_log2 = ak::lanes_log2(dim, rotary, VE);
-    bool vec = dim % VE == 0 && rotary % (2 * VE) == 0 && ak::vec_ok(table) && a.lpr_log2 <= 6;
-    for (const ak::GradRows& r : g.r) {
-      if (r.heads == 0) continue;
-      for (const void* p : {r.x, r.g, r.w, (const void*)r.dx}) vec = vec && ak::vec_ok(p);
-      for (int64_t st : {r.so, r.si, r.sh, r.go, r.gi, r.gh}) vec = vec && st % VE == 0 && st <= (int64_t)UINT32_MAX;
-      vec = vec && r.rows <= 1 << 30;
+    bool narrow = table_rows <= INT32_MAX;
+    for (ak::GradRows& r : g.r) {
+      r.by_heads = ak::Divisor(r.heads);
+      narrow = narrow && r.rows <= 1 << 30;
+      for (int64_t st : {r.so, r.si, r.sh, r.go, r.gi, r.gh}) narrow = narrow && (r.heads == 0 || st <= (int64_t)UINT32_MAX);
     }
-    for (ak::GradRows& r : g.r) r.by_heads = ak::Divisor(r.heads);
-    vec = vec && table_rows <= INT32_MAX;
+    const auto fits = [&](int w) {
+      bool ok = dim % w == 0 && rotary % (2 * w) == 0 && ak::on(table, std::min(w, 4) * 4) && ak::lanes_log2(dim, rotary, w) <= 6;
+      for (const ak::GradRows& r : g.r) {
+        if (r.heads == 0) continue;
+        for (const void* p : {r.x, r.g, r.w, (const void*)r.dx}) ok = ok && ak::on(p, w * (int)sizeof(T));
+        for (int64_t st : {r.so, r.si, r.sh, r.go, r.gi, r.gh}) ok = ok && st % w == 0;
+      }
+      return ok;
+    };
+    constexpr int VE = ak::Vec16<T>::VE;
+    const int w = !narrow ? 0 : fits(VE) ? VE : fits(VE / 2) ? VE / 2 : VE > 4 && fits(VE / 4) ? VE / 4 : 0;
+    if (w) a.lpr_log2 = ak::lanes_log2(dim, rotary, w);
     a.by_inner = ak::Divisor(a.inner);
     a.by_positions = ak::Divisor(a.n_positions);
     a.by_dim = 1.0f / (float)dim;
     a.past = tokens * (q_heads + k_heads) > ak::kL2Bytes / (dim * (int64_t)sizeof(T));
     if (bq + bk > 0) {
-      if (vec) ak::heads_bwd_kernel<T><<<dim3((unsigned)(bq + bk)), dim3(ak::kThreads), 0, s>>>(g);
-      else ak::heads_bwd_any_kernel<T><<<dim3((unsigned)(bq + bk)), dim3(ak::kThreads), 0, s>>>(g);
+      const dim3 grid((unsigned)(bq + bk)), block(ak::kThreads);
+      if (w == VE) ak::heads_bwd_kernel<T, VE><<<grid, block, 0, s>>>(g);
+      else if (w == VE / 2) ak::heads_bwd_kernel<T, VE / 2><<<grid, block, 0, s>>>(g);
+      else if (VE > 4 && w == VE / 4) ak::heads_bwd_kernel<T, (VE > 4 ? VE / 4 : 2)><<<grid, block, 0, s>>>(g);
+      else ak::heads_bwd_any_kernel<T><<<grid, block, 0, s>>>(g);
     }
     if (grad_q_weight || grad_k_weight)
       ak::grad_weight_kernel<T><<<dim3((unsigned)((dim + 15) / 16), 2), dim3(1024), 0, s>>>(g);

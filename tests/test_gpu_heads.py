@@ -33,6 +33,10 @@ SHAPES = [
     ((3,), 2, 1, 1030, 514, False, "dense"),      # more than a wave's vectors
     ((0,), 4, 2, 64, 64, False, "dense"),
     ((2, 6), 4, 2, 64, 64, True, "expanded"),
+    ((3, 5), 4, 2, 128, 56, False, "fused"),      # halves on 8 bytes,
+    ((37,), 2, 2, 128, 44, True, "dense"),        # on 4,
+    ((130,), 3, 1, 72, 36, False, "dense"),
+    ((7,), 2, 1, 256, 12, False, "bhsd2"),
 ]
 
 
@@ -42,6 +46,8 @@ def make(g, lead, heads, dim, dtype, layout):
         return randn(g, *lead, heads + 3, dim).to(dtype).to(DEV)[..., 2:2 + heads, :]
     if layout == "bhsd":
         return randn(g, lead[0], heads, lead[1], dim).to(dtype).to(DEV).transpose(1, 2)
+    if layout == "bhsd2":
+        return randn(g, heads, *lead, dim).to(dtype).to(DEV).movedim(0, -2)
     if layout == "offset":
         n = math.prod(lead) * heads * dim
         return randn(g, n + 1).to(dtype).to(DEV)[1:].view(*lead, heads, dim)
@@ -268,6 +274,8 @@ BATCHES = [
     ([4, 1], [4, 100], 7, 2, 2, 66, 66, False, True),
     ([3, 2], [2, 9], 4, 2, 1, 64, 32, False, False),     # a sequence shorter than its new tokens
     ([70] + [1] * 69, [70] + list(range(1, 70)), 16, 2, 1, 64, 64, False, True),
+    ([21, 1], [30, 8], 16, 4, 2, 72, 36, False, True),   # halves on 4 bytes
+    ([21, 1], [30, 8], 16, 4, 2, 128, 56, True, False),  # on 8
 ]
 
 
