@@ -22,7 +22,8 @@ namespace ak {
 namespace {
 
 constexpr int kRows = 32;          // rows of a wave
-constexpr int kPlanBatch = 1024;   // sequences that a workgroup lines up by itself
+constexpr int kPlanBatch = 1024;   // sequences that a workgroup of few-row workers lines up by itself,
+constexpr int kPlanMany = 64;      // and one of many rows, a wave a sequence (a launch for it: 3 us more of 17 to 25)
 
 typedef float f32x4_v __attribute__((ext_vector_type(4)));
 
@@ -60,6 +61,9 @@ __device__ __forceinline__ Args fresh(Args g) {
 }
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ int64_t uniform64(int64_t v) {
+  return (int64_t)((uint64_t)(uint32_t)uniform((int)(v >> 32)) << 32 | (uint32_t)uniform((int)v));
+}
 
 // Where a key lives.
 struct PageMath {
@@ -1011,7 +1015,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, DB * sizeof(T) <= 256 ? 2 : 1)
 // read before the barrier, loads sent out in the vector phase, tiles of 64 rows a wave, two
 // workgroups of four waves a CU: all the same or slower.
 template <typename T, int DB, int WAVES, int UNIT>
-__global__ void __launch_bounds__(64 * WAVES) attend_many_kernel(TileArgs) {
+__global__ void __launch_bounds__(64 * WAVES) attend_many_kernel(TileArgs, bool lined) {
   using S = Shape<T, DB>;
   constexpr int N = UNIT / S::kPerLoad / WAVES;  // loads of a wave, UNIT rows over all waves
   constexpr int NB = UNIT / 32;
@@ -1027,6 +1031,7 @@ __global__ void __launch_bounds__(64 * WAVES) attend_many_kernel(TileArgs) {
   __shared__ __attribute__((aligned(16))) char vl[vSlots][UNIT * S::vWidePitch];
   __shared__ u32x4 table[kTable][UNIT];
   __shared__ uint32_t there[2 * kTable][4];      // of a unit: the bits of its keys that are there; 1: partly seen, 2: not all there
+  __shared__ int64_t own_line[kPlanMany + 1];    // the line of a call of few sequences
   __shared__ int bad[vSlots];                    // the unit (by count) whose values are not all finite
   const Args g = kernel_args();
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
@@ -1034,7 +1039,26 @@ __global__ void __launch_bounds__(64 * WAVES) attend_many_kernel(TileArgs) {
   // neighbours in the line, which share keys, go to one XCD
   const int nb = (int)gridDim.x;
   const int worker = nb % 8 == 0 ? (int)(blockIdx.x % 8) * (nb / 8) + (int)blockIdx.x / 8 : (int)blockIdx.x;
-  const int64_t total = g->line[g->a.seq.batch];
+  const int batch = (int)g->a.seq.batch;
+  if (!lined) {
+    for (int b = wave; b < batch; b += WAVES) {
+      const int64_t n = wave_sum64(units_of(g, seq_at(g, b), lane, 64));
+      if (lane == 0) own_line[b + 1] = n * g->a.kv_heads;
+    }
+    __syncthreads();
+    if (wave == 0) {
+      int64_t upto = lane < batch ? own_line[lane + 1] : 0;
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const int64_t o = __shfl_up(upto, d);
+        if (lane >= d) upto += o;
+      }
+      if (lane == 0) own_line[0] = 0;
+      own_line[lane + 1] = upto;
+    }
+    __syncthreads();
+  }
+  const int64_t total = uniform64(lined ? g->line[batch] : own_line[batch]);
   const int64_t n_workers = active_workers(g, total);
   zero_other_rows<T>(g, worker * WAVES + wave, nb * WAVES);
   if (total == 0 || worker >= n_workers) {
@@ -1044,9 +1068,11 @@ __global__ void __launch_bounds__(64 * WAVES) attend_many_kernel(TileArgs) {
   const int64_t u0 = begin_of(worker, total, n_workers), u1 = begin_of(worker + 1, total, n_workers);
   const int n = uniform((int)min(u1 - u0, (int64_t)INT32_MAX));
   Place p;
-  p.b = sequence_at(g->line, (int)g->a.seq.batch, u0);
-  int64_t in_tile = u0 - g->line[p.b];
-  place_in_sequence(g, p, in_tile, g->line[p.b + 1] - g->line[p.b]);
+  p.b = lined ? sequence_at(g->line, batch, u0) : sequence_at(own_line, batch, u0);
+  const int64_t at = uniform64(lined ? g->line[p.b] : own_line[p.b]);
+  const int64_t next_at = uniform64(lined ? g->line[p.b + 1] : own_line[p.b + 1]);
+  int64_t in_tile = u0 - at;
+  place_in_sequence(g, p, in_tile, next_at - at);
   const int row0 = wave * kRows, first = wave * S::kPerLoad;
   constexpr int stride = WAVES * S::kPerLoad;
   const ScoreMath sm = score_math(g);
@@ -1167,7 +1193,8 @@ __global__ void __launch_bounds__(64 * WAVES) attend_many_kernel(TileArgs) {
       rows_end<T, DB, true>(g, p, row0, r, slot);
       if (j == n) {
         if (threadIdx.x == 0) {
-          const int64_t all = fresh(g)->line[fresh(g)->a.seq.batch], count = active_workers(fresh(g), all);
+          const int last = (int)fresh(g)->a.seq.batch;
+          const int64_t all = lined ? fresh(g)->line[last] : own_line[last], count = active_workers(fresh(g), all);
           const int64_t end = begin_of(worker + 1, all, count);
           const int parts = ended ? 0 : (int)(worker_of(end + (units - unit) - 1, all, count) - worker) + 1;
           leave_job(g, worker, begin == 0 && !ended ? &p : nullptr, slot, parts);
@@ -1390,8 +1417,9 @@ Plan plan_of(int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads, i
   // least units of a worker: of one token over 777 keys 1: 14.2 us, 2: 16.8, 4: 18.5, 32: 43.6
   // (of many rows 1 to 8 are alike)
   p.min_units = p.few ? 1 : 2;
-  // (many tiles of a sequence are lined up by 64 lanes: an understated max_chunk)
-  p.lined = !p.few || batch > kPlanBatch || tokens / p.per_tile > batch + 4096;
+  // (a thread of the few-row kernel lines up a whole sequence: of many tiles, by an understated
+  // max_chunk, 64 lanes do)
+  p.lined = batch > (p.few ? kPlanBatch : kPlanMany) || (p.few && tokens / p.per_tile > batch + 4096);
   // workgroups at once: two of the few-row kernel where their LDS and registers leave room
   const int64_t groups = (int64_t)cu_count() * (p.few && !wide ? 2 : 1);
   const double most = (double)kv_heads * ((double)tokens / p.per_tile + (double)batch) * ((double)max_keys / p.unit + 1.0);
@@ -1418,7 +1446,7 @@ void launch_tiles(const TileArgs& g, const Plan& p, hipStream_t s) {
   }
   if (!p.few) {
     constexpr int kWaves = DB * sizeof(T) > 256 ? 4 : 8, kUnit = DB * sizeof(T) > 256 ? 32 : 64;
-    attend_many_kernel<T, DB, kWaves, kUnit><<<dim3((unsigned)p.workers), dim3(64 * kWaves), 0, s>>>(g);
+    attend_many_kernel<T, DB, kWaves, kUnit><<<dim3((unsigned)p.workers), dim3(64 * kWaves), 0, s>>>(g, p.lined);
   }
   if (p.workers > 1) {
     const unsigned jobs = (unsigned)(p.workers - 1);
