@@ -93,10 +93,12 @@ __device__ __forceinline__ Vec<T, N> load_vec(const T* p) {
 }
 
 template <typename T, int N>
-__device__ __forceinline__ void store_vec(T* p, const Vec<T, N>& v, bool past) {
-  auto* to = reinterpret_cast<typename Vec<T, N>::W*>(p);
-  if (past) __builtin_nontemporal_store(v.u, to);
-  else *to = v.u;
+__device__ __forceinline__ void store_vec(T* p, const Vec<T, N>& v) {
+  *reinterpret_cast<typename Vec<T, N>::W*>(p) = v.u;
+}
+template <typename T, int N>
+__device__ __forceinline__ void store_past(T* p, const Vec<T, N>& v) {
+  __builtin_nontemporal_store(v.u, reinterpret_cast<typename Vec<T, N>::W*>(p));
 }
 
 // The sum over the 2^log2 lanes of a row (aligned to their number).
@@ -288,8 +290,8 @@ __global__ void __launch_bounds__(kThreads) heads_kernel(HeadArgs a) {
     if (unit.has1) v1 = load_vec<VE>(from.x + unit.off1);
     const Target<T> o = target_of<T, APPEND>(a, from, row < total);  // (its searches while the loads are on their way)
     if (!NORM && APPEND && !o.rotate) {  // values are copied
-      if (o.write && unit.has0) store_vec(o.y + unit.off0, v0, false);
-      if (o.write && unit.has1) store_vec(o.y + unit.off1, v1, false);
+      if (o.write && unit.has0) store_vec(o.y + unit.off0, v0);
+      if (o.write && unit.has1) store_vec(o.y + unit.off1, v1);
       continue;
     }
     float p[VE], q[VE];
@@ -328,8 +330,13 @@ __global__ void __launch_bounds__(kThreads) heads_kernel(HeadArgs a) {
         v1.e[e] = from_f32<T>(q[e]);
       }
       if (APPEND && o.zero) v0.u = v1.u = typename Vec<T, VE>::W{};
-      if (unit.has0) store_vec(o.y + unit.off0, v0, !APPEND && a.past);
-      if (unit.has1) store_vec(o.y + unit.off1, v1, !APPEND && a.past);
+      if (!APPEND && a.past) {
+        if (unit.has0) store_past(o.y + unit.off0, v0);
+        if (unit.has1) store_past(o.y + unit.off1, v1);
+      } else {
+        if (unit.has0) store_vec(o.y + unit.off0, v0);
+        if (unit.has1) store_vec(o.y + unit.off1, v1);
+      }
     }
   }
 }
@@ -503,8 +510,13 @@ __global__ void __launch_bounds__(kThreads, 4) heads_bwd_kernel(GradArgs ga) {
       d1[e] = fmaf(z1[e], n1, d1[e]);
     }
     T* y = static_cast<T*>(r.dx) + steps(row, a.dim);
-    if (unit.has0) store_vec(y + unit.off0, y0, a.past);
-    if (unit.has1) store_vec(y + unit.off1, y1, a.past);
+    if (a.past) {
+      if (unit.has0) store_past(y + unit.off0, y0);
+      if (unit.has1) store_past(y + unit.off1, y1);
+    } else {
+      if (unit.has0) store_vec(y + unit.off0, y0);
+      if (unit.has1) store_vec(y + unit.off1, y1);
+    }
   }
   if (r.dw == nullptr) return;
   // gather[element of the unit][thread]; then column by column over the row slots

@@ -1008,7 +1008,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, DB * sizeof(T) <= 256 ? 2 : 1)
 // stores after the barrier, which saves a slot.)
 //
 // Bound by what surrounds the products: prompts of up to 4096 tokens, 32 + 8 heads of 128 bf16,
-// 490 to 500 us, 750 TFLOP/s where a product of 8192^3 reaches 1420. Of a step's 5600 cycles
+// 488 us, 766 TFLOP/s where a product of 8192^3 reaches 1420. Of a step's 5600 cycles
 // (1.9 GHz under this load) a SIMD's matrix cores take 2050. The matrix phase has 900 for O^T's
 // products, 750 for the stores, loads and places of units ahead, 300 for tiles' ends, 660 for
 // the scores, the vector phase 1340 for weights and 530 for look-ups. A first unit's operands
