@@ -1428,7 +1428,7 @@ Plan plan_of(int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads, i
   if (p.few) p.workers = (p.workers + kFewWaves - 1) / kFewWaves * kFewWaves;
   const int64_t tiles = kv_heads * std::max(tokens / p.per_tile, (int64_t)1);
   p.cut = p.workers > 8 * tiles;
-  // (measured: half and double of either cost do the same to drawn calls, on the average; units of
+  // (measured: half and double of either cost do the same on the average of random calls; units of
   // fp32 take four times as long)
   p.join_cost = (p.few ? 0.02f * (float)((p.rows + 15) / 16) : 0.2f) / (f32 ? 4.0f : 1.0f) / (float)tiles;
   p.line_bytes = (size_t)(batch + 2) / 2 * 16;
