@@ -8,6 +8,7 @@ from typing import NamedTuple, Optional, Tuple
 import torch
 
 from kernels.hip import _lib
+from kernels.hip.token_logprobs import refuse_tangents
 
 MAX_HEAD_DIM = 2048
 
@@ -53,6 +54,7 @@ def check_table(table: torch.Tensor, dim: int) -> int:
         raise ValueError(f"table {tuple(table.shape)} does not turn an even part of a head of {dim}")
     if table.requires_grad:
         raise ValueError("the angles are constants: table must not require a gradient")
+    refuse_tangents("the table of angles", table)
     return rotary
 
 
@@ -77,9 +79,11 @@ def check_positions(positions: Optional[torch.Tensor], lead) -> Tuple[Optional[t
 
 
 def no_gradient(name: str, *tensors: Optional[torch.Tensor]) -> None:
-    """Refuse a call that autograd would have to record."""
+    """Refuse a call that autograd would have to record, or that brings tangents (a dual
+    tensor's requires_grad is False)."""
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad() or on detached tensors")
+    refuse_tangents(name, *tensors)
 
 
 def dense_places(t: torch.Tensor) -> bool:
