@@ -331,7 +331,7 @@ template <typename T, int DB>
 struct Rows {
   u32x4 q[Shape<T, DB>::kSteps];
   f32x16_t o[Shape<T, DB>::kBlocks];
-  float m, l;     // the running maximum (base 2; the lane's query) and this half's sum
+  float m, l;     // what the weights are taken beside (base 2; the lane's query) and this half's sum
   int lo, hi;     // the keys that the query sees
   int top, low;   // of the wave's rows: the least hi, the largest lo
   int beg, end;   // of the wave's rows: the keys that some of them see
@@ -439,11 +439,18 @@ __device__ __forceinline__ void hide32(const Rows<T, DB>& r, f32x16_t& s, int ke
   }
 }
 
-// The maximum that the weights are taken beside, over N x 32 new scores. It follows the
-// true one at a distance of up to 2^kLag: weights of up to 2^kLag are as exact as weights
-// of up to 1, and most units then leave what is summed up alone (raised at every new
-// maximum, [4, 4096 ..] prompts took 709 us, with the lag 663).
-constexpr float kLag = 8.0f;
+// The weights are taken beside a reference m that follows the true maximum at a distance of
+// up to 2^kLag: most units then leave what is summed up alone (raised at every new maximum,
+// [4, 4096 ..] prompts took 709 us, with the lag 663). A row's largest weight is 2^kTop to
+// 2^(kTop + kLag). bf16 and fp32 weights have the same digits at any size. fp16's end at 2^16,
+// and below 2^-14 they lose digits, so they stand as high as they can, at 2^11 to 2^15: one
+// keeps all of its digits down to 2^-25 of the row's largest, and is off by 2^-36 of it below
+// (from 1 on, 8192 weights of 2^-25 each were left out of the products and counted in the sum).
+template <typename T>
+struct Reference {
+  static constexpr bool kHalf = std::is_same<T, f16>::value;
+  static constexpr float kLag = kHalf ? 4.0f : 8.0f, kTop = kHalf ? 11.0f : 0.0f;
+};
 
 template <typename T, int DB, int N>
 __device__ __forceinline__ void new_maximum(const ScoreMath& sm, Rows<T, DB>& r, const f32x16_t (&s)[N]) {
@@ -453,8 +460,8 @@ __device__ __forceinline__ void new_maximum(const ScoreMath& sm, Rows<T, DB>& r,
 #pragma unroll
     for (int i = 0; i < 16; ++i) top = fmaxf(top, s[n][i]);
   top = other_half_max(top);
-  const float scaled = top * sm.c;
-  if (__any(scaled > r.m + kLag)) {
+  const float scaled = top * sm.c - Reference<T>::kTop;
+  if (__any(scaled > r.m + Reference<T>::kLag)) {
     const float m = fmaxf(r.m, scaled);
     const float keep = r.m == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(r.m - m);
     r.m = m;

@@ -1,10 +1,12 @@
 """Edges of the operators on attention heads and the paged cache on the GPU."""
 
+import math
+
 import pytest
 import torch
 
 from gpu_util import gpu, need_gpu, say
-from heads_util import make_batch
+from heads_util import E, close, half_eps, make_batch
 
 pytestmark = gpu
 DEV = "cuda"
@@ -35,3 +37,57 @@ def test_serving_refuses_forward_mode(recorded):
                 dual = fw.make_dual(args[name], torch.ones_like(args[name]))
                 with pytest.raises(RuntimeError, match="forward-mode"):
                     fn(**{**args, name: dual})
+
+
+# ---------------------------------------------------------------------------
+# Attention at its edges
+# ---------------------------------------------------------------------------
+def one_hot_call(scores, dtype, dim, tokens=1, heads=(2, 1), page=16, seed=22):
+    """A call of one sequence whose key j has the score scores[j] in every row, exactly: the
+    queries are 1 in their first element alone, where the keys hold their score (scale 1).
+    Returns (arguments, values [keys, kv heads, dim] that the caller may overwrite)."""
+    g = torch.Generator().manual_seed(seed)
+    n = len(scores)
+    pages, lens, starts, total = make_batch([tokens], [n], page, seed)
+    q = torch.zeros(tokens, heads[0], dim, dtype=dtype)
+    q[..., 0] = 1.0
+    kc = torch.zeros(total, page, heads[1], dim, dtype=dtype)
+    vc = torch.randn(total, page, heads[1], dim, generator=g).to(dtype)
+    j = torch.arange(n)
+    at = pages[0, j // page].long(), j % page
+    kc[..., 0][at] = scores.to(dtype)[:, None]
+    return [q, kc, vc, pages, lens, starts], at
+
+
+def attend_on_gpu(args, **kw):
+    from kernels.hip.paged_attention import kernel_fn
+    return kernel_fn(*(t.to(DEV) for t in args), **kw)
+
+
+@pytest.mark.parametrize("tokens, hint", [(1, 1), (1, 100), (40, 40)])
+@pytest.mark.parametrize("below", [12.0, 15.0, 17.5])
+def test_small_weights_of_fp16(below, tokens, hint):
+    """One key far above n equal ones: their weights e^-below keep their digits in the product.
+
+    Bound: a weight is rounded once, u = 2^-11 of it while it is normal in fp16; with the row's
+    top at 2^11 or more, one below 2^-14 is off by half of 2^-24, 2^-36 of the top, and the top
+    is at most the row's sum: 2^-36 sum |v| in all. The rest as in attend_bound; the scores are
+    exact, the exponential's argument is within E |s - top| log2(e), its result within 2 E."""
+    need_gpu()
+    n, dim, dtype = 8192, 64, torch.float16
+    say("small weights", below, tokens, hint)
+    scores = torch.full((n,), -below)
+    scores[3] = 0.0
+    args, at = one_hot_call(scores, dtype, dim, tokens)
+    args[2][at] = 100.0 + torch.arange(dim, dtype=dtype)  # (one row: every key's value)
+    args[2][at[0][3], at[1][3]] = 0.0                     # the top key's
+    got = attend_on_gpu(args, scale=1.0, max_chunk=hint)
+    for head in range(2):
+        for t in range(tokens):
+            seen = n - tokens + t + 1
+            w = (seen - 1) * math.exp(-below)
+            want = (100.0 + torch.arange(dim, dtype=torch.float64)) * (w / (1.0 + w))
+            mass = want
+            rest = 2.0 ** -36 * seen * (100.0 + dim)
+            bound = (2 * half_eps(dtype) + 2 * (2 * below + 8) * E + 2 * (n / 32 + 64) * E) * mass + rest + 2.0 ** -25
+            close(got[t, head], want, bound, f"{below} {t} {head}")
