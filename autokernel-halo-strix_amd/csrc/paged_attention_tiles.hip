@@ -409,9 +409,11 @@ __device__ __forceinline__ f32x16_t scores32(const Rows<T, DB>& r, const char* k
 
 // Capped scores. Of 16-bit types and caps up to kQuickCap: softcap tanh(x) is softcap -
 // 2 softcap / (exp(2 x) + 1), whose first term a softmax does not see. Its error of up to
-// 4 softcap 2^-24 is absolute, 2^-14 at most, a quarter of a weight's rounding; others take
-// the form with small results' own precision. (16 sequences of up to 7000 keys, chunks of up
-// to 500 tokens, 32 + 8 heads of 128: 361 us, in the other form 458 (each beside the other).)
+// 4 softcap 2^-24 is absolute, 2^-14 at most, a quarter of a weight's rounding. (16 sequences of
+// up to 7000 keys, chunks of up to 500 tokens, 32 + 8 heads of 128: 361 us, with tanh_f32 458
+// (each beside the other).) Beyond, fp16 and fp32 take cap_tanh, whose error is relative to the
+// score; bf16 tanh_f32, whose error of up to softcap 2^-24 is a third of its weights' rounding at
+// the largest cap (prompts of 4 x 2048 tokens, 32 + 8 heads of 128, 287 us, with cap_tanh 348).
 constexpr float kQuickCap = 256.0f;
 
 template <typename T>
@@ -421,7 +423,10 @@ __device__ __forceinline__ void cap32(const ScoreMath& sm, f32x16_t& s) {
     for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_rcpf(-1.0f - __builtin_amdgcn_exp2f(s[i] * sm.cap_in));
   } else {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) s[i] = sm.cap_out * tanh_f32(s[i] * sm.cap_in);
+    for (int i = 0; i < 16; ++i) {
+      const float x = s[i] * sm.cap_in;
+      s[i] = sm.cap_out * (std::is_same<T, bf16>::value ? tanh_f32(x) : cap_tanh(x));
+    }
   }
 }
 

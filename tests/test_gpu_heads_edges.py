@@ -91,3 +91,37 @@ def test_small_weights_of_fp16(below, tokens, hint):
             rest = 2.0 ** -36 * seen * (100.0 + dim)
             bound = (2 * half_eps(dtype) + 2 * (2 * below + 8) * E + 2 * (n / 32 + 64) * E) * mass + rest + 2.0 ** -25
             close(got[t, head], want, bound, f"{below} {t} {head}")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("dim", [64, 66])
+@pytest.mark.parametrize("cap", [1.0, 30.0, 256.0, 300.0, 1e4])
+def test_caps_keep_the_digits_of_scores(cap, dim, dtype):
+    """The cap's error is relative to the score: x = s / cap within 2 E, tanh within 8 E, its
+    product with the cap within 2 E: rho = 12 E |s|, and for fp16 with caps up to 256 and bf16
+    besides an absolute one, 4 cap 2^-24 (the dot product is exact here). Then the exponential: its argument
+    within 2 E (|s| + spread), its result within 4 E; a weight's error rho moves the quotient by
+    2 rho sum p |v| at most. The two sums are chains of at most as many terms as keys are seen,
+    64 and a 32nd of them, and the 8 of joining and dividing."""
+    need_gpu()
+    g = torch.Generator().manual_seed(23)
+    for n, tokens, spread in ((600, 3, 10.0), (600, 3, 1e-3), (600, 3, 100.0), (4, 2, 4.0), (5, 3, 1.0), (6, 1, 3.0)):
+        say("cap", cap, dim, dtype, n, spread)
+        scores = (spread * (2 * torch.rand(n, generator=g) - 1)).to(dtype).float()
+        args, at = one_hot_call(scores, dtype, dim, tokens)
+        values = args[2][at][:, 0].double()
+        for hint in (1, 100):
+            got = attend_on_gpu(args, scale=1.0, softcap=cap, max_chunk=hint)
+            for t in range(tokens):
+                seen = n - tokens + t + 1
+                s = cap * torch.tanh(scores[:seen].double() / cap)
+                p = torch.softmax(s, 0)[:, None]
+                want, mass = (p * values[:seen]).sum(0), (p * values[:seen].abs()).sum(0)
+                size = float(s.abs().max())
+                rho = 12 * E * size + 6 * E * size + 8 * E
+                quick = dtype == torch.bfloat16 or (dtype == torch.float16 and cap <= 256)
+                rho += 4 * cap * E if quick else 0.0
+                u = half_eps(dtype) if dtype != torch.float32 else 0.0
+                bound = half_eps(dtype) * want.abs() + (u + 2 * math.expm1(rho) + 2 * (seen / 32 + min(seen, 64) + 8) * E) * mass
+                for head in range(2):
+                    close(got[t, head], want, bound, f"cap {cap}, {n} scores to {spread}, hint {hint}, row {t}")
