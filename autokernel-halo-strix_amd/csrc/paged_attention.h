@@ -54,15 +54,17 @@ __device__ __forceinline__ float cap_tanh(float x) {
   return copysignf(r, x);
 }
 
+// A row's scores as the running maximum takes them: capped, or the bare products, whose factor
+// joins in the exponents (a product that fp32 holds counts as itself whatever the factor).
 __device__ __forceinline__ float score_of(const AttendArgs& a, float dot) {
-  const float s = dot * a.scale;
-  return a.softcap > 0.0f ? a.softcap * cap_tanh(s / a.softcap) : s;
+  return a.softcap > 0.0f ? a.softcap * cap_tanh(dot * a.scale / a.softcap) : dot;
 }
+__device__ __forceinline__ float score_factor(const AttendArgs& a) { return a.softcap > 0.0f ? 1.0f : a.scale; }
 
-// exp(s - m); beside a maximum of -inf (nothing seen yet, or NaN alone, which the
+// exp(factor (s - m)); beside a maximum of -inf (nothing seen yet, or NaN alone, which the
 // maximum passes over) 0 or that NaN.
-__device__ __forceinline__ float weight_of(float s, float m) {
-  return m == kNegInf ? (s == s ? 0.0f : s) : fast_exp(s - m);
+__device__ __forceinline__ float weight_of(float s, float m, float factor) {
+  return m == kNegInf ? (s == s ? 0.0f : s) : fast_exp((s - m) * factor);
 }
 
 // The kernels on the matrix cores (paged_attention_tiles.hip): fp16 / bf16 of head

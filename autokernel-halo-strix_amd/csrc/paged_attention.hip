@@ -29,6 +29,7 @@ __global__ void __launch_bounds__(256) attend_any_kernel(AttendArgs a, int64_t r
   __shared__ float sums[4][kMaxAttendDim];
   __shared__ float stat[4][2];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const float factor = score_factor(a);
   // (a row's sums are read before the next row's first barrier, and written after it)
   for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
     const int64_t token = (uint32_t)row / (uint32_t)a.q_heads;
@@ -64,8 +65,8 @@ __global__ void __launch_bounds__(256) attend_any_kernel(AttendArgs a, int64_t r
         s = score_of(a, dot);
       }
       const float top = fmaxf(m, wave_max(s));
-      const float p = page >= 0 ? weight_of(s, top) : 0.0f;
-      const float keep = weight_of(m, top);
+      const float p = page >= 0 ? weight_of(s, top, factor) : 0.0f;
+      const float keep = weight_of(m, top, factor);
       m = top;
       l = l * keep + p;
       prob[wave][lane] = p;
@@ -100,7 +101,7 @@ __global__ void __launch_bounds__(256) attend_any_kernel(AttendArgs a, int64_t r
     for (int w = 0; w < 4; ++w) top = fmaxf(top, stat[w][0]);
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      f[w] = weight_of(stat[w][0], top);
+      f[w] = weight_of(stat[w][0], top, factor);
       total += f[w] * stat[w][1];
     }
     if (a.splits > 1) {
@@ -130,11 +131,12 @@ __global__ void __launch_bounds__(256) attend_any_join_kernel(AttendArgs a, int6
   const int h = (int)(row - token * a.q_heads);
   if (sequence_of(a.seq, (int)token) < 0 && !a.zero_other) return;
   const float* part = a.part + row * a.splits * (a.dim + 2);
+  const float factor = score_factor(a);
   float top = kNegInf, total = 0.0f;
   for (int s = 0; s < a.splits; ++s) top = fmaxf(top, part[(int64_t)s * (a.dim + 2) + a.dim]);
   for (int s = 0; s < a.splits; ++s) {
     const float* x = part + (int64_t)s * (a.dim + 2) + a.dim;
-    total += weight_of(x[0], top) * x[1];
+    total += weight_of(x[0], top, factor) * x[1];
   }
   const float inv = total == 0.0f ? 0.0f : 1.0f / total;
   T* out = static_cast<T*>(a.out) + token * a.o_st + h * a.o_sh;
@@ -142,7 +144,7 @@ __global__ void __launch_bounds__(256) attend_any_join_kernel(AttendArgs a, int6
     float sum = 0.0f;
     for (int s = 0; s < a.splits; ++s) {
       const float* x = part + (int64_t)s * (a.dim + 2);
-      sum += weight_of(x[a.dim], top) * x[d];
+      sum += weight_of(x[a.dim], top, factor) * x[d];
     }
     out[d] = from_f32<T>(sum * inv);
   }

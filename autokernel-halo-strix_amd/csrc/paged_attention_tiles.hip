@@ -46,7 +46,8 @@ struct TileArgs {
   int64_t* line;                   // [batch + 1]: the units before each sequence
   Job* jobs;                       // [workers]
   float* part;                     // [2 workers]: sums of products, maxima, sums of a tile's rows
-  float c, cap_in, cap_out;        // scores in base 2: c s; cap_in > 0: c cap(s), see cap32
+  float c, cap_in, cap_out;        // exponents in base 2: c s; cap_in > 0: c cap(s), see cap32
+  float unit2;                     // the references' unit as an exponent in base 2: 1, or c, see Reference
 };
 
 // The kernels' argument where the launch left it. Held in registers all of it would crowd
@@ -331,18 +332,19 @@ template <typename T, int DB>
 struct Rows {
   u32x4 q[Shape<T, DB>::kSteps];
   f32x16_t o[Shape<T, DB>::kBlocks];
-  float m, l;     // what the weights are taken beside (base 2; the lane's query) and this half's sum
+  float m, l;     // what the weights are taken beside (the lane's query) and this half's sum
   int lo, hi;     // the keys that the query sees
   int top, low;   // of the wave's rows: the least hi, the largest lo
   int beg, end;   // of the wave's rows: the keys that some of them see
 };
 
-// Scores in base 2.
+// From scores to exponents in base 2 (Reference has the rest).
 struct ScoreMath {
-  float c, cap_in, cap_out;
-  bool cap;
+  float c, cap_in, cap_out, to_unit, lag;
+  bool cap, bare;
 };
-__device__ __forceinline__ ScoreMath score_math(Args g) { return {g->c, g->cap_in, g->cap_out, g->cap_in > 0.0f}; }
+template <typename T>
+__device__ __forceinline__ ScoreMath score_math(Args g);
 
 // Loads the queries of rows [row0, row0 + 32) of a tile.
 template <typename T, int DB>
@@ -451,28 +453,54 @@ __device__ __forceinline__ void hide32(const Rows<T, DB>& r, f32x16_t& s, int ke
 // and below 2^-14 they lose digits, so they stand as high as they can, at 2^11 to 2^15: one
 // keeps all of its digits down to 2^-25 of the row's largest, and is off by 2^-36 of it below
 // (from 1 on, 8192 weights of 2^-25 each were left out of the products and counted in the sum).
+//
+// m is an exponent in base 2, c s - kTop, and a weight exp2(c s - m), one operation on the score.
+// With c past 1 a finite score may leave fp32 there (bf16's lowest value times a scale of 1):
+// then m is a score itself (its unit is c) and a weight exp2(c (s - m)).
 template <typename T>
 struct Reference {
   static constexpr bool kHalf = std::is_same<T, f16>::value;
   static constexpr float kLag = kHalf ? 4.0f : 8.0f, kTop = kHalf ? 11.0f : 0.0f;
+  static constexpr bool kBare = !kHalf;  // (fp16's products end at 2^40)
+  // What sums beside m are worth beside top (at least m).
+  static __device__ __forceinline__ float factor(float m, float top, float unit2) {
+    return top == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(kBare ? (m - top) * unit2 : m - top);
+  }
 };
 
+template <typename T>
+__device__ __forceinline__ ScoreMath score_math(Args g) {
+  const bool bare = Reference<T>::kBare && g->unit2 != 1.0f;
+  return {g->c, g->cap_in, g->cap_out, bare ? 1.0f : g->c, bare ? Reference<T>::kLag / g->unit2 : Reference<T>::kLag,
+          g->cap_in > 0.0f, bare};
+}
+
+// Raises the references where N x 32 new scores ask for it, and makes the scores ready for
+// weights32 (bare ones: less the reference).
 template <typename T, int DB, int N>
-__device__ __forceinline__ void new_maximum(const ScoreMath& sm, Rows<T, DB>& r, const f32x16_t (&s)[N]) {
+__device__ __forceinline__ void new_maximum(const ScoreMath& sm, Rows<T, DB>& r, f32x16_t (&s)[N]) {
+  using R = Reference<T>;
   float top = s[0][0];
 #pragma unroll
   for (int n = 0; n < N; ++n)
 #pragma unroll
     for (int i = 0; i < 16; ++i) top = fmaxf(top, s[n][i]);
   top = other_half_max(top);
-  const float scaled = top * sm.c - Reference<T>::kTop;
-  if (__any(scaled > r.m + Reference<T>::kLag)) {
-    const float m = fmaxf(r.m, scaled);
-    const float keep = r.m == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(r.m - m);
+  const float x = fmaf(top, sm.to_unit, -R::kTop);
+  if (__any(x > r.m + sm.lag)) {
+    const float m = fmaxf(r.m, x);
+    const float keep = r.m == kNegInf ? 0.0f : R::factor(r.m, m, sm.bare ? sm.c : 1.0f);
     r.m = m;
     r.l *= keep;
 #pragma unroll
     for (int b = 0; b < Shape<T, DB>::kBlocks; ++b) r.o[b] *= keep;
+  }
+  if (R::kBare && __builtin_expect(sm.bare, 0)) {
+    const float m = r.m == kNegInf ? 0.0f : r.m;
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[n][i] -= m;
   }
 }
 
@@ -486,7 +514,7 @@ struct Weights {
 template <typename T, int DB>
 __device__ __forceinline__ Weights<T> weights32(const ScoreMath& sm, Rows<T, DB>& r, const f32x16_t& s) {
   // (nothing seen yet: every score is -inf or NaN, and the weight 0 or NaN)
-  const float m = r.m == kNegInf ? 0.0f : r.m;
+  const float m = r.m == kNegInf || (Reference<T>::kBare && sm.bare) ? 0.0f : r.m;
   float p[16];
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
@@ -949,7 +977,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, DB * sizeof(T) <= 256 ? 2 : 1)
 
   char* const kl = lds[wave];
   char* const vl = lds[wave] + 32 * S::kPitch;
-  const ScoreMath sm = score_math(g);
+  const ScoreMath sm = score_math<T>(g);
   const Cache cache = cache_of<T, DB>(g);
   Loads<T, DB, N, S::vPitch> x;
   LookUp next;
@@ -1087,7 +1115,7 @@ __global__ void __launch_bounds__(64 * WAVES) attend_many_kernel(TileArgs, bool 
   place_in_sequence(g, p, in_tile, next_at - at);
   const int row0 = wave * kRows, first = wave * S::kPerLoad;
   constexpr int stride = WAVES * S::kPerLoad;
-  const ScoreMath sm = score_math(g);
+  const ScoreMath sm = score_math<T>(g);
   const Cache cache = cache_of<T, DB>(g);
 
   // this wave's units on their way: the one that it looks up next
@@ -1275,11 +1303,11 @@ __global__ void __launch_bounds__(256) attend_join_many_kernel(TileArgs) {
   f32x16_t o[DB / 32];
 #pragma unroll
   for (int b = 0; b < DB / 32; ++b) o[b] = f32x16_t{};
+  const float unit2 = g->unit2;
   float top = kNegInf, sum = 0.0f;
   // adds (ml, what `from` gives) to the sums
   const auto add = [&](f32x2_v ml, auto from) {
-    const float now = fmaxf(top, ml[0]);
-    const float keep = now == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(top - now), f = now == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(ml[0] - now);
+    const float now = fmaxf(top, ml[0]), keep = Reference<T>::factor(top, now, unit2), f = Reference<T>::factor(ml[0], now, unit2);
     top = now;
     sum = sum * keep + ml[1] * f;
 #pragma unroll
@@ -1334,7 +1362,8 @@ __global__ void __launch_bounds__(256) attend_join_kernel(TileArgs) {
       if (64 * v + lane < g->a.dim) out[64 * v + lane] = from_f32<T>(acc[v] * inv);
   };
   typedef float f32x2_a __attribute__((ext_vector_type(2), aligned(8)));
-  const auto factor = [](float m, float top) { return top == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(m - top); };
+  const float unit2 = g->unit2;
+  const auto factor = [&](float m, float top) { return Reference<T>::factor(m, top, unit2); };
   if (parts <= 8) {
     // R rows a wave, their loads together; a row's maxima and sums in every lane
     constexpr int R = 4;
@@ -1524,6 +1553,8 @@ void attend_tiles(const AttendArgs& a, int64_t max_chunk, int dtype, void* works
   } else {
     g.c = a.scale * kLog2e;
   }
+  // (capped scores stay below 2^15 in base 2)
+  g.unit2 = a.softcap == 0.0f && g.c > 1.0f && dtype != AK_DTYPE_F16 ? g.c : 1.0f;
   if (dtype == AK_DTYPE_F32) launch_type<float>(g, p, s);
   else if (dtype == AK_DTYPE_F16) launch_type<f16>(g, p, s);
   else launch_type<bf16>(g, p, s);

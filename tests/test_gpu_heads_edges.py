@@ -6,7 +6,8 @@ import pytest
 import torch
 
 from gpu_util import gpu, need_gpu, say
-from heads_util import E, close, half_eps, make_batch
+from heads_util import E, attend_bound, close, half_eps, make_batch
+from oracle import heads as oracle
 
 pytestmark = gpu
 DEV = "cuda"
@@ -91,6 +92,65 @@ def test_small_weights_of_fp16(below, tokens, hint):
             rest = 2.0 ** -36 * seen * (100.0 + dim)
             bound = (2 * half_eps(dtype) + 2 * (2 * below + 8) * E + 2 * (n / 32 + 64) * E) * mass + rest + 2.0 ** -25
             close(got[t, head], want, bound, f"{below} {t} {head}")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("dim", [64, 66])
+@pytest.mark.parametrize("tokens", [1, 70])
+def test_scores_near_the_ends_of_fp32(tokens, dim, dtype):
+    """Finite scores that leave fp32 in base 2 (beyond 2.36e38) are scores like others: equal
+    ones share the row, the larger win alone (they differ by far more than exp's range), in
+    every kernel, in whichever order and part they come. The mean of n equal weights carries
+    its sums' roundings, each weight being the same number: (n / 32 + 64 + 4) E, and u of the
+    result and of the 16-bit weight."""
+    need_gpu()
+    n = 1500
+    low = torch.finfo(dtype).min
+    for name, pick in (("all lowest", lambda s: s.fill_(low)),
+                       ("all highest", lambda s: s.fill_(-low)),
+                       ("the last above the lowest", lambda s: s.fill_(low).__setitem__(slice(900, 950), low * 0.75)),
+                       ("the first above the lowest", lambda s: s.fill_(low).__setitem__(slice(3, 9), low * 0.75)),
+                       ("ordinary ones beside the lowest", lambda s: s.fill_(low).__setitem__(slice(1000, 1003), 1.0)),
+                       ("the highest beside ordinary ones", lambda s: s.fill_(1.0).__setitem__(slice(700, 720), -low)),
+                       ("higher and higher", lambda s: s.fill_(-1.0).__setitem__(slice(40, 44), -low * 0.75)
+                        or s.__setitem__(slice(1300, 1330), -low))):
+        say(name, tokens, dim, dtype)
+        scores = torch.zeros(n)
+        pick(scores)
+        args, at = one_hot_call(scores, dtype, dim, tokens)
+        scores = scores.to(dtype).float()
+        values = args[2][at][:, 0].double()
+        for hint in (1, tokens):
+            got = attend_on_gpu(args, scale=1.0, max_chunk=hint)
+            for t in (0, tokens - 1):
+                seen = n - tokens + t + 1
+                s = scores[:seen]
+                win = s == s.max()
+                want = values[:seen][win].mean(0)
+                mass = values[:seen][win].abs().mean(0)
+                u = half_eps(dtype) if dtype != torch.float32 else 0.0
+                bound = half_eps(dtype) * want.abs() + (u + 2 * (n / 32 + 68) * E) * mass
+                for head in range(2):
+                    close(got[t, head], want, bound, f"{name}, hint {hint}, row {t}")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("scale", [1e-3, 0.69, 0.7, 1.0, 3.0])
+def test_scales(scale, dtype):
+    """Ordinary scores at scales on both sides of 1 / log2(e), cut among workers."""
+    need_gpu()
+    for counts, lengths, heads, dim in (([1, 1], [2500, 70], (4, 2), 64), ([70, 1], [901, 1500], (4, 2), 128), ([3], [600], (2, 1), 66)):
+        say("scale", scale, counts, dtype)
+        g = torch.Generator().manual_seed(25)
+        pages, lens, starts, total = make_batch(counts, lengths, 16, 25)
+        q = torch.randn(sum(counts), heads[0], dim, generator=g).to(dtype)
+        kc, vc = (torch.randn(total, 16, heads[1], dim, generator=g).to(dtype) for _ in range(2))
+        want, spread, reach, mass = oracle.attend(q, kc, vc, pages, lens, starts, scale, bounds=True)
+        bound = attend_bound(want, spread, reach, mass, max(lengths), dim, dtype)
+        if dtype == torch.float16:  # (weights below 2^-25 of the top, as above)
+            bound = bound + 2.0 ** -36 * max(lengths) * float(vc.abs().max())
+        for hint in (1, max(counts)):
+            close(attend_on_gpu([q, kc, vc, pages, lens, starts], scale=scale, max_chunk=hint), want, bound, f"{scale} {counts} {hint}")
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=str)
