@@ -629,10 +629,45 @@ __device__ __forceinline__ void values_unit(Rows<T, DB>& r, const Weights<T> (&p
   }
 }
 
+// The lane's query's weight of key j of 32, as the product takes it.
+template <typename T>
+__device__ __forceinline__ float weight_at(const Weights<T>& p, int j) {
+  const int lane = threadIdx.x & 63, i = 4 * (j >> 3) + (j & 3);  // its place in the half that has it
+  constexpr int kEach = 4 / (int)sizeof(T), kWords = 16 / kEach;
+  uint32_t x = 0;
+#pragma unroll
+  for (int k = 0; k < kWords; ++k) x = k == i / kEach ? p.w[k / 4][k % 4] : x;
+  x = (uint32_t)__shfl((int)x, (lane & 31) + 32 * ((j >> 2) & 1));
+  if constexpr (sizeof(T) == 4) return __uint_as_float(x);
+  else return to_f32(__builtin_bit_cast(T, (uint16_t)(i & 1 ? x >> 16 : x)));
+}
+
+// Which of a lane's 16 weights are 0 as the product takes them: bits in their order (for the
+// many-row kernel, which has no registers for the weights past their product).
+template <typename T>
+__device__ __forceinline__ uint32_t zero_weights(const Weights<T>& p) {
+  constexpr int kEach = 4 / (int)sizeof(T);
+  uint32_t bits = 0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const uint32_t w = p.w[i / kEach / 4][i / kEach % 4], x = sizeof(T) == 4 ? w << 1 : (w >> (16 * (i % 2))) << 17;
+    bits |= (x == 0 ? 1u : 0u) << i;
+    asm volatile("" : "+v"(bits));  // one after the other: this path is rare, its registers are not
+  }
+  return bits;
+}
+// The weight of key j, or 1 for any that is not 0.
+__device__ __forceinline__ float zero_or_one(uint32_t zero, int j) {
+  const int lane = threadIdx.x & 63;
+  const uint32_t its = (uint32_t)__shfl((int)zero, (lane & 31) + 32 * ((j >> 2) & 1));
+  return (its >> (4 * (j >> 3) + (j & 3))) & 1 ? 0.0f : 1.0f;
+}
+
 // What values that are not finite (left out of LDS where only some rows see them) do to
-// the rows that see their keys.
-template <typename T, int DB>
-__device__ __forceinline__ void add_not_finite(Args g0, const Place& p, Rows<T, DB>& r, int key0, uint32_t seen) {
+// the rows that see their keys: times their weights (weight(j)), as in the product, they are
+// themselves, or NaN beside a weight of 0.
+template <typename T, int DB, typename W>
+__device__ __forceinline__ void add_not_finite(Args g0, const Place& p, Rows<T, DB>& r, W weight, int key0, uint32_t seen) {
   const Args g = fresh(g0);
   const int half = (threadIdx.x & 63) >> 5, dim = g->a.dim;
   const PageMath math = page_math(g);
@@ -645,6 +680,7 @@ __device__ __forceinline__ void add_not_finite(Args g0, const Place& p, Rows<T, 
     const int64_t page = g->a.pages[(int64_t)p.b * g->a.ld_pages + i];  // (there: its bit is set)
     const T* v = v0 + page * g->a.vp + (int64_t)slot * g->a.vs;
     const bool sees = key < r.hi && key >= r.lo;
+    const float w = weight(j);
 #pragma unroll
     for (int blk = 0; blk < Shape<T, DB>::kBlocks; ++blk)
 #pragma unroll
@@ -654,7 +690,7 @@ __device__ __forceinline__ void add_not_finite(Args g0, const Place& p, Rows<T, 
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const float x = to_f32(v[d + e]);
-            if (sees && !(fabsf(x) < __builtin_inff())) r.o[blk][4 * c + e] += x;
+            if (sees && !(fabsf(x) < __builtin_inff())) r.o[blk][4 * c + e] += x * w;
           }
         }
         asm volatile("" ::: "memory");  // one load at a time: this path is rare, its registers are not
@@ -1014,8 +1050,9 @@ __global__ void __launch_bounds__(64 * kFewWaves, DB * sizeof(T) <= 256 ? 2 : 1)
       if (sm.cap) cap32<T>(sm, s[0]);
       if (mask) hide32<T, DB>(r, s[0], key, now);
       new_maximum<T, DB, 1>(sm, r, s);
-      values32<T, DB, S::vPitch>(r, weights32<T, DB>(sm, r, s[0]), vl, 0);
-      if (__any(bad)) add_not_finite<T, DB>(g, p, r, key, now);
+      const Weights<T> w = weights32<T, DB>(sm, r, s[0]);
+      values32<T, DB, S::vPitch>(r, w, vl, 0);
+      if (__any(bad)) add_not_finite<T, DB>(g, p, r, [&](int j) { return weight_at<T>(w, j); }, key, now);
     }
     left -= n;
     unit += n;
@@ -1206,19 +1243,26 @@ __global__ void __launch_bounds__(64 * WAVES) attend_many_kernel(TileArgs, bool 
   int key = uniform((p.k.u0 + unit) * UNIT), units = uniform(p.k.u1 - p.k.u0);
   Place following = p;
   Weights<T> w[NB];
+  int spoilt = 0;                   // unit j - 1 has values that are not finite where it is j
   for (int j = 0;; ++j) {
     __builtin_amdgcn_s_setprio(1);  // the matrix cores' wave first
     if (before) {
-      const int spoilt = bad[vget];  // (on its way during the products)
+      uint32_t zero = 0;
+      if (__builtin_expect(spoilt == j, 0)) {
+#pragma unroll
+        for (int b = 0; b < NB; ++b) zero |= zero_weights<T>(w[b]) << (16 * b);
+      }
       if constexpr (sizeof(T) == 2) {
         values_unit<T, DB, NB>(r, w, vl[vget]);
       } else {
 #pragma unroll
         for (int b = 0; b < NB; ++b) values32<T, DB, S::vWidePitch>(r, w[b], vl[vget], 32 * b);
       }
-      if (uniform(spoilt) == j) {
+      if (__builtin_expect(spoilt == j, 0)) {
         const uint64_t seen = seen_of(j - 1);
-        for (int b = 0; b < NB; ++b) add_not_finite<T, DB>(g, p, r, key - UNIT + 32 * b, (uint32_t)(seen >> (32 * b)));
+        for (int b = 0; b < NB; ++b)
+          add_not_finite<T, DB>(g, p, r, [&](int j) { return zero_or_one(zero >> (16 * b), j); }, key - UNIT + 32 * b,
+                                (uint32_t)(seen >> (32 * b)));
       }
     }
     // Queries that may be on their way are waited for here, where the unit's loads are, too:
@@ -1267,6 +1311,7 @@ __global__ void __launch_bounds__(64 * WAVES) attend_many_kernel(TileArgs, bool 
         for (int b = 0; b < NB; ++b) cap32<T>(sm, s[b]);
       }
       const uint64_t seen = seen_of(j);
+      const int spoilt_by = bad[vget + 1 == vSlots ? 0 : vget + 1];
       if (key < r.low || key + UNIT > r.top || seen != (UNIT == 64 ? ~0ull : 0xFFFFFFFFull)) {
 #pragma unroll
         for (int b = 0; b < NB; ++b) hide32<T, DB>(r, s[b], key + 32 * b, (uint32_t)(seen >> (32 * b)));
@@ -1274,6 +1319,7 @@ __global__ void __launch_bounds__(64 * WAVES) attend_many_kernel(TileArgs, bool 
       new_maximum<T, DB, NB>(sm, r, s);
 #pragma unroll
       for (int b = 0; b < NB; ++b) w[b] = weights32<T, DB>(sm, r, s[b]);
+      spoilt = uniform(spoilt_by);
     }
     before = now;
     ++unit;

@@ -13,10 +13,11 @@ One pass over the keys with a running maximum and sum in fp32
 (``csrc/paged_attention.hip``); the keys of few rows are cut over the whole GPU and
 joined in a fixed order, so results are reproducible.
 
-Rules at the edges: a key past the sequence's length, past the window, on a page
-outside the cache or with a score of -inf takes no part, whatever it or its value
-holds (a value takes part with what its weight of 0 gives it where only its score
-is -inf); a token that sees no key gives 0; a NaN score gives a NaN row.
+Rules at the edges: a key past the sequence's length, past the window or on a page
+outside the cache takes no part, whatever it or its value holds. A key that is seen
+with a score of -inf has the weight 0, and its value takes part with that (0 times
+what is not finite is NaN). A token that sees no key gives 0, as does one that sees
+only scores of -inf beside finite values; a NaN score gives a NaN row.
 
 For serving: it has no gradient. No counterpart in the reference.
 """

@@ -155,6 +155,40 @@ def test_scales(scale, dtype):
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=str)
 @pytest.mark.parametrize("dim", [64, 66])
+def test_values_that_are_not_finite_by_their_weights(dim, dtype):
+    """A value that is not finite takes part by its weight, wherever its unit's border falls:
+    an infinity times 0 (a score of -inf) is NaN, times a weight above 0 itself; rows that
+    do not see its key do not see it."""
+    need_gpu()
+    n, page = 300, 16
+    for tokens in (3, 100):
+        for key in (5, n - 2):            # in a unit that all rows see; in one that only some see
+            for value in (math.inf, -math.inf, math.nan):
+                for score in (-math.inf, 0.0):
+                    say("not finite", dim, dtype, tokens, key, value, score)
+                    scores = torch.zeros(n)
+                    scores[key] = score
+                    args, at = one_hot_call(scores, dtype, dim, tokens, page=page)
+                    want_clean = attend_on_gpu(args, scale=1.0, max_chunk=tokens)
+                    args[2][at[0][key], at[1][key], 0, 7] = value
+                    for hint in (1, tokens):
+                        got = attend_on_gpu(args, scale=1.0, max_chunk=hint)
+                        for t in range(tokens):
+                            x = got[t, :, 7]
+                            if n - tokens + t < key:
+                                assert torch.isfinite(x).all()
+                            elif score == 0.0 and not math.isnan(value):
+                                assert (x == value).all(), (t, x)
+                            else:
+                                assert torch.isnan(x).all(), (t, x)
+                        rest = [d for d in range(dim) if d != 7]
+                        assert torch.isfinite(got[..., rest]).all()
+                        if hint == tokens:
+                            assert torch.equal(got[..., rest], want_clean[..., rest])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("dim", [64, 66])
 @pytest.mark.parametrize("cap", [1.0, 30.0, 256.0, 300.0, 1e4])
 def test_caps_keep_the_digits_of_scores(cap, dim, dtype):
     """The cap's error is relative to the score: x = s / cap within 2 E, tanh within 8 E, its
