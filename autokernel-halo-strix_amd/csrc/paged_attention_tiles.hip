@@ -1519,7 +1519,7 @@ Plan plan_of(int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads, i
   // fp32 take four times as long)
   p.join_cost = (p.few ? 0.02f * (float)((p.rows + 15) / 16) : 0.2f) / (f32 ? 4.0f : 1.0f) / (float)tiles;
   p.line_bytes = (size_t)(batch + 2) / 2 * 16;
-  p.job_bytes = (size_t)p.workers * sizeof(Job);
+  p.job_bytes = ((size_t)p.workers * sizeof(Job) + 15) / 16 * 16;  // (the parts behind them are read 16 bytes at a time)
   const size_t part = p.few ? (size_t)p.rows * (size_t)(p.padded + 2) : (size_t)((p.rows + 31) / 32) * 32 * (size_t)(p.padded + 4);
   p.part_bytes = (size_t)p.workers * 2 * part * sizeof(float);
   return p;

@@ -3,7 +3,7 @@
 import pytest
 import torch
 
-from kernels.hip import paged_append, paged_attention, qk_norm_rotary, rotary
+from kernels.hip import _lib, paged_append, paged_attention, qk_norm_rotary, rotary
 from test_heads_cpu import _cache_call, heads_backend  # noqa: F401 (a fixture)
 
 
@@ -40,3 +40,16 @@ def test_training_operators_refuse_a_tables_tangents(heads_backend):  # noqa: F8
         for call in (lambda: rotary.kernel_fn(x, None, t), lambda: qk_norm_rotary.kernel_fn(x, None, w, None, t)):
             with pytest.raises(RuntimeError, match="forward-mode"):
                 call()
+
+
+@pytest.mark.skipif(not _lib.is_available(), reason="libautokernel_gfx950.so not built")
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+def test_attention_workspace_keeps_its_parts_aligned(dtype):
+    """Behind the line and the jobs stand parts that are read and written 16 bytes at a time: with
+    an odd number of workers, of many rows, their base has to be a multiple of 16 all the same.
+    (Parts of many rows are whole multiples of 16 bytes, so the total tells the base.)"""
+    size = _lib.load().ak_paged_attention_workspace_bytes
+    for tokens, batch, heads, dim, keys in ((150, 1, 2, 64, 192), (150, 1, 2, 128, 192), (150, 1, 1, 64, 192), (130, 1, 3, 64, 130),
+                                            (77, 1, 1, 64, 200), (333, 3, 5, 64, 64), (999, 2, 7, 256, 250)):
+        need = size(tokens, batch, heads, heads, dim, keys, tokens, dtype)
+        assert need > 0 and need % 16 == 0, (tokens, batch, heads, dim, keys, need)
