@@ -579,19 +579,19 @@ __global__ void __launch_bounds__(kThreads) heads_bwd_any_kernel(GradArgs ga) {
     ss = wave_sum(ss);
     gx = wave_sum(gx);
     const float inv = 1.0f / sqrtf(ss / (float)a.dim + a.eps);
-    const float back = inv * inv * (gx / (float)a.dim);
+    const float back = inv * (gx / (float)a.dim);  // (of order one, as n is, whatever the size of x)
     T* y = static_cast<T*>(r.dx) + row * a.dim;
     for (int i = lane; i < n; i += 64) {
       int e0, e1;
       float z0, z1;
       pair(i, e0, e1, z0, z1);
-      const float x0 = to_f32(o.x[e0]);
-      y[e0] = from_f32<T>(inv * (z0 * to_f32(w[e0]) - x0 * back));
-      mine[e0] = fmaf(z0, x0 * inv, mine[e0]);
+      const float n0 = to_f32(o.x[e0]) * inv;
+      y[e0] = from_f32<T>(inv * fmaf(z0, to_f32(w[e0]), -(n0 * back)));
+      mine[e0] = fmaf(z0, n0, mine[e0]);
       if (e1 >= 0) {
-        const float x1 = to_f32(o.x[e1]);
-        y[e1] = from_f32<T>(inv * (z1 * to_f32(w[e1]) - x1 * back));
-        mine[e1] = fmaf(z1, x1 * inv, mine[e1]);
+        const float n1 = to_f32(o.x[e1]) * inv;
+        y[e1] = from_f32<T>(inv * fmaf(z1, to_f32(w[e1]), -(n1 * back)));
+        mine[e1] = fmaf(z1, n1, mine[e1]);
       }
     }
   }

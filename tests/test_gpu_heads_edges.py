@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from gpu_util import gpu, need_gpu, say
-from heads_util import E, attend_bound, close, half_eps, make_batch
+from heads_util import E, attend_bound, close, half_eps, make_batch, partner_abs
 from oracle import heads as oracle
 
 pytestmark = gpu
@@ -219,3 +219,39 @@ def test_caps_keep_the_digits_of_scores(cap, dim, dtype):
                 bound = half_eps(dtype) * want.abs() + (u + 2 * math.expm1(rho) + 2 * (seen / 32 + min(seen, 64) + 8) * E) * mass
                 for head in range(2):
                     close(got[t, head], want, bound, f"cap {cap}, {n} scores to {spread}, hint {hint}, row {t}")
+
+
+# ---------------------------------------------------------------------------
+# Head norms at far scales
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("layout", ["vectors", "pairs", "offset"])
+@pytest.mark.parametrize("size", [3e-20, 1e-10, 1e18])
+def test_norm_gradients_at_far_scales(size, layout):
+    """eps 0, heads of far sizes, in rows of whole vectors and off them: gradients as large as
+    the inverse of the heads. Squares near 1e-39 are below fp32's normal range and carry half
+    of 2^-149 each, which is 8e-7 of the smallest sum here (64 times 9e-40), 4e-7 = 7 E of its root; the
+    rest as in the norm's bound, 48 E, twice over for the two products, of the terms' sizes."""
+    need_gpu()
+    from kernels.hip.qk_norm_rotary import kernel_fn
+    from kernels.hip.rotary import rotary_table
+    g = torch.Generator().manual_seed(24)
+    dim, rotary = (66, 22) if layout == "pairs" else (64, 64)
+    say("far scales", size, layout)
+    sign = torch.where(torch.rand(9, 3, dim, generator=g) < 0.5, -1.0, 1.0)
+    x = size * sign * (1.0 + 0.5 * torch.rand(9, 3, dim, generator=g))
+    up = torch.randn(9, 3, dim, generator=g)
+    w = 1 + 0.1 * torch.randn(dim, generator=g)
+    table = rotary_table(rotary, 16)
+    xd = x.to(DEV)
+    if layout == "offset":
+        xd = torch.empty(x.numel() + 1, device=DEV)[1:].view(x.shape).copy_(xd)
+    xd, wd = xd.requires_grad_(), w.to(DEV).requires_grad_()
+    y, _ = kernel_fn(xd, None, wd, None, table.to(DEV), eps=0.0)
+    dx, dw = torch.autograd.grad(y, (xd, wd), up.to(DEV))
+    want, want_w = oracle.norm_turn_grad(x, w, 0.0, table, torch.arange(9), up)
+    turned = partner_abs(up, rotary, False) * w.double().abs()
+    inv = 1.0 / torch.sqrt((x.double() ** 2).mean(-1, keepdim=True))
+    n = (x.double() * inv).abs()
+    terms = inv * (turned + n * (turned * n).mean(-1, keepdim=True))
+    close(dx, want, 128 * E * terms, "dx")
+    close(dw, want_w, 128 * E * (partner_abs(up, rotary, False) * n).sum((0, 1)) + 1e-37, "dweight")
