@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from gpu_util import gpu, need_gpu, say
-from heads_util import E, attend_bound, close, half_eps, make_batch, partner_abs
+from heads_util import E, attend_bound, close, half_eps, make_batch, partner_abs, tiny, turn_bound
 from oracle import heads as oracle
 
 pytestmark = gpu
@@ -255,3 +255,133 @@ def test_norm_gradients_at_far_scales(size, layout):
     terms = inv * (turned + n * (turned * n).mean(-1, keepdim=True))
     close(dx, want, 128 * E * terms, "dx")
     close(dw, want_w, 128 * E * (partner_abs(up, rotary, False) * n).sum((0, 1)) + 1e-37, "dweight")
+
+
+# ---------------------------------------------------------------------------
+# Bad pages, lengths and starts write where they should and nowhere else
+# ---------------------------------------------------------------------------
+GUARD = 77.0
+
+
+def guarded(t, lead=1, heads=1):
+    """(a view that holds t, what surrounds it): t [n, .., heads, dim] inside a larger tensor of
+    guards, `lead` rows and `heads` heads more on either side."""
+    shape = list(t.shape)
+    shape[0] += 2 * lead
+    shape[-2] += 2 * heads
+    buf = torch.full(shape, GUARD, dtype=t.dtype, device=DEV)
+    view = buf[lead:lead + t.shape[0]][..., heads:heads + t.shape[-2], :]
+    view.copy_(t)
+
+    def untouched():
+        rest = buf.clone()
+        rest[lead:lead + t.shape[0]][..., heads:heads + t.shape[-2], :] = GUARD
+        return bool((rest == GUARD).all())
+
+    return view, untouched
+
+
+BAD_APPENDS = [  # lengths, starts as given, ordered starts that mean the same (None: one token each)
+    ([3, 3, 7, 2], None, None),
+    ([9, -5, 2 ** 31 - 1, -2 ** 31], None, None),
+    ([1, 1, 1, 1], [5, 9, -3, 100, 2 ** 31 - 1], [0, 0, 0, 4, 4]),
+    ([8, 8, 8, 8], [3, 2, 1, 0, -1], [0, 0, 0, 0, 0]),
+    ([2, 4, 1, 8], [1, 2, 2, 2, 3], [1, 2, 2, 2, 3]),
+    ([2, 4, 8, 8], [0, 1, 4, 2 ** 31 - 1, 2 ** 31 - 1], [0, 1, 4, 4, 4]),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("dim", [64, 66])
+@pytest.mark.parametrize("case", BAD_APPENDS, ids=str)
+def test_bad_appends_stay_inside(case, dim, dtype):
+    need_gpu()
+    from kernels.hip import paged_append
+    from kernels.hip.rotary import rotary_table
+    lengths, starts, ordered = case
+    say("bad append", case, dim, dtype)
+    g = torch.Generator().manual_seed(26)
+    k, v, q = (torch.randn(4, h, dim, generator=g).to(dtype) for h in (2, 2, 3))
+    pages = torch.tensor([[9, 1], [-1, 0], [0, 2 ** 31 - 1], [-2 ** 31, 1]], dtype=torch.int32)
+    table = rotary_table(dim - 2, 8)
+    lens = torch.tensor(lengths, dtype=torch.int32)
+    kc, vc = (torch.randn(2, 4, 2, dim, generator=g).to(dtype) for _ in range(2))
+    kd, k_kept = guarded(kc)
+    vd, v_kept = guarded(vc)
+    qd, q_kept = guarded(torch.full_like(q, 5.0))
+    st = None if starts is None else torch.tensor(starts, dtype=torch.int32)
+    got = paged_append.kernel_fn(k.to(DEV), v.to(DEV), kd, vd, pages.to(DEV), lens.to(DEV), None if st is None else st.to(DEV),
+                                 q=q.to(DEV), table=table.to(DEV), q_out=qd)
+    assert got is qd and k_kept() and v_kept() and q_kept()
+    so = None if ordered is None else torch.tensor(ordered, dtype=torch.int32)
+    # (lengths near the ends of int32 are places past the table's width or before the first)
+    want_q, want_k, want_v = oracle.append(q, k, v, kc, vc, pages, lens, so, None, None, 0.0, table, False)
+    where = oracle.sequences(lengths, None if so is None else ordered, 4)
+    none = torch.tensor([b < 0 for b, _ in where])
+    want_q[none] = 5.0
+    close(qd, want_q, turn_bound(want_q.nan_to_num(), q, dim - 2, False, dtype), "q")
+    # (a place's turned key came from elements of at most the largest key's size)
+    off = half_eps(dtype) * want_k.abs() + 4 * E * 2 * float(k.abs().max()) + tiny(dtype)
+    close(kd, want_k, torch.where(want_k == kc.double(), 0.0, off), "k_cache")
+    assert torch.equal(vd.cpu().double(), want_v)
+    # without q_out the rows of no sequence are 0
+    fresh = paged_append.kernel_fn(k.to(DEV), v.to(DEV), kd, vd, pages.to(DEV), lens.to(DEV), None if st is None else st.to(DEV),
+                                   q=q.to(DEV), table=table.to(DEV))
+    assert not fresh[none.to(DEV)].any() and k_kept() and v_kept()
+
+
+BAD_STARTS = [  # as given, ordered starts that mean the same
+    ([0, 50, 43], [0, 43, 43]),
+    ([-9, 2 ** 31 - 1, 3], [0, 43, 43]),
+    ([43, 0, 0], [0, 0, 0]),
+    ([7, 7, 7], [7, 7, 7]),
+    ([20, 30, 25], [20, 30, 30]),
+    ([5, 6, 40], [5, 6, 40]),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("dim", [64, 66])
+@pytest.mark.parametrize("case", BAD_STARTS, ids=str)
+def test_bad_starts_of_attention_stay_inside(case, dim, dtype):
+    """Rows that have a sequence are its attention, the others stay as they were or are 0, and
+    nothing around the output is written."""
+    need_gpu()
+    from kernels.hip.paged_attention import kernel_fn
+    given, ordered = case
+    say("bad starts", case, dim, dtype)
+    g = torch.Generator().manual_seed(27)
+    pages, lens, _, total = make_batch([3, 40], [90, 100], 16, 27)
+    pages[0, 2], pages[1, 3] = -7, 2 ** 31 - 1
+    q = torch.randn(43, 4, dim, generator=g).to(dtype)
+    kc, vc = (torch.randn(total, 16, 2, dim, generator=g).to(dtype) for _ in range(2))
+    args = [t.to(DEV) for t in (q, kc, vc, pages, lens, torch.tensor(given, dtype=torch.int32))]
+    want, spread, reach, mass = oracle.attend(q, kc, vc, pages, lens, torch.tensor(ordered), 1 / math.sqrt(dim), bounds=True)
+    bound = attend_bound(want, spread, reach, mass, 100, dim, dtype)
+    none = torch.tensor([b < 0 for b, _ in oracle.sequences(lens.tolist(), ordered, 43)])
+    for hint in (1, 43):
+        out, kept = guarded(torch.full_like(q, 5.0))
+        assert kernel_fn(*args, max_chunk=hint, out=out) is out and kept()
+        assert (out[none.to(DEV)] == 5).all()
+        close(out.cpu()[~none], want[~none], bound[~none], f"hint {hint}")
+        fresh = kernel_fn(*args, max_chunk=hint)
+        assert not fresh[none.to(DEV)].any() and torch.equal(fresh.cpu()[~none], out.cpu()[~none])
+
+
+def test_lengths_past_the_table_are_cut():
+    """Lengths past the page table's width: the token sees the positions that the table has."""
+    need_gpu()
+    from kernels.hip.paged_attention import kernel_fn
+    for dtype, dim in ((torch.bfloat16, 64), (torch.float32, 66)):
+        say("long lengths", dtype, dim)
+        g = torch.Generator().manual_seed(28)
+        pages = torch.tensor([[2, 0, 1], [3, 4, 5]], dtype=torch.int32)
+        q = torch.randn(2, 4, dim, generator=g).to(dtype)
+        kc, vc = (torch.randn(6, 16, 2, dim, generator=g).to(dtype) for _ in range(2))
+        want, spread, reach, mass = oracle.attend(q, kc, vc, pages, torch.tensor([48, 48]), None, 0.2, bounds=True)
+        bound = attend_bound(want, spread, reach, mass, 48, dim, dtype)
+        for lengths in ([2 ** 31 - 1, 49], [10 ** 6, 2 ** 31 - 1]):
+            out, kept = guarded(torch.full_like(q, 5.0))
+            kernel_fn(*(t.to(DEV) for t in (q, kc, vc, pages, torch.tensor(lengths, dtype=torch.int32))), scale=0.2, out=out)
+            assert kept()
+            close(out, want, bound, str(lengths))
