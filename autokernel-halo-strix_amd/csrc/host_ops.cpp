@@ -919,6 +919,44 @@ bool dense_places(const Tensor& t) {
   return true;
 }
 
+// n spans of `length` elements, `pitch` apart (n 0: strides of another kind, or nothing there).
+struct Spans {
+  int64_t n = 0, pitch = 0, length = 0;
+};
+
+Spans spans_of(const Tensor& t) {
+  std::array<std::pair<int64_t, int64_t>, 4> d;
+  int n = 0;
+  if (t.numel() == 0 || t.dim() > 4) return {};
+  for (int64_t i = 0; i < t.dim(); ++i)
+    if (t.size(i) > 1) d[n++] = {t.stride(i), t.size(i)};
+  std::sort(d.begin(), d.begin() + n);
+  int64_t length = 1;
+  int i = 0;
+  while (i < n && d[i].first == length) length *= d[i++].second;
+  if (i + 1 < n) return {};
+  if (i < n) return {d[i].second, d[i].first, length};
+  return {1, length, length};
+}
+
+// Whether two tensors of one type are sure to share a place, as far as each is one run of
+// elements, or rows at one pitch (the parts of a fused projection).
+bool share_memory(const Tensor& a, const Tensor& b) {
+  const Spans x = spans_of(a), y = spans_of(b);
+  if (x.n == 0 || y.n == 0 || (x.n > 1 && y.n > 1 && x.pitch != y.pitch)) return false;
+  const int64_t pitch = x.n > 1 ? x.pitch : y.pitch;
+  const auto floor_div = [](int64_t p, int64_t q) { return p / q - (p % q != 0 && (p < 0) != (q < 0)); };
+  const int64_t apart = floor_div(static_cast<char*>(b.data_ptr()) - static_cast<char*>(a.data_ptr()), a.element_size());
+  // spans i and j meet where apart - x's length < (i - j) pitch < apart + y's length
+  const int64_t least = std::max(floor_div(apart - x.length, pitch) + 1, 1 - y.n);
+  const int64_t most = std::min(-floor_div(-apart - y.length, pitch) - 1, x.n - 1);
+  return least <= most;
+}
+
+bool same_places(const Tensor& a, const Tensor& b) {
+  return a.data_ptr() == b.data_ptr() && a.sizes() == b.sizes() && a.strides() == b.strides();
+}
+
 bool table_ok(const Tensor& t, int64_t dim) {
   return t.dim() == 2 && dense_f32(t) && t.size(0) > 0 && t.size(1) >= 2 && t.size(1) % 2 == 0 && t.size(1) <= dim &&
          !t.requires_grad();
@@ -1115,8 +1153,10 @@ std::optional<std::tuple<bool, Tensor>> paged_append(const Tensor& k, const Tens
   if (code_of(type) < 0 || !rows3(k, type) || !rows3(v, type) || k.sizes() != v.sizes() || k.numel() == 0) return std::nullopt;
   const int64_t tokens = k.size(0), heads = k.size(1), dim = k.size(2);
   if (dim > kMaxHeadDim || !paged_args(k_cache, v_cache, pages, lengths, starts, heads, dim, type, tokens) || !dense_places(k_cache) ||
-      !dense_places(v_cache) || ptr(k_cache) == ptr(v_cache) || (q ? !rows3(*q, type) || q->size(0) != tokens || q->size(2) != dim : q_weight || q_out) ||
-      (q_out && (!rows3(*q_out, type) || q_out->sizes() != q->sizes() || !dense_places(*q_out))) || (q_weight && !weight_ok(*q_weight, k)) ||
+      !dense_places(v_cache) || ptr(k_cache) == ptr(v_cache) || share_memory(k_cache, v_cache) || (q ? !rows3(*q, type) || q->size(0) != tokens || q->size(2) != dim : q_weight || q_out) ||
+      (q_out && (!rows3(*q_out, type) || q_out->sizes() != q->sizes() || !dense_places(*q_out) ||
+                 (!same_places(*q_out, *q) && share_memory(*q_out, *q)) || share_memory(*q_out, k) || share_memory(*q_out, v) ||
+                 share_memory(*q_out, k_cache) || share_memory(*q_out, v_cache))) || (q_weight && !weight_ok(*q_weight, k)) ||
       (k_weight && !weight_ok(*k_weight, k)) || (table && !table_ok(*table, dim)))
     return std::nullopt;
   const Tensor qq = q.value_or(Tensor()), qw = q_weight.value_or(Tensor()), kw = k_weight.value_or(Tensor()),
@@ -1144,7 +1184,8 @@ Maybe paged_attention(const Tensor& q_, const Tensor& k_cache, const Tensor& v_c
   if (code_of(type) < 0 || !rows3(q_, type) || q_.numel() == 0 || k_cache.dim() != 4) return std::nullopt;
   const int64_t tokens = q_.size(0), heads = q_.size(1), dim = q_.size(2), kv = k_cache.size(2), esz = q_.element_size();
   if (dim > kMaxAttendDim || kv < 1 || heads % kv || !paged_args(k_cache, v_cache, pages, lengths, starts, kv, dim, type, tokens) ||
-      (out_ && (!rows3(*out_, type) || out_->sizes() != q_.sizes() || !dense_places(*out_))))
+      (out_ && (!rows3(*out_, type) || out_->sizes() != q_.sizes() || !dense_places(*out_) ||
+                (!same_places(*out_, q_) && share_memory(*out_, q_)) || share_memory(*out_, k_cache) || share_memory(*out_, v_cache))))
     return std::nullopt;
   const Tensor st = starts.value_or(Tensor());
   Tensor out = out_.value_or(Tensor());

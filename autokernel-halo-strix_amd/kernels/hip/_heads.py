@@ -96,6 +96,43 @@ def dense_places(t: torch.Tensor) -> bool:
     return True
 
 
+def _spans(t: torch.Tensor) -> Optional[Tuple[int, int, int]]:
+    """``(n, pitch, length)``: t fills n spans of `length` elements, `pitch` apart; None where
+    its strides are of another kind."""
+    length, rest = 1, []
+    for stride, size in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n > 1):
+        if not rest and stride == length:
+            length *= size
+        else:
+            rest.append((size, stride, length))
+    return None if len(rest) > 1 else rest[0] if rest else (1, length, length)
+
+
+def share_memory(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two tensors of one type are sure to share a place: as far as each is one run of
+    elements, or rows at one pitch (the parts of a fused projection)."""
+    if a.numel() == 0 or b.numel() == 0 or a.device != b.device:
+        return False
+    x, y = _spans(a), _spans(b)
+    if x is None or y is None or (x[0] > 1 and y[0] > 1 and x[1] != y[1]):
+        return False
+    pitch = x[1] if x[0] > 1 else y[1]
+    apart = (b.data_ptr() - a.data_ptr()) // a.element_size()
+    # spans i and j meet where apart - x's length < (i - j) pitch < apart + y's length
+    least = max((apart - x[2]) // pitch + 1, 1 - y[0])
+    most = min(-((-apart - y[2]) // pitch) - 1, x[0] - 1)
+    return least <= most
+
+
+def check_apart(out: torch.Tensor, name: str, may_be: Optional[torch.Tensor], **others: torch.Tensor) -> None:
+    """Refuse an output that shares memory with what is read (or written) beside it; it may be
+    `may_be` itself, whose rows are read before they are written."""
+    for other, t in others.items():
+        itself = t is may_be and out.data_ptr() == t.data_ptr() and out.shape == t.shape and out.stride() == t.stride()
+        if not itself and share_memory(out, t):
+            raise ValueError(f"{name} shares memory with {other}")
+
+
 def check_cache(k_cache: torch.Tensor, v_cache: torch.Tensor, heads: int, dim: int, dtype: torch.dtype) -> None:
     for t, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
         if t.dim() != 4 or t.shape[1] < 1 or tuple(t.shape[2:]) != (heads, dim):
@@ -152,4 +189,4 @@ def wrote(*tensors: torch.Tensor) -> None:
 
 
 __all__ = ["Heads", "as_heads", "check_table", "check_positions", "no_gradient", "check_cache", "check_batch", "Batch",
-           "check_out", "dense_places", "wrote", "MAX_HEAD_DIM", "_lib"]
+           "check_out", "check_apart", "share_memory", "dense_places", "wrote", "MAX_HEAD_DIM", "_lib"]

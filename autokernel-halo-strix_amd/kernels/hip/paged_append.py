@@ -54,7 +54,8 @@ def kernel_fn(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: 
         table, interleaved: as in ``kernels.hip.rotary``; None: no rotation. A
             position past the table is written as NaN.
         q_out: where q's result goes (rows of no sequence stay as they are), may be
-            q itself; None: a new tensor (with zeros there).
+            q itself and shares no memory with the other tensors; None: a new tensor
+            (with zeros there).
     """
     eps, interleaved = check_eps(eps), bool(interleaved)
     host = _lib.native(k, v, k_cache, v_cache, page_table, lengths, *_lib.given(starts, q, q_weight, k_weight, table, q_out))
@@ -78,6 +79,7 @@ def kernel_fn(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: 
         raise ValueError("two places of a cache share their memory")
     if k_cache.numel() and k_cache.data_ptr() == v_cache.data_ptr():
         raise ValueError("k_cache and v_cache begin at the same place")
+    _heads.check_apart(k_cache, "k_cache", None, v_cache=v_cache)
     batch = _heads.check_batch(page_table, lengths, starts, tokens)
     if q is None:
         if q_weight is not None or q_out is not None:
@@ -99,6 +101,7 @@ def kernel_fn(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: 
             q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         else:
             _heads.check_out(q_out, "q_out", q)
+            _heads.check_apart(q_out, "q_out", q, q=q, k=k, v=v, k_cache=k_cache, v_cache=v_cache)
         q = q if dim == 1 or q.stride(2) == 1 else q.contiguous()
     k = k if dim == 1 or k.stride(2) == 1 else k.contiguous()
     v = v if dim == 1 or v.stride(2) == 1 else v.contiguous()

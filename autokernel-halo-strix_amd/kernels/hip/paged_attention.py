@@ -68,8 +68,9 @@ def kernel_fn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, pag
         max_chunk: the most new tokens of one sequence, where the caller knows: it
             chooses the kernel, results do not depend on its being right. None: all of
             the call's tokens (without starts: those of each sequence).
-        out: where the result goes (rows of no sequence stay as they are); None: a new
-            tensor (with zeros there).
+        out: where the result goes (rows of no sequence stay as they are), may be q
+            itself and shares no memory with the caches; None: a new tensor (with zeros
+            there).
     """
     host = _lib.native(q, k_cache, v_cache, page_table, lengths, *_lib.given(starts, out))
     if host is not None and q.dim() == 3 and q.shape[2]:
@@ -106,6 +107,7 @@ def kernel_fn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, pag
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     else:
         _heads.check_out(out, "out", q)
+        _heads.check_apart(out, "out", q, q=q, k_cache=k_cache, v_cache=v_cache)
     q = q if dim == 1 or q.stride(2) == 1 else q.contiguous()
     size = q.element_size()
     if dim * size % 16 == 0 and (q.data_ptr() | q.stride(0) * size | q.stride(1) * size) % 16:

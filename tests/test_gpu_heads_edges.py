@@ -385,3 +385,38 @@ def test_lengths_past_the_table_are_cut():
             kernel_fn(*(t.to(DEV) for t in (q, kc, vc, pages, torch.tensor(lengths, dtype=torch.int32))), scale=0.2, out=out)
             assert kept()
             close(out, want, bound, str(lengths))
+
+
+def test_outputs_in_place_of_the_queries():
+    """q_out and out may be the queries themselves, parts of a fused projection too; nothing else
+    that a call reads or writes."""
+    need_gpu()
+    from kernels.hip import paged_append, paged_attention
+    for dtype, dim in ((torch.bfloat16, 64), (torch.float32, 66), (torch.float16, 128)):
+        for counts, lengths in (([1] * 9, [700, 3, 90, 1, 65, 300, 2000, 16, 17]), ([90, 1, 40], [500, 900, 40])):
+            say("in place", dtype, dim, len(counts))
+            g = torch.Generator().manual_seed(29)
+            pages, lens, starts, total = make_batch(counts, lengths, 16, 29)
+            pages, lens, starts = pages.to(DEV), lens.to(DEV), starts.to(DEV)
+            fused = torch.randn(sum(counts), 8, dim, generator=g).to(dtype).to(DEV)
+            kc, vc = (torch.randn(total, 16, 2, dim, generator=g).to(dtype).to(DEV) for _ in range(2))
+            w = torch.ones(dim, dtype=dtype, device=DEV)
+
+            def append(f, **kw):
+                caches = kc.clone(), vc.clone()
+                return paged_append.kernel_fn(f[:, 4:6], f[:, 6:], *caches, pages, lens, starts, q=f[:, :4], q_weight=w, k_weight=w,
+                                              **kw), *caches
+
+            fresh = append(fused)
+            own = fused.clone()
+            got = append(own, q_out=own[:, :4])
+            assert all(torch.equal(a, b) for a, b in zip(got, fresh)) and torch.equal(own[:, 4:], fused[:, 4:])
+            with pytest.raises(ValueError, match="q_out shares memory with k"):
+                append(own, q_out=own[:, 4:])
+            with pytest.raises(ValueError, match="q_out shares memory with q"):
+                append(own, q_out=own[:, 1:5])
+            want = paged_attention.kernel_fn(fused[:, :4], kc, vc, pages, lens, starts, max_chunk=max(counts))
+            got = paged_attention.kernel_fn(own.copy_(fused)[:, :4], kc, vc, pages, lens, starts, max_chunk=max(counts), out=own[:, :4])
+            assert torch.equal(got, want) and torch.equal(own[:, 4:], fused[:, 4:])
+            with pytest.raises(ValueError, match="out shares memory with q"):
+                paged_attention.kernel_fn(own[:, :4], kc, vc, pages, lens, starts, out=own[:, 2:6])

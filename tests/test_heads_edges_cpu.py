@@ -3,7 +3,7 @@
 import pytest
 import torch
 
-from kernels.hip import _lib, paged_append, paged_attention, qk_norm_rotary, rotary
+from kernels.hip import _heads, _lib, paged_append, paged_attention, qk_norm_rotary, rotary
 from test_heads_cpu import _cache_call, heads_backend  # noqa: F401 (a fixture)
 
 
@@ -53,3 +53,63 @@ def test_attention_workspace_keeps_its_parts_aligned(dtype):
                                             (77, 1, 1, 64, 200), (333, 3, 5, 64, 64), (999, 2, 7, 256, 250)):
         need = size(tokens, batch, heads, heads, dim, keys, tokens, dtype)
         assert need > 0 and need % 16 == 0, (tokens, batch, heads, dim, keys, need)
+
+
+def test_shared_memory_is_told():
+    """Against the sets of places, over random views of one buffer; what it cannot tell is False."""
+    import random
+    rng = random.Random(1)
+
+    def view(base):
+        kind = rng.randrange(4)
+        if kind == 0:
+            n = rng.randint(1, 40)
+            return base[rng.randint(0, 200):][:n]
+        rows, pitch = rng.randint(1, 6), rng.randint(6, 30)
+        heads, dim = rng.randint(1, 3), rng.randint(1, 3)
+        if kind == 1:
+            pitch = 20
+        dims = (rows, heads, dim), (pitch, dim, 1)
+        if kind == 3:
+            dims = (heads, rows, dim), (dim, pitch, 1)
+        return base.as_strided(*dims, rng.randint(0, 150))
+
+    base, places = torch.zeros(600), torch.arange(600.0)
+    told = 0
+    for _ in range(3000):
+        state = rng.getstate()
+        a, b = view(base), view(base)
+        rng.setstate(state)
+        pa, pb = view(places), view(places)
+        meet = bool(set(pa.reshape(-1).tolist()) & set(pb.reshape(-1).tolist()))
+        got = _heads.share_memory(a, b)
+        assert got == _heads.share_memory(b, a) and (meet or not got)
+        x, y = _heads._spans(a), _heads._spans(b)
+        if x is not None and y is not None and (x[0] == 1 or y[0] == 1 or x[1] == y[1]):
+            assert got == meet, (a.shape, a.stride(), b.shape, b.stride())
+            told += meet
+    assert told > 300
+    assert not _heads.share_memory(base[:0], base)
+
+
+def test_outputs_that_share_memory(heads_backend):  # noqa: F811
+    """A kernel's rows are read and written in no order: an output is apart from what is read
+    beside it, or the queries themselves."""
+    fused = torch.randn(5, 8, 6)
+    c = dict(_cache_call(), q=fused[:, :4], k=fused[:, 4:6], v=fused[:, 6:])
+    paged_append.kernel_fn(**c, q_out=c["q"])
+    for q_out, text in ((fused[:, 1:5], "q"), (fused[:, 4:], "k"), (fused[:, 2:6], "q")):
+        with pytest.raises(ValueError, match=f"q_out shares memory with {text}"):
+            paged_append.kernel_fn(**c, q_out=q_out)
+    both = torch.zeros(c["k_cache"].shape[0] + 1, 4, 2, 6)
+    with pytest.raises(ValueError, match="k_cache shares memory with v_cache"):
+        paged_append.kernel_fn(**dict(c, k_cache=both[1:], v_cache=both[:-1]))
+    pair = torch.zeros(c["k_cache"].shape[0], 2, 4, 2, 6)
+    paged_append.kernel_fn(**dict(c, k_cache=pair[:, 0], v_cache=pair[:, 1]))
+    long = torch.randn(7, 4, 6)
+    a = dict(q=long[1:6], k_cache=c["k_cache"], v_cache=c["v_cache"], page_table=c["page_table"], lengths=c["lengths"],
+             starts=c["starts"])
+    for out, text in ((long[:5], "q"), (long[2:], "q"), (c["k_cache"].view(-1, 4, 6)[:5], "k_cache")):
+        with pytest.raises(ValueError, match=f"out shares memory with {text}"):
+            paged_attention.kernel_fn(**a, out=out)
+    assert paged_attention.kernel_fn(**a, out=a["q"]) is a["q"]
