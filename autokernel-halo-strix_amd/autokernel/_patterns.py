@@ -15,9 +15,10 @@ On gfx950 two patterns replace modules:
 * ``rmsnorm`` (priority 50, reference :508-529): RMSNorm-like modules.
 
 The remaining reference patterns keep their names and priorities so that
-``list_patterns()`` and include / exclude lists stay valid, but their kernels
-(rotary, SwiGLU, Griffin scan) are not part of the gfx950 kernel set; they
-never match.
+``list_patterns()`` and include / exclude lists stay valid, but they never
+match: the kernels of SwiGLU and the Griffin scan are not part of the gfx950
+kernel set, and its rotary kernel (``kernels.hip.rotary``) takes queries and
+keys with a table of its own, which no module that could be swapped calls.
 
 The replacements always route through the autograd-registered custom ops
 (``torch.ops.autokernel.*``) for fp16, bf16 and fp32 activations, with the
@@ -175,7 +176,7 @@ class RMSNormPattern(Pattern):
 
 
 class _UnavailablePattern(Pattern):
-    """A reference pattern whose kernel is outside the gfx950 kernel set: never matches."""
+    """A reference pattern that no gfx950 kernel serves as a module: never matches."""
 
     def matches(self, name, module, model):
         return False

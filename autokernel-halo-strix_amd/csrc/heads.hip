@@ -25,9 +25,10 @@ namespace {
 
 constexpr int kThreads = 256;
 // Results that the eight L2s of 4 MiB cannot hold are stored past them: 84 MB of
-// queries and keys turned there and back in 65 us (5.2 TB/s), through them in 79
-// (normed too, in 85 and 93). Smaller ones stay for their reader; so does what
-// goes into a cache, 67 us for 133 MB of appended prompts, past the L2s 66.
+// queries and keys turned there and back in 65 us (5.2 TB/s; on other cards up to 70),
+// through them in 79 (normed too, in 85 to 90 and 93). Smaller ones stay for their
+// reader; so does what goes into a cache, 67 us for 133 MB of appended prompts, past
+// the L2s 66.
 constexpr int64_t kL2Bytes = 32 << 20;
 
 // One of the tensors whose heads a call walks over: element strides, the last

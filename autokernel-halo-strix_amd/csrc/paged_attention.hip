@@ -20,7 +20,7 @@ namespace {
 // a row (token and query head) and a cut of its keys. A wave takes 64 keys at a
 // time: a lane each for the scores, then a lane for every 64th element of the
 // values' sum. Bound by the strided reads of the keys: 16 sequences of
-// 1024 to 4096 keys, 32 + 8 heads of 128 bf16, off the alignment, 1270 us, in tiles 54.
+// 1024 to 4096 keys, 32 + 8 heads of 128 bf16, off the alignment, 1270 us, in tiles 49 to 54.
 template <typename T>
 __global__ void __launch_bounds__(256) attend_any_kernel(AttendArgs a, int64_t rows) {
   constexpr int kPer = kMaxAttendDim / 64;

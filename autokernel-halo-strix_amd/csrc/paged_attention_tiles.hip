@@ -926,7 +926,7 @@ __device__ __forceinline__ void clear_lds(char* to, int bytes, int thread, int t
 // Bound by the cache's bytes, each read once: a wave loads a unit of 32 keys' K and V while
 // it works on the one before, whose rows it has looked up a unit earlier. Of a tile of up to
 // 32 rows the matrix cores do mostly nothing (a decode step has the group's heads), and are
-// free. [64 sequences of 2048 to 8192 keys, 32 + 8 heads of 128] bf16 264 us, 5.1 TB/s, where
+// free. [64 sequences of 2048 to 8192 keys, 32 + 8 heads of 128] bf16 265 us, 5.1 TB/s, where
 // reads alone reach 6.0; two of 130001 keys 180, 4.8 TB/s with the join. Rows of 512 bytes
 // leave registers for one workgroup a CU, and still: 25 x 1882 keys, 4 heads of 256, bf16 51
 // us, in tiles of many rows 70.
@@ -1085,7 +1085,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, DB * sizeof(T) <= 256 ? 2 : 1)
 // stores after the barrier, which saves a slot.)
 //
 // Bound by what surrounds the products: prompts of up to 4096 tokens, 32 + 8 heads of 128 bf16,
-// 488 us, 766 TFLOP/s where a product of 8192^3 reaches 1420. Of a step's 5600 cycles
+// 485 to 505 us by card, 766 TFLOP/s where a product of 8192^3 reaches 1420. Of a step's 5600 cycles
 // (1.9 GHz under this load) a SIMD's matrix cores take 2050. The matrix phase has 900 for O^T's
 // products, 750 for the stores, loads and places of units ahead, 300 for tiles' ends, 660 for
 // the scores, the vector phase 1340 for weights and 530 for look-ups. A first unit's operands
@@ -1515,8 +1515,9 @@ Plan plan_of(int64_t tokens, int64_t batch, int64_t q_heads, int64_t kv_heads, i
   if (p.few) p.workers = (p.workers + kFewWaves - 1) / kFewWaves * kFewWaves;
   const int64_t tiles = kv_heads * std::max(tokens / p.per_tile, (int64_t)1);
   p.cut = p.workers > 8 * tiles;
-  // (measured: half and double of either cost do the same on the average of random calls; units of
-  // fp32 take four times as long)
+  // (measured: half and double of either cost do the same on the average of random calls. Units of
+  // fp32 take four times as long: with that in the cost chunks of 11 tokens over 3 x 2654 keys, 4
+  // heads of 96, take 44 us, without it 47; ten other random calls of fp32 the same either way)
   p.join_cost = (p.few ? 0.02f * (float)((p.rows + 15) / 16) : 0.2f) / (f32 ? 4.0f : 1.0f) / (float)tiles;
   p.line_bytes = (size_t)(batch + 2) / 2 * 16;
   p.job_bytes = ((size_t)p.workers * sizeof(Job) + 15) / 16 * 16;  // (the parts behind them are read 16 bytes at a time)

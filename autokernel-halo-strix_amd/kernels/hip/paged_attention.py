@@ -67,7 +67,9 @@ def kernel_fn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, pag
         window: the most keys that a token sees, its own the last (0 = all).
         max_chunk: the most new tokens of one sequence, where the caller knows: it
             chooses the kernel, results do not depend on its being right. None: all of
-            the call's tokens (without starts: those of each sequence).
+            the call's tokens (without starts: those of each sequence), which takes the
+            kernel for many rows: a decode step of 64 sequences given by starts alone
+            takes 298 us, with max_chunk=1 (or without starts) 265.
         out: where the result goes (rows of no sequence stay as they are), may be q
             itself and shares no memory with the caches; None: a new tensor (with zeros
             there).

@@ -4,10 +4,12 @@ pass, on gfx950 (MI355X).
     n = x / sqrt(mean(x^2) + eps) * weight        over a head's elements
     y = n with its pairs turned (``kernels.hip.rotary``), or n without a table
 
-in fp32 with one rounding. The forward reads and writes each element once
-(``csrc/heads.hip``); so does the backward with the upstream gradient beside it,
-which it turns back, and from which it sums the weights' gradients over tokens and
-heads in fp32, in a fixed order. Differentiable once.
+in fp32 with one rounding (the sum of squares too: heads whose squares leave
+fp32's range, past 1e18 or, with eps 0, below 1e-20, have no norm there). The
+forward reads and writes each element once (``csrc/heads.hip``); so does the
+backward with the upstream gradient beside it, which it turns back, and from
+which it sums the weights' gradients over tokens and heads in fp32, in a fixed
+order. Differentiable once.
 
 No counterpart in the reference, whose RMSNorm (``kernels/hip/rmsnorm.py:156-177``)
 takes whole rows and whose registry keeps the rotary pattern's name only.

@@ -13,9 +13,9 @@ the reference's class names, or a module with ``weight`` and ``eps`` and no
 ``fused_residual_add_rmsnorm`` (pre-norm blocks with attention,
 attention_norm, feed_forward and ffn_norm, or the other attribute families
 of ``autokernel._patterns``, :1033-1050). The reference's other types
-(matmul, layernorm, silu_gate_mul, rotary_embedding, fused_qkv) are outside
-this kernel set and are skipped with a note, as the reference does for types
-it has no strategy for.
+(matmul, layernorm, silu_gate_mul, rotary_embedding, fused_qkv) have no module
+to put in place here (``kernels.hip.rotary`` is called on queries and keys) and
+are skipped with a note, as the reference does for types it has no strategy for.
 """
 
 from __future__ import annotations

@@ -724,8 +724,9 @@ int ak_paged_append(const void* q, const void* k, const void* v, const void* q_w
  *   s_j = scale q . k_j  (softcap > 0: softcap tanh(s_j / softcap)),
  *   out = sum_j softmax(s)_j v_j
  * in fp32 (fp16 / bf16: the probabilities are rounded once, for the matrix cores). A
- * token that sees no key, or only scores of -inf, gives 0. Query head h reads key
- * head h * kv_heads / q_heads. max_chunk: the most new tokens of a sequence, as far as
+ * token that sees no key gives 0, as does one that sees only scores of -inf beside
+ * finite values (their weight is 0, and 0 times an infinity or NaN is NaN). Query head h
+ * reads key head h * kv_heads / q_heads. out may be q itself, row for row. max_chunk: the most new tokens of a sequence, as far as
  * the caller knows (it chooses the kernel; results hold for any). out rows of no
  * sequence: as in ak_paged_append. dim is at most 1024. No counterpart in the reference.
  */
